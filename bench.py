@@ -440,6 +440,7 @@ def run_gating(args):
 
 def run_model(args):
     import torch.nn.functional as F
+    from mathbrain.grad_clip import clip_grad_norm_
     from mathbrain.model import SlotTransformerLM
     from mathbrain.synthetic import make_doc_batch
     B, T, V, N, D, n_layers, H = 56, 512, 50257, 64, 512, 6, 8
@@ -464,7 +465,7 @@ def run_model(args):
             logits = model(x, unique_slots=uniq, c_base=cb, pad_mask=pm)
             loss = F.cross_entropy(logits.view(-1, V), tgt.view(-1), ignore_index=-1)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
+        clip_grad_norm_(model.parameters(), 1.0)
         opt.step()
         sched.step()
         return loss

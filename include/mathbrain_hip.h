@@ -609,6 +609,63 @@ int mb_swiglu_fwd(const void *a, const void *b, int64_t n, int dtype, void *m, v
 int mb_swiglu_bwd(const void *a, const void *b, const void *dm, int64_t n, int dtype, void *da,
                   void *db, void *stream);
 
+/*
+ * Query/key norm with the position rotation, for the comparison model's attention
+ * (mathbrain/baseline.py:31-70): for every head's row x of q and k, with that side's weight w
+ * and the row's position p,
+ *
+ *   n = x rsqrt(mean(x^2) + eps),  y = w n,
+ *   out[2i] = y[2i] cos[p,i] - y[2i+1] sin[p,i],  out[2i+1] = y[2i] sin[p,i] + y[2i+1] cos[p,i]
+ *
+ *   q, k           [B, L, H | Hk, hd], element strides (_sb, _sl, _sh), channels next to each
+ *                  other, rows at multiples of 16 bytes; dtype MB_DTYPE_F32 or MB_DTYPE_BF16
+ *   wq, wk         [hd] fp32;  cos, sin  [table_rows, hd / 2] fp32 contiguous
+ *   start          [B] position of each row's first token, int32 (start_bytes 4) or int64 (8),
+ *                  or NULL: start0 for all.  A position outside [0, table_rows) gives NaN.
+ *   q_out, k_out   [B, L, H | Hk, hd] contiguous, 16-byte aligned
+ *
+ * The backward takes the outputs' gradients dq_out, dk_out (strides as above) and writes
+ * dq, dk (contiguous) and dwq, dwk [hd] fp32; the weight sums have a fixed order.  Its
+ * workspace is mb_qk_norm_rotary_bwd_workspace(B, L, hd) bytes.  hd: 32, 64 or 128.
+ */
+int mb_qk_norm_rotary_fwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
+                          int64_t k_sb, int64_t k_sl, int64_t k_sh, const float *wq,
+                          const float *wk, const float *cos, const float *sin, int64_t table_rows,
+                          const void *start, int start_bytes, int64_t start0, int B, int L, int H,
+                          int Hk, int hd, float eps, int dtype, void *q_out, void *k_out,
+                          void *stream);
+int64_t mb_qk_norm_rotary_bwd_workspace(int B, int L, int hd);
+int mb_qk_norm_rotary_bwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
+                          int64_t k_sb, int64_t k_sl, int64_t k_sh, const void *dq_out,
+                          int64_t dq_sb, int64_t dq_sl, int64_t dq_sh, const void *dk_out,
+                          int64_t dk_sb, int64_t dk_sl, int64_t dk_sh, const float *wq,
+                          const float *wk, const float *cos, const float *sin, int64_t table_rows,
+                          const void *start, int start_bytes, int64_t start0, int B, int L, int H,
+                          int Hk, int hd, float eps, int dtype, void *dq, void *dk, float *dwq,
+                          float *dwk, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_ in the reference's training
+ * step):
+ *
+ *   norm = sqrt(sum_i sum_e src[i][e]^2)  (in 64 bits, fixed order),
+ *   dst[i] = src[i] * min(1, max_norm / (norm + 1e-6))
+ *
+ *   src, dst, n          HOST arrays of `count` device addresses and element counts; dst NULL:
+ *                        the norm alone.  dst[i] may be src[i] (with the same dtype): in place,
+ *                        where a factor of 1 writes nothing.  Memory that is written must not
+ *                        be another tensor's (checked).
+ *   src_dtype, dst_dtype HOST arrays of MB_DTYPE_F32 or MB_DTYPE_BF16
+ *   norm_out             one fp32
+ *   workspace            mb_grad_clip_workspace(count) bytes
+ *
+ * A norm that is NaN or infinite scales as max_norm / (norm + 1e-6) does (NaN, or 0).
+ */
+int64_t mb_grad_clip_workspace(int count);
+int mb_grad_clip(const void *const *src, const int32_t *src_dtype, void *const *dst,
+                 const int32_t *dst_dtype, const int64_t *n, int count, float max_norm,
+                 float *norm_out, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,6 +73,14 @@ SIGNATURES = {
     "mb_rmsnorm_bwd": ([_p, _p, _p, _p, _i64, _i, _p, _p, _p], _i),
     "mb_layernorm_fwd": ([_p, _p, _p, _i64, _i, _f, _p, _p, _p, _p], _i),
     "mb_layernorm_bwd": ([_p, _p, _p, _p, _p, _i64, _i, _p, _p, _p, _p], _i),
+    "mb_qk_norm_rotary_fwd": ([_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i, _i64,
+                               _i, _i, _i, _i, _i, _f, _i, _p, _p, _p], _i),
+    "mb_qk_norm_rotary_bwd": ([_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64,
+                               _i64, _p, _p, _p, _p, _i64, _p, _i, _i64, _i, _i, _i, _i, _i, _f, _i, _p, _p, _p,
+                               _p, _p, _i64, _p], _i),
+    "mb_qk_norm_rotary_bwd_workspace": ([_i, _i, _i], _i64),
+    "mb_grad_clip": ([_p, _p, _p, _p, _p, _i, _f, _p, _p, _i64, _p], _i),
+    "mb_grad_clip_workspace": ([_i], _i64),
     "mb_swiglu_fwd": ([_p, _p, _i64, _i, _p, _p], _i),
     "mb_swiglu_bwd": ([_p, _p, _p, _i64, _i, _p, _p, _p], _i),
 }

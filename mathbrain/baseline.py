@@ -7,12 +7,16 @@ by name); the blocks reuse this package's RMSNorm and SwiGLU (one HIP pass per
 direction) and torch's scaled_dot_product_attention.  The rotary embedding rotates the
 channel pairs (2i, 2i+1) of each head by t * theta^(-2i/hd), written with real cos/sin
 tables instead of the reference's complex multiply (the same rotation).
+
+``qk_norm=True`` (not in the reference) norms every query and key head before the rotation,
+in the rotation's own pass (``qk_norm_rotary``).
 """
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from .model import RMSNorm, SwiGLU
+from .qk_norm import qk_norm_rotary
 
 
 def rotary_tables(head_dim, max_len, theta=10000.0):
@@ -35,7 +39,7 @@ def rotate(x, cos, sin):
 class CausalSelfAttention(nn.Module):
     """baseline.py:31-70."""
 
-    def __init__(self, d_model: int, n_heads: int, dropout: float = 0.0):
+    def __init__(self, d_model: int, n_heads: int, dropout: float = 0.0, qk_norm: bool = False):
         super().__init__()
         assert d_model % n_heads == 0
         self.d_model = d_model
@@ -46,12 +50,21 @@ class CausalSelfAttention(nn.Module):
         self.wv = nn.Linear(d_model, d_model, bias=False)
         self.wo = nn.Linear(d_model, d_model, bias=False)
         self.resid_dropout = nn.Dropout(dropout)
+        if qk_norm:
+            # their weights and eps; the norms run in the rotation's pass
+            self.q_norm = RMSNorm(self.head_dim)
+            self.k_norm = RMSNorm(self.head_dim)
+        self.qk_norm = qk_norm
 
     def forward(self, x, cos, sin):
         B, L, D = x.shape
         shape = (B, L, self.n_heads, self.head_dim)
-        q = rotate(self.wq(x).view(shape), cos, sin).transpose(1, 2)
-        k = rotate(self.wk(x).view(shape), cos, sin).transpose(1, 2)
+        q, k = self.wq(x).view(shape), self.wk(x).view(shape)
+        if self.qk_norm:
+            q, k = qk_norm_rotary(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps)
+        else:
+            q, k = rotate(q, cos, sin), rotate(k, cos, sin)
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = self.wv(x).view(shape).transpose(1, 2)
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True,
                                              dropout_p=self.resid_dropout.p if self.training else 0.0)
@@ -61,10 +74,10 @@ class CausalSelfAttention(nn.Module):
 class RoPETransformerBlock(nn.Module):
     """baseline.py:72-84."""
 
-    def __init__(self, d_model: int, n_heads: int, d_ff: int, dropout: float = 0.0):
+    def __init__(self, d_model: int, n_heads: int, d_ff: int, dropout: float = 0.0, qk_norm: bool = False):
         super().__init__()
         self.attn_norm = RMSNorm(d_model)
-        self.attn = CausalSelfAttention(d_model, n_heads, dropout)
+        self.attn = CausalSelfAttention(d_model, n_heads, dropout, qk_norm)
         self.ffn_norm = RMSNorm(d_model)
         self.ffn = SwiGLU(d_model, d_ff)
 
@@ -75,16 +88,17 @@ class RoPETransformerBlock(nn.Module):
 
 class RoPETransformerLM(nn.Module):
     """baseline.py:86-129: RoPETransformerLM(vocab_size, d_model, n_layers, n_heads,
-    max_seq_len=4096, dropout=0.1); forward(x [B, L]) -> logits [B, L, vocab_size]."""
+    max_seq_len=4096, dropout=0.1); forward(x [B, L]) -> logits [B, L, vocab_size].
+    ``qk_norm``: RMS norms of every query and key head (head_dim 32, 64 or 128)."""
 
     def __init__(self, vocab_size: int, d_model: int, n_layers: int, n_heads: int,
-                 max_seq_len: int = 4096, dropout: float = 0.1):
+                 max_seq_len: int = 4096, dropout: float = 0.1, qk_norm: bool = False):
         super().__init__()
         self.vocab_size = vocab_size
         self.d_model = d_model
         self.embed = nn.Embedding(vocab_size, d_model)
         d_ff = 256 * ((int(8 * d_model / 3) + 255) // 256)
-        self.layers = nn.ModuleList([RoPETransformerBlock(d_model, n_heads, d_ff, dropout)
+        self.layers = nn.ModuleList([RoPETransformerBlock(d_model, n_heads, d_ff, dropout, qk_norm)
                                      for _ in range(n_layers)])
         self.final_norm = RMSNorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)

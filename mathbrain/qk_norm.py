@@ -1,0 +1,142 @@
+"""RMS norm of every query and key head with the position rotation, on the gfx950 kernels of
+mb_qk_norm_rotary_fwd / mb_qk_norm_rotary_bwd.
+
+``qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, eps, start)`` computes, for each head's
+row x of q and k,
+
+    y = weight * x * rsqrt(mean(x^2) + eps),  then turns the pairs (y[2i], y[2i+1]) by the
+    angle of the row's position (``cos`` / ``sin`` as baseline.rotary_tables makes them),
+
+evaluated in fp32 and rounded once to the inputs' dtype, with gradients for q, k and both
+weights.  One launch forward, two backward; the weight gradients are summed in a fixed order.
+CPU tensors raise NotImplementedError: there is no CPU path.  Both directions are registered
+as torch ops (mathbrain::qk_norm_rotary_fwd / _bwd) for tracing.
+"""
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.MB_DTYPE_F32, torch.bfloat16: _lib.MB_DTYPE_BF16}
+
+
+def _rows16(x):
+    """x with the head's channels next to each other and rows at multiples of 16 bytes."""
+    size = x.element_size()
+    sb, sl, sh, sd = x.stride()
+    if sd == 1 and not (x.data_ptr() | sb * size | sl * size | sh * size) & 15:
+        return x
+    return x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def _start_args(start_rows, start):
+    if start_rows is None:
+        return None, 4, start
+    return _lib.ptr(start_rows), start_rows.element_size(), 0
+
+
+def _fwd_fake(q, k, q_weight, k_weight, cos, sin, eps, start_rows, start):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@_lib.traced_op("qk_norm_rotary_fwd", _fwd_fake)
+def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                       cos: torch.Tensor, sin: torch.Tensor, eps: float, start_rows: Optional[torch.Tensor],
+                       start: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q', k'), contiguous."""
+    dev = q.device
+    B, L, H, hd = q.shape
+    q, k = _rows16(q.detach()), _rows16(k.detach())
+    wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
+    qo = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    at, size, first = _start_args(start_rows, start)
+    with torch.cuda.device(dev):
+        _lib.call("mb_qk_norm_rotary_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                  wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first,
+                  B, L, H, k.shape[2], hd, eps, _DTYPES[q.dtype], qo.data_ptr(), ko.data_ptr(),
+                  _lib.stream(dev))
+    return qo, ko
+
+
+def _bwd_fake(q, k, q_weight, k_weight, cos, sin, dq_out, dk_out, eps, start_rows, start):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), q_weight.new_empty(q_weight.shape),
+            k_weight.new_empty(k_weight.shape))
+
+
+@_lib.traced_op("qk_norm_rotary_bwd", _bwd_fake)
+def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                       cos: torch.Tensor, sin: torch.Tensor, dq_out: torch.Tensor, dk_out: torch.Tensor,
+                       eps: float, start_rows: Optional[torch.Tensor], start: int
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rotary_fwd for the output gradients."""
+    dev = q.device
+    B, L, H, hd = q.shape
+    q, k = _rows16(q.detach()), _rows16(k.detach())
+    gq, gk = _rows16(dq_out.detach().to(q.dtype)), _rows16(dk_out.detach().to(k.dtype))
+    wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
+    dq = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    dw = torch.empty((2, hd), dtype=torch.float32, device=dev)
+    ws = torch.empty(_lib.lib().mb_qk_norm_rotary_bwd_workspace(B, L, hd), dtype=torch.uint8, device=dev)
+    at, size, first = _start_args(start_rows, start)
+    with torch.cuda.device(dev):
+        _lib.call("mb_qk_norm_rotary_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                  gq.data_ptr(), *gq.stride()[:3], gk.data_ptr(), *gk.stride()[:3], wq.data_ptr(),
+                  wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first, B, L, H,
+                  k.shape[2], hd, eps, _DTYPES[q.dtype], dq.data_ptr(), dk.data_ptr(), dw.data_ptr(),
+                  dw.data_ptr() + 4 * hd, ws.data_ptr(), ws.numel(), _lib.stream(dev))
+    return dq, dk, dw[0].to(q_weight.dtype), dw[1].to(k_weight.dtype)
+
+
+class QKNormRotaryFunction(torch.autograd.Function):
+    """autograd for qk_norm_rotary: gradients for q, k and the two weights."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps, start_rows, start):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, start_rows)
+        ctx.rest = (eps, start)
+        return qk_norm_rotary_fwd(q, k, q_weight, k_weight, cos, sin, eps, start_rows, start)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, start_rows = ctx.saved_tensors
+        eps, start = ctx.rest
+        grads = qk_norm_rotary_bwd(q, k, q_weight, k_weight, cos, sin, dq_out, dk_out, eps, start_rows, start)
+        return (*grads, None, None, None, None, None)
+
+
+def _check(q, k, q_weight, k_weight, cos, sin, start):
+    what = "qk_norm_rotary"
+    rows = start if torch.is_tensor(start) else None
+    _lib.require_gpu(q, k, q_weight, k_weight, cos, sin, rows, what=what)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} are not [B, L, H, hd] and [B, L, Hk, hd]")
+    hd = q.shape[3]
+    if q.dtype not in _DTYPES or k.dtype != q.dtype:
+        raise ValueError(f"{what}: q {q.dtype} and k {k.dtype} (supported: both float32 or both bfloat16)")
+    if q_weight.shape != (hd,) or k_weight.shape != (hd,):
+        raise ValueError(f"{what}: weights {tuple(q_weight.shape)}, {tuple(k_weight.shape)} do not match head_dim {hd}")
+    if cos.dim() != 2 or cos.shape[1] * 2 != hd or cos.shape != sin.shape:
+        raise ValueError(f"{what}: tables {tuple(cos.shape)}, {tuple(sin.shape)} are not [positions, {hd // 2}]")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"{what}: the tables must be contiguous float32")
+    if rows is not None and (rows.shape != (q.shape[0],) or rows.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"{what}: start {tuple(rows.shape)} {rows.dtype} is not one int32 or int64 for each of "
+                         f"{q.shape[0]} rows")
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, eps=1e-6, start=0):
+    """Normalises and rotates q [B, L, H, hd] and k [B, L, Hk, hd] (fp32 or bf16, any strides);
+    weights [hd]; ``cos`` / ``sin`` [positions, hd / 2] fp32.  ``start`` is the position of each
+    row's first token: an int (checked against the tables), or an int32 / int64 tensor [B], as a
+    step that appends one token to sequences of different lengths has it; a position outside the
+    tables gives NaN rows there.  head_dim 32, 64 or 128."""
+    _check(q, k, q_weight, k_weight, cos, sin, start)
+    rows = start.contiguous() if torch.is_tensor(start) else None
+    args = (q, k, q_weight, k_weight, cos, sin, float(eps), rows, 0 if rows is not None else int(start))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
+                                    or k_weight.requires_grad):
+        return QKNormRotaryFunction.apply(*args)
+    return qk_norm_rotary_fwd(*args)
