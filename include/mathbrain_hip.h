@@ -645,6 +645,47 @@ int mb_qk_norm_rotary_bwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_s
                           float *dwk, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
+ * Attention with a learned relative position bias by distance buckets:
+ *
+ *   s_ij = scale q_i . k_j + bias[bucket(pos_i - j), h],  p = softmax_j(s),  o_i = sum_j p_ij v_j
+ *   dq, dk, dv and dbias[n, h] = sum over the pairs of bucket n of ds_ij for an output gradient d_o
+ *
+ *   q, o, d_o, dq   [B, H, Lq, hd];  k, v, dk, dv  [B, Hk, Lk, hd], Hk divides H.  dtype
+ *                   MB_DTYPE_F32 or MB_DTYPE_BF16, channels next to each other, rows at multiples
+ *                   of 16 bytes.  Each comes with a HOST array of its element strides (B, H, L).
+ *   bias, dbias     [buckets, H] contiguous, bias_dtype MB_DTYPE_F32 or MB_DTYPE_BF16
+ *   starts          HOST array: the first distance of each of n_starts buckets, not falling, from
+ *                   0 to at most 1024; the last bucket has no end.  n_starts <= 128.  causal:
+ *                   buckets = n_starts.  Otherwise buckets = 2 n_starts, the upper half for keys
+ *                   behind the query's position (distance j - pos_i >= 1).
+ *   lengths         [B] keys that count, or NULL: Lk (int32 or int64: lengths_bytes 4 or 8);
+ *                   rows of k and v from there on are not used, their gradients are zero
+ *   q_start         [B] position of each row's first query (likewise), or NULL: q_start0
+ *   causal          a query sees the keys j <= pos_i
+ *   lse             [B, H, Lq] fp32: log2 of the softmax denominators, written by the forward
+ *                   (NULL: not wanted), read by the backward
+ *
+ * Rows without a key give zeros.  The backward's workspace is mb_bias_attn_bwd_workspace(...)
+ * bytes; dbias may be NULL.  Its sums have a fixed order.  hd: 32, 64 or 128.
+ */
+int mb_bias_attn_fwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
+                     const void *v, const int64_t *v_st, const void *bias, int bias_dtype,
+                     int buckets, const int32_t *starts, int n_starts, const void *lengths,
+                     int lengths_bytes, const void *q_start, int q_start_bytes, int64_t q_start0,
+                     int B, int H, int Hk, int Lq, int Lk, int hd, float scale, int causal,
+                     int dtype, void *o, const int64_t *o_st, float *lse, void *stream);
+int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets);
+int mb_bias_attn_bwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
+                     const void *v, const int64_t *v_st, const void *bias, int bias_dtype,
+                     int buckets, const int32_t *starts, int n_starts, const void *lengths,
+                     int lengths_bytes, const void *q_start, int q_start_bytes, int64_t q_start0,
+                     int B, int H, int Hk, int Lq, int Lk, int hd, float scale, int causal,
+                     int dtype, const void *o, const int64_t *o_st, const void *d_o,
+                     const int64_t *do_st, const float *lse, void *dq, const int64_t *dq_st,
+                     void *dk, const int64_t *dk_st, void *dv, const int64_t *dv_st, void *dbias,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_ in the reference's training
  * step):
  *

@@ -24,6 +24,10 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
 
+# q, k, v, the bias table, lengths, positions, sizes: what both directions of the attention with
+# a learned bias begin with
+_BIAS_ATTN = ([_p] * 6 + [_p, _i, _i, _p, _i, _p, _i, _p, _i, _i64] + [_i] * 6 + [_f, _i, _i])
+
 # name -> argtypes; every entry is declared in include/mathbrain_hip.h
 SIGNATURES = {
     "mb_last_error": ([], ctypes.c_char_p),
@@ -79,6 +83,9 @@ SIGNATURES = {
                                _i64, _p, _p, _p, _p, _i64, _p, _i, _i64, _i, _i, _i, _i, _i, _f, _i, _p, _p, _p,
                                _p, _p, _i64, _p], _i),
     "mb_qk_norm_rotary_bwd_workspace": ([_i, _i, _i], _i64),
+    "mb_bias_attn_fwd": (_BIAS_ATTN + [_p, _p, _p, _p], _i),
+    "mb_bias_attn_bwd": (_BIAS_ATTN + [_p] * 5 + [_p] * 7 + [_p, _i64, _p], _i),
+    "mb_bias_attn_bwd_workspace": ([_i, _i, _i, _i], _i64),
     "mb_grad_clip": ([_p, _p, _p, _p, _p, _i, _f, _p, _p, _i64, _p], _i),
     "mb_grad_clip_workspace": ([_i], _i64),
     "mb_swiglu_fwd": ([_p, _p, _i64, _i, _p, _p], _i),

@@ -1,0 +1,233 @@
+// Attention with a learned bias by distance buckets: what the forward and backward share.
+//
+//   s_ij = scale q_i . k_j + bias[bucket(pos_i - j), h],   p = softmax_j(s),   o_i = sum_j p_ij v_j
+//
+// Layout of the products.  All of them run on the 32 x 32 matrix instructions, whose result a
+// lane holds as one column (lane % 32) and the 16 rows 8 (r / 4) + 4 (lane / 32) + r % 4.  The
+// score block is taken transposed (keys by queries), so that a lane holds 16 keys of one query:
+// the row's maximum and sum need one exchange between the two half waves, and the probabilities
+// are already the right-hand operand of the next product.  An operand's k index may run in any
+// order as long as both operands agree: slot (half wave g, element e) of the 16-deep step c is
+// row 16 c + 8 (e / 4) + 4 g + e % 4, which is where the results lie.  The other operand comes
+// out of LDS in that order by the transposing 16-bit LDS read (or, in fp32, by element).
+#pragma once
+
+#include "common.h"
+
+namespace mb {
+namespace battn {
+
+constexpr int kThreads = 256;   // four waves
+constexpr int kWaveRows = 32;   // queries (or keys) of a wave
+constexpr int kRows = 4 * kWaveRows;
+constexpr int kMaxStarts = 128;
+constexpr int kMaxReach = 1024; // the largest distance with a bucket of its own
+constexpr int kPad = 64;        // table entries beyond each end: a 32 x 32 block's distances that pass it
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef __attribute__((__ext_vector_type__(4))) __bf16 bf16x4;
+typedef __attribute__((__ext_vector_type__(8))) __bf16 bf16x8;
+typedef __attribute__((__ext_vector_type__(4))) short s16x4;
+typedef __attribute__((__ext_vector_type__(4))) float f32x4;
+typedef __attribute__((__ext_vector_type__(8))) float f32x8;
+typedef __attribute__((__ext_vector_type__(16))) float f32x16;
+typedef f32x8 f32x8u __attribute__((aligned(16)));  // rows begin at multiples of 16 bytes
+
+template <typename T>
+struct Ty;
+template <>
+struct Ty<__bf16> {
+    typedef bf16x8 Frag;
+    typedef bf16x8 FragMem;
+    typedef bf16x4 Quad;
+    static constexpr int kKeys = 64;   // rows of a staged tile
+    static __device__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Ty<float> {
+    typedef f32x8 Frag;
+    typedef f32x8u FragMem;
+    typedef f32x4 Quad;
+    static constexpr int kKeys = 32;
+    // the 16-deep product as eight 2-deep ones: element e of both operands is slot (g, e)
+    static __device__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+
+struct Args {
+    const void *q, *k, *v, *o, *d_o;        // o, d_o: backward
+    int64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl, o_sb, o_sh, o_sl, do_sb, do_sh, do_sl;
+    const void* bias;                        // [buckets, H]
+    const void *lengths, *start;             // [B] or NULL
+    void *out, *dk, *dv;                     // out: o (forward) or dq
+    int64_t out_sb, out_sh, out_sl, dk_sb, dk_sh, dk_sl, dv_sb, dv_sh, dv_sl;
+    float *lse, *delta, *dbias_part;         // [B, H, Lq] (log2 units), [B, H, Lq], [H, B * nq, buckets]
+    int lengths_bytes, start_bytes, start0;
+    int B, H, Hk, Lq, Lk, nq;
+    int causal, bias_bf16, buckets, n_starts, reach;
+    float scale;
+    int16_t starts[kMaxStarts];              // first distance of each bucket of one direction
+};
+
+// The distance table covers lo .. hi and is padded by kPad entries on both ends.  Distances from
+// hi on have one bucket, and so have those from lo down.
+struct Reach {
+    int lo, hi;
+    __host__ __device__ explicit Reach(const Args& a)
+        : lo(a.causal ? 0 : -(a.reach > 1 ? a.reach : 1)), hi(a.reach) {}
+    __host__ __device__ int entries() const { return hi - lo + 1 + 2 * kPad; }
+};
+
+__device__ inline int row_int(const void* p, int bytes, int b, int lo, int hi) {
+    const int64_t v = bytes == 8 ? ((const int64_t*)p)[b] : (int64_t)((const int32_t*)p)[b];
+    return (int)(v < lo ? lo : v > hi ? hi : v);
+}
+// Position of the row's first query, and how many of its keys count.
+__device__ inline int first_position(const Args& a, int b) {
+    return a.start ? row_int(a.start, a.start_bytes, b, -(1 << 30), 1 << 30) : a.start0;
+}
+__device__ inline int key_count(const Args& a, int b) {
+    return a.lengths ? row_int(a.lengths, a.lengths_bytes, b, 0, a.Lk) : a.Lk;
+}
+
+__device__ inline int bucket_of(const Args& a, int d) {
+    const int n = d < 0 ? -d : d;
+    int lo = 0, hi = a.n_starts - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.starts[mid] <= n) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo + (!a.causal && d < 0 ? a.n_starts : 0);
+}
+
+// tab[i] = log2(e) bias of distance lo - kPad + i (clamped to lo .. hi), by all threads.
+__device__ inline void fill_table(const Args& a, int h, float* tab) {
+    const Reach r(a);
+    for (int i = threadIdx.x; i < r.entries(); i += kThreads) {
+        const int d = r.lo - kPad + i;
+        const int64_t at = (int64_t)bucket_of(a, d < r.lo ? r.lo : d > r.hi ? r.hi : d) * a.H + h;
+        tab[i] = kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
+    }
+}
+
+// ---- staged tiles: rows of HD elements, 16 bytes of padding after each -------------------------
+
+template <typename T, int HD>
+struct Tile {
+    static constexpr int kStride = HD + 16 / (int)sizeof(T);
+    static constexpr int kN = Ty<T>::kKeys;
+    static constexpr int kPerRow = HD * (int)sizeof(T) / 16;
+    static constexpr int kVecs = kN * kPerRow / kThreads;   // 16-byte pieces of a thread
+    static constexpr int kBytes = kN * kStride * (int)sizeof(T);
+    static_assert(kN * kPerRow % kThreads == 0, "pieces");
+
+    // This thread's pieces of rows row0 .. row0 + kN - 1; rows from `rows` on are zero.
+    static __device__ void load(const T* base, int64_t sl, int row0, int rows, f32x4* v) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int p = i * kThreads + threadIdx.x;
+            const int r = row0 + p / kPerRow, c = p % kPerRow;
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+            v[i] = zero;
+            if (r < rows) v[i] = *reinterpret_cast<const f32x4*>(base + (int64_t)r * sl + c * (16 / sizeof(T)));
+        }
+    }
+    static __device__ void store(T* tile, const f32x4* v) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int p = i * kThreads + threadIdx.x;
+            *reinterpret_cast<f32x4*>(tile + (p / kPerRow) * kStride + (p % kPerRow) * (16 / sizeof(T))) = v[i];
+        }
+    }
+    // Operand with the tile's rows row0 + lane % 32 and channels 16 c ..: a lane's 8 are adjacent.
+    static __device__ typename Ty<T>::Frag rows(const T* tile, int row0, int c) {
+        const int lane = threadIdx.x & 63;
+        return *reinterpret_cast<const typename Ty<T>::FragMem*>(tile + (row0 + (lane & 31)) * kStride + 16 * c + 8 * (lane >> 5));
+    }
+};
+
+// Operand with channels d0 + lane % 32 and a tile's rows row0 + (the slots' order above).
+template <int STRIDE>
+__device__ inline bf16x8 cols_bf16(const __bf16* tile, int row0, int d0) {
+    // 16 lanes read 4 rows of 16 channels, 8 bytes each, and get 4 rows of one channel each
+    const int lane = threadIdx.x & 63;
+    const __bf16* p = tile + (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * STRIDE + d0 + (lane & 16) + 4 * (lane & 3);
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(__attribute__((address_space(3))) void*)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(__attribute__((address_space(3))) void*)(p + 8 * STRIDE));
+    const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int STRIDE>
+__device__ inline f32x8 cols_f32(const float* tile, int row0, int d0) {
+    const int lane = threadIdx.x & 63;
+    const float* p = tile + (row0 + 4 * (lane >> 5)) * STRIDE + d0 + (lane & 31);
+    f32x8 f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = p[(8 * (e / 4) + e % 4) * STRIDE];
+    return f;
+}
+template <typename T, int HD>
+__device__ inline typename Ty<T>::Frag cols_of(const T* tile, int row0, int d0) {
+    if constexpr (sizeof(T) == 2) return cols_bf16<Tile<T, HD>::kStride>(tile, row0, d0);
+    else return cols_f32<Tile<T, HD>::kStride>(tile, row0, d0);
+}
+
+// Rows of a wave in registers: row r0 + lane % 32, channels 16 c + 8 (lane / 32) ..; rows from
+// `rows` on are zero.
+template <typename T, int HD>
+__device__ inline void load_frags(const T* base, int64_t sl, int r0, int rows, typename Ty<T>::Frag* f) {
+    const int lane = threadIdx.x & 63;
+    const int r = r0 + (lane & 31);
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) {
+        typename Ty<T>::Frag z;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = (T)0.f;
+        f[c] = z;
+        if (r < rows)
+            f[c] = *reinterpret_cast<const typename Ty<T>::FragMem*>(base + (int64_t)r * sl + 16 * c + 8 * (lane >> 5));
+    }
+}
+
+// Eight of a block's 16 values as an operand of the next product (rounded to nearest in bf16).
+template <typename T>
+__device__ inline typename Ty<T>::Frag to_frag(const f32x16& x, int c) {
+    typename Ty<T>::Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (T)x[8 * c + e];
+    return f;
+}
+
+// A 32 x 32 result block (channels d0 .. by rows) into the wave's rows.
+template <typename T>
+__device__ inline void store_block(T* row, int d0, const f32x16& x, float mul) {
+    const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        typename Ty<T>::Quad v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(x[4 * r + e] * mul);
+        *reinterpret_cast<typename Ty<T>::Quad*>(row + d0 + 8 * r + 4 * g) = v;
+    }
+}
+
+__device__ inline f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// Row of a block's value r in this lane.
+__device__ inline int row_of(int r) { return 8 * (r / 4) + 4 * ((threadIdx.x & 63) >> 5) + r % 4; }
+
+}  // namespace battn
+}  // namespace mb

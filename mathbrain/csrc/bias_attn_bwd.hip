@@ -1,0 +1,416 @@
+// Backward of the attention with a learned bias by distance buckets.
+//
+//   p_ij = exp2(t_ij - lse_i),  delta_i = dO_i . o_i,  ds_ij = p_ij (dO_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dO_i,
+//   dbias[n, h] = sum over the pairs of bucket n of ds_ij
+//
+// Two passes over the pairs, one that owns queries (dq, delta, dbias) and one that owns keys (dk,
+// dv), so that every sum has one owner and a fixed order: 7 products of a pair instead of 5, and
+// neither atomics in memory nor fp32 copies of dq.
+#include "bias_attn_host.h"
+
+#include <algorithm>
+
+namespace mb {
+namespace battn {
+namespace {
+
+// Sum of a value over the wave's 64 lanes.
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// dbias: a block of pairs that lies within one bucket adds to a register; any other adds each
+// pair to its distance's entry in LDS.  Every half wave has entries of its own: the lanes of one
+// instruction then hit different ones, and the order of the additions is fixed.  In the end the
+// entries are added by buckets, into the workgroup's own row of a workspace.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) bias_attn_dq_kernel(const Args a) {
+    using X = Ty<T>;
+    using Tl = Tile<T, HD>;
+    constexpr int KT = X::kKeys;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ float far[4][2];
+    const Reach reach(a);
+    const int entries = reach.entries();
+    float* tab = reinterpret_cast<float*>(smem + 4 * Tl::kBytes);
+    float* hist = tab + entries;
+    auto ktile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s) * Tl::kBytes); };
+    auto vtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bh = blockIdx.x / a.nq, qb = a.nq - 1 - (int)(blockIdx.x % a.nq);
+    const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+    const int len = key_count(a, b), p0 = first_position(a, b);
+    const int w0 = qb * kRows + wave * kWaveRows;
+    const int i = w0 + (lane & 31), pos = p0 + i;
+    const int last = min(a.Lq, (qb + 1) * kRows) - 1;
+    const int kend = a.causal ? min(len, p0 + last + 1) : len;
+    const int wend = w0 >= a.Lq ? 0 : a.causal ? min(len, p0 + min(a.Lq, w0 + kWaveRows)) : len;
+    const int tiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+    const float sl2 = a.scale * kLog2e;
+    const bool want_bias = a.dbias_part != nullptr;
+
+    const T* kbase = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+    const T* vbase = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    typename X::Frag qf[HD / 16], gf[HD / 16];
+    float delta = 0.f;
+    {
+        load_frags<T, HD>((const T*)a.o + b * a.o_sb + h * a.o_sh, a.o_sl, w0, a.Lq, qf);
+        load_frags<T, HD>((const T*)a.d_o + b * a.do_sb + h * a.do_sh, a.do_sl, w0, a.Lq, gf);
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)qf[c][e], (float)gf[c][e], delta);
+        delta += __shfl_xor(delta, 32, 64);
+    }
+    load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
+    float lse = INFINITY;
+    if (i < a.Lq) {
+        lse = a.lse[(int64_t)bh * a.Lq + i];
+        if (lane < 32) a.delta[(int64_t)bh * a.Lq + i] = delta;
+    }
+    fill_table(a, h, tab);
+    if (want_bias)
+        for (int n = threadIdx.x; n < 8 * entries; n += kThreads) hist[n] = 0.f;
+    float* mine = hist + (2 * wave + (lane >> 5)) * entries;
+    float far_hi = 0.f, far_lo = 0.f;
+
+    f32x16 dq[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) dq[d] = zero16();
+    f32x4 kv[Tl::kVecs], vv[Tl::kVecs];
+    if (tiles > 0) {
+        Tl::load(kbase, a.k_sl, 0, len, kv);
+        Tl::load(vbase, a.v_sl, 0, len, vv);
+        Tl::store(ktile(0), kv);
+        Tl::store(vtile(0), vv);
+    }
+    __syncthreads();
+    for (int t = 0; t < tiles; ++t) {
+        const int s = t & 1;
+        if (t + 1 < tiles) {
+            Tl::load(kbase, a.k_sl, (t + 1) * KT, len, kv);
+            Tl::load(vbase, a.v_sl, (t + 1) * KT, len, vv);
+        }
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+            const int jb = t * KT + 32 * u;
+            if (jb >= wend) break;
+            f32x16 x = zero16(), y = zero16();
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                x = X::mma(Tl::rows(ktile(s), 32 * u, c), qf[c], x);
+                y = X::mma(Tl::rows(vtile(s), 32 * u, c), gf[c], y);
+            }
+            const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
+            const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
+            const int at = kPad - reach.lo + (pos - jb);
+            if (one) {
+                const float bias = tab[kPad + (above ? reach.hi - reach.lo : 0)];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, bias);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, tab[at - row_of(r)]);
+            }
+            if ((a.causal && dlo < 0) || jb + 32 > len) {
+                const int most = a.causal ? min(len, pos + 1) : len;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (jb + row_of(r) >= most) x[r] = -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
+            if (want_bias) {
+                if (one) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum += x[r];
+                    (above ? far_hi : far_lo) += sum;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) atomicAdd(mine + at - row_of(r), x[r]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const typename X::Frag f = to_frag<T>(x, c);
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d)
+                    dq[d] = X::mma(cols_of<T, HD>(ktile(s), 32 * u + 16 * c, 32 * d), f, dq[d]);
+            }
+        }
+        if (t + 1 < tiles) {
+            Tl::store(ktile(s ^ 1), kv);
+            Tl::store(vtile(s ^ 1), vv);
+        }
+        __syncthreads();
+    }
+    if (i < a.Lq) {
+        T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) store_block<T>(row, 32 * d, dq[d], a.scale);
+    }
+    if (!want_bias) return;
+    far_hi = wave_sum(far_hi);
+    far_lo = wave_sum(far_lo);
+    if (lane == 0) far[wave][0] = far_hi, far[wave][1] = far_lo;
+    for (int n = threadIdx.x; n < entries; n += kThreads) {   // all waves' adds lie before the loop's last barrier
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += hist[w * entries + n];
+        hist[n] = v;
+    }
+    __syncthreads();
+    float* part = a.dbias_part + ((int64_t)h * a.B * a.nq + (int64_t)b * a.nq + qb) * a.buckets;
+    for (int n = wave; n < a.buckets; n += 4) {
+        const bool back = n >= a.n_starts;        // keys behind the query's position
+        const int m = back ? n - a.n_starts : n;
+        const bool end = m == a.n_starts - 1;
+        // its distances' entries, those of the padding with the last bucket's
+        int e0 = a.starts[m], e1 = end ? reach.hi + kPad : a.starts[m + 1] - 1;
+        if (back) {
+            const int near = max(e0, 1);
+            e0 = -e1, e1 = -near;
+        }
+        float v = 0.f;
+        for (int e = e0 - reach.lo + kPad + lane; e <= e1 - reach.lo + kPad; e += 64) v += hist[e];
+        v = wave_sum(v);
+        // whole blocks: at or above the reach, and at or below its lower end, which is distance 0 in
+        // a causal table
+        const bool below = a.causal ? n == 0 : back && end;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (end && !back) v += far[w][0];
+            if (below) v += far[w][1];
+        }
+        if (lane == 0) part[n] = v;
+    }
+}
+
+// A workgroup takes 128 keys of one key head, 32 to a wave, and walks the queries of all query
+// heads that share it.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) bias_attn_dkv_kernel(const Args a) {
+    using X = Ty<T>;
+    using Tl = Tile<T, HD>;
+    constexpr int QT = X::kKeys;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];
+    float* tab = reinterpret_cast<float*>(smem + 4 * Tl::kBytes);
+    auto qtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s) * Tl::kBytes); };
+    auto gtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+    const int nk = (a.Lk + kRows - 1) / kRows;
+    const int bh = blockIdx.x / nk, kb = blockIdx.x % nk;
+    const int b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
+    const Reach reach(a);
+    const int len = key_count(a, b), p0 = first_position(a, b);
+    const int k0 = kb * kRows, w0 = k0 + wave * kWaveRows;
+    const int j = w0 + (lane & 31);
+    // queries from the first one that sees key k0
+    const int first = a.causal ? max(0, k0 - p0) / QT : 0;
+    const int tiles = k0 < len ? (a.Lq + QT - 1) / QT : 0;
+    const float sl2 = a.scale * kLog2e;
+
+    typename X::Frag kf[HD / 16], vf[HD / 16];
+    load_frags<T, HD>((const T*)a.k + b * a.k_sb + hk * a.k_sh, a.k_sl, w0, len, kf);
+    load_frags<T, HD>((const T*)a.v + b * a.v_sb + hk * a.v_sh, a.v_sl, w0, len, vf);
+    f32x16 dk[HD / 32], dv[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) dk[d] = zero16(), dv[d] = zero16();
+
+    f32x4 qv[Tl::kVecs], gv[Tl::kVecs];
+    float st = 0.f;
+    for (int hh = 0; hh < group; ++hh) {
+        const int h = hk * group + hh;
+        const T* qbase = (const T*)a.q + b * a.q_sb + h * a.q_sh;
+        const T* gbase = (const T*)a.d_o + b * a.do_sb + h * a.do_sh;
+        const float* lse = a.lse + ((int64_t)b * a.H + h) * a.Lq;
+        const float* delta = a.delta + ((int64_t)b * a.H + h) * a.Lq;
+        auto load = [&](int t) {
+            Tl::load(qbase, a.q_sl, t * QT, a.Lq, qv);
+            Tl::load(gbase, a.do_sl, t * QT, a.Lq, gv);
+            const int i = t * QT + (int)(threadIdx.x % QT);   // past the end: no probability
+            if (threadIdx.x < QT) st = i < a.Lq ? lse[i] : INFINITY;
+            else if (threadIdx.x < 2 * QT) st = i < a.Lq ? delta[i] : 0.f;
+        };
+        auto store = [&](int s) {
+            Tl::store(qtile(s), qv);
+            Tl::store(gtile(s), gv);
+            if (threadIdx.x < 2 * QT) stat[s][threadIdx.x / QT][threadIdx.x % QT] = st;
+        };
+        fill_table(a, h, tab);   // the previous head's last barrier lies behind its reads
+        if (first < tiles) {
+            load(first);
+            store(first & 1);
+        }
+        __syncthreads();
+        for (int t = first; t < tiles; ++t) {
+            const int s = t & 1;
+            if (t + 1 < tiles) load(t + 1);
+#pragma unroll
+            for (int u = 0; u < QT / 32; ++u) {
+                const int ib = t * QT + 32 * u;
+                if (ib >= a.Lq || w0 >= len || (a.causal && p0 + ib + 31 < w0)) continue;
+                f32x16 x = zero16(), y = zero16();
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    x = X::mma(Tl::rows(qtile(s), 32 * u, c), kf[c], x);
+                    y = X::mma(Tl::rows(gtile(s), 32 * u, c), vf[c], y);
+                }
+                const int dlo = p0 + ib - w0 - 31, dhi = p0 + ib + 31 - w0;
+                const bool above = dlo >= reach.hi;
+                if (above || dhi <= reach.lo) {
+                    const float bias = tab[kPad + (above ? reach.hi - reach.lo : 0)];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, bias);
+                } else {
+                    const float* at = tab + kPad - reach.lo + (p0 + ib - j);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, at[row_of(r)]);
+                }
+                if ((a.causal && dlo < 0) || w0 + 32 > len) {
+                    const int least = j >= len ? 0x7fffffff : a.causal ? j - p0 : -0x7fffffff;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (ib + row_of(r) < least) x[r] = -INFINITY;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[s][0][32 * u + 8 * r + 4 * g]);
+                    const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[s][1][32 * u + 8 * r + 4 * g]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[4 * r + e] = __builtin_amdgcn_exp2f(x[4 * r + e] - ls[e]);
+                        y[4 * r + e] = x[4 * r + e] * (y[4 * r + e] - de[e]);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const typename X::Frag p = to_frag<T>(x, c), ds = to_frag<T>(y, c);
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d) {
+                        dv[d] = X::mma(cols_of<T, HD>(gtile(s), 32 * u + 16 * c, 32 * d), p, dv[d]);
+                        dk[d] = X::mma(cols_of<T, HD>(qtile(s), 32 * u + 16 * c, 32 * d), ds, dk[d]);
+                    }
+                }
+            }
+            if (t + 1 < tiles) store(s ^ 1);
+            __syncthreads();
+        }
+    }
+    if (j < a.Lk) {
+        T* krow = (T*)a.dk + b * a.dk_sb + hk * a.dk_sh + (int64_t)j * a.dk_sl;
+        T* vrow = (T*)a.dv + b * a.dv_sb + hk * a.dv_sh + (int64_t)j * a.dv_sl;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+            store_block<T>(krow, 32 * d, dk[d], a.scale);
+            store_block<T>(vrow, 32 * d, dv[d], 1.f);
+        }
+    }
+}
+
+// dbias[n, h] = the sum of part[h, :, n], in a fixed order: a workgroup per head, strips of rows.
+__global__ void __launch_bounds__(kThreads) bias_attn_dbias_kernel(const float* __restrict__ part, int rows, int buckets,
+                                                                   int H, int bf16, void* dbias) {
+    __shared__ float sums[kThreads];
+    const int h = blockIdx.x;
+    const int strips = kThreads / buckets;   // at least one: buckets <= 256
+    const int n = threadIdx.x % buckets, strip = threadIdx.x / buckets;
+    float v = 0.f;
+    if (strip < strips)
+        for (int r = strip; r < rows; r += strips) v += part[((int64_t)h * rows + r) * buckets + n];
+    sums[threadIdx.x] = v;
+    __syncthreads();
+    if (strip == 0) {
+        for (int k = 1; k < strips; ++k) v += sums[k * buckets + n];
+        const int64_t at = (int64_t)n * H + h;
+        if (bf16) ((__bf16*)dbias)[at] = (__bf16)v;
+        else ((float*)dbias)[at] = v;
+    }
+}
+static_assert(2 * kMaxStarts <= kThreads, "a thread for every bucket");
+
+template <typename T, int HD>
+int launch(const Args& a, hipStream_t st) {
+    const int entries = Reach(a).entries();
+    const int base = 4 * Tile<T, HD>::kBytes + entries * (int)sizeof(float);
+    const int lds_q = base + (a.dbias_part ? 8 * entries * (int)sizeof(float) : 0);
+    if (a.Lq > 0) {
+        if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q)) return rc;
+        hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds_q, st, a);
+    }
+    if (a.Lk > 0) {
+        if (const int rc = allow_lds((const void*)bias_attn_dkv_kernel<T, HD>, base)) return rc;
+        const int nk = (a.Lk + kRows - 1) / kRows;
+        hipLaunchKernelGGL((bias_attn_dkv_kernel<T, HD>), dim3((unsigned)(a.B * a.Hk * nk)), dim3(kThreads), base, st, a);
+    }
+    return check_launch("mb_bias_attn_bwd");
+}
+
+int64_t padded(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
+
+}  // namespace
+}  // namespace battn
+}  // namespace mb
+
+using namespace mb;
+using namespace mb::battn;
+
+extern "C" int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets) {
+    if (B < 1 || H < 1 || Lq < 1 || buckets < 1) return 0;
+    const int64_t nq = ((int64_t)Lq + kRows - 1) / kRows;
+    return (padded((int64_t)B * H * Lq) + (int64_t)H * B * nq * buckets) * (int64_t)sizeof(float);
+}
+
+extern "C" int mb_bias_attn_bwd(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
+                                const int64_t* v_st, const void* bias, int bias_dtype, int buckets,
+                                const int32_t* starts, int n_starts, const void* lengths, int lengths_bytes,
+                                const void* q_start, int q_start_bytes, int64_t q_start0, int B, int H, int Hk, int Lq,
+                                int Lk, int hd, float scale, int causal, int dtype, const void* o, const int64_t* o_st,
+                                const void* d_o, const int64_t* do_st, const float* lse, void* dq, const int64_t* dq_st,
+                                void* dk, const int64_t* dk_st, void* dv, const int64_t* dv_st, void* dbias,
+                                void* workspace, int64_t workspace_bytes, void* stream) {
+    Args a = {};
+    if (const int rc = fill_args("mb_bias_attn_bwd", a, q, q_st, k, k_st, v, v_st, bias, bias_dtype, buckets, starts,
+                                 n_starts, lengths, lengths_bytes, q_start, q_start_bytes, q_start0, B, H, Hk, Lq, Lk,
+                                 hd, scale, causal, dtype))
+        return rc;
+    const int64_t need = mb_bias_attn_bwd_workspace(B, H, Lq, buckets);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MB_ERR_WORKSPACE, "mb_bias_attn_bwd: workspace of %lld bytes, %lld are needed",
+                    (long long)workspace_bytes, (long long)need);
+    if (B > 0 && Lq > 0) {
+        MB_REQUIRE(o && o_st && d_o && do_st && lse && dq && dq_st, "mb_bias_attn_bwd: null pointer argument");
+        MB_REQUIRE(rows16(o, o_st, dtype) && rows16(d_o, do_st, dtype) && rows16(dq, dq_st, dtype),
+                   "mb_bias_attn_bwd: rows must begin at multiples of 16 bytes");
+        a.o = o, a.o_sb = o_st[0], a.o_sh = o_st[1], a.o_sl = o_st[2];
+        a.d_o = d_o, a.do_sb = do_st[0], a.do_sh = do_st[1], a.do_sl = do_st[2];
+        a.out = dq, a.out_sb = dq_st[0], a.out_sh = dq_st[1], a.out_sl = dq_st[2];
+    }
+    if (B > 0 && Lk > 0) {
+        MB_REQUIRE(dk && dk_st && dv && dv_st, "mb_bias_attn_bwd: null pointer argument");
+        MB_REQUIRE(rows16(dk, dk_st, dtype) && rows16(dv, dv_st, dtype), "mb_bias_attn_bwd: rows must begin at multiples of 16 bytes");
+        a.dk = dk, a.dk_sb = dk_st[0], a.dk_sh = dk_st[1], a.dk_sl = dk_st[2];
+        a.dv = dv, a.dv_sb = dv_st[0], a.dv_sh = dv_st[1], a.dv_sl = dv_st[2];
+    }
+    a.lse = const_cast<float*>(lse);
+    a.delta = (float*)workspace;
+    a.dbias_part = dbias && need > 0 ? (float*)workspace + padded((int64_t)B * H * Lq) : nullptr;
+    hipStream_t st = (hipStream_t)stream;
+    if (B > 0) {
+        const int rc = dtype == MB_DTYPE_F32
+                           ? (hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st))
+                           : (hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st));
+        if (rc) return rc;
+    }
+    if (dbias)
+        hipLaunchKernelGGL(bias_attn_dbias_kernel, dim3(H), dim3(kThreads), 0, st, a.dbias_part,
+                           a.dbias_part ? a.B * a.nq : 0, buckets, H, a.bias_bf16, dbias);
+    return check_launch("mb_bias_attn_bwd");
+}

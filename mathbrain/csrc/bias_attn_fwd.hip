@@ -1,0 +1,170 @@
+// Forward of the attention with a learned bias by distance buckets.
+#include "bias_attn_host.h"
+
+namespace mb {
+namespace battn {
+namespace {
+
+// A workgroup takes 128 queries of one head, 32 to a wave, and walks the keys in tiles that all
+// four waves read out of LDS; the next tile's rows are on their way from memory meanwhile.
+// Running maximum, sum and output are in fp32; the probabilities are rounded to bf16 for the
+// product with V where the inputs are bf16 (half a step of 2^-8 of each), the sum is not.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) bias_attn_fwd_kernel(const Args a) {
+    using X = Ty<T>;
+    using Tl = Tile<T, HD>;
+    constexpr int KT = X::kKeys;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* tab = reinterpret_cast<float*>(smem + 4 * Tl::kBytes);
+    auto ktile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s) * Tl::kBytes); };
+    auto vtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bh = blockIdx.x / a.nq, qb = a.nq - 1 - (int)(blockIdx.x % a.nq);
+    const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+    const Reach reach(a);
+    const int len = key_count(a, b), p0 = first_position(a, b);
+    const int w0 = qb * kRows + wave * kWaveRows;   // the wave's first query
+    const int i = w0 + (lane & 31), pos = p0 + i;
+    const int last = min(a.Lq, (qb + 1) * kRows) - 1;
+    const int kend = a.causal ? min(len, p0 + last + 1) : len;
+    const int wend = w0 >= a.Lq ? 0 : a.causal ? min(len, p0 + min(a.Lq, w0 + kWaveRows)) : len;
+    const int tiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+    const float sl2 = a.scale * kLog2e;
+
+    const T* kbase = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+    const T* vbase = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    typename X::Frag qf[HD / 16];
+    load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
+    fill_table(a, h, tab);
+
+    f32x16 o[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) o[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+
+    f32x4 kv[Tl::kVecs], vv[Tl::kVecs];
+    if (tiles > 0) {
+        Tl::load(kbase, a.k_sl, 0, len, kv);
+        Tl::load(vbase, a.v_sl, 0, len, vv);
+        Tl::store(ktile(0), kv);
+        Tl::store(vtile(0), vv);
+    }
+    __syncthreads();
+    for (int t = 0; t < tiles; ++t) {
+        const int s = t & 1;
+        if (t + 1 < tiles) {
+            Tl::load(kbase, a.k_sl, (t + 1) * KT, len, kv);
+            Tl::load(vbase, a.v_sl, (t + 1) * KT, len, vv);
+        }
+        const int j0 = t * KT;
+        if (j0 < wend) {
+            f32x16 x[KT / 32];
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u) {
+                const int jb = j0 + 32 * u;
+                x[u] = zero16();
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) x[u] = X::mma(Tl::rows(ktile(s), 32 * u, c), qf[c], x[u]);
+                const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
+                if (dlo >= reach.hi || dhi <= reach.lo) {  // one bias for the whole block
+                    const float bias = tab[kPad + (dlo >= reach.hi ? reach.hi - reach.lo : 0)];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, bias);
+                } else {
+                    // dlo > lo - 63 and dhi < hi + 63: within the padded table, masked pairs too
+                    const float* at = tab + kPad - reach.lo + (pos - jb);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, at[-row_of(r)]);
+                }
+                if ((a.causal && dlo < 0) || jb + 32 > len) {
+                    const int most = a.causal ? min(len, pos + 1) : len;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (jb + row_of(r) >= most) x[u][r] = -INFINITY;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, x[u][r]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m, top);
+            const float mu = mn == -INFINITY ? 0.f : mn;   // no key yet: every term is 0
+            const float alpha = __builtin_amdgcn_exp2f(m - mu);
+            m = mn;
+            if (__any(alpha != 1.f)) {
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+            }
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - mu);
+                    l += x[u][r];
+                }
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const typename X::Frag p = to_frag<T>(x[u], c);
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d)
+                        o[d] = X::mma(cols_of<T, HD>(vtile(s), 32 * u + 16 * c, 32 * d), p, o[d]);
+                }
+        }
+        if (t + 1 < tiles) {
+            Tl::store(ktile(s ^ 1), kv);
+            Tl::store(vtile(s ^ 1), vv);
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (i < a.Lq) {
+        const float inv = l > 0.f ? 1.0f / l : 0.f;   // a row without keys: zeros
+        T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) store_block<T>(row, 32 * d, o[d], inv);
+        if (a.lse && lane < 32)
+            a.lse[(int64_t)bh * a.Lq + i] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    }
+}
+
+template <typename T, int HD>
+int launch(const Args& a, hipStream_t st) {
+    const int lds = 4 * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
+    if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD>, lds)) return rc;
+    hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds, st, a);
+    return check_launch("mb_bias_attn_fwd");
+}
+
+}  // namespace
+}  // namespace battn
+}  // namespace mb
+
+using namespace mb;
+using namespace mb::battn;
+
+extern "C" int mb_bias_attn_fwd(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
+                                const int64_t* v_st, const void* bias, int bias_dtype, int buckets,
+                                const int32_t* starts, int n_starts, const void* lengths, int lengths_bytes,
+                                const void* q_start, int q_start_bytes, int64_t q_start0, int B, int H, int Hk, int Lq,
+                                int Lk, int hd, float scale, int causal, int dtype, void* o, const int64_t* o_st,
+                                float* lse, void* stream) {
+    Args a = {};
+    if (const int rc = fill_args("mb_bias_attn_fwd", a, q, q_st, k, k_st, v, v_st, bias, bias_dtype, buckets, starts,
+                                 n_starts, lengths, lengths_bytes, q_start, q_start_bytes, q_start0, B, H, Hk, Lq, Lk,
+                                 hd, scale, causal, dtype))
+        return rc;
+    if (B == 0 || Lq == 0) return MB_OK;
+    MB_REQUIRE(o && o_st, "mb_bias_attn_fwd: null pointer argument");
+    MB_REQUIRE(rows16(o, o_st, dtype), "mb_bias_attn_fwd: o's rows must begin at multiples of 16 bytes");
+    a.out = o, a.out_sb = o_st[0], a.out_sh = o_st[1], a.out_sl = o_st[2];
+    a.lse = lse;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == MB_DTYPE_F32) return hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st);
+    return hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st);
+}
