@@ -137,6 +137,18 @@ def call(name, *args):
         raise HipKernelError(f"{name}: {kind}: {msg}")
 
 
+def call_on(dev, name, *args):
+    """call(name, *args, stream) on the current stream of device `dev`, whichever device is
+    current.  For entry points that take a few microseconds: the device is switched only where
+    it has to be."""
+    index = dev.index
+    if index is None or index == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        return
+    with torch.cuda.device(dev):
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def ptr(t):
     """Device address of a tensor (None for None)."""
     return None if t is None else ctypes.c_void_p(t.data_ptr())

@@ -9,12 +9,16 @@ channel pairs (2i, 2i+1) of each head by t * theta^(-2i/hd), written with real c
 tables instead of the reference's complex multiply (the same rotation).
 
 ``qk_norm=True`` (not in the reference) norms every query and key head before the rotation,
-in the rotation's own pass (``qk_norm_rotary``).
+in the rotation's own pass (``qk_norm_rotary``).  ``rel_buckets=n`` (not in the reference)
+adds a learned bias by distance buckets to every layer's scores, one table [n, heads] for all
+layers, in the attention that reads it (``relative_bias_attention``, which replaces torch's
+there; its probabilities are not dropped out, the block's output is).
 """
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .bias_attention import relative_bias_attention
 from .model import RMSNorm, SwiGLU
 from .qk_norm import qk_norm_rotary
 
@@ -56,7 +60,7 @@ class CausalSelfAttention(nn.Module):
             self.k_norm = RMSNorm(self.head_dim)
         self.qk_norm = qk_norm
 
-    def forward(self, x, cos, sin):
+    def forward(self, x, cos, sin, rel_bias=None, rel_max_distance=128):
         B, L, D = x.shape
         shape = (B, L, self.n_heads, self.head_dim)
         q, k = self.wq(x).view(shape), self.wk(x).view(shape)
@@ -66,8 +70,11 @@ class CausalSelfAttention(nn.Module):
             q, k = rotate(q, cos, sin), rotate(k, cos, sin)
         q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = self.wv(x).view(shape).transpose(1, 2)
-        out = F.scaled_dot_product_attention(q, k, v, is_causal=True,
-                                             dropout_p=self.resid_dropout.p if self.training else 0.0)
+        if rel_bias is not None:
+            out = relative_bias_attention(q, k, v, rel_bias, rel_max_distance)
+        else:
+            out = F.scaled_dot_product_attention(q, k, v, is_causal=True,
+                                                 dropout_p=self.resid_dropout.p if self.training else 0.0)
         return self.resid_dropout(self.wo(out.transpose(1, 2).reshape(B, L, D)))
 
 
@@ -81,18 +88,21 @@ class RoPETransformerBlock(nn.Module):
         self.ffn_norm = RMSNorm(d_model)
         self.ffn = SwiGLU(d_model, d_ff)
 
-    def forward(self, x, cos, sin):
-        x = x + self.attn(self.attn_norm(x), cos, sin)
+    def forward(self, x, cos, sin, rel_bias=None, rel_max_distance=128):
+        x = x + self.attn(self.attn_norm(x), cos, sin, rel_bias, rel_max_distance)
         return x + self.ffn(self.ffn_norm(x))
 
 
 class RoPETransformerLM(nn.Module):
     """baseline.py:86-129: RoPETransformerLM(vocab_size, d_model, n_layers, n_heads,
     max_seq_len=4096, dropout=0.1); forward(x [B, L]) -> logits [B, L, vocab_size].
-    ``qk_norm``: RMS norms of every query and key head (head_dim 32, 64 or 128)."""
+    ``qk_norm``: RMS norms of every query and key head.  ``rel_buckets``: a learned bias by that
+    many distance buckets, up to ``rel_max_distance`` (0: none).  Both take head_dim 32, 64 or
+    128; the bias starts as zeros."""
 
     def __init__(self, vocab_size: int, d_model: int, n_layers: int, n_heads: int,
-                 max_seq_len: int = 4096, dropout: float = 0.1, qk_norm: bool = False):
+                 max_seq_len: int = 4096, dropout: float = 0.1, qk_norm: bool = False,
+                 rel_buckets: int = 0, rel_max_distance: int = 128):
         super().__init__()
         self.vocab_size = vocab_size
         self.d_model = d_model
@@ -103,6 +113,8 @@ class RoPETransformerLM(nn.Module):
         self.final_norm = RMSNorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)
         self.lm_head.weight = self.embed.weight
+        self.rel_bias = nn.Parameter(torch.zeros(rel_buckets, n_heads)) if rel_buckets else None
+        self.rel_max_distance = rel_max_distance
         cos, sin = rotary_tables(d_model // n_heads, max_seq_len)
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
@@ -112,5 +124,5 @@ class RoPETransformerLM(nn.Module):
         cos, sin = self.rope_cos[:L], self.rope_sin[:L]
         h = self.embed(x)
         for layer in self.layers:
-            h = layer(h, cos, sin)
+            h = layer(h, cos, sin, self.rel_bias, self.rel_max_distance)
         return self.lm_head(self.final_norm(h))

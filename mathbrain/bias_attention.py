@@ -60,9 +60,8 @@ def _starts_array(num_buckets, max_distance, causal):
 
 def _rows16(x):
     """x with the channels next to each other and rows at multiples of 16 bytes."""
-    size = x.element_size()
     sb, sh, sl, sd = x.stride()
-    if sd == 1 and not (x.data_ptr() | sb * size | sh * size | sl * size) & 15:
+    if sd == 1 and not (x.data_ptr() | (sb | sh | sl) * x.element_size()) & 15:
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
 
@@ -105,13 +104,12 @@ def bias_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     backward, empty unless wanted."""
     dev = q.device
     B, H, Lq, hd = q.shape
-    q, k, v = _rows16(q.detach()), _rows16(k.detach()), _rows16(v.detach())
-    bias = bias.detach().contiguous()
+    q, k, v, bias = _rows16(q), _rows16(k), _rows16(v), bias.contiguous()
     o = _heads_last(B, H, Lq, hd, q)
     lse = torch.empty((B, H, Lq) if want_lse else (0,), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("mb_bias_attn_fwd", *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
-                  o.data_ptr(), _st(o), lse.data_ptr() if want_lse else None, _lib.stream(dev))
+    _lib.call_on(dev, "mb_bias_attn_fwd",
+                 *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
+                 o.data_ptr(), _st(o), lse.data_ptr() if want_lse else None)
     return o, lse
 
 
@@ -131,18 +129,16 @@ def bias_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     dev = q.device
     B, H, Lq, hd = q.shape
     Hk, Lk = k.shape[1:3]
-    q, k, v, o = (_rows16(x.detach()) for x in (q, k, v, o))
-    d_o = _rows16(d_o.detach().to(q.dtype))
-    bias = bias.detach().contiguous()
+    q, k, v, o, d_o = _rows16(q), _rows16(k), _rows16(v), _rows16(o), _rows16(d_o.to(q.dtype))
+    bias = bias.contiguous()
     dq, dk, dv = _heads_last(B, H, Lq, hd, q), _heads_last(B, Hk, Lk, hd, k), _heads_last(B, Hk, Lk, hd, v)
     dbias = torch.empty_like(bias)
     nbytes = _lib.lib().mb_bias_attn_bwd_workspace(B, H, Lq, bias.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("mb_bias_attn_bwd", *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
-                  o.data_ptr(), _st(o), d_o.data_ptr(), _st(d_o), lse.data_ptr(), dq.data_ptr(), _st(dq),
-                  dk.data_ptr(), _st(dk), dv.data_ptr(), _st(dv), dbias.data_ptr(), ws.data_ptr(), nbytes,
-                  _lib.stream(dev))
+    _lib.call_on(dev, "mb_bias_attn_bwd",
+                 *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
+                 o.data_ptr(), _st(o), d_o.data_ptr(), _st(d_o), lse.data_ptr(), dq.data_ptr(), _st(dq),
+                 dk.data_ptr(), _st(dk), dv.data_ptr(), _st(dv), dbias.data_ptr(), ws.data_ptr(), nbytes)
     return dq, dk, dv, dbias
 
 

@@ -11,7 +11,7 @@ Two launches for every 120 tensors, squares summed in 64 bits in a fixed order, 
 same gradients always give the same norm.  Where the factor is 1 an in-place call writes
 nothing.  fp32 and bf16 tensors, mixed as they come; CPU tensors raise NotImplementedError.
 """
-import ctypes
+import array
 import math
 
 import torch
@@ -33,33 +33,32 @@ def _dense(t):
     return True
 
 
-def _code(t, what):
-    code = _DTYPES.get(t.dtype)
-    if code is None or t.layout is not torch.strided:
+def _codes(tensors, device, what):
+    """The element types of the tensors, which have to be on one GPU (one of this library's types
+    each, dense)."""
+    codes = [_DTYPES.get(t.dtype, -1) for t in tensors]
+    strided = torch.strided
+    if -1 in codes or any([t.layout is not strided for t in tensors]):
+        t = next(t for t, c in zip(tensors, codes) if c < 0 or t.layout is not strided)
         raise ValueError(f"{what}: a {t.layout} tensor of {t.dtype} (supported: dense float32 and bfloat16)")
-    return code
+    index = device.index if device.type == "cuda" else -1
+    if index < 0 or any([t.get_device() != index for t in tensors]):
+        _lib.require_gpu(torch.empty(0, device=device), *tensors, what=what)
+    return array.array("i", codes)
 
 
-def _clip(src, codes, dst, max_norm, what):
+def _clip(src, codes, dst, dst_codes, max_norm, device):
     """The norm of src (element types: codes) as a 0-dim fp32 tensor; dst (None: no scaling) gets
     the scaled values."""
     n = len(src)
-    dev = src[0].device
-    codes = (ctypes.c_int32 * n)(*codes)
-    _lib.require_gpu(*src, what=what)
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in src])
-    srcs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
-    if dst is None or dst is src:
-        dsts, dst_codes = (None, None) if dst is None else (srcs, codes)
-    else:
-        dst_codes = (ctypes.c_int32 * n)(*[_code(t, what) for t in dst])
-        dsts = (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst])
+    sizes = array.array("q", [t.numel() for t in src])
+    srcs = array.array("Q", [t.data_ptr() for t in src])
+    dsts = srcs if dst is src else dst and array.array("Q", [t.data_ptr() for t in dst])
+    at = [a and a.buffer_info()[0] for a in (srcs, codes, dsts, dst_codes, sizes)]
     nbytes = _lib.lib().mb_grad_clip_workspace(n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("mb_grad_clip", srcs, codes, dsts, dst_codes, sizes, n, max_norm, norm.data_ptr(),
-                  ws.data_ptr(), nbytes, _lib.stream(dev))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    _lib.call_on(device, "mb_grad_clip", *at, n, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 
@@ -67,10 +66,11 @@ def _clip(src, codes, dst, max_norm, what):
 def grad_norm(grads):
     """The 2-norm of all tensors together, a 0-dim fp32 tensor; nothing is scaled."""
     grads = list(grads)
-    codes = [_code(g, "grad_norm") for g in grads]
     if not grads:
         return torch.tensor(0.0)
-    return _clip([g if _dense(g) else g.contiguous() for g in grads], codes, None, math.inf, "grad_norm")
+    device = grads[0].device
+    codes = _codes(grads, device, "grad_norm")
+    return _clip([g if _dense(g) else g.contiguous() for g in grads], codes, None, None, math.inf, device)
 
 
 @torch.no_grad()
@@ -87,27 +87,26 @@ def clip_gradients(grads, max_norm, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"{what}: max_norm={max_norm}")
-    codes = [_code(g, what) for g in grads]
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"{what}: {len(out)} outputs for {len(grads)} gradients")
+    if not grads:
+        return torch.tensor(0.0)
+    device = grads[0].device
+    codes = _codes(grads, device, what)
     if out is None:
         for g in grads:
             if not _dense(g):
                 raise ValueError(f"{what}: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or "
                                  "shares its own elements, and cannot be scaled in place")
-        dst = grads
-    else:
-        dst = list(out)
-        if len(dst) != len(grads):
-            raise ValueError(f"{what}: {len(dst)} outputs for {len(grads)} gradients")
-        for g, o in zip(grads, dst):
-            if o.shape != g.shape or not o.is_contiguous():
-                raise ValueError(f"{what}: an output of shape {tuple(o.shape)}, strides {o.stride()} for a gradient "
-                                 f"of shape {tuple(g.shape)}: contiguous tensors of the same shape are wanted")
-        if dst:
-            _lib.require_gpu(grads[0], *dst, what=what)
-        grads = [g.contiguous() for g in grads]
-    if not grads:
-        return torch.tensor(0.0)
-    return _clip(grads, codes, dst, max_norm, what)
+        return _clip(grads, codes, grads, codes, max_norm, device)
+    out_codes = _codes(out, device, what)
+    for g, o in zip(grads, out):
+        if o.shape != g.shape or not o.is_contiguous():
+            raise ValueError(f"{what}: an output of shape {tuple(o.shape)}, strides {o.stride()} for a gradient "
+                             f"of shape {tuple(g.shape)}: contiguous tensors of the same shape are wanted")
+    return _clip([g.contiguous() for g in grads], codes, out, out_codes, max_norm, device)
 
 
 @torch.no_grad()

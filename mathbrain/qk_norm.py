@@ -23,17 +23,20 @@ _DTYPES = {torch.float32: _lib.MB_DTYPE_F32, torch.bfloat16: _lib.MB_DTYPE_BF16}
 
 def _rows16(x):
     """x with the head's channels next to each other and rows at multiples of 16 bytes."""
-    size = x.element_size()
     sb, sl, sh, sd = x.stride()
-    if sd == 1 and not (x.data_ptr() | sb * size | sl * size | sh * size) & 15:
+    if sd == 1 and not (x.data_ptr() | (sb | sl | sh) * x.element_size()) & 15:
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def _weight(w):
+    return w if w.dtype is torch.float32 and w.stride(0) == 1 else w.float().contiguous()
 
 
 def _start_args(start_rows, start):
     if start_rows is None:
         return None, 4, start
-    return _lib.ptr(start_rows), start_rows.element_size(), 0
+    return start_rows.data_ptr(), start_rows.element_size(), 0
 
 
 def _fwd_fake(q, k, q_weight, k_weight, cos, sin, eps, start_rows, start):
@@ -47,16 +50,13 @@ def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     """(q', k'), contiguous."""
     dev = q.device
     B, L, H, hd = q.shape
-    q, k = _rows16(q.detach()), _rows16(k.detach())
-    wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
+    q, k, wq, wk = _rows16(q), _rows16(k), _weight(q_weight), _weight(k_weight)
     qo = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
     ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
     at, size, first = _start_args(start_rows, start)
-    with torch.cuda.device(dev):
-        _lib.call("mb_qk_norm_rotary_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
-                  wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first,
-                  B, L, H, k.shape[2], hd, eps, _DTYPES[q.dtype], qo.data_ptr(), ko.data_ptr(),
-                  _lib.stream(dev))
+    _lib.call_on(dev, "mb_qk_norm_rotary_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                 wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first,
+                 B, L, H, k.shape[2], hd, eps, _DTYPES[q.dtype], qo.data_ptr(), ko.data_ptr())
     return qo, ko
 
 
@@ -74,20 +74,20 @@ def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     dev = q.device
     B, L, H, hd = q.shape
     q, k = _rows16(q.detach()), _rows16(k.detach())
-    gq, gk = _rows16(dq_out.detach().to(q.dtype)), _rows16(dk_out.detach().to(k.dtype))
+    gq, gk = _rows16(dq_out.to(q.dtype)), _rows16(dk_out.to(k.dtype))
     wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
     dq = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
     dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    dw = torch.empty((2, hd), dtype=torch.float32, device=dev)
+    dwq = torch.empty(hd, dtype=torch.float32, device=dev)
+    dwk = torch.empty(hd, dtype=torch.float32, device=dev)
     ws = torch.empty(_lib.lib().mb_qk_norm_rotary_bwd_workspace(B, L, hd), dtype=torch.uint8, device=dev)
     at, size, first = _start_args(start_rows, start)
-    with torch.cuda.device(dev):
-        _lib.call("mb_qk_norm_rotary_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
-                  gq.data_ptr(), *gq.stride()[:3], gk.data_ptr(), *gk.stride()[:3], wq.data_ptr(),
-                  wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first, B, L, H,
-                  k.shape[2], hd, eps, _DTYPES[q.dtype], dq.data_ptr(), dk.data_ptr(), dw.data_ptr(),
-                  dw.data_ptr() + 4 * hd, ws.data_ptr(), ws.numel(), _lib.stream(dev))
-    return dq, dk, dw[0].to(q_weight.dtype), dw[1].to(k_weight.dtype)
+    _lib.call_on(dev, "mb_qk_norm_rotary_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                 gq.data_ptr(), *gq.stride()[:3], gk.data_ptr(), *gk.stride()[:3], wq.data_ptr(),
+                 wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first, B, L, H,
+                 k.shape[2], hd, eps, _DTYPES[q.dtype], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
+                 dwk.data_ptr(), ws.data_ptr(), ws.numel())
+    return dq, dk, dwq.to(q_weight.dtype), dwk.to(k_weight.dtype)
 
 
 class QKNormRotaryFunction(torch.autograd.Function):
