@@ -59,6 +59,13 @@ struct Ty<float> {
     }
 };
 
+// Waves of a SIMD that the registers have to be enough for.  Two (at most 256 registers) keep the
+// matrix instructions' results in VGPRs, where the softmax reads them; with one, the compiler puts
+// them into AGPRs and moves each of them (forward at 4 x 4096, 8 heads x 64: 279 us instead of
+// 131).  Heads of 128 do not fit that way in fp32, nor, with two results (`wide`), in bf16.
+template <typename T, int HD, bool WIDE = false>
+constexpr int waves_per_simd() { return HD == 128 && (WIDE || sizeof(T) == 4) ? 1 : 2; }
+
 struct Args {
     const void *q, *k, *v, *o, *d_o;        // o, d_o: backward
     int64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl, o_sb, o_sh, o_sl, do_sb, do_sh, do_sl;
@@ -217,6 +224,19 @@ __device__ inline void store_block(T* row, int d0, const f32x16& x, float mul) {
         for (int e = 0; e < 4; ++e) v[e] = (T)(x[4 * r + e] * mul);
         *reinterpret_cast<typename Ty<T>::Quad*>(row + d0 + 8 * r + 4 * g) = v;
     }
+}
+
+// The workgroup's row block and head.  Blocks with the most pairs go first (`first_most`: block 0,
+// else the last one), all heads of a block position one after another: a head's blocks then land
+// on one XCD where the heads are a multiple of 8, and read its keys out of that L2.  Every second
+// 256 workgroups (one for each CU) run backwards in steps of 8, so that a CU's share of a grid
+// that is resident at once comes out even.
+__device__ inline void place(int heads, int blocks, bool first_most, int& bh, int& blk) {
+    int id = blockIdx.x;
+    if ((id & 256) && (id | 255) < heads * blocks) id = (id & ~255) + (31 - ((id >> 3) & 31)) * 8 + (id & 7);
+    bh = id % heads;
+    blk = id / heads;
+    if (!first_most) blk = blocks - 1 - blk;
 }
 
 __device__ inline f32x16 zero16() {

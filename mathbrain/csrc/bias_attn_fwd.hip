@@ -10,7 +10,7 @@ namespace {
 // Running maximum, sum and output are in fp32; the probabilities are rounded to bf16 for the
 // product with V where the inputs are bf16 (half a step of 2^-8 of each), the sum is not.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads) bias_attn_fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn_fwd_kernel(const Args a) {
     using X = Ty<T>;
     using Tl = Tile<T, HD>;
     constexpr int KT = X::kKeys;
@@ -20,7 +20,8 @@ __global__ void __launch_bounds__(kThreads) bias_attn_fwd_kernel(const Args a) {
     auto vtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int bh = blockIdx.x / a.nq, qb = a.nq - 1 - (int)(blockIdx.x % a.nq);
+    int bh, qb;
+    place(a.B * a.H, a.nq, false, bh, qb);
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const Reach reach(a);
     const int len = key_count(a, b), p0 = first_position(a, b);
