@@ -665,15 +665,17 @@ int mb_qk_norm_rotary_bwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_s
  *   lse             [B, H, Lq] fp32: log2 of the softmax denominators, written by the forward
  *                   (NULL: not wanted), read by the backward
  *
- * Rows without a key give zeros.  The backward's workspace is mb_bias_attn_bwd_workspace(...)
- * bytes; dbias may be NULL.  Its sums have a fixed order.  hd: 32, 64 or 128.
+ * Rows without a key give zeros.  The workspaces are mb_bias_attn_fwd_workspace(...) (0 where the
+ * keys are not split over workgroups) and mb_bias_attn_bwd_workspace(...) bytes; dbias may be NULL.  Its sums have a fixed order.  hd: 32, 64 or 128.
  */
 int mb_bias_attn_fwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
                      const void *v, const int64_t *v_st, const void *bias, int bias_dtype,
                      int buckets, const int32_t *starts, int n_starts, const void *lengths,
                      int lengths_bytes, const void *q_start, int q_start_bytes, int64_t q_start0,
                      int B, int H, int Hk, int Lq, int Lk, int hd, float scale, int causal,
-                     int dtype, void *o, const int64_t *o_st, float *lse, void *stream);
+                     int dtype, void *o, const int64_t *o_st, float *lse, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd);
 int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets);
 int mb_bias_attn_bwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
                      const void *v, const int64_t *v_st, const void *bias, int bias_dtype,

@@ -20,6 +20,19 @@ inline bool rows16(const void* p, const int64_t* st, int dtype) {
     return (((uint64_t)(uintptr_t)p | (uint64_t)(st[0] * size) | (uint64_t)(st[1] * size) | (uint64_t)(st[2] * size)) & 15) == 0;
 }
 
+// Parts that the keys of a row are split into (bias_attn_split.hip), or 0 for the kernel whose
+// workgroups walk all keys for 128 queries of a head.
+inline int splits_of(int B, int H, int Hk, int Lq, int Lk) {
+    const int64_t G = H / Hk, tiles = (G * Lq + 31) / 32, nq = ((int64_t)Lq + kRows - 1) / kRows;
+    if (G * Lq > 32 && (int64_t)B * H * nq >= 256) return 0;
+    if (G > 32) return 0;
+    const int64_t wanted = 768 / ((int64_t)B * Hk * tiles);      // three workgroups a CU
+    const int64_t most = ((int64_t)Lk + 255) / 256;              // at least 64 keys a wave
+    const int64_t n = wanted < most ? wanted : most;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+int split_launch(const Args& a, int hd, int dtype, int splits, void* part, hipStream_t st);
+
 inline int fill_args(const char* what, Args& a, const void* q, const int64_t* q_st, const void* k, const int64_t* k_st,
                      const void* v, const int64_t* v_st, const void* bias, int bias_dtype, int buckets,
                      const int32_t* starts, int n_starts, const void* lengths, int lengths_bytes, const void* q_start,
