@@ -22,8 +22,12 @@ constexpr int kWaveRows = 32;   // queries (or keys) of a wave
 constexpr int kRows = 4 * kWaveRows;
 constexpr int kMaxStarts = 128;
 constexpr int kMaxReach = 1024; // the largest distance with a bucket of its own
-constexpr int kPad = 64;        // table entries beyond each end: a 32 x 32 block's distances that pass it
+constexpr int kPad = 96;        // table entries beyond each end: a 32 x 64 tile's distances that pass it
 constexpr float kLog2e = 1.4426950408889634f;
+// The running maximum follows a row's scores only where one passes it by more than this (in log2
+// units): probabilities up to 2^8 of the maximum's lose nothing in fp32 or bf16, and the output
+// is rescaled a few times a row instead of in most tiles.
+constexpr float kSlack = 8.f;
 
 typedef __attribute__((__ext_vector_type__(4))) __bf16 bf16x4;
 typedef __attribute__((__ext_vector_type__(8))) __bf16 bf16x8;
@@ -136,13 +140,19 @@ struct Tile {
 
     // This thread's pieces of rows row0 .. row0 + kN - 1; rows from `rows` on are zero.
     static __device__ void load(const T* base, int64_t sl, int row0, int rows, f32x4* v) {
+        constexpr int kStep = kThreads / kPerRow;   // rows between a thread's pieces
+        const int r = threadIdx.x / kPerRow;
+        const T* p = base + (row0 + r) * sl + (threadIdx.x % kPerRow) * (16 / (int)sizeof(T));
+        if (row0 + kN <= rows) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int p = i * kThreads + threadIdx.x;
-            const int r = row0 + p / kPerRow, c = p % kPerRow;
-            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-            v[i] = zero;
-            if (r < rows) v[i] = *reinterpret_cast<const f32x4*>(base + (int64_t)r * sl + c * (16 / sizeof(T)));
+            for (int i = 0; i < kVecs; ++i) v[i] = *reinterpret_cast<const f32x4*>(p + i * kStep * sl);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                v[i] = zero;
+                if (row0 + r + i * kStep < rows) v[i] = *reinterpret_cast<const f32x4*>(p + i * kStep * sl);
+            }
         }
     }
     static __device__ void store(T* tile, const f32x4* v) {
@@ -237,6 +247,26 @@ __device__ inline void place(int heads, int blocks, bool first_most, int& bh, in
     bh = id % heads;
     blk = id / heads;
     if (!first_most) blk = blocks - 1 - blk;
+}
+
+// A value of this lane and of the same lane of the other half wave: the first register's upper half
+// is swapped with the second's lower half.
+__device__ inline void halves(float v, float& lo, float& hi) {
+    const int a = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    const int x = r[0], y = r[1];
+    lo = __builtin_bit_cast(float, x);
+    hi = __builtin_bit_cast(float, y);
+}
+__device__ inline float half_max(float v) {
+    float lo, hi;
+    halves(v, lo, hi);
+    return fmaxf(lo, hi);
+}
+__device__ inline float half_sum(float v) {
+    float lo, hi;
+    halves(v, lo, hi);
+    return lo + hi;
 }
 
 __device__ inline f32x16 zero16() {

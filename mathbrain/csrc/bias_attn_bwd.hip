@@ -60,7 +60,7 @@ struct Diagonals {
         open = true;
     }
     __device__ void put(int d, float v) {
-        v += __shfl_xor(v, 32, 64);
+        v = half_sum(v);
         if ((threadIdx.x & 63) < 32) sums[d] = v;
     }
     // After the last block (d0): what was carried out of it.
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)qf[c][e], (float)gf[c][e], delta);
-        delta += __shfl_xor(delta, 32, 64);
+        delta = half_sum(delta);
     }
     load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
     float lse = INFINITY;

@@ -61,50 +61,55 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         const int j0 = t * KT;
         if (j0 < wend) {
             f32x16 x[KT / 32];
-            float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < KT / 32; ++u) {
-                const int jb = j0 + 32 * u;
-                x[u] = zero16();
+            for (int u = 0; u < KT / 32; ++u) x[u] = zero16();
 #pragma unroll
-                for (int c = 0; c < HD / 16; ++c) x[u] = X::mma(Tl::rows(ktile(s), 32 * u, c), qf[c], x[u]);
-                const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
-                if (dlo >= reach.hi || dhi <= reach.lo) {  // one bias for the whole block
-                    const float bias = tab[kPad + (dlo >= reach.hi ? reach.hi - reach.lo : 0)];
+            for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, bias);
-                } else {
-                    // dlo > lo - 63 and dhi < hi + 63: within the padded table, masked pairs too
-                    const float* at = tab + kPad - reach.lo + (pos - jb);
+                for (int u = 0; u < KT / 32; ++u) x[u] = X::mma(Tl::rows(ktile(s), 32 * u, c), qf[c], x[u]);
+            const int dlo = p0 + w0 - j0 - (KT - 1), dhi = p0 + w0 + 31 - j0;
+            float mul = sl2, add = 0.f;   // the scores in log2 units are mul x + add
+            if (dlo >= reach.hi || dhi <= reach.lo) {
+                add = tab[kPad + (dlo >= reach.hi ? reach.hi - reach.lo : 0)];   // one bias for the whole tile
+            } else {
+                // dlo > lo - 95 and dhi < hi + 95: within the padded table, masked pairs too
+                const float* at = tab + kPad - reach.lo + (pos - j0);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, at[-row_of(r)]);
-                }
-                if ((a.causal && dlo < 0) || jb + 32 > len) {
-                    const int most = a.causal ? min(len, pos + 1) : len;
+                for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, at[-32 * u - row_of(r)]);
+                mul = 1.f;
+            }
+            if ((a.causal && dlo < 0) || j0 + KT > len) {
+                const int most = (a.causal ? min(len, pos + 1) : len) - j0 - 4 * (lane >> 5);
+#pragma unroll
+                for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (jb + row_of(r) >= most) x[u][r] = -INFINITY;
-                }
+                        if (32 * u + 8 * (r / 4) + r % 4 >= most) x[u][r] = -INFINITY;
+            }
+            float top = x[0][0];
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, x[u][r]);
-            }
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m, top);
-            const float mu = mn == -INFINITY ? 0.f : mn;   // no key yet: every term is 0
-            const float alpha = __builtin_amdgcn_exp2f(m - mu);
-            m = mn;
-            if (__any(alpha != 1.f)) {
+            top = __builtin_fmaf(half_max(top), mul, add);   // mul > 0
+            if (__any(top > m + kSlack)) {
+                const float mn = fmaxf(m, top);
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
             }
+            const float mu = m == -INFINITY ? 0.f : m;   // no key yet: every term is 0
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - mu);
+                    x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], mul, add - mu));
                     l += x[u][r];
                 }
 #pragma unroll
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         }
         __syncthreads();
     }
-    l += __shfl_xor(l, 32, 64);
+    l = half_sum(l);
     if (i < a.Lq) {
         const float inv = l > 0.f ? 1.0f / l : 0.f;   // a row without keys: zeros
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;

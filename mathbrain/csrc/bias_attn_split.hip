@@ -123,17 +123,18 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         float top = x[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
-        if (__any(alpha != 1.f)) {
+        top = half_max(top);
+        if (__any(top > m + kSlack)) {
+            const float mn = fmaxf(m, top);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
         }
+        const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             x[e] = __builtin_amdgcn_exp2f(x[e] - mu);
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    l += __shfl_xor(l, 32, 64);
+    l = half_sum(l);
     // join the four waves
     if (lane < 32) stat[wave][0][lane] = m, stat[wave][1][lane] = l;
     float* mine = corner + wave * kWaveFloats;
