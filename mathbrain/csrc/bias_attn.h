@@ -77,7 +77,7 @@ struct Args {
     const void *lengths, *start;             // [B] or NULL
     void *out, *dk, *dv;                     // out: o (forward) or dq
     int64_t out_sb, out_sh, out_sl, dk_sb, dk_sh, dk_sl, dv_sb, dv_sh, dv_sl;
-    float *lse, *delta, *dbias_part;         // [B, H, Lq] (log2 units), [B, H, Lq], [H, B * nq, buckets]
+    float *lse, *rows, *dbias_part;          // [B, H, Lq] (log2 units), [2, B, H, Lq], [H, B * nq, buckets]
     int lengths_bytes, start_bytes, start0;
     int B, H, Hk, Lq, Lk, nq;
     int causal, bias_bf16, buckets, n_starts, reach;
@@ -127,75 +127,143 @@ __device__ inline void fill_table(const Args& a, int h, float* tab) {
     }
 }
 
-// ---- staged tiles: rows of HD elements, 16 bytes of padding after each -------------------------
+// ---- staged tiles ------------------------------------------------------------------------------
+//
+// Rows go from memory straight into LDS, 16 bytes a lane, two tiles ahead of the one that is used
+// (loads through registers, one tile ahead, left the waves waiting: forward at 4 x 4096, 8 heads x
+// 64, 117 us against 87 with the loads taken out).  Such a load puts its 64 pieces next to each
+// other, so a row has no padding; piece c of row r lies in the row's place c ^ swz(r) instead,
+// which spreads both ways of reading the tile over the banks.
 
-template <typename T, int HD>
+constexpr int kStages = 3;
+
+// 16 (or 4) bytes a lane from base + voff to LDS at lds + 16 (or 4) * lane.
+__device__ inline void dma16(uint32_t lds, uint32_t voff, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(voff), "s"(base)
+                 : "memory");
+}
+__device__ inline void dma4(uint32_t lds, uint32_t voff, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(lds), "v"(voff), "s"(base)
+                 : "memory");
+}
+// Waits until at most N of the wave's loads are on their way, and for the other waves.
+template <int N>
+__device__ inline void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+// Ends the compiler's own loads before a loop of dma16: it would wait for them at their first use,
+// inside the loop, and with them for the loads that are meant to be on their way.
+__device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0)
+
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+__device__ inline uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+template <typename T, int HD, int ROWS = Ty<T>::kKeys>
 struct Tile {
-    static constexpr int kStride = HD + 16 / (int)sizeof(T);
-    static constexpr int kN = Ty<T>::kKeys;
-    static constexpr int kPerRow = HD * (int)sizeof(T) / 16;
-    static constexpr int kVecs = kN * kPerRow / kThreads;   // 16-byte pieces of a thread
-    static constexpr int kBytes = kN * kStride * (int)sizeof(T);
-    static_assert(kN * kPerRow % kThreads == 0, "pieces");
+    static constexpr int kN = ROWS;
+    static constexpr int kRow = HD * (int)sizeof(T);               // bytes
+    static constexpr int kBytes = kN * kRow;
+    static constexpr int kPieces = kRow / 16;
+    static constexpr int kLoads = kBytes / 4096;                   // of each of the four waves
+    static_assert(kBytes % 4096 == 0, "a wave's load moves 1 KiB");
 
-    // This thread's pieces of rows row0 .. row0 + kN - 1; rows from `rows` on are zero.
-    static __device__ void load(const T* base, int64_t sl, int row0, int rows, f32x4* v) {
-        constexpr int kStep = kThreads / kPerRow;   // rows between a thread's pieces
-        const int r = threadIdx.x / kPerRow;
-        const T* p = base + (row0 + r) * sl + (threadIdx.x % kPerRow) * (16 / (int)sizeof(T));
+    static __device__ constexpr int swz(int row) {
+        if (kPieces == 4) return (row >> 2) & 3;
+        if (kPieces == 8) return ((row >> 1) & 1) << 2 | ((row >> 3) & 1) << 1 | ((row >> 2) & 1);
+        return (row & 3) << 2 | ((row >> 2) & 3);
+    }
+    static __device__ int at(int row, int piece) { return row * kRow + ((piece ^ swz(row & 15)) << 4); }
+
+    // This lane's part of each of its wave's loads: the row, and its offset from the tile's first.
+    struct Offsets {
+        uint32_t v[kLoads];
+        __device__ explicit Offsets(int64_t sl) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) v[i] = (uint32_t)(row(i) * (int)(sl * (int)sizeof(T))) + piece(i);
+        }
+        static __device__ int slot(int i) { return i * kThreads + (int)threadIdx.x; }
+        static __device__ int row(int i) { return slot(i) / kPieces; }
+        static __device__ uint32_t piece(int i) { return (uint32_t)((slot(i) % kPieces) ^ swz(row(i) & 15)) << 4; }
+    };
+    // Rows row0 .. row0 + kN - 1 of `base` on their way to the tile; rows from `rows` (at least 1)
+    // on are the last one again.
+    static __device__ void load(uint32_t tile, const T* base, int64_t sl, int row0, int rows, const Offsets& off) {
+        const uint32_t lds = tile + wave_id() * 1024;
+        const int first = min(row0, rows - 1);
+        const T* from = base + first * sl;
         if (row0 + kN <= rows) {
 #pragma unroll
-            for (int i = 0; i < kVecs; ++i) v[i] = *reinterpret_cast<const f32x4*>(p + i * kStep * sl);
+            for (int i = 0; i < kLoads; ++i) dma16(lds + i * 4096, off.v[i], from);
         } else {
 #pragma unroll
-            for (int i = 0; i < kVecs; ++i) {
-                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                v[i] = zero;
-                if (row0 + r + i * kStep < rows) v[i] = *reinterpret_cast<const f32x4*>(p + i * kStep * sl);
+            for (int i = 0; i < kLoads; ++i) {
+                const int r = min(Offsets::row(i), rows - 1 - first);
+                dma16(lds + i * 4096, (uint32_t)(r * (int)(sl * (int)sizeof(T))) + Offsets::piece(i), from);
             }
         }
     }
-    static __device__ void store(T* tile, const f32x4* v) {
+
+    // Where this lane reads, relative to a tile: with these kept, several reads cost one addition (the
+    // rest is the instruction's constant offset).  In fp32, whose products take 16 times as long, some
+    // of them are formed at the read instead of kept.
+    typedef __attribute__((address_space(3))) const char lds_char;
+    struct Lane {
+        uint32_t row[sizeof(T) == 2 ? HD / 16 : 2], col[sizeof(T) == 2 ? HD / 16 : 8];
+        __device__ Lane() {
+            const int lane = threadIdx.x & 63, g = lane >> 5;
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int p = i * kThreads + threadIdx.x;
-            *reinterpret_cast<f32x4*>(tile + (p / kPerRow) * kStride + (p % kPerRow) * (16 / sizeof(T))) = v[i];
+            for (int i = 0; i < (sizeof(T) == 2 ? HD / 16 : 2); ++i) row[i] = at(lane & 31, sizeof(T) == 2 ? 2 * i + g : 2 * g + i);
+            if constexpr (sizeof(T) == 2) {
+                // 16 lanes read 4 rows of 16 channels, 8 bytes each, and get 4 rows of one channel each
+                const int r = 4 * g + ((lane & 15) >> 2), d = (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) col[i] = at(r + 8 * (i % 2), 4 * (i / 2) + (d >> 3)) + 2 * (d & 7);
+            } else {
+                const int d = lane & 31;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) col[i] = at(4 * g + 8 * (i / 4) + i % 4, d >> 2) + 4 * (d & 3);
+            }
+        }
+    };
+    // Operand with the tile's rows row0 + lane % 32 (row0 a multiple of 32) and channels 16 c ..: a
+    // lane's 8 are adjacent.
+    static __device__ typename Ty<T>::Frag rows(uint32_t tile, const Lane& l, int row0, int c) {
+        if constexpr (sizeof(T) == 2) {
+            return *(__attribute__((address_space(3))) const bf16x8*)((lds_char*)(uintptr_t)(tile + l.row[c]) + row0 * kRow);
+        } else {
+            // channels 16 c further, piece n becomes n ^ 4 c
+            typedef __attribute__((address_space(3))) const f32x4 lds_f32x4;
+            const f32x4 x = *(lds_f32x4*)((lds_char*)(uintptr_t)(tile + (l.row[0] ^ (c << 6))) + row0 * kRow);
+            const f32x4 y = *(lds_f32x4*)((lds_char*)(uintptr_t)(tile + (l.row[1] ^ (c << 6))) + row0 * kRow);
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // Operand with the tile's rows row0 + lane % 32 and channels 16 c ..: a lane's 8 are adjacent.
-    static __device__ typename Ty<T>::Frag rows(const T* tile, int row0, int c) {
-        const int lane = threadIdx.x & 63;
-        return *reinterpret_cast<const typename Ty<T>::FragMem*>(tile + (row0 + (lane & 31)) * kStride + 16 * c + 8 * (lane >> 5));
+    // Operand with channels 32 d + lane % 32 and the tile's rows row0 + (the slots' order above), row0
+    // a multiple of 16.
+    static __device__ typename Ty<T>::Frag cols(uint32_t tile, const Lane& l, int row0, int d) {
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)((lds_char*)(uintptr_t)(tile + l.col[2 * d]) + row0 * kRow));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)((lds_char*)(uintptr_t)(tile + l.col[2 * d + 1]) + row0 * kRow));
+            return __builtin_shufflevector(__builtin_bit_cast(bf16x4, x), __builtin_bit_cast(bf16x4, y), 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            f32x8 f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)   // 32 channels further, piece c becomes c ^ 8
+                f[e] = *(__attribute__((address_space(3))) const float*)((lds_char*)(uintptr_t)(tile + (l.col[e] ^ (d << 7))) + row0 * kRow);
+            return f;
+        }
     }
 };
-
-// Operand with channels d0 + lane % 32 and a tile's rows row0 + (the slots' order above).
-template <int STRIDE>
-__device__ inline bf16x8 cols_bf16(const __bf16* tile, int row0, int d0) {
-    // 16 lanes read 4 rows of 16 channels, 8 bytes each, and get 4 rows of one channel each
-    const int lane = threadIdx.x & 63;
-    const __bf16* p = tile + (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * STRIDE + d0 + (lane & 16) + 4 * (lane & 3);
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(__attribute__((address_space(3))) void*)p);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4*)(__attribute__((address_space(3))) void*)(p + 8 * STRIDE));
-    const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-template <int STRIDE>
-__device__ inline f32x8 cols_f32(const float* tile, int row0, int d0) {
-    const int lane = threadIdx.x & 63;
-    const float* p = tile + (row0 + 4 * (lane >> 5)) * STRIDE + d0 + (lane & 31);
-    f32x8 f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = p[(8 * (e / 4) + e % 4) * STRIDE];
-    return f;
-}
-template <typename T, int HD>
-__device__ inline typename Ty<T>::Frag cols_of(const T* tile, int row0, int d0) {
-    if constexpr (sizeof(T) == 2) return cols_bf16<Tile<T, HD>::kStride>(tile, row0, d0);
-    else return cols_f32<Tile<T, HD>::kStride>(tile, row0, d0);
-}
 
 // Rows of a wave in registers: row r0 + lane % 32, channels 16 c + 8 (lane / 32) ..; rows from
 // `rows` on are zero.

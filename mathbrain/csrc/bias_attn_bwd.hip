@@ -36,7 +36,8 @@ struct Diagonals {
     float carry = 0.f;
     bool open = false;
 
-    __device__ void add(const f32x16& x, int d0) {
+    // The block into LDS; take() follows, with the products that need the block between them.
+    __device__ void give(const f32x16& x) {
         const int lane = threadIdx.x & 63, t = lane & 31, g = lane >> 5;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -45,6 +46,9 @@ struct Diagonals {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+    }
+    __device__ void take(int d0) {
+        const int lane = threadIdx.x & 63, t = lane & 31, g = lane >> 5;
         float here = carry, next = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -71,24 +75,27 @@ struct Diagonals {
     }
 };
 
+// Heads of 128 leave registers for 32 keys at a time in the queries' pass (8 x 1024 tokens, 8 heads, bf16: 71 us against
+// 112 with 64 keys, which spill).
+template <typename T, int HD>
+using QueryTile = Tile<T, HD, HD == 128 ? 32 : Ty<T>::kKeys>;
+
 // dbias: a block of pairs that lies within one bucket adds to a register, any other adds to its
 // distances' entries in LDS (Diagonals).  In the end the entries are added by buckets, into the
 // workgroup's own row of a workspace.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn_dq_kernel(const Args a) {
     using X = Ty<T>;
-    using Tl = Tile<T, HD>;
-    constexpr int KT = X::kKeys;
+    using Tl = QueryTile<T, HD>;
+    constexpr int KT = Tl::kN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float far[4][2];
     const Reach reach(a);
     const int entries = reach.entries();
-    float* tab = reinterpret_cast<float*>(smem + 4 * Tl::kBytes);
+    float* tab = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes);
     float* hist = tab + entries;   // [wave][entries], then the waves' blocks
-    auto ktile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s) * Tl::kBytes); };
-    auto vtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     int bh, qb;
     place(a.B * a.H, a.nq, false, bh, qb);
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
@@ -116,16 +123,28 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         delta = half_sum(delta);
     }
     load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
+    // The products' results start from -lse (in units of the scores) and -delta: p is then
+    // exp2(scale x + bias) and ds is p y.  Here two blocks of registers hold them where that leaves
+    // two waves a SIMD room; the keys' pass reads both rows from the workspace.
+    constexpr bool kStart = HD == 64;
+    float nlse = -INFINITY;
     float lse = INFINITY;
     if (i < a.Lq) {
         lse = a.lse[(int64_t)bh * a.Lq + i];
-        if (lane < 32) a.delta[(int64_t)bh * a.Lq + i] = delta;
+        nlse = -lse / sl2;
+        if (lane < 32) {
+            a.rows[(int64_t)bh * a.Lq + i] = nlse;
+            a.rows[((int64_t)a.B * a.H + bh) * a.Lq + i] = -delta;
+        }
     }
+    f32x16 x0, y0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x0[r] = kStart ? nlse : 0.f, y0[r] = kStart ? -delta : 0.f;
     fill_table(a, h, tab);
     if (want_bias)
         for (int n = threadIdx.x; n < 4 * entries; n += kThreads) hist[n] = 0.f;
     Diagonals diag;
-    diag.block = reinterpret_cast<float*>(smem + 4 * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
+    diag.block = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
     diag.sums = hist + wave * entries + kPad - reach.lo + (lane & 31);
     float far_hi = 0.f, far_lo = 0.f;
     int last_d0 = 0;
@@ -133,40 +152,41 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     f32x16 dq[HD / 32];
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d) dq[d] = zero16();
-    f32x4 kv[Tl::kVecs], vv[Tl::kVecs];
-    if (tiles > 0) {
-        Tl::load(kbase, a.k_sl, 0, len, kv);
-        Tl::load(vbase, a.v_sl, 0, len, vv);
-        Tl::store(ktile(0), kv);
-        Tl::store(vtile(0), vv);
-    }
-    __syncthreads();
+    const uint32_t lds = lds_address(smem);
+    const typename Tl::Lane at;
+    const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
+    auto load = [&](int t) {
+        const uint32_t tile = lds + t % kStages * (2 * Tl::kBytes);
+        Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
+        Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
+    };
+    loads_done();
+    if (tiles > 0)
+        for (int t = 0; t < kStages - 1; ++t) load(t);
     for (int t = 0; t < tiles; ++t) {
-        const int s = t & 1;
-        if (t + 1 < tiles) {
-            Tl::load(kbase, a.k_sl, (t + 1) * KT, len, kv);
-            Tl::load(vbase, a.v_sl, (t + 1) * KT, len, vv);
-        }
+        wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
+        load(t + kStages - 1);
+        const uint32_t ktile = lds + t % kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
             const int jb = t * KT + 32 * u;
             if (jb >= wend) break;
-            f32x16 x = zero16(), y = zero16();
+            f32x16 x = x0, y = y0;
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) {
-                x = X::mma(Tl::rows(ktile(s), 32 * u, c), qf[c], x);
-                y = X::mma(Tl::rows(vtile(s), 32 * u, c), gf[c], y);
+                x = X::mma(Tl::rows(ktile, at, 32 * u, c), qf[c], x);
+                y = X::mma(Tl::rows(vtile, at, 32 * u, c), gf[c], y);
             }
             const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
             const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
-            const int at = kPad - reach.lo + (pos - jb);
+            const int near = kPad - reach.lo + (pos - jb);
             if (one) {
                 const float bias = tab[kPad + (above ? reach.hi - reach.lo : 0)];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, bias);
             } else {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, tab[at - row_of(r)]);
+                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, tab[near - row_of(r)]);
             }
             if ((a.causal && dlo < 0) || jb + 32 > len) {
                 const int most = a.causal ? min(len, pos + 1) : len;
@@ -175,7 +195,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
                     if (jb + row_of(r) >= most) x[r] = -INFINITY;
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
+            for (int r = 0; r < 16; ++r)
+                x[r] = kStart ? __builtin_amdgcn_exp2f(x[r]) * y[r] : __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
             if (want_bias) {
                 if (one) {
                     diag.close(last_d0);
@@ -185,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
                     (above ? far_hi : far_lo) += sum;
                 } else {
                     last_d0 = dlo + 31;
-                    diag.add(x, last_d0);
+                    diag.give(x);
                 }
             }
 #pragma unroll
@@ -193,15 +214,12 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
                 const typename X::Frag f = to_frag<T>(x, c);
 #pragma unroll
                 for (int d = 0; d < HD / 32; ++d)
-                    dq[d] = X::mma(cols_of<T, HD>(ktile(s), 32 * u + 16 * c, 32 * d), f, dq[d]);
+                    dq[d] = X::mma(Tl::cols(ktile, at, 32 * u + 16 * c, d), f, dq[d]);
             }
+            if (want_bias && !one) diag.take(last_d0);
         }
-        if (t + 1 < tiles) {
-            Tl::store(ktile(s ^ 1), kv);
-            Tl::store(vtile(s ^ 1), vv);
-        }
-        __syncthreads();
     }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // LDS is written until then
     if (i < a.Lq) {
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
 #pragma unroll
@@ -252,14 +270,12 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bias_attn_dkv_kernel(const Args a) {
     using X = Ty<T>;
     using Tl = Tile<T, HD>;
-    constexpr int QT = X::kKeys;
+    constexpr int QT = Tl::kN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];
-    float* tab = reinterpret_cast<float*>(smem + 4 * Tl::kBytes);
-    auto qtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s) * Tl::kBytes); };
-    auto gtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
+    __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];   // rows' -lse and -delta
+    float* tab = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 5;
     const int nk = (a.Lk + kRows - 1) / kRows;
     int bh, kb;
     place(a.B * a.Hk, nk, true, bh, kb);
@@ -280,44 +296,50 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d) dk[d] = zero16(), dv[d] = zero16();
 
-    f32x4 qv[Tl::kVecs], gv[Tl::kVecs];
-    float st = 0.f;
+    const uint32_t lds = lds_address(smem);
+    const typename Tl::Lane at;
+    const typename Tl::Offsets qoff(a.q_sl), goff(a.do_sl);
     for (int hh = 0; hh < group; ++hh) {
         const int h = hk * group + hh;
         const T* qbase = (const T*)a.q + b * a.q_sb + h * a.q_sh;
         const T* gbase = (const T*)a.d_o + b * a.do_sb + h * a.do_sh;
-        const float* lse = a.lse + ((int64_t)b * a.H + h) * a.Lq;
-        const float* delta = a.delta + ((int64_t)b * a.H + h) * a.Lq;
+        const float* nlse = a.rows + ((int64_t)b * a.H + h) * a.Lq;
+        const float* ndelta = nlse + (int64_t)a.B * a.H * a.Lq;
         auto load = [&](int t) {
-            Tl::load(qbase, a.q_sl, t * QT, a.Lq, qv);
-            Tl::load(gbase, a.do_sl, t * QT, a.Lq, gv);
-            const int i = t * QT + (int)(threadIdx.x % QT);   // past the end: no probability
-            if (threadIdx.x < QT) st = i < a.Lq ? lse[i] : INFINITY;
-            else if (threadIdx.x < 2 * QT) st = i < a.Lq ? delta[i] : 0.f;
+            const int s = t % kStages;
+            if (wave < 2)   // one wave the rows' -lse, another their -delta; the last row's past the end
+                dma4(lds_address(&stat[s][wave][0]), 4u * (uint32_t)min(t * QT + lane, a.Lq - 1),
+                     wave ? ndelta : nlse);
+            const uint32_t tile = lds + s * (2 * Tl::kBytes);
+            Tl::load(tile, qbase, a.q_sl, t * QT, a.Lq, qoff);
+            Tl::load(tile + Tl::kBytes, gbase, a.do_sl, t * QT, a.Lq, goff);
         };
-        auto store = [&](int s) {
-            Tl::store(qtile(s), qv);
-            Tl::store(gtile(s), gv);
-            if (threadIdx.x < 2 * QT) stat[s][threadIdx.x / QT][threadIdx.x % QT] = st;
-        };
+        if (first >= tiles) break;
         fill_table(a, h, tab);   // the previous head's last barrier lies behind its reads
-        if (first < tiles) {
-            load(first);
-            store(first & 1);
-        }
-        __syncthreads();
+        loads_done();
+        for (int t = first; t < first + kStages - 1; ++t) load(t);
         for (int t = first; t < tiles; ++t) {
-            const int s = t & 1;
-            if (t + 1 < tiles) load(t + 1);
+            const int s = t % kStages;
+            // (two waves have a load more on their way: they wait for that one of the next tile too)
+            wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();
+            load(t + kStages - 1);
+            const uint32_t qtile = lds + s * (2 * Tl::kBytes), gtile = qtile + Tl::kBytes;
 #pragma unroll
             for (int u = 0; u < QT / 32; ++u) {
                 const int ib = t * QT + 32 * u;
                 if (ib >= a.Lq || w0 >= len || (a.causal && p0 + ib + 31 < w0)) continue;
-                f32x16 x = zero16(), y = zero16();
+                f32x16 x, y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 nl = *reinterpret_cast<const f32x4*>(&stat[s][0][32 * u + 8 * r + 4 * g]);
+                    const f32x4 nd = *reinterpret_cast<const f32x4*>(&stat[s][1][32 * u + 8 * r + 4 * g]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * r + e] = nl[e], y[4 * r + e] = nd[e];
+                }
 #pragma unroll
                 for (int c = 0; c < HD / 16; ++c) {
-                    x = X::mma(Tl::rows(qtile(s), 32 * u, c), kf[c], x);
-                    y = X::mma(Tl::rows(gtile(s), 32 * u, c), vf[c], y);
+                    x = X::mma(Tl::rows(qtile, at, 32 * u, c), kf[c], x);
+                    y = X::mma(Tl::rows(gtile, at, 32 * u, c), vf[c], y);
                 }
                 const int dlo = p0 + ib - w0 - 31, dhi = p0 + ib + 31 - w0;
                 const bool above = dlo >= reach.hi;
@@ -326,39 +348,35 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
 #pragma unroll
                     for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, bias);
                 } else {
-                    const float* at = tab + kPad - reach.lo + (p0 + ib - j);
+                    const float* near = tab + kPad - reach.lo + (p0 + ib - j);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, at[row_of(r)]);
+                    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, near[row_of(r)]);
                 }
-                if ((a.causal && dlo < 0) || w0 + 32 > len) {
+                if ((a.causal && dlo < 0) || w0 + 32 > len || ib + 32 > a.Lq) {
                     const int least = j >= len ? 0x7fffffff : a.causal ? j - p0 : -0x7fffffff;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (ib + row_of(r) < least) x[r] = -INFINITY;
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = ib + row_of(r);
+                        if (i < least || i >= a.Lq) x[r] = -INFINITY;
+                    }
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[s][0][32 * u + 8 * r + 4 * g]);
-                    const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[s][1][32 * u + 8 * r + 4 * g]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[4 * r + e] = __builtin_amdgcn_exp2f(x[4 * r + e] - ls[e]);
-                        y[4 * r + e] = x[4 * r + e] * (y[4 * r + e] - de[e]);
-                    }
+                for (int r = 0; r < 16; ++r) {
+                    x[r] = __builtin_amdgcn_exp2f(x[r]);
+                    y[r] *= x[r];
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const typename X::Frag p = to_frag<T>(x, c), ds = to_frag<T>(y, c);
 #pragma unroll
                     for (int d = 0; d < HD / 32; ++d) {
-                        dv[d] = X::mma(cols_of<T, HD>(gtile(s), 32 * u + 16 * c, 32 * d), p, dv[d]);
-                        dk[d] = X::mma(cols_of<T, HD>(qtile(s), 32 * u + 16 * c, 32 * d), ds, dk[d]);
+                        dv[d] = X::mma(Tl::cols(gtile, at, 32 * u + 16 * c, d), p, dv[d]);
+                        dk[d] = X::mma(Tl::cols(qtile, at, 32 * u + 16 * c, d), ds, dk[d]);
                     }
                 }
             }
-            if (t + 1 < tiles) store(s ^ 1);
-            __syncthreads();
         }
+        wait_and_meet<0>();   // the next head's loads and table go where this one's were
     }
     if (j < a.Lk) {
         T* krow = (T*)a.dk + b * a.dk_sb + hk * a.dk_sh + (int64_t)j * a.dk_sl;
@@ -395,8 +413,9 @@ static_assert(2 * kMaxStarts <= kThreads, "a thread for every bucket");
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
     const int entries = Reach(a).entries();
-    const int base = 4 * Tile<T, HD>::kBytes + entries * (int)sizeof(float);
-    const int lds_q = base + (a.dbias_part ? (4 * entries + 3 + 4 * 32 * Diagonals::kStride) * (int)sizeof(float) : 0);
+    const int table = entries * (int)sizeof(float);
+    const int base = 2 * kStages * Tile<T, HD>::kBytes + table;
+    const int lds_q = 2 * kStages * QueryTile<T, HD>::kBytes + table + (a.dbias_part ? (4 * entries + 3 + 4 * 32 * Diagonals::kStride) * (int)sizeof(float) : 0);
     if (a.Lq > 0) {
         if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q)) return rc;
         hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds_q, st, a);
@@ -421,7 +440,7 @@ using namespace mb::battn;
 extern "C" int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets) {
     if (B < 1 || H < 1 || Lq < 1 || buckets < 1) return 0;
     const int64_t nq = ((int64_t)Lq + kRows - 1) / kRows;
-    return (padded((int64_t)B * H * Lq) + (int64_t)H * B * nq * buckets) * (int64_t)sizeof(float);
+    return (padded(2 * (int64_t)B * H * Lq) + (int64_t)H * B * nq * buckets) * (int64_t)sizeof(float);
 }
 
 extern "C" int mb_bias_attn_bwd(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
@@ -445,6 +464,8 @@ extern "C" int mb_bias_attn_bwd(const void* q, const int64_t* q_st, const void* 
         MB_REQUIRE(o && o_st && d_o && do_st && lse && dq && dq_st, "mb_bias_attn_bwd: null pointer argument");
         MB_REQUIRE(rows16(o, o_st, dtype) && rows16(d_o, do_st, dtype) && rows16(dq, dq_st, dtype),
                    "mb_bias_attn_bwd: rows must begin at multiples of 16 bytes");
+        MB_REQUIRE(do_st[2] >= 0 && do_st[2] <= (1 << 24) / (dtype == MB_DTYPE_F32 ? 4 : 2),
+                   "mb_bias_attn_bwd: d_o's rows are %lld elements apart", (long long)do_st[2]);
         a.o = o, a.o_sb = o_st[0], a.o_sh = o_st[1], a.o_sl = o_st[2];
         a.d_o = d_o, a.do_sb = do_st[0], a.do_sh = do_st[1], a.do_sl = do_st[2];
         a.out = dq, a.out_sb = dq_st[0], a.out_sh = dq_st[1], a.out_sl = dq_st[2];
@@ -456,8 +477,8 @@ extern "C" int mb_bias_attn_bwd(const void* q, const int64_t* q_st, const void* 
         a.dv = dv, a.dv_sb = dv_st[0], a.dv_sh = dv_st[1], a.dv_sl = dv_st[2];
     }
     a.lse = const_cast<float*>(lse);
-    a.delta = (float*)workspace;
-    a.dbias_part = dbias && need > 0 ? (float*)workspace + padded((int64_t)B * H * Lq) : nullptr;
+    a.rows = (float*)workspace;
+    a.dbias_part = dbias && need > 0 ? (float*)workspace + padded(2 * (int64_t)B * H * Lq) : nullptr;
     hipStream_t st = (hipStream_t)stream;
     if (B > 0) {
         const int rc = dtype == MB_DTYPE_F32

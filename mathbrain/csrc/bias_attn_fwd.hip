@@ -13,13 +13,11 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn_fwd_kernel(const Args a) {
     using X = Ty<T>;
     using Tl = Tile<T, HD>;
-    constexpr int KT = X::kKeys;
+    constexpr int KT = Tl::kN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* tab = reinterpret_cast<float*>(smem + 4 * Tl::kBytes);
-    auto ktile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s) * Tl::kBytes); };
-    auto vtile = [&](int s) { return reinterpret_cast<T*>(smem + (2 * s + 1) * Tl::kBytes); };
+    float* tab = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_id();
     int bh, qb;
     place(a.B * a.H, a.nq, false, bh, qb);
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
@@ -44,40 +42,49 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     for (int d = 0; d < HD / 32; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
 
-    f32x4 kv[Tl::kVecs], vv[Tl::kVecs];
-    if (tiles > 0) {
-        Tl::load(kbase, a.k_sl, 0, len, kv);
-        Tl::load(vbase, a.v_sl, 0, len, vv);
-        Tl::store(ktile(0), kv);
-        Tl::store(vtile(0), vv);
-    }
-    __syncthreads();
+    const uint32_t lds = lds_address(smem);
+    const typename Tl::Lane at;
+    const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
+    auto load = [&](int t) {
+        const uint32_t tile = lds + t % kStages * (2 * Tl::kBytes);
+        Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
+        Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
+    };
+    loads_done();
+    if (tiles > 0)
+        for (int t = 0; t < kStages - 1; ++t) load(t);
     for (int t = 0; t < tiles; ++t) {
-        const int s = t & 1;
-        if (t + 1 < tiles) {
-            Tl::load(kbase, a.k_sl, (t + 1) * KT, len, kv);
-            Tl::load(vbase, a.v_sl, (t + 1) * KT, len, vv);
-        }
+        // tile t is there, and nobody reads the one before it any longer
+        wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();
+        load(t + kStages - 1);   // past the end too: the waits count loads
+        const uint32_t ktile = lds + t % kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
         const int j0 = t * KT;
         if (j0 < wend) {
             f32x16 x[KT / 32];
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u) x[u] = zero16();
+            typename X::Frag kf[KT / 32][HD / 16];
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
-                for (int u = 0; u < KT / 32; ++u) x[u] = X::mma(Tl::rows(ktile(s), 32 * u, c), qf[c], x[u]);
+                for (int u = 0; u < KT / 32; ++u) kf[u][c] = Tl::rows(ktile, at, 32 * u, c);
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_group_barrier(0x100, KT / 32 * HD / 16, 0);
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+                for (int u = 0; u < KT / 32; ++u) x[u] = X::mma(kf[u][c], qf[c], x[u]);
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_group_barrier(0x008, KT / 32 * HD / 16, 0);
             const int dlo = p0 + w0 - j0 - (KT - 1), dhi = p0 + w0 + 31 - j0;
             float mul = sl2, add = 0.f;   // the scores in log2 units are mul x + add
             if (dlo >= reach.hi || dhi <= reach.lo) {
                 add = tab[kPad + (dlo >= reach.hi ? reach.hi - reach.lo : 0)];   // one bias for the whole tile
             } else {
                 // dlo > lo - 95 and dhi < hi + 95: within the padded table, masked pairs too
-                const float* at = tab + kPad - reach.lo + (pos - j0);
+                const float* near = tab + kPad - reach.lo + (pos - j0);
 #pragma unroll
                 for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, at[-32 * u - row_of(r)]);
+                    for (int r = 0; r < 16; ++r) x[u][r] = __builtin_fmaf(x[u][r], sl2, near[-32 * u - row_of(r)]);
                 mul = 1.f;
             }
             if ((a.causal && dlo < 0) || j0 + KT > len) {
@@ -119,15 +126,11 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
                     const typename X::Frag p = to_frag<T>(x[u], c);
 #pragma unroll
                     for (int d = 0; d < HD / 32; ++d)
-                        o[d] = X::mma(cols_of<T, HD>(vtile(s), 32 * u + 16 * c, 32 * d), p, o[d]);
+                        o[d] = X::mma(Tl::cols(vtile, at, 32 * u + 16 * c, d), p, o[d]);
                 }
         }
-        if (t + 1 < tiles) {
-            Tl::store(ktile(s ^ 1), kv);
-            Tl::store(vtile(s ^ 1), vv);
-        }
-        __syncthreads();
     }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // LDS is written until then
     l = half_sum(l);
     if (i < a.Lq) {
         const float inv = l > 0.f ? 1.0f / l : 0.f;   // a row without keys: zeros
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
-    const int lds = 4 * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
+    const int lds = 2 * kStages * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
     if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD>, lds)) return rc;
     hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds, st, a);
     return check_launch("mb_bias_attn_fwd");

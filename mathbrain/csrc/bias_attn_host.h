@@ -66,6 +66,12 @@ inline int fill_args(const char* what, Args& a, const void* q, const int64_t* q_
     if (B > 0 && Lq > 0) MB_REQUIRE(rows16(q, q_st, dtype), "%s: q's rows must begin at multiples of 16 bytes", what);
     if (B > 0 && Lk > 0)
         MB_REQUIRE(rows16(k, k_st, dtype) && rows16(v, v_st, dtype), "%s: k's and v's rows must begin at multiples of 16 bytes", what);
+    // offsets within a tile of 64 rows have 32 bits
+    const int64_t most = (int64_t)(1 << 24) / (dtype == MB_DTYPE_F32 ? 4 : 2);
+    if (B > 0 && Lq > 0) MB_REQUIRE(q_st[2] >= 0 && q_st[2] <= most, "%s: q's rows are %lld elements apart", what, (long long)q_st[2]);
+    if (B > 0 && Lk > 0)
+        MB_REQUIRE(k_st[2] >= 0 && k_st[2] <= most && v_st[2] >= 0 && v_st[2] <= most,
+                   "%s: k's and v's rows are %lld and %lld elements apart", what, (long long)k_st[2], (long long)v_st[2]);
     a.q = q, a.k = k, a.v = v, a.bias = bias;
     if (q_st) a.q_sb = q_st[0], a.q_sh = q_st[1], a.q_sl = q_st[2];
     if (k_st) a.k_sb = k_st[0], a.k_sh = k_st[1], a.k_sl = k_st[2];

@@ -8,6 +8,29 @@ namespace mb {
 namespace battn {
 namespace {
 
+// Operand with channels d0 + lane % 32 and rows row0 + (the slots' order) of a tile with padded rows.
+template <int STRIDE>
+__device__ inline bf16x8 cols_bf16(const __bf16* tile, int row0, int d0) {
+    // 16 lanes read 4 rows of 16 channels, 8 bytes each, and get 4 rows of one channel each
+    const int lane = threadIdx.x & 63;
+    const __bf16* p = tile + (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * STRIDE + d0 + (lane & 16) + 4 * (lane & 3);
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(__attribute__((address_space(3))) void*)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(__attribute__((address_space(3))) void*)(p + 8 * STRIDE));
+    const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int STRIDE>
+__device__ inline f32x8 cols_f32(const float* tile, int row0, int d0) {
+    const int lane = threadIdx.x & 63;
+    const float* p = tile + (row0 + 4 * (lane >> 5)) * STRIDE + d0 + (lane & 31);
+    f32x8 f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = p[(8 * (e / 4) + e % 4) * STRIDE];
+    return f;
+}
+
 // Rows are the queries of all heads that share a key head, query by query: row r is query r / G of
 // head r % G.  A workgroup takes 32 of them (one column of the 32 x 32 products for each, so that 1
 // row costs what 32 cost) and one of `splits` parts of the keys that they see; each of its waves
