@@ -115,32 +115,33 @@ def bias_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     return o, lse
 
 
-def _bwd_fake(q, k, v, bias, o, d_o, lse, max_distance, causal, scale, lengths, start_rows, start):
+def _bwd_fake(q, k, v, bias, o, d_o, lse, max_distance, causal, scale, lengths, start_rows, start, want_dbias):
     def like(x):
         B, H, L, hd = x.shape
         return x.new_empty((B, L, H, hd)).transpose(1, 2)
-    return like(q), like(k), like(v), bias.new_empty(bias.shape)
+    return like(q), like(k), like(v), bias.new_empty(bias.shape if want_dbias else (0,))
 
 
 @_lib.traced_op("bias_attn_bwd", _bwd_fake)
 def bias_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch.Tensor, o: torch.Tensor,
                   d_o: torch.Tensor, lse: torch.Tensor, max_distance: int, causal: bool, scale: float,
-                  lengths: Optional[torch.Tensor], start_rows: Optional[torch.Tensor], start: int
-                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dq, dk, dv, dbias) of bias_attn_fwd for the output gradient d_o."""
+                  lengths: Optional[torch.Tensor], start_rows: Optional[torch.Tensor], start: int,
+                  want_dbias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv, dbias) of bias_attn_fwd for the output gradient d_o; dbias is empty unless wanted."""
     dev = q.device
     B, H, Lq, hd = q.shape
     Hk, Lk = k.shape[1:3]
     q, k, v, o, d_o = _rows16(q), _rows16(k), _rows16(v), _rows16(o), _rows16(d_o.to(q.dtype))
     bias = bias.contiguous()
     dq, dk, dv = _heads_last(B, H, Lq, hd, q), _heads_last(B, Hk, Lk, hd, k), _heads_last(B, Hk, Lk, hd, v)
-    dbias = torch.empty_like(bias)
+    dbias = torch.empty(bias.shape if want_dbias else (0,), dtype=bias.dtype, device=dev)
     nbytes = _lib.lib().mb_bias_attn_bwd_workspace(B, H, Lq, bias.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "mb_bias_attn_bwd",
                  *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
                  o.data_ptr(), _st(o), d_o.data_ptr(), _st(d_o), lse.data_ptr(), dq.data_ptr(), _st(dq),
-                 dk.data_ptr(), _st(dk), dv.data_ptr(), _st(dv), dbias.data_ptr(), ws.data_ptr(), nbytes)
+                 dk.data_ptr(), _st(dk), dv.data_ptr(), _st(dv), dbias.data_ptr() if want_dbias else None,
+                 ws.data_ptr(), nbytes)
     return dq, dk, dv, dbias
 
 
@@ -158,8 +159,10 @@ class RelativeBiasAttentionFunction(torch.autograd.Function):
     def backward(ctx, d_o):
         q, k, v, bias, o, lse, lengths, start_rows = ctx.saved_tensors
         max_distance, causal, scale, start = ctx.rest
-        grads = bias_attn_bwd(q, k, v, bias, o, d_o, lse, max_distance, causal, scale, lengths, start_rows, start)
-        return (*grads, None, None, None, None, None, None)
+        want = ctx.needs_input_grad[3]
+        dq, dk, dv, dbias = bias_attn_bwd(q, k, v, bias, o, d_o, lse, max_distance, causal, scale, lengths, start_rows,
+                                          start, want)
+        return dq, dk, dv, dbias if want else None, None, None, None, None, None, None
 
 
 def _check(q, k, v, bias, max_distance, causal, lengths, q_start):

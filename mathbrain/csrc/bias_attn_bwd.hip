@@ -146,7 +146,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     Diagonals diag;
     diag.block = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
     diag.sums = hist + wave * entries + kPad - reach.lo + (lane & 31);
-    float far_hi = 0.f, far_lo = 0.f;
+    // Keys go up, so the blocks at or above the reach come first, those at or below its lower end last.
+    float far_hi = 0.f, far_sum[4] = {0.f, 0.f, 0.f, 0.f};
+    bool first_part = true;
     int last_d0 = 0;
 
     f32x16 dq[HD / 32];
@@ -179,6 +181,11 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
             }
             const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
             const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
+            if (first_part && !above) {
+                first_part = false;
+                far_hi = (far_sum[0] + far_sum[1]) + (far_sum[2] + far_sum[3]);
+                far_sum[0] = far_sum[1] = far_sum[2] = far_sum[3] = 0.f;
+            }
             const int near = kPad - reach.lo + (pos - jb);
             if (one) {
                 const float bias = tab[kPad + (above ? reach.hi - reach.lo : 0)];
@@ -197,18 +204,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 x[r] = kStart ? __builtin_amdgcn_exp2f(x[r]) * y[r] : __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
-            if (want_bias) {
-                if (one) {
-                    diag.close(last_d0);
-                    float sum = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += x[r];
-                    (above ? far_hi : far_lo) += sum;
-                } else {
-                    last_d0 = dlo + 31;
-                    diag.give(x);
-                }
-            }
+            if (want_bias && !one) diag.give(x);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const typename X::Frag f = to_frag<T>(x, c);
@@ -216,7 +212,16 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
                 for (int d = 0; d < HD / 32; ++d)
                     dq[d] = X::mma(Tl::cols(ktile, at, 32 * u + 16 * c, d), f, dq[d]);
             }
-            if (want_bias && !one) diag.take(last_d0);
+            if (want_bias) {   // while the products run
+                if (one) {
+                    diag.close(last_d0);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) far_sum[r % 4] += x[r];
+                } else {
+                    last_d0 = dlo + 31;
+                    diag.take(last_d0);
+                }
+            }
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // LDS is written until then
@@ -227,6 +232,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     }
     if (!want_bias) return;
     diag.close(last_d0);
+    float far_lo = (far_sum[0] + far_sum[1]) + (far_sum[2] + far_sum[3]);
+    if (first_part) far_hi = far_lo, far_lo = 0.f;
     far_hi = wave_sum(far_hi);
     far_lo = wave_sum(far_lo);
     if (lane == 0) far[wave][0] = far_hi, far[wave][1] = far_lo;
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     }
     __syncthreads();
     float* part = a.dbias_part + ((int64_t)h * a.B * a.nq + (int64_t)b * a.nq + qb) * a.buckets;
-    for (int n = wave; n < a.buckets; n += 4) {
+    for (int n = threadIdx.x / 8; n < a.buckets; n += kThreads / 8) {   // eight lanes a bucket
         const bool back = n >= a.n_starts;        // keys behind the query's position
         const int m = back ? n - a.n_starts : n;
         const bool end = m == a.n_starts - 1;
@@ -250,8 +257,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
             e0 = -e1, e1 = -near;
         }
         float v = 0.f;
-        for (int e = e0 - reach.lo + kPad + lane; e <= e1 - reach.lo + kPad; e += 64) v += hist[e];
-        v = wave_sum(v);
+        for (int e = e0 - reach.lo + kPad + (lane & 7); e <= e1 - reach.lo + kPad; e += 8) v += hist[e];
+#pragma unroll
+        for (int o = 4; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
         // whole blocks: at or above the reach, and at or below its lower end, which is distance 0 in
         // a causal table
         const bool below = a.causal ? n == 0 : back && end;
@@ -260,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
             if (end && !back) v += far[w][0];
             if (below) v += far[w][1];
         }
-        if (lane == 0) part[n] = v;
+        if ((lane & 7) == 0) part[n] = v;
     }
 }
 
