@@ -15,6 +15,15 @@ namespace mb {
 namespace battn {
 namespace {
 
+// What the keys' pass needs of a row's lse (log2 units).  In bf16 its products start from -lse in
+// units of the scores.  In fp32 -lse is added after the product instead: the sum of a product that
+// starts from a number of another size is rounded to that one's (dk and dv off by 1.6e-6 of their
+// norms at 2 x 1500 tokens).
+template <typename T>
+__device__ inline float statistic(float lse, float sl2) {
+    return sizeof(T) == 2 ? -lse / sl2 : -lse;
+}
+
 // Sum of a value over the wave's 64 lanes.
 __device__ inline float wave_sum(float v) {
 #pragma unroll
@@ -112,10 +121,15 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     const T* kbase = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vbase = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     typename X::Frag qf[HD / 16], gf[HD / 16];
+    load_frags<T, HD>((const T*)a.d_o + b * a.do_sb + h * a.do_sh, a.do_sl, w0, a.Lq, gf);
+    // delta is dO . o, but o and the probabilities in it are rounded where the inputs are bf16, and
+    // delta's error is that of every ds of its row.  It falls with the number of keys that share
+    // the row's weight; where there are few of them delta is taken from the pairs themselves, in a
+    // walk of its own (64 sequences of 3 tokens, heads of 64: dbias off by 5e-3 of its norm with dO . o).
+    const bool from_pairs = sizeof(T) == 2 && kend <= kRows;
     float delta = 0.f;
-    {
+    if (!from_pairs) {
         load_frags<T, HD>((const T*)a.o + b * a.o_sb + h * a.o_sh, a.o_sl, w0, a.Lq, qf);
-        load_frags<T, HD>((const T*)a.d_o + b * a.do_sb + h * a.do_sh, a.do_sl, w0, a.Lq, gf);
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
@@ -123,20 +137,13 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         delta = half_sum(delta);
     }
     load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
-    // The products' results start from -lse (in units of the scores) and -delta: p is then
-    // exp2(scale x + bias) and ds is p y.  Here two blocks of registers hold them where that leaves
-    // two waves a SIMD room; the keys' pass reads both rows from the workspace.
-    constexpr bool kStart = HD == 64;
-    float nlse = -INFINITY;
-    float lse = INFINITY;
-    if (i < a.Lq) {
-        lse = a.lse[(int64_t)bh * a.Lq + i];
-        nlse = -lse / sl2;
-        if (lane < 32) {
-            a.rows[(int64_t)bh * a.Lq + i] = nlse;
-            a.rows[((int64_t)a.B * a.H + bh) * a.Lq + i] = -delta;
-        }
-    }
+    // In bf16 with heads of 64 the products' results start from -lse (in units of the scores) and
+    // -delta, in two blocks of registers that leave two waves a SIMD room: p is then
+    // exp2(scale x + bias) and ds is p y.
+    constexpr bool kStart = HD == 64 && sizeof(T) == 2;
+    const float lse = i < a.Lq ? a.lse[(int64_t)bh * a.Lq + i] : INFINITY;
+    const float nlse = statistic<T>(lse, sl2);
+    if (i < a.Lq && lane < 32) a.rows[(int64_t)bh * a.Lq + i] = nlse;
     f32x16 x0, y0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) x0[r] = kStart ? nlse : 0.f, y0[r] = kStart ? -delta : 0.f;
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     diag.block = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
     diag.sums = hist + wave * entries + kPad - reach.lo + (lane & 31);
     // Keys go up, so the blocks at or above the reach come first, those at or below its lower end last.
-    float far_hi = 0.f, far_sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float far_hi = 0.f, far_sum = 0.f, row_sum = 0.f;
     bool first_part = true;
     int last_d0 = 0;
 
@@ -157,82 +164,114 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     const uint32_t lds = lds_address(smem);
     const typename Tl::Lane at;
     const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
-    auto load = [&](int t) {
-        const uint32_t tile = lds + t % kStages * (2 * Tl::kBytes);
-        Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
-        Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
-    };
-    loads_done();
-    if (tiles > 0)
-        for (int t = 0; t < kStages - 1; ++t) load(t);
-    for (int t = 0; t < tiles; ++t) {
-        wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
-        load(t + kStages - 1);
-        const uint32_t ktile = lds + t % kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
+    // block(ktile, vtile, u, jb) for the wave's blocks of 32 keys from jb on, in rows 32 u of the tiles
+    auto walk = [&](auto&& block) {
+        auto load = [&](int t) {
+            const uint32_t tile = lds + t % kStages * (2 * Tl::kBytes);
+            Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
+            Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
+        };
+        if (tiles > 0)
+            for (int t = 0; t < kStages - 1; ++t) load(t);
+        for (int t = 0; t < tiles; ++t) {
+            wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
+            load(t + kStages - 1);
+            const uint32_t ktile = lds + t % kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) {
-            const int jb = t * KT + 32 * u;
-            if (jb >= wend) break;
-            f32x16 x = x0, y = y0;
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                x = X::mma(Tl::rows(ktile, at, 32 * u, c), qf[c], x);
-                y = X::mma(Tl::rows(vtile, at, 32 * u, c), gf[c], y);
-            }
-            const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
-            const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
-            if (first_part && !above) {
-                first_part = false;
-                far_hi = (far_sum[0] + far_sum[1]) + (far_sum[2] + far_sum[3]);
-                far_sum[0] = far_sum[1] = far_sum[2] = far_sum[3] = 0.f;
-            }
-            const int near = kPad - reach.lo + (pos - jb);
-            if (one) {
-                const float bias = tab[kPad + (above ? reach.hi - reach.lo : 0)];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, bias);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, tab[near - row_of(r)]);
-            }
-            if ((a.causal && dlo < 0) || jb + 32 > len) {
-                const int most = a.causal ? min(len, pos + 1) : len;
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (jb + row_of(r) >= most) x[r] = -INFINITY;
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                x[r] = kStart ? __builtin_amdgcn_exp2f(x[r]) * y[r] : __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
-            if (want_bias && !one) diag.give(x);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const typename X::Frag f = to_frag<T>(x, c);
-#pragma unroll
-                for (int d = 0; d < HD / 32; ++d)
-                    dq[d] = X::mma(Tl::cols(ktile, at, 32 * u + 16 * c, d), f, dq[d]);
-            }
-            if (want_bias) {   // while the products run
-                if (one) {
-                    diag.close(last_d0);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) far_sum[r % 4] += x[r];
-                } else {
-                    last_d0 = dlo + 31;
-                    diag.take(last_d0);
-                }
+            for (int u = 0; u < KT / 32; ++u) {
+                const int jb = t * KT + 32 * u;
+                if (jb >= wend) break;
+                block(ktile, vtile, u, jb);
             }
         }
+        wait_and_meet<0>();   // LDS is written until then
+    };
+    // A block's exponents (log2 of p, but for lse where the products do not start from it) and dO . v
+    // (less delta where they do).
+    auto products = [&](uint32_t ktile, uint32_t vtile, int u, int jb, f32x16& x, f32x16& y) {
+        x = x0, y = y0;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+            x = X::mma(Tl::rows(ktile, at, 32 * u, c), qf[c], x);
+            y = X::mma(Tl::rows(vtile, at, 32 * u, c), gf[c], y);
+        }
+        const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
+        if (dlo >= reach.hi || dhi <= reach.lo) {
+            const float bias = tab[kPad + (dlo >= reach.hi ? reach.hi - reach.lo : 0)];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, bias);
+        } else {
+            const float* near = tab + kPad - reach.lo + (pos - jb);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], sl2, near[-row_of(r)]);
+        }
+        if ((a.causal && dlo < 0) || jb + 32 > len) {
+            const int most = a.causal ? min(len, pos + 1) : len;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (jb + row_of(r) >= most) x[r] = -INFINITY;
+        }
+    };
+    loads_done();
+    if (from_pairs) {
+        walk([&](uint32_t ktile, uint32_t vtile, int u, int jb) {
+            f32x16 x, y;
+            products(ktile, vtile, u, jb, x, y);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) delta = __builtin_fmaf(__builtin_amdgcn_exp2f(kStart ? x[r] : x[r] - lse), y[r], delta);
+        });
+        delta = half_sum(delta);
+        if (kStart)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y0[r] = -delta;
     }
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // LDS is written until then
+    walk([&](uint32_t ktile, uint32_t vtile, int u, int jb) {
+        f32x16 x, y;
+        products(ktile, vtile, u, jb, x, y);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            x[r] = kStart ? __builtin_amdgcn_exp2f(x[r]) * y[r] : __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
+        const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
+        const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
+        if (first_part && !above) {
+            first_part = false;
+            far_hi = far_sum, far_sum = 0.f;
+        }
+        if (want_bias && !one) diag.give(x);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const typename X::Frag f = to_frag<T>(x, c);
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) dq[d] = X::mma(Tl::cols(ktile, at, 32 * u + 16 * c, d), f, dq[d]);
+        }
+        // while the products run:
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r % 4] += x[r];
+        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        row_sum += all;
+        if (want_bias) {
+            if (one) {
+                diag.close(last_d0);
+                far_sum += all;
+            } else {
+                last_d0 = dlo + 31;
+                diag.take(last_d0);
+            }
+        }
+    });
+    // A row's ds sum to zero but for delta's error, which comes from o's rounding and that of the
+    // probabilities in it: for the keys' pass delta is put right by what is left.
+    row_sum = half_sum(row_sum);
     if (i < a.Lq) {
+        if (lane < 32) a.rows[((int64_t)a.B * a.H + bh) * a.Lq + i] = -(delta + row_sum);
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d) store_block<T>(row, 32 * d, dq[d], a.scale);
     }
     if (!want_bias) return;
     diag.close(last_d0);
-    float far_lo = (far_sum[0] + far_sum[1]) + (far_sum[2] + far_sum[3]);
+    float far_lo = far_sum;
     if (first_part) far_hi = far_lo, far_lo = 0.f;
     far_hi = wave_sum(far_hi);
     far_lo = wave_sum(far_lo);
@@ -342,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
                     const f32x4 nl = *reinterpret_cast<const f32x4*>(&stat[s][0][32 * u + 8 * r + 4 * g]);
                     const f32x4 nd = *reinterpret_cast<const f32x4*>(&stat[s][1][32 * u + 8 * r + 4 * g]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[4 * r + e] = nl[e], y[4 * r + e] = nd[e];
+                    for (int e = 0; e < 4; ++e) x[4 * r + e] = sizeof(T) == 2 ? nl[e] : 0.f, y[4 * r + e] = nd[e];
                 }
 #pragma unroll
                 for (int c = 0; c < HD / 16; ++c) {
@@ -366,6 +405,14 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
                     for (int r = 0; r < 16; ++r) {
                         const int i = ib + row_of(r);
                         if (i < least || i >= a.Lq) x[r] = -INFINITY;
+                    }
+                }
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const f32x4 nl = *reinterpret_cast<const f32x4*>(&stat[s][0][32 * u + 8 * r + 4 * g]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[4 * r + e] += nl[e];
                     }
                 }
 #pragma unroll
