@@ -675,7 +675,7 @@ int mb_bias_attn_fwd(const void *q, const int64_t *q_st, const void *k, const in
                      int B, int H, int Hk, int Lq, int Lk, int hd, float scale, int causal,
                      int dtype, void *o, const int64_t *o_st, float *lse, void *workspace,
                      int64_t workspace_bytes, void *stream);
-int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd);
+int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal);
 int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets);
 int mb_bias_attn_bwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
                      const void *v, const int64_t *v_st, const void *bias, int bias_dtype,

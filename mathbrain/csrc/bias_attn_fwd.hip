@@ -157,9 +157,9 @@ int launch(const Args& a, hipStream_t st) {
 using namespace mb;
 using namespace mb::battn;
 
-extern "C" int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd) {
+extern "C" int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
     if (B < 1 || H < 1 || Hk < 1 || H % Hk || Lq < 1 || Lk < 0 || hd < 1) return 0;
-    const int64_t splits = splits_of(B, H, Hk, Lq, Lk);
+    const int64_t splits = splits_of(B, H, Hk, Lq, Lk, hd, causal);
     return splits > 1 ? (int64_t)B * H * Lq * splits * (hd + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -179,12 +179,12 @@ extern "C" int mb_bias_attn_fwd(const void* q, const int64_t* q_st, const void* 
     MB_REQUIRE(rows16(o, o_st, dtype), "mb_bias_attn_fwd: o's rows must begin at multiples of 16 bytes");
     a.out = o, a.out_sb = o_st[0], a.out_sh = o_st[1], a.out_sl = o_st[2];
     a.lse = lse;
-    const int64_t need = mb_bias_attn_fwd_workspace(B, H, Hk, Lq, Lk, hd);
+    const int64_t need = mb_bias_attn_fwd_workspace(B, H, Hk, Lq, Lk, hd, causal);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(MB_ERR_WORKSPACE, "mb_bias_attn_fwd: workspace of %lld bytes, %lld are needed",
                     (long long)workspace_bytes, (long long)need);
     hipStream_t st = (hipStream_t)stream;
-    if (const int splits = splits_of(B, H, Hk, Lq, Lk)) return split_launch(a, hd, dtype, splits, workspace, st);
+    if (const int splits = splits_of(B, H, Hk, Lq, Lk, hd, causal)) return split_launch(a, hd, dtype, splits, workspace, st);
     if (dtype == MB_DTYPE_F32) return hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st);
     return hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st);
 }

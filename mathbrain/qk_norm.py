@@ -74,7 +74,7 @@ def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     dev = q.device
     B, L, H, hd = q.shape
     q, k = _rows16(q.detach()), _rows16(k.detach())
-    gq, gk = _rows16(dq_out.to(q.dtype)), _rows16(dk_out.to(k.dtype))
+    gq, gk = (_rows16(g if g.dtype is q.dtype else g.to(q.dtype)) for g in (dq_out, dk_out))
     wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
     dq = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
     dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
@@ -87,7 +87,9 @@ def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
                  wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first, B, L, H,
                  k.shape[2], hd, eps, _DTYPES[q.dtype], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
                  dwk.data_ptr(), ws.data_ptr(), ws.numel())
-    return dq, dk, dwq.to(q_weight.dtype), dwk.to(k_weight.dtype)
+    if q_weight.dtype is not torch.float32 or k_weight.dtype is not torch.float32:
+        dwq, dwk = dwq.to(q_weight.dtype), dwk.to(k_weight.dtype)
+    return dq, dk, dwq, dwk
 
 
 class QKNormRotaryFunction(torch.autograd.Function):
