@@ -617,32 +617,31 @@ int mb_swiglu_bwd(const void *a, const void *b, const void *dm, int64_t n, int d
  *   n = x rsqrt(mean(x^2) + eps),  y = w n,
  *   out[2i] = y[2i] cos[p,i] - y[2i+1] sin[p,i],  out[2i+1] = y[2i] sin[p,i] + y[2i+1] cos[p,i]
  *
- *   q, k           [B, L, H | Hk, hd], element strides (_sb, _sl, _sh), channels next to each
- *                  other, rows at multiples of 16 bytes; dtype MB_DTYPE_F32 or MB_DTYPE_BF16
- *   wq, wk         [hd] fp32;  cos, sin  [table_rows, hd / 2] fp32 contiguous
- *   start          [B] position of each row's first token, int32 (start_bytes 4) or int64 (8),
- *                  or NULL: start0 for all.  A position outside [0, table_rows) gives NaN.
- *   q_out, k_out   [B, L, H | Hk, hd] contiguous, 16-byte aligned
- *
- * The backward takes the outputs' gradients dq_out, dk_out (strides as above) and writes
- * dq, dk (contiguous) and dwq, dwk [hd] fp32; the weight sums have a fixed order.  Its
- * workspace is mb_qk_norm_rotary_bwd_workspace(B, L, hd) bytes.  hd: 32, 64 or 128.
+ * The arguments come in a struct on the HOST, read before the call returns.
  */
-int mb_qk_norm_rotary_fwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
-                          int64_t k_sb, int64_t k_sl, int64_t k_sh, const float *wq,
-                          const float *wk, const float *cos, const float *sin, int64_t table_rows,
-                          const void *start, int start_bytes, int64_t start0, int B, int L, int H,
-                          int Hk, int hd, float eps, int dtype, void *q_out, void *k_out,
-                          void *stream);
+typedef struct mb_qk_norm_rotary {
+    const void *q, *k;            /* [B, L, H | Hk, hd], channels next to each other, rows at */
+    int64_t q_st[3], k_st[3];     /*   multiples of 16 bytes; element strides of B, L and H */
+    const float *wq, *wk;         /* [hd] */
+    const float *cos, *sin;       /* [table_rows, hd / 2] contiguous */
+    int64_t table_rows;
+    const void *start;            /* [B] position of each row's first token, or NULL: start0. A */
+    int64_t start_bytes, start0;  /*   position outside [0, table_rows) gives NaN. 4: int32, 8: int64 */
+    int64_t B, L, H, Hk, hd;      /* hd: 32, 64 or 128 */
+    int64_t dtype;                /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
+    double eps;
+    void *q_out, *k_out;          /* forward: [B, L, H | Hk, hd] contiguous, 16-byte aligned */
+    const void *dq_out, *dk_out;  /* backward: the outputs' gradients, as q and k */
+    int64_t dq_st[3], dk_st[3];
+    void *dq, *dk;                /* backward: contiguous, 16-byte aligned */
+    float *dwq, *dwk;             /* backward: [hd]; sums in a fixed order */
+    void *workspace;              /* backward: mb_qk_norm_rotary_bwd_workspace(B, L, hd) bytes */
+    int64_t workspace_bytes;
+} mb_qk_norm_rotary;
+
+int mb_qk_norm_rotary_fwd(const mb_qk_norm_rotary *args, void *stream);
 int64_t mb_qk_norm_rotary_bwd_workspace(int B, int L, int hd);
-int mb_qk_norm_rotary_bwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
-                          int64_t k_sb, int64_t k_sl, int64_t k_sh, const void *dq_out,
-                          int64_t dq_sb, int64_t dq_sl, int64_t dq_sh, const void *dk_out,
-                          int64_t dk_sb, int64_t dk_sl, int64_t dk_sh, const float *wq,
-                          const float *wk, const float *cos, const float *sin, int64_t table_rows,
-                          const void *start, int start_bytes, int64_t start0, int B, int L, int H,
-                          int Hk, int hd, float eps, int dtype, void *dq, void *dk, float *dwq,
-                          float *dwk, void *workspace, int64_t workspace_bytes, void *stream);
+int mb_qk_norm_rotary_bwd(const mb_qk_norm_rotary *args, void *stream);
 
 /*
  * Attention with a learned relative position bias by distance buckets:
@@ -650,42 +649,42 @@ int mb_qk_norm_rotary_bwd(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_s
  *   s_ij = scale q_i . k_j + bias[bucket(pos_i - j), h],  p = softmax_j(s),  o_i = sum_j p_ij v_j
  *   dq, dk, dv and dbias[n, h] = sum over the pairs of bucket n of ds_ij for an output gradient d_o
  *
- *   q, o, d_o, dq   [B, H, Lq, hd];  k, v, dk, dv  [B, Hk, Lk, hd], Hk divides H.  dtype
- *                   MB_DTYPE_F32 or MB_DTYPE_BF16, channels next to each other, rows at multiples
- *                   of 16 bytes.  Each comes with a HOST array of its element strides (B, H, L).
- *   bias, dbias     [buckets, H] contiguous, bias_dtype MB_DTYPE_F32 or MB_DTYPE_BF16
- *   starts          HOST array: the first distance of each of n_starts buckets, not falling, from
- *                   0 to at most 1024; the last bucket has no end.  n_starts <= 128.  causal:
- *                   buckets = n_starts.  Otherwise buckets = 2 n_starts, the upper half for keys
- *                   behind the query's position (distance j - pos_i >= 1).
- *   lengths         [B] keys that count, or NULL: Lk (int32 or int64: lengths_bytes 4 or 8);
- *                   rows of k and v from there on are not used, their gradients are zero
- *   q_start         [B] position of each row's first query (likewise), or NULL: q_start0
- *   causal          a query sees the keys j <= pos_i
- *   lse             [B, H, Lq] fp32: log2 of the softmax denominators, written by the forward
- *                   (NULL: not wanted), read by the backward
- *
- * Rows without a key give zeros.  The workspaces are mb_bias_attn_fwd_workspace(...) (0 where the
- * keys are not split over workgroups) and mb_bias_attn_bwd_workspace(...) bytes; dbias may be NULL.  Its sums have a fixed order.  hd: 32, 64 or 128.
+ * The arguments come in a struct on the HOST, read before the call returns.  Tensors have their
+ * channels next to each other and rows at multiples of 16 bytes, at most 16 MiB apart; strides are
+ * those of B, H and L in elements.  Rows without a key give zeros.  Sums have a fixed order.
  */
-int mb_bias_attn_fwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
-                     const void *v, const int64_t *v_st, const void *bias, int bias_dtype,
-                     int buckets, const int32_t *starts, int n_starts, const void *lengths,
-                     int lengths_bytes, const void *q_start, int q_start_bytes, int64_t q_start0,
-                     int B, int H, int Hk, int Lq, int Lk, int hd, float scale, int causal,
-                     int dtype, void *o, const int64_t *o_st, float *lse, void *workspace,
-                     int64_t workspace_bytes, void *stream);
+typedef struct mb_bias_attn {
+    const void *q, *k, *v;        /* [B, H, Lq, hd], [B, Hk, Lk, hd] twice; Hk divides H */
+    int64_t q_st[3], k_st[3], v_st[3];
+    const void *bias;             /* [buckets, H] contiguous */
+    const int32_t *starts;        /* HOST: the first distance of each of n_starts buckets, not falling, */
+    int64_t buckets, n_starts;    /*   from 0 to at most 1024; the last one has no end. n_starts <= 128. */
+                                  /*   causal: buckets = n_starts; otherwise 2 n_starts, the upper half */
+                                  /*   for keys behind the query (distance j - pos_i >= 1) */
+    const void *lengths;          /* [B] keys that count, or NULL: Lk. Rows of k and v from there on */
+    int64_t lengths_bytes;        /*   are not used, their gradients are zero. 4: int32, 8: int64 */
+    const void *q_start;          /* [B] position of each row's first query, or NULL: q_start0 */
+    int64_t q_start_bytes, q_start0;
+    int64_t B, H, Hk, Lq, Lk, hd; /* hd: 32, 64 or 128 */
+    int64_t causal;               /* a query sees the keys j <= pos_i */
+    int64_t dtype, bias_dtype;    /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
+    double scale;
+    void *o;                      /* [B, H, Lq, hd]: written by the forward, read by the backward */
+    int64_t o_st[3];
+    float *lse;                   /* [B, H, Lq] log2 of the softmax denominators, likewise (NULL: not wanted) */
+    const void *d_o;              /* backward from here on */
+    int64_t do_st[3];
+    void *dq, *dk, *dv;
+    int64_t dq_st[3], dk_st[3], dv_st[3];
+    void *dbias;                  /* [buckets, H] of bias_dtype, or NULL */
+    void *workspace;              /* both: mb_bias_attn_fwd_workspace(...) (0 where the keys are not split */
+    int64_t workspace_bytes;      /*   over workgroups) or mb_bias_attn_bwd_workspace(...) bytes */
+} mb_bias_attn;
+
 int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal);
+int mb_bias_attn_fwd(const mb_bias_attn *args, void *stream);
 int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets);
-int mb_bias_attn_bwd(const void *q, const int64_t *q_st, const void *k, const int64_t *k_st,
-                     const void *v, const int64_t *v_st, const void *bias, int bias_dtype,
-                     int buckets, const int32_t *starts, int n_starts, const void *lengths,
-                     int lengths_bytes, const void *q_start, int q_start_bytes, int64_t q_start0,
-                     int B, int H, int Hk, int Lq, int Lk, int hd, float scale, int causal,
-                     int dtype, const void *o, const int64_t *o_st, const void *d_o,
-                     const int64_t *do_st, const float *lse, void *dq, const int64_t *dq_st,
-                     void *dk, const int64_t *dk_st, void *dv, const int64_t *dv_st, void *dbias,
-                     void *workspace, int64_t workspace_bytes, void *stream);
+int mb_bias_attn_bwd(const mb_bias_attn *args, void *stream);
 
 /*
  * Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_ in the reference's training

@@ -24,10 +24,6 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
 
-# q, k, v, the bias table, lengths, positions, sizes: what both directions of the attention with
-# a learned bias begin with
-_BIAS_ATTN = ([_p] * 6 + [_p, _i, _i, _p, _i, _p, _i, _p, _i, _i64] + [_i] * 6 + [_f, _i, _i])
-
 # name -> argtypes; every entry is declared in include/mathbrain_hip.h
 SIGNATURES = {
     "mb_last_error": ([], ctypes.c_char_p),
@@ -77,15 +73,12 @@ SIGNATURES = {
     "mb_rmsnorm_bwd": ([_p, _p, _p, _p, _i64, _i, _p, _p, _p], _i),
     "mb_layernorm_fwd": ([_p, _p, _p, _i64, _i, _f, _p, _p, _p, _p], _i),
     "mb_layernorm_bwd": ([_p, _p, _p, _p, _p, _i64, _i, _p, _p, _p, _p], _i),
-    "mb_qk_norm_rotary_fwd": ([_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i, _i64,
-                               _i, _i, _i, _i, _i, _f, _i, _p, _p, _p], _i),
-    "mb_qk_norm_rotary_bwd": ([_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64,
-                               _i64, _p, _p, _p, _p, _i64, _p, _i, _i64, _i, _i, _i, _i, _i, _f, _i, _p, _p, _p,
-                               _p, _p, _i64, _p], _i),
+    "mb_qk_norm_rotary_fwd": ([_p, _p], _i),
+    "mb_qk_norm_rotary_bwd": ([_p, _p], _i),
     "mb_qk_norm_rotary_bwd_workspace": ([_i, _i, _i], _i64),
-    "mb_bias_attn_fwd": (_BIAS_ATTN + [_p, _p, _p, _p, _i64, _p], _i),
+    "mb_bias_attn_fwd": ([_p, _p], _i),
     "mb_bias_attn_fwd_workspace": ([_i] * 7, _i64),
-    "mb_bias_attn_bwd": (_BIAS_ATTN + [_p] * 5 + [_p] * 7 + [_p, _i64, _p], _i),
+    "mb_bias_attn_bwd": ([_p, _p], _i),
     "mb_bias_attn_bwd_workspace": ([_i, _i, _i, _i], _i64),
     "mb_grad_clip": ([_p, _p, _p, _p, _p, _i, _f, _p, _p, _i64, _p], _i),
     "mb_grad_clip_workspace": ([_i], _i64),
@@ -142,12 +135,18 @@ def call_on(dev, name, *args):
     """call(name, *args, stream) on the current stream of device `dev`, whichever device is
     current.  For entry points that take a few microseconds: the device is switched only where
     it has to be."""
-    index = dev.index
-    if index is None or index == torch.cuda.current_device():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    here = torch._C._cuda_getDevice()
+    if dev.index == here:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(here))
         return
     with torch.cuda.device(dev):
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
+@functools.lru_cache(maxsize=1024)
+def workspace_bytes(name, *sizes):
+    """What the library's function `name` says for these sizes."""
+    return getattr(lib(), name)(*sizes)
 
 
 def ptr(t):

@@ -20,6 +20,7 @@ torch ops (mathbrain::bias_attn_fwd / _bwd) for tracing.
 import ctypes
 import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -27,6 +28,9 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.MB_DTYPE_F32, torch.bfloat16: _lib.MB_DTYPE_BF16}
+# mb_bias_attn (include/mathbrain_hip.h): the inputs, o and lse, the backward's tensors, the workspace
+_ARGS = struct.Struct("3P9qPP2qPqP2q6qq2qd" + "P3qP" + "P3q3P9qP" + "Pq")
+_NO_BACKWARD = (0,) * 17
 MAX_BUCKETS = 128     # in one direction
 MAX_DISTANCE = 1024
 
@@ -54,8 +58,10 @@ def bucket_starts(num_buckets, max_distance):
 
 @functools.lru_cache(maxsize=64)
 def _starts_array(num_buckets, max_distance, causal):
+    """(array, its address, its length): the array is kept with the address."""
     starts = bucket_starts(num_buckets if causal else num_buckets // 2, max_distance)
-    return (ctypes.c_int32 * len(starts))(*starts), len(starts)
+    array = (ctypes.c_int32 * len(starts))(*starts)
+    return array, ctypes.addressof(array), len(starts)
 
 
 def _rows16(x):
@@ -66,28 +72,21 @@ def _rows16(x):
     return x.contiguous() if not x.is_contiguous() else x.clone()
 
 
-def _st(x):
-    return (ctypes.c_int64 * 3)(*x.stride()[:3])
-
-
-def _per_row(rows, value=0):
-    """(pointer, bytes of an element, value) of an optional int tensor [B]."""
-    return (None, 4, value) if rows is None else (rows.data_ptr(), rows.element_size(), 0)
-
-
 def _heads_last(B, H, L, hd, like):
     """[B, H, L, hd] over memory [B, L, H, hd], so that the projections around it need no copy."""
-    return torch.empty((B, L, H, hd), dtype=like.dtype, device=like.device).transpose(1, 2)
+    return torch.empty_strided((B, H, L, hd), (L * H * hd, hd, H * hd, 1), dtype=like.dtype, device=like.device)
 
 
 def _inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start):
-    """The arguments that both directions begin with."""
+    """The struct's fields up to scale."""
     B, H, Lq, hd = q.shape
-    starts, n_starts = _starts_array(bias.shape[0], max_distance, causal)
-    at, at_bytes, first = _per_row(start_rows, start)
-    return (q.data_ptr(), _st(q), k.data_ptr(), _st(k), v.data_ptr(), _st(v), bias.data_ptr(), _DTYPES[bias.dtype],
-            bias.shape[0], starts, n_starts, *_per_row(lengths)[:2], at, at_bytes, first, B, H, k.shape[1], Lq,
-            k.shape[2], hd, scale, int(causal), _DTYPES[q.dtype])
+    buckets = bias.shape[0]
+    _, starts, n_starts = _starts_array(buckets, max_distance, causal)
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bias.data_ptr(),
+            starts, buckets, n_starts, 0 if lengths is None else lengths.data_ptr(),
+            4 if lengths is None else lengths.element_size(), 0 if start_rows is None else start_rows.data_ptr(),
+            4 if start_rows is None else start_rows.element_size(), start, B, H, k.shape[1], Lq, k.shape[2], hd, causal,
+            _DTYPES[q.dtype], _DTYPES[bias.dtype], scale)
 
 
 def _fwd_fake(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start, want_lse):
@@ -107,11 +106,12 @@ def bias_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     q, k, v, bias = _rows16(q), _rows16(k), _rows16(v), bias.contiguous()
     o = _heads_last(B, H, Lq, hd, q)
     lse = torch.empty((B, H, Lq) if want_lse else (0,), dtype=torch.float32, device=dev)
-    nbytes = _lib.lib().mb_bias_attn_fwd_workspace(B, H, k.shape[1], Lq, k.shape[2], hd, int(causal))
+    nbytes = _lib.workspace_bytes("mb_bias_attn_fwd_workspace", B, H, k.shape[1], Lq, k.shape[2], hd, causal)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.call_on(dev, "mb_bias_attn_fwd",
-                 *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
-                 o.data_ptr(), _st(o), lse.data_ptr() if want_lse else None, ws.data_ptr() if nbytes else None, nbytes)
+                 _ARGS.pack(*_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
+                            o.data_ptr(), *o.stride()[:3], lse.data_ptr() if want_lse else 0, *_NO_BACKWARD,
+                            ws.data_ptr() if nbytes else 0, nbytes))
     return o, lse
 
 
@@ -131,17 +131,17 @@ def bias_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     dev = q.device
     B, H, Lq, hd = q.shape
     Hk, Lk = k.shape[1:3]
-    q, k, v, o, d_o = _rows16(q), _rows16(k), _rows16(v), _rows16(o), _rows16(d_o.to(q.dtype))
+    q, k, v, o, d_o = _rows16(q), _rows16(k), _rows16(v), _rows16(o), _rows16(d_o if d_o.dtype is q.dtype else d_o.to(q.dtype))
     bias = bias.contiguous()
     dq, dk, dv = _heads_last(B, H, Lq, hd, q), _heads_last(B, Hk, Lk, hd, k), _heads_last(B, Hk, Lk, hd, v)
     dbias = torch.empty(bias.shape if want_dbias else (0,), dtype=bias.dtype, device=dev)
-    nbytes = _lib.lib().mb_bias_attn_bwd_workspace(B, H, Lq, bias.shape[0])
+    nbytes = _lib.workspace_bytes("mb_bias_attn_bwd_workspace", B, H, Lq, bias.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "mb_bias_attn_bwd",
-                 *_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
-                 o.data_ptr(), _st(o), d_o.data_ptr(), _st(d_o), lse.data_ptr(), dq.data_ptr(), _st(dq),
-                 dk.data_ptr(), _st(dk), dv.data_ptr(), _st(dv), dbias.data_ptr() if want_dbias else None,
-                 ws.data_ptr(), nbytes)
+                 _ARGS.pack(*_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
+                            o.data_ptr(), *o.stride()[:3], lse.data_ptr(), d_o.data_ptr(), *d_o.stride()[:3],
+                            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3],
+                            *dv.stride()[:3], dbias.data_ptr() if want_dbias else 0, ws.data_ptr(), nbytes))
     return dq, dk, dv, dbias
 
 
@@ -168,16 +168,19 @@ class RelativeBiasAttentionFunction(torch.autograd.Function):
 def _check(q, k, v, bias, max_distance, causal, lengths, q_start):
     what = "relative_bias_attention"
     rows = q_start if torch.is_tensor(q_start) else None
-    _lib.require_gpu(q, k, v, bias, lengths, rows, what=what)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are not [B, H, Lq, hd] "
+    at = q.get_device()
+    if (at < 0 or k.get_device() != at or v.get_device() != at or bias.get_device() != at
+            or (lengths is not None and lengths.get_device() != at) or (rows is not None and rows.get_device() != at)):
+        _lib.require_gpu(q, k, v, bias, lengths, rows, what=what)
+    qs, ks, bs = q.shape, k.shape, bias.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[3] != ks[3]:
+        raise ValueError(f"{what}: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} are not [B, H, Lq, hd] "
                          "and twice [B, Hk, Lk, hd]")
     if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{what}: q {q.dtype}, k {k.dtype}, v {v.dtype} (supported: all float32 or all bfloat16)")
-    if bias.dim() != 2 or bias.shape[1] != q.shape[1] or bias.dtype not in _DTYPES:
-        raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} is not [buckets, {q.shape[1]}] in float32 or "
-                         "bfloat16")
-    buckets = bias.shape[0]
+    if len(bs) != 2 or bs[1] != qs[1] or bias.dtype not in _DTYPES:
+        raise ValueError(f"{what}: bias {tuple(bs)} {bias.dtype} is not [buckets, {qs[1]}] in float32 or bfloat16")
+    buckets = bs[0]
     if buckets < 1 or (not causal and buckets % 2):
         raise ValueError(f"{what}: {buckets} buckets (at least one, and an even number without causal)")
     side = buckets if causal else buckets // 2
@@ -185,9 +188,9 @@ def _check(q, k, v, bias, max_distance, causal, lengths, q_start):
         raise ValueError(f"{what}: {side} buckets in a direction up to distance {max_distance} (supported: at most "
                          f"{MAX_BUCKETS}, and a distance above half of them, at most {MAX_DISTANCE})")
     for name, t in (("lengths", lengths), ("q_start", rows)):
-        if t is not None and (t.shape != (q.shape[0],) or t.dtype not in (torch.int32, torch.int64)):
+        if t is not None and (t.shape != qs[:1] or t.dtype not in (torch.int32, torch.int64)):
             raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} is not one int32 or int64 for each of "
-                             f"{q.shape[0]} rows")
+                             f"{qs[0]} rows")
 
 
 def relative_bias_attention(q, k, v, bias, max_distance=128, causal=True, scale=None, lengths=None, q_start=None):

@@ -484,11 +484,13 @@ int launch(const Args& a, hipStream_t st) {
     const int base = 2 * kStages * Tile<T, HD>::kBytes + table;
     const int lds_q = 2 * kStages * QueryTile<T, HD>::kBytes + table + (a.dbias_part ? (4 * entries + 3 + 4 * 32 * Diagonals::kStride) * (int)sizeof(float) : 0);
     if (a.Lq > 0) {
-        if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q)) return rc;
+        static Told told;
+        if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q, told)) return rc;
         hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds_q, st, a);
     }
     if (a.Lk > 0) {
-        if (const int rc = allow_lds((const void*)bias_attn_dkv_kernel<T, HD>, base)) return rc;
+        static Told told;
+        if (const int rc = allow_lds((const void*)bias_attn_dkv_kernel<T, HD>, base, told)) return rc;
         const int nk = (a.Lk + kRows - 1) / kRows;
         hipLaunchKernelGGL((bias_attn_dkv_kernel<T, HD>), dim3((unsigned)(a.B * a.Hk * nk)), dim3(kThreads), base, st, a);
     }
@@ -510,51 +512,42 @@ extern "C" int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets)
     return (padded(2 * (int64_t)B * H * Lq) + (int64_t)H * B * nq * buckets) * (int64_t)sizeof(float);
 }
 
-extern "C" int mb_bias_attn_bwd(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
-                                const int64_t* v_st, const void* bias, int bias_dtype, int buckets,
-                                const int32_t* starts, int n_starts, const void* lengths, int lengths_bytes,
-                                const void* q_start, int q_start_bytes, int64_t q_start0, int B, int H, int Hk, int Lq,
-                                int Lk, int hd, float scale, int causal, int dtype, const void* o, const int64_t* o_st,
-                                const void* d_o, const int64_t* do_st, const float* lse, void* dq, const int64_t* dq_st,
-                                void* dk, const int64_t* dk_st, void* dv, const int64_t* dv_st, void* dbias,
-                                void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int mb_bias_attn_bwd(const mb_bias_attn* p, void* stream) {
     Args a = {};
-    if (const int rc = fill_args("mb_bias_attn_bwd", a, q, q_st, k, k_st, v, v_st, bias, bias_dtype, buckets, starts,
-                                 n_starts, lengths, lengths_bytes, q_start, q_start_bytes, q_start0, B, H, Hk, Lq, Lk,
-                                 hd, scale, causal, dtype))
-        return rc;
-    const int64_t need = mb_bias_attn_bwd_workspace(B, H, Lq, buckets);
-    if (need > 0 && (!workspace || workspace_bytes < need))
+    if (const int rc = fill_args("mb_bias_attn_bwd", p, a)) return rc;
+    const int hd = (int)p->hd, dtype = (int)p->dtype;
+    const int64_t need = mb_bias_attn_bwd_workspace(a.B, a.H, a.Lq, a.buckets);
+    if (need > 0 && (!p->workspace || p->workspace_bytes < need))
         return fail(MB_ERR_WORKSPACE, "mb_bias_attn_bwd: workspace of %lld bytes, %lld are needed",
-                    (long long)workspace_bytes, (long long)need);
-    if (B > 0 && Lq > 0) {
-        MB_REQUIRE(o && o_st && d_o && do_st && lse && dq && dq_st, "mb_bias_attn_bwd: null pointer argument");
-        MB_REQUIRE(rows16(o, o_st, dtype) && rows16(d_o, do_st, dtype) && rows16(dq, dq_st, dtype),
+                    (long long)p->workspace_bytes, (long long)need);
+    if (a.B > 0 && a.Lq > 0) {
+        MB_REQUIRE(p->o && p->d_o && p->lse && p->dq, "mb_bias_attn_bwd: null pointer argument");
+        MB_REQUIRE(rows16(p->o, p->o_st, dtype) && rows16(p->d_o, p->do_st, dtype) && rows16(p->dq, p->dq_st, dtype),
                    "mb_bias_attn_bwd: rows must begin at multiples of 16 bytes");
-        MB_REQUIRE(do_st[2] >= 0 && do_st[2] <= (1 << 24) / (dtype == MB_DTYPE_F32 ? 4 : 2),
-                   "mb_bias_attn_bwd: d_o's rows are %lld elements apart", (long long)do_st[2]);
-        a.o = o, a.o_sb = o_st[0], a.o_sh = o_st[1], a.o_sl = o_st[2];
-        a.d_o = d_o, a.do_sb = do_st[0], a.do_sh = do_st[1], a.do_sl = do_st[2];
-        a.out = dq, a.out_sb = dq_st[0], a.out_sh = dq_st[1], a.out_sl = dq_st[2];
+        MB_REQUIRE(p->do_st[2] >= 0 && p->do_st[2] <= (1 << 24) / (dtype == MB_DTYPE_F32 ? 4 : 2),
+                   "mb_bias_attn_bwd: d_o's rows are %lld elements apart", (long long)p->do_st[2]);
+        a.o = p->o, a.o_sb = p->o_st[0], a.o_sh = p->o_st[1], a.o_sl = p->o_st[2];
+        a.d_o = p->d_o, a.do_sb = p->do_st[0], a.do_sh = p->do_st[1], a.do_sl = p->do_st[2];
+        a.out = p->dq, a.out_sb = p->dq_st[0], a.out_sh = p->dq_st[1], a.out_sl = p->dq_st[2];
     }
-    if (B > 0 && Lk > 0) {
-        MB_REQUIRE(dk && dk_st && dv && dv_st, "mb_bias_attn_bwd: null pointer argument");
-        MB_REQUIRE(rows16(dk, dk_st, dtype) && rows16(dv, dv_st, dtype), "mb_bias_attn_bwd: rows must begin at multiples of 16 bytes");
-        a.dk = dk, a.dk_sb = dk_st[0], a.dk_sh = dk_st[1], a.dk_sl = dk_st[2];
-        a.dv = dv, a.dv_sb = dv_st[0], a.dv_sh = dv_st[1], a.dv_sl = dv_st[2];
+    if (a.B > 0 && a.Lk > 0) {
+        MB_REQUIRE(p->dk && p->dv, "mb_bias_attn_bwd: null pointer argument");
+        MB_REQUIRE(rows16(p->dk, p->dk_st, dtype) && rows16(p->dv, p->dv_st, dtype), "mb_bias_attn_bwd: rows must begin at multiples of 16 bytes");
+        a.dk = p->dk, a.dk_sb = p->dk_st[0], a.dk_sh = p->dk_st[1], a.dk_sl = p->dk_st[2];
+        a.dv = p->dv, a.dv_sb = p->dv_st[0], a.dv_sh = p->dv_st[1], a.dv_sl = p->dv_st[2];
     }
-    a.lse = const_cast<float*>(lse);
-    a.rows = (float*)workspace;
-    a.dbias_part = dbias && need > 0 ? (float*)workspace + padded(2 * (int64_t)B * H * Lq) : nullptr;
+    a.lse = p->lse;
+    a.rows = (float*)p->workspace;
+    a.dbias_part = p->dbias && need > 0 ? (float*)p->workspace + padded(2 * (int64_t)a.B * a.H * a.Lq) : nullptr;
     hipStream_t st = (hipStream_t)stream;
-    if (B > 0) {
+    if (a.B > 0) {
         const int rc = dtype == MB_DTYPE_F32
                            ? (hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st))
                            : (hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st));
         if (rc) return rc;
     }
-    if (dbias)
-        hipLaunchKernelGGL(bias_attn_dbias_kernel, dim3(H), dim3(kThreads), 0, st, a.dbias_part,
-                           a.dbias_part ? a.B * a.nq : 0, buckets, H, a.bias_bf16, dbias);
+    if (p->dbias)
+        hipLaunchKernelGGL(bias_attn_dbias_kernel, dim3(a.H), dim3(kThreads), 0, st, a.dbias_part,
+                           a.dbias_part ? a.B * a.nq : 0, a.buckets, a.H, a.bias_bf16, p->dbias);
     return check_launch("mb_bias_attn_bwd");
 }

@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
     const int lds = 2 * kStages * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
-    if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD>, lds)) return rc;
+    static Told told;
+    if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD>, lds, told)) return rc;
     hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds, st, a);
     return check_launch("mb_bias_attn_fwd");
 }
@@ -163,28 +164,21 @@ extern "C" int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int 
     return splits > 1 ? (int64_t)B * H * Lq * splits * (hd + 2) * (int64_t)sizeof(float) : 0;
 }
 
-extern "C" int mb_bias_attn_fwd(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
-                                const int64_t* v_st, const void* bias, int bias_dtype, int buckets,
-                                const int32_t* starts, int n_starts, const void* lengths, int lengths_bytes,
-                                const void* q_start, int q_start_bytes, int64_t q_start0, int B, int H, int Hk, int Lq,
-                                int Lk, int hd, float scale, int causal, int dtype, void* o, const int64_t* o_st,
-                                float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int mb_bias_attn_fwd(const mb_bias_attn* p, void* stream) {
     Args a = {};
-    if (const int rc = fill_args("mb_bias_attn_fwd", a, q, q_st, k, k_st, v, v_st, bias, bias_dtype, buckets, starts,
-                                 n_starts, lengths, lengths_bytes, q_start, q_start_bytes, q_start0, B, H, Hk, Lq, Lk,
-                                 hd, scale, causal, dtype))
-        return rc;
-    if (B == 0 || Lq == 0) return MB_OK;
-    MB_REQUIRE(o && o_st, "mb_bias_attn_fwd: null pointer argument");
-    MB_REQUIRE(rows16(o, o_st, dtype), "mb_bias_attn_fwd: o's rows must begin at multiples of 16 bytes");
-    a.out = o, a.out_sb = o_st[0], a.out_sh = o_st[1], a.out_sl = o_st[2];
-    a.lse = lse;
-    const int64_t need = mb_bias_attn_fwd_workspace(B, H, Hk, Lq, Lk, hd, causal);
-    if (need > 0 && (!workspace || workspace_bytes < need))
+    if (const int rc = fill_args("mb_bias_attn_fwd", p, a)) return rc;
+    if (a.B == 0 || a.Lq == 0) return MB_OK;
+    const int hd = (int)p->hd, dtype = (int)p->dtype;
+    MB_REQUIRE(p->o, "mb_bias_attn_fwd: null pointer argument");
+    MB_REQUIRE(rows16(p->o, p->o_st, dtype), "mb_bias_attn_fwd: o's rows must begin at multiples of 16 bytes");
+    a.out = p->o, a.out_sb = p->o_st[0], a.out_sh = p->o_st[1], a.out_sl = p->o_st[2];
+    a.lse = p->lse;
+    const int64_t need = mb_bias_attn_fwd_workspace(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal);
+    if (need > 0 && (!p->workspace || p->workspace_bytes < need))
         return fail(MB_ERR_WORKSPACE, "mb_bias_attn_fwd: workspace of %lld bytes, %lld are needed",
-                    (long long)workspace_bytes, (long long)need);
+                    (long long)p->workspace_bytes, (long long)need);
     hipStream_t st = (hipStream_t)stream;
-    if (const int splits = splits_of(B, H, Hk, Lq, Lk, hd, causal)) return split_launch(a, hd, dtype, splits, workspace, st);
+    if (const int splits = splits_of(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal)) return split_launch(a, hd, dtype, splits, p->workspace, st);
     if (dtype == MB_DTYPE_F32) return hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st);
     return hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st);
 }

@@ -3,15 +3,25 @@
 
 #include "bias_attn.h"
 
+#include <atomic>
+
 namespace mb {
 namespace battn {
 
-// A workgroup may use 160 KiB of LDS; beyond 64 KiB the kernel has to be told.
-inline int allow_lds(const void* kernel, int bytes) {
+// A workgroup may use 160 KiB of LDS; beyond 64 KiB a kernel has to be told, once on each device.
+// `told` is the kernel's own.
+struct Told {
+    std::atomic<int> bytes[64] = {};
+};
+inline int allow_lds(const void* kernel, int bytes, Told& told) {
     if (bytes <= 65536) return MB_OK;
     if (bytes > 163840) return fail(MB_ERR_UNSUPPORTED, "mb_bias_attn: %d bytes of LDS are wanted, 163840 are there", bytes);
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && dev < 64 && told.bytes[dev].load(std::memory_order_relaxed) >= bytes) return MB_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return fail((int)e, "mb_bias_attn: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+    if (dev < 64) told.bytes[dev].store(bytes, std::memory_order_relaxed);
     return MB_OK;
 }
 
@@ -44,55 +54,62 @@ inline int splits_of(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
 }
 int split_launch(const Args& a, int hd, int dtype, int splits, void* part, hipStream_t st);
 
-inline int fill_args(const char* what, Args& a, const void* q, const int64_t* q_st, const void* k, const int64_t* k_st,
-                     const void* v, const int64_t* v_st, const void* bias, int bias_dtype, int buckets,
-                     const int32_t* starts, int n_starts, const void* lengths, int lengths_bytes, const void* q_start,
-                     int q_start_bytes, int64_t q_start0, int B, int H, int Hk, int Lq, int Lk, int hd, float scale,
-                     int causal, int dtype) {
-    MB_REQUIRE(B >= 0 && Lq >= 0 && Lk >= 0 && H >= 1 && Hk >= 1, "%s: B=%d H=%d Hk=%d Lq=%d Lk=%d", what, B, H, Hk, Lq, Lk);
-    MB_REQUIRE(H % Hk == 0, "%s: H=%d is not a multiple of Hk=%d", what, H, Hk);
-    if (hd != 32 && hd != 64 && hd != 128)
-        return fail(MB_ERR_UNSUPPORTED, "%s: head_dim=%d (supported: 32, 64, 128)", what, hd);
-    MB_REQUIRE(dtype == MB_DTYPE_F32 || dtype == MB_DTYPE_BF16, "%s: dtype=%d", what, dtype);
-    MB_REQUIRE(bias_dtype == MB_DTYPE_F32 || bias_dtype == MB_DTYPE_BF16, "%s: bias_dtype=%d", what, bias_dtype);
-    MB_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale=%g", what, (double)scale);
-    MB_REQUIRE(starts && n_starts >= 1 && buckets == (causal ? n_starts : 2 * n_starts),
-               "%s: %d buckets for %d first distances", what, buckets, n_starts);
-    if (n_starts > kMaxStarts)
-        return fail(MB_ERR_UNSUPPORTED, "%s: %d buckets in a direction (at most %d)", what, n_starts, kMaxStarts);
+// Checks what both directions take and fills the kernels' arguments; 0 or an error code.
+inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
+    MB_REQUIRE(p, "%s: null args", what);
+    const int64_t top = 1 << 30;
+    MB_REQUIRE(p->B >= 0 && p->B <= top && p->Lq >= 0 && p->Lq <= top && p->Lk >= 0 && p->Lk <= top && p->H >= 1 && p->H <= top
+                   && p->Hk >= 1 && p->Hk <= top,
+               "%s: B=%lld H=%lld Hk=%lld Lq=%lld Lk=%lld", what, (long long)p->B, (long long)p->H, (long long)p->Hk,
+               (long long)p->Lq, (long long)p->Lk);
+    MB_REQUIRE(p->H % p->Hk == 0, "%s: H=%lld is not a multiple of Hk=%lld", what, (long long)p->H, (long long)p->Hk);
+    if (p->hd != 32 && p->hd != 64 && p->hd != 128)
+        return fail(MB_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 32, 64, 128)", what, (long long)p->hd);
+    MB_REQUIRE(p->dtype == MB_DTYPE_F32 || p->dtype == MB_DTYPE_BF16, "%s: dtype=%lld", what, (long long)p->dtype);
+    MB_REQUIRE(p->bias_dtype == MB_DTYPE_F32 || p->bias_dtype == MB_DTYPE_BF16, "%s: bias_dtype=%lld", what, (long long)p->bias_dtype);
+    MB_REQUIRE(p->scale > 0 && p->scale < INFINITY, "%s: scale=%g", what, p->scale);
+    MB_REQUIRE(p->starts && p->n_starts >= 1 && p->buckets == (p->causal ? p->n_starts : 2 * p->n_starts),
+               "%s: %lld buckets for %lld first distances", what, (long long)p->buckets, (long long)p->n_starts);
+    if (p->n_starts > kMaxStarts)
+        return fail(MB_ERR_UNSUPPORTED, "%s: %lld buckets in a direction (at most %d)", what, (long long)p->n_starts, kMaxStarts);
+    const int32_t* starts = p->starts;
+    const int n_starts = (int)p->n_starts;
     MB_REQUIRE(starts[0] == 0, "%s: the first bucket begins at distance %d, not at 0", what, starts[0]);
     for (int i = 1; i < n_starts; ++i)
         MB_REQUIRE(starts[i] >= starts[i - 1], "%s: first distances must not fall", what);
     if (starts[n_starts - 1] > kMaxReach)
         return fail(MB_ERR_UNSUPPORTED, "%s: the last bucket begins at distance %d (at most %d)", what, starts[n_starts - 1], kMaxReach);
-    MB_REQUIRE((!lengths || lengths_bytes == 4 || lengths_bytes == 8) && (!q_start || q_start_bytes == 4 || q_start_bytes == 8),
+    MB_REQUIRE((!p->lengths || p->lengths_bytes == 4 || p->lengths_bytes == 8)
+                   && (!p->q_start || p->q_start_bytes == 4 || p->q_start_bytes == 8),
                "%s: lengths and q_start hold integers of 4 or 8 bytes", what);
-    MB_REQUIRE(q_start || (q_start0 >= -(1 << 30) && q_start0 <= (1 << 30)), "%s: q_start=%lld", what, (long long)q_start0);
-    MB_REQUIRE(Lq <= (1 << 30) && Lk <= (1 << 30), "%s: Lq=%d Lk=%d", what, Lq, Lk);
-    const int64_t nq = ((int64_t)Lq + kRows - 1) / kRows;
-    MB_REQUIRE((int64_t)B * H * (nq > 0 ? nq : 1) <= 0x7fffffff && (int64_t)B * Hk * (((int64_t)Lk + kRows - 1) / kRows) <= 0x7fffffff,
-               "%s: B=%d H=%d Lq=%d Lk=%d are too many", what, B, H, Lq, Lk);
-    if (B > 0 && Lq > 0) MB_REQUIRE(q && q_st && bias, "%s: null pointer argument", what);
-    if (B > 0 && Lk > 0) MB_REQUIRE(k && k_st && v && v_st, "%s: null pointer argument", what);
-    if (B > 0 && Lq > 0) MB_REQUIRE(rows16(q, q_st, dtype), "%s: q's rows must begin at multiples of 16 bytes", what);
-    if (B > 0 && Lk > 0)
-        MB_REQUIRE(rows16(k, k_st, dtype) && rows16(v, v_st, dtype), "%s: k's and v's rows must begin at multiples of 16 bytes", what);
-    // offsets within a tile of 64 rows have 32 bits
-    const int64_t most = (int64_t)(1 << 24) / (dtype == MB_DTYPE_F32 ? 4 : 2);
-    if (B > 0 && Lq > 0) MB_REQUIRE(q_st[2] >= 0 && q_st[2] <= most, "%s: q's rows are %lld elements apart", what, (long long)q_st[2]);
-    if (B > 0 && Lk > 0)
-        MB_REQUIRE(k_st[2] >= 0 && k_st[2] <= most && v_st[2] >= 0 && v_st[2] <= most,
-                   "%s: k's and v's rows are %lld and %lld elements apart", what, (long long)k_st[2], (long long)v_st[2]);
-    a.q = q, a.k = k, a.v = v, a.bias = bias;
-    if (q_st) a.q_sb = q_st[0], a.q_sh = q_st[1], a.q_sl = q_st[2];
-    if (k_st) a.k_sb = k_st[0], a.k_sh = k_st[1], a.k_sl = k_st[2];
-    if (v_st) a.v_sb = v_st[0], a.v_sh = v_st[1], a.v_sl = v_st[2];
-    a.lengths = lengths, a.lengths_bytes = lengths_bytes;
-    a.start = q_start, a.start_bytes = q_start_bytes, a.start0 = (int)q_start0;
-    a.B = B, a.H = H, a.Hk = Hk, a.Lq = Lq, a.Lk = Lk, a.nq = (int)nq;
-    a.causal = causal != 0, a.bias_bf16 = bias_dtype == MB_DTYPE_BF16, a.buckets = buckets, a.n_starts = n_starts;
+    MB_REQUIRE(p->q_start || (p->q_start0 >= -top && p->q_start0 <= top), "%s: q_start=%lld", what, (long long)p->q_start0);
+    const int64_t nq = (p->Lq + kRows - 1) / kRows, nk = (p->Lk + kRows - 1) / kRows;
+    MB_REQUIRE((double)p->B * p->H * (nq > 0 ? nq : 1) <= 0x7fffffff && (double)p->B * p->Hk * nk <= 0x7fffffff,
+               "%s: B=%lld H=%lld Lq=%lld Lk=%lld are too many", what, (long long)p->B, (long long)p->H, (long long)p->Lq,
+               (long long)p->Lk);
+    const int dtype = (int)p->dtype;
+    const int64_t most = (int64_t)(1 << 24) / (dtype == MB_DTYPE_F32 ? 4 : 2);   // offsets within a tile have 32 bits
+    if (p->B > 0 && p->Lq > 0) {
+        MB_REQUIRE(p->q && p->bias, "%s: null pointer argument", what);
+        MB_REQUIRE(rows16(p->q, p->q_st, dtype), "%s: q's rows must begin at multiples of 16 bytes", what);
+        MB_REQUIRE(p->q_st[2] >= 0 && p->q_st[2] <= most, "%s: q's rows are %lld elements apart", what, (long long)p->q_st[2]);
+    }
+    if (p->B > 0 && p->Lk > 0) {
+        MB_REQUIRE(p->k && p->v, "%s: null pointer argument", what);
+        MB_REQUIRE(rows16(p->k, p->k_st, dtype) && rows16(p->v, p->v_st, dtype), "%s: k's and v's rows must begin at multiples of 16 bytes", what);
+        MB_REQUIRE(p->k_st[2] >= 0 && p->k_st[2] <= most && p->v_st[2] >= 0 && p->v_st[2] <= most,
+                   "%s: k's and v's rows are %lld and %lld elements apart", what, (long long)p->k_st[2], (long long)p->v_st[2]);
+    }
+    a.q = p->q, a.k = p->k, a.v = p->v, a.bias = p->bias;
+    a.q_sb = p->q_st[0], a.q_sh = p->q_st[1], a.q_sl = p->q_st[2];
+    a.k_sb = p->k_st[0], a.k_sh = p->k_st[1], a.k_sl = p->k_st[2];
+    a.v_sb = p->v_st[0], a.v_sh = p->v_st[1], a.v_sl = p->v_st[2];
+    a.lengths = p->lengths, a.lengths_bytes = (int)p->lengths_bytes;
+    a.start = p->q_start, a.start_bytes = (int)p->q_start_bytes, a.start0 = p->q_start ? 0 : (int)p->q_start0;
+    a.B = (int)p->B, a.H = (int)p->H, a.Hk = (int)p->Hk, a.Lq = (int)p->Lq, a.Lk = (int)p->Lk, a.nq = (int)nq;
+    a.causal = p->causal != 0, a.bias_bf16 = p->bias_dtype == MB_DTYPE_BF16, a.buckets = (int)p->buckets, a.n_starts = n_starts;
     a.reach = starts[n_starts - 1];
-    a.scale = scale;
+    a.scale = (float)p->scale;
     for (int i = 0; i < n_starts; ++i) a.starts[i] = (int16_t)starts[i];
     return MB_OK;
 }

@@ -259,7 +259,8 @@ int launch(const Args& a, int splits, float* part, hipStream_t st) {
     const int corner = std::max(HD * 33 * 4, 32 * (HD * (int)sizeof(T) + 16));
     const Reach r(a);
     const int lds = 4 * corner + a.buckets * G * 4 + (r.hi - r.lo + 1);
-    if (const int rc = allow_lds((const void*)bias_attn_split_kernel<T, HD>, lds)) return rc;
+    static Told told;
+    if (const int rc = allow_lds((const void*)bias_attn_split_kernel<T, HD>, lds, told)) return rc;
     hipLaunchKernelGGL((bias_attn_split_kernel<T, HD>), dim3((unsigned)(a.B * a.Hk * tiles * splits)), dim3(kThreads), lds, st,
                        a, splits, part);
     if (splits > 1) {

@@ -248,27 +248,35 @@ int64_t bwd_blocks(int64_t tokens) {
     return std::min<int64_t>((tokens + kQkWaves - 1) / kQkWaves, kQkBwdBlocks);
 }
 
-bool aligned16(const void* p, int64_t a, int64_t b, int64_t c, int size) {
-    return (((uintptr_t)p | (uint64_t)(a * size) | (uint64_t)(b * size) | (uint64_t)(c * size)) & 15) == 0;
+bool aligned16(const void* p, const int64_t* st, int size) {
+    return (((uintptr_t)p | (uint64_t)(st[0] * size) | (uint64_t)(st[1] * size) | (uint64_t)(st[2] * size)) & 15) == 0;
 }
 
-// The checks that both directions share; 0 or an error code.
-int check(const char* what, const QkArgs& a, int B, int hd, int dtype) {
-    MB_REQUIRE(B >= 0 && a.L >= 0 && a.H >= 1 && a.Hk >= 1, "%s: B=%d L=%d H=%d Hk=%d", what, B, a.L, a.H, a.Hk);
-    if (hd != 32 && hd != 64 && hd != 128)
-        return fail(MB_ERR_UNSUPPORTED, "%s: head_dim=%d (supported: 32, 64, 128)", what, hd);
-    MB_REQUIRE(dtype == MB_DTYPE_F32 || dtype == MB_DTYPE_BF16, "%s: dtype=%d", what, dtype);
-    MB_REQUIRE(!a.start || a.start_bytes == 4 || a.start_bytes == 8, "%s: start_bytes=%d (4 or 8)", what, a.start_bytes);
-    MB_REQUIRE(a.table_rows >= 0, "%s: table_rows=%lld", what, (long long)a.table_rows);
-    if (!a.start)
-        MB_REQUIRE(a.start0 >= 0 && a.start0 <= a.table_rows - a.L, "%s: positions %lld to %lld pass the table's %lld rows",
-                   what, (long long)a.start0, (long long)a.start0 + a.L, (long long)a.table_rows);
+// Checks what both directions take and fills the kernels' arguments; 0 or an error code.
+int fill(const char* what, const mb_qk_norm_rotary* p, QkArgs& a) {
+    MB_REQUIRE(p, "%s: null args", what);
+    const int64_t top = 0x7fffffff;
+    MB_REQUIRE(p->B >= 0 && p->B <= top && p->L >= 0 && p->L <= top && p->H >= 1 && p->H <= top / 2 && p->Hk >= 1 && p->Hk <= top / 2,
+               "%s: B=%lld L=%lld H=%lld Hk=%lld", what, (long long)p->B, (long long)p->L, (long long)p->H, (long long)p->Hk);
+    if (p->hd != 32 && p->hd != 64 && p->hd != 128)
+        return fail(MB_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 32, 64, 128)", what, (long long)p->hd);
+    MB_REQUIRE(p->dtype == MB_DTYPE_F32 || p->dtype == MB_DTYPE_BF16, "%s: dtype=%lld", what, (long long)p->dtype);
+    MB_REQUIRE(!p->start || p->start_bytes == 4 || p->start_bytes == 8, "%s: start_bytes=%lld (4 or 8)", what, (long long)p->start_bytes);
+    MB_REQUIRE(p->table_rows >= 0, "%s: table_rows=%lld", what, (long long)p->table_rows);
+    if (!p->start)
+        MB_REQUIRE(p->start0 >= 0 && p->start0 <= p->table_rows - p->L, "%s: positions %lld to %lld pass the table's %lld rows",
+                   what, (long long)p->start0, (long long)(p->start0 + p->L), (long long)p->table_rows);
+    a.tokens = p->B * p->L;
+    MB_REQUIRE((a.tokens + kQkWaves - 1) / kQkWaves <= top, "%s: %lld tokens are too many", what, (long long)a.tokens);
     if (a.tokens == 0) return MB_OK;
-    MB_REQUIRE(a.q && a.k && a.wq && a.wk && a.cos && a.sin && a.q_out && a.k_out, "%s: null pointer argument", what);
-    const int size = dtype == MB_DTYPE_F32 ? 4 : 2;
-    MB_REQUIRE(aligned16(a.q, a.q_sb, a.q_sl, a.q_sh, size) && aligned16(a.k, a.k_sb, a.k_sl, a.k_sh, size)
-                   && aligned16(a.q_out, 0, 0, 0, size) && aligned16(a.k_out, 0, 0, 0, size),
-               "%s: rows must begin at multiples of 16 bytes", what);
+    MB_REQUIRE(p->q && p->k && p->wq && p->wk && p->cos && p->sin, "%s: null pointer argument", what);
+    const int size = p->dtype == MB_DTYPE_F32 ? 4 : 2;
+    MB_REQUIRE(aligned16(p->q, p->q_st, size) && aligned16(p->k, p->k_st, size), "%s: rows must begin at multiples of 16 bytes", what);
+    a.q = p->q, a.q_sb = p->q_st[0], a.q_sl = p->q_st[1], a.q_sh = p->q_st[2];
+    a.k = p->k, a.k_sb = p->k_st[0], a.k_sl = p->k_st[1], a.k_sh = p->k_st[2];
+    a.wq = p->wq, a.wk = p->wk, a.cos = p->cos, a.sin = p->sin, a.table_rows = p->table_rows;
+    a.start = p->start, a.start_bytes = (int)p->start_bytes, a.start0 = p->start0;
+    a.L = (int)p->L, a.H = (int)p->H, a.Hk = (int)p->Hk, a.eps = (float)p->eps;
     return MB_OK;
 }
 
@@ -293,23 +301,16 @@ void launch_bwd(int hd, dim3 grid, hipStream_t st, const QkArgs& a) {
 
 using namespace mb;
 
-extern "C" int mb_qk_norm_rotary_fwd(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void* k,
-                                     int64_t k_sb, int64_t k_sl, int64_t k_sh, const float* wq, const float* wk,
-                                     const float* cos, const float* sin, int64_t table_rows, const void* start,
-                                     int start_bytes, int64_t start0, int B, int L, int H, int Hk, int hd, float eps,
-                                     int dtype, void* q_out, void* k_out, void* stream) {
+extern "C" int mb_qk_norm_rotary_fwd(const mb_qk_norm_rotary* p, void* stream) {
     QkArgs a = {};
-    a.q = q, a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh;
-    a.k = k, a.k_sb = k_sb, a.k_sl = k_sl, a.k_sh = k_sh;
-    a.wq = wq, a.wk = wk, a.cos = cos, a.sin = sin, a.table_rows = table_rows;
-    a.start = start, a.start_bytes = start_bytes, a.start0 = start0;
-    a.tokens = (int64_t)B * L, a.L = L, a.H = H, a.Hk = Hk, a.eps = eps, a.q_out = q_out, a.k_out = k_out;
-    if (const int rc = check("mb_qk_norm_rotary_fwd", a, B, hd, dtype)) return rc;
+    if (const int rc = fill("mb_qk_norm_rotary_fwd", p, a)) return rc;
     if (a.tokens == 0) return MB_OK;
-    const int64_t blocks = (a.tokens + kQkWaves - 1) / kQkWaves;
-    MB_REQUIRE(blocks <= 0x7fffffff, "mb_qk_norm_rotary_fwd: %lld tokens are too many", (long long)a.tokens);
-    if (dtype == MB_DTYPE_F32) launch_fwd<float>(hd, dim3((unsigned)blocks), (hipStream_t)stream, a);
-    else launch_fwd<__bf16>(hd, dim3((unsigned)blocks), (hipStream_t)stream, a);
+    MB_REQUIRE(p->q_out && p->k_out, "mb_qk_norm_rotary_fwd: null pointer argument");
+    MB_REQUIRE((((uintptr_t)p->q_out | (uintptr_t)p->k_out) & 15) == 0, "mb_qk_norm_rotary_fwd: rows must begin at multiples of 16 bytes");
+    a.q_out = p->q_out, a.k_out = p->k_out;
+    const dim3 grid((unsigned)((a.tokens + kQkWaves - 1) / kQkWaves));
+    if (p->dtype == MB_DTYPE_F32) launch_fwd<float>((int)p->hd, grid, (hipStream_t)stream, a);
+    else launch_fwd<__bf16>((int)p->hd, grid, (hipStream_t)stream, a);
     return check_launch("mb_qk_norm_rotary_fwd");
 }
 
@@ -318,38 +319,30 @@ extern "C" int64_t mb_qk_norm_rotary_bwd_workspace(int B, int L, int hd) {
     return bwd_blocks((int64_t)B * L) * 2 * hd * (int64_t)sizeof(float);
 }
 
-extern "C" int mb_qk_norm_rotary_bwd(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void* k,
-                                     int64_t k_sb, int64_t k_sl, int64_t k_sh, const void* dq_out, int64_t dq_sb,
-                                     int64_t dq_sl, int64_t dq_sh, const void* dk_out, int64_t dk_sb, int64_t dk_sl,
-                                     int64_t dk_sh, const float* wq, const float* wk, const float* cos,
-                                     const float* sin, int64_t table_rows, const void* start, int start_bytes,
-                                     int64_t start0, int B, int L, int H, int Hk, int hd, float eps, int dtype,
-                                     void* dq, void* dk, float* dwq, float* dwk, void* workspace,
-                                     int64_t workspace_bytes, void* stream) {
+extern "C" int mb_qk_norm_rotary_bwd(const mb_qk_norm_rotary* p, void* stream) {
     QkArgs a = {};
-    a.q = q, a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh;
-    a.k = k, a.k_sb = k_sb, a.k_sl = k_sl, a.k_sh = k_sh;
-    a.dqo = dq_out, a.dq_sb = dq_sb, a.dq_sl = dq_sl, a.dq_sh = dq_sh;
-    a.dko = dk_out, a.dk_sb = dk_sb, a.dk_sl = dk_sl, a.dk_sh = dk_sh;
-    a.wq = wq, a.wk = wk, a.cos = cos, a.sin = sin, a.table_rows = table_rows;
-    a.start = start, a.start_bytes = start_bytes, a.start0 = start0;
-    a.tokens = (int64_t)B * L, a.L = L, a.H = H, a.Hk = Hk, a.eps = eps, a.q_out = dq, a.k_out = dk;
-    a.part = (float*)workspace;
-    if (const int rc = check("mb_qk_norm_rotary_bwd", a, B, hd, dtype)) return rc;
-    MB_REQUIRE(dwq && dwk, "mb_qk_norm_rotary_bwd: null pointer argument");
+    if (const int rc = fill("mb_qk_norm_rotary_bwd", p, a)) return rc;
+    MB_REQUIRE(p->dwq && p->dwk, "mb_qk_norm_rotary_bwd: null pointer argument");
     hipStream_t st = (hipStream_t)stream;
+    const int hd = (int)p->hd;
     const int64_t blocks = bwd_blocks(a.tokens);
     if (a.tokens > 0) {
-        const int size = dtype == MB_DTYPE_F32 ? 4 : 2;
-        MB_REQUIRE(dq_out && dk_out, "mb_qk_norm_rotary_bwd: null pointer argument");
-        MB_REQUIRE(aligned16(dq_out, dq_sb, dq_sl, dq_sh, size) && aligned16(dk_out, dk_sb, dk_sl, dk_sh, size),
+        const int size = p->dtype == MB_DTYPE_F32 ? 4 : 2;
+        MB_REQUIRE(p->dq_out && p->dk_out && p->dq && p->dk, "mb_qk_norm_rotary_bwd: null pointer argument");
+        MB_REQUIRE(aligned16(p->dq_out, p->dq_st, size) && aligned16(p->dk_out, p->dk_st, size)
+                       && (((uintptr_t)p->dq | (uintptr_t)p->dk) & 15) == 0,
                    "mb_qk_norm_rotary_bwd: rows must begin at multiples of 16 bytes");
-        if (!workspace || workspace_bytes < mb_qk_norm_rotary_bwd_workspace(B, L, hd))
+        const int64_t need = mb_qk_norm_rotary_bwd_workspace((int)p->B, (int)p->L, hd);
+        if (!p->workspace || p->workspace_bytes < need)
             return fail(MB_ERR_WORKSPACE, "mb_qk_norm_rotary_bwd: workspace of %lld bytes, %lld are needed",
-                        (long long)workspace_bytes, (long long)mb_qk_norm_rotary_bwd_workspace(B, L, hd));
-        if (dtype == MB_DTYPE_F32) launch_bwd<float>(hd, dim3((unsigned)blocks), st, a);
+                        (long long)p->workspace_bytes, (long long)need);
+        a.dqo = p->dq_out, a.dq_sb = p->dq_st[0], a.dq_sl = p->dq_st[1], a.dq_sh = p->dq_st[2];
+        a.dko = p->dk_out, a.dk_sb = p->dk_st[0], a.dk_sl = p->dk_st[1], a.dk_sh = p->dk_st[2];
+        a.q_out = p->dq, a.k_out = p->dk, a.part = (float*)p->workspace;
+        if (p->dtype == MB_DTYPE_F32) launch_bwd<float>(hd, dim3((unsigned)blocks), st, a);
         else launch_bwd<__bf16>(hd, dim3((unsigned)blocks), st, a);
     }
-    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2 * hd / kDwCols), dim3(kDwCols * kDwStrips), 0, st, a.part, (int)blocks, hd, dwq, dwk);
+    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2 * hd / kDwCols), dim3(kDwCols * kDwStrips), 0, st, a.part, (int)blocks, hd,
+                       p->dwq, p->dwk);
     return check_launch("mb_qk_norm_rotary_bwd");
 }

@@ -12,6 +12,7 @@ weights.  One launch forward, two backward; the weight gradients are summed in a
 CPU tensors raise NotImplementedError: there is no CPU path.  Both directions are registered
 as torch ops (mathbrain::qk_norm_rotary_fwd / _bwd) for tracing.
 """
+import struct
 from typing import Optional
 
 import torch
@@ -19,6 +20,9 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.MB_DTYPE_F32, torch.bfloat16: _lib.MB_DTYPE_BF16}
+# mb_qk_norm_rotary (include/mathbrain_hip.h): the forward's fields, then the backward's
+_ARGS = struct.Struct("2P6q4PqP2q5qqd2P" + "2P6q4PPq")
+_NO_BACKWARD = (0,) * 14
 
 
 def _rows16(x):
@@ -33,10 +37,12 @@ def _weight(w):
     return w if w.dtype is torch.float32 and w.stride(0) == 1 else w.float().contiguous()
 
 
-def _start_args(start_rows, start):
-    if start_rows is None:
-        return None, 4, start
-    return start_rows.data_ptr(), start_rows.element_size(), 0
+def _inputs(q, k, wq, wk, cos, sin, eps, start_rows, start):
+    """The struct's fields up to eps."""
+    B, L, H, hd = q.shape
+    return (q.data_ptr(), k.data_ptr(), *q.stride()[:3], *k.stride()[:3], wq.data_ptr(), wk.data_ptr(), cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], 0 if start_rows is None else start_rows.data_ptr(),
+            4 if start_rows is None else start_rows.element_size(), start, B, L, H, k.shape[2], hd, _DTYPES[q.dtype], eps)
 
 
 def _fwd_fake(q, k, q_weight, k_weight, cos, sin, eps, start_rows, start):
@@ -53,10 +59,9 @@ def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     q, k, wq, wk = _rows16(q), _rows16(k), _weight(q_weight), _weight(k_weight)
     qo = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
     ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    at, size, first = _start_args(start_rows, start)
-    _lib.call_on(dev, "mb_qk_norm_rotary_fwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
-                 wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first,
-                 B, L, H, k.shape[2], hd, eps, _DTYPES[q.dtype], qo.data_ptr(), ko.data_ptr())
+    _lib.call_on(dev, "mb_qk_norm_rotary_fwd",
+                 _ARGS.pack(*_inputs(q, k, wq, wk, cos, sin, eps, start_rows, start), qo.data_ptr(), ko.data_ptr(),
+                            *_NO_BACKWARD))
     return qo, ko
 
 
@@ -80,13 +85,12 @@ def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
     dwq = torch.empty(hd, dtype=torch.float32, device=dev)
     dwk = torch.empty(hd, dtype=torch.float32, device=dev)
-    ws = torch.empty(_lib.lib().mb_qk_norm_rotary_bwd_workspace(B, L, hd), dtype=torch.uint8, device=dev)
-    at, size, first = _start_args(start_rows, start)
-    _lib.call_on(dev, "mb_qk_norm_rotary_bwd", q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
-                 gq.data_ptr(), *gq.stride()[:3], gk.data_ptr(), *gk.stride()[:3], wq.data_ptr(),
-                 wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at, size, first, B, L, H,
-                 k.shape[2], hd, eps, _DTYPES[q.dtype], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
-                 dwk.data_ptr(), ws.data_ptr(), ws.numel())
+    nbytes = _lib.workspace_bytes("mb_qk_norm_rotary_bwd_workspace", B, L, hd)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _lib.call_on(dev, "mb_qk_norm_rotary_bwd",
+                 _ARGS.pack(*_inputs(q, k, wq, wk, cos, sin, eps, start_rows, start), 0, 0, gq.data_ptr(), gk.data_ptr(),
+                            *gq.stride()[:3], *gk.stride()[:3], dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
+                            dwk.data_ptr(), ws.data_ptr(), nbytes))
     if q_weight.dtype is not torch.float32 or k_weight.dtype is not torch.float32:
         dwq, dwk = dwq.to(q_weight.dtype), dwk.to(k_weight.dtype)
     return dq, dk, dwq, dwk
@@ -112,10 +116,14 @@ class QKNormRotaryFunction(torch.autograd.Function):
 def _check(q, k, q_weight, k_weight, cos, sin, start):
     what = "qk_norm_rotary"
     rows = start if torch.is_tensor(start) else None
-    _lib.require_gpu(q, k, q_weight, k_weight, cos, sin, rows, what=what)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} are not [B, L, H, hd] and [B, L, Hk, hd]")
-    hd = q.shape[3]
+    at = q.get_device()
+    if (at < 0 or k.get_device() != at or q_weight.get_device() != at or k_weight.get_device() != at
+            or cos.get_device() != at or sin.get_device() != at or (rows is not None and rows.get_device() != at)):
+        _lib.require_gpu(q, k, q_weight, k_weight, cos, sin, rows, what=what)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[:2] != ks[:2] or qs[3] != ks[3]:
+        raise ValueError(f"{what}: q {tuple(qs)} and k {tuple(ks)} are not [B, L, H, hd] and [B, L, Hk, hd]")
+    hd = qs[3]
     if q.dtype not in _DTYPES or k.dtype != q.dtype:
         raise ValueError(f"{what}: q {q.dtype} and k {k.dtype} (supported: both float32 or both bfloat16)")
     if q_weight.shape != (hd,) or k_weight.shape != (hd,):
@@ -124,9 +132,9 @@ def _check(q, k, q_weight, k_weight, cos, sin, start):
         raise ValueError(f"{what}: tables {tuple(cos.shape)}, {tuple(sin.shape)} are not [positions, {hd // 2}]")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"{what}: the tables must be contiguous float32")
-    if rows is not None and (rows.shape != (q.shape[0],) or rows.dtype not in (torch.int32, torch.int64)):
+    if rows is not None and (rows.shape != qs[:1] or rows.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"{what}: start {tuple(rows.shape)} {rows.dtype} is not one int32 or int64 for each of "
-                         f"{q.shape[0]} rows")
+                         f"{qs[0]} rows")
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, eps=1e-6, start=0):

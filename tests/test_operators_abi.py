@@ -1,5 +1,5 @@
-"""The argument checks of the query/key norm's and the gradient clipping's entry points: they run on
-the host before anything is launched (no GPU needed)."""
+"""The argument checks of the query/key norm's, the attention's with a bucket bias and the gradient
+clipping's entry points: they run on the host before anything is launched (no GPU needed)."""
 import ctypes
 
 import pytest
@@ -20,42 +20,123 @@ def message(lib):
 P = 1 << 20
 
 
-def qk_fwd(**bad):
-    a = dict(q=P, q_sb=8192, q_sl=512, q_sh=64, k=P, k_sb=8192, k_sl=512, k_sh=64, wq=P, wk=P, cos=P, sin=P,
-             table_rows=64, start=None, start_bytes=4, start0=0, B=2, L=16, H=8, Hk=8, hd=64, eps=1e-6, dtype=0,
-             q_out=P, k_out=P) | bad
-    return tuple(a.values()) + (None,)
+def qk(**fields):
+    """The packed struct with some fields changed: (name, index) as in the header."""
+    from mathbrain.qk_norm import _ARGS
+    names = ("q k q0 q1 q2 k0 k1 k2 wq wk cos sin table_rows start start_bytes start0 B L H Hk hd dtype eps q_out k_out "
+             "dq_out dk_out g0 g1 g2 h0 h1 h2 dq dk dwq dwk workspace workspace_bytes").split()
+    a = dict.fromkeys(names, P) | dict(q0=8192, q1=512, q2=64, k0=8192, k1=512, k2=64, g0=8192, g1=512, g2=64, h0=8192,
+                                       h1=512, h2=64, table_rows=64, start=0, start_bytes=4, start0=0, B=2, L=16, H=8,
+                                       Hk=8, hd=64, dtype=0, eps=1e-6, workspace_bytes=1 << 30)
+    assert set(fields) <= set(names)
+    return _ARGS.pack(*(a | fields).values())
 
 
-@pytest.mark.parametrize("bad,said", [
-    (dict(hd=48), "head_dim=48"), (dict(dtype=2), "dtype=2"), (dict(q=None), "null"), (dict(sin=None), "null"),
-    (dict(B=-1), "B=-1"), (dict(H=0), "H=0"), (dict(start=P, start_bytes=2), "start_bytes=2"),
-    (dict(start0=49), "pass the table"), (dict(start0=-1), "pass the table"), (dict(table_rows=15), "pass the table"),
-    (dict(q=P + 4), "16 bytes"), (dict(k_sl=513), "16 bytes"), (dict(k_out=P + 8), "16 bytes")])
-def test_qk_norm_forward_refusals(lib, bad, said):
-    assert lib.mb_qk_norm_rotary_fwd(*qk_fwd(**bad)) < 0
-    assert said in message(lib)
+REFUSED_QK = [
+    (dict(hd=48), "head_dim=48"), (dict(dtype=2), "dtype=2"), (dict(q=0), "null"), (dict(sin=0), "null"),
+    (dict(B=-1), "B=-1"), (dict(B=1 << 40), "B=1099511627776"), (dict(H=0), "H=0"),
+    (dict(start=P, start_bytes=2), "start_bytes=2"), (dict(start0=49), "pass the table"),
+    (dict(start0=-1), "pass the table"), (dict(table_rows=15), "pass the table"), (dict(q=P + 4), "16 bytes"),
+    (dict(k1=513), "16 bytes")]
+
+
+@pytest.mark.parametrize("bad,said", REFUSED_QK)
+def test_qk_norm_refusals(lib, bad, said):
+    for name in ("mb_qk_norm_rotary_fwd", "mb_qk_norm_rotary_bwd"):
+        assert getattr(lib, name)(qk(**bad), None) < 0
+        assert said in message(lib) and name in message(lib)
+
+
+def test_qk_norm_refusals_of_one_direction(lib):
+    from mathbrain import _lib
+    assert lib.mb_qk_norm_rotary_fwd(None, None) < 0 and "null args" in message(lib)
+    for bad, said in ((dict(k_out=0), "null"), (dict(k_out=P + 8), "16 bytes")):
+        assert lib.mb_qk_norm_rotary_fwd(qk(**bad), None) < 0 and said in message(lib)
+    for bad, rc, said in ((dict(dq_out=0), -1, "null"), (dict(dq=0), -1, "null"), (dict(g1=513), -1, "16 bytes"),
+                          (dict(dwq=0), -1, "null"), (dict(workspace=0), _lib.MB_ERR_WORKSPACE, "workspace"),
+                          (dict(workspace_bytes=8), _lib.MB_ERR_WORKSPACE, "workspace of 8 bytes")):
+        assert lib.mb_qk_norm_rotary_bwd(qk(**bad), None) == rc and said in message(lib)
 
 
 def test_qk_norm_empty_batches_launch_nothing(lib):
-    assert lib.mb_qk_norm_rotary_fwd(*qk_fwd(B=0)) == 0
-    assert lib.mb_qk_norm_rotary_fwd(*qk_fwd(L=0, q=None)) == 0
+    assert lib.mb_qk_norm_rotary_fwd(qk(B=0), None) == 0
+    assert lib.mb_qk_norm_rotary_fwd(qk(L=0, q=0), None) == 0
     assert lib.mb_qk_norm_rotary_bwd_workspace(0, 5, 64) == 0
     assert lib.mb_qk_norm_rotary_bwd_workspace(1, 1, 64) == 2 * 64 * 4
     assert lib.mb_qk_norm_rotary_bwd_workspace(64, 4096, 128) == 1024 * 2 * 128 * 4
 
 
-def test_qk_norm_backward_refusals(lib):
-    f = qk_fwd()
-    strides = (8192, 512, 64)
+def attn(first=(0, 1, 5), **fields):
+    from mathbrain.bias_attention import _ARGS
+    names = ("q k v q0 q1 q2 k0 k1 k2 v0 v1 v2 bias starts buckets n_starts lengths lengths_bytes q_start q_start_bytes "
+             "q_start0 B H Hk Lq Lk hd causal dtype bias_dtype scale o o0 o1 o2 lse d_o g0 g1 g2 dq dk dv dq0 dq1 dq2 dk0 "
+             "dk1 dk2 dv0 dv1 dv2 dbias workspace workspace_bytes").split()
+    attn.keep = (ctypes.c_int32 * len(first))(*first)
+    a = dict.fromkeys(names, P)
+    for n in names:
+        if n[-1] in "012" and n[:-1] in ("q", "k", "v", "o", "g", "dq", "dk", "dv"):
+            a[n] = (64 * 8 * 100, 64, 512)[int(n[-1])]
+    a |= dict(starts=ctypes.addressof(attn.keep), buckets=len(first), n_starts=len(first), lengths=0, lengths_bytes=4,
+              q_start=0, q_start_bytes=4, q_start0=0, B=2, H=8, Hk=8, Lq=100, Lk=100, hd=64, causal=1, dtype=1, bias_dtype=0,
+              scale=0.125, workspace_bytes=1 << 40)
+    assert set(fields) <= set(names)
+    return _ARGS.pack(*(a | fields).values())
 
-    def call(dq=P, ws=P, nbytes=1 << 30, dw=P):
-        return lib.mb_qk_norm_rotary_bwd(*f[:8], dq, *strides, P, *strides, *f[8:23], P, P, dw, P, ws, nbytes, None)
+
+@pytest.mark.parametrize("bad,said", [
+    (dict(hd=96), "head_dim=96"), (dict(dtype=3), "dtype=3"), (dict(bias_dtype=-1), "bias_dtype=-1"), (dict(q=0), "null"),
+    (dict(v=0), "null"), (dict(bias=0), "null"), (dict(Lq=-1), "Lq=-1"), (dict(Lk=1 << 31), "Lk=2147483648"),
+    (dict(Hk=3), "multiple of Hk=3"), (dict(Hk=0), "Hk=0"), (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(starts=0), "first distances"), (dict(buckets=4), "4 buckets for 3"), (dict(causal=0), "3 buckets for 3"),
+    (dict(lengths=P, lengths_bytes=2), "4 or 8 bytes"), (dict(q_start=P, q_start_bytes=1), "4 or 8 bytes"),
+    (dict(q_start0=1 << 31), "q_start=2147483648"), (dict(q=P + 2), "16 bytes"), (dict(k2=513), "16 bytes"),
+    (dict(v2=-512), "elements apart"), (dict(q2=1 << 24), "elements apart"), (dict(B=1 << 20, H=1 << 12), "too many")])
+def test_bias_attention_refusals(lib, bad, said):
+    for name in ("mb_bias_attn_fwd", "mb_bias_attn_bwd"):
+        assert getattr(lib, name)(attn(**bad), None) < 0
+        assert said in message(lib) and name in message(lib)
+
+
+@pytest.mark.parametrize("starts,said", [((1, 2), "distance 1, not at 0"), ((0, 5, 4), "must not fall"),
+                                         ((0, 1025), "distance 1025"), (tuple(range(129)), "129 buckets")])
+def test_bias_attention_bucket_refusals(lib, starts, said):
+    assert lib.mb_bias_attn_fwd(attn(starts), None) < 0 and said in message(lib)
+
+
+def test_bias_attention_refusals_of_one_direction(lib):
     from mathbrain import _lib
-    for args, rc, said in ((dict(dq=None), -1, "null"), (dict(dq=P + 4), -1, "16 bytes"), (dict(dw=None), -1, "null"),
-                           (dict(ws=None), _lib.MB_ERR_WORKSPACE, "workspace"),
-                           (dict(nbytes=8), _lib.MB_ERR_WORKSPACE, "workspace of 8 bytes")):
-        assert call(**args) == rc and said in message(lib)
+    assert lib.mb_bias_attn_fwd(None, None) < 0 and "null args" in message(lib)
+    for bad, rc, said in ((dict(o=0), -1, "null"), (dict(o=P + 8), -1, "16 bytes"),
+                          (dict(Lq=1, Lk=4096, workspace=0), _lib.MB_ERR_WORKSPACE, "workspace"),
+                          (dict(Lq=1, Lk=4096, workspace_bytes=64), _lib.MB_ERR_WORKSPACE, "workspace of 64 bytes")):
+        assert lib.mb_bias_attn_fwd(attn(**bad), None) == rc and said in message(lib)
+    for bad, rc, said in ((dict(d_o=0), -1, "null"), (dict(lse=0), -1, "null"), (dict(dk=0), -1, "null"),
+                          (dict(g2=513), -1, "16 bytes"), (dict(g2=1 << 24), -1, "elements apart"), (dict(dv=P + 4), -1, "16 bytes"),
+                          (dict(workspace=0), _lib.MB_ERR_WORKSPACE, "workspace"),
+                          (dict(workspace_bytes=64), _lib.MB_ERR_WORKSPACE, "workspace of 64 bytes")):
+        assert lib.mb_bias_attn_bwd(attn(**bad), None) == rc and said in message(lib)
+
+
+def test_bias_attention_workspaces(lib):
+    assert lib.mb_bias_attn_fwd(attn(B=0), None) == 0 and lib.mb_bias_attn_fwd(attn(Lq=0), None) == 0
+    size = lib.mb_bias_attn_fwd_workspace
+    assert size(56, 8, 8, 512, 512, 64, 1) == 0                    # a grid that fills the device
+    assert size(16, 8, 8, 1, 4096, 64, 1) > 0 and size(16, 8, 8, 1, 100, 64, 1) == 0
+    assert size(0, 8, 8, 1, 4096, 64, 1) == 0 and size(1, 8, 3, 1, 4096, 64, 1) == 0
+    assert size(1 << 30, 1 << 30, 1, 1 << 30, 1 << 30, 64, 1) == 0  # no overflow on the way to "no"
+    assert lib.mb_bias_attn_bwd_workspace(2, 8, 100, 32) == (2 * 2 * 8 * 100 + 8 * 2 * 32) * 4
+    assert lib.mb_bias_attn_bwd_workspace(2, 8, 0, 32) == 0
+
+
+def test_bucket_starts():
+    from mathbrain.bias_attention import bucket_starts
+    assert bucket_starts(1, 5) == (0,) and bucket_starts(2, 100) == (0, 1) and bucket_starts(3, 100) == (0, 1, 10)
+    assert bucket_starts(32, 128)[:17] == tuple(range(17)) and bucket_starts(32, 128)[-1] == 113
+    # the border of 4 buckets up to 16 lies at sqrt(2 * 16) = 5.66, that of 4 up to 18 at 6 itself
+    assert bucket_starts(4, 16) == (0, 1, 2, 6) and bucket_starts(4, 18) == (0, 1, 2, 6) and bucket_starts(4, 19)[-1] == 7
+    for n, reach in ((16, 9), (31, 200), (128, 1024)):
+        starts = bucket_starts(n, reach)
+        assert len(starts) == n and list(starts) == sorted(starts) and starts[-1] <= reach
 
 
 def clip(lib, src, dst, n, codes=None, dcodes=None, max_norm=1.0, norm=P, ws=P, nbytes=1 << 30):
@@ -83,6 +164,7 @@ def test_grad_clip_refusals(lib, args, said):
 
 
 def test_cpu_tensors_are_refused():
+    from mathbrain.bias_attention import relative_bias_attention
     from mathbrain.grad_clip import clip_gradients
     from mathbrain.qk_norm import qk_norm_rotary
     x = torch.zeros(1, 1, 1, 32)
@@ -90,3 +172,5 @@ def test_cpu_tensors_are_refused():
         qk_norm_rotary(x, x, x[0, 0, 0], x[0, 0, 0], x[0, 0, :, :16], x[0, 0, :, :16])
     with pytest.raises(NotImplementedError, match="no CPU path"):
         clip_gradients([x], 1.0)
+    with pytest.raises(NotImplementedError, match="no CPU path"):
+        relative_bias_attention(x, x, x, torch.zeros(4, 1))
