@@ -663,10 +663,11 @@ typedef struct mb_bias_attn {
                                   /*   for keys behind the query (distance j - pos_i >= 1) */
     const void *lengths;          /* [B] keys that count, or NULL: Lk. Rows of k and v from there on */
     int64_t lengths_bytes;        /*   are not used, their gradients are zero. 4: int32, 8: int64 */
-    const void *q_start;          /* [B] position of each row's first query, or NULL: q_start0 */
-    int64_t q_start_bytes, q_start0;
+    const void *q_start;          /* [B] position of each row's first query (within +-2^29), or NULL: */
+    int64_t q_start_bytes, q_start0; /* q_start0 */
     int64_t B, H, Hk, Lq, Lk, hd; /* hd: 32, 64 or 128 */
-    int64_t causal;               /* a query sees the keys j <= pos_i */
+    int64_t causal;               /* a query sees the keys j <= pos_i; keys behind the last query are */
+                                  /*   not used, as those behind lengths */
     int64_t dtype, bias_dtype;    /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
     double scale;
     void *o;                      /* [B, H, Lq, hd]: written by the forward, read by the backward */

@@ -65,7 +65,8 @@ class CausalSelfAttention(nn.Module):
         shape = (B, L, self.n_heads, self.head_dim)
         q, k = self.wq(x).view(shape), self.wk(x).view(shape)
         if self.qk_norm:
-            q, k = qk_norm_rotary(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps)
+            q, k = qk_norm_rotary(q, k, self.q_norm.weight, self.k_norm.weight, cos.float(), sin.float(),
+                                  self.q_norm.eps)
         else:
             q, k = rotate(q, cos, sin), rotate(k, cos, sin)
         q, k = q.transpose(1, 2), k.transpose(1, 2)

@@ -156,6 +156,7 @@ class RelativeBiasAttentionFunction(torch.autograd.Function):
         return o
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
         q, k, v, bias, o, lse, lengths, start_rows = ctx.saved_tensors
         max_distance, causal, scale, start = ctx.rest
@@ -199,11 +200,12 @@ def relative_bias_attention(q, k, v, bias, max_distance=128, causal=True, scale=
     [buckets, H] (fp32 or bf16) added to the scores by distance.  Returns [B, H, Lq, hd].
 
     ``q_start``: the position of each row's first query among the keys, an int or an int32 / int64
-    tensor [B] (within +-2^30); None: Lk - Lq, so that the last query stands at the last key.
+    tensor [B] (within +-2^29); None: Lk - Lq, so that the last query stands at the last key.
     ``causal``: a query sees the keys up to its position.  ``lengths``: an int32 / int64 tensor [B];
-    keys from there on are not seen, whatever their rows hold (values in 0 .. Lk; others are taken
-    as the nearest of these).  A query that sees no key gets zeros, and passes on no gradient.
-    Other values have to be finite.  ``scale``: 1 / sqrt(hd) by default.
+    keys from there on are not seen (values in 0 .. Lk; others are taken as the nearest of these).
+    Rows of k and v behind these ends, and with ``causal`` behind the last query's position, may hold
+    anything; other values have to be finite.  A query that sees no key gets zeros, and passes on no
+    gradient.  ``scale``: 1 / sqrt(hd) by default.
 
     In bf16 the probabilities and the scores' gradients are rounded to bf16 for the products that
     they enter; all sums are in fp32.  Gradients come out the same each time."""

@@ -98,12 +98,16 @@ __device__ inline int row_int(const void* p, int bytes, int b, int lo, int hi) {
     const int64_t v = bytes == 8 ? ((const int64_t*)p)[b] : (int64_t)((const int32_t*)p)[b];
     return (int)(v < lo ? lo : v > hi ? hi : v);
 }
-// Position of the row's first query, and how many of its keys count.
+constexpr int kFarthest = 1 << 29;   // positions and lengths: sums and differences of them fit 32 bits
+// Position of the row's first query.
 __device__ inline int first_position(const Args& a, int b) {
-    return a.start ? row_int(a.start, a.start_bytes, b, -(1 << 30), 1 << 30) : a.start0;
+    return a.start ? row_int(a.start, a.start_bytes, b, -kFarthest, kFarthest) : a.start0;
 }
+// How many of the row's keys may be seen: rows from there on are not used at all, so that a cache
+// may hold anything behind its last token.
 __device__ inline int key_count(const Args& a, int b) {
-    return a.lengths ? row_int(a.lengths, a.lengths_bytes, b, 0, a.Lk) : a.Lk;
+    const int n = a.lengths ? row_int(a.lengths, a.lengths_bytes, b, 0, a.Lk) : a.Lk;
+    return a.causal ? max(0, min(n, first_position(a, b) + a.Lq)) : n;
 }
 
 __device__ inline int bucket_of(const Args& a, int d) {

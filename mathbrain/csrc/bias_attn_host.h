@@ -57,7 +57,7 @@ int split_launch(const Args& a, int hd, int dtype, int splits, void* part, hipSt
 // Checks what both directions take and fills the kernels' arguments; 0 or an error code.
 inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
     MB_REQUIRE(p, "%s: null args", what);
-    const int64_t top = 1 << 30;
+    const int64_t top = kFarthest;
     MB_REQUIRE(p->B >= 0 && p->B <= top && p->Lq >= 0 && p->Lq <= top && p->Lk >= 0 && p->Lk <= top && p->H >= 1 && p->H <= top
                    && p->Hk >= 1 && p->Hk <= top,
                "%s: B=%lld H=%lld Hk=%lld Lq=%lld Lk=%lld", what, (long long)p->B, (long long)p->H, (long long)p->Hk,

@@ -114,7 +114,8 @@ def clip_gradients(grads, max_norm, out=None):
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """torch.nn.utils.clip_grad_norm_ for the 2-norm, on one GPU: scales the parameters' gradients
-    in place and returns their norm before that.  Parameters without a gradient are passed over.
+    in place and returns their norm before that.  Parameters without a gradient are passed over; one
+    that is listed twice is refused (HipKernelError), as are gradients that share memory.
     ``error_if_nonfinite`` raises RuntimeError, before anything is scaled, where the norm is not
     finite (that reads the norm back to the host).  ``foreach`` is accepted and has no effect."""
     if float(norm_type) != 2.0:

@@ -106,6 +106,7 @@ class QKNormRotaryFunction(torch.autograd.Function):
         return qk_norm_rotary_fwd(q, k, q_weight, k_weight, cos, sin, eps, start_rows, start)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, start_rows = ctx.saved_tensors
         eps, start = ctx.rest

@@ -117,6 +117,22 @@ def test_steps_under_bf16_autocast():
         opt.step()
 
 
+def test_a_model_in_bf16_throughout():
+    """model.bfloat16(): weights, tables and bias in bf16; finite losses and gradients of that type, and
+    logits within bf16's steps of the fp32 model's (as under autocast, and the tables' and weights'
+    roundings: held to 1e-1)."""
+    m = model(qk_norm=True, rel_buckets=32)
+    x = torch.randint(0, V, (4, 130), device="cuda")
+    with torch.no_grad():
+        full = m(x)
+    m = m.bfloat16()
+    logits = m(x)
+    assert logits.dtype == torch.bfloat16 and off(logits.float(), full.cpu().double()) < 1e-1
+    F.cross_entropy(logits.view(-1, V).float(), x.view(-1)).backward()
+    for k, v in m.named_parameters():
+        assert v.grad.dtype == torch.bfloat16 and torch.isfinite(v.grad).all(), k
+
+
 def test_the_model_without_options_is_what_it_was():
     m = model()
     assert not any("norm.weight" in k and ("q_norm" in k or "k_norm" in k) or "rel_bias" in k for k in m.state_dict())

@@ -168,6 +168,35 @@ def test_lengths_and_rows_without_keys(causal, kind, t):
 
 
 @pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("Lq,H,Hk", [(1, 4, 4), (3, 8, 2), (70, 4, 4), (200, 2, 1)])
+def test_rows_behind_the_last_query_may_hold_anything(Lq, H, Hk, t):
+    """A cache that is longer than what it holds, without lengths."""
+    q, k, v, bias, do = inputs(4, H, Hk, Lq, 900, 64, t, 32, 37)
+    rows = torch.tensor([0, 5, 600, 899 - Lq], device="cuda")
+    behind = torch.arange(900, device="cuda") >= (rows + Lq)[:, None]
+    for bad in (float("nan"), float("inf")):
+        k = torch.where(behind[:, None, :, None], torch.tensor(bad, dtype=t, device="cuda"), k)
+        v = torch.where(behind[:, None, :, None], torch.tensor(bad, dtype=t, device="cuda"), v)
+        check(q, k, v, bias, do, q_start=rows, grads=Lq > 1)
+
+
+def test_farthest_positions():
+    q, k, v, bias, do = inputs(4, 2, 2, 5, 40, 32, F32, 32, 41)
+    for q_start in (1 << 29, -(1 << 29), torch.tensor([1 << 29, -(1 << 29), 1 << 29, 0], device="cuda")):
+        check(q, k, v, bias, do, q_start=q_start)
+        check(q, k, v, bias, do, q_start=q_start, causal=False)
+
+
+def test_no_second_derivatives():
+    from mathbrain.bias_attention import relative_bias_attention
+    q, k, v, bias, do = inputs(1, 1, 1, 4, 4, 32, F32, 4, 43)
+    q, do = q.detach().requires_grad_(), do.detach().requires_grad_()
+    dq, = torch.autograd.grad(relative_bias_attention(q, k, v, bias), q, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dq.sum().backward()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("causal", [True, False])
 def test_positions(causal, t):
     args = inputs(6, 4, 2, 40, 210, 64, t, 32, 7)
@@ -329,6 +358,6 @@ def test_refusals():
             relative_bias_attention(**(base | bad))
     for bad, said in ((dict(k=k[:, :1].expand(2, 3, 8, 64), v=v[:, :1].expand(2, 3, 8, 64)), "multiple of Hk=3"),
                       (dict(q=q[..., :48], k=k[..., :48], v=v[..., :48]), "head_dim=48"), (dict(scale=0.0), "scale"),
-                      (dict(scale=float("nan")), "scale"), (dict(q_start=1 << 31), "q_start")):
+                      (dict(scale=float("nan")), "scale"), (dict(q_start=(1 << 29) + 1), "q_start")):
         with pytest.raises(_lib.HipKernelError, match=said):
             relative_bias_attention(**(base | bad))

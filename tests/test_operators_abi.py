@@ -85,11 +85,11 @@ def attn(first=(0, 1, 5), **fields):
 
 @pytest.mark.parametrize("bad,said", [
     (dict(hd=96), "head_dim=96"), (dict(dtype=3), "dtype=3"), (dict(bias_dtype=-1), "bias_dtype=-1"), (dict(q=0), "null"),
-    (dict(v=0), "null"), (dict(bias=0), "null"), (dict(Lq=-1), "Lq=-1"), (dict(Lk=1 << 31), "Lk=2147483648"),
+    (dict(v=0), "null"), (dict(bias=0), "null"), (dict(Lq=-1), "Lq=-1"), (dict(Lk=(1 << 29) + 1), "Lk=536870913"),
     (dict(Hk=3), "multiple of Hk=3"), (dict(Hk=0), "Hk=0"), (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(starts=0), "first distances"), (dict(buckets=4), "4 buckets for 3"), (dict(causal=0), "3 buckets for 3"),
     (dict(lengths=P, lengths_bytes=2), "4 or 8 bytes"), (dict(q_start=P, q_start_bytes=1), "4 or 8 bytes"),
-    (dict(q_start0=1 << 31), "q_start=2147483648"), (dict(q=P + 2), "16 bytes"), (dict(k2=513), "16 bytes"),
+    (dict(q_start0=1 << 30), "q_start=1073741824"), (dict(q=P + 2), "16 bytes"), (dict(k2=513), "16 bytes"),
     (dict(v2=-512), "elements apart"), (dict(q2=1 << 24), "elements apart"), (dict(B=1 << 20, H=1 << 12), "too many")])
 def test_bias_attention_refusals(lib, bad, said):
     for name in ("mb_bias_attn_fwd", "mb_bias_attn_bwd"):
