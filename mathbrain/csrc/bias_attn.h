@@ -139,8 +139,6 @@ __device__ inline void fill_table(const Args& a, int h, float* tab) {
 // other, so a row has no padding; piece c of row r lies in the row's place c ^ swz(r) instead,
 // which spreads both ways of reading the tile over the banks.
 
-constexpr int kStages = 3;
-
 // 16 (or 4) bytes a lane from base + voff to LDS at lds + 16 (or 4) * lane.
 __device__ inline void dma16(uint32_t lds, uint32_t voff, const void* base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
@@ -177,6 +175,9 @@ struct Tile {
     static constexpr int kPieces = kRow / 16;
     static constexpr int kLoads = kBytes / 4096;                   // of each of the four waves
     static_assert(kBytes % 4096 == 0, "a wave's load moves 1 KiB");
+    // Tiles of each kind in LDS: two on their way beside the one in use, or one where three would leave
+    // a CU a single workgroup of the two that its registers hold (heads of 128 in bf16).
+    static constexpr int kStages = sizeof(T) == 2 && kBytes > 8192 ? 2 : 3;
 
     static __device__ constexpr int swz(int row) {
         if (kPieces == 4) return (row >> 2) & 3;

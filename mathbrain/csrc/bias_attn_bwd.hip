@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     __shared__ float far[4][2];
     const Reach reach(a);
     const int entries = reach.entries();
-    float* tab = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes);
+    float* tab = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes);
     float* hist = tab + entries;   // [wave][entries], then the waves' blocks
 
     const int lane = threadIdx.x & 63, wave = wave_id();
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     if (want_bias)
         for (int n = threadIdx.x; n < 4 * entries; n += kThreads) hist[n] = 0.f;
     Diagonals diag;
-    diag.block = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
+    diag.block = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
     diag.sums = hist + wave * entries + kPad - reach.lo + (lane & 31);
     // Keys go up, so the blocks at or above the reach come first, those at or below its lower end last.
     float far_hi = 0.f, far_sum = 0.f, row_sum = 0.f;
@@ -167,16 +167,16 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     // block(ktile, vtile, u, jb) for the wave's blocks of 32 keys from jb on, in rows 32 u of the tiles
     auto walk = [&](auto&& block) {
         auto load = [&](int t) {
-            const uint32_t tile = lds + t % kStages * (2 * Tl::kBytes);
+            const uint32_t tile = lds + t % Tl::kStages * (2 * Tl::kBytes);
             Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
             Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
         };
         if (tiles > 0)
-            for (int t = 0; t < kStages - 1; ++t) load(t);
+            for (int t = 0; t < Tl::kStages - 1; ++t) load(t);
         for (int t = 0; t < tiles; ++t) {
-            wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
-            load(t + kStages - 1);
-            const uint32_t ktile = lds + t % kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
+            wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
+            load(t + Tl::kStages - 1);
+            const uint32_t ktile = lds + t % Tl::kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u) {
                 const int jb = t * KT + 32 * u;
@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     using Tl = Tile<T, HD>;
     constexpr int QT = Tl::kN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ __attribute__((aligned(16))) float stat[kStages][2][64];   // rows' -lse and -delta
-    float* tab = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes);
+    __shared__ __attribute__((aligned(16))) float stat[Tl::kStages][2][64];   // rows' -lse and -delta
+    float* tab = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes);
 
     const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 5;
     const int nk = (a.Lk + kRows - 1) / kRows;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         const float* nlse = a.rows + ((int64_t)b * a.H + h) * a.Lq;
         const float* ndelta = nlse + (int64_t)a.B * a.H * a.Lq;
         auto load = [&](int t) {
-            const int s = t % kStages;
+            const int s = t % Tl::kStages;
             if (wave < 2)   // one wave the rows' -lse, another their -delta; the last row's past the end
                 dma4(lds_address(&stat[s][wave][0]), 4u * (uint32_t)min(t * QT + lane, a.Lq - 1),
                      wave ? ndelta : nlse);
@@ -370,12 +370,12 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         if (first >= tiles) break;
         fill_table(a, h, tab);   // the previous head's last barrier lies behind its reads
         loads_done();
-        for (int t = first; t < first + kStages - 1; ++t) load(t);
+        for (int t = first; t < first + Tl::kStages - 1; ++t) load(t);
         for (int t = first; t < tiles; ++t) {
-            const int s = t % kStages;
+            const int s = t % Tl::kStages;
             // (two waves have a load more on their way: they wait for that one of the next tile too)
-            wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();
-            load(t + kStages - 1);
+            wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();
+            load(t + Tl::kStages - 1);
             const uint32_t qtile = lds + s * (2 * Tl::kBytes), gtile = qtile + Tl::kBytes;
 #pragma unroll
             for (int u = 0; u < QT / 32; ++u) {
@@ -481,8 +481,8 @@ template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
     const int entries = Reach(a).entries();
     const int table = entries * (int)sizeof(float);
-    const int base = 2 * kStages * Tile<T, HD>::kBytes + table;
-    const int lds_q = 2 * kStages * QueryTile<T, HD>::kBytes + table + (a.dbias_part ? (4 * entries + 3 + 4 * 32 * Diagonals::kStride) * (int)sizeof(float) : 0);
+    const int base = 2 * Tile<T, HD>::kStages * Tile<T, HD>::kBytes + table;
+    const int lds_q = 2 * QueryTile<T, HD>::kStages * QueryTile<T, HD>::kBytes + table + (a.dbias_part ? (4 * entries + 3 + 4 * 32 * Diagonals::kStride) * (int)sizeof(float) : 0);
     if (a.Lq > 0) {
         static Told told;
         if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q, told)) return rc;

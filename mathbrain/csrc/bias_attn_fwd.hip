@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     using Tl = Tile<T, HD>;
     constexpr int KT = Tl::kN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* tab = reinterpret_cast<float*>(smem + 2 * kStages * Tl::kBytes);
+    float* tab = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes);
 
     const int lane = threadIdx.x & 63, wave = wave_id();
     int bh, qb;
@@ -46,18 +46,18 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     const typename Tl::Lane at;
     const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
     auto load = [&](int t) {
-        const uint32_t tile = lds + t % kStages * (2 * Tl::kBytes);
+        const uint32_t tile = lds + t % Tl::kStages * (2 * Tl::kBytes);
         Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
         Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
     };
     loads_done();
     if (tiles > 0)
-        for (int t = 0; t < kStages - 1; ++t) load(t);
+        for (int t = 0; t < Tl::kStages - 1; ++t) load(t);
     for (int t = 0; t < tiles; ++t) {
         // tile t is there, and nobody reads the one before it any longer
-        wait_and_meet<(kStages - 2) * 2 * Tl::kLoads>();
-        load(t + kStages - 1);   // past the end too: the waits count loads
-        const uint32_t ktile = lds + t % kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
+        wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();
+        load(t + Tl::kStages - 1);   // past the end too: the waits count loads
+        const uint32_t ktile = lds + t % Tl::kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
         const int j0 = t * KT;
         if (j0 < wend) {
             f32x16 x[KT / 32];
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
-    const int lds = 2 * kStages * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
+    const int lds = 2 * Tile<T, HD>::kStages * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
     static Told told;
     if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD>, lds, told)) return rc;
     hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds, st, a);
