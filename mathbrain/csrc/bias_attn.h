@@ -124,7 +124,7 @@ __device__ inline int bucket_of(const Args& a, int d) {
 // tab[i] = log2(e) bias of distance lo - kPad + i (clamped to lo .. hi), by all threads.
 __device__ inline void fill_table(const Args& a, int h, float* tab) {
     const Reach r(a);
-    for (int i = threadIdx.x; i < r.entries(); i += kThreads) {
+    for (int i = threadIdx.x; i < r.entries(); i += blockDim.x) {
         const int d = r.lo - kPad + i;
         const int64_t at = (int64_t)bucket_of(a, d < r.lo ? r.lo : d > r.hi ? r.hi : d) * a.H + h;
         tab[i] = kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
@@ -193,14 +193,14 @@ struct Tile {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) v[i] = (uint32_t)(row(i) * (int)(sl * (int)sizeof(T))) + piece(i);
         }
-        static __device__ int slot(int i) { return i * kThreads + (int)threadIdx.x; }
+        static __device__ int slot(int i) { return i * kThreads + (int)(threadIdx.x % kThreads); }
         static __device__ int row(int i) { return slot(i) / kPieces; }
         static __device__ uint32_t piece(int i) { return (uint32_t)((slot(i) % kPieces) ^ swz(row(i) & 15)) << 4; }
     };
     // Rows row0 .. row0 + kN - 1 of `base` on their way to the tile; rows from `rows` (at least 1)
     // on are the last one again.
     static __device__ void load(uint32_t tile, const T* base, int64_t sl, int row0, int rows, const Offsets& off) {
-        const uint32_t lds = tile + wave_id() * 1024;
+        const uint32_t lds = tile + wave_id() % 4 * 1024;
         const int first = min(row0, rows - 1);
         const T* from = base + first * sl;
         if (row0 + kN <= rows) {

@@ -9,15 +9,20 @@ namespace {
 // four waves read out of LDS; the next tile's rows are on their way from memory meanwhile.
 // Running maximum, sum and output are in fp32; the probabilities are rounded to bf16 for the
 // product with V where the inputs are bf16 (half a step of 2^-8 of each), the sum is not.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn_fwd_kernel(const Args a) {
+//
+// SETS = 2: a second set of four waves takes every second tile for the same queries, and the two
+// are joined through LDS in the end.  A workgroup's walk, which takes 1.2 us (heads of 128: 1.5) a
+// tile with nothing beside it on the CU, is then half as long.
+template <typename T, int HD, int SETS>
+__global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bias_attn_fwd_kernel(const Args a) {
     using X = Ty<T>;
     using Tl = Tile<T, HD>;
     constexpr int KT = Tl::kN;
+    constexpr int kStage = 2 * Tl::kBytes;            // a tile of K and one of V
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* tab = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes);
+    float* tab = reinterpret_cast<float*>(smem + SETS * Tl::kStages * kStage);
 
-    const int lane = threadIdx.x & 63, wave = wave_id();
+    const int lane = threadIdx.x & 63, wave = wave_id() % 4, set = wave_id() / 4;
     int bh, qb;
     place(a.B * a.H, a.nq, false, bh, qb);
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
@@ -42,23 +47,24 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     for (int d = 0; d < HD / 32; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
 
-    const uint32_t lds = lds_address(smem);
+    const uint32_t lds = lds_address(smem) + set * kStage;
     const typename Tl::Lane at;
     const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
-    auto load = [&](int t) {
-        const uint32_t tile = lds + t % Tl::kStages * (2 * Tl::kBytes);
-        Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
-        Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
+    auto load = [&](int n) {   // the set's n-th tiles
+        const uint32_t tile = lds + n % Tl::kStages * (SETS * kStage);
+        const int j0 = (n * SETS + set) * KT;
+        Tl::load(tile, kbase, a.k_sl, j0, len, koff);
+        Tl::load(tile + Tl::kBytes, vbase, a.v_sl, j0, len, voff);
     };
     loads_done();
     if (tiles > 0)
-        for (int t = 0; t < Tl::kStages - 1; ++t) load(t);
-    for (int t = 0; t < tiles; ++t) {
-        // tile t is there, and nobody reads the one before it any longer
+        for (int n = 0; n < Tl::kStages - 1; ++n) load(n);
+    for (int n = 0; n * SETS < tiles; ++n) {
+        // the n-th tiles are there, and nobody reads those before them any longer
         wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();
-        load(t + Tl::kStages - 1);   // past the end too: the waits count loads
-        const uint32_t ktile = lds + t % Tl::kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
-        const int j0 = t * KT;
+        load(n + Tl::kStages - 1);   // past the end too: the waits count loads
+        const uint32_t ktile = lds + n % Tl::kStages * (SETS * kStage), vtile = ktile + Tl::kBytes;
+        const int j0 = (n * SETS + set) * KT;
         if (j0 < wend) {
             f32x16 x[KT / 32];
 #pragma unroll
@@ -130,8 +136,30 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
                 }
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // LDS is written until then
+    wait_and_meet<0>();   // LDS is written until then
     l = half_sum(l);
+    if constexpr (SETS == 2) {
+        // the second set's maximum, sum and output, a column a lane
+        float* other = reinterpret_cast<float*>(smem) + wave * (HD + 2) * 33 + (lane & 31);
+        if (set == 1) {
+            if (lane < 32) other[HD * 33] = m, other[(HD + 1) * 33] = l;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) other[(32 * d + row_of(r)) * 33] = o[d][r];
+        }
+        __syncthreads();
+        if (set == 1) return;
+        const float m1 = other[HD * 33], l1 = other[(HD + 1) * 33];
+        const float mn = fmaxf(m, m1), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
+        m = mn;
+        l = l * f0 + l1 * f1;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f0 + other[(32 * d + row_of(r)) * 33] * f1;
+    }
     if (i < a.Lq) {
         const float inv = l > 0.f ? 1.0f / l : 0.f;   // a row without keys: zeros
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
@@ -142,13 +170,28 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     }
 }
 
+template <typename T, int HD, int SETS>
+int launch_sets(const Args& a, hipStream_t st) {
+    using Tl = Tile<T, HD>;
+    static_assert(SETS == 1 || 4 * (HD + 2) * 33 * 4 <= SETS * 2 * Tl::kStages * Tl::kBytes, "the sets are joined where the tiles were");
+    const int lds = SETS * 2 * Tl::kStages * Tl::kBytes + Reach(a).entries() * (int)sizeof(float);
+    static Told told;
+    if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD, SETS>, lds, told)) return rc;
+    hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD, SETS>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(SETS * kThreads), lds, st, a);
+    return check_launch("mb_bias_attn_fwd");
+}
+
+// Two sets of waves where the grid leaves room for them on its CUs and the walks are long.  Measured
+// in bf16, two sets against one, 8 heads: of 64: 2 x 2048 (256 workgroups) 32 us against 41, 3 x 2048 36
+// against 44, 12 x 512 24 against 21, 4 x 2048 46 against 44; of 128: 2 x 2048 44 against 53, 3 x 2048 53 against
+// 59, 12 x 512 31 against 27; of 32: 4 x 2048 29 against 37.  fp32 heads of 128 leave no LDS for them.
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
-    const int lds = 2 * Tile<T, HD>::kStages * Tile<T, HD>::kBytes + Reach(a).entries() * (int)sizeof(float);
-    static Told told;
-    if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD>, lds, told)) return rc;
-    hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds, st, a);
-    return check_launch("mb_bias_attn_fwd");
+    if constexpr (sizeof(T) == 2 || HD < 128) {
+        const int blocks = a.B * a.H * a.nq;
+        if (a.Lk >= 256 && (blocks <= 256 || (a.Lk >= 1024 && blocks <= (HD == 32 ? 512 : 384)))) return launch_sets<T, HD, 2>(a, st);
+    }
+    return launch_sets<T, HD, 1>(a, st);
 }
 
 }  // namespace

@@ -32,20 +32,21 @@ inline bool rows16(const void* p, const int64_t* st, int dtype) {
 
 // Parts that the keys of a row are split into (bias_attn_split.hip), or 0 for the kernel whose
 // workgroups walk all keys for 128 queries of a head.  The latter leaves CUs idle where its grid is
-// small, and its longest workgroup takes 1.2 us (heads of 128: 1.5) for every 64 keys; the former
-// takes about 8 us to start and join, and 1.6 ns (3.5) for every 32 queries by 32 keys.  The one is
-// the shorter where the pairs that a mask leaves fill less than about 80 (40) workgroups and the
-// keys are not few.  Measured in bf16, split against not: 1 x 2048, 8 heads x 64 35 us against 42, 2 x
-// 2048 53 against 42, 1 x 512 17 against 21, 8 x 128 15 against 13; 8 heads x 128: 1 x 1024 41
-// against 31, 1 x 2048 75 against 50, 4 x 128 queries of 4096 keys 54 against 90.  Up to 32 rows for a key head are one column
-// block of the split kernel (16 x 1 of 4096, 8 heads x 64: 27 us against 97).
+// small, and its time is that of its longest walk; the former takes a few us more to start and
+// join, and a time that grows with the pairs.  The one is the shorter where the pairs that a mask
+// leaves fill few workgroups and the keys are many.  Measured in bf16, split against not, 8 heads:
+// of 64: 1 x 1024 23 us against 22, 1 x 2048 34 against 32, 4 x 128 queries of 4096 keys 36 against 52, 1 x 256
+// of 4096 22 against 50; of 128: 1 x 2048 75 against 50, 4 x 128 of 4096 55 against 70; of 32: 1 x 2048
+// 25 against 27.  Up to 32 rows for a key head are one column block of the split kernel (16 x 1 of
+// 4096, 8 heads x 64: 27 us against 97).
 inline int splits_of(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
     const int64_t G = H / Hk, tiles = (G * Lq + 31) / 32, nq = ((int64_t)Lq + kRows - 1) / kRows;
     if (G > 32 || (double)B * Hk * tiles > 0x7fffffff / 64) return 0;
     if (G * Lq > 32) {
         // a causal mask leaves Lk - Lq / 2 of Lk keys where the last query sees them all
         const double share = causal && Lk > 0 ? 1.0 - 0.5 * (Lq < Lk ? Lq : Lk) / Lk : 1.0;
-        if (Lk < (hd == 128 ? 2048 : 512) || (double)B * H * nq * share > (hd == 128 ? 40.0 : 80.0)) return 0;
+        const double most = hd == 128 ? 40.0 : hd == 64 ? 52.0 : 70.0;
+        if (Lk <= 400 || (double)B * H * nq * share > most * (1.0 - 400.0 / Lk)) return 0;
     }
     const int64_t wanted = (hd == 128 ? 512 : 768) / ((int64_t)B * Hk * tiles);  // two or three workgroups a CU
     const int64_t most = ((int64_t)Lk + 511) / 512;                              // at least 128 keys a wave
