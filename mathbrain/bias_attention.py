@@ -67,7 +67,8 @@ def _starts_array(num_buckets, max_distance, causal):
 def _rows16(x):
     """x with the channels next to each other and rows at multiples of 16 bytes, at most 16 MiB apart."""
     sb, sh, sl, sd = x.stride()
-    if sd == 1 and not (x.data_ptr() | (sb | sh | sl) * x.element_size()) & 15 and sl * x.element_size() <= 1 << 24:
+    size = x.element_size()
+    if sd == 1 and not (x.data_ptr() | (sb | sh | sl) * size) & 15 and sl * size <= 1 << 24:
         return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
 

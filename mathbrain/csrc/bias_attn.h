@@ -75,7 +75,7 @@ struct Args {
     int64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl, o_sb, o_sh, o_sl, do_sb, do_sh, do_sl;
     const void* bias;                        // [buckets, H]
     const void *lengths, *start;             // [B] or NULL
-    void *out, *dk, *dv;                     // out: o (forward) or dq
+    void *out, *dk, *dv, *dbias;             // out: o (forward) or dq
     int64_t out_sb, out_sh, out_sl, dk_sb, dk_sh, dk_sl, dv_sb, dv_sh, dv_sl;
     float *lse, *rows, *dbias_part;          // [B, H, Lq] (log2 units), [2, B, H, Lq], [H, B * nq, buckets]
     int lengths_bytes, start_bytes, start0;
@@ -309,13 +309,12 @@ __device__ inline void store_block(T* row, int d0, const f32x16& x, float mul) {
     }
 }
 
-// The workgroup's row block and head.  Blocks with the most pairs go first (`first_most`: block 0,
+// The row block and head of workgroup id.  Blocks with the most pairs go first (`first_most`: block 0,
 // else the last one), all heads of a block position one after another: a head's blocks then land
 // on one XCD where the heads are a multiple of 8, and read its keys out of that L2.  Every second
 // 256 workgroups (one for each CU) run backwards in steps of 8, so that a CU's share of a grid
 // that is resident at once comes out even.
-__device__ inline void place(int heads, int blocks, bool first_most, int& bh, int& blk) {
-    int id = blockIdx.x;
+__device__ inline void place(int id, int heads, int blocks, bool first_most, int& bh, int& blk) {
     if ((id & 256) && (id | 255) < heads * blocks) id = (id & ~255) + (31 - ((id >> 3) & 31)) * 8 + (id & 7);
     bh = id % heads;
     blk = id / heads;

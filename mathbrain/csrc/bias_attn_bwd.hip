@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 
     const int lane = threadIdx.x & 63, wave = wave_id();
     int bh, qb;
-    place(a.B * a.H, a.nq, false, bh, qb);
+    place(blockIdx.x, a.B * a.H, a.nq, false, bh, qb);
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const int len = key_count(a, b), p0 = first_position(a, b);
     const int w0 = qb * kRows + wave * kWaveRows;
@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     diag.sums = hist + wave * entries + kPad - reach.lo + (lane & 31);
     // Keys go up, so the blocks at or above the reach come first, those at or below its lower end last.
     float far_hi = 0.f, far_sum = 0.f, row_sum = 0.f;
+    float far_p_hi = 0.f, far_p = 0.f;   // the blocks' probabilities
     bool first_part = true;
     int last_d0 = 0;
 
@@ -232,17 +233,25 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
             for (int r = 0; r < 16; ++r) y0[r] = -delta;
     }
     walk([&](uint32_t ktile, uint32_t vtile, int u, int jb) {
-        f32x16 x, y;
-        products(ktile, vtile, u, jb, x, y);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            x[r] = kStart ? __builtin_amdgcn_exp2f(x[r]) * y[r] : __builtin_amdgcn_exp2f(x[r] - lse) * (y[r] - delta);
         const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
         const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
         if (first_part && !above) {
             first_part = false;
             far_hi = far_sum, far_sum = 0.f;
+            far_p_hi = far_p, far_p = 0.f;
         }
+        f32x16 x, y;
+        products(ktile, vtile, u, jb, x, y);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(kStart ? x[r] : x[r] - lse);
+        if (sizeof(T) == 2 && want_bias && one) {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r % 4] += x[r];
+            far_p += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= kStart ? y[r] : y[r] - delta;
         if (want_bias && !one) diag.give(x);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -278,7 +287,10 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     if (!want_bias) return;
     diag.close(last_d0);
     float far_lo = far_sum;
-    if (first_part) far_hi = far_lo, far_lo = 0.f;
+    if (first_part) far_hi = far_lo, far_lo = 0.f, far_p_hi = far_p, far_p = 0.f;
+    // delta's error again: what is left of a row's sum belongs to its pairs by their probability.  The
+    // blocks of one bucket, which have most of it in long rows, are put right here.
+    if (sizeof(T) == 2) far_hi -= row_sum * far_p_hi, far_lo -= row_sum * far_p;
     far_hi = wave_sum(far_hi);
     far_lo = wave_sum(far_lo);
     if (lane == 0) far[wave][0] = far_hi, far[wave][1] = far_lo;
@@ -317,8 +329,28 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     }
 }
 
+// dbias[n, h] = the sum of part[h, :, n], in a fixed order, by a workgroup: strips of rows.
+__device__ inline void add_parts(const Args& a, int h, float* sums) {
+    const int rows = a.B * a.nq;
+    const int strips = kThreads / a.buckets;   // at least one: buckets <= 256
+    const int n = threadIdx.x % a.buckets, strip = threadIdx.x / a.buckets;
+    const float* part = a.dbias_part + (int64_t)h * rows * a.buckets + n;
+    float v = 0.f;
+    if (strip < strips)
+        for (int r = strip; r < rows; r += strips) v += part[(int64_t)r * a.buckets];
+    sums[threadIdx.x] = v;
+    __syncthreads();
+    if (strip == 0) {
+        for (int k = 1; k < strips; ++k) v += sums[k * a.buckets + n];
+        const int64_t at = (int64_t)n * a.H + h;
+        if (a.bias_bf16) ((__bf16*)a.dbias)[at] = (__bf16)v;
+        else ((float*)a.dbias)[at] = v;
+    }
+}
+static_assert(2 * kMaxStarts <= kThreads, "a thread for every bucket");
+
 // A workgroup takes 128 keys of one key head, 32 to a wave, and walks the queries of all query
-// heads that share it.
+// heads that share it.  Where dbias is wanted, H workgroups before these add the queries' pass's parts of it.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bias_attn_dkv_kernel(const Args a) {
     using X = Ty<T>;
@@ -328,10 +360,15 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     __shared__ __attribute__((aligned(16))) float stat[Tl::kStages][2][64];   // rows' -lse and -delta
     float* tab = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes);
 
-    const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 5;
     const int nk = (a.Lk + kRows - 1) / kRows;
+    const int id = (int)blockIdx.x - (a.dbias ? a.H : 0);
+    if (id < 0) {
+        add_parts(a, blockIdx.x, reinterpret_cast<float*>(smem));
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 5;
     int bh, kb;
-    place(a.B * a.Hk, nk, true, bh, kb);
+    place(id, a.B * a.Hk, nk, true, bh, kb);
     const int b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
     const Reach reach(a);
     const int len = key_count(a, b), p0 = first_position(a, b);
@@ -456,43 +493,22 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     }
 }
 
-// dbias[n, h] = the sum of part[h, :, n], in a fixed order: a workgroup per head, strips of rows.
-__global__ void __launch_bounds__(kThreads) bias_attn_dbias_kernel(const float* __restrict__ part, int rows, int buckets,
-                                                                   int H, int bf16, void* dbias) {
-    __shared__ float sums[kThreads];
-    const int h = blockIdx.x;
-    const int strips = kThreads / buckets;   // at least one: buckets <= 256
-    const int n = threadIdx.x % buckets, strip = threadIdx.x / buckets;
-    float v = 0.f;
-    if (strip < strips)
-        for (int r = strip; r < rows; r += strips) v += part[((int64_t)h * rows + r) * buckets + n];
-    sums[threadIdx.x] = v;
-    __syncthreads();
-    if (strip == 0) {
-        for (int k = 1; k < strips; ++k) v += sums[k * buckets + n];
-        const int64_t at = (int64_t)n * H + h;
-        if (bf16) ((__bf16*)dbias)[at] = (__bf16)v;
-        else ((float*)dbias)[at] = v;
-    }
-}
-static_assert(2 * kMaxStarts <= kThreads, "a thread for every bucket");
-
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
     const int entries = Reach(a).entries();
     const int table = entries * (int)sizeof(float);
     const int base = 2 * Tile<T, HD>::kStages * Tile<T, HD>::kBytes + table;
     const int lds_q = 2 * QueryTile<T, HD>::kStages * QueryTile<T, HD>::kBytes + table + (a.dbias_part ? (4 * entries + 3 + 4 * 32 * Diagonals::kStride) * (int)sizeof(float) : 0);
-    if (a.Lq > 0) {
+    if (a.B > 0 && a.Lq > 0) {
         static Told told;
         if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q, told)) return rc;
         hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds_q, st, a);
     }
-    if (a.Lk > 0) {
+    const int nk = (a.Lk + kRows - 1) / kRows, blocks = a.B * a.Hk * nk + (a.dbias ? a.H : 0);
+    if (blocks > 0) {
         static Told told;
         if (const int rc = allow_lds((const void*)bias_attn_dkv_kernel<T, HD>, base, told)) return rc;
-        const int nk = (a.Lk + kRows - 1) / kRows;
-        hipLaunchKernelGGL((bias_attn_dkv_kernel<T, HD>), dim3((unsigned)(a.B * a.Hk * nk)), dim3(kThreads), base, st, a);
+        hipLaunchKernelGGL((bias_attn_dkv_kernel<T, HD>), dim3((unsigned)blocks), dim3(kThreads), base, st, a);
     }
     return check_launch("mb_bias_attn_bwd");
 }
@@ -538,16 +554,10 @@ extern "C" int mb_bias_attn_bwd(const mb_bias_attn* p, void* stream) {
     }
     a.lse = p->lse;
     a.rows = (float*)p->workspace;
+    a.dbias = p->dbias;
     a.dbias_part = p->dbias && need > 0 ? (float*)p->workspace + padded(2 * (int64_t)a.B * a.H * a.Lq) : nullptr;
     hipStream_t st = (hipStream_t)stream;
-    if (a.B > 0) {
-        const int rc = dtype == MB_DTYPE_F32
-                           ? (hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st))
-                           : (hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st));
-        if (rc) return rc;
-    }
-    if (p->dbias)
-        hipLaunchKernelGGL(bias_attn_dbias_kernel, dim3(a.H), dim3(kThreads), 0, st, a.dbias_part,
-                           a.dbias_part ? a.B * a.nq : 0, a.buckets, a.H, a.bias_bf16, p->dbias);
-    return check_launch("mb_bias_attn_bwd");
+    return dtype == MB_DTYPE_F32
+               ? (hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st))
+               : (hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st));
 }

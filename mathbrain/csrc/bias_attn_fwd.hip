@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
 
     const int lane = threadIdx.x & 63, wave = wave_id() % 4, set = wave_id() / 4;
     int bh, qb;
-    place(a.B * a.H, a.nq, false, bh, qb);
+    place(blockIdx.x, a.B * a.H, a.nq, false, bh, qb);
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const Reach reach(a);
     const int len = key_count(a, b), p0 = first_position(a, b);

@@ -85,7 +85,7 @@ inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
                "%s: lengths and q_start hold integers of 4 or 8 bytes", what);
     MB_REQUIRE(p->q_start || (p->q_start0 >= -top && p->q_start0 <= top), "%s: q_start=%lld", what, (long long)p->q_start0);
     const int64_t nq = (p->Lq + kRows - 1) / kRows, nk = (p->Lk + kRows - 1) / kRows;
-    MB_REQUIRE((double)p->B * p->H * (nq > 0 ? nq : 1) <= 0x7fffffff && (double)p->B * p->Hk * nk <= 0x7fffffff,
+    MB_REQUIRE((double)p->B * p->H * (nq > 0 ? nq : 1) <= 0x7fffffff && (double)p->B * p->Hk * nk + p->H <= 0x7fffffff,
                "%s: B=%lld H=%lld Lq=%lld Lk=%lld are too many", what, (long long)p->B, (long long)p->H, (long long)p->Lq,
                (long long)p->Lk);
     const int dtype = (int)p->dtype;
