@@ -82,7 +82,7 @@ struct Args {
     int B, H, Hk, Lq, Lk, nq;
     int causal, bias_bf16, buckets, n_starts, reach;
     float scale;
-    int16_t starts[kMaxStarts];              // first distance of each bucket of one direction
+    int starts[kMaxStarts];                  // first distance of each bucket of one direction
 };
 
 // The distance table covers lo .. hi and is padded by kPad entries on both ends.  Distances from
@@ -110,24 +110,41 @@ __device__ inline int key_count(const Args& a, int b) {
     return a.causal ? max(0, min(n, first_position(a, b) + a.Lq)) : n;
 }
 
-__device__ inline int bucket_of(const Args& a, int d) {
-    const int n = d < 0 ? -d : d;
-    int lo = 0, hi = a.n_starts - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.starts[mid] <= n) lo = mid;
-        else hi = mid - 1;
+// Buckets of N distances: how many first distances are no larger.  All of them are compared, at
+// uniform addresses: a search would take a chain of loads for each lane's own (3 us a workgroup).
+template <int N>
+__device__ inline void buckets_of(const Args& a, const int* d, int* bucket) {
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) n[i] = d[i] < 0 ? -d[i] : d[i], bucket[i] = -1;
+#pragma unroll 8
+    for (int k = 0; k < a.n_starts; ++k) {
+        const int first = a.starts[k];
+#pragma unroll
+        for (int i = 0; i < N; ++i) bucket[i] += first <= n[i] ? 1 : 0;
     }
-    return lo + (!a.causal && d < 0 ? a.n_starts : 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) bucket[i] += !a.causal && d[i] < 0 ? a.n_starts : 0;
+}
+
+__device__ inline float bias_at(const Args& a, int64_t at) {
+    return kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
 }
 
 // tab[i] = log2(e) bias of distance lo - kPad + i (clamped to lo .. hi), by all threads.
 __device__ inline void fill_table(const Args& a, int h, float* tab) {
     const Reach r(a);
-    for (int i = threadIdx.x; i < r.entries(); i += blockDim.x) {
-        const int d = r.lo - kPad + i;
-        const int64_t at = (int64_t)bucket_of(a, d < r.lo ? r.lo : d > r.hi ? r.hi : d) * a.H + h;
-        tab[i] = kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
+    for (int i = threadIdx.x; i < r.entries(); i += 2 * blockDim.x) {
+        int d[2], n[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            d[e] = r.lo - kPad + i + e * (int)blockDim.x;
+            d[e] = d[e] < r.lo ? r.lo : d[e] > r.hi ? r.hi : d[e];
+        }
+        buckets_of<2>(a, d, n);
+        const float x = bias_at(a, (int64_t)n[0] * a.H + h), y = bias_at(a, (int64_t)n[1] * a.H + h);
+        tab[i] = x;
+        if (i + (int)blockDim.x < r.entries()) tab[i + blockDim.x] = y;
     }
 }
 

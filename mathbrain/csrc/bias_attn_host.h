@@ -111,7 +111,7 @@ inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
     a.causal = p->causal != 0, a.bias_bf16 = p->bias_dtype == MB_DTYPE_BF16, a.buckets = (int)p->buckets, a.n_starts = n_starts;
     a.reach = starts[n_starts - 1];
     a.scale = (float)p->scale;
-    for (int i = 0; i < n_starts; ++i) a.starts[i] = (int16_t)starts[i];
+    for (int i = 0; i < n_starts; ++i) a.starts[i] = starts[i];
     return MB_OK;
 }
 

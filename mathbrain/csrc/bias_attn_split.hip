@@ -78,15 +78,17 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     if (w0 < w1 && pmin - (w1 + 31) < reach.hi && pmax - w0 > reach.lo) {
         for (int n = threadIdx.x; n < a.buckets * G; n += kThreads) {
             const int64_t at = (int64_t)(n / G) * a.H + hk * G + n % G;
-            values[n] = kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
+            values[n] = bias_at(a, at);
         }
-        for (int n = threadIdx.x; n <= reach.hi - reach.lo; n += kThreads) bucket[n] = (uint8_t)bucket_of(a, n + reach.lo);
+        for (int n = threadIdx.x; n <= reach.hi - reach.lo; n += kThreads) {
+            const int d = n + reach.lo;
+            int k;
+            buckets_of<1>(a, &d, &k);
+            bucket[n] = (uint8_t)k;
+        }
     }
     const int64_t far_hi = (int64_t)(a.n_starts - 1) * a.H + h, far_lo = (int64_t)(a.causal ? 0 : 2 * a.n_starts - 1) * a.H + h;
-    auto bias_at = [&](int64_t at) {
-        return kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
-    };
-    const float bias_hi = bias_at(far_hi), bias_lo = bias_at(far_lo);
+    const float bias_hi = bias_at(a, far_hi), bias_lo = bias_at(a, far_lo);
 
     typename X::Frag qf[HD / 16], kf[HD / 16];
     {
