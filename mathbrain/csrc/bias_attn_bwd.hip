@@ -122,6 +122,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     const T* vbase = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     typename X::Frag qf[HD / 16], gf[HD / 16];
     load_frags<T, HD>((const T*)a.d_o + b * a.do_sb + h * a.do_sh, a.do_sl, w0, a.Lq, gf);
+    load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
+    const float lse = i < a.Lq ? a.lse[(int64_t)bh * a.Lq + i] : INFINITY;
     // delta is dO . o, but o and the probabilities in it are rounded where the inputs are bf16, and
     // delta's error is that of every ds of its row.  It falls with the number of keys that share
     // the row's weight; where there are few of them delta is taken from the pairs themselves, in a
@@ -129,25 +131,26 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     const bool from_pairs = sizeof(T) == 2 && kend <= kRows;
     float delta = 0.f;
     if (!from_pairs) {
-        load_frags<T, HD>((const T*)a.o + b * a.o_sb + h * a.o_sh, a.o_sl, w0, a.Lq, qf);
+        typename X::Frag of[HD / 16];
+        load_frags<T, HD>((const T*)a.o + b * a.o_sb + h * a.o_sh, a.o_sl, w0, a.Lq, of);
+        fill_table(a, h, tab);
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)qf[c][e], (float)gf[c][e], delta);
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)of[c][e], (float)gf[c][e], delta);
         delta = half_sum(delta);
+    } else {
+        fill_table(a, h, tab);
     }
-    load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
     // In bf16 with heads of 64 the products' results start from -lse (in units of the scores) and
     // -delta, in two blocks of registers that leave two waves a SIMD room: p is then
     // exp2(scale x + bias) and ds is p y.
     constexpr bool kStart = HD == 64 && sizeof(T) == 2;
-    const float lse = i < a.Lq ? a.lse[(int64_t)bh * a.Lq + i] : INFINITY;
     const float nlse = statistic<T>(lse, sl2);
     if (i < a.Lq && lane < 32) a.rows[(int64_t)bh * a.Lq + i] = nlse;
     f32x16 x0, y0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) x0[r] = kStart ? nlse : 0.f, y0[r] = kStart ? -delta : 0.f;
-    fill_table(a, h, tab);
     if (want_bias)
         for (int n = threadIdx.x; n < 4 * entries; n += kThreads) hist[n] = 0.f;
     Diagonals diag;
