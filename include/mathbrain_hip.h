@@ -656,7 +656,7 @@ int mb_qk_norm_rotary_bwd(const mb_qk_norm_rotary *args, void *stream);
 typedef struct mb_bias_attn {
     const void *q, *k, *v;        /* [B, H, Lq, hd], [B, Hk, Lk, hd] twice; Hk divides H */
     int64_t q_st[3], k_st[3], v_st[3];
-    const void *bias;             /* [buckets, H] contiguous */
+    const void *bias;             /* [buckets, H] contiguous; below -65536: the bucket's pairs are hidden */
     const int32_t *starts;        /* HOST: the first distance of each of n_starts buckets, not falling, */
     int64_t buckets, n_starts;    /*   from 0 to at most 1024; the last one has no end. n_starts <= 128. */
                                   /*   causal: buckets = n_starts; otherwise 2 n_starts, the upper half */
@@ -669,7 +669,7 @@ typedef struct mb_bias_attn {
     int64_t causal;               /* a query sees the keys j <= pos_i; keys behind the last query are */
                                   /*   not used, as those behind lengths */
     int64_t dtype, bias_dtype;    /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
-    double scale;
+    double scale;                 /* 1e-20 to 1e20 */
     void *o;                      /* [B, H, Lq, hd]: written by the forward, read by the backward */
     int64_t o_st[3];
     float *lse;                   /* [B, H, Lq] log2 of the softmax denominators, likewise (NULL: not wanted) */

@@ -70,7 +70,7 @@ def _rows16(x):
     size = x.element_size()
     if sd == 1 and not (x.data_ptr() | (sb | sh | sl) * size) & 15 and sl * size <= 1 << 24:
         return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _heads_last(B, H, L, hd, like):
@@ -205,8 +205,9 @@ def relative_bias_attention(q, k, v, bias, max_distance=128, causal=True, scale=
     ``causal``: a query sees the keys up to its position.  ``lengths``: an int32 / int64 tensor [B];
     keys from there on are not seen (values in 0 .. Lk; others are taken as the nearest of these).
     Rows of k and v behind these ends, and with ``causal`` behind the last query's position, may hold
-    anything; other values have to be finite.  A query that sees no key gets zeros, and passes on no
-    gradient.  ``scale``: 1 / sqrt(hd) by default.
+    anything; other values of q, k and v have to be finite.  A bias below -65536 (-inf, or its type's
+    lowest value) hides the pairs of its bucket.  A query that sees no key gets zeros, and passes on
+    no gradient.  ``scale``: 1 / sqrt(hd) by default, otherwise 1e-20 to 1e20.
 
     In bf16 the probabilities and the scores' gradients are rounded to bf16 for the products that
     they enter; all sums are in fp32.  Gradients come out the same each time."""

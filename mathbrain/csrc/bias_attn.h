@@ -127,8 +127,12 @@ __device__ inline void buckets_of(const Args& a, const int* d, int* bucket) {
     for (int i = 0; i < N; ++i) bucket[i] += !a.causal && d[i] < 0 ? a.n_starts : 0;
 }
 
+// A bias below -2^16 hides its pairs: were it kept, a row that has no others would get a denominator of
+// that size, next to which the backward's products lose the scores (at -1e9 p comes out at 2^100).
+constexpr float kHidden = -65536.f;
 __device__ inline float bias_at(const Args& a, int64_t at) {
-    return kLog2e * (a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at]);
+    const float v = a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at];
+    return v < kHidden ? -INFINITY : kLog2e * v;
 }
 
 // tab[i] = log2(e) bias of distance lo - kPad + i (clamped to lo .. hi), by all threads.

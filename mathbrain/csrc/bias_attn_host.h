@@ -8,13 +8,13 @@
 namespace mb {
 namespace battn {
 
-// A workgroup may use 160 KiB of LDS; beyond 64 KiB a kernel has to be told, once on each device.
-// `told` is the kernel's own.
+// A workgroup may use 160 KiB of LDS; beyond 64 KiB, of which a few are the kernels' static arrays, a
+// kernel has to be told, once on each device.  `told` is the kernel's own.
 struct Told {
     std::atomic<int> bytes[64] = {};
 };
 inline int allow_lds(const void* kernel, int bytes, Told& told) {
-    if (bytes <= 65536) return MB_OK;
+    if (bytes <= 61440) return MB_OK;
     if (bytes > 163840) return fail(MB_ERR_UNSUPPORTED, "mb_bias_attn: %d bytes of LDS are wanted, 163840 are there", bytes);
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -24,6 +24,8 @@ inline int allow_lds(const void* kernel, int bytes, Told& told) {
     if (dev < 64) told.bytes[dev].store(bytes, std::memory_order_relaxed);
     return MB_OK;
 }
+
+constexpr int kMostGroups = 0xffffff;   // of a launch, whose threads are counted in 32 bits
 
 inline bool rows16(const void* p, const int64_t* st, int dtype) {
     const int64_t size = dtype == MB_DTYPE_F32 ? 4 : 2;
@@ -41,7 +43,7 @@ inline bool rows16(const void* p, const int64_t* st, int dtype) {
 // 4096, 8 heads x 64: 27 us against 97).
 inline int splits_of(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
     const int64_t G = H / Hk, tiles = (G * Lq + 31) / 32, nq = ((int64_t)Lq + kRows - 1) / kRows;
-    if (G > 32 || (double)B * Hk * tiles > 0x7fffffff / 64) return 0;
+    if (G > 32 || (double)B * Hk * tiles > kMostGroups) return 0;
     if (G * Lq > 32) {
         // a causal mask leaves Lk - Lq / 2 of Lk keys where the last query sees them all
         const double share = causal && Lk > 0 ? 1.0 - 0.5 * (Lq < Lk ? Lq : Lk) / Lk : 1.0;
@@ -68,7 +70,7 @@ inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
         return fail(MB_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 32, 64, 128)", what, (long long)p->hd);
     MB_REQUIRE(p->dtype == MB_DTYPE_F32 || p->dtype == MB_DTYPE_BF16, "%s: dtype=%lld", what, (long long)p->dtype);
     MB_REQUIRE(p->bias_dtype == MB_DTYPE_F32 || p->bias_dtype == MB_DTYPE_BF16, "%s: bias_dtype=%lld", what, (long long)p->bias_dtype);
-    MB_REQUIRE(p->scale > 0 && p->scale < INFINITY, "%s: scale=%g", what, p->scale);
+    MB_REQUIRE(p->scale >= 1e-20 && p->scale <= 1e20, "%s: scale=%g (1e-20 to 1e20)", what, p->scale);
     MB_REQUIRE(p->starts && p->n_starts >= 1 && p->buckets == (p->causal ? p->n_starts : 2 * p->n_starts),
                "%s: %lld buckets for %lld first distances", what, (long long)p->buckets, (long long)p->n_starts);
     if (p->n_starts > kMaxStarts)
@@ -85,7 +87,7 @@ inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
                "%s: lengths and q_start hold integers of 4 or 8 bytes", what);
     MB_REQUIRE(p->q_start || (p->q_start0 >= -top && p->q_start0 <= top), "%s: q_start=%lld", what, (long long)p->q_start0);
     const int64_t nq = (p->Lq + kRows - 1) / kRows, nk = (p->Lk + kRows - 1) / kRows;
-    MB_REQUIRE((double)p->B * p->H * (nq > 0 ? nq : 1) <= 0x7fffffff && (double)p->B * p->Hk * nk + p->H <= 0x7fffffff,
+    MB_REQUIRE((double)p->B * p->H * (nq > 0 ? nq : 1) <= kMostGroups && (double)p->B * p->Hk * nk + p->H <= kMostGroups,
                "%s: B=%lld H=%lld Lq=%lld Lk=%lld are too many", what, (long long)p->B, (long long)p->H, (long long)p->Lq,
                (long long)p->Lk);
     const int dtype = (int)p->dtype;

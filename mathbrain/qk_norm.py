@@ -30,7 +30,7 @@ def _rows16(x):
     sb, sl, sh, sd = x.stride()
     if sd == 1 and not (x.data_ptr() | (sb | sl | sh) * x.element_size()) & 15:
         return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _weight(w):

@@ -229,6 +229,26 @@ def test_large_scores(t):
 
 
 @pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("low", ["-inf", "lowest", -1e9, -70000.0])
+@pytest.mark.parametrize("Lq,Lk,hd", [(200, 200, 64), (1, 700, 64), (150, 150, 128)])
+def test_biases_that_hide_their_buckets(Lq, Lk, hd, low, t):
+    """The buckets of far keys are hidden; the first sequence is short, and its last queries see none."""
+    from mathbrain.bias_attention import relative_bias_attention
+    q, k, v, bias, do = inputs(2, 4, 2, Lq, Lk, hd, t, 8, 5)
+    lengths = torch.tensor([20, Lk], device="cuda")
+    hidden = torch.tensor([0, 0, 0, 1, 0, 0, 0, 1], dtype=torch.bool)
+    bias[hidden.cuda()] = {"-inf": -math.inf, "lowest": torch.finfo(t).min}.get(low, low)
+    n, seen = plan(2, Lq, Lk, 8, 16, False, lengths, None)
+    seen = seen & ~hidden[n]
+    assert not seen[0, -1].any() and seen[1].any(-1).all()
+    want = definition(q, k, v, bias.masked_fill(hidden.cuda()[:, None], 0.0), do, n, seen, 1 / math.sqrt(hd), t)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, bias)]
+    o = relative_bias_attention(*leaves, max_distance=16, causal=False, lengths=lengths)
+    for x, w, name in zip([o, *torch.autograd.grad(o, leaves, do)], want, NAMES):
+        near(x, w, name)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
 def test_scale_and_bias_types(t):
     q, k, v, bias, do = inputs(2, 2, 2, 50, 50, 32, t, 32, 13)
     check(q, k, v, bias, do, scale=1.0)

@@ -87,10 +87,12 @@ def attn(first=(0, 1, 5), **fields):
     (dict(hd=96), "head_dim=96"), (dict(dtype=3), "dtype=3"), (dict(bias_dtype=-1), "bias_dtype=-1"), (dict(q=0), "null"),
     (dict(v=0), "null"), (dict(bias=0), "null"), (dict(Lq=-1), "Lq=-1"), (dict(Lk=(1 << 29) + 1), "Lk=536870913"),
     (dict(Hk=3), "multiple of Hk=3"), (dict(Hk=0), "Hk=0"), (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=1e-30), "scale=1e-30"), (dict(scale=1e30), "scale=1e+30"),
     (dict(starts=0), "first distances"), (dict(buckets=4), "4 buckets for 3"), (dict(causal=0), "3 buckets for 3"),
     (dict(lengths=P, lengths_bytes=2), "4 or 8 bytes"), (dict(q_start=P, q_start_bytes=1), "4 or 8 bytes"),
     (dict(q_start0=1 << 30), "q_start=1073741824"), (dict(q=P + 2), "16 bytes"), (dict(k2=513), "16 bytes"),
-    (dict(v2=-512), "elements apart"), (dict(q2=1 << 24), "elements apart"), (dict(B=1 << 20, H=1 << 12), "too many")])
+    (dict(v2=-512), "elements apart"), (dict(q2=1 << 24), "elements apart"), (dict(B=1 << 20, H=1 << 12), "too many"),
+    (dict(B=1 << 21), "too many")])
 def test_bias_attention_refusals(lib, bad, said):
     for name in ("mb_bias_attn_fwd", "mb_bias_attn_bwd"):
         assert getattr(lib, name)(attn(**bad), None) < 0
@@ -137,6 +139,15 @@ def test_bucket_starts():
     for n, reach in ((16, 9), (31, 200), (128, 1024)):
         starts = bucket_starts(n, reach)
         assert len(starts) == n and list(starts) == sorted(starts) and starts[-1] <= reach
+
+
+def test_rows_of_one_token_with_odd_strides_are_copied():
+    """A tensor may be contiguous by its sizes and have any strides where a size is 1."""
+    from mathbrain import bias_attention, qk_norm
+    x = torch.arange(200.0)[2:].as_strided((1, 1, 1, 64), (7, 5, 3, 1))
+    for rows16 in (bias_attention._rows16, qk_norm._rows16):
+        y = rows16(x)
+        assert y.data_ptr() % 16 == 0 and all(s % 4 == 0 for s in y.stride()[:3]) and torch.equal(x, y)
 
 
 def clip(lib, src, dst, n, codes=None, dcodes=None, max_norm=1.0, norm=P, ws=P, nbytes=1 << 30):
