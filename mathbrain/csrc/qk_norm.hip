@@ -19,6 +19,7 @@ namespace {
 constexpr int kQkThreads = 256;
 constexpr int kQkWaves = kQkThreads / 64;
 constexpr int kQkBwdBlocks = 1024;  // four workgroups per CU, each walking tokens
+constexpr int64_t kQkMost = 1 << 25;  // tokens of a forward launch, whose threads are counted in 32 bits
 
 typedef __attribute__((__ext_vector_type__(8))) __bf16 bf16x8v;
 
@@ -61,7 +62,7 @@ struct QkArgs {
     const float *wq, *wk, *cos, *sin;
     const void* start;                         // [B] int32 / int64 or NULL
     int64_t start0, table_rows;
-    int64_t tokens;
+    int64_t t0, tokens;                        // the launch's first token (forward), the end
     int start_bytes, L, H, Hk;
     float eps;
     void *q_out, *k_out;                       // [B, L, H, hd], [B, L, Hk, hd]
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_fwd_kernel(QkArgs a) {
     constexpr int RPW = 64 / LPR;   // rows of a wave's step
     const int lane = threadIdx.x & 63;
     const int chunk = lane % LPR;
-    const int64_t t = (int64_t)blockIdx.x * kQkWaves + (threadIdx.x >> 6);
+    const int64_t t = a.t0 + (int64_t)blockIdx.x * kQkWaves + (threadIdx.x >> 6);
     if (t >= a.tokens) return;
     const int64_t b = t / a.L, l = t - b * a.L;
     float c[N / 2], s[N / 2], wq[N], wk[N];
@@ -267,7 +268,6 @@ int fill(const char* what, const mb_qk_norm_rotary* p, QkArgs& a) {
         MB_REQUIRE(p->start0 >= 0 && p->start0 <= p->table_rows - p->L, "%s: positions %lld to %lld pass the table's %lld rows",
                    what, (long long)p->start0, (long long)(p->start0 + p->L), (long long)p->table_rows);
     a.tokens = p->B * p->L;
-    MB_REQUIRE((a.tokens + kQkWaves - 1) / kQkWaves <= top, "%s: %lld tokens are too many", what, (long long)a.tokens);
     if (a.tokens == 0) return MB_OK;
     MB_REQUIRE(p->q && p->k && p->wq && p->wk && p->cos && p->sin, "%s: null pointer argument", what);
     const int size = p->dtype == MB_DTYPE_F32 ? 4 : 2;
@@ -308,9 +308,11 @@ extern "C" int mb_qk_norm_rotary_fwd(const mb_qk_norm_rotary* p, void* stream) {
     MB_REQUIRE(p->q_out && p->k_out, "mb_qk_norm_rotary_fwd: null pointer argument");
     MB_REQUIRE((((uintptr_t)p->q_out | (uintptr_t)p->k_out) & 15) == 0, "mb_qk_norm_rotary_fwd: rows must begin at multiples of 16 bytes");
     a.q_out = p->q_out, a.k_out = p->k_out;
-    const dim3 grid((unsigned)((a.tokens + kQkWaves - 1) / kQkWaves));
-    if (p->dtype == MB_DTYPE_F32) launch_fwd<float>((int)p->hd, grid, (hipStream_t)stream, a);
-    else launch_fwd<__bf16>((int)p->hd, grid, (hipStream_t)stream, a);
+    for (; a.t0 < a.tokens; a.t0 += kQkMost) {
+        const dim3 grid((unsigned)((std::min(a.tokens - a.t0, kQkMost) + kQkWaves - 1) / kQkWaves));
+        if (p->dtype == MB_DTYPE_F32) launch_fwd<float>((int)p->hd, grid, (hipStream_t)stream, a);
+        else launch_fwd<__bf16>((int)p->hd, grid, (hipStream_t)stream, a);
+    }
     return check_launch("mb_qk_norm_rotary_fwd");
 }
 

@@ -112,6 +112,18 @@ def test_more_tokens_than_the_backward_has_waves():
     check(q, q, 0, 32, 13)
 
 
+def test_more_tokens_than_a_launch_takes():
+    from mathbrain.qk_norm import qk_norm_rotary
+    n = (1 << 25) + 5
+    cos, sin = (t.cuda() for t in tables(32, 1))
+    w = torch.rand(32, device="cuda")
+    q = torch.randn(n, 1, 1, 32, device="cuda", dtype=torch.bfloat16)
+    got = qk_norm_rotary(q, q, w, w, cos, sin)
+    for part in (slice(0, 9), slice(n - 9, n)):
+        for x, y in zip(got, qk_norm_rotary(q[part], q[part], w, w, cos, sin)):
+            assert torch.equal(x[part], y)
+
+
 def test_zero_rows_and_empty_batches():
     from mathbrain.qk_norm import qk_norm_rotary
     cos, sin = (t.cuda() for t in tables(64, 16))
