@@ -60,6 +60,8 @@ def _clip(src, codes, dst, dst_codes, max_norm, device):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     _lib.call_on(device, "mb_grad_clip", *at, n, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes)
+    if dst:
+        torch.autograd.graph.increment_version(dst)   # a graph that saved one of them says so in its backward
     return norm
 
 

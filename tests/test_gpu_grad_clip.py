@@ -209,6 +209,17 @@ def test_same_norm_each_time_streams_and_graphs():
         assert torch.equal(norm, want) and all(torch.equal(a, b) for a, b in zip(got, out)), i
 
 
+@pytest.mark.parametrize("out", [False, True])
+def test_a_graph_notices_that_what_it_saved_was_scaled(out):
+    from mathbrain.grad_clip import clip_gradients
+    x = torch.randn(50, device="cuda", requires_grad=True)
+    saved = torch.randn(50, device="cuda")
+    y = (x * saved).sum()
+    clip_gradients([torch.ones_like(saved)] if out else [saved], 0.1, out=[saved] if out else None)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_refusals():
     from mathbrain.grad_clip import clip_grad_norm_, clip_gradients, grad_norm
     x = torch.randn(4, 4, device="cuda")
