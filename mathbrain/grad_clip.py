@@ -34,27 +34,30 @@ def _dense(t):
 
 
 def _codes(tensors, device, what):
-    """The element types of the tensors, which have to be on one GPU (one of this library's types
-    each, dense).  Whole lists are compared, tensor by tensor only to name the one that fails: with
-    many small tensors the host's time is the call's (80 us for 86 tensors and as many outputs)."""
+    """(the tensors' element types, whether all are contiguous): they have to be on one GPU, of one of
+    this library's types each, dense.  Whole lists are compared, tensor by tensor only to name the one that fails: with
+    many small tensors the host's time is the call's."""
     codes = [_DTYPES.get(t.dtype, -1) for t in tensors]
-    layouts = [t.layout for t in tensors]
-    if -1 in codes or layouts.count(torch.strided) != len(layouts):
+    try:
+        contiguous = False not in list(map(torch.Tensor.is_contiguous, tensors))
+    except RuntimeError:    # some sparse layouts' answer; others say False
+        contiguous = False
+    if -1 in codes or not contiguous and any(t.layout is not torch.strided for t in tensors):
         t = next(t for t, c in zip(tensors, codes) if c < 0 or t.layout is not torch.strided)
         raise ValueError(f"{what}: a {t.layout} tensor of {t.dtype} (supported: dense float32 and bfloat16)")
     index = device.index if device.type == "cuda" else -2
-    if [t.get_device() for t in tensors].count(index) != len(codes):
+    if list(map(torch.Tensor.get_device, tensors)).count(index) != len(codes):
         _lib.require_gpu(torch.empty(0, device=device), *tensors, what=what)
-    return array.array("i", codes)
+    return array.array("i", codes), contiguous
 
 
 def _clip(src, codes, dst, dst_codes, max_norm, device):
     """The norm of src (element types: codes) as a 0-dim fp32 tensor; dst (None: no scaling) gets
     the scaled values."""
     n = len(src)
-    sizes = array.array("q", [t.numel() for t in src])
-    srcs = array.array("Q", [t.data_ptr() for t in src])
-    dsts = srcs if dst is src else dst and array.array("Q", [t.data_ptr() for t in dst])
+    sizes = array.array("q", map(torch.Tensor.numel, src))
+    srcs = array.array("Q", map(torch.Tensor.data_ptr, src))
+    dsts = srcs if dst is src else dst and array.array("Q", map(torch.Tensor.data_ptr, dst))
     at = [a and a.buffer_info()[0] for a in (srcs, codes, dsts, dst_codes, sizes)]
     nbytes = _lib.lib().mb_grad_clip_workspace(n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -72,8 +75,9 @@ def grad_norm(grads):
     if not grads:
         return torch.tensor(0.0)
     device = grads[0].device
-    codes = _codes(grads, device, "grad_norm")
-    return _clip([g if _dense(g) else g.contiguous() for g in grads], codes, None, None, math.inf, device)
+    codes, contiguous = _codes(grads, device, "grad_norm")
+    return _clip(grads if contiguous else [g if _dense(g) else g.contiguous() for g in grads], codes, None, None, math.inf,
+                 device)
 
 
 @torch.no_grad()
@@ -97,16 +101,15 @@ def clip_gradients(grads, max_norm, out=None):
     if not grads:
         return torch.tensor(0.0)
     device = grads[0].device
-    codes = _codes(grads, device, what)
-    contiguous = False not in [g.is_contiguous() for g in grads]
+    codes, contiguous = _codes(grads, device, what)
     if out is None:
         for g in () if contiguous else grads:
             if not _dense(g):
                 raise ValueError(f"{what}: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or "
                                  "shares its own elements, and cannot be scaled in place")
         return _clip(grads, codes, grads, codes, max_norm, device)
-    out_codes = _codes(out, device, what)
-    if [o.shape for o in out] != [g.shape for g in grads] or False in [o.is_contiguous() for o in out]:
+    out_codes, whole = _codes(out, device, what)
+    if not whole or False in list(map(torch.Tensor.is_same_size, out, grads)):
         g, o = next((g, o) for g, o in zip(grads, out) if o.shape != g.shape or not o.is_contiguous())
         raise ValueError(f"{what}: an output of shape {tuple(o.shape)}, strides {o.stride()} for a gradient "
                          f"of shape {tuple(g.shape)}: contiguous tensors of the same shape are wanted")

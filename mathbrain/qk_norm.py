@@ -33,6 +33,10 @@ def _rows16(x):
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def _like(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _weight(w):
     return w if w.dtype is torch.float32 and w.stride(0) == 1 else w.float().contiguous()
 
@@ -54,12 +58,9 @@ def qk_norm_rotary_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
                        cos: torch.Tensor, sin: torch.Tensor, eps: float, start_rows: Optional[torch.Tensor],
                        start: int) -> tuple[torch.Tensor, torch.Tensor]:
     """(q', k'), contiguous."""
-    dev = q.device
-    B, L, H, hd = q.shape
     q, k, wq, wk = _rows16(q), _rows16(k), _weight(q_weight), _weight(k_weight)
-    qo = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    _lib.call_on(dev, "mb_qk_norm_rotary_fwd",
+    qo, ko = _like(q), _like(k)
+    _lib.call_on(q.device, "mb_qk_norm_rotary_fwd",
                  _ARGS.pack(*_inputs(q, k, wq, wk, cos, sin, eps, start_rows, start), qo.data_ptr(), ko.data_ptr(),
                             *_NO_BACKWARD))
     return qo, ko
@@ -78,13 +79,10 @@ def qk_norm_rotary_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rotary_fwd for the output gradients."""
     dev = q.device
     B, L, H, hd = q.shape
-    q, k = _rows16(q.detach()), _rows16(k.detach())
-    gq, gk = (_rows16(g if g.dtype is q.dtype else g.to(q.dtype)) for g in (dq_out, dk_out))
-    wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
-    dq = torch.empty((B, L, H, hd), dtype=q.dtype, device=dev)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    dwq = torch.empty(hd, dtype=torch.float32, device=dev)
-    dwk = torch.empty(hd, dtype=torch.float32, device=dev)
+    q, k, wq, wk = _rows16(q), _rows16(k), _weight(q_weight), _weight(k_weight)
+    gq = _rows16(dq_out if dq_out.dtype is q.dtype else dq_out.to(q.dtype))
+    gk = _rows16(dk_out if dk_out.dtype is q.dtype else dk_out.to(q.dtype))
+    dq, dk, dwq, dwk = _like(q), _like(k), torch.empty_like(wq), torch.empty_like(wk)
     nbytes = _lib.workspace_bytes("mb_qk_norm_rotary_bwd_workspace", B, L, hd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "mb_qk_norm_rotary_bwd",

@@ -232,6 +232,9 @@ def test_refusals():
             clip_gradients([x], bad)
     with pytest.raises(ValueError, match="float16"):
         clip_gradients([x.half()], 1.0)
+    for layout in (torch.sparse_coo, torch.sparse_csr):
+        with pytest.raises(ValueError, match="dense float32"):
+            clip_gradients([x, x.to_sparse(layout=layout)], 1.0)
     with pytest.raises(ValueError, match="1 outputs for 2"):
         clip_gradients([x, x], 1.0, out=[x])
     with pytest.raises(ValueError, match="contiguous"):
