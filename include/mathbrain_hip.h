@@ -684,7 +684,7 @@ typedef struct mb_bias_attn {
 
 int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal);
 int mb_bias_attn_fwd(const mb_bias_attn *args, void *stream);
-int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets);
+int64_t mb_bias_attn_bwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal, int dtype, int buckets);
 int mb_bias_attn_bwd(const mb_bias_attn *args, void *stream);
 
 /*

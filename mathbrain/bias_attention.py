@@ -136,7 +136,8 @@ def bias_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     bias = bias.contiguous()
     dq, dk, dv = _heads_last(B, H, Lq, hd, q), _heads_last(B, Hk, Lk, hd, k), _heads_last(B, Hk, Lk, hd, v)
     dbias = torch.empty(bias.shape if want_dbias else (0,), dtype=bias.dtype, device=dev)
-    nbytes = _lib.workspace_bytes("mb_bias_attn_bwd_workspace", B, H, Lq, bias.shape[0])
+    nbytes = _lib.workspace_bytes("mb_bias_attn_bwd_workspace", B, H, Hk, Lq, Lk, hd, causal,
+                                  _DTYPES[q.dtype], bias.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "mb_bias_attn_bwd",
                  _ARGS.pack(*_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),

@@ -10,6 +10,7 @@
 #include "bias_attn_host.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace mb {
 namespace battn {
@@ -89,6 +90,8 @@ struct Diagonals {
 template <typename T, int HD>
 using QueryTile = Tile<T, HD, HD == 128 ? 32 : Ty<T>::kKeys>;
 
+// A workgroup takes 128 queries of a head and walks their keys, or one of q_parts equal runs of this
+// walk; bias_attn_add_q_kernel then adds what the runs found.
 // dbias: a block of pairs that lies within one bucket adds to a register, any other adds to its
 // distances' entries in LDS (Diagonals).  In the end the entries are added by buckets, into the
 // workgroup's own row of a workspace.
@@ -106,7 +109,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 
     const int lane = threadIdx.x & 63, wave = wave_id();
     int bh, qb;
-    place(blockIdx.x, a.B * a.H, a.nq, false, bh, qb);
+    place(blockIdx.x, a.B * a.H, a.nq * a.q_parts, false, bh, qb);
+    const int part = qb % a.q_parts;
+    qb /= a.q_parts;
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const int len = key_count(a, b), p0 = first_position(a, b);
     const int w0 = qb * kRows + wave * kWaveRows;
@@ -168,16 +173,16 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     const uint32_t lds = lds_address(smem);
     const typename Tl::Lane at;
     const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
-    // block(ktile, vtile, u, jb) for the wave's blocks of 32 keys from jb on, in rows 32 u of the tiles
-    auto walk = [&](auto&& block) {
+    // block(ktile, vtile, u, jb) for the wave's blocks of 32 keys from jb on, in rows 32 u of the tiles t0 .. t1 - 1
+    auto walk = [&](int t0, int t1, auto&& block) {
         auto load = [&](int t) {
             const uint32_t tile = lds + t % Tl::kStages * (2 * Tl::kBytes);
             Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
             Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
         };
-        if (tiles > 0)
-            for (int t = 0; t < Tl::kStages - 1; ++t) load(t);
-        for (int t = 0; t < tiles; ++t) {
+        if (t0 < t1)
+            for (int t = t0; t < t0 + Tl::kStages - 1; ++t) load(t);
+        for (int t = t0; t < t1; ++t) {
             wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
             load(t + Tl::kStages - 1);
             const uint32_t ktile = lds + t % Tl::kStages * (2 * Tl::kBytes), vtile = ktile + Tl::kBytes;
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     };
     loads_done();
     if (from_pairs) {
-        walk([&](uint32_t ktile, uint32_t vtile, int u, int jb) {
+        walk(0, tiles, [&](uint32_t ktile, uint32_t vtile, int u, int jb) {
             f32x16 x, y;
             products(ktile, vtile, u, jb, x, y);
 #pragma unroll
@@ -235,7 +240,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 #pragma unroll
             for (int r = 0; r < 16; ++r) y0[r] = -delta;
     }
-    walk([&](uint32_t ktile, uint32_t vtile, int u, int jb) {
+    walk((int)((int64_t)tiles * part / a.q_parts), (int)((int64_t)tiles * (part + 1) / a.q_parts),
+         [&](uint32_t ktile, uint32_t vtile, int u, int jb) {
         const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
         const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
         if (first_part && !above) {
@@ -281,7 +287,17 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     // A row's ds sum to zero but for delta's error, which comes from o's rounding and that of the
     // probabilities in it: for the keys' pass delta is put right by what is left.
     row_sum = half_sum(row_sum);
-    if (i < a.Lq) {
+    float far_lo = far_sum;
+    if (first_part) far_hi = far_lo, far_lo = 0.f, far_p_hi = far_p, far_p = 0.f;
+    if (i < a.Lq && a.q_parts > 1) {
+        const int64_t all = (int64_t)a.B * a.H * a.Lq, at = (int64_t)bh * a.Lq + i;
+        const float p_hi = half_sum(far_p_hi), p_lo = half_sum(far_p);
+        float* stat = a.q_stat + 4 * part * all + at;
+        if (lane < 32) stat[0] = row_sum, stat[all] = p_hi, stat[2 * all] = p_lo, stat[3 * all] = delta;
+        float* row = a.q_part + (part * all + at) * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) store_block<float>(row, 32 * d, dq[d], a.scale);
+    } else if (i < a.Lq) {
         if (lane < 32) a.rows[((int64_t)a.B * a.H + bh) * a.Lq + i] = -(delta + row_sum);
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
 #pragma unroll
@@ -289,11 +305,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     }
     if (!want_bias) return;
     diag.close(last_d0);
-    float far_lo = far_sum;
-    if (first_part) far_hi = far_lo, far_lo = 0.f, far_p_hi = far_p, far_p = 0.f;
     // delta's error again: what is left of a row's sum belongs to its pairs by their probability.  The
     // blocks of one bucket, which have most of it in long rows, are put right here.
-    if (sizeof(T) == 2) far_hi -= row_sum * far_p_hi, far_lo -= row_sum * far_p;
+    if (sizeof(T) == 2 && a.q_parts == 1) far_hi -= row_sum * far_p_hi, far_lo -= row_sum * far_p;
     far_hi = wave_sum(far_hi);
     far_lo = wave_sum(far_lo);
     if (lane == 0) far[wave][0] = far_hi, far[wave][1] = far_lo;
@@ -305,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         hist[n] = v;
     }
     __syncthreads();
-    float* part = a.dbias_part + ((int64_t)h * a.B * a.nq + (int64_t)b * a.nq + qb) * a.buckets;
+    float* sums = a.dbias_part + (h * a.bias_rows + ((int64_t)b * a.nq + qb) * a.q_parts + part) * a.buckets;
     for (int n = threadIdx.x / 8; n < a.buckets; n += kThreads / 8) {   // eight lanes a bucket
         const bool back = n >= a.n_starts;        // keys behind the query's position
         const int m = back ? n - a.n_starts : n;
@@ -328,13 +342,69 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
             if (end && !back) v += far[w][0];
             if (below) v += far[w][1];
         }
-        if ((lane & 7) == 0) part[n] = v;
+        if ((lane & 7) == 0) sums[n] = v;
+    }
+}
+
+// Where the queries' pass is split: dq and the rows' sums of ds from the runs', in order, and in bf16
+// what delta's error left in the blocks of one bucket, as a row of dbias's parts of its own.  A
+// workgroup takes 128 queries of a head.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) bias_attn_add_q_kernel(const Args a) {
+    __shared__ float left[kThreads / 64][2];
+    const int qb = blockIdx.x % a.nq, bh = blockIdx.x / a.nq, b = bh / a.H, h = bh % a.H;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t all = (int64_t)a.B * a.H * a.Lq, first = (int64_t)bh * a.Lq + (int64_t)qb * kRows;
+    const int rows = min(kRows, a.Lq - qb * kRows);
+    float hi = 0.f, lo = 0.f;
+    if ((int)threadIdx.x < rows) {
+        const float* stat = a.q_stat + first + threadIdx.x;
+        float sum = 0.f;
+        for (int s = 0; s < a.q_parts; ++s, stat += 4 * all) sum += stat[0], hi += stat[all], lo += stat[2 * all];
+        a.rows[all + first + threadIdx.x] = -(a.q_stat[3 * all + first + threadIdx.x] + sum);
+        hi *= sum, lo *= sum;
+    }
+    const bool correct = sizeof(T) == 2 && a.dbias_part;
+    if (correct) {
+        hi = wave_sum(hi), lo = wave_sum(lo);
+        if (lane == 0) left[wave][0] = hi, left[wave][1] = lo;
+        __syncthreads();
+        float* sums = a.dbias_part + (h * a.bias_rows + (int64_t)a.B * a.nq * a.q_parts + (int64_t)b * a.nq + qb) * a.buckets;
+        for (int n = threadIdx.x; n < a.buckets; n += kThreads) {
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kThreads / 64; ++w) {
+                if (n == a.n_starts - 1) v -= left[w][0];
+                if (n == (a.causal ? 0 : a.buckets - 1)) v -= left[w][1];
+            }
+            sums[n] = v;
+        }
+    }
+    for (int n = threadIdx.x; n < rows * (HD / 4); n += kThreads) {
+        const int r = n / (HD / 4), d = n % (HD / 4) * 4;
+        const float* p = a.q_part + (first + r) * HD + d;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < a.q_parts; s0 += 4) {   // four loads on their way together
+            f32x4 x[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                x[s] = zero;
+                if (s0 + s < a.q_parts) x[s] = *reinterpret_cast<const f32x4*>(p + (s0 + s) * all * HD);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) sum += x[s];
+        }
+        typename Ty<T>::Quad v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)sum[e];
+        *reinterpret_cast<typename Ty<T>::Quad*>((T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)(qb * kRows + r) * a.out_sl + d) = v;
     }
 }
 
 // dbias[n, h] = the sum of part[h, :, n], in a fixed order, by a workgroup: strips of rows.
 __device__ inline void add_parts(const Args& a, int h, float* sums) {
-    const int rows = a.B * a.nq;
+    const int rows = (int)a.bias_rows;
     const int strips = kThreads / a.buckets;   // at least one: buckets <= 256
     const int n = threadIdx.x % a.buckets, strip = threadIdx.x / a.buckets;
     const float* part = a.dbias_part + (int64_t)h * rows * a.buckets + n;
@@ -353,7 +423,9 @@ __device__ inline void add_parts(const Args& a, int h, float* sums) {
 static_assert(2 * kMaxStarts <= kThreads, "a thread for every bucket");
 
 // A workgroup takes 128 keys of one key head, 32 to a wave, and walks the queries of all query
-// heads that share it.  Where dbias is wanted, H workgroups before these add the queries' pass's parts of it.
+// heads that share it, or one of kv_parts equal runs of this walk; the runs' sums are then added by
+// bias_attn_add_kv_kernel.  Where dbias is wanted, H workgroups before these add the queries' pass's
+// parts of it.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bias_attn_dkv_kernel(const Args a) {
     using X = Ty<T>;
@@ -371,7 +443,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     }
     const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 5;
     int bh, kb;
-    place(id, a.B * a.Hk, nk, true, bh, kb);
+    place(id, a.B * a.Hk, nk * a.kv_parts, true, bh, kb);
+    const int part = kb % a.kv_parts;
+    kb /= a.kv_parts;
     const int b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
     const Reach reach(a);
     const int len = key_count(a, b), p0 = first_position(a, b);
@@ -380,6 +454,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     // queries from the first one that sees key k0
     const int first = a.causal ? max(0, k0 - p0) / QT : 0;
     const int tiles = k0 < len ? (a.Lq + QT - 1) / QT : 0;
+    const int steps = max(0, tiles - first);   // of a head
+    const int64_t step0 = (int64_t)group * steps * part / a.kv_parts, step1 = (int64_t)group * steps * (part + 1) / a.kv_parts;
     const float sl2 = a.scale * kLog2e;
 
     typename X::Frag kf[HD / 16], vf[HD / 16];
@@ -407,11 +483,14 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
             Tl::load(tile, qbase, a.q_sl, t * QT, a.Lq, qoff);
             Tl::load(tile + Tl::kBytes, gbase, a.do_sl, t * QT, a.Lq, goff);
         };
-        if (first >= tiles) break;
+        // the run's share of this head
+        const int64_t at0 = step0 - (int64_t)hh * steps, at1 = step1 - (int64_t)hh * steps;
+        const int t0 = first + (int)(at0 < 0 ? 0 : at0 < steps ? at0 : steps), t1 = first + (int)(at1 < 0 ? 0 : at1 < steps ? at1 : steps);
+        if (t0 >= t1) continue;
         fill_table(a, h, tab);   // the previous head's last barrier lies behind its reads
         loads_done();
-        for (int t = first; t < first + Tl::kStages - 1; ++t) load(t);
-        for (int t = first; t < tiles; ++t) {
+        for (int t = t0; t < t0 + Tl::kStages - 1; ++t) load(t);
+        for (int t = t0; t < t1; ++t) {
             const int s = t % Tl::kStages;
             // (two waves have a load more on their way: they wait for that one of the next tile too)
             wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();
@@ -485,7 +564,14 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         }
         wait_and_meet<0>();   // the next head's loads and table go where this one's were
     }
-    if (j < a.Lk) {
+    if (j < a.Lk && a.kv_parts > 1) {
+        float* row = a.kv_part + (((int64_t)part * a.B * a.Hk + bh) * a.Lk + j) * 2 * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+            store_block<float>(row, 32 * d, dk[d], a.scale);
+            store_block<float>(row + HD, 32 * d, dv[d], 1.f);
+        }
+    } else if (j < a.Lk) {
         T* krow = (T*)a.dk + b * a.dk_sb + hk * a.dk_sh + (int64_t)j * a.dk_sl;
         T* vrow = (T*)a.dv + b * a.dv_sb + hk * a.dv_sh + (int64_t)j * a.dv_sl;
 #pragma unroll
@@ -494,6 +580,34 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
             store_block<T>(vrow, 32 * d, dv[d], 1.f);
         }
     }
+}
+
+// dk and dv where the keys' pass is split: the runs' sums in order, four channels a thread.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) bias_attn_add_kv_kernel(const Args a) {
+    const int64_t rows = (int64_t)a.B * a.Hk * a.Lk, n = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (n >= rows * (HD / 2)) return;
+    const int64_t row = n / (HD / 2);
+    const int c = (int)(n % (HD / 2)) * 4, which = c / HD, d = c % HD;
+    const float* p = a.kv_part + row * 2 * HD + c;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < a.kv_parts; s0 += 4) {   // four loads on their way together
+        f32x4 x[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+            x[s] = zero;
+            if (s0 + s < a.kv_parts) x[s] = *reinterpret_cast<const f32x4*>(p + (s0 + s) * rows * 2 * HD);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) sum += x[s];
+    }
+    const int64_t bh = row / a.Lk, j = row - bh * a.Lk, b = bh / a.Hk, h = bh - b * a.Hk;
+    T* out = which ? (T*)a.dv + b * a.dv_sb + h * a.dv_sh + j * a.dv_sl : (T*)a.dk + b * a.dk_sb + h * a.dk_sh + j * a.dk_sl;
+    typename Ty<T>::Quad v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)sum[e];
+    *reinterpret_cast<typename Ty<T>::Quad*>(out + d) = v;
 }
 
 template <typename T, int HD>
@@ -505,18 +619,69 @@ int launch(const Args& a, hipStream_t st) {
     if (a.B > 0 && a.Lq > 0) {
         static Told told;
         if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q, told)) return rc;
-        hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), lds_q, st, a);
+        hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq * a.q_parts)), dim3(kThreads), lds_q, st, a);
+        if (a.q_parts > 1)
+            hipLaunchKernelGGL((bias_attn_add_q_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), 0, st, a);
     }
-    const int nk = (a.Lk + kRows - 1) / kRows, blocks = a.B * a.Hk * nk + (a.dbias ? a.H : 0);
+    const int nk = (a.Lk + kRows - 1) / kRows, blocks = a.B * a.Hk * nk * a.kv_parts + (a.dbias ? a.H : 0);
     if (blocks > 0) {
         static Told told;
         if (const int rc = allow_lds((const void*)bias_attn_dkv_kernel<T, HD>, base, told)) return rc;
         hipLaunchKernelGGL((bias_attn_dkv_kernel<T, HD>), dim3((unsigned)blocks), dim3(kThreads), base, st, a);
     }
+    if (a.kv_parts > 1) {
+        const int64_t threads = (int64_t)a.B * a.Hk * a.Lk * (HD / 2);
+        hipLaunchKernelGGL((bias_attn_add_kv_kernel<T, HD>), dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
+                           st, a);
+    }
     return check_launch("mb_bias_attn_bwd");
 }
 
 int64_t padded(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
+
+// Runs that a pass splits each walk into, for `groups` workgroups of `steps` 64-row tiles each: where
+// there are few, most of the device would wait for the longest.  The time is counted in tiles: a run's
+// own start and end, that of the launch which adds the runs, and what two workgroups of a CU take
+// from each other.  Measured, split against not, dq / dk and dv, launches that add included:
+// causal bf16 heads of 64, 2 x 1310, 8 heads (176 workgroups, 21 tiles) 36 us against 44 / 31 against
+// 39; 9 x 2259, one head 44 against 67 / 39 against 62; heads of 128, 2 x 1516, 4 heads on 2 key
+// heads 55 against 74 / 46 against 131; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key
+// heads 209 against 254 / 245 against 1180.
+int parts_of(int64_t groups, int64_t steps, int per_cu, bool causal, int dtype) {
+    if (groups < 1 || groups > 512) return 1;
+    const double start = dtype == MB_DTYPE_F32 ? 1.5 : 4.0, join = 1.2 * start;
+    int best = 1;
+    double least = INFINITY;
+    for (int n = 1; n <= 8 && (n == 1 || n <= steps / 2); ++n) {
+        const double wgs = (causal ? 0.95 : 1.0) * groups * n;
+        const double cost = std::ceil(wgs / (256 * per_cu)) * ((double)steps / n + start) * (wgs > 256 && per_cu == 2 ? 1.6 : 1.0)
+                            + (n > 1 ? join : 0.0);
+        if (cost < least) least = cost, best = n;
+    }
+    // the longest walk is twice the mean under a causal mask (3 x 3461, 5 heads of 32, 420 workgroups of 55 tiles: 64 us
+    // against 91 / 56 against 73; but 448 of 16 tiles: 52 against 42 / 50 against 37)
+    if (best == 1 && causal && per_cu == 2 && groups > 256 && steps >= 24) best = 2;
+    return best;
+}
+
+// The workspace's parts in floats: the rows' statistics, dbias's sums (and how many for each bucket and
+// head), and what the passes' runs find where they are split.
+struct Space {
+    int q_parts, kv_parts;
+    int64_t bias_rows, rows, bias, q, q_stat, kv;
+    Space(int B, int H, int Hk, int Lq, int Lk, int hd, bool causal, int dtype, int buckets) {
+        const int64_t all = (int64_t)B * H * Lq, nq = ((int64_t)Lq + kRows - 1) / kRows, nk = ((int64_t)Lk + kRows - 1) / kRows;
+        q_parts = parts_of(B * H * nq, ((int64_t)Lk + 63) / 64, dtype == MB_DTYPE_F32 && hd == 128 ? 1 : 2, causal, dtype);
+        kv_parts = parts_of(B * Hk * nk, (int64_t)(H / Hk) * (((int64_t)Lq + 63) / 64), hd == 128 ? 1 : 2, causal, dtype);
+        bias_rows = B * nq * (q_parts > 1 ? q_parts + 1 : 1);
+        rows = padded(2 * all);
+        bias = padded(H * bias_rows * buckets);
+        q = q_parts > 1 ? q_parts * all * hd : 0;
+        q_stat = q_parts > 1 ? padded(4 * q_parts * all) : 0;
+        kv = kv_parts > 1 ? (int64_t)kv_parts * B * Hk * Lk * 2 * hd : 0;
+    }
+    int64_t floats() const { return rows + bias + q + q_stat + kv; }
+};
 
 }  // namespace
 }  // namespace battn
@@ -525,17 +690,16 @@ int64_t padded(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
 using namespace mb;
 using namespace mb::battn;
 
-extern "C" int64_t mb_bias_attn_bwd_workspace(int B, int H, int Lq, int buckets) {
-    if (B < 1 || H < 1 || Lq < 1 || buckets < 1) return 0;
-    const int64_t nq = ((int64_t)Lq + kRows - 1) / kRows;
-    return (padded(2 * (int64_t)B * H * Lq) + (int64_t)H * B * nq * buckets) * (int64_t)sizeof(float);
+extern "C" int64_t mb_bias_attn_bwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal, int dtype, int buckets) {
+    if (B < 1 || H < 1 || Hk < 1 || H % Hk || Lq < 1 || Lk < 0 || hd < 1 || buckets < 1) return 0;
+    return Space(B, H, Hk, Lq, Lk, hd, causal != 0, dtype, buckets).floats() * (int64_t)sizeof(float);
 }
 
 extern "C" int mb_bias_attn_bwd(const mb_bias_attn* p, void* stream) {
     Args a = {};
     if (const int rc = fill_args("mb_bias_attn_bwd", p, a)) return rc;
     const int hd = (int)p->hd, dtype = (int)p->dtype;
-    const int64_t need = mb_bias_attn_bwd_workspace(a.B, a.H, a.Lq, a.buckets);
+    const int64_t need = mb_bias_attn_bwd_workspace(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal, dtype, a.buckets);
     if (need > 0 && (!p->workspace || p->workspace_bytes < need))
         return fail(MB_ERR_WORKSPACE, "mb_bias_attn_bwd: workspace of %lld bytes, %lld are needed",
                     (long long)p->workspace_bytes, (long long)need);
@@ -556,9 +720,18 @@ extern "C" int mb_bias_attn_bwd(const mb_bias_attn* p, void* stream) {
         a.dv = p->dv, a.dv_sb = p->dv_st[0], a.dv_sh = p->dv_st[1], a.dv_sl = p->dv_st[2];
     }
     a.lse = p->lse;
-    a.rows = (float*)p->workspace;
     a.dbias = p->dbias;
-    a.dbias_part = p->dbias && need > 0 ? (float*)p->workspace + padded(2 * (int64_t)a.B * a.H * a.Lq) : nullptr;
+    a.q_parts = a.kv_parts = 1;
+    if (need > 0) {
+        const Space w(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal, dtype, a.buckets);
+        a.q_parts = w.q_parts, a.kv_parts = w.kv_parts;
+        a.bias_rows = dtype == MB_DTYPE_F32 && w.q_parts > 1 ? w.bias_rows / (w.q_parts + 1) * w.q_parts : w.bias_rows;
+        a.rows = (float*)p->workspace;
+        a.dbias_part = p->dbias ? a.rows + w.rows : nullptr;
+        a.q_part = a.rows + w.rows + w.bias;
+        a.q_stat = a.q_part + w.q;
+        a.kv_part = a.q_stat + w.q_stat;
+    }
     hipStream_t st = (hipStream_t)stream;
     return dtype == MB_DTYPE_F32
                ? (hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st))

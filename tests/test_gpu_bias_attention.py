@@ -135,6 +135,24 @@ def test_matches_the_definition(size, hd, t, causal):
     check(*inputs(*size, hd, t, 32, sum(size) + hd), causal=causal)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("size", [(1, 4, 2, 700, 700), (2, 2, 1, 300, 1100), (1, 2, 2, 1500, 90), (2, 3, 1, 1, 1000)])
+def test_walks_that_the_backward_splits(size, hd, t, causal):
+    from mathbrain.bias_attention import relative_bias_attention
+    q, k, v, bias, do = inputs(*size, hd, t, 32, sum(size) + hd)
+    lengths = None if size[0] == 1 else torch.tensor([size[4], size[4] // 3], device="cuda")
+    got = check(q, k, v, bias, do, causal=causal, lengths=lengths)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, bias.detach())]
+    o = relative_bias_attention(*leaves[:3], bias, causal=causal, lengths=lengths)      # no gradient of the bias
+    for x, y in zip(torch.autograd.grad(o, leaves[:3], do), got[1:]):
+        assert torch.equal(x, y)
+    o = relative_bias_attention(*leaves, causal=causal, lengths=lengths)
+    for x, y in zip(torch.autograd.grad(o, leaves, do), got[1:]):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("buckets,reach,causal", [(1, 1, True), (2, 9, True), (3, 100, True), (31, 200, True),
                                                   (128, 1024, True), (16, 9, True), (2, 1, False), (6, 2, False),
@@ -337,6 +355,34 @@ def test_captured_and_replayed(Lq, Lk):
         want = once()
         torch.cuda.synchronize()
         assert torch.equal(o, want), i
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("L", [100, 1200])
+def test_both_directions_captured_and_replayed(L, t):
+    from mathbrain.bias_attention import bias_attn_bwd, bias_attn_fwd
+    q, k, v, bias, do = inputs(1, 4, 2, L, L, 64, t, 32, 31)
+    rest = (128, True, 0.125, None, None, 0)
+
+    def once():
+        o, lse = bias_attn_fwd(q, k, v, bias, *rest, True)
+        return o, *bias_attn_bwd(q, k, v, bias, o, do, lse, *rest, True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    for i in range(4):
+        for x in (q, v, do, bias):
+            x.copy_(torch.randn_like(x))
+        graph.replay()
+        want = once()
+        torch.cuda.synchronize()
+        for x, y, name in zip(got, want, NAMES):
+            assert torch.equal(x, y), (i, name)
 
 
 def test_differences_agree_with_the_gradient():

@@ -126,8 +126,11 @@ def test_bias_attention_workspaces(lib):
     assert size(16, 8, 8, 1, 4096, 64, 1) > 0 and size(16, 8, 8, 1, 100, 64, 1) == 0
     assert size(0, 8, 8, 1, 4096, 64, 1) == 0 and size(1, 8, 3, 1, 4096, 64, 1) == 0
     assert size(1 << 30, 1 << 30, 1, 1 << 30, 1 << 30, 64, 1) == 0  # no overflow on the way to "no"
-    assert lib.mb_bias_attn_bwd_workspace(2, 8, 100, 32) == (2 * 2 * 8 * 100 + 8 * 2 * 32) * 4
-    assert lib.mb_bias_attn_bwd_workspace(2, 8, 0, 32) == 0
+    size = lib.mb_bias_attn_bwd_workspace
+    assert size(2, 8, 8, 100, 100, 64, 1, 1, 32) == (2 * 2 * 8 * 100 + 8 * 2 * 32) * 4
+    assert size(2, 8, 8, 0, 100, 64, 1, 1, 32) == 0 and size(1, 8, 3, 5, 5, 64, 1, 1, 32) == 0
+    # few blocks of long walks: the runs that they are split into
+    assert size(1, 8, 2, 1000, 1000, 64, 1, 1, 32) > (2 * 8 * 1000 + 8 * 8 * 32) * 4 + 2 * 8 * 1000 * 64 * 4
 
 
 def test_bucket_starts():
