@@ -41,10 +41,26 @@ __device__ inline float wave_sum(float v) {
 // this kernel at 56 x 512 tokens, 8 heads x 64.
 struct Diagonals {
     static constexpr int kStride = 36;
+    typedef __attribute__((address_space(3))) const float lds_float;
     float* block;    // the wave's [32][kStride]
     float* sums;     // the wave's entry of distance 0 + lane % 32
+    // of this lane's 16 values: where they lie in LDS, and 1 where the value is of distance t (0: t - 32)
+    uint32_t at[16];
+    float here[16];
     float carry = 0.f;
     bool open = false;
+
+    __device__ void start(float* block_, float* sums_) {
+        const int lane = threadIdx.x & 63, t = lane & 31, g = lane >> 5;
+        block = block_;
+        sums = sums_ + t;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int i = 16 * g + k;
+            at[k] = lds_address(block + i * kStride + ((i - t) & 31));
+            here[k] = i >= t ? 1.f : 0.f;
+        }
+    }
 
     // The block into LDS; take() follows, with the products that need the block between them.
     __device__ void give(const f32x16& x) {
@@ -58,18 +74,17 @@ struct Diagonals {
         __builtin_amdgcn_wave_barrier();
     }
     __device__ void take(int d0) {
-        const int lane = threadIdx.x & 63, t = lane & 31, g = lane >> 5;
-        float here = carry, next = 0.f;
+        const int t = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
+        float mine = carry, next = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-            const int i = 16 * g + k;
-            const float v = block[i * kStride + ((i - t) & 31)];
-            here += i >= t ? v : 0.f;
-            next += i >= t ? 0.f : v;
+            const float v = *(lds_float*)(uintptr_t)at[k];
+            mine = __builtin_fmaf(v, here[k], mine);
+            next += 16 * g + k >= t ? 0.f : v;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        put(d0, here);
+        put(d0, mine);
         carry = next;
         open = true;
     }
@@ -159,8 +174,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     if (want_bias)
         for (int n = threadIdx.x; n < 4 * entries; n += kThreads) hist[n] = 0.f;
     Diagonals diag;
-    diag.block = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride;
-    diag.sums = hist + wave * entries + kPad - reach.lo + (lane & 31);
+    if (want_bias)
+        diag.start(reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes) + ((5 * entries + 3) & ~3) + wave * 32 * Diagonals::kStride,
+                   hist + wave * entries + kPad - reach.lo);
     // Keys go up, so the blocks at or above the reach come first, those at or below its lower end last.
     float far_hi = 0.f, far_sum = 0.f, row_sum = 0.f;
     float far_p_hi = 0.f, far_p = 0.f;   // the blocks' probabilities
