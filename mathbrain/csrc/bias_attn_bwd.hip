@@ -150,16 +150,31 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     // walk of its own (64 sequences of 3 tokens, heads of 64: dbias off by 5e-3 of its norm with dO . o).
     const bool from_pairs = sizeof(T) == 2 && kend <= kRows;
     float delta = 0.f;
+    const uint32_t lds = lds_address(smem);
+    const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
+    auto load = [&](int t) {
+        const uint32_t tile = lds + t % Tl::kStages * (2 * Tl::kBytes);
+        Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
+        Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
+    };
+    // the first of the tiles t0 .. t1 - 1
+    auto begin = [&](int t0, int t1) {
+        if (t0 < t1)
+            for (int t = t0; t < t0 + Tl::kStages - 1; ++t) load(t);
+    };
+    const int run0 = (int)((int64_t)tiles * part / a.q_parts), run1 = (int)((int64_t)tiles * (part + 1) / a.q_parts);
     if (!from_pairs) {
         typename X::Frag of[HD / 16];
         load_frags<T, HD>((const T*)a.o + b * a.o_sb + h * a.o_sh, a.o_sl, w0, a.Lq, of);
-        fill_table(a, h, tab);
+        begin(run0, run1);
+        fill_table(a, h, tab);   // while all of these are on their way
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)of[c][e], (float)gf[c][e], delta);
         delta = half_sum(delta);
     } else {
+        begin(0, tiles);
         fill_table(a, h, tab);
     }
     // In bf16 with heads of 64 the products' results start from -lse (in units of the scores) and
@@ -186,18 +201,10 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     f32x16 dq[HD / 32];
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d) dq[d] = zero16();
-    const uint32_t lds = lds_address(smem);
     const typename Tl::Lane at;
-    const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
-    // block(ktile, vtile, u, jb) for the wave's blocks of 32 keys from jb on, in rows 32 u of the tiles t0 .. t1 - 1
+    // block(ktile, vtile, u, jb) for the wave's blocks of 32 keys from jb on, in rows 32 u of the tiles
+    // t0 .. t1 - 1, whose first are on their way
     auto walk = [&](int t0, int t1, auto&& block) {
-        auto load = [&](int t) {
-            const uint32_t tile = lds + t % Tl::kStages * (2 * Tl::kBytes);
-            Tl::load(tile, kbase, a.k_sl, t * KT, len, koff);
-            Tl::load(tile + Tl::kBytes, vbase, a.v_sl, t * KT, len, voff);
-        };
-        if (t0 < t1)
-            for (int t = t0; t < t0 + Tl::kStages - 1; ++t) load(t);
         for (int t = t0; t < t1; ++t) {
             wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();   // as in the forward
             load(t + Tl::kStages - 1);
@@ -251,13 +258,13 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
 #pragma unroll
             for (int r = 0; r < 16; ++r) delta = __builtin_fmaf(__builtin_amdgcn_exp2f(kStart ? x[r] : x[r] - lse), y[r], delta);
         });
+        begin(run0, run1);
         delta = half_sum(delta);
         if (kStart)
 #pragma unroll
             for (int r = 0; r < 16; ++r) y0[r] = -delta;
     }
-    walk((int)((int64_t)tiles * part / a.q_parts), (int)((int64_t)tiles * (part + 1) / a.q_parts),
-         [&](uint32_t ktile, uint32_t vtile, int u, int jb) {
+    walk(run0, run1, [&](uint32_t ktile, uint32_t vtile, int u, int jb) {
         const int dlo = p0 + w0 - jb - 31, dhi = p0 + w0 + 31 - jb;
         const bool above = dlo >= reach.hi, one = above || dhi <= reach.lo;
         if (first_part && !above) {
@@ -503,9 +510,10 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         const int64_t at0 = step0 - (int64_t)hh * steps, at1 = step1 - (int64_t)hh * steps;
         const int t0 = first + (int)(at0 < 0 ? 0 : at0 < steps ? at0 : steps), t1 = first + (int)(at1 < 0 ? 0 : at1 < steps ? at1 : steps);
         if (t0 >= t1) continue;
-        fill_table(a, h, tab);   // the previous head's last barrier lies behind its reads
-        loads_done();
+        // the previous head's last barrier lies behind its reads
         for (int t = t0; t < t0 + Tl::kStages - 1; ++t) load(t);
+        fill_table(a, h, tab);   // while these are on their way
+        loads_done();
         for (int t = t0; t < t1; ++t) {
             const int s = t % Tl::kStages;
             // (two waves have a load more on their way: they wait for that one of the next tile too)

@@ -40,7 +40,6 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
     const T* vbase = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     typename X::Frag qf[HD / 16];
     load_frags<T, HD>((const T*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, w0, a.Lq, qf);
-    fill_table(a, h, tab);
 
     f32x16 o[HD / 32];
 #pragma unroll
@@ -56,9 +55,10 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
         Tl::load(tile, kbase, a.k_sl, j0, len, koff);
         Tl::load(tile + Tl::kBytes, vbase, a.v_sl, j0, len, voff);
     };
-    loads_done();
     if (tiles > 0)
         for (int n = 0; n < Tl::kStages - 1; ++n) load(n);
+    fill_table(a, h, tab);   // while the first tiles are on their way
+    loads_done();
     for (int n = 0; n * SETS < tiles; ++n) {
         // the n-th tiles are there, and nobody reads those before them any longer
         wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();
