@@ -658,7 +658,7 @@ typedef struct mb_bias_attn {
     int64_t q_st[3], k_st[3], v_st[3];
     const void *bias;             /* [buckets, H] contiguous; below -65536: the bucket's pairs are hidden */
     const int32_t *starts;        /* HOST: the first distance of each of n_starts buckets, not falling, */
-    int64_t buckets, n_starts;    /*   from 0 to at most 1024; the last one has no end. n_starts <= 128. */
+    int64_t buckets, n_starts;    /*   from one 0 to at most 1024; the last has no end. n_starts <= 128. */
                                   /*   causal: buckets = n_starts; otherwise 2 n_starts, the upper half */
                                   /*   for keys behind the query (distance j - pos_i >= 1) */
     const void *lengths;          /* [B] keys that count, or NULL: Lk. Rows of k and v from there on */

@@ -21,6 +21,8 @@ constexpr int kThreads = 256;   // four waves
 constexpr int kWaveRows = 32;   // queries (or keys) of a wave
 constexpr int kRows = 4 * kWaveRows;
 constexpr int kMaxStarts = 128;
+constexpr int kStartStep = 16;  // starts[] is filled up to a multiple of it with distances that none reaches
+static_assert(kMaxStarts % kStartStep == 0, "");
 constexpr int kMaxReach = 1024; // the largest distance with a bucket of its own
 constexpr int kPad = 96;        // table entries beyond each end: a 32 x 64 tile's distances that pass it
 constexpr float kLog2e = 1.4426950408889634f;
@@ -121,12 +123,13 @@ __device__ inline void buckets_of(const Args& a, const int* d, int* bucket) {
     int n[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) n[i] = d[i] < 0 ? -d[i] : d[i], bucket[i] = -1;
-#pragma unroll 8
-    for (int k = 0; k < a.n_starts; ++k) {
-        const int first = a.starts[k];
+    for (int k0 = 0; k0 < a.n_starts; k0 += kStartStep)
 #pragma unroll
-        for (int i = 0; i < N; ++i) bucket[i] += first <= n[i] ? 1 : 0;
-    }
+        for (int k = 0; k < kStartStep; ++k) {
+            const int first = a.starts[k0 + k];
+#pragma unroll
+            for (int i = 0; i < N; ++i) bucket[i] += first <= n[i] ? 1 : 0;
+        }
 #pragma unroll
     for (int i = 0; i < N; ++i) bucket[i] += !a.causal && d[i] < 0 ? a.n_starts : 0;
 }

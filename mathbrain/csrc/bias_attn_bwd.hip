@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     using Tl = QueryTile<T, HD>;
     constexpr int KT = Tl::kN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ float far[4][2];
     const Reach reach(a);
     const int entries = reach.entries();
     float* tab = reinterpret_cast<float*>(smem + 2 * Tl::kStages * Tl::kBytes);
@@ -162,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
         if (t0 < t1)
             for (int t = t0; t < t0 + Tl::kStages - 1; ++t) load(t);
     };
-    const int run0 = (int)((int64_t)tiles * part / a.q_parts), run1 = (int)((int64_t)tiles * (part + 1) / a.q_parts);
+    // (at most 2^24 tiles and 8 parts)
+    const int run0 = (int)((uint32_t)(tiles * part) / (uint32_t)a.q_parts), run1 = (int)((uint32_t)(tiles * (part + 1)) / (uint32_t)a.q_parts);
     if (!from_pairs) {
         typename X::Frag of[HD / 16];
         load_frags<T, HD>((const T*)a.o + b * a.o_sb + h * a.o_sh, a.o_sl, w0, a.Lq, of);
@@ -331,40 +331,36 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn
     // delta's error again: what is left of a row's sum belongs to its pairs by their probability.  The
     // blocks of one bucket, which have most of it in long rows, are put right here.
     if (sizeof(T) == 2 && a.q_parts == 1) far_hi -= row_sum * far_p_hi, far_lo -= row_sum * far_p;
-    far_hi = wave_sum(far_hi);
-    far_lo = wave_sum(far_lo);
-    if (lane == 0) far[wave][0] = far_hi, far[wave][1] = far_lo;
-    __syncthreads();
-    for (int n = threadIdx.x; n < entries; n += kThreads) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) v += hist[w * entries + n];
-        hist[n] = v;
-    }
+    // The whole blocks' sums go where no diagonal reaches: the padding's 63rd entries and on.
+    far_hi = half_sum(far_hi);
+    far_lo = half_sum(far_lo);
+    if (lane < 32) diag.sums[reach.hi + 63] = far_hi, diag.sums[reach.lo - 94] = far_lo;
     __syncthreads();
     float* sums = a.dbias_part + (h * a.bias_rows + ((int64_t)b * a.nq + qb) * a.q_parts + part) * a.buckets;
     for (int n = threadIdx.x / 8; n < a.buckets; n += kThreads / 8) {   // eight lanes a bucket
         const bool back = n >= a.n_starts;        // keys behind the query's position
         const int m = back ? n - a.n_starts : n;
         const bool end = m == a.n_starts - 1;
-        // its distances' entries, those of the padding with the last bucket's
+        // its distances' entries, those of the padding with the last bucket's (and, in a causal table,
+        // the first one's: a whole block at or below distance 0 has nothing else that counts)
         int e0 = a.starts[m], e1 = end ? reach.hi + kPad : a.starts[m + 1] - 1;
         if (back) {
             const int near = max(e0, 1);
             e0 = -e1, e1 = -near;
+        } else if (a.causal && n == 0) {
+            e0 = -kPad;
         }
+        e0 += kPad - reach.lo, e1 += kPad - reach.lo;
         float v = 0.f;
-        for (int e = e0 - reach.lo + kPad + (lane & 7); e <= e1 - reach.lo + kPad; e += 8) v += hist[e];
+        for (int e = e0 + (lane & 7); e <= e1; e += 16) {
+            const int next = e + 8 <= e1 ? e + 8 : e;
+            float x = 0.f, y = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x += hist[w * entries + e], y += hist[w * entries + next];
+            v += next > e ? x + y : x;
+        }
 #pragma unroll
         for (int o = 4; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-        // whole blocks: at or above the reach, and at or below its lower end, which is distance 0 in
-        // a causal table
-        const bool below = a.causal ? n == 0 : back && end;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            if (end && !back) v += far[w][0];
-            if (below) v += far[w][1];
-        }
         if ((lane & 7) == 0) sums[n] = v;
     }
 }
@@ -478,7 +474,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     const int first = a.causal ? max(0, k0 - p0) / QT : 0;
     const int tiles = k0 < len ? (a.Lq + QT - 1) / QT : 0;
     const int steps = max(0, tiles - first);   // of a head
-    const int64_t step0 = (int64_t)group * steps * part / a.kv_parts, step1 = (int64_t)group * steps * (part + 1) / a.kv_parts;
+    const bool whole = a.kv_parts == 1;
+    const int64_t all = (int64_t)group * steps, step0 = whole ? 0 : all * part / a.kv_parts, step1 = whole ? all : all * (part + 1) / a.kv_parts;
     const float sl2 = a.scale * kLog2e;
 
     typename X::Frag kf[HD / 16], vf[HD / 16];

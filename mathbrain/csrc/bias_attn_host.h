@@ -79,7 +79,7 @@ inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
     const int n_starts = (int)p->n_starts;
     MB_REQUIRE(starts[0] == 0, "%s: the first bucket begins at distance %d, not at 0", what, starts[0]);
     for (int i = 1; i < n_starts; ++i)
-        MB_REQUIRE(starts[i] >= starts[i - 1], "%s: first distances must not fall", what);
+        MB_REQUIRE(starts[i] >= starts[i - 1] && starts[i] > 0, "%s: first distances must not fall, and one alone is 0", what);
     if (starts[n_starts - 1] > kMaxReach)
         return fail(MB_ERR_UNSUPPORTED, "%s: the last bucket begins at distance %d (at most %d)", what, starts[n_starts - 1], kMaxReach);
     MB_REQUIRE((!p->lengths || p->lengths_bytes == 4 || p->lengths_bytes == 8)
@@ -113,7 +113,7 @@ inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {
     a.causal = p->causal != 0, a.bias_bf16 = p->bias_dtype == MB_DTYPE_BF16, a.buckets = (int)p->buckets, a.n_starts = n_starts;
     a.reach = starts[n_starts - 1];
     a.scale = (float)p->scale;
-    for (int i = 0; i < n_starts; ++i) a.starts[i] = starts[i];
+    for (int i = 0; i < kMaxStarts; ++i) a.starts[i] = i < n_starts ? starts[i] : 0x7fffffff;
     return MB_OK;
 }
 

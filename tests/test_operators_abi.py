@@ -99,7 +99,7 @@ def test_bias_attention_refusals(lib, bad, said):
         assert said in message(lib) and name in message(lib)
 
 
-@pytest.mark.parametrize("starts,said", [((1, 2), "distance 1, not at 0"), ((0, 5, 4), "must not fall"),
+@pytest.mark.parametrize("starts,said", [((1, 2), "distance 1, not at 0"), ((0, 5, 4), "must not fall"), ((0, 0, 4), "one alone is 0"),
                                          ((0, 1025), "distance 1025"), (tuple(range(129)), "129 buckets")])
 def test_bias_attention_bucket_refusals(lib, starts, said):
     assert lib.mb_bias_attn_fwd(attn(starts), None) < 0 and said in message(lib)
