@@ -68,9 +68,10 @@ struct Ty<float> {
 // Waves of a SIMD that the registers have to be enough for.  Two (at most 256 registers) keep the
 // matrix instructions' results in VGPRs, where the softmax reads them; with one, the compiler puts
 // them into AGPRs and moves each of them (forward at 4 x 4096, 8 heads x 64: 279 us instead of
-// 131).  Heads of 128 do not fit that way in fp32, nor, with two results (`wide`), in bf16.
+// 131; in fp32 at 8 x 1000, 8 heads x 128: 178 instead of 238).  Heads of 128 do not fit that way with
+// two results (`wide`), nor, in fp32, in the queries' pass (178 spills).
 template <typename T, int HD, bool WIDE = false>
-constexpr int waves_per_simd() { return HD == 128 && (WIDE || sizeof(T) == 4) ? 1 : 2; }
+constexpr int waves_per_simd() { return HD == 128 && WIDE ? 1 : 2; }
 
 struct Args {
     const void *q, *k, *v, *o, *d_o;        // o, d_o: backward
@@ -204,8 +205,8 @@ struct Tile {
     static constexpr int kLoads = kBytes / 4096;                   // of each of the four waves
     static_assert(kBytes % 4096 == 0, "a wave's load moves 1 KiB");
     // Tiles of each kind in LDS: two on their way beside the one in use, or one where three would leave
-    // a CU a single workgroup of the two that its registers hold (heads of 128 in bf16).
-    static constexpr int kStages = sizeof(T) == 2 && kBytes > 8192 ? 2 : 3;
+    // a CU a single workgroup of the two that its registers hold (heads of 128).
+    static constexpr int kStages = kBytes > 8192 ? 2 : 3;
 
     static __device__ constexpr int swz(int row) {
         if (kPieces == 4) return (row >> 2) & 3;

@@ -111,7 +111,7 @@ using QueryTile = Tile<T, HD, HD == 128 ? 32 : Ty<T>::kKeys>;
 // distances' entries in LDS (Diagonals).  In the end the entries are added by buckets, into the
 // workgroup's own row of a workspace.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD>())) bias_attn_dq_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, sizeof(T) == 4>())) bias_attn_dq_kernel(const Args a) {
     using X = Ty<T>;
     using Tl = QueryTile<T, HD>;
     constexpr int KT = Tl::kN;

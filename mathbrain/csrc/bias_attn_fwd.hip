@@ -184,13 +184,12 @@ int launch_sets(const Args& a, hipStream_t st) {
 // Two sets of waves where the grid leaves room for them on its CUs and the walks are long.  Measured
 // in bf16, two sets against one, 8 heads: of 64: 2 x 2048 (256 workgroups) 32 us against 41, 3 x 2048 36
 // against 44, 12 x 512 24 against 21, 4 x 2048 46 against 44; of 128: 2 x 2048 44 against 53, 3 x 2048 53 against
-// 59, 12 x 512 31 against 27; of 32: 4 x 2048 29 against 37.  fp32 heads of 128 leave no LDS for them.
+// 59, 12 x 512 31 against 27; of 32: 4 x 2048 29 against 37;
+// fp32, 16 heads of 128, 1 x 1081 157 against 165, but 8 heads, 8 x 1000 (512 workgroups) 209 against 178.
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
-    if constexpr (sizeof(T) == 2 || HD < 128) {
-        const int blocks = a.B * a.H * a.nq;
-        if (a.Lk >= 256 && (blocks <= 256 || (a.Lk >= 1024 && blocks <= (HD == 32 ? 512 : 384)))) return launch_sets<T, HD, 2>(a, st);
-    }
+    const int blocks = a.B * a.H * a.nq;
+    if (a.Lk >= 256 && (blocks <= 256 || (a.Lk >= 1024 && blocks <= (HD == 32 ? 512 : 384)))) return launch_sets<T, HD, 2>(a, st);
     return launch_sets<T, HD, 1>(a, st);
 }
 
