@@ -366,24 +366,24 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, sizeof(T) == 
 }
 
 // Where the queries' pass is split: dq and the rows' sums of ds from the runs', in order, and in bf16
-// what delta's error left in the blocks of one bucket, as a row of dbias's parts of its own.  A
-// workgroup takes 128 queries of a head.
+// what delta's error left in the blocks of one bucket, as a row of dbias's parts of its own.  Four
+// workgroups take 128 queries of a head, 32 each; the first of them has all the sums of ds.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) bias_attn_add_q_kernel(const Args a) {
     __shared__ float left[kThreads / 64][2];
-    const int qb = blockIdx.x % a.nq, bh = blockIdx.x / a.nq, b = bh / a.H, h = bh % a.H;
+    const int quarter = blockIdx.x % 4, qb = blockIdx.x / 4 % a.nq, bh = blockIdx.x / 4 / a.nq, b = bh / a.H, h = bh % a.H;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t all = (int64_t)a.B * a.H * a.Lq, first = (int64_t)bh * a.Lq + (int64_t)qb * kRows;
     const int rows = min(kRows, a.Lq - qb * kRows);
     float hi = 0.f, lo = 0.f;
-    if ((int)threadIdx.x < rows) {
+    if (quarter == 0 && (int)threadIdx.x < rows) {
         const float* stat = a.q_stat + first + threadIdx.x;
         float sum = 0.f;
         for (int s = 0; s < a.q_parts; ++s, stat += 4 * all) sum += stat[0], hi += stat[all], lo += stat[2 * all];
         a.rows[all + first + threadIdx.x] = -(a.q_stat[3 * all + first + threadIdx.x] + sum);
         hi *= sum, lo *= sum;
     }
-    const bool correct = sizeof(T) == 2 && a.dbias_part;
+    const bool correct = sizeof(T) == 2 && a.dbias_part && quarter == 0;
     if (correct) {
         hi = wave_sum(hi), lo = wave_sum(lo);
         if (lane == 0) left[wave][0] = hi, left[wave][1] = lo;
@@ -399,8 +399,8 @@ __global__ void __launch_bounds__(kThreads) bias_attn_add_q_kernel(const Args a)
             sums[n] = v;
         }
     }
-    for (int n = threadIdx.x; n < rows * (HD / 4); n += kThreads) {
-        const int r = n / (HD / 4), d = n % (HD / 4) * 4;
+    for (int n = threadIdx.x; n < min(kWaveRows, rows - quarter * kWaveRows) * (HD / 4); n += kThreads) {
+        const int r = quarter * kWaveRows + n / (HD / 4), d = n % (HD / 4) * 4;
         const float* p = a.q_part + (first + r) * HD + d;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         for (int s0 = 0; s0 < a.q_parts; s0 += 4) {   // four loads on their way together
@@ -642,7 +642,7 @@ int launch(const Args& a, hipStream_t st) {
         if (const int rc = allow_lds((const void*)bias_attn_dq_kernel<T, HD>, lds_q, told)) return rc;
         hipLaunchKernelGGL((bias_attn_dq_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq * a.q_parts)), dim3(kThreads), lds_q, st, a);
         if (a.q_parts > 1)
-            hipLaunchKernelGGL((bias_attn_add_q_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(kThreads), 0, st, a);
+            hipLaunchKernelGGL((bias_attn_add_q_kernel<T, HD>), dim3((unsigned)(a.B * a.H * a.nq * 4)), dim3(kThreads), 0, st, a);
     }
     const int nk = (a.Lk + kRows - 1) / kRows, blocks = a.B * a.Hk * nk * a.kv_parts + (a.dbias ? a.H : 0);
     if (blocks > 0) {
