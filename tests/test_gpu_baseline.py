@@ -154,3 +154,44 @@ def test_traced_without_breaks():
     gb = torch.autograd.grad(b.square().sum(), list(m.parameters()))
     for u, v in zip(ga, gb):
         assert torch.allclose(u, v, rtol=1e-4, atol=1e-4 * float(u.abs().max()))
+
+
+def test_tokens_one_by_one_agree_with_the_whole_sequence():
+    """Prompts of different lengths read into caches, then a token at a time, against each sequence
+    read at once.  Both sides are off from the exact output by at most dp |v| with (in units of 2^-24)
+    dp = 2 (hd + 8) (|q||k| / sqrt(hd) + |bias|) + 2 n + 16 for n keys, where normed rows with weights
+    of 1 have |q||k| <= hd: 144 (8 + 4) + 156 = 1884, 1.2e-4 each; the rotated rows' own error of
+    2e-6 moves a score by 4e-6 * 8 at most, p by 7e-5.  Together under 4e-4 of the largest |v|."""
+    from mathbrain.baseline import rotary_tables
+    from mathbrain.bias_attention import relative_bias_attention
+    from mathbrain.qk_norm import qk_norm_rotary
+    B, H, Hk, hd, room, steps = 3, 4, 2, 64, 70, 6
+    g = torch.Generator().manual_seed(9)
+    prompts = [5, 17, 40]
+    x = [torch.randn(B, room, n, hd, generator=g).cuda() for n in (H, Hk, Hk)]
+    bias = torch.randn(32, H, generator=g).clamp(-4, 4).cuda()
+    w = torch.ones(hd, device="cuda")
+    cos, sin = (t.cuda() for t in rotary_tables(hd, room))
+
+    def layer(b, upto):
+        q, k = qk_norm_rotary(x[0][b:b + 1, :upto], x[1][b:b + 1, :upto], w, w, cos, sin)
+        return relative_bias_attention(q.transpose(1, 2), k.transpose(1, 2), x[2][b:b + 1, :upto].transpose(1, 2), bias)
+    caches = [torch.full((B, room, Hk, hd), float("nan"), device="cuda") for _ in range(2)]
+    most = max(prompts)
+    lengths = torch.tensor(prompts, device="cuda")
+    # the padded batch of prompts; what stands behind a prompt's end is written over token by token
+    q, k = qk_norm_rotary(x[0][:, :most], x[1][:, :most], w, w, cos, sin)
+    caches[0][:, :most], caches[1][:, :most] = k, x[2][:, :most]
+    out = relative_bias_attention(q.transpose(1, 2), *(c.transpose(1, 2) for c in caches), bias, lengths=lengths, q_start=0)
+    bound = 4e-4 * float(x[2].abs().max())
+    for b, n in enumerate(prompts):
+        assert float((out[b, :, :n] - layer(b, n)[0]).abs().max()) <= bound
+    rows = torch.arange(B, device="cuda")
+    for _ in range(steps):
+        q, k = qk_norm_rotary(x[0][rows, lengths][:, None], x[1][rows, lengths][:, None], w, w, cos, sin, start=lengths)
+        caches[0][rows, lengths], caches[1][rows, lengths] = k[:, 0], x[2][rows, lengths]
+        lengths = lengths + 1
+        out = relative_bias_attention(q.transpose(1, 2), *(c.transpose(1, 2) for c in caches), bias, lengths=lengths,
+                                      q_start=lengths - 1)
+        for b, n in enumerate(lengths.tolist()):
+            assert float((out[b, :, 0] - layer(b, n)[0, :, -1]).abs().max()) <= bound, (b, n)
