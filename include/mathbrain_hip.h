@@ -678,11 +678,11 @@ typedef struct mb_bias_attn {
     void *dq, *dk, *dv;
     int64_t dq_st[3], dk_st[3], dv_st[3];
     void *dbias;                  /* [buckets, H] of bias_dtype, or NULL */
-    void *workspace;              /* both: mb_bias_attn_fwd_workspace(...) (0 where the keys are not split */
-    int64_t workspace_bytes;      /*   over workgroups) or mb_bias_attn_bwd_workspace(...) bytes */
+    void *workspace;              /* both, 16-byte aligned: mb_bias_attn_fwd_workspace(...) (0 where no */
+    int64_t workspace_bytes;      /*   keys are split over workgroups) or mb_bias_attn_bwd_workspace(...) */
 } mb_bias_attn;
 
-int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal);
+int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal, int dtype);
 int mb_bias_attn_fwd(const mb_bias_attn *args, void *stream);
 int64_t mb_bias_attn_bwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal, int dtype, int buckets);
 int mb_bias_attn_bwd(const mb_bias_attn *args, void *stream);

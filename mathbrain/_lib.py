@@ -77,7 +77,7 @@ SIGNATURES = {
     "mb_qk_norm_rotary_bwd": ([_p, _p], _i),
     "mb_qk_norm_rotary_bwd_workspace": ([_i, _i, _i], _i64),
     "mb_bias_attn_fwd": ([_p, _p], _i),
-    "mb_bias_attn_fwd_workspace": ([_i] * 7, _i64),
+    "mb_bias_attn_fwd_workspace": ([_i] * 8, _i64),
     "mb_bias_attn_bwd": ([_p, _p], _i),
     "mb_bias_attn_bwd_workspace": ([_i] * 9, _i64),
     "mb_grad_clip": ([_p, _p, _p, _p, _p, _i, _f, _p, _p, _i64, _p], _i),

@@ -107,7 +107,8 @@ def bias_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     q, k, v, bias = _rows16(q), _rows16(k), _rows16(v), bias.contiguous()
     o = _heads_last(B, H, Lq, hd, q)
     lse = torch.empty((B, H, Lq) if want_lse else (0,), dtype=torch.float32, device=dev)
-    nbytes = _lib.workspace_bytes("mb_bias_attn_fwd_workspace", B, H, k.shape[1], Lq, k.shape[2], hd, causal)
+    nbytes = _lib.workspace_bytes("mb_bias_attn_fwd_workspace", B, H, k.shape[1], Lq, k.shape[2], hd, causal,
+                                  _DTYPES[q.dtype])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.call_on(dev, "mb_bias_attn_fwd",
                  _ARGS.pack(*_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),

@@ -81,6 +81,8 @@ struct Args {
     void *out, *dk, *dv, *dbias;             // out: o (forward) or dq
     int64_t out_sb, out_sh, out_sl, dk_sb, dk_sh, dk_sl, dv_sb, dv_sh, dv_sl;
     float *lse, *rows, *dbias_part;          // [B, H, Lq] (log2 units), [2, B, H, Lq], [H, bias_rows, buckets]
+    float* o_part;                           // [B, Hk, Lq, H / Hk, o_parts, hd + 2] where the forward's walks are split
+    int o_parts;
     // where the backward's passes are split: [q_parts, B, H, Lq, hd], [q_parts, 4, B, H, Lq], [kv_parts, B, Hk, Lk, 2, hd]
     float *q_part, *q_stat, *kv_part;
     int64_t bias_rows;

@@ -724,6 +724,7 @@ extern "C" int mb_bias_attn_bwd(const mb_bias_attn* p, void* stream) {
     if (need > 0 && (!p->workspace || p->workspace_bytes < need))
         return fail(MB_ERR_WORKSPACE, "mb_bias_attn_bwd: workspace of %lld bytes, %lld are needed",
                     (long long)p->workspace_bytes, (long long)need);
+    MB_REQUIRE(need == 0 || ((uintptr_t)p->workspace & 15) == 0, "mb_bias_attn_bwd: the workspace must begin at a multiple of 16 bytes");
     if (a.B > 0 && a.Lq > 0) {
         MB_REQUIRE(p->o && p->d_o && p->lse && p->dq, "mb_bias_attn_bwd: null pointer argument");
         MB_REQUIRE(rows16(p->o, p->o_st, dtype) && rows16(p->d_o, p->do_st, dtype) && rows16(p->dq, p->dq_st, dtype),

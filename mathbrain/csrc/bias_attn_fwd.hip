@@ -1,6 +1,8 @@
 // Forward of the attention with a learned bias by distance buckets.
 #include "bias_attn_host.h"
 
+#include <algorithm>
+
 namespace mb {
 namespace battn {
 namespace {
@@ -24,7 +26,11 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
 
     const int lane = threadIdx.x & 63, wave = wave_id() % 4, set = wave_id() / 4;
     int bh, qb;
-    place(blockIdx.x, a.B * a.H, a.nq, false, bh, qb);
+    constexpr bool kRuns = sizeof(T) == 4 && SETS == 1;   // the walk may be split into runs
+    const int parts = kRuns ? a.o_parts : 1;
+    place(blockIdx.x, a.B * a.H, a.nq * parts, false, bh, qb);
+    const int part = qb % parts;
+    qb /= parts;
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const Reach reach(a);
     const int len = key_count(a, b), p0 = first_position(a, b);
@@ -34,6 +40,8 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
     const int kend = a.causal ? min(len, p0 + last + 1) : len;
     const int wend = w0 >= a.Lq ? 0 : a.causal ? min(len, p0 + min(a.Lq, w0 + kWaveRows)) : len;
     const int tiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+    // the workgroup's run of them (at most 2^24 tiles and 8 parts)
+    const int t0 = (int)((uint32_t)(tiles * part) / (uint32_t)parts), t1 = (int)((uint32_t)(tiles * (part + 1)) / (uint32_t)parts);
     const float sl2 = a.scale * kLog2e;
 
     const T* kbase = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
@@ -51,20 +59,20 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
     const typename Tl::Offsets koff(a.k_sl), voff(a.v_sl);
     auto load = [&](int n) {   // the set's n-th tiles
         const uint32_t tile = lds + n % Tl::kStages * (SETS * kStage);
-        const int j0 = (n * SETS + set) * KT;
+        const int j0 = (t0 + n * SETS + set) * KT;
         Tl::load(tile, kbase, a.k_sl, j0, len, koff);
         Tl::load(tile + Tl::kBytes, vbase, a.v_sl, j0, len, voff);
     };
-    if (tiles > 0)
+    if (t0 < t1)
         for (int n = 0; n < Tl::kStages - 1; ++n) load(n);
     fill_table(a, h, tab);   // while the first tiles are on their way
     loads_done();
-    for (int n = 0; n * SETS < tiles; ++n) {
+    for (int n = 0; t0 + n * SETS < t1; ++n) {
         // the n-th tiles are there, and nobody reads those before them any longer
         wait_and_meet<(Tl::kStages - 2) * 2 * Tl::kLoads>();
         load(n + Tl::kStages - 1);   // past the end too: the waits count loads
         const uint32_t ktile = lds + n % Tl::kStages * (SETS * kStage), vtile = ktile + Tl::kBytes;
-        const int j0 = (n * SETS + set) * KT;
+        const int j0 = (t0 + n * SETS + set) * KT;
         if (j0 < wend) {
             f32x16 x[KT / 32];
 #pragma unroll
@@ -160,7 +168,21 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f0 + other[(32 * d + row_of(r)) * 33] * f1;
     }
-    if (i < a.Lq) {
+    if (parts > 1) {
+        if (i < a.Lq) {
+            const int G = a.H / a.Hk;
+            float* p = a.o_part + ((((int64_t)(b * a.Hk + hk) * a.Lq + i) * G + h % G) * parts + part) * (HD + 2);
+            typedef __attribute__((__ext_vector_type__(2))) float f32x2;   // rows begin at multiples of 8 bytes
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const f32x2 v = {o[d][r], o[d][r + 1]};
+                    *reinterpret_cast<f32x2*>(p + 32 * d + row_of(r)) = v;
+                }
+            if (lane < 32) p[HD] = m, p[HD + 1] = l;
+        }
+    } else if (i < a.Lq) {
         const float inv = l > 0.f ? 1.0f / l : 0.f;   // a row without keys: zeros
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
 #pragma unroll
@@ -177,7 +199,7 @@ int launch_sets(const Args& a, hipStream_t st) {
     const int lds = SETS * 2 * Tl::kStages * Tl::kBytes + Reach(a).entries() * (int)sizeof(float);
     static Told told;
     if (const int rc = allow_lds((const void*)bias_attn_fwd_kernel<T, HD, SETS>, lds, told)) return rc;
-    hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD, SETS>), dim3((unsigned)(a.B * a.H * a.nq)), dim3(SETS * kThreads), lds, st, a);
+    hipLaunchKernelGGL((bias_attn_fwd_kernel<T, HD, SETS>), dim3((unsigned)(a.B * a.H * a.nq * a.o_parts)), dim3(SETS * kThreads), lds, st, a);
     return check_launch("mb_bias_attn_fwd");
 }
 
@@ -189,8 +211,21 @@ int launch_sets(const Args& a, hipStream_t st) {
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
     const int blocks = a.B * a.H * a.nq;
-    if (a.Lk >= 256 && (blocks <= 256 || (a.Lk >= 1024 && blocks <= (HD == 32 ? 512 : 384)))) return launch_sets<T, HD, 2>(a, st);
+    if (a.o_parts == 1 && a.Lk >= 256 && (blocks <= 256 || (a.Lk >= 1024 && blocks <= (HD == 32 ? 512 : 384)))) return launch_sets<T, HD, 2>(a, st);
     return launch_sets<T, HD, 1>(a, st);
+}
+
+// Runs that a workgroup's walk is split into, in fp32, where a tile takes three times as long as in
+// bf16 and uneven shares of the CUs cost as much more.  Measured, with the launch that joins the
+// runs, against one run of two sets of waves: 2 x 2854 both directions, 6 heads of 32 (276 workgroups), 3 runs
+// 174 us against 223; 1 x 1102 queries of 1936, 16 heads of 64, 5 runs 94 against 143; 10 x 1466, 2 heads
+// of 64, 3 runs 87 against 112; 1 x 1081 both directions, 16 heads of 128, 3 runs 114 against 146 (4 runs 133).
+// bf16 at these sizes: 2 runs 2 to 50 % slower.
+int o_parts_of(int B, int H, int Lq, int Lk, int hd, int dtype) {
+    const int64_t blocks = (int64_t)B * H * (((int64_t)Lq + kRows - 1) / kRows);
+    if (dtype != MB_DTYPE_F32 || blocks < 1 || blocks > 400 || Lk < 768) return 1;
+    const int64_t n = hd == 128 ? 512 / blocks : (640 + blocks - 1) / blocks;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(n, 8));
 }
 
 }  // namespace
@@ -200,9 +235,10 @@ int launch(const Args& a, hipStream_t st) {
 using namespace mb;
 using namespace mb::battn;
 
-extern "C" int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
+extern "C" int64_t mb_bias_attn_fwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd, int causal, int dtype) {
     if (B < 1 || H < 1 || Hk < 1 || H % Hk || Lq < 1 || Lk < 0 || hd < 1) return 0;
-    const int64_t splits = splits_of(B, H, Hk, Lq, Lk, hd, causal);
+    int64_t splits = splits_of(B, H, Hk, Lq, Lk, hd, causal);
+    if (splits == 0) splits = o_parts_of(B, H, Lq, Lk, hd, dtype);
     return splits > 1 ? (int64_t)B * H * Lq * splits * (hd + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -215,12 +251,17 @@ extern "C" int mb_bias_attn_fwd(const mb_bias_attn* p, void* stream) {
     MB_REQUIRE(rows16(p->o, p->o_st, dtype), "mb_bias_attn_fwd: o's rows must begin at multiples of 16 bytes");
     a.out = p->o, a.out_sb = p->o_st[0], a.out_sh = p->o_st[1], a.out_sl = p->o_st[2];
     a.lse = p->lse;
-    const int64_t need = mb_bias_attn_fwd_workspace(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal);
+    const int64_t need = mb_bias_attn_fwd_workspace(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal, dtype);
     if (need > 0 && (!p->workspace || p->workspace_bytes < need))
         return fail(MB_ERR_WORKSPACE, "mb_bias_attn_fwd: workspace of %lld bytes, %lld are needed",
                     (long long)p->workspace_bytes, (long long)need);
+    MB_REQUIRE(need == 0 || ((uintptr_t)p->workspace & 15) == 0, "mb_bias_attn_fwd: the workspace must begin at a multiple of 16 bytes");
     hipStream_t st = (hipStream_t)stream;
     if (const int splits = splits_of(a.B, a.H, a.Hk, a.Lq, a.Lk, hd, a.causal)) return split_launch(a, hd, dtype, splits, p->workspace, st);
-    if (dtype == MB_DTYPE_F32) return hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st);
-    return hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st);
+    a.o_parts = o_parts_of(a.B, a.H, a.Lq, a.Lk, hd, dtype);
+    a.o_part = (float*)p->workspace;
+    const int rc = dtype == MB_DTYPE_F32
+                       ? (hd == 32 ? launch<float, 32>(a, st) : hd == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st))
+                       : (hd == 32 ? launch<__bf16, 32>(a, st) : hd == 64 ? launch<__bf16, 64>(a, st) : launch<__bf16, 128>(a, st));
+    return rc == MB_OK && a.o_parts > 1 ? join_launch(a, hd, dtype, a.o_parts, a.o_part, st) : rc;
 }

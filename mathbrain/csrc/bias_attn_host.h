@@ -56,6 +56,8 @@ inline int splits_of(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 int split_launch(const Args& a, int hd, int dtype, int splits, void* part, hipStream_t st);
+// o and lse from parts [B, Hk, Lq, H / Hk, splits, hd + 2] of rows: sums of p v, the maximum, the sum of p.
+int join_launch(const Args& a, int hd, int dtype, int splits, const void* part, hipStream_t st);
 
 // Checks what both directions take and fills the kernels' arguments; 0 or an error code.
 inline int fill_args(const char* what, const mb_bias_attn* p, Args& a) {

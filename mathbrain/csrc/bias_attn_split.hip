@@ -256,6 +256,13 @@ __global__ void __launch_bounds__(kThreads) bias_attn_join_kernel(const Args a, 
 }
 
 template <typename T, int HD>
+int join(const Args& a, int splits, const float* part, hipStream_t st) {
+    const int64_t total = (int64_t)a.B * a.H * a.Lq;
+    hipLaunchKernelGGL((bias_attn_join_kernel<T, HD>), dim3((unsigned)((total + 3) / 4)), dim3(kThreads), 0, st, a, splits, part);
+    return check_launch("mb_bias_attn_fwd");
+}
+
+template <typename T, int HD>
 int launch(const Args& a, int splits, float* part, hipStream_t st) {
     const int G = a.H / a.Hk, rows = G * a.Lq, tiles = (rows + 31) / 32;
     const int corner = std::max(HD * 33 * 4, 32 * (HD * (int)sizeof(T) + 16));
@@ -265,10 +272,7 @@ int launch(const Args& a, int splits, float* part, hipStream_t st) {
     if (const int rc = allow_lds((const void*)bias_attn_split_kernel<T, HD>, lds, told)) return rc;
     hipLaunchKernelGGL((bias_attn_split_kernel<T, HD>), dim3((unsigned)(a.B * a.Hk * tiles * splits)), dim3(kThreads), lds, st,
                        a, splits, part);
-    if (splits > 1) {
-        const int64_t total = (int64_t)a.B * a.Hk * rows;
-        hipLaunchKernelGGL((bias_attn_join_kernel<T, HD>), dim3((unsigned)((total + 3) / 4)), dim3(kThreads), 0, st, a, splits, part);
-    }
+    if (splits > 1) return join<T, HD>(a, splits, part, st);
     return check_launch("mb_bias_attn_fwd");
 }
 
@@ -279,6 +283,12 @@ int split_launch(const Args& a, int hd, int dtype, int splits, void* part, hipSt
     if (dtype == MB_DTYPE_F32)
         return hd == 32 ? launch<float, 32>(a, splits, p, st) : hd == 64 ? launch<float, 64>(a, splits, p, st) : launch<float, 128>(a, splits, p, st);
     return hd == 32 ? launch<__bf16, 32>(a, splits, p, st) : hd == 64 ? launch<__bf16, 64>(a, splits, p, st) : launch<__bf16, 128>(a, splits, p, st);
+}
+
+int join_launch(const Args& a, int hd, int dtype, int splits, const void* part, hipStream_t st) {
+    const float* p = (const float*)part;
+    if (dtype == MB_DTYPE_F32) return hd == 32 ? join<float, 32>(a, splits, p, st) : hd == 64 ? join<float, 64>(a, splits, p, st) : join<float, 128>(a, splits, p, st);
+    return hd == 32 ? join<__bf16, 32>(a, splits, p, st) : hd == 64 ? join<__bf16, 64>(a, splits, p, st) : join<__bf16, 128>(a, splits, p, st);
 }
 
 }  // namespace battn

@@ -138,8 +138,8 @@ def test_matches_the_definition(size, hd, t, causal):
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("hd", [32, 64, 128])
-@pytest.mark.parametrize("size", [(1, 4, 2, 700, 700), (2, 2, 1, 300, 1100), (1, 2, 2, 1500, 90), (2, 3, 1, 1, 1000)])
-def test_walks_that_the_backward_splits(size, hd, t, causal):
+@pytest.mark.parametrize("size", [(1, 4, 2, 700, 700), (2, 2, 1, 300, 1100), (1, 2, 2, 1500, 90), (2, 3, 1, 1, 1000), (2, 12, 4, 500, 800)])
+def test_walks_that_are_split(size, hd, t, causal):
     from mathbrain.bias_attention import relative_bias_attention
     q, k, v, bias, do = inputs(*size, hd, t, 32, sum(size) + hd)
     lengths = None if size[0] == 1 else torch.tensor([size[4], size[4] // 3], device="cuda")

@@ -109,11 +109,13 @@ def test_bias_attention_refusals_of_one_direction(lib):
     from mathbrain import _lib
     assert lib.mb_bias_attn_fwd(None, None) < 0 and "null args" in message(lib)
     for bad, rc, said in ((dict(o=0), -1, "null"), (dict(o=P + 8), -1, "16 bytes"),
+                          (dict(Lq=1, Lk=4096, workspace=P + 8), -1, "multiple of 16"),
                           (dict(Lq=1, Lk=4096, workspace=0), _lib.MB_ERR_WORKSPACE, "workspace"),
                           (dict(Lq=1, Lk=4096, workspace_bytes=64), _lib.MB_ERR_WORKSPACE, "workspace of 64 bytes")):
         assert lib.mb_bias_attn_fwd(attn(**bad), None) == rc and said in message(lib)
     for bad, rc, said in ((dict(d_o=0), -1, "null"), (dict(lse=0), -1, "null"), (dict(dk=0), -1, "null"),
                           (dict(g2=513), -1, "16 bytes"), (dict(g2=1 << 24), -1, "elements apart"), (dict(dv=P + 4), -1, "16 bytes"),
+                          (dict(workspace=P + 4), -1, "multiple of 16"),
                           (dict(workspace=0), _lib.MB_ERR_WORKSPACE, "workspace"),
                           (dict(workspace_bytes=64), _lib.MB_ERR_WORKSPACE, "workspace of 64 bytes")):
         assert lib.mb_bias_attn_bwd(attn(**bad), None) == rc and said in message(lib)
@@ -122,10 +124,10 @@ def test_bias_attention_refusals_of_one_direction(lib):
 def test_bias_attention_workspaces(lib):
     assert lib.mb_bias_attn_fwd(attn(B=0), None) == 0 and lib.mb_bias_attn_fwd(attn(Lq=0), None) == 0
     size = lib.mb_bias_attn_fwd_workspace
-    assert size(56, 8, 8, 512, 512, 64, 1) == 0                    # a grid that fills the device
-    assert size(16, 8, 8, 1, 4096, 64, 1) > 0 and size(16, 8, 8, 1, 100, 64, 1) == 0
-    assert size(0, 8, 8, 1, 4096, 64, 1) == 0 and size(1, 8, 3, 1, 4096, 64, 1) == 0
-    assert size(1 << 30, 1 << 30, 1, 1 << 30, 1 << 30, 64, 1) == 0  # no overflow on the way to "no"
+    assert size(56, 8, 8, 512, 512, 64, 1, 1) == 0                    # a grid that fills the device
+    assert size(16, 8, 8, 1, 4096, 64, 1, 1) > 0 and size(16, 8, 8, 1, 100, 64, 1, 1) == 0
+    assert size(0, 8, 8, 1, 4096, 64, 1, 1) == 0 and size(1, 8, 3, 1, 4096, 64, 1, 1) == 0
+    assert size(1 << 30, 1 << 30, 1, 1 << 30, 1 << 30, 64, 1, 1) == 0  # no overflow on the way to "no"
     size = lib.mb_bias_attn_bwd_workspace
     assert size(2, 8, 8, 100, 100, 64, 1, 1, 32) == (2 * 2 * 8 * 100 + 8 * 2 * 32) * 4
     assert size(2, 8, 8, 0, 100, 64, 1, 1, 32) == 0 and size(1, 8, 3, 5, 5, 64, 1, 1, 32) == 0
