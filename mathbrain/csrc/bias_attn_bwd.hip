@@ -666,22 +666,26 @@ int64_t padded(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
 // from each other.  Measured, split against not, dq / dk and dv, launches that add included:
 // causal bf16 heads of 64, 2 x 1310, 8 heads (176 workgroups, 21 tiles) 36 us against 44 / 31 against
 // 39; 9 x 2259, one head 44 against 67 / 39 against 62; heads of 128, 2 x 1516, 4 heads on 2 key
-// heads 55 against 74 / 46 against 131; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key
-// heads 209 against 254 / 245 against 1180.
+// heads 55 against 74 / 46 against 131; fp32 heads of 64, 3 x 1000, 8 heads 79 against 128 / 98 against
+// 158; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key heads 209 against 254 / 245 against 1180.
 int parts_of(int64_t groups, int64_t steps, int per_cu, bool causal, int dtype) {
     if (groups < 1 || groups > 512) return 1;
-    const double start = dtype == MB_DTYPE_F32 ? 1.5 : 4.0, join = 1.2 * start;
+    const bool f32 = dtype == MB_DTYPE_F32;   // whose tiles keep a CU busy by one workgroup
+    const double start = f32 ? causal ? 1.0 : 1.5 : 4.0, join = 1.2 * start;
     int best = 1;
     double least = INFINITY;
     for (int n = 1; n <= 8 && (n == 1 || n <= steps / 2); ++n) {
         const double wgs = (causal ? 0.95 : 1.0) * groups * n;
-        const double cost = std::ceil(wgs / (256 * per_cu)) * ((double)steps / n + start) * (wgs > 256 && per_cu == 2 ? 1.6 : 1.0)
+        const double run = (double)steps / n + start;
+        const double cost = (f32 && causal ? std::max(run, groups * (0.5 * steps + n * start) / 256)
+                                           : std::ceil(wgs / (256 * per_cu)) * run * (wgs > 256 && per_cu == 2 ? 1.6 : 1.0))
                             + (n > 1 ? join : 0.0);
-        if (cost < least) least = cost, best = n;
+        if (cost < (best == 1 ? 0.95 : 1.0) * least) least = cost, best = n;
     }
     // the longest walk is twice the mean under a causal mask (3 x 3461, 5 heads of 32, 420 workgroups of 55 tiles: 64 us
-    // against 91 / 56 against 73; but 448 of 16 tiles: 52 against 42 / 50 against 37)
-    if (best == 1 && causal && per_cu == 2 && groups > 256 && steps >= 24) best = 2;
+    // against 91 / 56 against 73; but 448 of 16 tiles: 52 against 42 / 50 against 37; fp32, 9 x 900, 6 heads of 64, 432 of 15
+    // tiles: 141 against 151 / 157 against 190)
+    if (best == 1 && causal && per_cu == 2 && groups > 256 && steps >= (f32 ? 12 : 24)) best = 2;
     return best;
 }
 
