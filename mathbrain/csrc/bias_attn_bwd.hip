@@ -667,14 +667,15 @@ int64_t padded(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
 // causal bf16 heads of 64, 2 x 1310, 8 heads (176 workgroups, 21 tiles) 36 us against 44 / 31 against
 // 39; 9 x 2259, one head 44 against 67 / 39 against 62; heads of 128, 2 x 1516, 4 heads on 2 key
 // heads 55 against 74 / 46 against 131; fp32 heads of 64, 3 x 1000, 8 heads 79 against 128 / 98 against
-// 158; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key heads 209 against 254 / 245 against 1180.
+// 158; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key heads 209 against 254 / 245 against 1180;
+// 1 x 383, 5 heads of 128, runs of 64 rows 38 against 49 / 36 against 52 with three runs.
 int parts_of(int64_t groups, int64_t steps, int per_cu, bool causal, int dtype) {
     if (groups < 1 || groups > 512) return 1;
     const bool f32 = dtype == MB_DTYPE_F32;   // whose tiles keep a CU busy by one workgroup
     const double start = f32 ? causal ? 1.0 : 1.5 : 4.0, join = 1.2 * start;
     int best = 1;
     double least = INFINITY;
-    for (int n = 1; n <= 8 && (n == 1 || n <= steps / 2); ++n) {
+    for (int n = 1; n <= 8 && (n == 1 || n <= (f32 ? steps : steps / 2)); ++n) {
         const double wgs = (causal ? 0.95 : 1.0) * groups * n;
         const double run = (double)steps / n + start;
         const double cost = (f32 && causal ? std::max(run, groups * (0.5 * steps + n * start) / 256)

@@ -220,14 +220,15 @@ int launch(const Args& a, hipStream_t st) {
 // runs, against one run of two sets of waves: 2 x 2854 both directions, 6 heads of 32 (276 workgroups), 3 runs
 // 174 us against 223; 1 x 1102 queries of 1936, 16 heads of 64, 5 runs 94 against 143; 10 x 1466, 2 heads
 // of 64, 3 runs 87 against 112; 1 x 1081 both directions, 16 heads of 128, 3 runs 114 against 146 (4 runs 133);
-// 2 x 700, 4 heads of 128, 5 runs 37 against 96; 4 x 553, 4 heads of 64, 4 runs 30 against 47; but 8 x 400, 6 heads of
-// 64 (192 workgroups), 3 runs 39 against 36.
+// 2 x 700, 4 heads of 128, 5 runs 37 against 96; 1 x 383, 5 heads of 128, 5 runs 27 against 61; 4 x 553, 4 heads of 64, 4
+// runs 30 against 47; but 8 x 400, 6 heads of 64 (192 workgroups), 3 runs 39 against 36.
 // bf16 at these sizes: 2 runs 2 to 50 % slower.
 int o_parts_of(int B, int H, int Lq, int Lk, int hd, int dtype) {
     const int64_t blocks = (int64_t)B * H * (((int64_t)Lq + kRows - 1) / kRows);
-    if (dtype != MB_DTYPE_F32 || blocks < 1 || blocks > 400 || Lk < 448) return 1;
+    const bool early = hd == 128 || blocks <= 64;
+    if (dtype != MB_DTYPE_F32 || blocks < 1 || blocks > 400 || Lk < (early ? 192 : 448)) return 1;
     const int64_t n = hd == 128 ? 512 / blocks : (640 + blocks - 1) / blocks;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(n, std::min(Lk / 128, 8)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(n, std::min(Lk / (early ? 64 : 128), 8)));
 }
 
 }  // namespace
