@@ -15,6 +15,9 @@ namespace {
 // SETS = 2: a second set of four waves takes every second tile for the same queries, and the two
 // are joined through LDS in the end.  A workgroup's walk, which takes 1.2 us (heads of 128: 1.5) a
 // tile with nothing beside it on the CU, is then half as long.
+//
+// In fp32 the walk may be split into o_parts runs, a workgroup each (o_parts_of), whose maxima, sums
+// and outputs bias_attn_join_kernel joins through memory.
 template <typename T, int HD, int SETS>
 __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bias_attn_fwd_kernel(const Args a) {
     using X = Ty<T>;

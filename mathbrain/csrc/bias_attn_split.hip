@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     }
 }
 
-// Joins the parts of a row: a wave a row, a lane a part for the weights, then a lane a channel.
+// Joins the parts of a row, the forward's runs too (bias_attn_fwd.hip): a wave a row, a lane a part for the weights, then a lane a channel.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) bias_attn_join_kernel(const Args a, int splits, const float* __restrict__ part) {
     const int lane = threadIdx.x & 63;
