@@ -100,7 +100,7 @@ def _fwd_fake(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, s
 def bias_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch.Tensor, max_distance: int,
                   causal: bool, scale: float, lengths: Optional[torch.Tensor], start_rows: Optional[torch.Tensor],
                   start: int, want_lse: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """(o, lse): lse [B, H, Lq] = log2 of the row's softmax denominator (inf without keys) for the
+    """(o, lse): lse [B, H, Lq] = log2 of the row's softmax denominator (inf without keys, NaN from NaN) for the
     backward, empty unless wanted."""
     dev = q.device
     B, H, Lq, hd = q.shape
@@ -207,7 +207,8 @@ def relative_bias_attention(q, k, v, bias, max_distance=128, causal=True, scale=
     ``causal``: a query sees the keys up to its position.  ``lengths``: an int32 / int64 tensor [B];
     keys from there on are not seen (values in 0 .. Lk; others are taken as the nearest of these).
     Rows of k and v behind these ends, and with ``causal`` behind the last query's position, may hold
-    anything; other values of q, k and v have to be finite.  A bias below -65536 (-inf, or its type's
+    anything; other values of q, k and v have to be finite (NaN there, or in the bias, comes out as
+    NaN in the rows that it reaches).  A bias below -65536 (-inf, or its type's
     lowest value) hides the pairs of its bucket.  A query that sees no key gets zeros, and passes on
     no gradient.  ``scale``: 1 / sqrt(hd) by default, otherwise 1e-20 to 1e20.
 

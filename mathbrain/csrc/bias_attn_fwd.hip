@@ -186,12 +186,12 @@ __global__ void __launch_bounds__(SETS * kThreads, (waves_per_simd<T, HD>())) bi
             if (lane < 32) p[HD] = m, p[HD + 1] = l;
         }
     } else if (i < a.Lq) {
-        const float inv = l > 0.f ? 1.0f / l : 0.f;   // a row without keys: zeros
+        const float inv = l == 0.f ? 0.f : 1.0f / l;   // a row without keys: zeros; NaN stays NaN
         T* row = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d) store_block<T>(row, 32 * d, o[d], inv);
         if (a.lse && lane < 32)
-            a.lse[(int64_t)bh * a.Lq + i] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+            a.lse[(int64_t)bh * a.Lq + i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
     }
 }
 

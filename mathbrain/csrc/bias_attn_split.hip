@@ -211,9 +211,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
             if (d == 0) p[HD] = top, p[HD + 1] = sum;
         } else {
             const int iq = (tile * 32 + q) / G, hq = hk * G + (tile * 32 + q) % G;
-            ((T*)a.out)[b * a.out_sb + hq * a.out_sh + (int64_t)iq * a.out_sl + d] = (T)(sum > 0.f ? acc / sum : 0.f);
+            ((T*)a.out)[b * a.out_sb + hq * a.out_sh + (int64_t)iq * a.out_sl + d] = (T)(sum == 0.f ? 0.f : acc / sum);   // NaN stays NaN
             if (d == 0 && a.lse)
-                a.lse[((int64_t)b * a.H + hq) * a.Lq + iq] = sum > 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+                a.lse[((int64_t)b * a.H + hq) * a.Lq + iq] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
         }
     }
 }
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) bias_attn_join_kernel(const Args a, 
     float sum = l * f;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const float w = sum > 0.f ? f / sum : 0.f;
+    const float w = sum == 0.f ? 0.f : f / sum;
     const int bhk = (int)(row / rows), rr = (int)(row - (int64_t)bhk * rows);
     const int b = bhk / a.Hk, h = bhk % a.Hk * G + rr % G, i = rr / G;
     T* out = (T*)a.out + b * a.out_sb + h * a.out_sh + (int64_t)i * a.out_sl;
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads) bias_attn_join_kernel(const Args a, 
         }
         if (d < HD) out[d] = (T)acc;
     }
-    if (lane == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum > 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+    if (lane == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Lq + i] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 template <typename T, int HD>

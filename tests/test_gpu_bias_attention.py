@@ -427,3 +427,68 @@ def test_refusals():
                       (dict(scale=float("nan")), "scale"), (dict(q_start=(1 << 29) + 1), "q_start")):
         with pytest.raises(_lib.HipKernelError, match=said):
             relative_bias_attention(**(base | bad))
+
+
+def with_nan(kind, q, k, v, bias):
+    """The inputs with one NaN, and the rows of o [B, H, Lq] that it reaches without a mask."""
+    B, H, Lq, _ = q.shape
+    q, k, v, bias = (x.clone() for x in (q, k, v, bias))
+    rows = torch.zeros(B, H, Lq, dtype=torch.bool)
+    G = H // k.shape[1]
+    if kind == "q":
+        q[0, H - 1, Lq // 2, 3] = math.nan
+        rows[0, H - 1, Lq // 2] = True
+    elif kind == "bias":       # the bucket of distance 0, which every query here meets
+        bias[0, 0] = math.nan
+        rows[:, 0] = True
+    else:                      # the first key: all queries of its heads see it
+        (k if kind == "k" else v)[B - 1, 0, 0] = math.nan
+        rows[B - 1, :G] = True
+    return q, k, v, bias, rows
+
+
+# one token and few keys: one part a row; a long cache: several; 128 queries a workgroup: one set of waves, two, and
+# (in fp32) runs
+@pytest.mark.parametrize("kind", ["q", "k", "v", "bias"])
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("B,H,Hk,Lq,Lk,hd", [(2, 4, 2, 1, 100, 64), (400, 1, 1, 1, 700, 32), (2, 4, 2, 1, 3000, 64), (2, 4, 2, 130, 130, 64),
+                                             (2, 8, 4, 300, 300, 128), (2, 20, 4, 512, 600, 64)])
+def test_not_a_number_comes_out(B, H, Hk, Lq, Lk, hd, t, kind):
+    from mathbrain.bias_attention import bias_attn_fwd, relative_bias_attention
+    q, k, v, bias, _ = inputs(B, H, Hk, Lq, Lk, hd, t, 32, 3)
+    q, k, v, bias, rows = with_nan(kind, q, k, v, bias)
+    o = relative_bias_attention(q, k, v, bias)
+    assert torch.equal(torch.isnan(o).any(-1).cpu(), rows)
+    if kind != "v":
+        assert torch.isnan(o[rows.cuda()]).all()
+    _, lse = bias_attn_fwd(q, k, v, bias, 128, True, 0.125, None, None, Lk - Lq, True)
+    assert torch.equal(torch.isnan(lse).cpu(), rows if kind != "v" else torch.zeros_like(rows))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("L,hd", [(40, 64), (300, 128)])
+def test_not_a_number_comes_out_of_the_gradients(L, hd, t):
+    """A NaN in head 0's bias: that head's rows have no probabilities, and so have no gradients."""
+    from mathbrain.bias_attention import relative_bias_attention
+    q, k, v, bias, do = inputs(1, 4, 2, L, L, hd, t, 32, 3)
+    q, k, v, bias, _ = with_nan("bias", q, k, v, bias)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, bias)]
+    dq, dk, dv, dbias = torch.autograd.grad(relative_bias_attention(*leaves), leaves, do)
+    for x in (dq[:, :1], dk[:, :1], dv[:, :1], dbias[0, :1]):
+        assert torch.isnan(x).all()
+    for x in (dq[:, 1:], dk[:, 1:], dv[:, 1:], dbias[:, 1:]):
+        assert torch.isfinite(x).all()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_a_position_outside_the_rotation_shows_in_a_decoded_token(t):
+    from mathbrain.baseline import rotary_tables
+    from mathbrain.qk_norm import qk_norm_rotary
+    from mathbrain.bias_attention import relative_bias_attention
+    _, k, v, bias, _ = inputs(3, 4, 4, 1, 50, 64, t, 32, 5)
+    cos, sin = (x.cuda() for x in rotary_tables(64, 50))
+    w = torch.ones(64, device="cuda")
+    x = torch.randn(3, 1, 4, 64, device="cuda").to(t)
+    q, _ = qk_norm_rotary(x, x, w, w, cos, sin, start=torch.tensor([49, 50, 3], device="cuda"))
+    o = relative_bias_attention(q.transpose(1, 2), k, v, bias, lengths=torch.tensor([50, 50, 4], device="cuda"), q_start=torch.tensor([49, 49, 3], device="cuda"))
+    assert torch.isnan(o[1]).all() and torch.isfinite(o[0]).all() and torch.isfinite(o[2]).all()
