@@ -10,6 +10,7 @@ import functools
 import os
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmathbrain_hip.so")
@@ -178,6 +179,13 @@ def traced_op(name, fake):
         call.op = op
         return call
     return deco
+
+
+def wants_derivatives(*tensors):
+    """Whether an autograd function has to see these tensors: one requires a gradient, or may have a
+    tangent (forward-mode dual tensors require none, with gradients enabled or not).  Where it does not,
+    an entry point of a few microseconds calls its kernels directly."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
 
 
 def require_gpu(*tensors, what="mathbrain"):

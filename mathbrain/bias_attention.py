@@ -221,6 +221,6 @@ def relative_bias_attention(q, k, v, bias, max_distance=128, causal=True, scale=
     start = k.shape[2] - q.shape[2] if q_start is None else 0 if rows is not None else int(q_start)
     lengths = None if lengths is None else lengths.contiguous()
     args = (q, k, v, bias, max_distance, causal, scale, lengths, rows, start)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or bias.requires_grad):
+    if _lib.wants_derivatives(q, k, v, bias):
         return RelativeBiasAttentionFunction.apply(*args)
     return bias_attn_fwd(*args, False)[0]

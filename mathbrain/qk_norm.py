@@ -145,7 +145,6 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, eps=1e-6, start=0):
     _check(q, k, q_weight, k_weight, cos, sin, start)
     rows = start.contiguous() if torch.is_tensor(start) else None
     args = (q, k, q_weight, k_weight, cos, sin, float(eps), rows, 0 if rows is not None else int(start))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
-                                    or k_weight.requires_grad):
+    if _lib.wants_derivatives(q, k, q_weight, k_weight):
         return QKNormRotaryFunction.apply(*args)
     return qk_norm_rotary_fwd(*args)

@@ -492,3 +492,20 @@ def test_a_position_outside_the_rotation_shows_in_a_decoded_token(t):
     q, _ = qk_norm_rotary(x, x, w, w, cos, sin, start=torch.tensor([49, 50, 3], device="cuda"))
     o = relative_bias_attention(q.transpose(1, 2), k, v, bias, lengths=torch.tensor([50, 50, 4], device="cuda"), q_start=torch.tensor([49, 49, 3], device="cuda"))
     assert torch.isnan(o[1]).all() and torch.isfinite(o[0]).all() and torch.isfinite(o[2]).all()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor asks for a tangent without requiring a gradient; an output without one would be
+    a derivative of zero."""
+    import torch.autograd.forward_ad as fw
+    from mathbrain.bias_attention import relative_bias_attention
+    q, k, v, bias, _ = inputs(1, 2, 1, 5, 5, 32, F32, 8, 1)
+    want = relative_bias_attention(q, k, v, bias)
+    with fw.dual_level():
+        for i in range(4):
+            args = [q, k, v, bias]
+            args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(NotImplementedError, match="jvp"):
+                    relative_bias_attention(*args)
+        assert torch.equal(relative_bias_attention(q, k, v, bias), want)     # no tangents: as ever

@@ -242,3 +242,22 @@ def test_differences_agree_with_the_gradient():
         diff = (value(q + h * dq, k + h * dk, w + h * dw) - value(q - h * dq, k - h * dk, w - h * dw)) / (2 * h)
     along = sum((a.double() * b.double()).sum() for a, b in zip(grads, (dq, dk, dw)))
     assert abs(float(diff - along)) < 2e-2, (float(diff), float(along))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor asks for a tangent without requiring a gradient; an output without one would be
+    a derivative of zero."""
+    import torch.autograd.forward_ad as fw
+    from mathbrain.qk_norm import qk_norm_rotary
+    cos, sin = (t.cuda() for t in tables(32, 8))
+    w = torch.rand(32, device="cuda")
+    x = torch.randn(2, 3, 2, 32, device="cuda")
+    want = qk_norm_rotary(x, x, w, w, cos, sin)
+    with fw.dual_level():
+        for i in range(4):
+            args = [x, x, w, w]
+            args[i] = fw.make_dual(args[i].clone(), torch.ones_like(args[i]))
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(NotImplementedError, match="jvp"):
+                    qk_norm_rotary(*args, cos, sin)
+        assert all(torch.equal(a, b) for a, b in zip(qk_norm_rotary(x, x, w, w, cos, sin), want))
