@@ -15,6 +15,7 @@ import array
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 
@@ -48,6 +49,8 @@ def _codes(tensors, device, what):
     index = device.index if device.type == "cuda" else -2
     if list(map(torch.Tensor.get_device, tensors)).count(index) != len(codes):
         _lib.require_gpu(torch.empty(0, device=device), *tensors, what=what)
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode tangents are not scaled with their tensors")
     return array.array("i", codes), contiguous
 
 

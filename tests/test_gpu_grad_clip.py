@@ -247,3 +247,18 @@ def test_refusals():
         clip_gradients([torch.sparse_coo_tensor([[0], [1]], [1.0], (4, 4), device="cuda")], 1.0)
     assert float(clip_grad_norm_([], 1.0)) == 0.0 and float(grad_norm([])) == 0.0
     assert float(clip_gradients([torch.empty(0, device="cuda")], 1.0)) == 0.0
+
+
+def test_tangents_are_refused():
+    """A dual tensor's tangent would have to be scaled with it."""
+    import torch.autograd.forward_ad as fw
+    from mathbrain.grad_clip import clip_gradients, grad_norm
+    x = torch.randn(6, device="cuda")
+    before = x.clone()
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: clip_gradients([d], 0.1), lambda: clip_gradients([x[:3]], 0.1, out=[d[3:]]), lambda: grad_norm([d])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert float(grad_norm([x])) > 0
+    assert torch.equal(x, before)
