@@ -12,6 +12,7 @@ same gradients always give the same norm.  Where the factor is 1 an in-place cal
 nothing.  fp32 and bf16 tensors, mixed as they come; CPU tensors raise NotImplementedError.
 """
 import array
+import bisect
 import math
 
 import torch
@@ -54,6 +55,25 @@ def _codes(tensors, device, what):
     return array.array("i", codes), contiguous
 
 
+def _stretch(t):
+    """The addresses of a tensor's first byte and of the one behind its last."""
+    at = t.data_ptr()
+    return at, at + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _refuse_overwritten(grads, out, what):
+    """The library sees copies of the gradients that are not contiguous: their own memory must not be
+    an output's.  (Outputs that share memory among them are refused there.)"""
+    written = sorted(_stretch(o) for o in out if o.numel())
+    starts = [first for first, _ in written]
+    for g in grads:
+        if g.numel() and not g.is_contiguous():
+            first, end = _stretch(g)
+            i = bisect.bisect_left(starts, end) - 1
+            if i >= 0 and written[i][1] > first:
+                raise _lib.HipKernelError(f"{what}: tensors share memory that the call writes")
+
+
 def _clip(src, codes, dst, dst_codes, max_norm, device):
     """The norm of src (element types: codes) as a 0-dim fp32 tensor; dst (None: no scaling) gets
     the scaled values."""
@@ -90,8 +110,9 @@ def clip_gradients(grads, max_norm, out=None):
     ``out`` None: in place; the tensors must fill their memory without gaps (any order of the
     dimensions).  Otherwise one contiguous tensor of the same shape for each gradient, fp32 or
     bf16, which gets the scaled values; ``grads`` are left as they are.  No written tensor may
-    share memory with another tensor of the call, and no tensor may be listed twice where it is
-    written; such calls raise HipKernelError before anything is launched."""
+    share memory with another tensor of the call (a gradient with gaps counts with them), and no
+    tensor may be listed twice where it is written; such calls raise HipKernelError before anything
+    is launched."""
     what = "clip_gradients"
     grads = list(grads)
     max_norm = float(max_norm)
@@ -116,7 +137,10 @@ def clip_gradients(grads, max_norm, out=None):
         g, o = next((g, o) for g, o in zip(grads, out) if o.shape != g.shape or not o.is_contiguous())
         raise ValueError(f"{what}: an output of shape {tuple(o.shape)}, strides {o.stride()} for a gradient "
                          f"of shape {tuple(g.shape)}: contiguous tensors of the same shape are wanted")
-    return _clip(grads if contiguous else [g.contiguous() for g in grads], codes, out, out_codes, max_norm, device)
+    if not contiguous:
+        _refuse_overwritten(grads, out, what)
+        grads = [g.contiguous() for g in grads]
+    return _clip(grads, codes, out, out_codes, max_norm, device)
 
 
 @torch.no_grad()

@@ -262,3 +262,23 @@ def test_tangents_are_refused():
                 call()
         assert float(grad_norm([x])) > 0
     assert torch.equal(x, before)
+
+
+def test_memory_shared_with_a_copied_gradient_is_refused():
+    """A gradient that is not contiguous is copied before the library sees it; the output that would
+    overwrite it is refused all the same."""
+    from mathbrain import _lib
+    from mathbrain.grad_clip import clip_gradients
+    x = torch.randn(40, 50, device="cuda")
+    before, spare = x.clone(), torch.empty(50, 40, device="cuda")
+    for grads, out in (([x.t()], [x.view(50, 40)]), ([x[:, ::2]], [x.view(-1)[:1000].view(40, 25)]),
+                       ([spare[:, :1].t(), x.t()], [torch.empty(1, 50, device="cuda"), x.view(50, 40)])):
+        with pytest.raises(_lib.HipKernelError, match="share memory"):
+            clip_gradients(grads, 0.1, out=out)
+    assert torch.equal(x, before)
+    clip_gradients([x.t()], 1e9, out=[spare])
+    assert torch.equal(spare, x.t())
+    both = torch.randn(80, 50, device="cuda")                                   # neighbours
+    want = both[:40].t().clone()
+    clip_gradients([both[:40].t()], 1e9, out=[both[40:].view(50, 40)])
+    assert torch.equal(both[40:].view(50, 40), want) and torch.equal(both[:40].t(), want)
