@@ -657,6 +657,7 @@ typedef struct mb_bias_attn {
     const void *q, *k, *v;        /* [B, H, Lq, hd], [B, Hk, Lk, hd] twice; Hk divides H */
     int64_t q_st[3], k_st[3], v_st[3];
     const void *bias;             /* [buckets, H] contiguous; below -65536: the bucket's pairs are hidden */
+                                  /*   (where a head has none above, its largest is taken off first) */
     const int32_t *starts;        /* HOST: the first distance of each of n_starts buckets, not falling, */
     int64_t buckets, n_starts;    /*   from one 0 to at most 1024; the last has no end. n_starts <= 128. */
                                   /*   causal: buckets = n_starts; otherwise 2 n_starts, the upper half */
@@ -672,7 +673,8 @@ typedef struct mb_bias_attn {
     double scale;                 /* 1e-20 to 1e20 */
     void *o;                      /* [B, H, Lq, hd]: written by the forward, read by the backward */
     int64_t o_st[3];
-    float *lse;                   /* [B, H, Lq] log2 of the softmax denominators, likewise (NULL: not wanted) */
+    float *lse;                   /* [B, H, Lq] log2 of the softmax denominators (less what was taken off the */
+                                  /*   biases), likewise (NULL: not wanted) */
     const void *d_o;              /* backward from here on */
     int64_t do_st[3];
     void *dq, *dk, *dv;

@@ -208,8 +208,8 @@ def relative_bias_attention(q, k, v, bias, max_distance=128, causal=True, scale=
     keys from there on are not seen (values in 0 .. Lk; others are taken as the nearest of these).
     Rows of k and v behind these ends, and with ``causal`` behind the last query's position, may hold
     anything; other values of q, k and v have to be finite (NaN there, or in the bias, comes out as
-    NaN in the rows that it reaches).  A bias below -65536 (-inf, or its type's
-    lowest value) hides the pairs of its bucket.  A query that sees no key gets zeros, and passes on
+    NaN in the rows that it reaches).  A bias below -65536 (-inf, or its type's lowest value) hides the
+    pairs of its bucket; where all of a head's lie there, the largest is taken off them first.  A query that sees no key gets zeros, and passes on
     no gradient.  ``scale``: 1 / sqrt(hd) by default, otherwise 1e-20 to 1e20.
 
     In bf16 the probabilities and the scores' gradients are rounded to bf16 for the products that

@@ -77,8 +77,9 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     const int64_t w0 = (int64_t)s * 4 * per, w1 = w0 + 4 * per < kend ? w0 + 4 * per : kend;
     if (w0 < w1 && pmin - (w1 + 31) < reach.hi && pmax - w0 > reach.lo) {
         for (int n = threadIdx.x; n < a.buckets * G; n += kThreads) {
-            const int64_t at = (int64_t)(n / G) * a.H + hk * G + n % G;
-            values[n] = bias_at(a, at);
+            const int head = hk * G + n % G;
+            const float v = bias_value(a, n / G, head), first = bias_value(a, 0, head);
+            values[n] = in_log2(v - taken_off<false>(head, first));
         }
         for (int n = threadIdx.x; n <= reach.hi - reach.lo; n += kThreads) {
             const int d = n + reach.lo;
@@ -87,8 +88,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
             bucket[n] = (uint8_t)k;
         }
     }
-    const int64_t far_hi = (int64_t)(a.n_starts - 1) * a.H + h, far_lo = (int64_t)(a.causal ? 0 : 2 * a.n_starts - 1) * a.H + h;
-    const float bias_hi = bias_at(a, far_hi), bias_lo = bias_at(a, far_lo);
+    float bias_hi = bias_value(a, a.n_starts - 1, h), bias_lo = bias_value(a, a.causal ? 0 : 2 * a.n_starts - 1, h);
+    const float bias_first = bias_value(a, 0, h);
 
     typename X::Frag qf[HD / 16], kf[HD / 16];
     {
@@ -115,6 +116,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     for (int d = 0; d < HD / 32; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
     if (j0 < j1) load(j0);
+    const float off = taken_off<false>(h, bias_first);   // while these are on their way
+    bias_hi = in_log2(bias_hi - off), bias_lo = in_log2(bias_lo - off);
     __syncthreads();
     for (int jb = j0; jb < j1; jb += 32) {
         f32x16 x = zero16();

@@ -509,3 +509,44 @@ def test_forward_mode_derivatives_are_refused():
                 with grad(), pytest.raises(NotImplementedError, match="jvp"):
                     relative_bias_attention(*args)
         assert torch.equal(relative_bias_attention(q, k, v, bias), want)     # no tangents: as ever
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("low", [-1e5, -3e30])
+@pytest.mark.parametrize("Lq,Lk,hd,causal", [(200, 200, 64, True), (150, 300, 128, False), (1, 700, 64, True), (2, 90, 32, False)])
+def test_a_whole_table_far_below_zero(Lq, Lk, hd, causal, low, t):
+    """What a softmax leaves out, one number added to all scores, does not change the answer: head 0's
+    biases are all low, head 1's and head 2's hide one bucket (head 1's others are low too), head 3's are the
+    lowest of their type.  Differences within a low head are exact in fp32 (neighbours of one size), so
+    the bounds are those of the biases less their head's largest."""
+    from mathbrain.bias_attention import relative_bias_attention
+    q, k, v, bias, do = inputs(2, 4, 2, Lq, Lk, hd, t, 8, 7)
+    bias = bias.float()
+    bias[:, 0] = low
+    if low == -1e5:    # in steps of fp32's there; at -3e30 a step is more than scores can make up for
+        bias[:, 0] += 2.0 ** -7 * torch.arange(8, device="cuda")
+    bias[:, 1] = low
+    bias[6, 1] = 2 * low
+    bias[6, 2] = low
+    bias[:, 3] = torch.finfo(F32).min
+    rest = bias.double().cpu()
+    rest = rest - rest.amax(0)
+    hidden = rest < -65536
+    assert hidden.sum() == 2
+    n, seen = plan(2, Lq, Lk, 8, 16, causal, None, None)
+    seen = seen[:, None].expand(2, 4, Lq, Lk) & ~hidden.t()[:, n].transpose(0, 1)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, bias)]
+    o = relative_bias_attention(*leaves, max_distance=16, causal=causal)
+    got = [o, *torch.autograd.grad(o, leaves, do)]
+    for h in range(4):    # a head at a time: their pairs differ
+        kv = h // 2
+        alone = [x.detach().requires_grad_() for x in (q[:, h:h + 1], k[:, kv:kv + 1], v[:, kv:kv + 1], bias[:, h:h + 1])]
+        o1 = relative_bias_attention(*alone, max_distance=16, causal=causal)
+        g1 = torch.autograd.grad(o1, alone, do[:, h:h + 1])
+        want = definition(*(x.detach() for x in alone[:3]), rest[:, h:h + 1].masked_fill(hidden[:, h:h + 1], 0.0), do[:, h:h + 1], n,
+                          seen[:, h], 1 / math.sqrt(hd), t)
+        for x, w, name in zip([o1, *g1], want, NAMES):
+            near(x, w, name)
+        near(got[0][:, h:h + 1], want[0], "o of all heads")
+        near(got[1][:, h:h + 1], want[1], "dq of all heads")
+        near(got[4][:, h:h + 1], want[4], "dbias of all heads")
