@@ -194,19 +194,24 @@ __device__ inline void fill_table(const Args& a, int h, float* tab) {
 // other, so a row has no padding; piece c of row r lies in the row's place c ^ swz(r) instead,
 // which spreads both ways of reading the tile over the banks.
 
-// 16 (or 4) bytes a lane from base + voff to LDS at lds + 16 (or 4) * lane.
+// 16 (or 4) bytes a lane from base + voff to LDS at lds + 16 (or 4) * lane.  M0 holds the LDS address; the compiler
+// reserves it for its own instructions, which set it before they use it, warns of the clobber for that reason, and
+// has to know of it so that it keeps no value there from one of them to the next.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ inline void dma16(uint32_t lds, uint32_t voff, const void* base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(lds), "v"(voff), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ inline void dma4(uint32_t lds, uint32_t voff, const void* base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                  :
                  : "s"(lds), "v"(voff), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // Waits until at most N of the wave's loads are on their way, and for the other waves.
 template <int N>
 __device__ inline void wait_and_meet() {

@@ -190,3 +190,20 @@ def test_cpu_tensors_are_refused():
         clip_gradients([x], 1.0)
     with pytest.raises(NotImplementedError, match="no CPU path"):
         relative_bias_attention(x, x, x, torch.zeros(4, 1))
+
+
+def test_inline_assembly_that_writes_m0_says_so():
+    """The compiler uses M0 itself; a statement that sets it has to name it as overwritten."""
+    import glob
+    import os
+    import re
+
+    import mathbrain
+    found = 0
+    for path in glob.glob(os.path.join(os.path.dirname(mathbrain.__file__), "csrc", "*.h*")):
+        for statement in re.findall(r"\basm\b[^;]*;", open(path).read()):
+            code, *rest = statement.split("\n                 :")   # the operands' lines
+            if re.search(r"s_mov_b32 m0\b", code):
+                found += 1
+                assert '"m0"' in "".join(rest), (path, statement)
+    assert found == 2
