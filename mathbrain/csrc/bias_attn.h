@@ -145,26 +145,25 @@ __device__ inline float bias_value(const Args& a, int n, int h) {
     const int64_t at = (int64_t)n * a.H + h;
     return a.bias_bf16 ? (float)((const __bf16*)a.bias)[at] : ((const float*)a.bias)[at];
 }
-// What is taken off head h's biases, of which `first` is the one of bucket 0: few heads look further.  Those read
-// the kernel's arguments (Args is the first one) once more from where they came: kept in registers for this, they
-// take dk and dv's loop the room to read ahead of its products (heads of 128, 8 x 1024: 84 us against 80).
+__device__ inline bool is_low(float v) { return v < kHidden && v > -INFINITY; }
+// What is taken off head h's biases where one of them is low; no other thread pays for it.  The kernel's arguments
+// (Args is the first one) are read once more from where they came: kept in registers for this, they take dk and dv's
+// loop the room to read ahead of its products (heads of 128, 8 x 1024: 84 us against 80).
 // UNIFORM: h is the whole wave's.
 template <bool UNIFORM>
-__device__ inline float taken_off(int h, float first) {
-    float top = first;
-    if (top < kHidden) {
-        auto* a = (__attribute__((address_space(4))) const Args*)__builtin_amdgcn_kernarg_segment_ptr();
-        asm volatile("" : "+s"(a));
-        if constexpr (UNIFORM) asm volatile("" : "+s"(h));
-        const void* bias = a->bias;
-        const int buckets = a->buckets, heads = a->H, bf16 = a->bias_bf16;
+__device__ inline float taken_off(int h) {
+    auto* a = (__attribute__((address_space(4))) const Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    if constexpr (UNIFORM) asm volatile("" : "+s"(h));
+    const void* bias = a->bias;
+    const int buckets = a->buckets, heads = a->H, bf16 = a->bias_bf16;
+    float top = -INFINITY;
 #pragma unroll 1
-        for (int n = 1; n < buckets; ++n) {
-            const int64_t at = (int64_t)n * heads + h;
-            top = fmaxf(top, bf16 ? (float)((const __bf16*)bias)[at] : ((const float*)bias)[at]);
-        }
+    for (int n = 0; n < buckets; ++n) {
+        const int64_t at = (int64_t)n * heads + h;
+        top = fmaxf(top, bf16 ? (float)((const __bf16*)bias)[at] : ((const float*)bias)[at]);
     }
-    return top < kHidden && top > -INFINITY ? top : 0.f;
+    return top < kHidden ? top : 0.f;
 }
 __device__ inline float in_log2(float v) { return v < kHidden ? -INFINITY : kLog2e * v; }
 
@@ -179,8 +178,8 @@ __device__ inline void fill_table(const Args& a, int h, float* tab) {
             d[e] = d[e] < r.lo ? r.lo : d[e] > r.hi ? r.hi : d[e];
         }
         buckets_of<2>(a, d, n);
-        const float x = bias_value(a, n[0], h), y = bias_value(a, n[1], h), first = bias_value(a, 0, h);
-        const float off = taken_off<true>(h, first);
+        const float x = bias_value(a, n[0], h), y = bias_value(a, n[1], h);
+        const float off = __any(is_low(x) || is_low(y)) ? taken_off<true>(h) : 0.f;
         tab[i] = in_log2(x - off);
         if (i + (int)blockDim.x < r.entries()) tab[i + blockDim.x] = in_log2(y - off);
     }

@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     if (w0 < w1 && pmin - (w1 + 31) < reach.hi && pmax - w0 > reach.lo) {
         for (int n = threadIdx.x; n < a.buckets * G; n += kThreads) {
             const int head = hk * G + n % G;
-            const float v = bias_value(a, n / G, head), first = bias_value(a, 0, head);
-            values[n] = in_log2(v - taken_off<false>(head, first));
+            const float v = bias_value(a, n / G, head);
+            values[n] = in_log2(is_low(v) ? v - taken_off<false>(head) : v);
         }
         for (int n = threadIdx.x; n <= reach.hi - reach.lo; n += kThreads) {
             const int d = n + reach.lo;
@@ -89,7 +89,6 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
         }
     }
     float bias_hi = bias_value(a, a.n_starts - 1, h), bias_lo = bias_value(a, a.causal ? 0 : 2 * a.n_starts - 1, h);
-    const float bias_first = bias_value(a, 0, h);
 
     typename X::Frag qf[HD / 16], kf[HD / 16];
     {
@@ -116,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, (waves_per_simd<T, HD, true>())) bia
     for (int d = 0; d < HD / 32; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
     if (j0 < j1) load(j0);
-    const float off = taken_off<false>(h, bias_first);   // while these are on their way
+    const float off = is_low(bias_hi) || is_low(bias_lo) ? taken_off<false>(h) : 0.f;   // while these are on their way
     bias_hi = in_log2(bias_hi - off), bias_lo = in_log2(bias_lo - off);
     __syncthreads();
     for (int jb = j0; jb < j1; jb += 32) {
