@@ -14,6 +14,8 @@ adds a learned bias by distance buckets to every layer's scores, one table [n, h
 layers, in the attention that reads it (``relative_bias_attention``, which replaces torch's
 there; its probabilities are not dropped out, the block's output is).
 """
+import warnings
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -98,13 +100,17 @@ class RoPETransformerLM(nn.Module):
     """baseline.py:86-129: RoPETransformerLM(vocab_size, d_model, n_layers, n_heads,
     max_seq_len=4096, dropout=0.1); forward(x [B, L]) -> logits [B, L, vocab_size].
     ``qk_norm``: RMS norms of every query and key head.  ``rel_buckets``: a learned bias by that
-    many distance buckets, up to ``rel_max_distance`` (0: none).  Both take head_dim 32, 64 or
-    128; the bias starts as zeros."""
+    many distance buckets, up to ``rel_max_distance`` (0: none); the probabilities are not dropped
+    out then, and a ``dropout`` above 0 warns of it.  Both take head_dim 32, 64 or 128; the bias
+    starts as zeros."""
 
     def __init__(self, vocab_size: int, d_model: int, n_layers: int, n_heads: int,
                  max_seq_len: int = 4096, dropout: float = 0.1, qk_norm: bool = False,
                  rel_buckets: int = 0, rel_max_distance: int = 128):
         super().__init__()
+        if rel_buckets and dropout:
+            warnings.warn(f"RoPETransformerLM: with rel_buckets the attention's probabilities are not dropped out; "
+                          f"dropout={dropout} is that of the blocks' outputs alone", stacklevel=2)
         self.vocab_size = vocab_size
         self.d_model = d_model
         self.embed = nn.Embedding(vocab_size, d_model)

@@ -207,3 +207,15 @@ def test_inline_assembly_that_writes_m0_says_so():
                 found += 1
                 assert '"m0"' in "".join(rest), (path, statement)
     assert found == 2
+
+
+def test_a_model_that_does_not_drop_out_probabilities_says_so():
+    import warnings
+
+    from mathbrain.baseline import RoPETransformerLM
+    with pytest.warns(UserWarning, match="not dropped out"):
+        RoPETransformerLM(10, 64, 1, 2, max_seq_len=8, rel_buckets=8)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        RoPETransformerLM(10, 64, 1, 2, max_seq_len=8, dropout=0.0, rel_buckets=8)
+        RoPETransformerLM(10, 64, 1, 2, max_seq_len=8)
