@@ -58,7 +58,7 @@ def bucket_starts(num_buckets, max_distance):
 
 @functools.lru_cache(maxsize=64)
 def _starts_array(num_buckets, max_distance, causal):
-    """(array, its address, its length): the array is kept with the address."""
+    """(array, its address, its length): a caller keeps the array while it uses the address."""
     starts = bucket_starts(num_buckets if causal else num_buckets // 2, max_distance)
     array = (ctypes.c_int32 * len(starts))(*starts)
     return array, ctypes.addressof(array), len(starts)
@@ -78,13 +78,11 @@ def _heads_last(B, H, L, hd, like):
     return torch.empty_strided((B, H, L, hd), (L * H * hd, hd, H * hd, 1), dtype=like.dtype, device=like.device)
 
 
-def _inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start):
+def _inputs(q, k, v, bias, starts, causal, scale, lengths, start_rows, start):
     """The struct's fields up to scale."""
     B, H, Lq, hd = q.shape
-    buckets = bias.shape[0]
-    _, starts, n_starts = _starts_array(buckets, max_distance, causal)
     return (q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bias.data_ptr(),
-            starts, buckets, n_starts, 0 if lengths is None else lengths.data_ptr(),
+            starts[1], bias.shape[0], starts[2], 0 if lengths is None else lengths.data_ptr(),
             4 if lengths is None else lengths.element_size(), 0 if start_rows is None else start_rows.data_ptr(),
             4 if start_rows is None else start_rows.element_size(), start, B, H, k.shape[1], Lq, k.shape[2], hd, causal,
             _DTYPES[q.dtype], _DTYPES[bias.dtype], scale)
@@ -110,8 +108,9 @@ def bias_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     nbytes = _lib.workspace_bytes("mb_bias_attn_fwd_workspace", B, H, k.shape[1], Lq, k.shape[2], hd, causal,
                                   _DTYPES[q.dtype])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    starts = _starts_array(bias.shape[0], max_distance, causal)
     _lib.call_on(dev, "mb_bias_attn_fwd",
-                 _ARGS.pack(*_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
+                 _ARGS.pack(*_inputs(q, k, v, bias, starts, causal, scale, lengths, start_rows, start),
                             o.data_ptr(), *o.stride()[:3], lse.data_ptr() if want_lse else 0, *_NO_BACKWARD,
                             ws.data_ptr() if nbytes else 0, nbytes))
     return o, lse
@@ -140,8 +139,9 @@ def bias_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch
     nbytes = _lib.workspace_bytes("mb_bias_attn_bwd_workspace", B, H, Hk, Lq, Lk, hd, causal,
                                   _DTYPES[q.dtype], bias.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    starts = _starts_array(bias.shape[0], max_distance, causal)
     _lib.call_on(dev, "mb_bias_attn_bwd",
-                 _ARGS.pack(*_inputs(q, k, v, bias, max_distance, causal, scale, lengths, start_rows, start),
+                 _ARGS.pack(*_inputs(q, k, v, bias, starts, causal, scale, lengths, start_rows, start),
                             o.data_ptr(), *o.stride()[:3], lse.data_ptr(), d_o.data_ptr(), *d_o.stride()[:3],
                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3],
                             *dv.stride()[:3], dbias.data_ptr() if want_dbias else 0, ws.data_ptr(), nbytes))

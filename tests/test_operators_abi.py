@@ -219,3 +219,28 @@ def test_a_model_that_does_not_drop_out_probabilities_says_so():
         warnings.simplefilter("error")
         RoPETransformerLM(10, 64, 1, 2, max_seq_len=8, dropout=0.0, rel_buckets=8)
         RoPETransformerLM(10, 64, 1, 2, max_seq_len=8)
+
+
+def test_the_first_distances_live_until_the_call_is_made(monkeypatch):
+    """The struct holds their address; a cache may drop the array meanwhile (another thread's calls)."""
+    import weakref
+
+    from mathbrain import _lib, bias_attention
+    alive, calls = [], []
+
+    def starts(num_buckets, max_distance, causal):
+        array = (ctypes.c_int32 * 4)(0, 1, 2, 3)
+        alive.append(weakref.ref(array))
+        return array, ctypes.addressof(array), 4
+
+    def call(dev, name, args):
+        calls.append(name)
+        assert alive[-1]() is not None, name
+    monkeypatch.setattr(bias_attention, "_starts_array", starts)
+    monkeypatch.setattr(_lib, "call_on", call)
+    monkeypatch.setattr(_lib, "workspace_bytes", lambda *sizes: 16)
+    x = torch.zeros(1, 1, 2, 32)
+    rest = (8, True, 1.0, None, None, 0, True)
+    o, lse = bias_attention.bias_attn_fwd(x, x, x, torch.zeros(4, 1), *rest)
+    bias_attention.bias_attn_bwd(x, x, x, torch.zeros(4, 1), o, x, lse, *rest)
+    assert calls == ["mb_bias_attn_fwd", "mb_bias_attn_bwd"]
