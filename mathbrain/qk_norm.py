@@ -131,6 +131,8 @@ def _check(q, k, q_weight, k_weight, cos, sin, start):
         raise ValueError(f"{what}: tables {tuple(cos.shape)}, {tuple(sin.shape)} are not [positions, {hd // 2}]")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"{what}: the tables must be contiguous float32")
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
+        raise ValueError(f"{what}: the tables get no gradient, and one of them requires it")
     if rows is not None and (rows.shape != qs[:1] or rows.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"{what}: start {tuple(rows.shape)} {rows.dtype} is not one int32 or int64 for each of "
                          f"{qs[0]} rows")
@@ -138,7 +140,7 @@ def _check(q, k, q_weight, k_weight, cos, sin, start):
 
 def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, eps=1e-6, start=0):
     """Normalises and rotates q [B, L, H, hd] and k [B, L, Hk, hd] (fp32 or bf16, any strides);
-    weights [hd]; ``cos`` / ``sin`` [positions, hd / 2] fp32.  ``start`` is the position of each
+    weights [hd]; ``cos`` / ``sin`` [positions, hd / 2] fp32, without gradients.  ``start`` is the position of each
     row's first token: an int (checked against the tables), or an int32 / int64 tensor [B], as a
     step that appends one token to sequences of different lengths has it; a position outside the
     tables gives NaN rows there.  head_dim 32, 64 or 128."""

@@ -261,3 +261,18 @@ def test_forward_mode_derivatives_are_refused():
                 with grad(), pytest.raises(NotImplementedError, match="jvp"):
                     qk_norm_rotary(*args, cos, sin)
         assert all(torch.equal(a, b) for a, b in zip(qk_norm_rotary(x, x, w, w, cos, sin), want))
+
+
+def test_tables_that_require_a_gradient_are_refused():
+    """They would get none."""
+    from mathbrain.qk_norm import qk_norm_rotary
+    cos, sin = (t.cuda() for t in tables(32, 8))
+    w = torch.rand(32, device="cuda", requires_grad=True)
+    x = torch.randn(2, 3, 2, 32, device="cuda")
+    want = qk_norm_rotary(x, x, w, w, cos, sin)
+    for c, s in ((cos.clone().requires_grad_(), sin), (cos, sin.clone().requires_grad_())):
+        for weight in (w, w.detach()):
+            with pytest.raises(ValueError, match="get no gradient"):
+                qk_norm_rotary(x, x, weight, weight, c, s)
+        with torch.no_grad():
+            assert all(torch.equal(a, b) for a, b in zip(qk_norm_rotary(x, x, w, w, c, s), want))
