@@ -664,11 +664,11 @@ int64_t padded(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
 // there are few, most of the device would wait for the longest.  The time is counted in tiles: a run's
 // own start and end, that of the launch which adds the runs, and what two workgroups of a CU take
 // from each other.  Measured, split against not, dq / dk and dv, launches that add included:
-// causal bf16 heads of 64, 2 x 1310, 8 heads (176 workgroups, 21 tiles) 36 us against 44 / 31 against
-// 39; 9 x 2259, one head 44 against 67 / 39 against 62; heads of 128, 2 x 1516, 4 heads on 2 key
-// heads 55 against 74 / 46 against 131; fp32 heads of 64, 3 x 1000, 8 heads 79 against 128 / 98 against
-// 158; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key heads 209 against 254 / 245 against 1180;
-// 1 x 383, 5 heads of 128, runs of 64 rows 38 against 49 / 36 against 52 with three runs.
+// causal bf16 heads of 64, 2 x 1310, 8 heads (176 workgroups, 21 tiles) 32 us against 41 / 31 against
+// 38; 9 x 2259, one head 40 against 63 / 39 against 59; heads of 128, 2 x 1516, 4 heads on 2 key
+// heads 41 against 72 / 45 against 122; fp32 heads of 64, 3 x 1000, 8 heads 77 against 124 / 100 against
+// 160; fp32 heads of 128, 1 x 1081 both directions, 16 heads on 4 key heads 193 against 252 / 204 against 1180;
+// 1 x 383, 5 heads of 128, runs of 64 rows 37 against 47 / 36 against 52 with three runs.
 int parts_of(int64_t groups, int64_t steps, int per_cu, bool causal, int dtype) {
     if (groups < 1 || groups > 512) return 1;
     const bool f32 = dtype == MB_DTYPE_F32;   // whose tiles keep a CU busy by one workgroup
@@ -684,8 +684,8 @@ int parts_of(int64_t groups, int64_t steps, int per_cu, bool causal, int dtype) 
         if (cost < (best == 1 ? 0.95 : 1.0) * least) least = cost, best = n;
     }
     // the longest walk is twice the mean under a causal mask (3 x 3461, 5 heads of 32, 420 workgroups of 55 tiles: 64 us
-    // against 91 / 56 against 73; but 448 of 16 tiles: 52 against 42 / 50 against 37; fp32, 9 x 900, 6 heads of 64, 432 of 15
-    // tiles: 141 against 151 / 157 against 190)
+    // against 89 / 58 against 72; but 448 of 16 tiles: 49 against 38 / 50 against 35; fp32, 9 x 900, 6 heads of 64, 432 of 15
+    // tiles: 147 against 150 / 164 against 193)
     if (best == 1 && causal && per_cu == 2 && groups > 256 && steps >= (f32 ? 12 : 24)) best = 2;
     return best;
 }

@@ -206,11 +206,11 @@ int launch_sets(const Args& a, hipStream_t st) {
     return check_launch("mb_bias_attn_fwd");
 }
 
-// Two sets of waves where the grid leaves room for them on its CUs and the walks are long.  Measured
-// in bf16, two sets against one, 8 heads: of 64: 2 x 2048 (256 workgroups) 32 us against 41, 3 x 2048 36
-// against 44, 12 x 512 24 against 21, 4 x 2048 46 against 44; of 128: 2 x 2048 44 against 53, 3 x 2048 53 against
-// 59, 12 x 512 31 against 27; of 32: 4 x 2048 29 against 37;
-// fp32, 16 heads of 128, 1 x 1081 157 against 165, but 8 heads, 8 x 1000 (512 workgroups) 209 against 178.
+// Two sets of waves where the grid leaves room for them on its CUs and the walks are long.  Measured in a
+// captured graph, two sets against one, causal, 8 heads: bf16 of 64: 2 x 2048 (256 workgroups) 28 us against 35, 3 x 2048
+// 29 against 35, 12 x 512 18 against 15, 4 x 2048 42 against 37; of 128: 2 x 2048 38 against 45, 3 x 2048 43 against
+// 49, 12 x 512 27 against 23; of 32: 4 x 2048 25 against 32; fp32 of 64: 3 x 400 35 against 39; of 32, both directions: 23
+// against 26; of 128: 4 x 1100 152 against 177, but 8 x 1000 (512 workgroups) 200 against 168.
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t st) {
     const int blocks = a.B * a.H * a.nq;
@@ -219,13 +219,13 @@ int launch(const Args& a, hipStream_t st) {
 }
 
 // Runs that a workgroup's walk is split into, in fp32, where a tile takes three times as long as in
-// bf16 and uneven shares of the CUs cost as much more.  Measured, with the launch that joins the
+// bf16 and uneven shares of the CUs cost as much more.  Measured in a captured graph, with the launch that joins the
 // runs, against one run of two sets of waves: 2 x 2854 both directions, 6 heads of 32 (276 workgroups), 3 runs
-// 174 us against 223; 1 x 1102 queries of 1936, 16 heads of 64, 5 runs 94 against 143; 10 x 1466, 2 heads
-// of 64, 3 runs 87 against 112; 1 x 1081 both directions, 16 heads of 128, 3 runs 114 against 146 (4 runs 133);
-// 2 x 700, 4 heads of 128, 5 runs 37 against 96; 1 x 383, 5 heads of 128, 5 runs 27 against 61; 4 x 553, 4 heads of 64, 4
-// runs 30 against 47; but 8 x 400, 6 heads of 64 (192 workgroups), 3 runs 39 against 36.
-// bf16 at these sizes: 2 runs 2 to 50 % slower.
+// 159 us against 210; 1 x 1102 queries of 1936, 16 heads of 64, 5 runs 81 against 139; 10 x 1466, 2 heads
+// of 64, 3 runs 81 against 107; 1 x 1081 both directions, 16 heads of 128, 3 runs 116 against 150 (4 runs 134);
+// 2 x 700, 4 heads of 128, 8 runs 39 against 97 (5 runs 39; both directions 48 and 42 against 99); 1 x 383, 5 heads of 128,
+// 5 runs 27 against 60; 4 x 553, 4 heads of 64, 4 runs 30 against 45; but 8 x 400, 6 heads of 64 (192 workgroups), 3 runs
+// 42 against 36.  bf16 at these sizes: 2 runs 2 to 50 % slower.
 int o_parts_of(int B, int H, int Lq, int Lk, int hd, int dtype) {
     const int64_t blocks = (int64_t)B * H * (((int64_t)Lq + kRows - 1) / kRows);
     const bool early = hd == 128 || blocks <= 64;

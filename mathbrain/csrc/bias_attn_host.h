@@ -36,11 +36,11 @@ inline bool rows16(const void* p, const int64_t* st, int dtype) {
 // workgroups walk all keys for 128 queries of a head.  The latter leaves CUs idle where its grid is
 // small, and its time is that of its longest walk; the former takes a few us more to start and
 // join, and a time that grows with the pairs.  The one is the shorter where the pairs that a mask
-// leaves fill few workgroups and the keys are many.  Measured in bf16, split against not, 8 heads:
-// of 64: 1 x 1024 23 us against 22, 1 x 2048 34 against 32, 4 x 128 queries of 4096 keys 36 against 52, 1 x 256
-// of 4096 22 against 50; of 128: 1 x 2048 75 against 50, 4 x 128 of 4096 55 against 70; of 32: 1 x 2048
-// 25 against 27.  Up to 32 rows for a key head are one column block of the split kernel (16 x 1 of
-// 4096, 8 heads x 64: 27 us against 97).
+// leaves fill few workgroups and the keys are many.  Measured in bf16 in a captured graph, split against not, 8 heads:
+// of 64: 1 x 1024 15 us against 17, 1 x 2048 30 against 27, 4 x 128 queries of 4096 keys 32 against 46, 1 x 256 of 4096
+// 18 against 45; of 128: 1 x 2048 71 against 37, 4 x 128 of 4096 50 against 64; of 32: 1 x 2048 21 against 23.  Up to
+// 32 rows for a key head are one column block of the split kernel: 16 x 1 of 4096, 8 heads x 64, 29 us against 44, in
+// fp32, for which the number of parts was not fitted, 67 against 75 (with 4 parts instead of 6: 58).
 inline int splits_of(int B, int H, int Hk, int Lq, int Lk, int hd, int causal) {
     const int64_t G = H / Hk, tiles = (G * Lq + 31) / 32, nq = ((int64_t)Lq + kRows - 1) / kRows;
     if (G > 32 || (double)B * Hk * tiles > kMostGroups) return 0;
