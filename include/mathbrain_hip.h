@@ -644,6 +644,32 @@ int64_t mb_qk_norm_rotary_bwd_workspace(int B, int L, int hd);
 int mb_qk_norm_rotary_bwd(const mb_qk_norm_rotary *args, void *stream);
 
 /*
+ * Rotary positions (the rotation of mathbrain/baseline.py:31-70, in two layouts and for a part of
+ * the head): with pair i = channels (a, b) of the row at position p,
+ *
+ *   out[a] = x[a] cos[p,i] - x[b] sin[p,i],  out[b] = x[a] sin[p,i] + x[b] cos[p,i]
+ *
+ * in fp32, every operation rounded by itself, the results to the dtype; channels from `turned` on are
+ * copied.  The arguments come in a struct on the HOST, read before the call returns.
+ */
+typedef struct mb_rotary {
+    const void *q, *k;            /* [B, L, H | Hk, hd], channels next to each other; element strides */
+    int64_t q_st[3], k_st[3];     /*   of B, L and H.  H or Hk may be 0 (that side is not used) */
+    const float *cos, *sin;       /* [table_rows, turned / 2] contiguous */
+    int64_t table_rows;
+    const void *start;            /* [B] position of each row's first token, or [B, L] of each token, or */
+    int64_t start_bytes, start_per_token, start0; /* NULL: start0. A position outside the tables gives NaN */
+                                  /*   start_bytes 4: int32, 8: int64 */
+    int64_t B, L, H, Hk, hd, turned;
+    int64_t layout;               /* 0: pairs (2i, 2i + 1), 1: pairs (i, i + turned / 2) */
+    int64_t inverse;              /* 1: by the opposite angles (the gradients) */
+    int64_t dtype;                /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
+    void *q_out, *k_out;          /* [B, L, H | Hk, hd] contiguous; not the inputs' memory */
+} mb_rotary;
+
+int mb_apply_rotary(const mb_rotary *args, void *stream);
+
+/*
  * Attention with a learned relative position bias by distance buckets:
  *
  *   s_ij = scale q_i . k_j + bias[bucket(pos_i - j), h],  p = softmax_j(s),  o_i = sum_j p_ij v_j

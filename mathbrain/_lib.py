@@ -77,6 +77,7 @@ SIGNATURES = {
     "mb_qk_norm_rotary_fwd": ([_p, _p], _i),
     "mb_qk_norm_rotary_bwd": ([_p, _p], _i),
     "mb_qk_norm_rotary_bwd_workspace": ([_i, _i, _i], _i64),
+    "mb_apply_rotary": ([_p, _p], _i),
     "mb_bias_attn_fwd": ([_p, _p], _i),
     "mb_bias_attn_fwd_workspace": ([_i] * 8, _i64),
     "mb_bias_attn_bwd": ([_p, _p], _i),
@@ -186,6 +187,11 @@ def wants_derivatives(*tensors):
     tangent (forward-mode dual tensors require none, with gradients enabled or not).  Where it does not,
     an entry point of a few microseconds calls its kernels directly."""
     return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+
+
+def has_tangent(*tensors):
+    """Whether one of the tensors has a forward-mode tangent."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def require_gpu(*tensors, what="mathbrain"):

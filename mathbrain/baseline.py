@@ -12,7 +12,10 @@ tables instead of the reference's complex multiply (the same rotation).
 in the rotation's own pass (``qk_norm_rotary``).  ``rel_buckets=n`` (not in the reference)
 adds a learned bias by distance buckets to every layer's scores, one table [n, heads] for all
 layers, in the attention that reads it (``relative_bias_attention``, which replaces torch's
-there; its probabilities are not dropped out, the block's output is).
+there; its probabilities are not dropped out, the block's output is).  The rotation without head
+norms is one launch a direction (``apply_rotary``); ``rope_layout``, ``rope_dims`` and ``rope_scaling``
+(not in the reference) choose its pairs, the part of each head that turns, and tables for longer
+contexts.
 """
 import warnings
 
@@ -23,6 +26,8 @@ import torch.nn.functional as F
 from .bias_attention import relative_bias_attention
 from .model import RMSNorm, SwiGLU
 from .qk_norm import qk_norm_rotary
+from .rotary import LAYOUTS, apply_rotary
+from .rotary import rotary_tables as scaled_rotary_tables
 
 
 def rotary_tables(head_dim, max_len, theta=10000.0):
@@ -45,9 +50,11 @@ def rotate(x, cos, sin):
 class CausalSelfAttention(nn.Module):
     """baseline.py:31-70."""
 
-    def __init__(self, d_model: int, n_heads: int, dropout: float = 0.0, qk_norm: bool = False):
+    def __init__(self, d_model: int, n_heads: int, dropout: float = 0.0, qk_norm: bool = False,
+                 rope_layout: str = "interleaved"):
         super().__init__()
         assert d_model % n_heads == 0
+        self.rope_layout = rope_layout
         self.d_model = d_model
         self.n_heads = n_heads
         self.head_dim = d_model // n_heads
@@ -69,7 +76,11 @@ class CausalSelfAttention(nn.Module):
         if self.qk_norm:
             q, k = qk_norm_rotary(q, k, self.q_norm.weight, self.k_norm.weight, cos.float(), sin.float(),
                                   self.q_norm.eps)
+        elif q.dtype in (torch.float32, torch.bfloat16):
+            q, k = apply_rotary(q, k, cos.float(), sin.float(), layout=self.rope_layout)
         else:
+            if self.rope_layout != "interleaved" or 2 * cos.shape[1] != self.head_dim:
+                raise ValueError(f"CausalSelfAttention: rope_layout and rope_dims take float32 or bfloat16 (got {q.dtype})")
             q, k = rotate(q, cos, sin), rotate(k, cos, sin)
         q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = self.wv(x).view(shape).transpose(1, 2)
@@ -84,10 +95,11 @@ class CausalSelfAttention(nn.Module):
 class RoPETransformerBlock(nn.Module):
     """baseline.py:72-84."""
 
-    def __init__(self, d_model: int, n_heads: int, d_ff: int, dropout: float = 0.0, qk_norm: bool = False):
+    def __init__(self, d_model: int, n_heads: int, d_ff: int, dropout: float = 0.0, qk_norm: bool = False,
+                 rope_layout: str = "interleaved"):
         super().__init__()
         self.attn_norm = RMSNorm(d_model)
-        self.attn = CausalSelfAttention(d_model, n_heads, dropout, qk_norm)
+        self.attn = CausalSelfAttention(d_model, n_heads, dropout, qk_norm, rope_layout)
         self.ffn_norm = RMSNorm(d_model)
         self.ffn = SwiGLU(d_model, d_ff)
 
@@ -102,12 +114,22 @@ class RoPETransformerLM(nn.Module):
     ``qk_norm``: RMS norms of every query and key head.  ``rel_buckets``: a learned bias by that
     many distance buckets, up to ``rel_max_distance`` (0: none); the probabilities are not dropped
     out then, and a ``dropout`` above 0 warns of it.  Both take head_dim 32, 64 or 128; the bias
-    starts as zeros."""
+    starts as zeros.  ``rope_layout``: "interleaved" (the reference's) or "half"; ``rope_dims``: the first channels of
+    each head that turn (all); ``rope_scaling``: keyword arguments of rotary.rotary_tables for longer contexts, such as
+    dict(scaling="yarn", factor=4, trained=4096).  With ``qk_norm`` whole heads turn, interleaved."""
 
     def __init__(self, vocab_size: int, d_model: int, n_layers: int, n_heads: int,
                  max_seq_len: int = 4096, dropout: float = 0.1, qk_norm: bool = False,
-                 rel_buckets: int = 0, rel_max_distance: int = 128):
+                 rel_buckets: int = 0, rel_max_distance: int = 128, rope_layout: str = "interleaved", rope_dims=None,
+                 rope_scaling=None):
         super().__init__()
+        head_dim = d_model // n_heads
+        if rope_layout not in LAYOUTS:
+            raise ValueError(f"RoPETransformerLM: rope_layout={rope_layout!r} ('interleaved' or 'half')")
+        if rope_dims is not None and not (0 < rope_dims <= head_dim and rope_dims % 2 == 0):
+            raise ValueError(f"RoPETransformerLM: rope_dims={rope_dims} (an even number, at most head_dim {head_dim})")
+        if qk_norm and (rope_layout != "interleaved" or rope_dims not in (None, head_dim)):
+            raise ValueError("RoPETransformerLM: qk_norm turns whole heads, interleaved")
         if rel_buckets and dropout:
             warnings.warn(f"RoPETransformerLM: with rel_buckets the attention's probabilities are not dropped out; "
                           f"dropout={dropout} is that of the blocks' outputs alone", stacklevel=2)
@@ -115,14 +137,17 @@ class RoPETransformerLM(nn.Module):
         self.d_model = d_model
         self.embed = nn.Embedding(vocab_size, d_model)
         d_ff = 256 * ((int(8 * d_model / 3) + 255) // 256)
-        self.layers = nn.ModuleList([RoPETransformerBlock(d_model, n_heads, d_ff, dropout, qk_norm)
+        self.layers = nn.ModuleList([RoPETransformerBlock(d_model, n_heads, d_ff, dropout, qk_norm, rope_layout)
                                      for _ in range(n_layers)])
         self.final_norm = RMSNorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)
         self.lm_head.weight = self.embed.weight
         self.rel_bias = nn.Parameter(torch.zeros(rel_buckets, n_heads)) if rel_buckets else None
         self.rel_max_distance = rel_max_distance
-        cos, sin = rotary_tables(d_model // n_heads, max_seq_len)
+        if rope_dims is None and rope_scaling is None:
+            cos, sin = rotary_tables(head_dim, max_seq_len)
+        else:
+            cos, sin = scaled_rotary_tables(rope_dims or head_dim, max_seq_len, **(rope_scaling or {}))
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
 
