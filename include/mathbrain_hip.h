@@ -716,6 +716,37 @@ int64_t mb_bias_attn_bwd_workspace(int B, int H, int Hk, int Lq, int Lk, int hd,
 int mb_bias_attn_bwd(const mb_bias_attn *args, void *stream);
 
 /*
+ * Softmax cross entropy of a linear layer's outputs (the tied lm_head of mathbrain/model.py:186 and the
+ * loss of the training step), which are not kept, and its gradients:
+ *
+ *   s_nv = hidden_n . weight_v,  loss_n = log sum_v exp(s_nv) - s_n,target(n)
+ *   dhidden_n = g_n sum_v (softmax(s_n)_v - [v = target]) weight_v,  dweight_v = sum_n (...) g_n hidden_n
+ *
+ * Products of bf16 values are exact; fp32 values go as two fp16 planes (24 bits).  Sums have a fixed order.
+ * The arguments come in a struct on the HOST, read before the call returns.
+ */
+typedef struct mb_linear_ce {
+    const void *hidden, *weight;  /* [N, D], [V, D], elements of a row next to each other, rows */
+    int64_t hidden_ld, weight_ld; /*   this many elements apart */
+    const void *target;           /* [N]; ignore_index: the row has loss 0 and no gradient. Another one */
+    int64_t target_bytes, ignore_index; /* outside [0, V): NaN. 4: int32, 8: int64 */
+    int64_t N, V, D, dtype;       /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
+    int64_t reduction;            /* 0: each row's loss, 1: the mean over the rows that count (NaN for */
+                                  /*   none), 2: the sum */
+    float *loss;                  /* forward: [N] or one */
+    float *lse, *count;           /* [2, N] the rows' maxima and log2 of their sums; the rows that count: */
+                                  /*   written by the forward, read by the backward */
+    const float *dloss;           /* backward: [N] or one */
+    void *dhidden, *dweight;      /* backward: [N, D], [V, D] contiguous, of dtype; either may be NULL */
+    void *workspace;              /* at a multiple of 256 bytes, mb_linear_ce_workspace(args, backward) */
+    int64_t workspace_bytes;      /*   bytes (-1: the arguments are refused) */
+} mb_linear_ce;
+
+int64_t mb_linear_ce_workspace(const mb_linear_ce *args, int backward);
+int mb_linear_ce_fwd(const mb_linear_ce *args, void *stream);
+int mb_linear_ce_bwd(const mb_linear_ce *args, void *stream);
+
+/*
  * Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_ in the reference's training
  * step):
  *

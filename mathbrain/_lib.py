@@ -82,6 +82,9 @@ SIGNATURES = {
     "mb_bias_attn_fwd_workspace": ([_i] * 8, _i64),
     "mb_bias_attn_bwd": ([_p, _p], _i),
     "mb_bias_attn_bwd_workspace": ([_i] * 9, _i64),
+    "mb_linear_ce_workspace": ([_p, _i], _i64),
+    "mb_linear_ce_fwd": ([_p, _p], _i),
+    "mb_linear_ce_bwd": ([_p, _p], _i),
     "mb_grad_clip": ([_p, _p, _p, _p, _p, _i, _f, _p, _p, _i64, _p], _i),
     "mb_grad_clip_workspace": ([_i], _i64),
     "mb_swiglu_fwd": ([_p, _p, _i64, _i, _p, _p], _i),

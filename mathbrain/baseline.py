@@ -24,6 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .bias_attention import relative_bias_attention
+from .linear_cross_entropy import linear_cross_entropy
 from .model import RMSNorm, SwiGLU
 from .qk_norm import qk_norm_rotary
 from .rotary import LAYOUTS, apply_rotary
@@ -116,7 +117,10 @@ class RoPETransformerLM(nn.Module):
     out then, and a ``dropout`` above 0 warns of it.  Both take head_dim 32, 64 or 128; the bias
     starts as zeros.  ``rope_layout``: "interleaved" (the reference's) or "half"; ``rope_dims``: the first channels of
     each head that turn (all); ``rope_scaling``: keyword arguments of rotary.rotary_tables for longer contexts, such as
-    dict(scaling="yarn", factor=4, trained=4096).  With ``qk_norm`` whole heads turn, interleaved."""
+    dict(scaling="yarn", factor=4, trained=4096).  With ``qk_norm`` whole heads turn, interleaved.
+
+    forward(x, targets) is the mean cross entropy over the targets that are not ``ignore_index``, without the logits
+    (``linear_cross_entropy`` with lm_head's weight)."""
 
     def __init__(self, vocab_size: int, d_model: int, n_layers: int, n_heads: int,
                  max_seq_len: int = 4096, dropout: float = 0.1, qk_norm: bool = False,
@@ -151,10 +155,13 @@ class RoPETransformerLM(nn.Module):
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
 
-    def forward(self, x):
+    def forward(self, x, targets=None, ignore_index=-1):
         L = x.shape[1]
         cos, sin = self.rope_cos[:L], self.rope_sin[:L]
         h = self.embed(x)
         for layer in self.layers:
             h = layer(h, cos, sin, self.rel_bias, self.rel_max_distance)
-        return self.lm_head(self.final_norm(h))
+        h = self.final_norm(h)
+        if targets is not None:
+            return linear_cross_entropy(h, self.lm_head.weight, targets, ignore_index)
+        return self.lm_head(h)

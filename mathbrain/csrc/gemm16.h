@@ -1,0 +1,278 @@
+// Products of matrices held in 16-bit planes, for the kernels that fuse something around them.
+//
+//   acc[p][q] = sum_k P[p][k] Q[q][k],  fp32 accumulation in the 32 x 32 x 16 matrix instructions
+//
+// One plane: bf16 or fp16 values.  Two planes: fp32 values as x = hi + lo, both fp16 (24 bits of x
+// where it is within 2^-17 of the matrix's largest, see split.h's scales), from three products
+// lo hi + hi lo + hi hi; the fourth is below fp32's own rounding.
+//
+// A workgroup of four waves (2 x 2) takes a TP x TQ tile of the result and walks k in steps of 32.
+// Operand tiles go from memory straight into LDS, kStages - 1 steps ahead, 16 bytes a lane.  Such a
+// load puts its 64 pieces next to each other, so a row has no padding; piece c of row r lies in the
+// place c ^ swz(r) instead, which spreads the reads over the banks.  An operand may have its k next to
+// each other (kRows) or its free index (kCols: read back by the transposing 16-bit LDS read).
+//
+// Buffers are padded: kRows operands have whole steps of 32 k (zeros behind the matrix on one side at
+// least), kCols operands whole steps of 32 rows and rows of a multiple of 8 elements.  Tiles that pass
+// the free index's end read the last rows (or pieces) again; whoever uses acc leaves those out.
+//
+// A lane holds, of each 32 x 32 block, column q = lane % 32 and the rows p = 8 (r / 4) + 4 (lane / 32) + r % 4.
+#pragma once
+
+#include "common.h"
+
+#include <atomic>
+
+namespace mb {
+namespace g16 {
+
+constexpr int kThreads = 256;
+constexpr int kStep = 32;       // k of a step
+
+typedef __attribute__((__ext_vector_type__(8))) _Float16 f16x8;
+typedef __attribute__((__ext_vector_type__(4))) _Float16 f16x4;
+typedef __attribute__((__ext_vector_type__(8))) __bf16 bf16x8;
+typedef __attribute__((__ext_vector_type__(4))) short s16x4;
+typedef __attribute__((__ext_vector_type__(8))) short s16x8;
+typedef __attribute__((__ext_vector_type__(16))) float f32x16;
+
+enum Order { kRows, kCols };
+
+// One operand: element (i, k) of a plane at p + i * ld + k (kRows) or p + k * ld + i (kCols).
+struct Side {
+    const void* p;
+    int64_t plane;   // bytes from the first plane (hi) to the second (lo)
+    int64_t ld;      // elements
+    int n;           // free indices that are there (at least 1)
+};
+
+__device__ inline f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ inline f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+template <typename T>
+struct Frag;
+template <>
+struct Frag<_Float16> { typedef f16x8 type; };
+template <>
+struct Frag<__bf16> { typedef bf16x8 type; };
+
+// 16 bytes a lane from base + voff to LDS at lds + 16 * lane.  M0 holds the LDS address; the compiler reserves it for
+// its own instructions, which set it before they use it, warns of the clobber for that reason, and has to know of it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ inline void dma16(uint32_t lds, uint32_t voff, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(voff), "s"(base)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// Waits until at most N of the wave's loads are on their way, and for the other waves.
+template <int N>
+__device__ inline void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+__device__ inline uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// A tile of N free indices by 32 k in LDS.
+template <typename T, int N, Order ORDER>
+struct Tile {
+    static constexpr int kBytes = N * kStep * 2;
+    static constexpr int kLoads = kBytes / 4096;                    // of each wave
+    static constexpr int kRow = ORDER == kRows ? kStep * 2 : N * 2; // bytes
+    static constexpr int kPieces = kRow / 16;
+    static_assert(kBytes % 4096 == 0 && N % 64 == 0, "a wave's load moves 1 KiB");
+    typedef __attribute__((address_space(3))) const char lds_char;
+
+    static __device__ constexpr int swz(int row) {
+        if (kPieces == 4) return (row >> 2) & 3;
+        if (kPieces == 8) return ((row >> 1) & 1) << 2 | ((row >> 3) & 1) << 1 | ((row >> 2) & 1);
+        return (row & 3) << 2 | ((row >> 2) & 3);
+    }
+    // This lane's offset of each of its wave's loads, from the tile's first element; i0 is the tile's first
+    // free index.
+    struct Offsets {
+        uint32_t v[kLoads];
+        __device__ Offsets(const Side& s, int i0) {
+            const int left = s.n - 1 - i0;
+            const int last = ORDER == kRows ? left : (int)(s.ld - 8) - i0;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int slot = j * kThreads + (int)threadIdx.x, row = slot / kPieces;
+                const int piece = (slot % kPieces) ^ swz(row);
+                if (ORDER == kRows) v[j] = (uint32_t)(min(row, last) * (int64_t)s.ld * 2) + piece * 16;
+                else v[j] = (uint32_t)(row * s.ld * 2) + min(piece * 8, last) * 2;
+            }
+        }
+    };
+    static __device__ void load(uint32_t tile, const char* base, const Offsets& off) {
+        const uint32_t lds = tile + wave_id() * 1024;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) dma16(lds + j * 4096, off.v[j], base);
+    }
+    // Bytes from the matrix's first element to the tile's.
+    static __device__ int64_t at(const Side& s, int i0, int k0) {
+        return (ORDER == kRows ? i0 * s.ld + k0 : (int64_t)k0 * s.ld + i0) * 2;
+    }
+    // Where this lane reads within a tile: the fragment of free indices i0 + lane % 32 (i0 a multiple of 32) and
+    // k = 16 c + 8 (lane / 32) + 0 .. 7.
+    struct Lane {
+        uint32_t v[ORDER == kRows ? 2 : 4];
+        __device__ Lane() {
+            const int lane = threadIdx.x & 63, g = lane >> 5;
+            if (ORDER == kRows) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) v[c] = (lane & 31) * kRow + (((2 * c + g) ^ swz(lane & 31)) << 4);
+            } else {
+                // 16 lanes read 4 rows of 16 free indices, 8 bytes each, and get 4 rows of one index each
+                const int d = (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int r = 16 * (c / 2) + 8 * g + 4 * (c % 2) + ((lane & 15) >> 2);
+                    v[c] = r * kRow + (((d >> 3) ^ swz(r)) << 4) + 2 * (d & 7);
+                }
+            }
+        }
+    };
+    static __device__ typename Frag<T>::type read(uint32_t tile, const Lane& l, int i0, int c) {
+        typedef typename Frag<T>::type F;
+        if constexpr (ORDER == kRows) {
+            return *(__attribute__((address_space(3))) const F*)((lds_char*)(uintptr_t)(tile + l.v[c]) + i0 * kRow);
+        } else {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            // 32 indices further, piece n becomes n ^ 4
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)(uintptr_t)(tile + (l.v[2 * c] ^ (i0 * 2))));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)(uintptr_t)(tile + (l.v[2 * c + 1] ^ (i0 * 2))));
+            return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+template <typename T_, int PLANES, int TP_, int TQ_, Order OP, Order OQ>
+struct Product {
+    typedef T_ T;
+    static constexpr int TP = TP_, TQ = TQ_;
+    static constexpr int WP = TP / 2, WQ = TQ / 2;     // of a wave
+    static constexpr int FP = WP / 32, FQ = WQ / 32;   // its 32 x 32 blocks
+    typedef Tile<T, TP, OP> TileP;
+    typedef Tile<T, TQ, OQ> TileQ;
+    static constexpr int kStage = PLANES * (TileP::kBytes + TileQ::kBytes);
+    // two workgroups a CU: 80 KiB of LDS each
+    static constexpr int kStages = 3 * kStage <= 81920 ? 3 : 2;
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kLoads = PLANES * (TileP::kLoads + TileQ::kLoads);
+
+    f32x16 acc[FP][FQ];
+
+    __device__ static int wave_p() { return (wave_id() & 1) * WP; }
+    __device__ static int wave_q() { return (wave_id() >> 1) * WQ; }
+    // the row within the tile of element r of block i, the column of block j
+    __device__ static int row(int i, int r) {
+        return wave_p() + 32 * i + 8 * (r / 4) + 4 * ((threadIdx.x & 63) >> 5) + r % 4;
+    }
+    __device__ static int col(int j) { return wave_q() + 32 * j + (threadIdx.x & 31); }
+
+    // k from k0 to k1, multiples of 32 (k1 > k0).  All waves have to be here; LDS is free again after the next barrier.
+    __device__ void run(const Side& p, const Side& q, int p0, int q0, int k0, int k1, void* smem) {
+        const uint32_t lds = lds_address(smem);
+        const typename TileP::Offsets po(p, p0);
+        const typename TileQ::Offsets qo(q, q0);
+        const typename TileP::Lane pl;
+        const typename TileQ::Lane ql;
+        const char* pb = (const char*)p.p + TileP::at(p, p0, k0);
+        const char* qb = (const char*)q.p + TileQ::at(q, q0, k0);
+        const int64_t pstep = TileP::at(p, 0, kStep), qstep = TileQ::at(q, 0, kStep);
+        const int steps = (k1 - k0) / kStep;
+        auto issue = [&](int t) {
+            const uint32_t tile = lds + t % kStages * kStage;
+#pragma unroll
+            for (int h = 0; h < PLANES; ++h) {
+                TileP::load(tile + h * TileP::kBytes, pb + h * p.plane, po);
+                TileQ::load(tile + PLANES * TileP::kBytes + h * TileQ::kBytes, qb + h * q.plane, qo);
+            }
+            pb += pstep, qb += qstep;
+        };
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // the compiler's own loads are done: it would wait for the DMA with them
+        for (int t = 0; t < kStages - 1 && t < steps; ++t) issue(t);
+        for (int t = 0; t < steps; ++t) {
+            if (t + kStages - 2 < steps) wait_and_meet<(kStages - 2) * kLoads>();
+            else wait_and_meet<0>();
+            if (t + kStages - 1 < steps) issue(t + kStages - 1);
+            const uint32_t ptile = lds + t % kStages * kStage, qtile = ptile + PLANES * TileP::kBytes;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                typename Frag<T>::type a[PLANES][FP], b[PLANES][FQ];
+#pragma unroll
+                for (int h = 0; h < PLANES; ++h) {
+#pragma unroll
+                    for (int i = 0; i < FP; ++i) a[h][i] = TileP::read(ptile + h * TileP::kBytes, pl, wave_p() + 32 * i, c);
+#pragma unroll
+                    for (int j = 0; j < FQ; ++j) b[h][j] = TileQ::read(qtile + h * TileQ::kBytes, ql, wave_q() + 32 * j, c);
+                }
+                if constexpr (PLANES == 2) {
+#pragma unroll
+                    for (int i = 0; i < FP; ++i)
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(a[1][i], b[0][j], acc[i][j]);
+#pragma unroll
+                    for (int i = 0; i < FP; ++i)
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(a[0][i], b[1][j], acc[i][j]);
+                }
+#pragma unroll
+                for (int i = 0; i < FP; ++i)
+#pragma unroll
+                    for (int j = 0; j < FQ; ++j) acc[i][j] = mma(a[0][i], b[0][j], acc[i][j]);
+            }
+        }
+    }
+};
+
+// ---- planes ------------------------------------------------------------------------------
+//
+// fp16 holds 11 bits within 2^-14 .. 65504 and 24 - k below 2^-14 2^-k; a matrix is scaled by the power of two that
+// brings its largest value to 2^14 .. 2^15, so that one plane holds bf16 values exactly down to 2^-21 of the largest
+// and within 2^-39 of the largest below, and two planes hold fp32 values to 24 bits down to 2^-15 of the largest.
+
+// The scale for a largest (finite) magnitude of these bits: 2^-46 to 2^74.
+__device__ inline float plane_scale(uint32_t bits) {
+    int e = (int)(bits >> 23);
+    e = e < 127 - 60 ? 127 - 60 : e > 127 + 60 ? 127 + 60 : e;
+    return __builtin_bit_cast(float, (uint32_t)(127 + 14 - (e - 127)) << 23);
+}
+// x = hi + lo; an infinite hi (or NaN) stands alone.
+__device__ inline void split(float x, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)x;
+    const float rest = x - (float)hi;
+    lo = (_Float16)(__builtin_isfinite(rest) ? rest : 0.f);
+}
+
+// ---- host side ---------------------------------------------------------------------------
+
+// Beyond 64 KiB of LDS a kernel has to be told, once on each device.  `told` is the kernel's own.
+struct Told {
+    std::atomic<bool> done[64] = {};
+};
+inline int allow_lds(const char* what, const void* kernel, int bytes, Told& told) {
+    if (bytes <= 65536) return MB_OK;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && dev < 64 && told.done[dev].load(std::memory_order_relaxed)) return MB_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail((int)e, "%s: %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+    if (dev < 64) told.done[dev].store(true, std::memory_order_relaxed);
+    return MB_OK;
+}
+
+inline int64_t pad(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+}  // namespace g16
+}  // namespace mb

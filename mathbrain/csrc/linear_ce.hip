@@ -1,0 +1,669 @@
+// Softmax cross entropy of a linear layer's outputs, without keeping them, with its gradients, on gfx950.
+//
+//   s_nv = h_n . w_v,   loss_n = log sum_v exp(s_nv) - s_n,t(n)
+//   U_nv = exp(s_nv) / sum_v' exp(s_nv') - [v = t(n)],   dh_n = g_n sum_v U_nv w_v,   dw_v = sum_n U_nv (g_n h_n)
+//
+// with the loss's gradient g_n of each row.  Rows with the ignored target have loss 0 and g_n = 0.
+//
+// Bound by the matrix instructions (gemm16.h).  Forward: workgroups take tiles of vocabulary x rows; a lane holds
+// the tile's vocabulary entries of a row in registers, so the tile's maximum and sum of exponentials need one
+// exchange; they go to memory, two floats for a tile's row, and a second kernel joins them in a fixed order.
+// Backward, for pieces of the vocabulary: the tile again, U as 16-bit planes to memory (U is within [-1, 1]: scaled
+// by 2^15, without g, whatever the gradient's size), then the two products with it.  Recomputing the scores takes
+// the time of one product; keeping them would take N V values.
+//
+// Scores are in units of log 2 (s log2 e, rounded once); a row's sum is kept as maximum and logarithm, two floats,
+// so that neither the loss nor a probability rounds their sum.
+#include "gemm16.h"
+
+#include <algorithm>
+
+namespace mb {
+namespace {
+
+using namespace g16;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kUScale = 32768.f;
+constexpr int kMaxBlocks = 512;     // of the kernels that look for the largest value
+constexpr int kRowsPerBlock = 16;   // of the joining kernel
+
+struct Targets {
+    const void* target;
+    int bytes;
+    int64_t ignore, V;
+    // the row's target, -1 where it is ignored, -2 where it is outside the vocabulary
+    __device__ int at(int64_t n) const {
+        const int64_t t = bytes == 8 ? ((const int64_t*)target)[n] : (int64_t)((const int32_t*)target)[n];
+        return t == ignore ? -1 : t < 0 || t >= V ? -2 : (int)t;
+    }
+};
+// The gradient of each row's loss; without dloss 1, and 0 for the ignored rows.
+struct RowGrad {
+    Targets t;
+    const float* dloss;      // [N] (reduction 0) or one
+    const float* count;      // rows that count (reduction 1)
+    int reduction;
+    __device__ float at(int64_t n) const {
+        if (t.at(n) == -1) return 0.f;
+        if (!dloss) return 1.f;
+        return reduction == 0 ? dloss[n] : reduction == 1 ? dloss[0] / count[0] : dloss[0];
+    }
+};
+
+__device__ inline float block_max(float v) {
+    __shared__ float s[kThreads / 64];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+
+template <typename T>
+__device__ inline void load8(const T* p, bool vec, int left, float* v) {
+    if (vec && left >= 8) {
+        typedef T vec8 __attribute__((ext_vector_type(8), aligned(16)));
+        const vec8 q = *reinterpret_cast<const vec8*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)q[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+    }
+}
+
+// A user's matrix: [rows, D], rows ld apart.
+struct Matrix {
+    const void* p;
+    int64_t ld;
+    int rows, D, vec;
+};
+
+// The largest finite magnitude of x (with g: of g_n x_n) of each workgroup's part: part[blockIdx.x].
+template <typename T, bool G>
+__global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Matrix x, const RowGrad g, float* part) {
+    const int pieces = (x.D + 7) / 8;
+    float most = 0.f;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)x.rows * pieces; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t n = i / pieces;
+        const int d = (int)(i - n * pieces) * 8;
+        float v[8];
+        load8((const T*)x.p + n * x.ld + d, x.vec, x.D - d, v);
+        const float gn = G ? fabsf(g.at(n)) : 1.f;
+        if (gn == 0.f) continue;   // whatever an ignored row holds
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float m = fabsf(v[e]) * gn;
+            most = fmaxf(most, m < INFINITY ? m : 0.f);
+        }
+    }
+    most = block_max(most);
+    if (threadIdx.x == 0) part[blockIdx.x] = most;
+}
+
+__device__ inline float scale_from(const float* part, int n) {
+    float m = 0.f;
+    for (int i = threadIdx.x; i < n; i += kThreads) m = fmaxf(m, part[i]);
+    return plane_scale(__builtin_bit_cast(uint32_t, block_max(m)));
+}
+
+// x (with g: g_n x_n) as PL planes [rows_pad, Dp] of O, zeros around it, scaled by the largest value of `part`
+// (parts 0: not scaled).  The scale goes to *scale.
+template <typename T, typename O, int PL, bool G>
+__global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Matrix x, const RowGrad g, const float* part, int parts, float* scale,
+                                                             O* out, int rows_pad, int Dp) {
+    float s = 1.f;
+    if (parts) {
+        s = scale_from(part, parts);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *scale = s;
+    }
+    const int pieces = Dp / 8;
+    typedef O vec8 __attribute__((ext_vector_type(8), aligned(16)));
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)rows_pad * pieces; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t n = i / pieces;
+        const int d = (int)(i - n * pieces) * 8;
+        float v[8];
+        if (n < x.rows) load8((const T*)x.p + n * x.ld + d, x.vec, x.D - d, v);
+        else
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (G && n < x.rows) {
+            const float gn = g.at(n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = gn == 0.f ? 0.f : v[e] * gn;
+        }
+        vec8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (PL == 2) {
+                _Float16 a, b;
+                split(v[e] * s, a, b);
+                hi[e] = a, lo[e] = b;
+            } else {
+                hi[e] = (O)(v[e] * s);
+            }
+        }
+        *reinterpret_cast<vec8*>(out + n * Dp + d) = hi;
+        if constexpr (PL == 2) *reinterpret_cast<vec8*>(out + ((int64_t)rows_pad + n) * Dp + d) = lo;
+    }
+}
+
+// Tiles to workgroups: each of the eight XCDs, to which workgroups go in turn, takes a run of the tiles, in which
+// eight tiles of rows walk the vocabulary together: what is at work at once on an XCD fits its L2.
+constexpr int kXcds = 8, kTogether = 8;
+__device__ inline bool tile_of(int tiles_p, int tiles_q, int& p, int& q) {
+    const int each = gridDim.x / kXcds;
+    const int64_t id = (int64_t)(blockIdx.x % kXcds) * each + blockIdx.x / kXcds;
+    if (id >= (int64_t)tiles_p * tiles_q) return false;
+    const int64_t run = (int64_t)tiles_p * kTogether;
+    const int group = (int)(id / run), rest = (int)(id - group * run);
+    const int wide = min(kTogether, tiles_q - group * kTogether);
+    p = rest / wide;
+    q = group * kTogether + rest % wide;
+    return true;
+}
+inline unsigned tile_grid(int64_t tiles) { return (unsigned)pad(tiles, kXcds); }
+
+struct ScoreArgs {
+    Side w, h;                    // kRows: [V, Dp], [N, Dp]
+    const float *scale_w, *scale_h;   // NULL: 1
+    Targets t;
+    int V, N, Dp, tiles_p, tiles_q;
+    float2* part;                 // forward: [tiles_p, N] maximum and sum
+    float* target_score;          // forward: [N]
+    const float* lse;             // backward: [2, N]
+    _Float16* u;                  // backward: [PL][n_pad, width], the piece's entries from v0 on
+    int v0, v1, n_pad;
+    int64_t width;
+};
+
+template <typename P>
+__device__ inline float score_factor(const ScoreArgs& a) {
+    return a.scale_w ? (1.f / *a.scale_w) * (1.f / *a.scale_h) * kLog2e : kLog2e;
+}
+
+template <typename P>
+__global__ void __launch_bounds__(kThreads, 2) ce_stats_kernel(const ScoreArgs a) {
+    extern __shared__ char smem[];
+    int tp, tq;
+    if (!tile_of(a.tiles_p, a.tiles_q, tp, tq)) return;
+    const int p0 = tp * P::TP, q0 = tq * P::TQ;
+    P prod;
+    const float f = score_factor<P>(a);
+    prod.run(a.w, a.h, p0, q0, 0, a.Dp, smem);
+    float2* both = (float2*)smem;   // [2][TQ]
+    float m[P::FQ], sum[P::FQ];
+    const bool tail = p0 + P::TP > a.V;
+#pragma unroll
+    for (int j = 0; j < P::FQ; ++j) {
+        const int n = q0 + P::col(j);
+        const int target = n < a.N ? a.t.at(n) : -1;
+        m[j] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float s = prod.acc[i][j][r] * f;
+                if (tail && p0 + P::row(i, r) >= a.V) s = -INFINITY;
+                prod.acc[i][j][r] = s;
+                m[j] = fmaxf(m[j], s);
+            }
+        m[j] = fmaxf(m[j], __shfl_xor(m[j], 32, 64));
+        const float base = m[j] == -INFINITY ? 0.f : m[j];
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t += __builtin_amdgcn_exp2f(prod.acc[i][j][r] - base);
+        sum[j] = t + __shfl_xor(t, 32, 64);
+        // the target's score, from the lane that holds it
+        const int at = target - p0 - P::wave_p();
+        if (__any(at >= 0 && at < P::WP)) {
+#pragma unroll
+            for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (target >= 0 && p0 + P::row(i, r) == target) a.target_score[n] = prod.acc[i][j][r];
+        }
+    }
+    __syncthreads();
+    const int half = wave_id() & 1;
+#pragma unroll
+    for (int j = 0; j < P::FQ; ++j)
+        if ((threadIdx.x & 63) < 32) both[half * P::TQ + P::col(j)] = make_float2(m[j], sum[j]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < P::TQ; c += kThreads)
+        if (q0 + c < a.N) {
+            const float2 x = both[c], y = both[P::TQ + c];
+            const float top = fmaxf(x.x, y.x), base = top == -INFINITY ? 0.f : top;
+            a.part[(int64_t)tp * a.N + q0 + c] =
+                make_float2(top, x.y * __builtin_amdgcn_exp2f(x.x - base) + y.y * __builtin_amdgcn_exp2f(y.x - base));
+        }
+}
+
+struct JoinArgs {
+    const float2* part;
+    const float* target_score;
+    Targets t;
+    int N, parts, reduction;
+    float *loss, *lse, *count;
+    double* sums;     // [2, blocks]: losses and counted rows (reduction 1 and 2)
+};
+
+__global__ void __launch_bounds__(kThreads) ce_join_kernel(const JoinArgs a) {
+    constexpr int kSlices = kThreads / kRowsPerBlock;
+    __shared__ float2 s[kSlices][kRowsPerBlock + 1];
+    __shared__ double both[2][kRowsPerBlock];
+    const int c = threadIdx.x % kRowsPerBlock, slice = threadIdx.x / kRowsPerBlock;
+    const int n = blockIdx.x * kRowsPerBlock + c;
+    float m = -INFINITY, sum = 0.f;
+    auto take = [&](float2 x) {
+        const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.f : top;
+        sum = sum * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+        m = top;
+    };
+    if (n < a.N)
+        for (int i = slice; i < a.parts; i += kSlices) take(a.part[(int64_t)i * a.N + n]);
+    s[slice][c] = make_float2(m, sum);
+    __syncthreads();
+    if (slice == 0) {
+        for (int i = 1; i < kSlices; ++i) take(s[i][c]);
+        float loss = 0.f;
+        bool counts = false;
+        if (n < a.N) {
+            const int target = a.t.at(n);
+            counts = target != -1;
+            const float l = __builtin_log2f(sum);
+            if (counts) loss = target < 0 ? NAN : kLn2 * ((m - a.target_score[n]) + l);
+            a.lse[n] = target < 0 && counts ? NAN : m;     // a target outside the vocabulary: NaN, in the gradients too
+            a.lse[a.N + n] = l;
+            if (a.reduction == 0) a.loss[n] = loss;
+        }
+        both[0][c] = (double)loss;
+        both[1][c] = counts ? 1.0 : 0.0;
+    }
+    __syncthreads();
+    if (a.reduction && threadIdx.x < 2) {
+        double v = 0.0;
+        for (int i = 0; i < kRowsPerBlock; ++i) v += both[threadIdx.x][i];
+        a.sums[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = v;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) ce_total_kernel(const double* sums, int n, int reduction, float* loss, float* count) {
+    __shared__ double s[2][kThreads];
+    double a = 0.0, b = 0.0;
+    for (int i = threadIdx.x; i < n; i += kThreads) a += sums[i], b += sums[n + i];
+    s[0][threadIdx.x] = a, s[1][threadIdx.x] = b;
+    __syncthreads();
+    for (int half = kThreads / 2; half >= 1; half >>= 1) {
+        if (threadIdx.x < half) {
+            s[0][threadIdx.x] += s[0][threadIdx.x + half];
+            s[1][threadIdx.x] += s[1][threadIdx.x + half];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        *loss = (float)(reduction == 1 ? s[0][0] / s[1][0] : s[0][0]);
+        *count = (float)s[1][0];
+    }
+}
+
+// U of a piece of the vocabulary, zeros behind its end and behind the last row.
+template <typename P, int PL>
+__global__ void __launch_bounds__(kThreads, 2) ce_u_kernel(const ScoreArgs a) {
+    extern __shared__ char smem[];
+    int tp, tq;
+    if (!tile_of(a.tiles_p, a.tiles_q, tp, tq)) return;
+    const int p0 = a.v0 + tp * P::TP, q0 = tq * P::TQ;
+    P prod;
+    const float f = score_factor<P>(a);
+    prod.run(a.w, a.h, p0, q0, 0, a.Dp, smem);
+#pragma unroll
+    for (int j = 0; j < P::FQ; ++j) {
+        const int n = q0 + P::col(j);
+        if (n >= a.n_pad) continue;
+        const int target = n < a.N ? a.t.at(n) : -1;
+        const bool counts = target != -1;
+        const float m = counts ? a.lse[n] : 0.f, l = counts ? a.lse[a.N + n] : 0.f;
+        _Float16* to = a.u + (int64_t)n * a.width - a.v0;
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int v = p0 + P::row(i, r);
+                if (v - a.v0 >= a.width) continue;
+                f16x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float u = __builtin_amdgcn_exp2f((prod.acc[i][j][r + e] * f - m) - l);
+                    u = v + e == target ? u - 1.f : u;
+                    u = counts && v + e < a.v1 ? u * kUScale : 0.f;
+                    if constexpr (PL == 2) {
+                        _Float16 x, y;
+                        split(u, x, y);
+                        hi[e] = x, lo[e] = y;
+                    } else {
+                        hi[e] = (_Float16)u;
+                    }
+                }
+                *reinterpret_cast<f16x4*>(to + v) = hi;
+                if constexpr (PL == 2) *reinterpret_cast<f16x4*>(to + (int64_t)a.n_pad * a.width + v) = lo;
+            }
+    }
+}
+
+struct PartArgs {
+    Side p, q;
+    int tiles_p, tiles_q, splits, k1;   // k from 0 to k1, shared out to the splits in whole steps
+    float* out;                         // [splits][q.n, ld]
+    int64_t ld;
+    int add;                            // onto what is there
+};
+
+template <typename P>
+__global__ void __launch_bounds__(kThreads, 2) ce_part_kernel(const PartArgs a) {
+    extern __shared__ char smem[];
+    const int tiles = a.tiles_p * a.tiles_q;
+    const int split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
+    const int p0 = tile % a.tiles_p * P::TP, q0 = tile / a.tiles_p * P::TQ;
+    const int steps = a.k1 / kStep;
+    const int k0 = (int)((int64_t)steps * split / a.splits) * kStep, k1 = (int)((int64_t)steps * (split + 1) / a.splits) * kStep;
+    P prod;
+    prod.run(a.p, a.q, p0, q0, k0, k1, smem);
+#pragma unroll
+    for (int j = 0; j < P::FQ; ++j) {
+        const int q = q0 + P::col(j);
+        if (q >= a.q.n) continue;
+        float* to = a.out + ((int64_t)split * a.q.n + q) * a.ld;
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int p = p0 + P::row(i, r);
+                if (p >= a.ld) continue;
+                f32x4v v = {prod.acc[i][j][r], prod.acc[i][j][r + 1], prod.acc[i][j][r + 2], prod.acc[i][j][r + 3]};
+                if (a.add) v += *reinterpret_cast<const f32x4v*>(to + p);
+                *reinterpret_cast<f32x4v*>(to + p) = v;
+            }
+    }
+}
+
+// out[n, d] = factor (g_n) sum_s part[s][n, d], in the parts' order.
+template <typename T, bool G>
+__global__ void __launch_bounds__(kThreads) ce_sum_kernel(const float* part, int splits, int rows, int D, int ld, const float* scale,
+                                                          const RowGrad g, T* out) {
+    const float f = 1.f / *scale / kUScale;
+    const int pieces = ld / 4;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)rows * pieces; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t n = i / pieces;
+        const int d = (int)(i - n * pieces) * 4;
+        f32x4v v = *reinterpret_cast<const f32x4v*>(part + n * ld + d);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4v*>(part + ((int64_t)s * rows + n) * ld + d);
+        float fn = f;
+        if (G) {
+            const float gn = g.at(n);
+            fn = f * gn;
+            if (gn == 0.f) v = f32x4v{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) out[n * D + d + e] = (T)(v[e] * fn);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------
+
+// Cuts a workspace; with a null base only the size is wanted.
+struct Carve {
+    char* base;
+    int64_t used = 0;
+    template <typename T>
+    T* take(int64_t n) {
+        T* p = base ? (T*)(base + used) : nullptr;
+        used += pad(n * (int64_t)sizeof(T), 256);
+        return p;
+    }
+};
+
+// U's bytes in a piece: pieces are large enough to fill the card and small beside the scores.
+constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+constexpr int kSlots = 512;       // workgroups at work at once
+
+struct Plan {
+    int64_t N, V, D, Dp, Np, Vp, width;
+    bool f32, direct_h, direct_w;
+    int planes, tp, tq, tiles_p, tiles_q;   // of the scores
+    int s_h, s_w;                            // splits of the two gradients' products
+};
+
+int splits_of(int64_t tiles, int64_t k) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>({kSlots / tiles, k / 512, 64}));
+}
+
+Plan plan_of(const mb_linear_ce* a) {
+    Plan p = {};
+    p.N = a->N, p.V = a->V, p.D = a->D;
+    p.Dp = pad(p.D, kStep), p.Np = pad(p.N, kStep), p.Vp = pad(p.V, kStep);
+    p.f32 = a->dtype == MB_DTYPE_F32;
+    p.planes = p.f32 ? 2 : 1;
+    auto direct = [&](const void* x, int64_t ld) { return !p.f32 && p.D % kStep == 0 && ((uintptr_t)x & 15) == 0 && ld % 8 == 0; };
+    p.direct_h = direct(a->hidden, a->hidden_ld), p.direct_w = direct(a->weight, a->weight_ld);
+    p.tp = p.f32 ? 128 : 256, p.tq = 128;
+    p.tiles_p = (int)((p.V + p.tp - 1) / p.tp), p.tiles_q = (int)((p.N + p.tq - 1) / p.tq);
+    p.width = std::min<int64_t>(pad(p.V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np * 2 * p.planes) / 256 * 256));
+    const int64_t tiles_d = (p.D + p.tp - 1) / p.tp;
+    p.s_h = splits_of(tiles_d * p.tiles_q, std::min(p.width, p.Vp));
+    p.s_w = splits_of(tiles_d * ((p.width + p.tq - 1) / p.tq), p.Np);
+    return p;
+}
+
+struct Buffers {
+    float *largest_h, *largest_w, *largest_g, *scales;   // scales: h, w, g h
+    void *h, *w;                 // copies for the scores (planes, or padded bf16)
+    float2* part;
+    float* target_score;
+    double* sums;
+    _Float16 *w16, *h16, *u;     // backward
+    float *part_h, *part_w;
+    int64_t bytes;
+};
+
+Buffers buffers_of(const Plan& p, bool backward, void* base) {
+    Carve c = {(char*)base};
+    Buffers b = {};
+    b.largest_h = c.take<float>(kMaxBlocks), b.largest_w = c.take<float>(kMaxBlocks), b.largest_g = c.take<float>(kMaxBlocks);
+    b.scales = c.take<float>(4);
+    if (!p.direct_h) b.h = c.take<_Float16>(p.planes * p.Np * p.Dp);
+    if (!p.direct_w) b.w = c.take<_Float16>(p.planes * p.Vp * p.Dp);
+    if (!backward) {
+        b.part = c.take<float2>((int64_t)p.tiles_p * p.N);
+        b.target_score = c.take<float>(p.N);
+        b.sums = c.take<double>(2 * ((p.N + kRowsPerBlock - 1) / kRowsPerBlock));
+    } else {
+        b.w16 = p.f32 ? (_Float16*)b.w : c.take<_Float16>(p.Vp * p.Dp);
+        b.h16 = c.take<_Float16>(p.planes * p.Np * p.Dp);
+        b.u = c.take<_Float16>(p.planes * p.Np * p.width);
+        b.part_h = c.take<float>(p.s_h * p.N * p.Dp);
+        b.part_w = c.take<float>(p.s_w * p.width * p.Dp);
+    }
+    b.bytes = c.used;
+    return b;
+}
+
+unsigned blocks_for(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + kThreads - 1) / kThreads, 4096)); }
+
+template <typename T, bool G>
+int largest(const Matrix& x, const RowGrad& g, float* part, hipStream_t st) {
+    const int n = (int)std::min<int64_t>(blocks_for((int64_t)x.rows * ((x.D + 7) / 8)), kMaxBlocks);
+    hipLaunchKernelGGL((ce_largest_kernel<T, G>), dim3(n), dim3(kThreads), 0, st, x, g, part);
+    return n;
+}
+template <typename T, typename O, int PL, bool G>
+void planes(const Matrix& x, const RowGrad& g, const float* part, int parts, float* scale, O* out, int64_t rows_pad, int64_t Dp, hipStream_t st) {
+    hipLaunchKernelGGL((ce_planes_kernel<T, O, PL, G>), dim3(blocks_for(rows_pad * Dp / 8)), dim3(kThreads), 0, st, x, g, part, parts,
+                       scale, out, (int)rows_pad, (int)Dp);
+}
+
+Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t D, int size) {
+    const bool vec = ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0;
+    return {p, ld, (int)rows, (int)D, vec};
+}
+
+// The operands of the scores: the user's own, or copies of them.
+template <typename T>
+void score_sides(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs& s, hipStream_t st) {
+    const Matrix h = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T)), w = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T));
+    s.t = {a->target, (int)a->target_bytes, a->ignore_index, a->V};
+    const RowGrad none = {}, counts = {s.t, nullptr, nullptr, 0};
+    if constexpr (sizeof(T) == 4) {
+        const int nh = largest<T, true>(h, counts, b.largest_h, st), nw = largest<T, false>(w, none, b.largest_w, st);
+        planes<T, _Float16, 2, true>(h, counts, b.largest_h, nh, b.scales, (_Float16*)b.h, p.Np, p.Dp, st);
+        planes<T, _Float16, 2, false>(w, none, b.largest_w, nw, b.scales + 1, (_Float16*)b.w, p.Vp, p.Dp, st);
+        s.scale_h = b.scales, s.scale_w = b.scales + 1;
+    } else {
+        if (!p.direct_h) planes<T, __bf16, 1, false>(h, none, nullptr, 0, nullptr, (__bf16*)b.h, p.Np, p.Dp, st);
+        if (!p.direct_w) planes<T, __bf16, 1, false>(w, none, nullptr, 0, nullptr, (__bf16*)b.w, p.Vp, p.Dp, st);
+    }
+    s.h = {p.direct_h ? a->hidden : b.h, p.Np * p.Dp * 2, p.direct_h ? a->hidden_ld : p.Dp, (int)p.N};
+    s.w = {p.direct_w ? a->weight : b.w, p.Vp * p.Dp * 2, p.direct_w ? a->weight_ld : p.Dp, (int)p.V};
+    s.V = (int)p.V, s.N = (int)p.N, s.Dp = (int)p.Dp, s.tiles_p = p.tiles_p, s.tiles_q = p.tiles_q;
+}
+
+template <typename K, typename A>
+int launch(const char* what, K kernel, int lds, Told& told, unsigned grid, hipStream_t st, const A& args) {
+    if (const int rc = allow_lds(what, (const void*)kernel, lds, told)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, st, args);
+    return MB_OK;
+}
+
+template <typename P>
+int stats(const ScoreArgs& s, hipStream_t st) {
+    static Told told;
+    return launch("mb_linear_ce_fwd", ce_stats_kernel<P>, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
+}
+template <typename P, int PL>
+int piece_of_u(const ScoreArgs& s, hipStream_t st) {
+    static Told told;
+    return launch("mb_linear_ce_bwd", ce_u_kernel<P, PL>, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
+}
+template <typename P>
+int part(PartArgs a, hipStream_t st) {
+    static Told told;
+    a.tiles_p = (int)((a.p.n + P::TP - 1) / P::TP), a.tiles_q = (int)((a.q.n + P::TQ - 1) / P::TQ);
+    return launch("mb_linear_ce_bwd", ce_part_kernel<P>, P::kLds, told, (unsigned)(a.tiles_p * a.tiles_q * a.splits), st, a);
+}
+
+int check(const char* what, const mb_linear_ce* a) {
+    MB_REQUIRE(a, "%s: null args", what);
+    MB_REQUIRE(a->N >= 1 && a->N <= (1 << 28), "%s: N=%lld (1 to 2^28)", what, (long long)a->N);
+    MB_REQUIRE(a->V >= 1 && a->V <= (1 << 24), "%s: V=%lld (1 to 2^24)", what, (long long)a->V);
+    MB_REQUIRE(a->D >= 1 && a->D <= (1 << 16), "%s: D=%lld (1 to 2^16)", what, (long long)a->D);
+    MB_REQUIRE(a->dtype == MB_DTYPE_F32 || a->dtype == MB_DTYPE_BF16, "%s: dtype=%lld", what, (long long)a->dtype);
+    MB_REQUIRE(a->reduction >= 0 && a->reduction <= 2, "%s: reduction=%lld", what, (long long)a->reduction);
+    MB_REQUIRE(a->target_bytes == 4 || a->target_bytes == 8, "%s: target_bytes=%lld (4 or 8)", what, (long long)a->target_bytes);
+    MB_REQUIRE(a->hidden && a->weight && a->target && a->lse && a->count, "%s: null pointer argument", what);
+    for (const int64_t ld : {a->hidden_ld, a->weight_ld})
+        MB_REQUIRE(ld >= a->D && ld <= (1 << 22), "%s: rows are %lld elements apart (D to 2^22)", what, (long long)ld);
+    return MB_OK;
+}
+
+int enough(const char* what, const mb_linear_ce* a, int64_t need) {
+    MB_REQUIRE(((uintptr_t)a->workspace & 255) == 0, "%s: the workspace has to begin at a multiple of 256 bytes", what);
+    if (!a->workspace || a->workspace_bytes < need)
+        return fail(MB_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld are needed", what, (long long)a->workspace_bytes, (long long)need);
+    return MB_OK;
+}
+
+template <typename T, typename E, int PL, int TP>
+int forward(const mb_linear_ce* a, hipStream_t st) {
+    const Plan p = plan_of(a);
+    const Buffers b = buffers_of(p, false, a->workspace);
+    if (const int rc = enough("mb_linear_ce_fwd", a, b.bytes)) return rc;
+    ScoreArgs s = {};
+    score_sides<T>(a, p, b, s, st);
+    s.part = b.part, s.target_score = b.target_score;
+    if (const int rc = stats<Product<E, PL, TP, 128, kRows, kRows>>(s, st)) return rc;
+    const int blocks = (int)((p.N + kRowsPerBlock - 1) / kRowsPerBlock);
+    const JoinArgs j = {b.part, b.target_score, s.t, (int)p.N, p.tiles_p, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
+    hipLaunchKernelGGL(ce_join_kernel, dim3(blocks), dim3(kThreads), 0, st, j);
+    if (a->reduction)
+        hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(kThreads), 0, st, b.sums, blocks, (int)a->reduction, a->loss, a->count);
+    return check_launch("mb_linear_ce_fwd");
+}
+
+template <typename T, typename E, int PL, int TP>
+int backward(const mb_linear_ce* a, hipStream_t st) {
+    const Plan p = plan_of(a);
+    const Buffers b = buffers_of(p, true, a->workspace);
+    if (const int rc = enough("mb_linear_ce_bwd", a, b.bytes)) return rc;
+    const bool wants_h = a->dhidden, wants_w = a->dweight;
+    if (!wants_h && !wants_w) return MB_OK;
+    ScoreArgs s = {};
+    score_sides<T>(a, p, b, s, st);
+    s.lse = a->lse, s.u = b.u, s.width = p.width, s.n_pad = (int)p.Np;
+    const RowGrad g = {s.t, a->dloss, a->count, (int)a->reduction};
+    const Matrix h = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T)), w = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T));
+    if constexpr (sizeof(T) == 2)     // fp32: the scores' planes
+        if (wants_h) {
+            const int n = largest<T, false>(w, g, b.largest_w, st);
+            planes<T, _Float16, 1, false>(w, g, b.largest_w, n, b.scales + 1, b.w16, p.Vp, p.Dp, st);
+        }
+    if (wants_w) {
+        const int n = largest<T, true>(h, g, b.largest_g, st);
+        planes<T, _Float16, PL, true>(h, g, b.largest_g, n, b.scales + 2, b.h16, p.Np, p.Dp, st);
+    }
+    const int64_t plane_u = p.Np * p.width * 2, tiles_q = p.tiles_q;
+    for (int64_t v0 = 0; v0 < p.V; v0 += p.width) {
+        const int64_t v1 = std::min(p.V, v0 + p.width), kv = pad(v1 - v0, kStep);
+        s.v0 = (int)v0, s.v1 = (int)v1;
+        s.tiles_p = (int)((v1 - v0 + TP - 1) / TP), s.tiles_q = (int)tiles_q;
+        if (const int rc = piece_of_u<Product<E, PL, TP, 128, kRows, kRows>, PL>(s, st)) return rc;
+        if (wants_h) {
+            PartArgs x = {};
+            x.p = {b.w16 + v0 * p.Dp, p.Vp * p.Dp * 2, p.Dp, (int)p.D};
+            x.q = {b.u, plane_u, p.width, (int)p.N};
+            x.splits = (int)std::min<int64_t>(p.s_h, kv / kStep), x.k1 = (int)kv, x.out = b.part_h, x.ld = p.Dp, x.add = v0 > 0;
+            if (const int rc = part<Product<_Float16, PL, TP, 128, kCols, kRows>>(x, st)) return rc;
+        }
+        if (wants_w) {
+            PartArgs x = {};
+            x.p = {b.h16, p.Np * p.Dp * 2, p.Dp, (int)p.D};
+            x.q = {b.u, plane_u, p.width, (int)(v1 - v0)};
+            x.splits = p.s_w, x.k1 = (int)p.Np, x.out = b.part_w, x.ld = p.Dp;
+            if (const int rc = part<Product<_Float16, PL, TP, 128, kCols, kCols>>(x, st)) return rc;
+            hipLaunchKernelGGL((ce_sum_kernel<T, false>), dim3(blocks_for((v1 - v0) * p.Dp / 4)), dim3(kThreads), 0, st, b.part_w, p.s_w,
+                               (int)(v1 - v0), (int)p.D, (int)p.Dp, b.scales + 2, g, (T*)a->dweight + v0 * p.D);
+        }
+    }
+    if (wants_h)
+        hipLaunchKernelGGL((ce_sum_kernel<T, true>), dim3(blocks_for(p.N * p.Dp / 4)), dim3(kThreads), 0, st, b.part_h, p.s_h, (int)p.N,
+                           (int)p.D, (int)p.Dp, b.scales + 1, g, (T*)a->dhidden);
+    return check_launch("mb_linear_ce_bwd");
+}
+
+}  // namespace
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" int64_t mb_linear_ce_workspace(const mb_linear_ce* a, int backward) {
+    if (check("mb_linear_ce_workspace", a)) return -1;
+    return buffers_of(plan_of(a), backward != 0, nullptr).bytes;
+}
+
+extern "C" int mb_linear_ce_fwd(const mb_linear_ce* a, void* stream) {
+    if (const int rc = check("mb_linear_ce_fwd", a)) return rc;
+    MB_REQUIRE(a->loss, "mb_linear_ce_fwd: null pointer argument");
+    return a->dtype == MB_DTYPE_F32 ? forward<float, _Float16, 2, 128>(a, (hipStream_t)stream)
+                                    : forward<__bf16, __bf16, 1, 256>(a, (hipStream_t)stream);
+}
+
+extern "C" int mb_linear_ce_bwd(const mb_linear_ce* a, void* stream) {
+    if (const int rc = check("mb_linear_ce_bwd", a)) return rc;
+    MB_REQUIRE(a->dloss, "mb_linear_ce_bwd: null pointer argument");
+    return a->dtype == MB_DTYPE_F32 ? backward<float, _Float16, 2, 128>(a, (hipStream_t)stream)
+                                    : backward<__bf16, __bf16, 1, 256>(a, (hipStream_t)stream);
+}

@@ -21,6 +21,7 @@ from .triton_flash_ema import (FlashEMAFunction, GatedQueryFlashEMAFunction, _bu
                                check_counter_range, precompute_boundaries)
 from .triton_fused_gating import fused_apply_symmetric_query_gating
 from .layernorm import layer_norm
+from .linear_cross_entropy import linear_cross_entropy
 from .rmsnorm import rms_norm
 from .swiglu import swiglu_product
 
@@ -163,6 +164,10 @@ class SlotTransformerLM(nn.Module):
     tokens of each row (``_build_unique_index``) with no carried state.  As in the
     reference, ``inverse_indices`` and ``doc_ids`` are accepted and unused (a chunk is one
     document).
+
+    With ``targets`` [B, L] (not in the reference) the mean cross entropy over the targets that are not
+    ``ignore_index`` is returned instead of the logits, which are not formed (``linear_cross_entropy``
+    with lm_head's weight).
     """
 
     def __init__(self, vocab_size, d_model, n_layers, n_heads, N=16, dropout=0.1, use_silu=True,
@@ -192,7 +197,8 @@ class SlotTransformerLM(nn.Module):
         # (False), or whichever has fewer rows (None)
         self.kv_table = None
 
-    def forward(self, x, unique_slots=None, inverse_indices=None, c_base=None, doc_ids=None, pad_mask=None):
+    def forward(self, x, unique_slots=None, inverse_indices=None, c_base=None, doc_ids=None, pad_mask=None,
+                targets=None, ignore_index=-1):
         device = x.device
         if device.type != "cuda":
             raise NotImplementedError(
@@ -244,4 +250,6 @@ class SlotTransformerLM(nn.Module):
         for layer in self.layers:
             x_q = layer(x_q, x, E_slots, self.ema_rhos, C_seq, unique_tensor, K_max, C_bounds, E_active)
         x_q = self.final_norm(x_q)
+        if targets is not None:
+            return linear_cross_entropy(x_q, self.lm_head.weight, targets, ignore_index)
         return self.lm_head(x_q)
