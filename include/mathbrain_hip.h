@@ -747,6 +747,38 @@ int mb_linear_ce_fwd(const mb_linear_ce *args, void *stream);
 int mb_linear_ce_bwd(const mb_linear_ce *args, void *stream);
 
 /*
+ * Orthogonalised matrices by Newton-Schulz products, and the optimiser's step that applies them:
+ *
+ *   X = G / (|G|_F + eps) (transposed where rows > cols);  steps times:  A = X X^T,  X <- a X + (b A + c A^2) X
+ *   is_step 0: dst = X.   is_step 1: momentum <- mu momentum + src,  G = src + mu momentum (nesterov) or momentum,
+ *   dst <- dst (1 - lr weight_decay) - lr rate X
+ *
+ * All matrices go through every launch together; the products are those of fp32 values (24 bits, in two fp16
+ * planes).  The arguments come in structs on the HOST, read before the call returns.
+ */
+typedef struct mb_muon_matrix {
+    const void *src;              /* [rows, cols] contiguous, as the others: the matrix, or a step's gradient */
+    void *dst, *momentum;         /* memory that is written must not be another tensor's (checked) */
+    int64_t rows, cols;
+    int64_t src_dtype, dst_dtype, momentum_dtype;  /* MB_DTYPE_F32 or MB_DTYPE_BF16 each */
+    double rate;
+} mb_muon_matrix;
+
+typedef struct mb_muon {
+    const mb_muon_matrix *matrices;
+    int64_t count, steps, is_step, nesterov;
+    double a, b, c, eps;
+    int64_t x_exponent, a_exponent, b_exponent; /* 2^exponent times the largest singular value of any iterate X */
+                                  /*   (at most 1 at first), A and b A + c A^2 must stay below 65504 */
+    double lr, momentum, weight_decay;
+    void *workspace;              /* at a multiple of 256 bytes, mb_muon_workspace(args) bytes (-1: refused) */
+    int64_t workspace_bytes;
+} mb_muon;
+
+int64_t mb_muon_workspace(const mb_muon *args);
+int mb_muon_run(const mb_muon *args, void *stream);
+
+/*
  * Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_ in the reference's training
  * step):
  *

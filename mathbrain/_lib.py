@@ -85,6 +85,8 @@ SIGNATURES = {
     "mb_linear_ce_workspace": ([_p, _i], _i64),
     "mb_linear_ce_fwd": ([_p, _p], _i),
     "mb_linear_ce_bwd": ([_p, _p], _i),
+    "mb_muon_workspace": ([_p], _i64),
+    "mb_muon_run": ([_p, _p], _i),
     "mb_grad_clip": ([_p, _p, _p, _p, _p, _i, _f, _p, _p, _i64, _p], _i),
     "mb_grad_clip_workspace": ([_i], _i64),
     "mb_swiglu_fwd": ([_p, _p, _i64, _i, _p, _p], _i),

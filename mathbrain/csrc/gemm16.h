@@ -72,6 +72,16 @@ __device__ inline void wait_and_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 __device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+// A value that is the same in all lanes, where the compiler cannot see that.
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <typename T>
+__device__ inline T* uniform(T* p) {
+    const uint64_t x = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (T*)((uint64_t)hi << 32 | lo);
+}
+__device__ inline int64_t uniform(int64_t x) { return (int64_t)uniform((char*)x); }
+__device__ inline Side uniform(const Side& s) { return {uniform((char*)s.p), uniform(s.plane), uniform(s.ld), uniform(s.n)}; }
 __device__ inline uint32_t lds_address(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
@@ -175,8 +185,10 @@ struct Product {
     __device__ static int col(int j) { return wave_q() + 32 * j + (threadIdx.x & 31); }
 
     // k from k0 to k1, multiples of 32 (k1 > k0).  All waves have to be here; LDS is free again after the next barrier.
-    __device__ void run(const Side& p, const Side& q, int p0, int q0, int k0, int k1, void* smem) {
+    __device__ void run(const Side& p_, const Side& q_, int p0, int q0, int k0, int k1, void* smem) {
         const uint32_t lds = lds_address(smem);
+        const Side p = uniform(p_), q = uniform(q_);
+        p0 = uniform(p0), q0 = uniform(q0), k0 = uniform(k0);
         const typename TileP::Offsets po(p, p0);
         const typename TileQ::Offsets qo(q, q0);
         const typename TileP::Lane pl;
@@ -184,7 +196,7 @@ struct Product {
         const char* pb = (const char*)p.p + TileP::at(p, p0, k0);
         const char* qb = (const char*)q.p + TileQ::at(q, q0, k0);
         const int64_t pstep = TileP::at(p, 0, kStep), qstep = TileQ::at(q, 0, kStep);
-        const int steps = (k1 - k0) / kStep;
+        const int steps = uniform((k1 - k0) / kStep);
         auto issue = [&](int t) {
             const uint32_t tile = lds + t % kStages * kStage;
 #pragma unroll
