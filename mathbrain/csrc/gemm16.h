@@ -12,8 +12,8 @@
 // place c ^ swz(r) instead, which spreads the reads over the banks.  An operand may have its k next to
 // each other (kRows) or its free index (kCols: read back by the transposing 16-bit LDS read).
 //
-// Buffers are padded: kRows operands have whole steps of 32 k (zeros behind the matrix on one side at
-// least), kCols operands whole steps of 32 rows and rows of a multiple of 8 elements.  Tiles that pass
+// Buffers are padded: kRows operands have whole steps of k (zeros behind the matrix on one side at
+// least), kCols operands whole steps of rows and rows of a multiple of 8 elements.  Tiles that pass
 // the free index's end read the last rows (or pieces) again; whoever uses acc leaves those out.
 //
 // A lane holds, of each 32 x 32 block, column q = lane % 32 and the rows p = 8 (r / 4) + 4 (lane / 32) + r % 4.
@@ -22,12 +22,12 @@
 #include "common.h"
 
 #include <atomic>
+#include <type_traits>
 
 namespace mb {
 namespace g16 {
 
-constexpr int kThreads = 256;
-constexpr int kStep = 32;       // k of a step
+constexpr int kPad = 64;        // what k is padded to: a step of any of the products
 
 typedef __attribute__((__ext_vector_type__(8))) _Float16 f16x8;
 typedef __attribute__((__ext_vector_type__(4))) _Float16 f16x4;
@@ -86,14 +86,15 @@ __device__ inline uint32_t lds_address(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
-// A tile of N free indices by 32 k in LDS.
-template <typename T, int N, Order ORDER>
+// A tile of N free indices by STEP k in LDS.
+template <typename T, int N, Order ORDER, int STEP, int THREADS>
 struct Tile {
+    static constexpr int kStep = STEP;
     static constexpr int kBytes = N * kStep * 2;
-    static constexpr int kLoads = kBytes / 4096;                    // of each wave
+    static constexpr int kLoads = kBytes / (THREADS * 16);          // of each wave
     static constexpr int kRow = ORDER == kRows ? kStep * 2 : N * 2; // bytes
     static constexpr int kPieces = kRow / 16;
-    static_assert(kBytes % 4096 == 0 && N % 64 == 0, "a wave's load moves 1 KiB");
+    static_assert(kBytes % (THREADS * 16) == 0 && N % 64 == 0 && STEP % 32 == 0, "a wave's load moves 1 KiB");
     typedef __attribute__((address_space(3))) const char lds_char;
 
     static __device__ constexpr int swz(int row) {
@@ -110,17 +111,15 @@ struct Tile {
             const int last = ORDER == kRows ? left : (int)(s.ld - 8) - i0;
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
-                const int slot = j * kThreads + (int)threadIdx.x, row = slot / kPieces;
+                const int slot = j * THREADS + (int)threadIdx.x, row = slot / kPieces;
                 const int piece = (slot % kPieces) ^ swz(row);
                 if (ORDER == kRows) v[j] = (uint32_t)(min(row, last) * (int64_t)s.ld * 2) + piece * 16;
                 else v[j] = (uint32_t)(row * s.ld * 2) + min(piece * 8, last) * 2;
             }
         }
     };
-    static __device__ void load(uint32_t tile, const char* base, const Offsets& off) {
-        const uint32_t lds = tile + wave_id() * 1024;
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) dma16(lds + j * 4096, off.v[j], base);
+    static __device__ void load(uint32_t tile, int j, const char* base, const Offsets& off) {
+        dma16(tile + wave_id() * 1024 + j * THREADS * 16, off.v[j], base);
     }
     // Bytes from the matrix's first element to the tile's.
     static __device__ int64_t at(const Side& s, int i0, int k0) {
@@ -129,17 +128,17 @@ struct Tile {
     // Where this lane reads within a tile: the fragment of free indices i0 + lane % 32 (i0 a multiple of 32) and
     // k = 16 c + 8 (lane / 32) + 0 .. 7.
     struct Lane {
-        uint32_t v[ORDER == kRows ? 2 : 4];
+        uint32_t v[ORDER == kRows ? STEP / 16 : STEP / 8];
         __device__ Lane() {
             const int lane = threadIdx.x & 63, g = lane >> 5;
             if (ORDER == kRows) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) v[c] = (lane & 31) * kRow + (((2 * c + g) ^ swz(lane & 31)) << 4);
+                for (int c = 0; c < STEP / 16; ++c) v[c] = (lane & 31) * kRow + (((2 * c + g) ^ swz(lane & 31)) << 4);
             } else {
                 // 16 lanes read 4 rows of 16 free indices, 8 bytes each, and get 4 rows of one index each
                 const int d = (lane & 16) + 4 * (lane & 3);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < STEP / 8; ++c) {
                     const int r = 16 * (c / 2) + 8 * g + 4 * (c % 2) + ((lane & 15) >> 2);
                     v[c] = r * kRow + (((d >> 3) ^ swz(r)) << 4) + 2 * (d & 7);
                 }
@@ -160,31 +159,45 @@ struct Tile {
     }
 };
 
-template <typename T_, int PLANES, int TP_, int TQ_, Order OP, Order OQ>
+// NP x NQ waves, each with TP / NP x TQ / NQ of the tile.
+template <typename T_, int PLANES, int TP_, int TQ_, Order OP, Order OQ, int NP = 2, int NQ = 2, int STEP = 32, int kMost = 5>
 struct Product {
     typedef T_ T;
+    static constexpr int kThreads = 64 * NP * NQ, kStep = STEP;
     static constexpr int TP = TP_, TQ = TQ_;
-    static constexpr int WP = TP / 2, WQ = TQ / 2;     // of a wave
+    static constexpr int WP = TP / NP, WQ = TQ / NQ;   // of a wave
     static constexpr int FP = WP / 32, FQ = WQ / 32;   // its 32 x 32 blocks
-    typedef Tile<T, TP, OP> TileP;
-    typedef Tile<T, TQ, OQ> TileQ;
+    static constexpr int kWavesP = NP;
+    typedef Tile<T, TP, OP, STEP, kThreads> TileP;
+    typedef Tile<T, TQ, OQ, STEP, kThreads> TileQ;
     static constexpr int kStage = PLANES * (TileP::kBytes + TileQ::kBytes);
-    // two workgroups a CU: 80 KiB of LDS each
-    static constexpr int kStages = 3 * kStage <= 81920 ? 3 : 2;
+    // Waves that a SIMD's registers are enough for, and the LDS of a workgroup then.
+    static constexpr int kWaves = FP * FQ > 8 ? 1 : 2;
+    static constexpr int kRoom = 163840 * kThreads / (256 * kWaves);
+    // Whether the waves meet before a step's last instructions, with the next step's first fragments on their way during
+    // these: with eight waves in one workgroup all wait at the same time (8192^3, 256 x 256: 1146 TFLOP/s against 1120),
+    // with two workgroups a CU the one works while the other waits (256 x 128: 1114 against 1081 with this).
+    static constexpr bool kAhead = kThreads > 256;
+    static constexpr int kFit = kRoom / kStage, kStages = kFit < kMost ? kFit : kMost;
+    static_assert(kStages >= 2, "a step's operands on their way beside the one in use");
     static constexpr int kLds = kStages * kStage;
     static constexpr int kLoads = PLANES * (TileP::kLoads + TileQ::kLoads);
 
     f32x16 acc[FP][FQ];
 
-    __device__ static int wave_p() { return (wave_id() & 1) * WP; }
-    __device__ static int wave_q() { return (wave_id() >> 1) * WQ; }
+    __device__ static int wave_p() { return wave_id() % NP * WP; }
+    __device__ static int wave_q() { return wave_id() / NP * WQ; }
     // the row within the tile of element r of block i, the column of block j
     __device__ static int row(int i, int r) {
         return wave_p() + 32 * i + 8 * (r / 4) + 4 * ((threadIdx.x & 63) >> 5) + r % 4;
     }
     __device__ static int col(int j) { return wave_q() + 32 * j + (threadIdx.x & 31); }
 
-    // k from k0 to k1, multiples of 32 (k1 > k0).  All waves have to be here; LDS is free again after the next barrier.
+    struct Frags {
+        typename Frag<T>::type a[PLANES][FP], b[PLANES][FQ];
+    };
+
+    // k from k0 to k1, multiples of kStep (k1 > k0).  All waves have to be here; LDS is free again after the next barrier.
     __device__ void run(const Side& p_, const Side& q_, int p0, int q0, int k0, int k1, void* smem) {
         const uint32_t lds = lds_address(smem);
         const Side p = uniform(p_), q = uniform(q_);
@@ -197,15 +210,14 @@ struct Product {
         const char* qb = (const char*)q.p + TileQ::at(q, q0, k0);
         const int64_t pstep = TileP::at(p, 0, kStep), qstep = TileQ::at(q, 0, kStep);
         const int steps = uniform((k1 - k0) / kStep);
-        auto issue = [&](int t) {
-            const uint32_t tile = lds + t % kStages * kStage;
-#pragma unroll
-            for (int h = 0; h < PLANES; ++h) {
-                TileP::load(tile + h * TileP::kBytes, pb + h * p.plane, po);
-                TileQ::load(tile + PLANES * TileP::kBytes + h * TileQ::kBytes, qb + h * q.plane, qo);
-            }
-            pb += pstep, qb += qstep;
+        // load n of the wave's for a step
+        auto load = [&](uint32_t tile, int n) {
+            constexpr int all = PLANES * TileP::kLoads;
+            if (n < all) TileP::load(tile + n / TileP::kLoads * TileP::kBytes, n % TileP::kLoads, pb + n / TileP::kLoads * p.plane, po);
+            else TileQ::load(tile + PLANES * TileP::kBytes + (n - all) / TileQ::kLoads * TileQ::kBytes, (n - all) % TileQ::kLoads,
+                             qb + (n - all) / TileQ::kLoads * q.plane, qo);
         };
+        auto stage = [&](int t) { return lds + t % kStages * kStage; };
 #pragma unroll
         for (int i = 0; i < FP; ++i)
 #pragma unroll
@@ -213,37 +225,85 @@ struct Product {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
         __builtin_amdgcn_s_waitcnt(0x0F70);   // the compiler's own loads are done: it would wait for the DMA with them
-        for (int t = 0; t < kStages - 1 && t < steps; ++t) issue(t);
-        for (int t = 0; t < steps; ++t) {
-            if (t + kStages - 2 < steps) wait_and_meet<(kStages - 2) * kLoads>();
-            else wait_and_meet<0>();
-            if (t + kStages - 1 < steps) issue(t + kStages - 1);
-            const uint32_t ptile = lds + t % kStages * kStage, qtile = ptile + PLANES * TileP::kBytes;
+        for (int t = 0; t < kStages - 1 && t < steps; ++t) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                typename Frag<T>::type a[PLANES][FP], b[PLANES][FQ];
+            for (int n = 0; n < kLoads; ++n) load(stage(t), n);
+            pb += pstep, qb += qstep;
+        }
+        auto read = [&](Frags& x, uint32_t ptile, int c) {
+            const uint32_t qtile = ptile + PLANES * TileP::kBytes;
 #pragma unroll
-                for (int h = 0; h < PLANES; ++h) {
+            for (int h = 0; h < PLANES; ++h) {
 #pragma unroll
-                    for (int i = 0; i < FP; ++i) a[h][i] = TileP::read(ptile + h * TileP::kBytes, pl, wave_p() + 32 * i, c);
+                for (int j = 0; j < FQ; ++j) x.b[h][j] = TileQ::read(qtile + h * TileQ::kBytes, ql, wave_q() + 32 * j, c);
 #pragma unroll
-                    for (int j = 0; j < FQ; ++j) b[h][j] = TileQ::read(qtile + h * TileQ::kBytes, ql, wave_q() + 32 * j, c);
-                }
-                if constexpr (PLANES == 2) {
-#pragma unroll
-                    for (int i = 0; i < FP; ++i)
-#pragma unroll
-                        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(a[1][i], b[0][j], acc[i][j]);
-#pragma unroll
-                    for (int i = 0; i < FP; ++i)
-#pragma unroll
-                        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(a[0][i], b[1][j], acc[i][j]);
-                }
-#pragma unroll
-                for (int i = 0; i < FP; ++i)
-#pragma unroll
-                    for (int j = 0; j < FQ; ++j) acc[i][j] = mma(a[0][i], b[0][j], acc[i][j]);
+                for (int i = 0; i < FP; ++i) x.a[h][i] = TileP::read(ptile + h * TileP::kBytes, pl, wave_p() + 32 * i, c);
             }
+        };
+        // A step: fragments come out of LDS one k of 16 ahead of the instructions that use them.  The loads for a later
+        // step go out between the instructions, a few at a time: a wave that sends all of them at once waits for the
+        // others' before it can go on.
+        Frags f[2];
+        auto step = [&](int t, auto more, auto last) {
+            constexpr int C = STEP / 16, kProducts = PLANES == 2 ? 3 : 1, kGroups = (kAhead ? C - 1 : C) * kProducts * FP;
+            const uint32_t to = stage(t + kStages - 1);
+            if constexpr (!kAhead) {
+                wait_and_meet<decltype(more)::value ? (kStages - 2) * kLoads : 0>();
+                read(f[0], stage(t), 0);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                if (c + 1 < C) {
+                    read(f[(c + 1) % 2], stage(t), c + 1);
+                } else if constexpr (kAhead && !decltype(last)::value) {
+                    wait_and_meet<decltype(more)::value ? (kStages - 2) * kLoads : 0>();
+                    read(f[0], stage(t + 1), 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                const Frags& x = f[c % 2];
+#pragma unroll
+                for (int k = 3 - kProducts; k < 3; ++k)   // lo hi, hi lo, hi hi
+#pragma unroll
+                    for (int i = 0; i < FP; ++i) {
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(x.a[k == 0][i], x.b[k == 1][j], acc[i][j]);
+                        const int g = (c * kProducts + k - 3 + kProducts) * FP + i;
+                        if constexpr (decltype(more)::value) {
+#pragma unroll
+                            for (int n = g * kLoads / kGroups; g < kGroups && n < (g + 1) * kLoads / kGroups; ++n) load(to, n);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+            if constexpr (decltype(more)::value) pb += pstep, qb += qstep;
+        };
+        if constexpr (kAhead) {
+            if (steps >= kStages - 1) wait_and_meet<(kStages - 2) * kLoads>();
+            else wait_and_meet<0>();
+            read(f[0], stage(0), 0);
+        }
+        int t = 0;
+        for (; t + kStages - 1 < steps; ++t) step(t, std::true_type(), std::false_type());
+        for (; t + 1 < steps; ++t) step(t, std::false_type(), std::false_type());
+        step(t, std::false_type(), std::true_type());
+    }
+
+    // The result as 16-bit values next to each other in p, by way of LDS: a lane's own four of a row would go out in 32
+    // pieces of 16 bytes an instruction.  hold() puts them there, after a barrier; store() takes a whole tile out, 16 bytes a
+    // lane, rows of q (q0 + r < q_end) and pieces of 8 p (p_end a multiple of 8) that are there.
+    static constexpr int kOutPieces = TP / 8;
+    static constexpr int kOutTurn = kOutPieces % 16 == 0 ? 15 : 7;
+    static constexpr int kOutPlane = TP * TQ * 2;
+    __device__ static void hold(void* smem, int plane, int i, int j, int r, f16x4 v) {
+        const int q = col(j), piece = (wave_p() + 32 * i + 8 * (r / 4)) / 8, half = (threadIdx.x & 63) >> 5;
+        *(f16x4*)((char*)smem + plane * kOutPlane + q * (2 * TP) + ((piece ^ (q & kOutTurn)) << 4) + half * 8) = v;
+    }
+    __device__ static void store(const void* smem, int plane, _Float16* out, int64_t ld, int p0, int q0, int p_end, int q_end) {
+#pragma unroll 4
+        for (int n = threadIdx.x; n < TQ * kOutPieces; n += kThreads) {
+            const int q = n / kOutPieces, piece = n % kOutPieces;
+            const f16x8 v = *(const f16x8*)((const char*)smem + plane * kOutPlane + q * (2 * TP) + ((piece ^ (q & kOutTurn)) << 4));
+            if (q0 + q < q_end && p0 + piece * 8 < p_end) *(f16x8*)(out + (int64_t)(q0 + q) * ld + p0 + piece * 8) = v;
         }
     }
 };

@@ -23,6 +23,7 @@ namespace {
 
 using namespace g16;
 
+constexpr int kThreads = 256;       // of the kernels around the products
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kUScale = 32768.f;
@@ -185,7 +186,7 @@ __device__ inline float score_factor(const ScoreArgs& a) {
 }
 
 template <typename P>
-__global__ void __launch_bounds__(kThreads, 2) ce_stats_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const ScoreArgs a) {
     extern __shared__ char smem[];
     int tp, tq;
     if (!tile_of(a.tiles_p, a.tiles_q, tp, tq)) return;
@@ -229,17 +230,20 @@ __global__ void __launch_bounds__(kThreads, 2) ce_stats_kernel(const ScoreArgs a
         }
     }
     __syncthreads();
-    const int half = wave_id() & 1;
+    const int half = wave_id() % P::kWavesP;
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j)
         if ((threadIdx.x & 63) < 32) both[half * P::TQ + P::col(j)] = make_float2(m[j], sum[j]);
     __syncthreads();
-    for (int c = threadIdx.x; c < P::TQ; c += kThreads)
+    for (int c = threadIdx.x; c < P::TQ; c += P::kThreads)
         if (q0 + c < a.N) {
-            const float2 x = both[c], y = both[P::TQ + c];
-            const float top = fmaxf(x.x, y.x), base = top == -INFINITY ? 0.f : top;
-            a.part[(int64_t)tp * a.N + q0 + c] =
-                make_float2(top, x.y * __builtin_amdgcn_exp2f(x.x - base) + y.y * __builtin_amdgcn_exp2f(y.x - base));
+            float top = both[c].x, t = 0.f;
+#pragma unroll
+            for (int w = 1; w < P::kWavesP; ++w) top = fmaxf(top, both[w * P::TQ + c].x);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < P::kWavesP; ++w) t += both[w * P::TQ + c].y * __builtin_amdgcn_exp2f(both[w * P::TQ + c].x - base);
+            a.part[(int64_t)tp * a.N + q0 + c] = make_float2(top, t);
         }
 }
 
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) ce_total_kernel(const double* sums, 
 
 // U of a piece of the vocabulary, zeros behind its end and behind the last row.
 template <typename P, int PL>
-__global__ void __launch_bounds__(kThreads, 2) ce_u_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const ScoreArgs a) {
     extern __shared__ char smem[];
     int tp, tq;
     if (!tile_of(a.tiles_p, a.tiles_q, tp, tq)) return;
@@ -321,20 +325,18 @@ __global__ void __launch_bounds__(kThreads, 2) ce_u_kernel(const ScoreArgs a) {
     P prod;
     const float f = score_factor<P>(a);
     prod.run(a.w, a.h, p0, q0, 0, a.Dp, smem);
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j) {
         const int n = q0 + P::col(j);
-        if (n >= a.n_pad) continue;
         const int target = n < a.N ? a.t.at(n) : -1;
         const bool counts = target != -1;
         const float m = counts ? a.lse[n] : 0.f, l = counts ? a.lse[a.N + n] : 0.f;
-        _Float16* to = a.u + (int64_t)n * a.width - a.v0;
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int v = p0 + P::row(i, r);
-                if (v - a.v0 >= a.width) continue;
                 f16x4 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -349,10 +351,15 @@ __global__ void __launch_bounds__(kThreads, 2) ce_u_kernel(const ScoreArgs a) {
                         hi[e] = (_Float16)u;
                     }
                 }
-                *reinterpret_cast<f16x4*>(to + v) = hi;
-                if constexpr (PL == 2) *reinterpret_cast<f16x4*>(to + (int64_t)a.n_pad * a.width + v) = lo;
+                P::hold(smem, 0, i, j, r, hi);
+                if constexpr (PL == 2) P::hold(smem, 1, i, j, r, lo);
             }
     }
+    static_assert(PL * P::kOutPlane <= P::kLds, "");
+    __syncthreads();
+    const int64_t plane = (int64_t)a.n_pad * a.width;
+#pragma unroll
+    for (int h = 0; h < PL; ++h) P::store(smem, h, a.u + h * plane - a.v0, a.width, p0, q0, a.v0 + (int)a.width, a.n_pad);
 }
 
 struct PartArgs {
@@ -361,16 +368,16 @@ struct PartArgs {
     float* out;                         // [splits][q.n, ld]
     int64_t ld;
     int add;                            // onto what is there
+    __host__ __device__ int blocks() const { return tiles_p * tiles_q * splits; }
 };
 
 template <typename P>
-__global__ void __launch_bounds__(kThreads, 2) ce_part_kernel(const PartArgs a) {
-    extern __shared__ char smem[];
+__device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     const int tiles = a.tiles_p * a.tiles_q;
-    const int split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
+    const int split = block / tiles, tile = block - split * tiles;
     const int p0 = tile % a.tiles_p * P::TP, q0 = tile / a.tiles_p * P::TQ;
-    const int steps = a.k1 / kStep;
-    const int k0 = (int)((int64_t)steps * split / a.splits) * kStep, k1 = (int)((int64_t)steps * (split + 1) / a.splits) * kStep;
+    const int steps = a.k1 / P::kStep;
+    const int k0 = (int)((int64_t)steps * split / a.splits) * P::kStep, k1 = (int)((int64_t)steps * (split + 1) / a.splits) * P::kStep;
     P prod;
     prod.run(a.p, a.q, p0, q0, k0, k1, smem);
 #pragma unroll
@@ -389,6 +396,18 @@ __global__ void __launch_bounds__(kThreads, 2) ce_part_kernel(const PartArgs a) 
                 *reinterpret_cast<f32x4v*>(to + p) = v;
             }
     }
+}
+
+// Both gradients' products with a piece of U in one launch, either without tiles where it is not wanted: the one's
+// workgroups fill what the other's leave of the card's last round.  The longer ones come first.
+template <typename H, typename W>
+__global__ void __launch_bounds__(H::kThreads, H::kWaves) ce_part_kernel(const PartArgs h, const PartArgs w) {
+    static_assert(H::kThreads == W::kThreads && H::kWaves == W::kWaves, "");
+    extern __shared__ char smem[];
+    const bool h_first = (int64_t)h.k1 * w.splits >= (int64_t)w.k1 * h.splits;
+    const int n = h_first ? h.blocks() : w.blocks(), block = blockIdx.x;
+    if ((block < n) == h_first) part_of<H>(h, h_first ? block : block - n, smem);
+    else part_of<W>(w, h_first ? block - n : block, smem);
 }
 
 // out[n, d] = factor (g_n) sum_s part[s][n, d], in the parts' order.
@@ -430,33 +449,73 @@ struct Carve {
 
 // U's bytes in a piece: pieces are large enough to fill the card and small beside the scores.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
-constexpr int kSlots = 512;       // workgroups at work at once
+constexpr int kCus = 256;
+
+// The products of each type: the scores (vocabulary x rows), dh (D x rows) and dw (D x vocabulary).
+struct Bf16 {
+    typedef __bf16 T;
+    static constexpr int kPlanes = 1;
+    typedef Product<__bf16, 1, 192, 128, kRows, kRows, 2, 2, 64> Score;
+    typedef Product<_Float16, 1, 256, 128, kCols, kRows> GradH;
+    typedef Product<_Float16, 1, 256, 128, kCols, kCols> GradW;
+};
+struct F32 {
+    typedef float T;
+    static constexpr int kPlanes = 2;
+    typedef Product<_Float16, 2, 256, 128, kRows, kRows, 4, 2> Score;
+    typedef Product<_Float16, 2, 256, 128, kCols, kRows, 4, 2> GradH;
+    typedef Product<_Float16, 2, 256, 128, kCols, kCols, 4, 2> GradW;
+};
 
 struct Plan {
     int64_t N, V, D, Dp, Np, Vp, width;
-    bool f32, direct_h, direct_w;
-    int planes, tp, tq, tiles_p, tiles_q;   // of the scores
+    bool direct_h, direct_w;
+    int planes, tiles_p, tiles_q;           // of the scores
     int s_h, s_w;                            // splits of the two gradients' products
 };
 
-int splits_of(int64_t tiles, int64_t k) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>({kSlots / tiles, k / 512, 64}));
+// Splits of the two gradients' k.  Workgroups of one launch fill the card in rounds of kSlots; the time is about that of
+// the fullest slot, in steps of k, plus what a workgroup takes to begin and end (kOverhead steps), plus the traffic of the partial results.
+// All pairs of splits are tried (at most 32 x 32), with the workgroups dealt out in their order.
+template <typename P>
+int64_t tiles_of(int64_t np, int64_t nq) { return ((np + P::TP - 1) / P::TP) * ((nq + P::TQ - 1) / P::TQ); }
+
+constexpr int kOverhead = 12;
+void choose_splits(int64_t tiles_h, int64_t k_h, int64_t tiles_w, int64_t k_w, int64_t slots, int& s_h, int& s_w) {
+    double best = 1e300;
+    s_h = s_w = 1;
+    for (int x = 1; x <= 32 && (x == 1 || k_h / x >= 256); ++x)
+        for (int y = 1; y <= 32 && (y == 1 || k_w / y >= 256); ++y) {
+            const int64_t nh = tiles_h * x, nw = tiles_w * y;
+            const double th = (double)k_h / x / kPad + kOverhead, tw = (double)k_w / y / kPad + kOverhead;
+            // the longer ones go first, in whole rounds and a part of one; the shorter ones fill up
+            const int64_t n1 = th >= tw ? nh : nw, n2 = th >= tw ? nw : nh;
+            const double t1 = th >= tw ? th : tw, t2 = th >= tw ? tw : th;
+            const int64_t full = n1 / slots, rest = n1 % slots;     // `rest` slots end t1 later than the others
+            int64_t left = n2;
+            const double lead = rest ? t1 : 0.0;
+            const int64_t early = rest ? (int64_t)(lead / t2) * (slots - rest) : 0;
+            left -= std::min(left, early);
+            const double span = full * t1 + lead + (double)((left + slots - 1) / slots) * t2;
+            const double cost = span + 0.02 * (nh + nw) * kOverhead / slots;
+            if (cost < best * 0.999) best = cost, s_h = x, s_w = y;
+        }
 }
 
+template <typename C>
 Plan plan_of(const mb_linear_ce* a) {
     Plan p = {};
     p.N = a->N, p.V = a->V, p.D = a->D;
-    p.Dp = pad(p.D, kStep), p.Np = pad(p.N, kStep), p.Vp = pad(p.V, kStep);
-    p.f32 = a->dtype == MB_DTYPE_F32;
-    p.planes = p.f32 ? 2 : 1;
-    auto direct = [&](const void* x, int64_t ld) { return !p.f32 && p.D % kStep == 0 && ((uintptr_t)x & 15) == 0 && ld % 8 == 0; };
+    p.Dp = pad(p.D, kPad), p.Np = pad(p.N, kPad), p.Vp = pad(p.V, kPad);
+    p.planes = C::kPlanes;
+    auto direct = [&](const void* x, int64_t ld) {
+        return p.planes == 1 && p.D % C::Score::kStep == 0 && ((uintptr_t)x & 15) == 0 && ld % 8 == 0;
+    };
     p.direct_h = direct(a->hidden, a->hidden_ld), p.direct_w = direct(a->weight, a->weight_ld);
-    p.tp = p.f32 ? 128 : 256, p.tq = 128;
-    p.tiles_p = (int)((p.V + p.tp - 1) / p.tp), p.tiles_q = (int)((p.N + p.tq - 1) / p.tq);
+    p.tiles_p = (int)((p.V + C::Score::TP - 1) / C::Score::TP), p.tiles_q = (int)((p.N + C::Score::TQ - 1) / C::Score::TQ);
     p.width = std::min<int64_t>(pad(p.V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np * 2 * p.planes) / 256 * 256));
-    const int64_t tiles_d = (p.D + p.tp - 1) / p.tp;
-    p.s_h = splits_of(tiles_d * p.tiles_q, std::min(p.width, p.Vp));
-    p.s_w = splits_of(tiles_d * ((p.width + p.tq - 1) / p.tq), p.Np);
+    choose_splits(tiles_of<typename C::GradH>(p.D, p.N), std::min(p.width, p.Vp), tiles_of<typename C::GradW>(p.D, std::min(p.width, p.V)), p.Np,
+                  kCus * (C::GradH::kThreads == 256 ? C::GradH::kWaves : 1), p.s_h, p.s_w);
     return p;
 }
 
@@ -483,7 +542,7 @@ Buffers buffers_of(const Plan& p, bool backward, void* base) {
         b.target_score = c.take<float>(p.N);
         b.sums = c.take<double>(2 * ((p.N + kRowsPerBlock - 1) / kRowsPerBlock));
     } else {
-        b.w16 = p.f32 ? (_Float16*)b.w : c.take<_Float16>(p.Vp * p.Dp);
+        b.w16 = p.planes == 2 ? (_Float16*)b.w : c.take<_Float16>(p.Vp * p.Dp);
         b.h16 = c.take<_Float16>(p.planes * p.Np * p.Dp);
         b.u = c.take<_Float16>(p.planes * p.Np * p.width);
         b.part_h = c.take<float>(p.s_h * p.N * p.Dp);
@@ -529,31 +588,39 @@ void score_sides(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreAr
     }
     s.h = {p.direct_h ? a->hidden : b.h, p.Np * p.Dp * 2, p.direct_h ? a->hidden_ld : p.Dp, (int)p.N};
     s.w = {p.direct_w ? a->weight : b.w, p.Vp * p.Dp * 2, p.direct_w ? a->weight_ld : p.Dp, (int)p.V};
-    s.V = (int)p.V, s.N = (int)p.N, s.Dp = (int)p.Dp, s.tiles_p = p.tiles_p, s.tiles_q = p.tiles_q;
+    s.V = (int)p.V, s.N = (int)p.N, s.Dp = (int)(p.direct_h && p.direct_w ? p.D : p.Dp), s.tiles_p = p.tiles_p, s.tiles_q = p.tiles_q;
 }
 
 template <typename K, typename A>
-int launch(const char* what, K kernel, int lds, Told& told, unsigned grid, hipStream_t st, const A& args) {
+int launch(const char* what, K kernel, int threads, int lds, Told& told, unsigned grid, hipStream_t st, const A& args) {
     if (const int rc = allow_lds(what, (const void*)kernel, lds, told)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, st, args);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, args);
     return MB_OK;
 }
 
 template <typename P>
 int stats(const ScoreArgs& s, hipStream_t st) {
     static Told told;
-    return launch("mb_linear_ce_fwd", ce_stats_kernel<P>, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
+    return launch("mb_linear_ce_fwd", ce_stats_kernel<P>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
 }
 template <typename P, int PL>
 int piece_of_u(const ScoreArgs& s, hipStream_t st) {
     static Told told;
-    return launch("mb_linear_ce_bwd", ce_u_kernel<P, PL>, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
+    return launch("mb_linear_ce_bwd", ce_u_kernel<P, PL>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
 }
 template <typename P>
-int part(PartArgs a, hipStream_t st) {
-    static Told told;
+void tiles_for(PartArgs& a) {
     a.tiles_p = (int)((a.p.n + P::TP - 1) / P::TP), a.tiles_q = (int)((a.q.n + P::TQ - 1) / P::TQ);
-    return launch("mb_linear_ce_bwd", ce_part_kernel<P>, P::kLds, told, (unsigned)(a.tiles_p * a.tiles_q * a.splits), st, a);
+}
+template <typename C>
+int parts(const PartArgs& h, const PartArgs& w, hipStream_t st) {
+    typedef typename C::GradH H;
+    typedef typename C::GradW W;
+    static Told told;
+    constexpr int lds = std::max(H::kLds, W::kLds);
+    if (const int rc = allow_lds("mb_linear_ce_bwd", (const void*)ce_part_kernel<H, W>, lds, told)) return rc;
+    hipLaunchKernelGGL((ce_part_kernel<H, W>), dim3((unsigned)(h.blocks() + w.blocks())), dim3(H::kThreads), lds, st, h, w);
+    return MB_OK;
 }
 
 int check(const char* what, const mb_linear_ce* a) {
@@ -577,15 +644,16 @@ int enough(const char* what, const mb_linear_ce* a, int64_t need) {
     return MB_OK;
 }
 
-template <typename T, typename E, int PL, int TP>
+template <typename C>
 int forward(const mb_linear_ce* a, hipStream_t st) {
-    const Plan p = plan_of(a);
+    typedef typename C::T T;
+    const Plan p = plan_of<C>(a);
     const Buffers b = buffers_of(p, false, a->workspace);
     if (const int rc = enough("mb_linear_ce_fwd", a, b.bytes)) return rc;
     ScoreArgs s = {};
     score_sides<T>(a, p, b, s, st);
     s.part = b.part, s.target_score = b.target_score;
-    if (const int rc = stats<Product<E, PL, TP, 128, kRows, kRows>>(s, st)) return rc;
+    if (const int rc = stats<typename C::Score>(s, st)) return rc;
     const int blocks = (int)((p.N + kRowsPerBlock - 1) / kRowsPerBlock);
     const JoinArgs j = {b.part, b.target_score, s.t, (int)p.N, p.tiles_p, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
     hipLaunchKernelGGL(ce_join_kernel, dim3(blocks), dim3(kThreads), 0, st, j);
@@ -594,9 +662,11 @@ int forward(const mb_linear_ce* a, hipStream_t st) {
     return check_launch("mb_linear_ce_fwd");
 }
 
-template <typename T, typename E, int PL, int TP>
+template <typename C>
 int backward(const mb_linear_ce* a, hipStream_t st) {
-    const Plan p = plan_of(a);
+    typedef typename C::T T;
+    constexpr int PL = C::kPlanes;
+    const Plan p = plan_of<C>(a);
     const Buffers b = buffers_of(p, true, a->workspace);
     if (const int rc = enough("mb_linear_ce_bwd", a, b.bytes)) return rc;
     const bool wants_h = a->dhidden, wants_w = a->dweight;
@@ -617,26 +687,27 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
     }
     const int64_t plane_u = p.Np * p.width * 2, tiles_q = p.tiles_q;
     for (int64_t v0 = 0; v0 < p.V; v0 += p.width) {
-        const int64_t v1 = std::min(p.V, v0 + p.width), kv = pad(v1 - v0, kStep);
+        const int64_t v1 = std::min(p.V, v0 + p.width), kv = pad(v1 - v0, kPad);
         s.v0 = (int)v0, s.v1 = (int)v1;
-        s.tiles_p = (int)((v1 - v0 + TP - 1) / TP), s.tiles_q = (int)tiles_q;
-        if (const int rc = piece_of_u<Product<E, PL, TP, 128, kRows, kRows>, PL>(s, st)) return rc;
+        s.tiles_p = (int)((v1 - v0 + C::Score::TP - 1) / C::Score::TP), s.tiles_q = (int)tiles_q;
+        if (const int rc = piece_of_u<typename C::Score, PL>(s, st)) return rc;
+        PartArgs ph = {}, pw = {};
         if (wants_h) {
-            PartArgs x = {};
-            x.p = {b.w16 + v0 * p.Dp, p.Vp * p.Dp * 2, p.Dp, (int)p.D};
-            x.q = {b.u, plane_u, p.width, (int)p.N};
-            x.splits = (int)std::min<int64_t>(p.s_h, kv / kStep), x.k1 = (int)kv, x.out = b.part_h, x.ld = p.Dp, x.add = v0 > 0;
-            if (const int rc = part<Product<_Float16, PL, TP, 128, kCols, kRows>>(x, st)) return rc;
+            ph.p = {b.w16 + v0 * p.Dp, p.Vp * p.Dp * 2, p.Dp, (int)p.D};
+            ph.q = {b.u, plane_u, p.width, (int)p.N};
+            ph.splits = (int)std::min<int64_t>(p.s_h, kv / kPad), ph.k1 = (int)kv, ph.out = b.part_h, ph.ld = p.Dp, ph.add = v0 > 0;
+            tiles_for<typename C::GradH>(ph);
         }
         if (wants_w) {
-            PartArgs x = {};
-            x.p = {b.h16, p.Np * p.Dp * 2, p.Dp, (int)p.D};
-            x.q = {b.u, plane_u, p.width, (int)(v1 - v0)};
-            x.splits = p.s_w, x.k1 = (int)p.Np, x.out = b.part_w, x.ld = p.Dp;
-            if (const int rc = part<Product<_Float16, PL, TP, 128, kCols, kCols>>(x, st)) return rc;
+            pw.p = {b.h16, p.Np * p.Dp * 2, p.Dp, (int)p.D};
+            pw.q = {b.u, plane_u, p.width, (int)(v1 - v0)};
+            pw.splits = p.s_w, pw.k1 = (int)p.Np, pw.out = b.part_w, pw.ld = p.Dp;
+            tiles_for<typename C::GradW>(pw);
+        }
+        if (const int rc = parts<C>(ph, pw, st)) return rc;
+        if (wants_w)
             hipLaunchKernelGGL((ce_sum_kernel<T, false>), dim3(blocks_for((v1 - v0) * p.Dp / 4)), dim3(kThreads), 0, st, b.part_w, p.s_w,
                                (int)(v1 - v0), (int)p.D, (int)p.Dp, b.scales + 2, g, (T*)a->dweight + v0 * p.D);
-        }
     }
     if (wants_h)
         hipLaunchKernelGGL((ce_sum_kernel<T, true>), dim3(blocks_for(p.N * p.Dp / 4)), dim3(kThreads), 0, st, b.part_h, p.s_h, (int)p.N,
@@ -651,19 +722,20 @@ using namespace mb;
 
 extern "C" int64_t mb_linear_ce_workspace(const mb_linear_ce* a, int backward) {
     if (check("mb_linear_ce_workspace", a)) return -1;
-    return buffers_of(plan_of(a), backward != 0, nullptr).bytes;
+    const Plan p = a->dtype == MB_DTYPE_F32 ? plan_of<F32>(a) : plan_of<Bf16>(a);
+    return buffers_of(p, backward != 0, nullptr).bytes;
 }
 
 extern "C" int mb_linear_ce_fwd(const mb_linear_ce* a, void* stream) {
     if (const int rc = check("mb_linear_ce_fwd", a)) return rc;
     MB_REQUIRE(a->loss, "mb_linear_ce_fwd: null pointer argument");
-    return a->dtype == MB_DTYPE_F32 ? forward<float, _Float16, 2, 128>(a, (hipStream_t)stream)
-                                    : forward<__bf16, __bf16, 1, 256>(a, (hipStream_t)stream);
+    return a->dtype == MB_DTYPE_F32 ? forward<F32>(a, (hipStream_t)stream)
+                                    : forward<Bf16>(a, (hipStream_t)stream);
 }
 
 extern "C" int mb_linear_ce_bwd(const mb_linear_ce* a, void* stream) {
     if (const int rc = check("mb_linear_ce_bwd", a)) return rc;
     MB_REQUIRE(a->dloss, "mb_linear_ce_bwd: null pointer argument");
-    return a->dtype == MB_DTYPE_F32 ? backward<float, _Float16, 2, 128>(a, (hipStream_t)stream)
-                                    : backward<__bf16, __bf16, 1, 256>(a, (hipStream_t)stream);
+    return a->dtype == MB_DTYPE_F32 ? backward<F32>(a, (hipStream_t)stream)
+                                    : backward<Bf16>(a, (hipStream_t)stream);
 }

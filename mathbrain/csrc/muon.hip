@@ -23,10 +23,12 @@ namespace {
 
 using namespace g16;
 
+constexpr int kThreads = 256;
 constexpr int kChunk = 8192;     // elements of a workgroup in the norms' launch
 constexpr int kSquare = 64;      // of the planes' launch
 typedef Product<_Float16, 2, 128, 128, kRows, kRows> Gram;
 typedef Product<_Float16, 2, 128, 128, kCols, kRows> Apply;
+static_assert(Gram::kThreads == kThreads && Apply::kThreads == kThreads, "");
 
 struct Mat {
     const void* src;             // the matrix, or the gradient of a step
@@ -317,7 +319,7 @@ int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
         m.rows = (int)from.rows, m.cols = (int)from.cols;
         m.tall = m.rows > m.cols;
         m.m = std::min(m.rows, m.cols), m.n = std::max(m.rows, m.cols);
-        m.mp = (int)pad(m.m, kStep), m.np = (int)pad(m.n, kStep);
+        m.mp = (int)pad(m.m, kPad), m.np = (int)pad(m.n, kPad);
         m.src_bf16 = from.src_dtype == MB_DTYPE_BF16, m.dst_bf16 = from.dst_dtype == MB_DTYPE_BF16;
         m.momentum_bf16 = from.momentum_dtype == MB_DTYPE_BF16;
         m.rate = (float)from.rate;
