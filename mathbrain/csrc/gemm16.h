@@ -289,23 +289,52 @@ struct Product {
     }
 
     // The result as 16-bit values next to each other in p, by way of LDS: a lane's own four of a row would go out in 32
-    // pieces of 16 bytes an instruction.  hold() puts them there, after a barrier; store() takes a whole tile out, 16 bytes a
-    // lane, rows of q (q0 + r < q_end) and pieces of 8 p (p_end a multiple of 8) that are there.
+    // pieces of 16 bytes an instruction.  held() is a lane's place there for its elements r .. r + 3 of a block, to be written
+    // after a barrier; store() takes a whole tile out, 16 bytes a lane, rows of q (q0 + r < q_end) and pieces of 8 p
+    // (p_end a multiple of 8) that are there, fetch() brings one in.
     static constexpr int kOutPieces = TP / 8;
     static constexpr int kOutTurn = kOutPieces % 16 == 0 ? 15 : 7;
     static constexpr int kOutPlane = TP * TQ * 2;
-    __device__ static void hold(void* smem, int plane, int i, int j, int r, f16x4 v) {
-        const int q = col(j), piece = (wave_p() + 32 * i + 8 * (r / 4)) / 8, half = (threadIdx.x & 63) >> 5;
-        *(f16x4*)((char*)smem + plane * kOutPlane + q * (2 * TP) + ((piece ^ (q & kOutTurn)) << 4) + half * 8) = v;
+    __device__ static int out_at(int plane, int q, int piece) {
+        return plane * kOutPlane + q * (2 * TP) + ((piece ^ (q & kOutTurn)) << 4);
+    }
+    __device__ static f16x4& held(void* smem, int plane, int i, int j, int r) {
+        const int half = (threadIdx.x & 63) >> 5;
+        return *(f16x4*)((char*)smem + out_at(plane, col(j), (wave_p() + 32 * i + 8 * (r / 4)) / 8) + half * 8);
     }
     __device__ static void store(const void* smem, int plane, _Float16* out, int64_t ld, int p0, int q0, int p_end, int q_end) {
 #pragma unroll 4
         for (int n = threadIdx.x; n < TQ * kOutPieces; n += kThreads) {
             const int q = n / kOutPieces, piece = n % kOutPieces;
-            const f16x8 v = *(const f16x8*)((const char*)smem + plane * kOutPlane + q * (2 * TP) + ((piece ^ (q & kOutTurn)) << 4));
+            const f16x8 v = *(const f16x8*)((const char*)smem + out_at(plane, q, piece));
             if (q0 + q < q_end && p0 + piece * 8 < p_end) *(f16x8*)(out + (int64_t)(q0 + q) * ld + p0 + piece * 8) = v;
         }
     }
+    __device__ static void fetch(void* smem, int plane, const _Float16* in, int64_t ld, int p0, int q0, int p_end, int q_end) {
+#pragma unroll 4
+        for (int n = threadIdx.x; n < TQ * kOutPieces; n += kThreads) {
+            const int q = n / kOutPieces, piece = n % kOutPieces;
+            if (q0 + q < q_end && p0 + piece * 8 < p_end)
+                *(f16x8*)((char*)smem + out_at(plane, q, piece)) = *(const f16x8*)(in + (int64_t)(q0 + q) * ld + p0 + piece * 8);
+        }
+    }
+    // The tile's transpose: rows of p, pieces of 8 q (q_end a multiple of 8); 16 rows of 64 bytes an instruction.
+    __device__ static void store_turned(const void* smem, int plane, _Float16* out, int64_t ld, int p0, int q0, int p_end, int q_end) {
+        for (int n = threadIdx.x; n < TP * (TQ / 8); n += kThreads) {
+            const int p = n % 16 + n / (2 * TQ) * 16, piece = n / 16 % (TQ / 8);
+            f16x8 v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = *((const _Float16*)((const char*)smem + out_at(plane, piece * 8 + e, p / 8)) + p % 8);
+            if (p0 + p < p_end && q0 + piece * 8 < q_end) *(f16x8*)(out + (int64_t)(p0 + p) * ld + q0 + piece * 8) = v;
+        }
+    }
+    // The same for fp32 values, four next to each other.
+    static constexpr int kOut32 = TP * TQ * 4;
+    __device__ static int out32_at(int q, int piece) { return q * (4 * TP) + ((piece ^ (q & 15)) << 4); }
+    __device__ static f32x4v& held32(void* smem, int i, int j, int r) {
+        return *(f32x4v*)((char*)smem + out32_at(col(j), row(i, r) / 4));
+    }
+    __device__ static float out32(const void* smem, int q, int p) { return *((const float*)((const char*)smem + out32_at(q, p / 4)) + p % 4); }
 };
 
 // ---- planes ------------------------------------------------------------------------------

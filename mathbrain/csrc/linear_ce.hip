@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const Scor
                         hi[e] = (_Float16)u;
                     }
                 }
-                P::hold(smem, 0, i, j, r, hi);
-                if constexpr (PL == 2) P::hold(smem, 1, i, j, r, lo);
+                P::held(smem, 0, i, j, r) = hi;
+                if constexpr (PL == 2) P::held(smem, 1, i, j, r) = lo;
             }
     }
     static_assert(PL * P::kOutPlane <= P::kLds, "");
@@ -463,8 +463,8 @@ struct F32 {
     typedef float T;
     static constexpr int kPlanes = 2;
     typedef Product<_Float16, 2, 256, 128, kRows, kRows, 4, 2> Score;
-    typedef Product<_Float16, 2, 256, 128, kCols, kRows, 4, 2> GradH;
-    typedef Product<_Float16, 2, 256, 128, kCols, kCols, 4, 2> GradW;
+    typedef Product<_Float16, 2, 128, 128, kCols, kRows> GradH;
+    typedef Product<_Float16, 2, 128, 128, kCols, kCols> GradW;
 };
 
 struct Plan {

@@ -26,9 +26,15 @@ using namespace g16;
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;     // elements of a workgroup in the norms' launch
 constexpr int kSquare = 64;      // of the planes' launch
-typedef Product<_Float16, 2, 128, 128, kRows, kRows> Gram;
-typedef Product<_Float16, 2, 128, 128, kCols, kRows> Apply;
-static_assert(Gram::kThreads == kThreads && Apply::kThreads == kThreads, "");
+
+// The products by tiles of TILE x TILE: A and B (X and A with themselves), and X (B with X).
+template <int TILE>
+struct By {
+    typedef Product<_Float16, 2, TILE, TILE, kRows, kRows> Gram;
+    typedef Product<_Float16, 2, TILE, TILE, kCols, kRows> Apply;
+    static_assert(Gram::kThreads == kThreads && Apply::kThreads == kThreads, "");
+    static_assert(2 * Gram::kOutPlane <= Gram::kLds && Apply::kOut32 <= Apply::kLds, "results go out through LDS");
+};
 
 struct Mat {
     const void* src;             // the matrix, or the gradient of a step
@@ -40,7 +46,7 @@ struct Mat {
     uint8_t src_bf16, dst_bf16, momentum_bf16, tall;
     float rate;
 };
-enum { kFirstChunk, kFirstSquare, kFirstPair, kFirstTile, kFirsts };
+enum { kFirstChunk, kFirstSquare, kFirstPair, kFirstPair64, kFirstTile, kFirstTile64, kFirsts };
 
 constexpr int kMatsOfLaunch = 24;
 struct TableArgs {
@@ -59,12 +65,15 @@ __global__ void muon_table_kernel(const TableArgs a) {
     for (int f = 0; f < kFirsts; ++f) a.to_first[f * a.count + a.at + i] = a.first[f][i];
 }
 
+// Fewer tiles of 128 than this in a launch leave most of the card idle: tiles of 64 then.
+constexpr int64_t kFewTiles = 300;
+
 struct Args {
     const Mat* mats;
     const int* first;            // [kFirsts][count]
     int count;
     int from, to;                // X's buffers
-    float a, b, c;
+    float a, b, c;               // X <- X (a + b A + c A^2)
     float x_scale, a_scale, b_scale;
     double eps;
     float lr, mu, keep;          // keep = 1 - lr decay
@@ -91,13 +100,56 @@ __device__ inline void store1(void* p, int64_t i, bool bf16, float v) {
     else ((float*)p)[i] = v;
 }
 
+__device__ inline f32x4v load4(const void* p, int64_t i, bool bf16) {
+    if (!bf16) return *reinterpret_cast<const f32x4v*>((const float*)p + i);
+    typedef __bf16 bf16x4v __attribute__((ext_vector_type(4)));
+    const bf16x4v q = *reinterpret_cast<const bf16x4v*>((const __bf16*)p + i);
+    return f32x4v{(float)q[0], (float)q[1], (float)q[2], (float)q[3]};
+}
+__device__ inline void store4(void* p, int64_t i, bool bf16, f32x4v v) {
+    if (!bf16) {
+        *reinterpret_cast<f32x4v*>((float*)p + i) = v;
+    } else {
+        typedef __bf16 bf16x4v __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<bf16x4v*>((__bf16*)p + i) = bf16x4v{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    }
+}
+// Whether four elements at a multiple of four are aligned as load4 wants them.
+__device__ inline bool fours(const void* p, bool bf16) { return ((uintptr_t)p & (bf16 ? 7 : 15)) == 0; }
+
+__device__ inline double block_sum(double v) {
+    __shared__ double s[16];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s[0];
+    for (int i = 1; i < (int)blockDim.x / 64; ++i) v += s[i];
+    __syncthreads();
+    return v;
+}
+
 // Sums of squares in 64 bits; a step's momentum and G first.
 __global__ void __launch_bounds__(kThreads) muon_norm_kernel(const Args a) {
     int chunk = blockIdx.x;
     const Mat m = find(a, kFirstChunk, chunk);
     const int64_t total = (int64_t)m.rows * m.cols, e0 = (int64_t)chunk * kChunk, e1 = std::min(total, e0 + kChunk);
     double sum = 0.0;
-    for (int64_t e = e0 + threadIdx.x; e < e1; e += kThreads) {
+    const bool four = fours(m.src, m.src_bf16) && (!a.is_step || fours(m.momentum, m.momentum_bf16));
+    const int64_t e4 = four ? e0 + (e1 - e0) / 4 * 4 : e0;
+#pragma unroll 4
+    for (int64_t e = e0 + 4 * threadIdx.x; e < e4; e += 4 * kThreads) {
+        f32x4v g = load4(m.src, e, m.src_bf16);
+        if (a.is_step) {
+            const f32x4v mom = a.mu * load4(m.momentum, e, m.momentum_bf16) + g;
+            store4(m.momentum, e, m.momentum_bf16, mom);
+            g = a.nesterov ? g + a.mu * mom : mom;
+            *reinterpret_cast<f32x4v*>(m.u + e) = g;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = __builtin_fma((double)g[i], (double)g[i], sum);
+    }
+    for (int64_t e = e4 + threadIdx.x; e < e1; e += kThreads) {
         float g = load1(m.src, e, m.src_bf16);
         if (a.is_step) {
             const float mom = a.mu * load1(m.momentum, e, m.momentum_bf16) + g;
@@ -107,157 +159,164 @@ __global__ void __launch_bounds__(kThreads) muon_norm_kernel(const Args a) {
         }
         sum = __builtin_fma((double)g, (double)g, sum);
     }
-    __shared__ double s[kThreads / 64];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) m.part[chunk] = (s[0] + s[1]) + (s[2] + s[3]);
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) m.part[chunk] = sum;
 }
 
 // X's planes from G, 64 x 64 of X at a time, zeros around it.
 __global__ void __launch_bounds__(kThreads) muon_planes_kernel(const Args a) {
-    __shared__ double s[kThreads / 64];
     __shared__ float tile[kSquare][kSquare + 1];
     int id = blockIdx.x;
     const Mat m = find(a, kFirstSquare, id);
     double sum = 0.0;
     for (int i = threadIdx.x; i < m.chunks; i += kThreads) sum += m.part[i];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    const double norm = sqrt((s[0] + s[1]) + (s[2] + s[3]));
-    const double f = (double)a.x_scale / (norm + a.eps);
-    const int across = (m.np + kSquare - 1) / kSquare;
+    const double f = (double)a.x_scale / (sqrt(block_sum(sum)) + a.eps);
+    const int across = m.np / kSquare;
     const int i0 = id / across * kSquare, j0 = id % across * kSquare;
     const void* src = a.is_step ? (const void*)m.u : m.src;
     const bool bf16 = !a.is_step && m.src_bf16;
-    const int c = threadIdx.x % kSquare, r0 = threadIdx.x / kSquare;
-#pragma unroll 4
-    for (int r = r0; r < kSquare; r += kThreads / kSquare) {
-        // a tall matrix's squares are read along its own rows, and turned in LDS
-        const int i = m.tall ? i0 + c : i0 + r, j = m.tall ? j0 + r : j0 + c;
-        float v = 0.f;
-        if (i < m.m && j < m.n) v = (float)((double)load1(src, m.tall ? (int64_t)j * m.cols + i : (int64_t)i * m.cols + j, bf16) * f);
-        if (m.tall) tile[c][r] = v;
-        else tile[r][c] = v;
+    // rows and columns of the source's own square; a tall matrix's is turned on the way to LDS
+    const int r0 = m.tall ? j0 : i0, c0 = m.tall ? i0 : j0;
+    const bool four = m.cols % 4 == 0 && fours(src, bf16);
+    const int c = threadIdx.x % 16 * 4;
+#pragma unroll
+    for (int r = threadIdx.x / 16; r < kSquare; r += kThreads / 16) {
+        f32x4v v = {0.f, 0.f, 0.f, 0.f};
+        const int64_t at = (int64_t)(r0 + r) * m.cols + c0 + c;
+        if (r0 + r < m.rows) {
+            if (four && c0 + c < m.cols) {
+                v = load4(src, at, bf16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c0 + c + e < m.cols) v[e] = load1(src, at + e, bf16);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) (m.tall ? tile[c + e][r] : tile[r][c + e]) = (float)((double)v[e] * f);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int r = r0; r < kSquare; r += kThreads / kSquare) {
-        const int i = i0 + r, j = j0 + c;
-        if (i < m.mp && j < m.np) {
-            _Float16 hi, lo;
-            split(tile[r][c], hi, lo);
-            m.x[0][(int64_t)i * m.np + j] = hi;
-            m.x[0][(int64_t)(m.mp + i) * m.np + j] = lo;
+#pragma unroll
+    for (int n = threadIdx.x; n < kSquare * kSquare / 8; n += kThreads) {
+        const int r = n / 8, p = n % 8 * 8;
+        f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 h, l;
+            split(tile[r][p + e], h, l);
+            hi[e] = h, lo[e] = l;
         }
+        const int64_t to = (int64_t)(i0 + r) * m.np + j0 + p;
+        *reinterpret_cast<f16x8*>(m.x[0] + to) = hi;
+        *reinterpret_cast<f16x8*>(m.x[0] + (int64_t)m.mp * m.np + to) = lo;
     }
 }
 
-// Four values next to each other as planes; `at` of the first, `plane` elements to the second plane.
-__device__ inline void store_planes(_Float16* x, int64_t at, int64_t plane, const float* v, f16x4& hi, f16x4& lo) {
+__device__ inline void split4(const float* v, f16x4& hi, f16x4& lo) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         _Float16 h, l;
         split(v[e], h, l);
         hi[e] = h, lo[e] = l;
     }
-    *reinterpret_cast<f16x4*>(x + at) = hi;
-    *reinterpret_cast<f16x4*>(x + plane + at) = lo;
 }
 
-// POLY: B = b A + c A^2 from A's planes; otherwise A = X X^T.
-template <bool POLY>
-__global__ void __launch_bounds__(kThreads, 2) muon_pair_kernel(const Args a) {
+// POLY: B = a + b A + c A^2 from A's planes; otherwise A = X X^T.
+template <bool POLY, int TILE>
+__global__ void __launch_bounds__(kThreads, By<TILE>::Gram::kWaves) muon_pair_kernel(const Args a) {
+    typedef typename By<TILE>::Gram Gram;
     extern __shared__ char smem[];
     int id = blockIdx.x;
-    const Mat m = find(a, kFirstPair, id);
+    const Mat m = find(a, TILE == 64 ? kFirstPair64 : kFirstPair, id);
     int q = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);   // id = q (q + 1) / 2 + p, p <= q
     while (q * (q + 1) / 2 > id) --q;
     while ((q + 1) * (q + 2) / 2 <= id) ++q;
     q = uniform(q);
-    const int p = id - q * (q + 1) / 2, p0 = p * Gram::TP, q0 = q * Gram::TQ;
+    const int p = id - q * (q + 1) / 2, p0 = p * TILE, q0 = q * TILE;
     const int64_t plane = (int64_t)m.mp * m.mp;
     const Side side = POLY ? Side{m.a, plane * 2, m.mp, m.mp} : Side{m.x[a.from], (int64_t)m.mp * m.np * 2, m.np, m.mp};
     Gram g;
     g.run(side, side, p0, q0, 0, POLY ? m.mp : m.np, smem);
+    __syncthreads();
+    if (POLY) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) Gram::fetch(smem, h, m.a + h * plane, m.mp, p0, q0, m.mp, m.mp);
+        __syncthreads();
+    }
     _Float16* out = POLY ? m.b : m.a;
     const float from = POLY ? a.a_scale : a.x_scale, to = POLY ? a.b_scale : a.a_scale;
-    const float f = (POLY ? a.c : 1.f) * to / from / from, fb = a.b * to / a.a_scale;
+    const float f = (POLY ? a.c : 1.f) * to / from / from, fb = a.b * to / a.a_scale, one = a.a * to;
 #pragma unroll
-    for (int j = 0; j < Gram::FQ; ++j) {
-        const int col = q0 + Gram::col(j);
-        if (col >= m.mp) continue;
+    for (int j = 0; j < Gram::FQ; ++j)
 #pragma unroll
         for (int i = 0; i < Gram::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const int row = p0 + Gram::row(i, r);
-                if (row >= m.mp) continue;
-                const int64_t at = (int64_t)col * m.mp + row;
+                f16x4 &hi = Gram::held(smem, 0, i, j, r), &lo = Gram::held(smem, 1, i, j, r);
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = g.acc[i][j][r + e] * f;
-                if (POLY) {
-                    const f16x4 hi = *reinterpret_cast<const f16x4*>(m.a + at), lo = *reinterpret_cast<const f16x4*>(m.a + plane + at);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += fb * ((float)hi[e] + (float)lo[e]);
-                }
-                f16x4 hi, lo;
-                store_planes(out, at, plane, v, hi, lo);
-                if (p != q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        out[(int64_t)(row + e) * m.mp + col] = hi[e];
-                        out[plane + (int64_t)(row + e) * m.mp + col] = lo[e];
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = g.acc[i][j][r + e] * f;
+                    if (POLY) {
+                        v[e] += fb * ((float)hi[e] + (float)lo[e]);
+                        if (p0 + Gram::row(i, r) + e == q0 + Gram::col(j)) v[e] += one;
                     }
+                }
+                split4(v, hi, lo);
             }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        Gram::store(smem, h, out + h * plane, m.mp, p0, q0, m.mp, m.mp);
+        if (p != q) Gram::store_turned(smem, h, out + h * plane, m.mp, p0, q0, m.mp, m.mp);
     }
 }
 
-__global__ void __launch_bounds__(kThreads, 2) muon_apply_kernel(const Args a) {
+template <int TILE>
+__global__ void __launch_bounds__(kThreads, By<TILE>::Apply::kWaves) muon_apply_kernel(const Args a) {
+    typedef typename By<TILE>::Apply Apply;
     extern __shared__ char smem[];
     int id = blockIdx.x;
-    const Mat m = find(a, kFirstTile, id);
-    const int across = (m.np + Apply::TP - 1) / Apply::TP;
-    const int p0 = id % across * Apply::TP, q0 = id / across * Apply::TQ;
+    const Mat m = find(a, TILE == 64 ? kFirstTile64 : kFirstTile, id);
+    const int across = (m.np + TILE - 1) / TILE;
+    const int p0 = id % across * TILE, q0 = id / across * TILE;
     const int64_t plane = (int64_t)m.mp * m.np;
-    const _Float16* x = m.x[a.from];
     Apply g;
-    g.run(Side{x, plane * 2, m.np, m.np}, Side{m.b, (int64_t)m.mp * m.mp * 2, m.mp, m.mp}, p0, q0, 0, m.mp, smem);
-    const float out = a.last ? 1.f / a.x_scale : 1.f;
-    const float f = out / a.b_scale, fx = a.a * out;
+    g.run(Side{m.x[a.from], plane * 2, m.np, m.np}, Side{m.b, (int64_t)m.mp * m.mp * 2, m.mp, m.mp}, p0, q0, 0, m.mp, smem);
+    const float f = (a.last ? 1.f / a.x_scale : 1.f) / a.b_scale;
+    __syncthreads();
+    if (!a.last) {
 #pragma unroll
-    for (int j = 0; j < Apply::FQ; ++j) {
-        const int i = q0 + Apply::col(j);
-        if (i >= m.mp) continue;
+        for (int j = 0; j < Apply::FQ; ++j)
 #pragma unroll
-        for (int k = 0; k < Apply::FP; ++k)
+            for (int i = 0; i < Apply::FP; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int c = p0 + Apply::row(k, r);
-                if (c >= m.np) continue;
-                const int64_t at = (int64_t)i * m.np + c;
-                const f16x4 hi = *reinterpret_cast<const f16x4*>(x + at), lo = *reinterpret_cast<const f16x4*>(x + plane + at);
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = g.acc[k][j][r + e] * f + fx * ((float)hi[e] + (float)lo[e]);
-                if (!a.last) {
-                    f16x4 h, l;
-                    store_planes(m.x[a.to], at, plane, v, h, l);
-                    continue;
+                for (int r = 0; r < 16; r += 4) {
+                    const float v[4] = {g.acc[i][j][r] * f, g.acc[i][j][r + 1] * f, g.acc[i][j][r + 2] * f, g.acc[i][j][r + 3] * f};
+                    split4(v, Apply::held(smem, 0, i, j, r), Apply::held(smem, 1, i, j, r));
                 }
+        __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (i >= m.m || c + e >= m.n) continue;
-                    const int64_t to = m.tall ? (int64_t)(c + e) * m.cols + i : (int64_t)i * m.cols + c + e;
-                    float y = v[e];
-                    if (a.is_step) y = load1(m.dst, to, m.dst_bf16) * a.keep - a.lr * m.rate * y;
-                    store1(m.dst, to, m.dst_bf16, y);
-                }
-            }
+        for (int h = 0; h < 2; ++h) Apply::store(smem, h, m.x[a.to] + h * plane, m.np, p0, q0, m.np, m.mp);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < Apply::FQ; ++j)
+#pragma unroll
+        for (int i = 0; i < Apply::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                Apply::held32(smem, i, j, r) = f32x4v{g.acc[i][j][r], g.acc[i][j][r + 1], g.acc[i][j][r + 2], g.acc[i][j][r + 3]} * f;
+    __syncthreads();
+    // lanes next to each other along the result's own rows
+#pragma unroll 4
+    for (int n = threadIdx.x; n < TILE * TILE; n += kThreads) {
+        const int q = m.tall ? n % TILE : n / TILE, p = m.tall ? n / TILE : n % TILE;
+        if (q0 + q >= m.m || p0 + p >= m.n) continue;
+        const int64_t to = m.tall ? (int64_t)(p0 + p) * m.cols + q0 + q : (int64_t)(q0 + q) * m.cols + p0 + p;
+        float y = Apply::out32(smem, q, p);
+        if (a.is_step) y = load1(m.dst, to, m.dst_bf16) * a.keep - a.lr * m.rate * y;
+        store1(m.dst, to, m.dst_bf16, y);
     }
 }
 
@@ -330,9 +389,8 @@ int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
         if (p->is_step) m.u = (float*)take(elements * 4);
         m.part = (double*)take(m.chunks * 8);
         if (out) {
-            const int64_t pairs = (m.mp + Gram::TP - 1) / Gram::TP;
-            const int64_t items[kFirsts] = {m.chunks, pad(m.mp, kSquare) / kSquare * (pad(m.np, kSquare) / kSquare), pairs * (pairs + 1) / 2,
-                                            pad(m.np, Apply::TP) / Apply::TP * (pad(m.mp, Apply::TQ) / Apply::TQ)};
+            const int64_t m64 = m.mp / 64, n64 = m.np / 64, m128 = (m64 + 1) / 2, n128 = (n64 + 1) / 2;
+            const int64_t items[kFirsts] = {m.chunks, m64 * n64, m128 * (m128 + 1) / 2, m64 * (m64 + 1) / 2, m128 * n128, m64 * n64};
             for (int f = 0; f < kFirsts; ++f) {
                 out->first[f].push_back((int)out->blocks[f]);
                 out->blocks[f] += items[f];
@@ -373,15 +431,35 @@ int run(const char* what, const mb_muon* p, hipStream_t st) {
     const dim3 blk(kThreads);
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.blocks[kFirstChunk]), blk, 0, st, a);
     hipLaunchKernelGGL(muon_planes_kernel, dim3((unsigned)l.blocks[kFirstSquare]), blk, 0, st, a);
+    const bool small_pairs = l.blocks[kFirstPair] < kFewTiles, small_tiles = l.blocks[kFirstTile] < kFewTiles;
     for (int step = 0; step < p->steps; ++step) {
         a.from = step & 1, a.to = a.from ^ 1, a.last = step + 1 == p->steps;
-        hipLaunchKernelGGL(muon_pair_kernel<false>, dim3((unsigned)l.blocks[kFirstPair]), blk, Gram::kLds, st, a);
-        hipLaunchKernelGGL(muon_pair_kernel<true>, dim3((unsigned)l.blocks[kFirstPair]), blk, Gram::kLds, st, a);
-        hipLaunchKernelGGL(muon_apply_kernel, dim3((unsigned)l.blocks[kFirstTile]), blk, Apply::kLds, st, a);
+        const auto pair = [&](auto tile, unsigned blocks) {
+            constexpr int TILE = decltype(tile)::value;
+            static Told told[2];
+            constexpr int lds = By<TILE>::Gram::kLds;
+            if (const int rc = allow_lds(what, (const void*)muon_pair_kernel<false, TILE>, lds, told[0])) return rc;
+            if (const int rc = allow_lds(what, (const void*)muon_pair_kernel<true, TILE>, lds, told[1])) return rc;
+            hipLaunchKernelGGL((muon_pair_kernel<false, TILE>), dim3(blocks), blk, lds, st, a);
+            hipLaunchKernelGGL((muon_pair_kernel<true, TILE>), dim3(blocks), blk, lds, st, a);
+            return MB_OK;
+        };
+        const auto apply = [&](auto tile, unsigned blocks) {
+            constexpr int TILE = decltype(tile)::value;
+            static Told told;
+            constexpr int lds = By<TILE>::Apply::kLds;
+            if (const int rc = allow_lds(what, (const void*)muon_apply_kernel<TILE>, lds, told)) return rc;
+            hipLaunchKernelGGL((muon_apply_kernel<TILE>), dim3(blocks), blk, lds, st, a);
+            return MB_OK;
+        };
+        typedef std::integral_constant<int, 64> T64;
+        typedef std::integral_constant<int, 128> T128;
+        int rc = small_pairs ? pair(T64(), (unsigned)l.blocks[kFirstPair64]) : pair(T128(), (unsigned)l.blocks[kFirstPair]);
+        if (rc == MB_OK) rc = small_tiles ? apply(T64(), (unsigned)l.blocks[kFirstTile64]) : apply(T128(), (unsigned)l.blocks[kFirstTile]);
+        if (rc != MB_OK) return rc;
     }
     return check_launch(what);
 }
-static_assert(Gram::kLds <= 65536 && Apply::kLds <= 65536, "more has to be asked for");
 
 }  // namespace
 }  // namespace mb
