@@ -769,7 +769,7 @@ typedef struct mb_muon {
     int64_t count, steps, is_step, nesterov;
     double a, b, c, eps;
     int64_t x_exponent, a_exponent, b_exponent; /* 2^exponent times the largest singular value of any iterate X */
-                                  /*   (at most 1 at first), A and a + b A + c A^2 must stay below 65504 */
+                                  /*   (at most 1 at first), A and b A + c A^2 must stay below 65504 */
     double lr, momentum, weight_decay;
     void *workspace;              /* at a multiple of 256 bytes, mb_muon_workspace(args) bytes (-1: refused) */
     int64_t workspace_bytes;

@@ -145,6 +145,12 @@ struct Tile {
             }
         }
     };
+    // Four values of free indices i .. i + 3 (i a multiple of 4) at k of a kCols tile.
+    typedef T four_t __attribute__((ext_vector_type(4)));
+    static __device__ four_t four(uint32_t tile, int i, int k) {
+        static_assert(ORDER == kCols, "");
+        return *(__attribute__((address_space(3))) const four_t*)(uintptr_t)(tile + k * kRow + (((i >> 3) ^ swz(k)) << 4) + 2 * (i & 7));
+    }
     static __device__ typename Frag<T>::type read(uint32_t tile, const Lane& l, int i0, int c) {
         typedef typename Frag<T>::type F;
         if constexpr (ORDER == kRows) {
@@ -198,7 +204,12 @@ struct Product {
     };
 
     // k from k0 to k1, multiples of kStep (k1 > k0).  All waves have to be here; LDS is free again after the next barrier.
-    __device__ void run(const Side& p_, const Side& q_, int p0, int q0, int k0, int k1, void* smem) {
+    // peek(k, tile) sees every step's operands in LDS (P's planes, then Q's) while they are there.
+    __device__ void run(const Side& p, const Side& q, int p0, int q0, int k0, int k1, void* smem) {
+        run(p, q, p0, q0, k0, k1, smem, [](int, uint32_t) {});
+    }
+    template <typename F>
+    __device__ void run(const Side& p_, const Side& q_, int p0, int q0, int k0, int k1, void* smem, F peek) {
         const uint32_t lds = lds_address(smem);
         const Side p = uniform(p_), q = uniform(q_);
         p0 = uniform(p0), q0 = uniform(q0), k0 = uniform(k0);
@@ -210,6 +221,10 @@ struct Product {
         const char* qb = (const char*)q.p + TileQ::at(q, q0, k0);
         const int64_t pstep = TileP::at(p, 0, kStep), qstep = TileQ::at(q, 0, kStep);
         const int steps = uniform((k1 - k0) / kStep);
+        // A wave with a single block has two results, of alternate instructions, added at the end: each instruction would
+        // wait for the one before.
+        constexpr bool kTwo = FP * FQ == 1;
+        f32x16 second = {};
         // load n of the wave's for a step
         auto load = [&](uint32_t tile, int n) {
             constexpr int all = PLANES * TileP::kLoads;
@@ -251,6 +266,7 @@ struct Product {
                 wait_and_meet<decltype(more)::value ? (kStages - 2) * kLoads : 0>();
                 read(f[0], stage(t), 0);
             }
+            peek(k0 + t * kStep, stage(t));
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 if (c + 1 < C) {
@@ -266,7 +282,10 @@ struct Product {
 #pragma unroll
                     for (int i = 0; i < FP; ++i) {
 #pragma unroll
-                        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(x.a[k == 0][i], x.b[k == 1][j], acc[i][j]);
+                        for (int j = 0; j < FQ; ++j) {
+                            f32x16& to_ = kTwo && (c * kProducts + k) % 2 ? second : acc[i][j];
+                            to_ = mma(x.a[k == 0][i], x.b[k == 1][j], to_);
+                        }
                         const int g = (c * kProducts + k - 3 + kProducts) * FP + i;
                         if constexpr (decltype(more)::value) {
 #pragma unroll
@@ -286,6 +305,7 @@ struct Product {
         for (; t + kStages - 1 < steps; ++t) step(t, std::true_type(), std::false_type());
         for (; t + 1 < steps; ++t) step(t, std::false_type(), std::false_type());
         step(t, std::false_type(), std::true_type());
+        if constexpr (kTwo) acc[0][0] += second;
     }
 
     // The result as 16-bit values next to each other in p, by way of LDS: a lane's own four of a row would go out in 32

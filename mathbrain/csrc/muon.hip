@@ -29,11 +29,16 @@ constexpr int kSquare = 64;      // of the planes' launch
 
 // The products by tiles of TILE x TILE: A and B (X and A with themselves), and X (B with X).
 template <int TILE>
-struct By {
-    typedef Product<_Float16, 2, TILE, TILE, kRows, kRows> Gram;
-    typedef Product<_Float16, 2, TILE, TILE, kCols, kRows> Apply;
-    static_assert(Gram::kThreads == kThreads && Apply::kThreads == kThreads, "");
-    static_assert(2 * Gram::kOutPlane <= Gram::kLds && Apply::kOut32 <= Apply::kLds, "results go out through LDS");
+struct By;
+template <>
+struct By<128> {
+    typedef Product<_Float16, 2, 128, 128, kRows, kRows, 2, 4, 64> Gram;
+    typedef Product<_Float16, 2, 128, 128, kCols, kRows> Apply;
+};
+template <>
+struct By<64> {
+    typedef Product<_Float16, 2, 64, 64, kRows, kRows, 2, 2, 64> Gram;
+    typedef Product<_Float16, 2, 64, 64, kCols, kRows, 2, 2, 64> Apply;
 };
 
 struct Mat {
@@ -65,20 +70,31 @@ __global__ void muon_table_kernel(const TableArgs a) {
     for (int f = 0; f < kFirsts; ++f) a.to_first[f * a.count + a.at + i] = a.first[f][i];
 }
 
-// Fewer tiles of 128 than this in a launch leave most of the card idle: tiles of 64 then.
-constexpr int64_t kFewTiles = 300;
+// Each of the eight XCDs, to which workgroups go in turn, takes a run of a launch's tiles, of about the same cost each:
+// what a matrix's tiles share is fetched into one or two L2s instead of all eight.
+constexpr int kXcds = 8;
+struct Runs {
+    int from[kXcds + 1];
+};
 
 struct Args {
     const Mat* mats;
     const int* first;            // [kFirsts][count]
     int count;
     int from, to;                // X's buffers
-    float a, b, c;               // X <- X (a + b A + c A^2)
+    float a, b, c;
     float x_scale, a_scale, b_scale;
     double eps;
     float lr, mu, keep;          // keep = 1 - lr decay
     int nesterov, is_step, last;
+    Runs runs;                   // of this launch
 };
+
+// The workgroup's tile, or -1.
+__device__ inline int tile_of(const Runs& r) {
+    const int xcd = blockIdx.x % kXcds, id = r.from[xcd] + (int)(blockIdx.x / kXcds);
+    return id < r.from[xcd + 1] ? id : -1;
+}
 
 // The matrix that holds item `id` of a launch, and the item's number in it.
 __device__ inline Mat find(const Args& a, int which, int& id) {
@@ -221,12 +237,14 @@ __device__ inline void split4(const float* v, f16x4& hi, f16x4& lo) {
     }
 }
 
-// POLY: B = a + b A + c A^2 from A's planes; otherwise A = X X^T.
+// POLY: B = b A + c A^2 from A's planes; otherwise A = X X^T.
 template <bool POLY, int TILE>
-__global__ void __launch_bounds__(kThreads, By<TILE>::Gram::kWaves) muon_pair_kernel(const Args a) {
+__global__ void __launch_bounds__(By<TILE>::Gram::kThreads, By<TILE>::Gram::kWaves) muon_pair_kernel(const Args a) {
     typedef typename By<TILE>::Gram Gram;
+    static_assert(2 * Gram::kOutPlane <= Gram::kLds, "results go out through LDS");
     extern __shared__ char smem[];
-    int id = blockIdx.x;
+    int id = tile_of(a.runs);
+    if (id < 0) return;
     const Mat m = find(a, TILE == 64 ? kFirstPair64 : kFirstPair, id);
     int q = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);   // id = q (q + 1) / 2 + p, p <= q
     while (q * (q + 1) / 2 > id) --q;
@@ -245,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, By<TILE>::Gram::kWaves) muon_pair_ke
     }
     _Float16* out = POLY ? m.b : m.a;
     const float from = POLY ? a.a_scale : a.x_scale, to = POLY ? a.b_scale : a.a_scale;
-    const float f = (POLY ? a.c : 1.f) * to / from / from, fb = a.b * to / a.a_scale, one = a.a * to;
+    const float f = (POLY ? a.c : 1.f) * to / from / from, fb = a.b * to / a.a_scale;
 #pragma unroll
     for (int j = 0; j < Gram::FQ; ++j)
 #pragma unroll
@@ -257,10 +275,7 @@ __global__ void __launch_bounds__(kThreads, By<TILE>::Gram::kWaves) muon_pair_ke
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] = g.acc[i][j][r + e] * f;
-                    if (POLY) {
-                        v[e] += fb * ((float)hi[e] + (float)lo[e]);
-                        if (p0 + Gram::row(i, r) + e == q0 + Gram::col(j)) v[e] += one;
-                    }
+                    if (POLY) v[e] += fb * ((float)hi[e] + (float)lo[e]);
                 }
                 split4(v, hi, lo);
             }
@@ -273,50 +288,273 @@ __global__ void __launch_bounds__(kThreads, By<TILE>::Gram::kWaves) muon_pair_ke
 }
 
 template <int TILE>
-__global__ void __launch_bounds__(kThreads, By<TILE>::Apply::kWaves) muon_apply_kernel(const Args a) {
+__global__ void __launch_bounds__(By<TILE>::Apply::kThreads, By<TILE>::Apply::kWaves) muon_apply_kernel(const Args a) {
     typedef typename By<TILE>::Apply Apply;
+    static_assert(2 * Apply::kOutPlane <= Apply::kLds && Apply::kOut32 <= Apply::kLds, "results go out through LDS");
     extern __shared__ char smem[];
-    int id = blockIdx.x;
+    int id = tile_of(a.runs);
+    if (id < 0) return;
     const Mat m = find(a, TILE == 64 ? kFirstTile64 : kFirstTile, id);
     const int across = (m.np + TILE - 1) / TILE;
     const int p0 = id % across * TILE, q0 = id / across * TILE;
     const int64_t plane = (int64_t)m.mp * m.np;
+    const _Float16* x = m.x[a.from];
     Apply g;
-    g.run(Side{m.x[a.from], plane * 2, m.np, m.np}, Side{m.b, (int64_t)m.mp * m.mp * 2, m.mp, m.mp}, p0, q0, 0, m.mp, smem);
-    const float f = (a.last ? 1.f / a.x_scale : 1.f) / a.b_scale;
-    __syncthreads();
-    if (!a.last) {
+    // X's own tile comes by among the rows of X that are multiplied: at k = the lane's row of the result
+    f16x4 xh[Apply::FQ][Apply::FP][4], xl[Apply::FQ][Apply::FP][4];
+    g.run(Side{x, plane * 2, m.np, m.np}, Side{m.b, (int64_t)m.mp * m.mp * 2, m.mp, m.mp}, p0, q0, 0, m.mp, smem, [&](int k, uint32_t tile) {
 #pragma unroll
-        for (int j = 0; j < Apply::FQ; ++j)
+        for (int j = 0; j < Apply::FQ; ++j) {
+            const int i = q0 + Apply::wave_q() + 32 * j - k;
+            if (i < 0 || i >= Apply::kStep) continue;
 #pragma unroll
-            for (int i = 0; i < Apply::FP; ++i)
+            for (int n = 0; n < Apply::FP; ++n)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const float v[4] = {g.acc[i][j][r] * f, g.acc[i][j][r + 1] * f, g.acc[i][j][r + 2] * f, g.acc[i][j][r + 3] * f};
-                    split4(v, Apply::held(smem, 0, i, j, r), Apply::held(smem, 1, i, j, r));
+                for (int r = 0; r < 4; ++r) {
+                    xh[j][n][r] = Apply::TileP::four(tile, Apply::row(n, 4 * r), i + (threadIdx.x & 31));
+                    xl[j][n][r] = Apply::TileP::four(tile + Apply::TileP::kBytes, Apply::row(n, 4 * r), i + (threadIdx.x & 31));
                 }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) Apply::store(smem, h, m.x[a.to] + h * plane, m.np, p0, q0, m.np, m.mp);
-        return;
-    }
+        }
+    });
+    // a X is added here: as a B with a on its diagonal every sum over k would be rounded at a X's size
+    const float out = a.last ? 1.f / a.x_scale : 1.f, f = out / a.b_scale, fx = a.a * out;
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < Apply::FQ; ++j)
 #pragma unroll
         for (int i = 0; i < Apply::FP; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                Apply::held32(smem, i, j, r) = f32x4v{g.acc[i][j][r], g.acc[i][j][r + 1], g.acc[i][j][r + 2], g.acc[i][j][r + 3]} * f;
+            for (int r = 0; r < 16; r += 4) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = g.acc[i][j][r + e] * f + fx * ((float)xh[j][i][r / 4][e] + (float)xl[j][i][r / 4][e]);
+                if (!a.last) split4(v, Apply::held(smem, 0, i, j, r), Apply::held(smem, 1, i, j, r));
+                else Apply::held32(smem, i, j, r) = f32x4v{v[0], v[1], v[2], v[3]};
+            }
     __syncthreads();
-    // lanes next to each other along the result's own rows
-#pragma unroll 4
-    for (int n = threadIdx.x; n < TILE * TILE; n += kThreads) {
-        const int q = m.tall ? n % TILE : n / TILE, p = m.tall ? n / TILE : n % TILE;
-        if (q0 + q >= m.m || p0 + p >= m.n) continue;
-        const int64_t to = m.tall ? (int64_t)(p0 + p) * m.cols + q0 + q : (int64_t)(q0 + q) * m.cols + p0 + p;
-        float y = Apply::out32(smem, q, p);
-        if (a.is_step) y = load1(m.dst, to, m.dst_bf16) * a.keep - a.lr * m.rate * y;
-        store1(m.dst, to, m.dst_bf16, y);
+    if (!a.last) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) Apply::store(smem, h, m.x[a.to] + h * plane, m.np, p0, q0, m.np, m.mp);
+        return;
+    }
+    // four values of a row of the result a thread, all that a step wants of the old weights on their way at once
+    constexpr int kEach = TILE * TILE / 4 / Apply::kThreads;
+    const bool four = m.cols % 4 == 0 && fours(m.dst, m.dst_bf16);
+    const int r0 = m.tall ? p0 : q0, c0 = m.tall ? q0 : p0;
+    f32x4v old[kEach];
+    auto place = [&](int n, int& r, int& c) {
+        const int i = n * Apply::kThreads + threadIdx.x;
+        r = i / (TILE / 4), c = i % (TILE / 4) * 4;
+        return (int64_t)(r0 + r) * m.cols + c0 + c;
+    };
+    if (a.is_step) {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            int r, c;
+            const int64_t at = place(n, r, c);
+            if (r0 + r >= m.rows) continue;
+            if (four && c0 + c < m.cols) {
+                old[n] = load4(m.dst, at, m.dst_bf16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) old[n][e] = c0 + c + e < m.cols ? load1(m.dst, at + e, m.dst_bf16) : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+        int r, c;
+        const int64_t at = place(n, r, c);
+        if (r0 + r >= m.rows) continue;
+        f32x4v y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = m.tall ? Apply::out32(smem, c + e, r) : Apply::out32(smem, r, c + e);
+        if (a.is_step) y = old[n] * a.keep - (a.lr * m.rate) * y;
+        if (four && c0 + c < m.cols) {
+            store4(m.dst, at, m.dst_bf16, y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c0 + c + e < m.cols) store1(m.dst, at + e, m.dst_bf16, y[e]);
+        }
+    }
+}
+
+// ---- small matrices ----------------------------------------------------------------------
+//
+// Where X's and A's planes fit into a CU's LDS, one workgroup of 16 waves takes a matrix through all steps: what the
+// launches of the general case, some 5 us each whatever they do, cost most there.  A wave takes 32 x 32 blocks of each
+// product; B stands in A's place and X's new columns in the old ones', after a barrier: 16 blocks at a time.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallLds = 159 * 1024;
+constexpr int kSmallEach = kSmallLds / 4 / kSmallThreads;    // elements of a thread, at most
+
+struct SmallArgs {
+    Mat m[kMatsOfLaunch];
+    Args a;
+    int steps;
+};
+static_assert(sizeof(SmallArgs) <= 4096, "kernel arguments");
+
+__host__ __device__ inline int small_lds(int mp, int np) { return 4 * mp * np + 4 * mp * mp; }
+
+// A matrix's planes in LDS, rows of a multiple of 8 pieces, piece c of row r in the place c ^ swz(r).
+struct Held {
+    uint32_t lds;       // address of the first plane
+    int row, plane;     // bytes
+    __device__ int turn(int r) const {
+        return row % 256 == 0 ? (r & 3) << 2 | ((r >> 2) & 3) : ((r >> 1) & 1) << 2 | ((r >> 3) & 1) << 1 | ((r >> 2) & 1);
+    }
+    __device__ uint32_t at(int h, int r, int i) const { return lds + h * plane + r * row + (((i >> 3) ^ turn(r)) << 4) + 2 * (i & 7); }
+    // rows r0 + lane % 32, k = k0 + 8 (lane / 32) + 0 .. 7
+    __device__ f16x8 rows(int h, int r0, int k0) const {
+        const int lane = threadIdx.x & 63;
+        return *(__attribute__((address_space(3))) const f16x8*)(uintptr_t)at(h, r0 + (lane & 31), k0 + 8 * (lane >> 5));
+    }
+    // columns i0 + lane % 32, rows k0 + 8 (lane / 32) + 0 .. 7
+    __device__ f16x8 cols(int h, int i0, int k0) const {
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const int lane = threadIdx.x & 63, r = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2), d = i0 + (lane & 16) + 4 * (lane & 3);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at(h, r, d));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at(h, r + 4, d));
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ f16x4 four(int h, int r, int i) const { return *(__attribute__((address_space(3))) const f16x4*)(uintptr_t)at(h, r, i); }
+    __device__ void four(int h, int r, int i, f16x4 v) const { *(__attribute__((address_space(3))) f16x4*)(uintptr_t)at(h, r, i) = v; }
+    __device__ void one(int h, int r, int i, _Float16 v) const { *(__attribute__((address_space(3))) _Float16*)(uintptr_t)at(h, r, i) = v; }
+};
+
+// A 32 x 32 block: rows p0.. of P (or its columns), rows q0.. of Q, over k.
+template <bool COLS>
+__device__ inline f32x16 small_block(const Held& p, const Held& q, int p0, int q0, int k) {
+    f32x16 x = {}, y = {};
+    for (int k0 = 0; k0 < k; k0 += 16) {
+        const f16x8 ah = COLS ? p.cols(0, p0, k0) : p.rows(0, p0, k0), al = COLS ? p.cols(1, p0, k0) : p.rows(1, p0, k0);
+        const f16x8 bh = q.rows(0, q0, k0), bl = q.rows(1, q0, k0);
+        y = mma(al, bh, y);
+        x = mma(ah, bh, x);
+        y = mma(ah, bl, y);
+    }
+    return x + y;
+}
+
+__global__ void __launch_bounds__(kSmallThreads) muon_small_kernel(const SmallArgs s) {
+    extern __shared__ char smem[];
+    const Args& a = s.a;
+    const Mat& m = s.m[blockIdx.x];
+    const int mp = m.mp, np = m.np, lane = threadIdx.x & 63, wave = wave_id(), total = m.rows * m.cols;
+    const Held x = {lds_address(smem), 2 * np, 2 * mp * np}, g = {lds_address(smem) + 4 * mp * np, 2 * mp, 2 * mp * mp};
+    // G, a few elements a thread, and its norm
+    float v[kSmallEach];
+    double sum = 0.0;
+#pragma unroll
+    for (int n = 0; n < kSmallEach; ++n) {
+        const int e = n * kSmallThreads + (int)threadIdx.x;
+        v[n] = 0.f;
+        if (e >= total) continue;
+        v[n] = load1(m.src, e, m.src_bf16);
+        if (a.is_step) {
+            const float mom = a.mu * load1(m.momentum, e, m.momentum_bf16) + v[n];
+            store1(m.momentum, e, m.momentum_bf16, mom);
+            v[n] = a.nesterov ? v[n] + a.mu * mom : mom;
+        }
+        sum = __builtin_fma((double)v[n], (double)v[n], sum);
+    }
+    for (int i = threadIdx.x; i < mp * np / 4; i += kSmallThreads) ((f32x4v*)smem)[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    const double f = (double)a.x_scale / (sqrt(block_sum(sum)) + a.eps);     // its barriers are those of the zeros, too
+#pragma unroll
+    for (int n = 0; n < kSmallEach; ++n) {
+        const int e = n * kSmallThreads + (int)threadIdx.x;
+        if (e >= total) continue;
+        const int r = e / m.cols, c = e - r * m.cols;
+        _Float16 hi, lo;
+        split((float)((double)v[n] * f), hi, lo);
+        x.one(0, m.tall ? c : r, m.tall ? r : c, hi);
+        x.one(1, m.tall ? c : r, m.tall ? r : c, lo);
+    }
+    __syncthreads();
+    const int bm = mp / 32, bn = np / 32;
+    const float to_a = a.a_scale / a.x_scale / a.x_scale, square = a.c * a.b_scale / a.a_scale / a.a_scale, linear = a.b * a.b_scale / a.a_scale;
+    const int col = lane & 31, row0 = 4 * (lane >> 5);
+    for (int step = 0; step < s.steps; ++step) {
+        const bool last = step + 1 == s.steps;
+        const int q0 = wave / bm * 32, p0 = wave % bm * 32;      // bm * bm is at most 16
+        if (wave < bm * bm) {
+            const f32x16 acc = small_block<false>(x, x, p0, q0, np);
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const float w[4] = {acc[r] * to_a, acc[r + 1] * to_a, acc[r + 2] * to_a, acc[r + 3] * to_a};
+                f16x4 hi, lo;
+                split4(w, hi, lo);
+                g.four(0, q0 + col, p0 + 2 * r + row0, hi);
+                g.four(1, q0 + col, p0 + 2 * r + row0, lo);
+            }
+        }
+        __syncthreads();
+        f16x4 hi[4], lo[4];
+        if (wave < bm * bm) {
+            const f32x16 acc = small_block<false>(g, g, p0, q0, mp);
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int p = p0 + 2 * r + row0;
+                const f16x4 h = g.four(0, q0 + col, p), l = g.four(1, q0 + col, p);
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = acc[r + e] * square + linear * ((float)h[e] + (float)l[e]);
+                split4(w, hi[r / 4], lo[r / 4]);
+            }
+        }
+        __syncthreads();
+        if (wave < bm * bm)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                g.four(0, q0 + col, p0 + 2 * r + row0, hi[r / 4]);
+                g.four(1, q0 + col, p0 + 2 * r + row0, lo[r / 4]);
+            }
+        __syncthreads();
+        const float out = last ? 1.f / a.x_scale : 1.f, f = out / a.b_scale, fx = a.a * out;
+        const int wide = 16 / bm;                                 // columns' blocks at a time
+        for (int b0 = 0; b0 < bn; b0 += wide) {
+            const int i0 = wave % bm * 32, j0 = (b0 + wave / bm) * 32;
+            const bool mine = wave < bm * wide && j0 < np;
+            f32x16 acc = {};
+            if (mine) {
+                acc = small_block<true>(x, g, j0, i0, mp);
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f16x4 h = x.four(0, i0 + col, j0 + 2 * r + row0), l = x.four(1, i0 + col, j0 + 2 * r + row0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[r + e] = acc[r + e] * f + fx * ((float)h[e] + (float)l[e]);
+                }
+            }
+            if (last) {
+                const int i = i0 + col;
+                if (mine && i < m.m)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = j0 + 8 * (r / 4) + row0 + r % 4;
+                        if (j >= m.n) continue;
+                        const int to = m.tall ? j * m.cols + i : i * m.cols + j;
+                        float y = acc[r];
+                        if (a.is_step) y = load1(m.dst, to, m.dst_bf16) * a.keep - (a.lr * m.rate) * y;
+                        store1(m.dst, to, m.dst_bf16, y);
+                    }
+                continue;
+            }
+            __syncthreads();
+            if (mine)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const float w[4] = {acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
+                    f16x4 h, l;
+                    split4(w, h, l);
+                    x.four(0, i0 + col, j0 + 2 * r + row0, h);
+                    x.four(1, i0 + col, j0 + 2 * r + row0, l);
+                }
+        }
+        __syncthreads();
     }
 }
 
@@ -353,7 +591,27 @@ struct Layout {
     std::vector<Mat> mats;
     std::vector<int> first[kFirsts];
     int64_t blocks[kFirsts] = {};
-    int64_t bytes = 0;
+
+    // The XCDs' runs of a launch whose tiles cost their matrix's n (or m) each, and its grid.
+    Runs runs(int which, bool by_n, unsigned& grid) const {
+        auto cost = [&](size_t i) { return (int64_t)(by_n ? mats[i].np : mats[i].mp) + 128; };   // and what a tile takes to begin and end
+        auto end = [&](size_t i) { return i + 1 < mats.size() ? first[which][i + 1] : (int)blocks[which]; };
+        int64_t total = 0, before = 0;
+        for (size_t i = 0; i < mats.size(); ++i) total += cost(i) * (end(i) - first[which][i]);
+        Runs r = {};
+        int x = 1;
+        for (size_t i = 0; i < mats.size(); ++i) {
+            const int n = end(i) - first[which][i];
+            for (; x < kXcds && total * x / kXcds <= before + cost(i) * n; ++x)
+                r.from[x] = first[which][i] + (int)((total * x / kXcds - before + cost(i) / 2) / cost(i));
+            before += cost(i) * n;
+        }
+        for (; x <= kXcds; ++x) r.from[x] = (int)blocks[which];
+        int most = 0;
+        for (x = 0; x < kXcds; ++x) most = std::max(most, r.from[x + 1] - r.from[x]);
+        grid = (unsigned)(most * kXcds);
+        return r;
+    }
 };
 
 int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
@@ -401,6 +659,12 @@ int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
     return used;
 }
 
+bool small_ones(const std::vector<Mat>& mats) {
+    return std::all_of(mats.begin(), mats.end(), [](const Mat& m) {
+        return m.mp <= 128 && (int64_t)4 * m.mp * (m.np + m.mp) <= kSmallLds && (int64_t)m.rows * m.cols <= kSmallEach * kSmallThreads;
+    });
+}
+
 int64_t table_bytes(int64_t count) { return pad(count * (int64_t)sizeof(Mat), 256) + pad(count * (int64_t)sizeof(int) * kFirsts, 256); }
 
 int run(const char* what, const mb_muon* p, hipStream_t st) {
@@ -419,6 +683,20 @@ int run(const char* what, const mb_muon* p, hipStream_t st) {
     a.x_scale = ldexpf(1.f, (int)p->x_exponent), a.a_scale = ldexpf(1.f, (int)p->a_exponent), a.b_scale = ldexpf(1.f, (int)p->b_exponent);
     a.lr = (float)p->lr, a.mu = (float)p->momentum, a.keep = (float)(1.0 - p->lr * p->weight_decay);
     a.nesterov = p->nesterov != 0, a.is_step = p->is_step != 0;
+    // Small matrices alone: with larger ones among them the general launches are there anyway, and the small ones cost little in them.
+    if (small_ones(l.mats)) {
+        static Told told;
+        if (const int rc = allow_lds(what, (const void*)muon_small_kernel, kSmallLds, told)) return rc;
+        for (int at = 0; at < count; at += kMatsOfLaunch) {
+            SmallArgs t = {};
+            const int n = std::min(kMatsOfLaunch, count - at);
+            t.a = a, t.steps = (int)p->steps;
+            int lds = 0;
+            for (int i = 0; i < n; ++i) t.m[i] = l.mats[at + i], lds = std::max(lds, small_lds(t.m[i].mp, t.m[i].np));
+            hipLaunchKernelGGL(muon_small_kernel, dim3(n), dim3(kSmallThreads), lds, st, t);
+        }
+        return check_launch(what);
+    }
     for (int at = 0; at < count; at += kMatsOfLaunch) {
         TableArgs t = {};
         t.to = (Mat*)a.mats, t.to_first = (int*)a.first, t.at = at, t.n = std::min(kMatsOfLaunch, count - at), t.count = count;
@@ -431,31 +709,44 @@ int run(const char* what, const mb_muon* p, hipStream_t st) {
     const dim3 blk(kThreads);
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.blocks[kFirstChunk]), blk, 0, st, a);
     hipLaunchKernelGGL(muon_planes_kernel, dim3((unsigned)l.blocks[kFirstSquare]), blk, 0, st, a);
-    const bool small_pairs = l.blocks[kFirstPair] < kFewTiles, small_tiles = l.blocks[kFirstTile] < kFewTiles;
+    // Tiles of 64 or 128, by what a round of them took for 64 k (us; 4 matrices of 2816 x 1024, 3 of 777 x 1234): pairs 1.0
+    // for up to 512 of 64 and 1.4 for 256 of 128, B X 1.35 for 512 of 64, 2.9 for 512 of 128.
+    auto rounds = [](int64_t n, int64_t most) { return (double)((n + most - 1) / most); };
+    const bool small_pairs = rounds(l.blocks[kFirstPair64], 512) * 1.0 < rounds(l.blocks[kFirstPair], 256) * 1.4;
+    const bool small_tiles = rounds(l.blocks[kFirstTile64], 512) * 1.35 < rounds(l.blocks[kFirstTile], 512) * 2.9;
+    const int pairs = small_pairs ? kFirstPair64 : kFirstPair, tiles = small_tiles ? kFirstTile64 : kFirstTile;
+    unsigned gram_grid, poly_grid, apply_grid;
+    const Runs gram_runs = l.runs(pairs, true, gram_grid), poly_runs = l.runs(pairs, false, poly_grid),
+               apply_runs = l.runs(tiles, false, apply_grid);
     for (int step = 0; step < p->steps; ++step) {
         a.from = step & 1, a.to = a.from ^ 1, a.last = step + 1 == p->steps;
-        const auto pair = [&](auto tile, unsigned blocks) {
+        const auto pair = [&](auto tile) {
             constexpr int TILE = decltype(tile)::value;
             static Told told[2];
             constexpr int lds = By<TILE>::Gram::kLds;
+            const dim3 blk(By<TILE>::Gram::kThreads);
             if (const int rc = allow_lds(what, (const void*)muon_pair_kernel<false, TILE>, lds, told[0])) return rc;
             if (const int rc = allow_lds(what, (const void*)muon_pair_kernel<true, TILE>, lds, told[1])) return rc;
-            hipLaunchKernelGGL((muon_pair_kernel<false, TILE>), dim3(blocks), blk, lds, st, a);
-            hipLaunchKernelGGL((muon_pair_kernel<true, TILE>), dim3(blocks), blk, lds, st, a);
+            a.runs = gram_runs;
+            hipLaunchKernelGGL((muon_pair_kernel<false, TILE>), dim3(gram_grid), blk, lds, st, a);
+            a.runs = poly_runs;
+            hipLaunchKernelGGL((muon_pair_kernel<true, TILE>), dim3(poly_grid), blk, lds, st, a);
             return MB_OK;
         };
-        const auto apply = [&](auto tile, unsigned blocks) {
+        const auto apply = [&](auto tile) {
             constexpr int TILE = decltype(tile)::value;
             static Told told;
             constexpr int lds = By<TILE>::Apply::kLds;
+            const dim3 blk(By<TILE>::Apply::kThreads);
             if (const int rc = allow_lds(what, (const void*)muon_apply_kernel<TILE>, lds, told)) return rc;
-            hipLaunchKernelGGL((muon_apply_kernel<TILE>), dim3(blocks), blk, lds, st, a);
+            a.runs = apply_runs;
+            hipLaunchKernelGGL((muon_apply_kernel<TILE>), dim3(apply_grid), blk, lds, st, a);
             return MB_OK;
         };
         typedef std::integral_constant<int, 64> T64;
         typedef std::integral_constant<int, 128> T128;
-        int rc = small_pairs ? pair(T64(), (unsigned)l.blocks[kFirstPair64]) : pair(T128(), (unsigned)l.blocks[kFirstPair]);
-        if (rc == MB_OK) rc = small_tiles ? apply(T64(), (unsigned)l.blocks[kFirstTile64]) : apply(T128(), (unsigned)l.blocks[kFirstTile]);
+        int rc = small_pairs ? pair(T64()) : pair(T128());
+        if (rc == MB_OK) rc = small_tiles ? apply(T64()) : apply(T128());
         if (rc != MB_OK) return rc;
     }
     return check_launch(what);

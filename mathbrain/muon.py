@@ -28,16 +28,16 @@ _ARGS = struct.Struct("P4q4d3q3dPq")       # mb_muon
 
 @functools.lru_cache(maxsize=64)
 def _exponents(steps, coefficients):
-    """Powers of two for the planes of X, A and a + b A + c A^2 from bounds on their singular values: X's are at most 1 at
+    """Powers of two for the planes of X, A and b A + c A^2 from bounds on their singular values: X's are at most 1 at
     first, and after each step at most the polynomial's largest value on the interval so far."""
     a, b, c = coefficients
     top, most = 1.0, [1.0, 1.0, 0.0]
     for _ in range(steps):
         s = torch.linspace(0.0, top, 20001, dtype=torch.float64)
         gram = s * s
-        second = a + b * gram + c * gram * gram
+        second = b * gram + c * gram * gram
         most = [max(most[0], top), max(most[1], top * top), max(most[2], float(second.abs().max()))]
-        top = 1.01 * float((s * second).abs().max())     # between the points, and roundings
+        top = 1.01 * float((s * (a + second)).abs().max())     # between the points, and roundings
         if not top < 64.0:
             raise ValueError(f"orthogonalize: with coefficients {coefficients} the iterates grow beyond 64 in {steps} steps")
     return tuple(min(15, math.floor(math.log2(32768.0 / max(1.05 * m, 2.0**-10)))) for m in most)

@@ -49,7 +49,7 @@ def test_all_shapes_together_and_alone(t):
     assert all(x.dtype == t for x in got)
     for x, y in zip(got, mats):
         check(x, definition(y), what=tuple(y.shape))
-        assert torch.equal(orthogonalize([y])[0], x), tuple(y.shape)
+        check(orthogonalize([y])[0], definition(y), what=tuple(y.shape))       # small ones alone have a kernel of their own
     for x, y in zip(orthogonalize(mats, dtype=torch.float32), mats):
         check(x, definition(y), what=tuple(y.shape))
 
@@ -105,13 +105,30 @@ def test_forms_of_the_input():
     assert torch.equal(orthogonalize(view), orthogonalize(view.contiguous()))
     assert torch.equal(orthogonalize(view.t()), orthogonalize(view.t().contiguous()))
     assert orthogonalize([]) == [] and orthogonalize(x[:, :0]).shape == (3, 0, 40, 70) and orthogonalize(x[..., :0]).shape == (3, 2, 40, 0)
-    a, b, c = orthogonalize([x[0, 0], torch.empty(0, 5, device="cuda"), x[0, 1]])
+    a, b, c = orthogonalize([x[0, 0], torch.empty(0, 5, device="cuda"), x[0, 1]])     # (all of them small)
     assert b.shape == (0, 5) and torch.equal(a, got[0, 0]) and torch.equal(c, got[0, 1])
     assert torch.equal(orthogonalize([x[0, 0], x[0, 0]])[1], got[0, 0])      # the same tensor twice is read twice
     w = torch.nn.Parameter(x[0, 0])
     assert not orthogonalize(w).requires_grad
     mixed = orthogonalize([x[0, 0], x[0, 1].bfloat16()])
     assert mixed[0].dtype == torch.float32 and mixed[1].dtype == torch.bfloat16
+
+
+def test_small_matrices_alone():
+    """Up to what a CU's LDS holds, and just beyond: rows, columns, both ways round, every type, steps and decay."""
+    from mathbrain.muon import muon_step, orthogonalize
+    g = torch.Generator("cuda").manual_seed(8)
+    for shape in ((1, 1), (64, 64), (65, 64), (128, 128), (128, 192), (192, 128), (128, 193), (64, 570), (570, 64), (64, 577), (1, 570),
+                  (33, 300), (129, 5), (100, 190), (17, 63)):
+        for t in (torch.float32, torch.bfloat16):
+            x = (torch.randn(shape, generator=g, device="cuda") * 3).to(t)
+            check(orthogonalize(x), definition(x), what=shape)
+            check(orthogonalize(x, steps=2), definition(x, 2), 2, what=shape)
+            p, m = torch.zeros_like(x), torch.randn(shape, generator=g, device="cuda").to(t)
+            want_m = 0.9 * m.double() + x.double()
+            muon_step([p], [x], [m], 1.0, momentum=0.9, nesterov=False)
+            check(-p / math.sqrt(max(1.0, shape[0] / shape[1])), definition(want_m), what=shape)
+            assert ((m.double() - want_m).abs() <= half_step(t) * want_m.abs() + 2.0**-22 * (want_m.abs() + 30)).all()
 
 
 def test_many_matrices():
