@@ -199,6 +199,15 @@ struct Product {
     }
     __device__ static int col(int j) { return wave_q() + 32 * j + (threadIdx.x & 31); }
 
+    __device__ void clear() {
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    }
+
     struct Frags {
         typename Frag<T>::type a[PLANES][FP], b[PLANES][FQ];
     };
@@ -233,12 +242,7 @@ struct Product {
                              qb + (n - all) / TileQ::kLoads * q.plane, qo);
         };
         auto stage = [&](int t) { return lds + t % kStages * kStage; };
-#pragma unroll
-        for (int i = 0; i < FP; ++i)
-#pragma unroll
-            for (int j = 0; j < FQ; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        clear();
         __builtin_amdgcn_s_waitcnt(0x0F70);   // the compiler's own loads are done: it would wait for the DMA with them
         for (int t = 0; t < kStages - 1 && t < steps; ++t) {
 #pragma unroll

@@ -40,6 +40,15 @@ struct Targets {
         return t == ignore ? -1 : t < 0 || t >= V ? -2 : (int)t;
     }
 };
+// The rows that the scores are taken for: with many rows those that count alone, next to each other (`rows` their
+// numbers, `pos` each row's place or -1, `m` how many); otherwise all, in their places.
+struct Rows {
+    const int *rows, *pos, *m;
+    int N;
+    __device__ int count() const { return m ? __builtin_amdgcn_readfirstlane(*m) : N; }
+    __device__ int at(int c) const { return rows ? rows[c] : c; }
+    __device__ int of(int64_t n) const { return pos ? pos[n] : (int)n; }
+};
 // The gradient of each row's loss; without dloss 1, and 0 for the ignored rows.
 struct RowGrad {
     Targets t;
@@ -76,25 +85,61 @@ __device__ inline void load8(const T* p, bool vec, int left, float* v) {
     }
 }
 
-// A user's matrix: [rows, D], rows ld apart.
+// Places for the rows that count.  A workgroup takes a run of rows, and first counts what counts before it: its targets are
+// read by the workgroups behind it, too, out of L2, and nobody waits for another.
+__global__ void __launch_bounds__(kThreads) ce_rows_kernel(const Targets t, int N, int each, int* rows, int* pos, int* m) {
+    __shared__ int s[64];
+    const int n0 = blockIdx.x * each, n1 = min(N, n0 + each);
+    int before = 0, total;
+#pragma unroll 16
+    for (int n = threadIdx.x; n < n0; n += kThreads) before += t.at(n) != -1;
+    block_exclusive_scan(before, s, total);
+    int base = total;
+    for (int n = n0; n < n1; n += kThreads) {
+        const int i = n + (int)threadIdx.x;
+        const bool counts = i < n1 && t.at(i) != -1;
+        const int c = base + block_exclusive_scan(counts, s, total);
+        if (i < n1) pos[i] = counts ? c : -1;
+        if (counts) rows[c] = i;
+        base += total;
+    }
+    if (n1 == N && threadIdx.x == 0) *m = base;
+}
+
+// A user's matrix [rows, D], rows ld apart, with what the scaling and the copies of it want to know.
 struct Matrix {
     const void* p;
     int64_t ld;
     int rows, D, vec;
+    int graded;                  // times each row's g; an ignored row counts for nothing, whatever it holds
+    float* largest;              // the largest magnitudes of the workgroups' parts; copies without: not scaled
+    int blocks;
+    float* scale;
+    void* out;                   // planes [rows_pad, Dp]
+    int rows_pad, Dp, gathered;  // gathered: rows in their places of Rows
+};
+// Two matrices a launch; the second may have no blocks.
+struct Pair {
+    Matrix x, y;
+    RowGrad g;
+    Rows r;
 };
 
-// The largest finite magnitude of x (with g: of g_n x_n) of each workgroup's part: part[blockIdx.x].
-template <typename T, bool G>
-__global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Matrix x, const RowGrad g, float* part) {
+// The largest finite magnitude of each workgroup's part of x (graded: of g_n x_n).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Pair a) {
+    const bool first = (int)blockIdx.x < a.x.blocks;
+    const Matrix& x = first ? a.x : a.y;
+    const int block = first ? blockIdx.x : blockIdx.x - a.x.blocks;
     const int pieces = (x.D + 7) / 8;
     float most = 0.f;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)x.rows * pieces; i += (int64_t)gridDim.x * kThreads) {
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)x.rows * pieces; i += (int64_t)x.blocks * kThreads) {
         const int64_t n = i / pieces;
         const int d = (int)(i - n * pieces) * 8;
+        const float gn = x.graded ? fabsf(a.g.at(n)) : 1.f;
+        if (gn == 0.f) continue;
         float v[8];
         load8((const T*)x.p + n * x.ld + d, x.vec, x.D - d, v);
-        const float gn = G ? fabsf(g.at(n)) : 1.f;
-        if (gn == 0.f) continue;   // whatever an ignored row holds
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float m = fabsf(v[e]) * gn;
@@ -102,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Matrix x, co
         }
     }
     most = block_max(most);
-    if (threadIdx.x == 0) part[blockIdx.x] = most;
+    if (threadIdx.x == 0) x.largest[block] = most;
 }
 
 __device__ inline float scale_from(const float* part, int n) {
@@ -111,43 +156,44 @@ __device__ inline float scale_from(const float* part, int n) {
     return plane_scale(__builtin_bit_cast(uint32_t, block_max(m)));
 }
 
-// x (with g: g_n x_n) as PL planes [rows_pad, Dp] of O, zeros around it, scaled by the largest value of `part`
-// (parts 0: not scaled).  The scale goes to *scale.
-template <typename T, typename O, int PL, bool G>
-__global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Matrix x, const RowGrad g, const float* part, int parts, float* scale,
-                                                             O* out, int rows_pad, int Dp) {
+// x (graded: g_n x_n) as PL planes [rows_pad, Dp] of O, zeros around it, scaled by its largest value, which goes to *scale.
+template <typename T, typename O, int PL>
+__global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Pair a, int x_blocks) {
+    const bool first = (int)blockIdx.x < x_blocks;
+    const Matrix& x = first ? a.x : a.y;
+    const int block = first ? blockIdx.x : blockIdx.x - x_blocks, blocks = first ? x_blocks : gridDim.x - x_blocks;
     float s = 1.f;
-    if (parts) {
-        s = scale_from(part, parts);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *scale = s;
+    if (x.largest) {
+        s = scale_from(x.largest, x.blocks);
+        if (block == 0 && threadIdx.x == 0) *x.scale = s;
     }
-    const int pieces = Dp / 8;
+    const int pieces = x.Dp / 8, count = x.gathered ? a.r.count() : x.rows;
+    O* out = (O*)x.out;
     typedef O vec8 __attribute__((ext_vector_type(8), aligned(16)));
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)rows_pad * pieces; i += (int64_t)gridDim.x * kThreads) {
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)x.rows_pad * pieces; i += (int64_t)blocks * kThreads) {
         const int64_t n = i / pieces;
         const int d = (int)(i - n * pieces) * 8;
-        float v[8];
-        if (n < x.rows) load8((const T*)x.p + n * x.ld + d, x.vec, x.D - d, v);
-        else
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        if (G && n < x.rows) {
-            const float gn = g.at(n);
+        float v[8] = {};
+        if (n < count) {
+            const int64_t row = x.gathered ? a.r.at((int)n) : n;
+            const float gn = x.graded ? a.g.at(row) : 1.f;
+            load8((const T*)x.p + row * x.ld + d, x.vec, x.D - d, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = gn == 0.f ? 0.f : v[e] * gn;
+            for (int e = 0; e < 8; ++e) v[e] = gn == 0.f ? 0.f : v[e] * gn * s;
         }
         vec8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if constexpr (PL == 2) {
-                _Float16 a, b;
-                split(v[e] * s, a, b);
-                hi[e] = a, lo[e] = b;
+                _Float16 h, l;
+                split(v[e], h, l);
+                hi[e] = h, lo[e] = l;
             } else {
-                hi[e] = (O)(v[e] * s);
+                hi[e] = (O)v[e];
             }
         }
-        *reinterpret_cast<vec8*>(out + n * Dp + d) = hi;
-        if constexpr (PL == 2) *reinterpret_cast<vec8*>(out + ((int64_t)rows_pad + n) * Dp + d) = lo;
+        *reinterpret_cast<vec8*>(out + n * x.Dp + d) = hi;
+        if constexpr (PL == 2) *reinterpret_cast<vec8*>(out + ((int64_t)x.rows_pad + n) * x.Dp + d) = lo;
     }
 }
 
@@ -155,9 +201,9 @@ __global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Matrix x, con
 // eight tiles of rows walk the vocabulary together: what is at work at once on an XCD fits its L2.
 constexpr int kXcds = 8, kTogether = 8;
 __device__ inline bool tile_of(int tiles_p, int tiles_q, int& p, int& q) {
-    const int each = gridDim.x / kXcds;
+    const int64_t tiles = (int64_t)tiles_p * tiles_q, each = (tiles + kXcds - 1) / kXcds;
     const int64_t id = (int64_t)(blockIdx.x % kXcds) * each + blockIdx.x / kXcds;
-    if (id >= (int64_t)tiles_p * tiles_q) return false;
+    if (blockIdx.x / kXcds >= each || id >= tiles) return false;
     const int64_t run = (int64_t)tiles_p * kTogether;
     const int group = (int)(id / run), rest = (int)(id - group * run);
     const int wide = min(kTogether, tiles_q - group * kTogether);
@@ -171,13 +217,14 @@ struct ScoreArgs {
     Side w, h;                    // kRows: [V, Dp], [N, Dp]
     const float *scale_w, *scale_h;   // NULL: 1
     Targets t;
-    int V, N, Dp, tiles_p, tiles_q;
+    Rows r;
+    int V, N, Dp, tiles_p;
     float2* part;                 // forward: [tiles_p, N] maximum and sum
     float* target_score;          // forward: [N]
     const float* lse;             // backward: [2, N]
-    _Float16* u;                  // backward: [PL][n_pad, width], the piece's entries from v0 on
-    int v0, v1, n_pad;
-    int64_t width;
+    _Float16* u;                  // backward: [PL][rows, width], the piece's entries from v0 on
+    int v0, v1;
+    int64_t plane, width;         // elements to the second plane, and to the next row
 };
 
 template <typename P>
@@ -189,18 +236,19 @@ template <typename P>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const ScoreArgs a) {
     extern __shared__ char smem[];
     int tp, tq;
-    if (!tile_of(a.tiles_p, a.tiles_q, tp, tq)) return;
+    const int count = a.r.count();
+    if (!tile_of(a.tiles_p, (count + P::TQ - 1) / P::TQ, tp, tq)) return;
     const int p0 = tp * P::TP, q0 = tq * P::TQ;
     P prod;
     const float f = score_factor<P>(a);
-    prod.run(a.w, a.h, p0, q0, 0, a.Dp, smem);
+    prod.run(a.w, Side{a.h.p, a.h.plane, a.h.ld, count}, p0, q0, 0, a.Dp, smem);
     float2* both = (float2*)smem;   // [2][TQ]
     float m[P::FQ], sum[P::FQ];
     const bool tail = p0 + P::TP > a.V;
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j) {
         const int n = q0 + P::col(j);
-        const int target = n < a.N ? a.t.at(n) : -1;
+        const int target = n < count ? a.t.at(a.r.at(n)) : -1;
         m[j] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
@@ -236,7 +284,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const 
         if ((threadIdx.x & 63) < 32) both[half * P::TQ + P::col(j)] = make_float2(m[j], sum[j]);
     __syncthreads();
     for (int c = threadIdx.x; c < P::TQ; c += P::kThreads)
-        if (q0 + c < a.N) {
+        if (q0 + c < count) {
             float top = both[c].x, t = 0.f;
 #pragma unroll
             for (int w = 1; w < P::kWavesP; ++w) top = fmaxf(top, both[w * P::TQ + c].x);
@@ -251,6 +299,7 @@ struct JoinArgs {
     const float2* part;
     const float* target_score;
     Targets t;
+    Rows r;
     int N, parts, reduction;
     float *loss, *lse, *count;
     double* sums;     // [2, blocks]: losses and counted rows (reduction 1 and 2)
@@ -268,8 +317,9 @@ __global__ void __launch_bounds__(kThreads) ce_join_kernel(const JoinArgs a) {
         sum = sum * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
         m = top;
     };
-    if (n < a.N)
-        for (int i = slice; i < a.parts; i += kSlices) take(a.part[(int64_t)i * a.N + n]);
+    const int place = n < a.N ? a.r.of(n) : -1;
+    if (place >= 0)
+        for (int i = slice; i < a.parts; i += kSlices) take(a.part[(int64_t)i * a.N + place]);
     s[slice][c] = make_float2(m, sum);
     __syncthreads();
     if (slice == 0) {
@@ -280,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) ce_join_kernel(const JoinArgs a) {
             const int target = a.t.at(n);
             counts = target != -1;
             const float l = __builtin_log2f(sum);
-            if (counts) loss = target < 0 ? NAN : kLn2 * ((m - a.target_score[n]) + l);
+            if (counts) loss = target < 0 ? NAN : kLn2 * ((m - a.target_score[place]) + l);
             a.lse[n] = target < 0 && counts ? NAN : m;     // a target outside the vocabulary: NaN, in the gradients too
             a.lse[a.N + n] = l;
             if (a.reduction == 0) a.loss[n] = loss;
@@ -320,16 +370,17 @@ template <typename P, int PL>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const ScoreArgs a) {
     extern __shared__ char smem[];
     int tp, tq;
-    if (!tile_of(a.tiles_p, a.tiles_q, tp, tq)) return;
+    const int count = a.r.count();
+    if (!tile_of(a.tiles_p, (count + P::TQ - 1) / P::TQ, tp, tq)) return;
     const int p0 = a.v0 + tp * P::TP, q0 = tq * P::TQ;
     P prod;
     const float f = score_factor<P>(a);
-    prod.run(a.w, a.h, p0, q0, 0, a.Dp, smem);
+    prod.run(a.w, Side{a.h.p, a.h.plane, a.h.ld, count}, p0, q0, 0, a.Dp, smem);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j) {
-        const int n = q0 + P::col(j);
-        const int target = n < a.N ? a.t.at(n) : -1;
+        const int n = q0 + P::col(j) < count ? a.r.at(q0 + P::col(j)) : -1;
+        const int target = n >= 0 ? a.t.at(n) : -1;
         const bool counts = target != -1;
         const float m = counts ? a.lse[n] : 0.f, l = counts ? a.lse[a.N + n] : 0.f;
 #pragma unroll
@@ -357,14 +408,16 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const Scor
     }
     static_assert(PL * P::kOutPlane <= P::kLds, "");
     __syncthreads();
-    const int64_t plane = (int64_t)a.n_pad * a.width;
+    const int end = (count + kPad - 1) / kPad * kPad;
 #pragma unroll
-    for (int h = 0; h < PL; ++h) P::store(smem, h, a.u + h * plane - a.v0, a.width, p0, q0, a.v0 + (int)a.width, a.n_pad);
+    for (int h = 0; h < PL; ++h) P::store(smem, h, a.u + h * a.plane - a.v0, a.width, p0, q0, a.v0 + (int)a.width, end);
 }
 
 struct PartArgs {
     Side p, q;
-    int tiles_p, tiles_q, splits, k1;   // k from 0 to k1, shared out to the splits in whole steps
+    Rows r;                             // of one of the two
+    int k_rows;                         // whether k is the rows; otherwise the result's rows are
+    int tiles_p, tiles_q, splits, k1;   // k from 0 to k1 (or the last row that counts), shared out to the splits in whole steps
     float* out;                         // [splits][q.n, ld]
     int64_t ld;
     int add;                            // onto what is there
@@ -376,14 +429,17 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     const int tiles = a.tiles_p * a.tiles_q;
     const int split = block / tiles, tile = block - split * tiles;
     const int p0 = tile % a.tiles_p * P::TP, q0 = tile / a.tiles_p * P::TQ;
-    const int steps = a.k1 / P::kStep;
+    const int count = a.r.count(), end = a.k_rows ? a.q.n : count;
+    if (q0 >= end) return;
+    const int steps = (a.k_rows ? (count + kPad - 1) / kPad * kPad : a.k1) / P::kStep;
     const int k0 = (int)((int64_t)steps * split / a.splits) * P::kStep, k1 = (int)((int64_t)steps * (split + 1) / a.splits) * P::kStep;
     P prod;
-    prod.run(a.p, a.q, p0, q0, k0, k1, smem);
+    if (k1 > k0) prod.run(a.p, Side{a.q.p, a.q.plane, a.q.ld, end}, p0, q0, k0, k1, smem);
+    else prod.clear();
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j) {
         const int q = q0 + P::col(j);
-        if (q >= a.q.n) continue;
+        if (q >= end) continue;
         float* to = a.out + ((int64_t)split * a.q.n + q) * a.ld;
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
@@ -410,26 +466,35 @@ __global__ void __launch_bounds__(H::kThreads, H::kWaves) ce_part_kernel(const P
     else part_of<W>(w, h_first ? block - n : block, smem);
 }
 
-// out[n, d] = factor (g_n) sum_s part[s][n, d], in the parts' order.
-template <typename T, bool G>
-__global__ void __launch_bounds__(kThreads) ce_sum_kernel(const float* part, int splits, int rows, int D, int ld, const float* scale,
-                                                          const RowGrad g, T* out) {
-    const float f = 1.f / *scale / kUScale;
-    const int pieces = ld / 4;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)rows * pieces; i += (int64_t)gridDim.x * kThreads) {
+// out[n, d] = factor (g_n) sum_s part[s][n, d], in the parts' order; graded rows come from their places.
+struct SumArgs {
+    const float* part;
+    int splits, rows, D, ld, graded, blocks;
+    const float* scale;
+    void* out;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const SumArgs y, const RowGrad g, const Rows r) {
+    const bool first = (int)blockIdx.x < x.blocks;
+    const SumArgs& a = first ? x : y;
+    const int block = first ? blockIdx.x : blockIdx.x - x.blocks;
+    const float f = 1.f / *a.scale / kUScale;
+    const int pieces = a.ld / 4;
+    T* out = (T*)a.out;
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)a.rows * pieces; i += (int64_t)a.blocks * kThreads) {
         const int64_t n = i / pieces;
         const int d = (int)(i - n * pieces) * 4;
-        f32x4v v = *reinterpret_cast<const f32x4v*>(part + n * ld + d);
-        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4v*>(part + ((int64_t)s * rows + n) * ld + d);
-        float fn = f;
-        if (G) {
-            const float gn = g.at(n);
-            fn = f * gn;
-            if (gn == 0.f) v = f32x4v{0.f, 0.f, 0.f, 0.f};
+        const int64_t from = a.graded ? r.of(n) : n;
+        f32x4v v = {0.f, 0.f, 0.f, 0.f};
+        const float gn = a.graded ? g.at(n) : 1.f;
+        if (from >= 0 && gn != 0.f) {
+            v = *reinterpret_cast<const f32x4v*>(a.part + from * a.ld + d);
+            for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4v*>(a.part + ((int64_t)s * a.rows + from) * a.ld + d);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (d + e < D) out[n * D + d + e] = (T)(v[e] * fn);
+            if (d + e < a.D) out[n * a.D + d + e] = (T)(v[e] * f * gn);
     }
 }
 
@@ -450,6 +515,8 @@ struct Carve {
 // U's bytes in a piece: pieces are large enough to fill the card and small beside the scores.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 constexpr int kCus = 256;
+// From so many rows on the ones that count are put next to each other first: a launch more, and a copy of the rows.
+constexpr int64_t kGatherRows = 1024;
 
 // The products of each type: the scores (vocabulary x rows), dh (D x rows) and dw (D x vocabulary).
 struct Bf16 {
@@ -469,7 +536,7 @@ struct F32 {
 
 struct Plan {
     int64_t N, V, D, Dp, Np, Vp, width;
-    bool direct_h, direct_w;
+    bool direct_h, direct_w, gather;
     int planes, tiles_p, tiles_q;           // of the scores
     int s_h, s_w;                            // splits of the two gradients' products
 };
@@ -511,7 +578,8 @@ Plan plan_of(const mb_linear_ce* a) {
     auto direct = [&](const void* x, int64_t ld) {
         return p.planes == 1 && p.D % C::Score::kStep == 0 && ((uintptr_t)x & 15) == 0 && ld % 8 == 0;
     };
-    p.direct_h = direct(a->hidden, a->hidden_ld), p.direct_w = direct(a->weight, a->weight_ld);
+    p.gather = p.N >= kGatherRows;
+    p.direct_h = !p.gather && direct(a->hidden, a->hidden_ld), p.direct_w = direct(a->weight, a->weight_ld);
     p.tiles_p = (int)((p.V + C::Score::TP - 1) / C::Score::TP), p.tiles_q = (int)((p.N + C::Score::TQ - 1) / C::Score::TQ);
     p.width = std::min<int64_t>(pad(p.V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np * 2 * p.planes) / 256 * 256));
     choose_splits(tiles_of<typename C::GradH>(p.D, p.N), std::min(p.width, p.Vp), tiles_of<typename C::GradW>(p.D, std::min(p.width, p.V)), p.Np,
@@ -520,6 +588,7 @@ Plan plan_of(const mb_linear_ce* a) {
 }
 
 struct Buffers {
+    int *rows, *pos, *m;
     float *largest_h, *largest_w, *largest_g, *scales;   // scales: h, w, g h
     void *h, *w;                 // copies for the scores (planes, or padded bf16)
     float2* part;
@@ -535,6 +604,7 @@ Buffers buffers_of(const Plan& p, bool backward, void* base) {
     Buffers b = {};
     b.largest_h = c.take<float>(kMaxBlocks), b.largest_w = c.take<float>(kMaxBlocks), b.largest_g = c.take<float>(kMaxBlocks);
     b.scales = c.take<float>(4);
+    if (p.gather) b.rows = c.take<int>(p.N), b.pos = c.take<int>(p.N), b.m = c.take<int>(1);
     if (!p.direct_h) b.h = c.take<_Float16>(p.planes * p.Np * p.Dp);
     if (!p.direct_w) b.w = c.take<_Float16>(p.planes * p.Vp * p.Dp);
     if (!backward) {
@@ -554,41 +624,48 @@ Buffers buffers_of(const Plan& p, bool backward, void* base) {
 
 unsigned blocks_for(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + kThreads - 1) / kThreads, 4096)); }
 
-template <typename T, bool G>
-int largest(const Matrix& x, const RowGrad& g, float* part, hipStream_t st) {
-    const int n = (int)std::min<int64_t>(blocks_for((int64_t)x.rows * ((x.D + 7) / 8)), kMaxBlocks);
-    hipLaunchKernelGGL((ce_largest_kernel<T, G>), dim3(n), dim3(kThreads), 0, st, x, g, part);
-    return n;
+Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t D, int size, float* largest, float* scale, void* out, int64_t rows_pad, int64_t Dp) {
+    Matrix x = {};
+    x.p = p, x.ld = ld, x.rows = (int)rows, x.D = (int)D, x.vec = ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0;
+    x.largest = largest, x.scale = scale, x.out = out, x.rows_pad = (int)rows_pad, x.Dp = (int)Dp;
+    x.blocks = (int)std::min<int64_t>(blocks_for(rows * ((D + 7) / 8)), kMaxBlocks);
+    return x;
 }
-template <typename T, typename O, int PL, bool G>
-void planes(const Matrix& x, const RowGrad& g, const float* part, int parts, float* scale, O* out, int64_t rows_pad, int64_t Dp, hipStream_t st) {
-    hipLaunchKernelGGL((ce_planes_kernel<T, O, PL, G>), dim3(blocks_for(rows_pad * Dp / 8)), dim3(kThreads), 0, st, x, g, part, parts,
-                       scale, out, (int)rows_pad, (int)Dp);
+// Copies of the pair's matrices that have an `out`; scaled ones after a launch that looks for their largest values.
+template <typename T, typename O, int PL>
+void copies(Pair a, hipStream_t st) {
+    if (!a.x.out) std::swap(a.x, a.y);
+    if (!a.x.out) return;
+    if (!a.y.out) a.y.blocks = 0;
+    if (a.x.largest) hipLaunchKernelGGL((ce_largest_kernel<T>), dim3(a.x.blocks + a.y.blocks), dim3(kThreads), 0, st, a);
+    const unsigned x_blocks = blocks_for((int64_t)a.x.rows_pad * a.x.Dp / 8), y_blocks = a.y.out ? blocks_for((int64_t)a.y.rows_pad * a.y.Dp / 8) : 0;
+    hipLaunchKernelGGL((ce_planes_kernel<T, O, PL>), dim3(x_blocks + y_blocks), dim3(kThreads), 0, st, a, (int)x_blocks);
 }
 
-Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t D, int size) {
-    const bool vec = ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0;
-    return {p, ld, (int)rows, (int)D, vec};
-}
-
-// The operands of the scores: the user's own, or copies of them.
+// The rows' places and the operands of the scores: the user's own, or copies of them.
 template <typename T>
 void score_sides(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs& s, hipStream_t st) {
-    const Matrix h = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T)), w = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T));
     s.t = {a->target, (int)a->target_bytes, a->ignore_index, a->V};
-    const RowGrad none = {}, counts = {s.t, nullptr, nullptr, 0};
+    s.r = {b.rows, b.pos, b.m, (int)p.N};
+    if (p.gather) {
+        const int each = (int)pad((p.N + kMaxBlocks - 1) / kMaxBlocks, kThreads);
+        hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((p.N + each - 1) / each)), dim3(kThreads), 0, st, s.t, (int)p.N, each, b.rows, b.pos, b.m);
+    }
+    const bool f32 = sizeof(T) == 4;
+    Pair x = {};
+    x.x = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T), f32 ? b.largest_h : nullptr, b.scales, b.h, p.Np, p.Dp);
+    x.y = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T), f32 ? b.largest_w : nullptr, b.scales + 1, b.w, p.Vp, p.Dp);
+    x.x.gathered = p.gather, x.x.graded = f32;     // (without dloss: an ignored row's values are not looked at)
+    x.g.t = s.t, x.r = s.r;
     if constexpr (sizeof(T) == 4) {
-        const int nh = largest<T, true>(h, counts, b.largest_h, st), nw = largest<T, false>(w, none, b.largest_w, st);
-        planes<T, _Float16, 2, true>(h, counts, b.largest_h, nh, b.scales, (_Float16*)b.h, p.Np, p.Dp, st);
-        planes<T, _Float16, 2, false>(w, none, b.largest_w, nw, b.scales + 1, (_Float16*)b.w, p.Vp, p.Dp, st);
+        copies<T, _Float16, 2>(x, st);
         s.scale_h = b.scales, s.scale_w = b.scales + 1;
     } else {
-        if (!p.direct_h) planes<T, __bf16, 1, false>(h, none, nullptr, 0, nullptr, (__bf16*)b.h, p.Np, p.Dp, st);
-        if (!p.direct_w) planes<T, __bf16, 1, false>(w, none, nullptr, 0, nullptr, (__bf16*)b.w, p.Vp, p.Dp, st);
+        copies<T, __bf16, 1>(x, st);
     }
     s.h = {p.direct_h ? a->hidden : b.h, p.Np * p.Dp * 2, p.direct_h ? a->hidden_ld : p.Dp, (int)p.N};
     s.w = {p.direct_w ? a->weight : b.w, p.Vp * p.Dp * 2, p.direct_w ? a->weight_ld : p.Dp, (int)p.V};
-    s.V = (int)p.V, s.N = (int)p.N, s.Dp = (int)(p.direct_h && p.direct_w ? p.D : p.Dp), s.tiles_p = p.tiles_p, s.tiles_q = p.tiles_q;
+    s.V = (int)p.V, s.N = (int)p.N, s.Dp = (int)(p.direct_h && p.direct_w ? p.D : p.Dp), s.tiles_p = p.tiles_p;
 }
 
 template <typename K, typename A>
@@ -599,14 +676,14 @@ int launch(const char* what, K kernel, int threads, int lds, Told& told, unsigne
 }
 
 template <typename P>
-int stats(const ScoreArgs& s, hipStream_t st) {
+int stats(const ScoreArgs& s, int tiles_q, hipStream_t st) {
     static Told told;
-    return launch("mb_linear_ce_fwd", ce_stats_kernel<P>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
+    return launch("mb_linear_ce_fwd", ce_stats_kernel<P>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * tiles_q), st, s);
 }
 template <typename P, int PL>
-int piece_of_u(const ScoreArgs& s, hipStream_t st) {
+int piece_of_u(const ScoreArgs& s, int tiles_q, hipStream_t st) {
     static Told told;
-    return launch("mb_linear_ce_bwd", ce_u_kernel<P, PL>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * s.tiles_q), st, s);
+    return launch("mb_linear_ce_bwd", ce_u_kernel<P, PL>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * tiles_q), st, s);
 }
 template <typename P>
 void tiles_for(PartArgs& a) {
@@ -653,9 +730,9 @@ int forward(const mb_linear_ce* a, hipStream_t st) {
     ScoreArgs s = {};
     score_sides<T>(a, p, b, s, st);
     s.part = b.part, s.target_score = b.target_score;
-    if (const int rc = stats<typename C::Score>(s, st)) return rc;
+    if (const int rc = stats<typename C::Score>(s, p.tiles_q, st)) return rc;
     const int blocks = (int)((p.N + kRowsPerBlock - 1) / kRowsPerBlock);
-    const JoinArgs j = {b.part, b.target_score, s.t, (int)p.N, p.tiles_p, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
+    const JoinArgs j = {b.part, b.target_score, s.t, s.r, (int)p.N, p.tiles_p, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
     hipLaunchKernelGGL(ce_join_kernel, dim3(blocks), dim3(kThreads), 0, st, j);
     if (a->reduction)
         hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(kThreads), 0, st, b.sums, blocks, (int)a->reduction, a->loss, a->count);
@@ -673,45 +750,43 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
     if (!wants_h && !wants_w) return MB_OK;
     ScoreArgs s = {};
     score_sides<T>(a, p, b, s, st);
-    s.lse = a->lse, s.u = b.u, s.width = p.width, s.n_pad = (int)p.Np;
+    s.lse = a->lse, s.u = b.u, s.width = p.width, s.plane = p.Np * p.width;
     const RowGrad g = {s.t, a->dloss, a->count, (int)a->reduction};
-    const Matrix h = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T)), w = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T));
-    if constexpr (sizeof(T) == 2)     // fp32: the scores' planes
-        if (wants_h) {
-            const int n = largest<T, false>(w, g, b.largest_w, st);
-            planes<T, _Float16, 1, false>(w, g, b.largest_w, n, b.scales + 1, b.w16, p.Vp, p.Dp, st);
-        }
-    if (wants_w) {
-        const int n = largest<T, true>(h, g, b.largest_g, st);
-        planes<T, _Float16, PL, true>(h, g, b.largest_g, n, b.scales + 2, b.h16, p.Np, p.Dp, st);
-    }
-    const int64_t plane_u = p.Np * p.width * 2, tiles_q = p.tiles_q;
+    // g h for dw, and for dh w in fp16 (fp32: the scores' planes)
+    Pair x = {};
+    x.x = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T), b.largest_g, b.scales + 2, wants_w ? b.h16 : nullptr, p.Np, p.Dp);
+    x.y = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T), b.largest_w, b.scales + 1, wants_h && PL == 1 ? b.w16 : nullptr, p.Vp, p.Dp);
+    x.x.gathered = p.gather, x.x.graded = 1;
+    x.g = g, x.r = s.r;
+    copies<T, _Float16, PL>(x, st);
     for (int64_t v0 = 0; v0 < p.V; v0 += p.width) {
         const int64_t v1 = std::min(p.V, v0 + p.width), kv = pad(v1 - v0, kPad);
         s.v0 = (int)v0, s.v1 = (int)v1;
-        s.tiles_p = (int)((v1 - v0 + C::Score::TP - 1) / C::Score::TP), s.tiles_q = (int)tiles_q;
-        if (const int rc = piece_of_u<typename C::Score, PL>(s, st)) return rc;
+        s.tiles_p = (int)((v1 - v0 + C::Score::TP - 1) / C::Score::TP);
+        if (const int rc = piece_of_u<typename C::Score, PL>(s, p.tiles_q, st)) return rc;
         PartArgs ph = {}, pw = {};
+        SumArgs sh = {}, sw = {};
+        ph.r = pw.r = s.r, pw.k_rows = 1;
         if (wants_h) {
             ph.p = {b.w16 + v0 * p.Dp, p.Vp * p.Dp * 2, p.Dp, (int)p.D};
-            ph.q = {b.u, plane_u, p.width, (int)p.N};
+            ph.q = {b.u, s.plane * 2, p.width, (int)p.N};
             ph.splits = (int)std::min<int64_t>(p.s_h, kv / kPad), ph.k1 = (int)kv, ph.out = b.part_h, ph.ld = p.Dp, ph.add = v0 > 0;
             tiles_for<typename C::GradH>(ph);
+            if (v1 == p.V)
+                sh = {b.part_h, p.s_h, (int)p.N, (int)p.D, (int)p.Dp, 1, (int)blocks_for(p.N * p.Dp / 4), b.scales + 1, a->dhidden};
         }
         if (wants_w) {
             pw.p = {b.h16, p.Np * p.Dp * 2, p.Dp, (int)p.D};
-            pw.q = {b.u, plane_u, p.width, (int)(v1 - v0)};
+            pw.q = {b.u, s.plane * 2, p.width, (int)(v1 - v0)};
             pw.splits = p.s_w, pw.k1 = (int)p.Np, pw.out = b.part_w, pw.ld = p.Dp;
             tiles_for<typename C::GradW>(pw);
+            sw = {b.part_w, p.s_w, (int)(v1 - v0), (int)p.D, (int)p.Dp, 0, (int)blocks_for((v1 - v0) * p.Dp / 4), b.scales + 2,
+                  (T*)a->dweight + v0 * p.D};
         }
         if (const int rc = parts<C>(ph, pw, st)) return rc;
-        if (wants_w)
-            hipLaunchKernelGGL((ce_sum_kernel<T, false>), dim3(blocks_for((v1 - v0) * p.Dp / 4)), dim3(kThreads), 0, st, b.part_w, p.s_w,
-                               (int)(v1 - v0), (int)p.D, (int)p.Dp, b.scales + 2, g, (T*)a->dweight + v0 * p.D);
+        if (sh.blocks + sw.blocks)
+            hipLaunchKernelGGL((ce_sum_kernel<T>), dim3(sh.blocks + sw.blocks), dim3(kThreads), 0, st, sh, sw, g, s.r);
     }
-    if (wants_h)
-        hipLaunchKernelGGL((ce_sum_kernel<T, true>), dim3(blocks_for(p.N * p.Dp / 4)), dim3(kThreads), 0, st, b.part_h, p.s_h, (int)p.N,
-                           (int)p.D, (int)p.Dp, b.scales + 1, g, (T*)a->dhidden);
     return check_launch("mb_linear_ce_bwd");
 }
 

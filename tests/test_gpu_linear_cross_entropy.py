@@ -150,6 +150,29 @@ def test_rows_that_do_not_count():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_many_rows_of_which_few_or_none_count(t):
+    """From 1024 rows on those that count are put next to each other."""
+    h, w, target = make(1500, 700, 64, t)
+    at = torch.arange(1500, device="cuda")
+    for keep in (at < 0, at == 1499, at == 0, at % 500 == 3, at < 1024, at >= 1200, at % 2 == 1, at >= 0):
+        left = torch.where(keep, target, IGN)
+        h2 = torch.where(keep[:, None], h, math.nan)
+        for reduction in ("sum", "none", "mean"):
+            dloss = 0.5 + torch.rand((1500,) if reduction == "none" else (), device="cuda")
+            got, want = call(h2, w, left, reduction, dloss), definition(h, w, left, reduction, dloss)
+            if reduction == "mean" and not keep.any():
+                assert got[0].isnan() and not got[1].any() and not got[2].any()
+                continue
+            check(got, want, h, w, (reduction, int(keep.sum())))
+            assert not got[1][~keep].any()
+    wrong = target.clone()
+    wrong[::3], wrong[1000] = IGN, 700
+    loss, dh, dw = call(h, w, wrong, "none")
+    row = at == 1000
+    assert torch.equal(loss.isnan(), row) and torch.equal(dh.isnan().all(1), row) and not dh[~row].isnan().any() and dw.isnan().all()
+
+
 def test_targets_outside_the_vocabulary_and_special_values():
     h, w, target = make(40, 90, 32, torch.float32)
     for bad in (90, -1, 2**40):
@@ -254,8 +277,10 @@ def test_under_autocast():
         linear_cross_entropy(h, w, target)
 
 
-def test_captured_replayed_and_on_another_stream():
-    h, w, target = make(200, 3000, 64, torch.bfloat16)
+@pytest.mark.parametrize("N", [200, 1300])
+def test_captured_replayed_and_on_another_stream(N):
+    h, w, target = make(N, 3000, 64, torch.bfloat16)
+    target[::7] = IGN
     h.requires_grad_(), w.requires_grad_()
     from mathbrain.linear_cross_entropy import linear_cross_entropy
 
@@ -276,7 +301,7 @@ def test_captured_replayed_and_on_another_stream():
     for i in range(3):
         with torch.no_grad():
             h.mul_(1.1)
-            target.add_(i).remainder_(3000)
+            target.copy_(torch.where(target == IGN, (i * 100 + 5) % 3000, torch.where(target % 5 == i, IGN, target)))
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
