@@ -512,7 +512,8 @@ struct Carve {
     }
 };
 
-// U's bytes in a piece: pieces are large enough to fill the card and small beside the scores.
+// U's bytes in a piece (of 256 words at least): few launches and few passes over dh's sums against what stays in the
+// caches and the memory that is wanted.  56 x 512 rows, 50257 words: 256 MiB 7.14 ms, 512 6.88, 1024 6.93, 2048 7.05.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 constexpr int kCus = 256;
 // From so many rows on the ones that count are put next to each other first: a launch more, and a copy of the rows.
@@ -714,6 +715,15 @@ int check(const char* what, const mb_linear_ce* a) {
     return MB_OK;
 }
 
+// Workgroups of a launch, whose threads are counted in 32 bits.
+int fits(const char* what, const mb_linear_ce* a, const Plan& p, int64_t tiles_d) {
+    const int64_t most = 0x7fffff;
+    if ((int64_t)p.tiles_p * p.tiles_q > most || tiles_d * (p.tiles_q * p.s_h + (p.width / 128 + 1) * p.s_w) > most)
+        return fail(MB_ERR_UNSUPPORTED, "%s: %lld rows of %lld on %lld words are too many for a launch", what, (long long)a->N, (long long)a->D,
+                    (long long)a->V);
+    return MB_OK;
+}
+
 int enough(const char* what, const mb_linear_ce* a, int64_t need) {
     MB_REQUIRE(((uintptr_t)a->workspace & 255) == 0, "%s: the workspace has to begin at a multiple of 256 bytes", what);
     if (!a->workspace || a->workspace_bytes < need)
@@ -726,6 +736,7 @@ int forward(const mb_linear_ce* a, hipStream_t st) {
     typedef typename C::T T;
     const Plan p = plan_of<C>(a);
     const Buffers b = buffers_of(p, false, a->workspace);
+    if (const int rc = fits("mb_linear_ce_fwd", a, p, 0)) return rc;
     if (const int rc = enough("mb_linear_ce_fwd", a, b.bytes)) return rc;
     ScoreArgs s = {};
     score_sides<T>(a, p, b, s, st);
@@ -745,6 +756,7 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
     constexpr int PL = C::kPlanes;
     const Plan p = plan_of<C>(a);
     const Buffers b = buffers_of(p, true, a->workspace);
+    if (const int rc = fits("mb_linear_ce_bwd", a, p, (p.D + C::GradH::TP - 1) / C::GradH::TP)) return rc;
     if (const int rc = enough("mb_linear_ce_bwd", a, b.bytes)) return rc;
     const bool wants_h = a->dhidden, wants_w = a->dweight;
     if (!wants_h && !wants_w) return MB_OK;

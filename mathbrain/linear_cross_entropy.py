@@ -3,12 +3,13 @@ mb_linear_ce_fwd / mb_linear_ce_bwd.
 
 ``linear_cross_entropy(hidden, weight, target)`` is F.cross_entropy(F.linear(hidden, weight), target)
 with gradients for hidden and weight, for the tied output matrix over a vocabulary of any size: the
-scores exist a tile at a time, and in the backward pass a piece of the vocabulary at a time (512 MiB
-at most), where F.cross_entropy keeps [rows, vocabulary] several times.  fp32 and bf16; scores,
+scores exist a tile at a time, and in the backward pass a piece of the vocabulary at a time (about
+512 MiB), where F.cross_entropy keeps [rows, vocabulary] several times.  fp32 and bf16; scores,
 maxima, sums and both gradients' sums are fp32 or more, the scores are never rounded to bf16, and the
 loss is fp32.  Sums have a fixed order.  CPU tensors raise NotImplementedError.  Both directions
 are registered as torch ops (mathbrain::linear_ce_fwd / linear_ce_bwd) for tracing.
 """
+import functools
 import struct
 
 import torch
@@ -18,6 +19,7 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.MB_DTYPE_F32, torch.bfloat16: _lib.MB_DTYPE_BF16}
 REDUCTIONS = ("none", "mean", "sum")
 _ARGS = struct.Struct("2P2qP2q4qq3PP2PPq")   # mb_linear_ce (include/mathbrain_hip.h)
+_ANY = 1 << 20                               # an aligned address that nothing is done with
 
 
 def _rows(x):
@@ -27,58 +29,61 @@ def _rows(x):
     return x.contiguous()
 
 
-def _pack(hidden, weight, target, ignore_index, reduction, loss, lse, count, dloss=None, dh=None, dw=None, ws=None):
+@functools.lru_cache(maxsize=256)
+def _workspace(backward, h_at, w_at, h_ld, w_ld, N, V, D, dtype):
+    """The library's workspace for these sizes, row distances and addresses modulo 16."""
+    nbytes = _lib.lib().mb_linear_ce_workspace(
+        _ARGS.pack(_ANY + h_at, _ANY + w_at, h_ld, w_ld, _ANY, 8, 0, N, V, D, dtype, 0, _ANY, _ANY, _ANY, 0, 0, 0, 0, 0), backward)
+    if nbytes < 0:
+        raise _lib.HipKernelError(_lib.lib().mb_last_error().decode(errors="replace"))
+    return nbytes
+
+
+def _call(name, backward, hidden, weight, target, ignore_index, reduction, loss, stats, dloss=None, dh=None, dw=None):
     N, D = hidden.shape
     V = weight.shape[0]
-    at = [0 if t is None else t.data_ptr() for t in (loss, lse, count, dloss, dh, dw, ws)]
-    return _ARGS.pack(hidden.data_ptr(), weight.data_ptr(), hidden.stride(0) if N > 1 else D, weight.stride(0) if V > 1 else D,
-                      target.data_ptr(), target.element_size(), ignore_index, N, V, D, _DTYPES[hidden.dtype], reduction, *at,
-                      0 if ws is None else ws.numel())
-
-
-def _call(name, backward, hidden, *args, **kwargs):
-    lib = _lib.lib()
-    nbytes = lib.mb_linear_ce_workspace(_pack(hidden, *args, **kwargs), backward)
-    if nbytes < 0:
-        raise _lib.HipKernelError(lib.mb_last_error().decode(errors="replace"))
+    h, w, t = hidden.data_ptr(), weight.data_ptr(), _DTYPES[hidden.dtype]
+    h_ld, w_ld = hidden.stride(0) if N > 1 else D, weight.stride(0) if V > 1 else D
+    nbytes = _workspace(backward, h % 16, w % 16, h_ld, w_ld, N, V, D, t)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=hidden.device)
-    _lib.call_on(hidden.device, name, _pack(hidden, *args, **kwargs, ws=ws))
+    lse = stats.data_ptr()
+    _lib.call_on(hidden.device, name,
+                 _ARGS.pack(h, w, h_ld, w_ld, target.data_ptr(), target.element_size(), ignore_index, N, V, D, t, reduction,
+                            0 if loss is None else loss.data_ptr(), lse, lse + 8 * N, 0 if dloss is None else dloss.data_ptr(),
+                            0 if dh is None else dh.data_ptr(), 0 if dw is None else dw.data_ptr(), ws.data_ptr(), nbytes))
 
 
 def _fwd_fake(hidden, weight, target, ignore_index, reduction):
     N = hidden.shape[0]
     return (hidden.new_empty((N,) if reduction == 0 else (), dtype=torch.float32),
-            hidden.new_empty((2, N), dtype=torch.float32), hidden.new_empty((1,), dtype=torch.float32))
+            hidden.new_empty((2 * N + 1,), dtype=torch.float32))
 
 
 @_lib.traced_op("linear_ce_fwd", _fwd_fake)
 def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int,
-                  reduction: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(loss, the rows' maxima and logarithms of sums [2, N], the number of rows that count [1])."""
-    loss, lse, count = (torch.empty_like(t, device=hidden.device) for t in _fwd_fake(hidden, weight, target, ignore_index, reduction))
+                  reduction: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss, what the backward wants of the rows: their maxima, logarithms of sums and how many count [2 N + 1])."""
+    loss, stats = _fwd_fake(hidden, weight, target, ignore_index, reduction)
     if hidden.shape[0] == 0:
-        return loss.fill_(float("nan") if reduction == 1 else 0.0), lse, count.zero_()
-    hidden, weight = _rows(hidden), _rows(weight)
-    _call("mb_linear_ce_fwd", 0, hidden, weight, target, ignore_index, reduction, loss, lse, count)
-    return loss, lse, count
+        return loss.fill_(float("nan") if reduction == 1 else 0.0), stats.zero_()
+    _call("mb_linear_ce_fwd", 0, _rows(hidden), _rows(weight), target, ignore_index, reduction, loss, stats)
+    return loss, stats
 
 
-def _bwd_fake(hidden, weight, target, lse, count, dloss, ignore_index, reduction, wants_hidden, wants_weight):
+def _bwd_fake(hidden, weight, target, stats, dloss, ignore_index, reduction, wants_hidden, wants_weight):
     return (hidden.new_empty(hidden.shape if wants_hidden else (0,)),
             weight.new_empty(weight.shape if wants_weight else (0,)))
 
 
 @_lib.traced_op("linear_ce_bwd", _bwd_fake)
-def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, count: torch.Tensor,
-                  dloss: torch.Tensor, ignore_index: int, reduction: int, wants_hidden: bool,
-                  wants_weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
+def linear_ce_bwd(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, stats: torch.Tensor, dloss: torch.Tensor,
+                  ignore_index: int, reduction: int, wants_hidden: bool, wants_weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """(dhidden, dweight), contiguous, of linear_ce_fwd's inputs and results; an empty tensor for one that is not wanted."""
-    dh, dw = _bwd_fake(hidden, weight, target, lse, count, dloss, ignore_index, reduction, wants_hidden, wants_weight)
+    dh, dw = _bwd_fake(hidden, weight, target, stats, dloss, ignore_index, reduction, wants_hidden, wants_weight)
     if hidden.shape[0] == 0:
         return dh, dw.zero_()
     dloss = dloss.to(torch.float32).contiguous()
-    hidden, weight = _rows(hidden), _rows(weight)
-    _call("mb_linear_ce_bwd", 1, hidden, weight, target, ignore_index, reduction, None, lse, count, dloss,
+    _call("mb_linear_ce_bwd", 1, _rows(hidden), _rows(weight), target, ignore_index, reduction, None, stats, dloss,
           dh if wants_hidden else None, dw if wants_weight else None)
     return dh, dw
 
@@ -88,17 +93,17 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        loss, lse, count = linear_ce_fwd(hidden, weight, target, ignore_index, reduction)
-        ctx.save_for_backward(hidden, weight, target, lse, count)
+        loss, stats = linear_ce_fwd(hidden, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, target, stats)
         ctx.rest = (ignore_index, reduction)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        hidden, weight, target, lse, count = ctx.saved_tensors
+        hidden, weight, target, stats = ctx.saved_tensors
         wants_h, wants_w = ctx.needs_input_grad[:2]
-        dh, dw = linear_ce_bwd(hidden, weight, target, lse, count, dloss, *ctx.rest, wants_h, wants_w)
+        dh, dw = linear_ce_bwd(hidden, weight, target, stats, dloss, *ctx.rest, wants_h, wants_w)
         return dh if wants_h else None, dw if wants_w else None, None, None, None
 
 
