@@ -49,7 +49,7 @@ struct Rows {
     __device__ int at(int c) const { return rows ? rows[c] : c; }
     __device__ int of(int64_t n) const { return pos ? pos[n] : (int)n; }
 };
-// The gradient of each row's loss; without dloss 1, and 0 for the ignored rows.
+// The gradient of each row's loss.
 struct RowGrad {
     Targets t;
     const float* dloss;      // [N] (reduction 0) or one
@@ -57,7 +57,6 @@ struct RowGrad {
     int reduction;
     __device__ float at(int64_t n) const {
         if (t.at(n) == -1) return 0.f;
-        if (!dloss) return 1.f;
         return reduction == 0 ? dloss[n] : reduction == 1 ? dloss[0] / count[0] : dloss[0];
     }
 };
@@ -111,32 +110,39 @@ struct Matrix {
     const void* p;
     int64_t ld;
     int rows, D, vec;
-    int graded;                  // times each row's g; an ignored row counts for nothing, whatever it holds
+    int graded;                  // 1: times each row's g; 1 or 2: an ignored row counts for nothing, whatever it holds
     float* largest;              // the largest magnitudes of the workgroups' parts; copies without: not scaled
-    int blocks;
+    int blocks, copy_blocks;
     float* scale;
     void* out;                   // planes [rows_pad, Dp]
     int rows_pad, Dp, gathered;  // gathered: rows in their places of Rows
 };
-// Two matrices a launch; the second may have no blocks.
-struct Pair {
-    Matrix x, y;
+// Up to three matrices a launch, each with workgroups of its own.
+constexpr int kMatrices = 3;
+struct Set {
+    Matrix x[kMatrices];
+    int n, first[kMatrices];     // their first workgroups
     RowGrad g;
     Rows r;
+    __device__ const Matrix& mine(int& block) const {
+        int i = 0;
+        while (i + 1 < n && (int)blockIdx.x >= first[i + 1]) ++i;
+        block = (int)blockIdx.x - first[i];
+        return x[i];
+    }
 };
 
 // The largest finite magnitude of each workgroup's part of x (graded: of g_n x_n).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Pair a) {
-    const bool first = (int)blockIdx.x < a.x.blocks;
-    const Matrix& x = first ? a.x : a.y;
-    const int block = first ? blockIdx.x : blockIdx.x - a.x.blocks;
+__global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Set a) {
+    int block;
+    const Matrix& x = a.mine(block);
     const int pieces = (x.D + 7) / 8;
     float most = 0.f;
     for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)x.rows * pieces; i += (int64_t)x.blocks * kThreads) {
         const int64_t n = i / pieces;
         const int d = (int)(i - n * pieces) * 8;
-        const float gn = x.graded ? fabsf(a.g.at(n)) : 1.f;
+        const float gn = !x.graded ? 1.f : x.graded == 1 ? fabsf(a.g.at(n)) : a.g.t.at(n) == -1 ? 0.f : 1.f;
         if (gn == 0.f) continue;
         float v[8];
         load8((const T*)x.p + n * x.ld + d, x.vec, x.D - d, v);
@@ -158,10 +164,9 @@ __device__ inline float scale_from(const float* part, int n) {
 
 // x (graded: g_n x_n) as PL planes [rows_pad, Dp] of O, zeros around it, scaled by its largest value, which goes to *scale.
 template <typename T, typename O, int PL>
-__global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Pair a, int x_blocks) {
-    const bool first = (int)blockIdx.x < x_blocks;
-    const Matrix& x = first ? a.x : a.y;
-    const int block = first ? blockIdx.x : blockIdx.x - x_blocks, blocks = first ? x_blocks : gridDim.x - x_blocks;
+__global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Set a) {
+    int block;
+    const Matrix& x = a.mine(block);
     float s = 1.f;
     if (x.largest) {
         s = scale_from(x.largest, x.blocks);
@@ -170,13 +175,13 @@ __global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Pair a, int x
     const int pieces = x.Dp / 8, count = x.gathered ? a.r.count() : x.rows;
     O* out = (O*)x.out;
     typedef O vec8 __attribute__((ext_vector_type(8), aligned(16)));
-    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)x.rows_pad * pieces; i += (int64_t)blocks * kThreads) {
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)x.rows_pad * pieces; i += (int64_t)x.copy_blocks * kThreads) {
         const int64_t n = i / pieces;
         const int d = (int)(i - n * pieces) * 8;
         float v[8] = {};
         if (n < count) {
             const int64_t row = x.gathered ? a.r.at((int)n) : n;
-            const float gn = x.graded ? a.g.at(row) : 1.f;
+            const float gn = !x.graded ? 1.f : x.graded == 1 ? a.g.at(row) : a.g.t.at(row) == -1 ? 0.f : 1.f;
             load8((const T*)x.p + row * x.ld + d, x.vec, x.D - d, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = gn == 0.f ? 0.f : v[e] * gn * s;
@@ -421,10 +426,12 @@ struct PartArgs {
     float* out;                         // [splits][q.n, ld]
     int64_t ld;
     int add;                            // onto what is there
+    const float* scale;                 // set: the result itself, [q.n, p.n] of the tensors' type, to `result`
+    void* result;
     __host__ __device__ int blocks() const { return tiles_p * tiles_q * splits; }
 };
 
-template <typename P>
+template <typename T, typename P>
 __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     const int tiles = a.tiles_p * a.tiles_q;
     const int split = block / tiles, tile = block - split * tiles;
@@ -440,6 +447,28 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     for (int j = 0; j < P::FQ; ++j) {
         const int q = q0 + P::col(j);
         if (q >= end) continue;
+        if (a.scale) {
+            const float f = 1.f / *a.scale / kUScale;
+            T* to = (T*)a.result + (int64_t)q * a.p.n;
+            const bool four = a.p.n % 4 == 0 && ((uintptr_t)a.result & 15) == 0;
+#pragma unroll
+            for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int p = p0 + P::row(i, r);
+                    typedef T four_t __attribute__((ext_vector_type(4)));
+                    const four_t v = {(T)(prod.acc[i][j][r] * f), (T)(prod.acc[i][j][r + 1] * f), (T)(prod.acc[i][j][r + 2] * f),
+                                      (T)(prod.acc[i][j][r + 3] * f)};
+                    if (four && p < a.p.n) {
+                        *reinterpret_cast<four_t*>(to + p) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (p + e < a.p.n) to[p + e] = v[e];
+                    }
+                }
+            continue;
+        }
         float* to = a.out + ((int64_t)split * a.q.n + q) * a.ld;
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
@@ -456,14 +485,14 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
 
 // Both gradients' products with a piece of U in one launch, either without tiles where it is not wanted: the one's
 // workgroups fill what the other's leave of the card's last round.  The longer ones come first.
-template <typename H, typename W>
+template <typename T, typename H, typename W>
 __global__ void __launch_bounds__(H::kThreads, H::kWaves) ce_part_kernel(const PartArgs h, const PartArgs w) {
     static_assert(H::kThreads == W::kThreads && H::kWaves == W::kWaves, "");
     extern __shared__ char smem[];
     const bool h_first = (int64_t)h.k1 * w.splits >= (int64_t)w.k1 * h.splits;
     const int n = h_first ? h.blocks() : w.blocks(), block = blockIdx.x;
-    if ((block < n) == h_first) part_of<H>(h, h_first ? block : block - n, smem);
-    else part_of<W>(w, h_first ? block - n : block, smem);
+    if ((block < n) == h_first) part_of<T, H>(h, h_first ? block : block - n, smem);
+    else part_of<T, W>(w, h_first ? block - n : block, smem);
 }
 
 // out[n, d] = factor (g_n) sum_s part[s][n, d], in the parts' order; graded rows come from their places.
@@ -492,9 +521,15 @@ __global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const
             v = *reinterpret_cast<const f32x4v*>(a.part + from * a.ld + d);
             for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4v*>(a.part + ((int64_t)s * a.rows + from) * a.ld + d);
         }
+        typedef T four_t __attribute__((ext_vector_type(4)));
+        const four_t y = {(T)(v[0] * f * gn), (T)(v[1] * f * gn), (T)(v[2] * f * gn), (T)(v[3] * f * gn)};
+        if (a.D % 4 == 0 && ((uintptr_t)out & 15) == 0) {
+            if (d < a.D) *reinterpret_cast<four_t*>(out + n * a.D + d) = y;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < a.D) out[n * a.D + d + e] = (T)(v[e] * f * gn);
+            for (int e = 0; e < 4; ++e)
+                if (d + e < a.D) out[n * a.D + d + e] = y[e];
+        }
     }
 }
 
@@ -617,7 +652,7 @@ Buffers buffers_of(const Plan& p, bool backward, void* base) {
         b.h16 = c.take<_Float16>(p.planes * p.Np * p.Dp);
         b.u = c.take<_Float16>(p.planes * p.Np * p.width);
         b.part_h = c.take<float>(p.s_h * p.N * p.Dp);
-        b.part_w = c.take<float>(p.s_w * p.width * p.Dp);
+        if (p.s_w > 1) b.part_w = c.take<float>(p.s_w * p.width * p.Dp);
     }
     b.bytes = c.used;
     return b;
@@ -632,37 +667,56 @@ Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t D, int size, floa
     x.blocks = (int)std::min<int64_t>(blocks_for(rows * ((D + 7) / 8)), kMaxBlocks);
     return x;
 }
-// Copies of the pair's matrices that have an `out`; scaled ones after a launch that looks for their largest values.
+// Copies of the set's matrices; scaled ones after a launch that looks for their largest values.
 template <typename T, typename O, int PL>
-void copies(Pair a, hipStream_t st) {
-    if (!a.x.out) std::swap(a.x, a.y);
-    if (!a.x.out) return;
-    if (!a.y.out) a.y.blocks = 0;
-    if (a.x.largest) hipLaunchKernelGGL((ce_largest_kernel<T>), dim3(a.x.blocks + a.y.blocks), dim3(kThreads), 0, st, a);
-    const unsigned x_blocks = blocks_for((int64_t)a.x.rows_pad * a.x.Dp / 8), y_blocks = a.y.out ? blocks_for((int64_t)a.y.rows_pad * a.y.Dp / 8) : 0;
-    hipLaunchKernelGGL((ce_planes_kernel<T, O, PL>), dim3(x_blocks + y_blocks), dim3(kThreads), 0, st, a, (int)x_blocks);
+void copies(Set a, hipStream_t st) {
+    if (a.n == 0) return;
+    int total = 0;
+    if (a.x[0].largest) {
+        for (int i = 0; i < a.n; ++i) a.first[i] = total, total += a.x[i].blocks;
+        hipLaunchKernelGGL((ce_largest_kernel<T>), dim3(total), dim3(kThreads), 0, st, a);
+    }
+    total = 0;
+    for (int i = 0; i < a.n; ++i) {
+        a.x[i].copy_blocks = (int)blocks_for((int64_t)a.x[i].rows_pad * a.x[i].Dp / 8);
+        a.first[i] = total, total += a.x[i].copy_blocks;
+    }
+    hipLaunchKernelGGL((ce_planes_kernel<T, O, PL>), dim3(total), dim3(kThreads), 0, st, a);
 }
 
-// The rows' places and the operands of the scores: the user's own, or copies of them.
-template <typename T>
-void score_sides(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs& s, hipStream_t st) {
-    s.t = {a->target, (int)a->target_bytes, a->ignore_index, a->V};
+// The rows' places and the operands of the scores: the user's own, or copies of them; and what the gradients want copied: g h
+// for dw, and for dh w in fp16 (fp32: the scores' planes).
+template <typename C>
+void operands(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs& s, const RowGrad& g, bool wants_h, bool wants_w, hipStream_t st) {
+    typedef typename C::T T;
+    s.t = g.t;
     s.r = {b.rows, b.pos, b.m, (int)p.N};
     if (p.gather) {
         const int each = (int)pad((p.N + kMaxBlocks - 1) / kMaxBlocks, kThreads);
         hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((p.N + each - 1) / each)), dim3(kThreads), 0, st, s.t, (int)p.N, each, b.rows, b.pos, b.m);
     }
-    const bool f32 = sizeof(T) == 4;
-    Pair x = {};
-    x.x = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T), f32 ? b.largest_h : nullptr, b.scales, b.h, p.Np, p.Dp);
-    x.y = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T), f32 ? b.largest_w : nullptr, b.scales + 1, b.w, p.Vp, p.Dp);
-    x.x.gathered = p.gather, x.x.graded = f32;     // (without dloss: an ignored row's values are not looked at)
-    x.g.t = s.t, x.r = s.r;
-    if constexpr (sizeof(T) == 4) {
-        copies<T, _Float16, 2>(x, st);
+    constexpr bool f32 = sizeof(T) == 4;
+    Set scores = {}, grads = {};
+    scores.g = grads.g = g, scores.r = grads.r = s.r;
+    auto hidden = [&](float* largest, float* scale, void* out, int graded) {
+        Matrix x = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T), largest, scale, out, p.Np, p.Dp);
+        x.gathered = p.gather, x.graded = graded;
+        return x;
+    };
+    auto weight = [&](float* largest, float* scale, void* out) {
+        return matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T), largest, scale, out, p.Vp, p.Dp);
+    };
+    if (!p.direct_h) scores.x[scores.n++] = hidden(f32 ? b.largest_h : nullptr, b.scales, b.h, f32 ? 2 : 0);
+    if (!p.direct_w) scores.x[scores.n++] = weight(f32 ? b.largest_w : nullptr, b.scales + 1, b.w);
+    Set& more = f32 ? scores : grads;
+    if (wants_w) more.x[more.n++] = hidden(b.largest_g, b.scales + 2, b.h16, 1);
+    if (wants_h && !f32) more.x[more.n++] = weight(b.largest_w, b.scales + 1, b.w16);
+    if constexpr (f32) {
+        copies<T, _Float16, 2>(scores, st);
         s.scale_h = b.scales, s.scale_w = b.scales + 1;
     } else {
-        copies<T, __bf16, 1>(x, st);
+        copies<T, __bf16, 1>(scores, st);
+        copies<T, _Float16, 1>(grads, st);
     }
     s.h = {p.direct_h ? a->hidden : b.h, p.Np * p.Dp * 2, p.direct_h ? a->hidden_ld : p.Dp, (int)p.N};
     s.w = {p.direct_w ? a->weight : b.w, p.Vp * p.Dp * 2, p.direct_w ? a->weight_ld : p.Dp, (int)p.V};
@@ -692,12 +746,13 @@ void tiles_for(PartArgs& a) {
 }
 template <typename C>
 int parts(const PartArgs& h, const PartArgs& w, hipStream_t st) {
+    typedef typename C::T T;
     typedef typename C::GradH H;
     typedef typename C::GradW W;
     static Told told;
     constexpr int lds = std::max(H::kLds, W::kLds);
-    if (const int rc = allow_lds("mb_linear_ce_bwd", (const void*)ce_part_kernel<H, W>, lds, told)) return rc;
-    hipLaunchKernelGGL((ce_part_kernel<H, W>), dim3((unsigned)(h.blocks() + w.blocks())), dim3(H::kThreads), lds, st, h, w);
+    if (const int rc = allow_lds("mb_linear_ce_bwd", (const void*)ce_part_kernel<T, H, W>, lds, told)) return rc;
+    hipLaunchKernelGGL((ce_part_kernel<T, H, W>), dim3((unsigned)(h.blocks() + w.blocks())), dim3(H::kThreads), lds, st, h, w);
     return MB_OK;
 }
 
@@ -733,13 +788,13 @@ int enough(const char* what, const mb_linear_ce* a, int64_t need) {
 
 template <typename C>
 int forward(const mb_linear_ce* a, hipStream_t st) {
-    typedef typename C::T T;
     const Plan p = plan_of<C>(a);
     const Buffers b = buffers_of(p, false, a->workspace);
     if (const int rc = fits("mb_linear_ce_fwd", a, p, 0)) return rc;
     if (const int rc = enough("mb_linear_ce_fwd", a, b.bytes)) return rc;
     ScoreArgs s = {};
-    score_sides<T>(a, p, b, s, st);
+    const RowGrad g = {{a->target, (int)a->target_bytes, a->ignore_index, a->V}, nullptr, nullptr, 0};
+    operands<C>(a, p, b, s, g, false, false, st);
     s.part = b.part, s.target_score = b.target_score;
     if (const int rc = stats<typename C::Score>(s, p.tiles_q, st)) return rc;
     const int blocks = (int)((p.N + kRowsPerBlock - 1) / kRowsPerBlock);
@@ -761,16 +816,9 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
     const bool wants_h = a->dhidden, wants_w = a->dweight;
     if (!wants_h && !wants_w) return MB_OK;
     ScoreArgs s = {};
-    score_sides<T>(a, p, b, s, st);
+    const RowGrad g = {{a->target, (int)a->target_bytes, a->ignore_index, a->V}, a->dloss, a->count, (int)a->reduction};
+    operands<C>(a, p, b, s, g, wants_h, wants_w, st);
     s.lse = a->lse, s.u = b.u, s.width = p.width, s.plane = p.Np * p.width;
-    const RowGrad g = {s.t, a->dloss, a->count, (int)a->reduction};
-    // g h for dw, and for dh w in fp16 (fp32: the scores' planes)
-    Pair x = {};
-    x.x = matrix(a->hidden, a->hidden_ld, p.N, p.D, sizeof(T), b.largest_g, b.scales + 2, wants_w ? b.h16 : nullptr, p.Np, p.Dp);
-    x.y = matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T), b.largest_w, b.scales + 1, wants_h && PL == 1 ? b.w16 : nullptr, p.Vp, p.Dp);
-    x.x.gathered = p.gather, x.x.graded = 1;
-    x.g = g, x.r = s.r;
-    copies<T, _Float16, PL>(x, st);
     for (int64_t v0 = 0; v0 < p.V; v0 += p.width) {
         const int64_t v1 = std::min(p.V, v0 + p.width), kv = pad(v1 - v0, kPad);
         s.v0 = (int)v0, s.v1 = (int)v1;
@@ -792,7 +840,8 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
             pw.q = {b.u, s.plane * 2, p.width, (int)(v1 - v0)};
             pw.splits = p.s_w, pw.k1 = (int)p.Np, pw.out = b.part_w, pw.ld = p.Dp;
             tiles_for<typename C::GradW>(pw);
-            sw = {b.part_w, p.s_w, (int)(v1 - v0), (int)p.D, (int)p.Dp, 0, (int)blocks_for((v1 - v0) * p.Dp / 4), b.scales + 2,
+            if (p.s_w == 1) pw.scale = b.scales + 2, pw.result = (T*)a->dweight + v0 * p.D;
+            else sw = {b.part_w, p.s_w, (int)(v1 - v0), (int)p.D, (int)p.Dp, 0, (int)blocks_for((v1 - v0) * p.Dp / 4), b.scales + 2,
                   (T*)a->dweight + v0 * p.D};
         }
         if (const int rc = parts<C>(ph, pw, st)) return rc;

@@ -709,10 +709,10 @@ int run(const char* what, const mb_muon* p, hipStream_t st) {
     const dim3 blk(kThreads);
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.blocks[kFirstChunk]), blk, 0, st, a);
     hipLaunchKernelGGL(muon_planes_kernel, dim3((unsigned)l.blocks[kFirstSquare]), blk, 0, st, a);
-    // Tiles of 64 or 128, by what a round of them took for 64 k (us; 4 matrices of 2816 x 1024, 3 of 777 x 1234): pairs 1.0
-    // for up to 512 of 64 and 1.4 for 256 of 128, B X 1.35 for 512 of 64, 2.9 for 512 of 128.
+    // Tiles of 64 or 128, by what a round of them took for 64 k (us; 4 matrices of 2816 x 1024, 3 of 777 x 1234, 48
+    // of the six-layer model): pairs 0.8 to 1.0 for up to 512 of 64 and 1.4 for 256 of 128, B X 1.35 for 512 of 64, 2.9 for 512 of 128.
     auto rounds = [](int64_t n, int64_t most) { return (double)((n + most - 1) / most); };
-    const bool small_pairs = rounds(l.blocks[kFirstPair64], 512) * 1.0 < rounds(l.blocks[kFirstPair], 256) * 1.4;
+    const bool small_pairs = rounds(l.blocks[kFirstPair64], 512) * 0.8 < rounds(l.blocks[kFirstPair], 256) * 1.4;
     const bool small_tiles = rounds(l.blocks[kFirstTile64], 512) * 1.35 < rounds(l.blocks[kFirstTile], 512) * 2.9;
     const int pairs = small_pairs ? kFirstPair64 : kFirstPair, tiles = small_tiles ? kFirstTile64 : kFirstTile;
     unsigned gram_grid, poly_grid, apply_grid;
