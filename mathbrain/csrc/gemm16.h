@@ -352,13 +352,17 @@ struct Product {
             if (p0 + p < p_end && q0 + piece * 8 < q_end) *(f16x8*)(out + (int64_t)(p0 + p) * ld + q0 + piece * 8) = v;
         }
     }
-    // The same for fp32 values, four next to each other.
-    static constexpr int kOut32 = TP * TQ * 4;
-    __device__ static int out32_at(int q, int piece) { return q * (4 * TP) + ((piece ^ (q & 15)) << 4); }
-    __device__ static f32x4v& held32(void* smem, int i, int j, int r) {
-        return *(f32x4v*)((char*)smem + out32_at(col(j), row(i, r) / 4));
+    // The same for fp32 values, four next to each other, for the blocks j0 .. j0 + n - 1 of every wave: row of LDS
+    // (wave's number along q) * 32 n + 32 (j - j0) + lane % 32.
+    __device__ static int out32_row(int j, int n) { return wave_id() / NP * 32 * n + 32 * j + (threadIdx.x & 31); }
+    __device__ static int out32_col(int row, int j0, int n) { return row / (32 * n) * WQ + 32 * j0 + row % (32 * n); }
+    __device__ static int out32_at(int r, int piece) { return r * (4 * TP) + ((piece ^ (r & 15)) << 4); }
+    __device__ static f32x4v& held32(void* smem, int i, int j, int r, int n = FQ) {
+        return *(f32x4v*)((char*)smem + out32_at(out32_row(j, n), row(i, r) / 4));
     }
-    __device__ static float out32(const void* smem, int q, int p) { return *((const float*)((const char*)smem + out32_at(q, p / 4)) + p % 4); }
+    __device__ static f32x4v& out32x4(void* smem, int r, int p) { return *(f32x4v*)((char*)smem + out32_at(r, p / 4)); }
+    __device__ static float out32(const void* smem, int r, int p) { return *((const float*)((const char*)smem + out32_at(r, p / 4)) + p % 4); }
+    static constexpr int kOut32 = TP * TQ * 4;
 };
 
 // ---- planes ------------------------------------------------------------------------------

@@ -27,7 +27,8 @@ constexpr int kThreads = 256;       // of the kernels around the products
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kUScale = 32768.f;
-constexpr int kMaxBlocks = 512;     // of the kernels that look for the largest value
+constexpr int kMaxBlocks = 2048;     // of the kernels that look for the largest value
+constexpr int kRowRuns = 512;       // of the kernel that finds the rows' places
 constexpr int kRowsPerBlock = 16;   // of the joining kernel
 
 struct Targets {
@@ -139,6 +140,7 @@ __global__ void __launch_bounds__(kThreads) ce_largest_kernel(const Set a) {
     const Matrix& x = a.mine(block);
     const int pieces = (x.D + 7) / 8;
     float most = 0.f;
+#pragma unroll 4
     for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)x.rows * pieces; i += (int64_t)x.blocks * kThreads) {
         const int64_t n = i / pieces;
         const int d = (int)(i - n * pieces) * 8;
@@ -324,6 +326,7 @@ __global__ void __launch_bounds__(kThreads) ce_join_kernel(const JoinArgs a) {
     };
     const int place = n < a.N ? a.r.of(n) : -1;
     if (place >= 0)
+#pragma unroll 8
         for (int i = slice; i < a.parts; i += kSlices) take(a.part[(int64_t)i * a.N + place]);
     s[slice][c] = make_float2(m, sum);
     __syncthreads();
@@ -443,43 +446,47 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     P prod;
     if (k1 > k0) prod.run(a.p, Side{a.q.p, a.q.plane, a.q.ld, end}, p0, q0, k0, k1, smem);
     else prod.clear();
+    // out by way of LDS, kAtOnce blocks of every wave at a time: a thread four values of a row, a wave whole rows
+    constexpr int kAtOnce = P::kOut32 <= P::kLds ? P::FQ : 1;
+    static_assert(P::kOut32 / P::FQ * kAtOnce <= P::kLds, "");
+    constexpr int kRowsOut = P::TQ / P::FQ * kAtOnce, kPieces = P::TP / 4;
+    const float f = a.scale ? 1.f / *a.scale / kUScale : 1.f;
+    const bool four = a.p.n % 4 == 0 && ((uintptr_t)a.result & 15) == 0;
+    typedef T four_t __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int j = 0; j < P::FQ; ++j) {
-        const int q = q0 + P::col(j);
-        if (q >= end) continue;
-        if (a.scale) {
-            const float f = 1.f / *a.scale / kUScale;
-            T* to = (T*)a.result + (int64_t)q * a.p.n;
-            const bool four = a.p.n % 4 == 0 && ((uintptr_t)a.result & 15) == 0;
+    for (int j0 = 0; j0 < P::FQ; j0 += kAtOnce) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
 #pragma unroll
             for (int i = 0; i < P::FP; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    const int p = p0 + P::row(i, r);
-                    typedef T four_t __attribute__((ext_vector_type(4)));
-                    const four_t v = {(T)(prod.acc[i][j][r] * f), (T)(prod.acc[i][j][r + 1] * f), (T)(prod.acc[i][j][r + 2] * f),
-                                      (T)(prod.acc[i][j][r + 3] * f)};
-                    if (four && p < a.p.n) {
-                        *reinterpret_cast<four_t*>(to + p) = v;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (p + e < a.p.n) to[p + e] = v[e];
-                    }
+                    const f32x16& v = prod.acc[i][j0 + j];
+                    P::held32(smem, i, j, r, kAtOnce) = f32x4v{v[r], v[r + 1], v[r + 2], v[r + 3]};
                 }
-            continue;
-        }
-        float* to = a.out + ((int64_t)split * a.q.n + q) * a.ld;
+        __syncthreads();
+#pragma unroll 4
+        for (int n = threadIdx.x; n < kRowsOut * kPieces; n += P::kThreads) {
+            const int row = n / kPieces, p = p0 + n % kPieces * 4, q = q0 + P::out32_col(row, j0, kAtOnce);
+            if (q >= end) continue;
+            f32x4v v = P::out32x4(smem, row, p - p0);
+            if (a.scale) {
+                T* to = (T*)a.result + (int64_t)q * a.p.n + p;
+                const four_t y = {(T)(v[0] * f), (T)(v[1] * f), (T)(v[2] * f), (T)(v[3] * f)};
+                if (four && p < a.p.n) {
+                    *reinterpret_cast<four_t*>(to) = y;
+                } else {
 #pragma unroll
-        for (int i = 0; i < P::FP; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int p = p0 + P::row(i, r);
-                if (p >= a.ld) continue;
-                f32x4v v = {prod.acc[i][j][r], prod.acc[i][j][r + 1], prod.acc[i][j][r + 2], prod.acc[i][j][r + 3]};
-                if (a.add) v += *reinterpret_cast<const f32x4v*>(to + p);
-                *reinterpret_cast<f32x4v*>(to + p) = v;
+                    for (int e = 0; e < 4; ++e)
+                        if (p + e < a.p.n) to[e] = y[e];
+                }
+            } else if (p < a.ld) {
+                float* to = a.out + ((int64_t)split * a.q.n + q) * a.ld + p;
+                if (a.add) v += *reinterpret_cast<const f32x4v*>(to);
+                *reinterpret_cast<f32x4v*>(to) = v;
             }
+        }
     }
 }
 
@@ -568,6 +575,16 @@ struct F32 {
     typedef Product<_Float16, 2, 256, 128, kRows, kRows, 4, 2> Score;
     typedef Product<_Float16, 2, 128, 128, kCols, kRows> GradH;
     typedef Product<_Float16, 2, 128, 128, kCols, kCols> GradW;
+};
+
+// Up to 64 rows: the scores' tiles take 64 rows and more of the vocabulary, whose reads are the time then (12 rows on 100 000
+// words of 1024, bf16: maxima and sums 67 -> 52 us, U 56 -> 42).
+constexpr int64_t kFewRows = 64;
+struct FewBf16 : Bf16 {
+    typedef Product<__bf16, 1, 256, 64, kRows, kRows, 2, 2, 64> Score;
+};
+struct FewF32 : F32 {
+    typedef Product<_Float16, 2, 128, 64, kRows, kRows, 2, 2, 32> Score;
 };
 
 struct Plan {
@@ -692,7 +709,7 @@ void operands(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs&
     s.t = g.t;
     s.r = {b.rows, b.pos, b.m, (int)p.N};
     if (p.gather) {
-        const int each = (int)pad((p.N + kMaxBlocks - 1) / kMaxBlocks, kThreads);
+        const int each = (int)pad((p.N + kRowRuns - 1) / kRowRuns, kThreads);
         hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((p.N + each - 1) / each)), dim3(kThreads), 0, st, s.t, (int)p.N, each, b.rows, b.pos, b.m);
     }
     constexpr bool f32 = sizeof(T) == 4;
@@ -858,20 +875,23 @@ using namespace mb;
 
 extern "C" int64_t mb_linear_ce_workspace(const mb_linear_ce* a, int backward) {
     if (check("mb_linear_ce_workspace", a)) return -1;
-    const Plan p = a->dtype == MB_DTYPE_F32 ? plan_of<F32>(a) : plan_of<Bf16>(a);
+    const bool few = a->N <= kFewRows;
+    const Plan p = a->dtype == MB_DTYPE_F32 ? few ? plan_of<FewF32>(a) : plan_of<F32>(a) : few ? plan_of<FewBf16>(a) : plan_of<Bf16>(a);
     return buffers_of(p, backward != 0, nullptr).bytes;
 }
 
 extern "C" int mb_linear_ce_fwd(const mb_linear_ce* a, void* stream) {
     if (const int rc = check("mb_linear_ce_fwd", a)) return rc;
     MB_REQUIRE(a->loss, "mb_linear_ce_fwd: null pointer argument");
-    return a->dtype == MB_DTYPE_F32 ? forward<F32>(a, (hipStream_t)stream)
-                                    : forward<Bf16>(a, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (a->N <= kFewRows) return a->dtype == MB_DTYPE_F32 ? forward<FewF32>(a, st) : forward<FewBf16>(a, st);
+    return a->dtype == MB_DTYPE_F32 ? forward<F32>(a, st) : forward<Bf16>(a, st);
 }
 
 extern "C" int mb_linear_ce_bwd(const mb_linear_ce* a, void* stream) {
     if (const int rc = check("mb_linear_ce_bwd", a)) return rc;
     MB_REQUIRE(a->dloss, "mb_linear_ce_bwd: null pointer argument");
-    return a->dtype == MB_DTYPE_F32 ? backward<F32>(a, (hipStream_t)stream)
-                                    : backward<Bf16>(a, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (a->N <= kFewRows) return a->dtype == MB_DTYPE_F32 ? backward<FewF32>(a, st) : backward<FewBf16>(a, st);
+    return a->dtype == MB_DTYPE_F32 ? backward<F32>(a, st) : backward<Bf16>(a, st);
 }
