@@ -3,11 +3,11 @@
 //   acc[p][q] = sum_k P[p][k] Q[q][k],  fp32 accumulation in the 32 x 32 x 16 matrix instructions
 //
 // One plane: bf16 or fp16 values.  Two planes: fp32 values as x = hi + lo, both fp16 (24 bits of x
-// where it is within 2^-17 of the matrix's largest, see split.h's scales), from three products
+// where it is within 2^-17 of the matrix's largest, see plane_scale), from three products
 // lo hi + hi lo + hi hi; the fourth is below fp32's own rounding.
 //
-// A workgroup of four waves (2 x 2) takes a TP x TQ tile of the result and walks k in steps of 32.
-// Operand tiles go from memory straight into LDS, kStages - 1 steps ahead, 16 bytes a lane.  Such a
+// A workgroup of four or eight waves takes a TP x TQ tile of the result and walks k in steps of 32 or 64.  Operand tiles go
+// from memory straight into LDS, kStages - 1 steps ahead, 16 bytes a lane.  Such a
 // load puts its 64 pieces next to each other, so a row has no padding; piece c of row r lies in the
 // place c ^ swz(r) instead, which spreads the reads over the banks.  An operand may have its k next to
 // each other (kRows) or its free index (kCols: read back by the transposing 16-bit LDS read).
@@ -15,6 +15,10 @@
 // Buffers are padded: kRows operands have whole steps of k (zeros behind the matrix on one side at
 // least), kCols operands whole steps of rows and rows of a multiple of 8 elements.  Tiles that pass
 // the free index's end read the last rows (or pieces) again; whoever uses acc leaves those out.
+//
+// What bounds it: power first (under such load the clock falls to 1.6 - 1.85 GHz), then the loads into LDS.  8192^3 in tiles of
+// 256 x 256 takes 955 - 1013 us, 1085 - 1150 TFLOP/s; its loads alone take 765 us, its instructions 560, its LDS reads 270.
+// kRows operands load best in whole lines of 128 bytes, steps of 64 (out of the L2: 382 us against 540 and more).
 //
 // A lane holds, of each 32 x 32 block, column q = lane % 32 and the rows p = 8 (r / 4) + 4 (lane / 32) + r % 4.
 #pragma once
@@ -166,7 +170,7 @@ struct Tile {
 };
 
 // NP x NQ waves, each with TP / NP x TQ / NQ of the tile.
-template <typename T_, int PLANES, int TP_, int TQ_, Order OP, Order OQ, int NP = 2, int NQ = 2, int STEP = 32, int kMost = 5>
+template <typename T_, int PLANES, int TP_, int TQ_, Order OP, Order OQ, int NP = 2, int NQ = 2, int STEP = 32>
 struct Product {
     typedef T_ T;
     static constexpr int kThreads = 64 * NP * NQ, kStep = STEP;
@@ -177,14 +181,16 @@ struct Product {
     typedef Tile<T, TP, OP, STEP, kThreads> TileP;
     typedef Tile<T, TQ, OQ, STEP, kThreads> TileQ;
     static constexpr int kStage = PLANES * (TileP::kBytes + TileQ::kBytes);
-    // Waves that a SIMD's registers are enough for, and the LDS of a workgroup then.
-    static constexpr int kWaves = FP * FQ > 8 ? 1 : 2;
-    static constexpr int kRoom = 163840 * kThreads / (256 * kWaves);
+    // Two waves a SIMD: two workgroups of four waves a CU, or one of eight.  One wave with twice the block (128 x 128) reads LDS
+    // less and stalls more: 8192^3 in tiles of 256 x 256 1013 TFLOP/s with four waves, 1085 - 1116 with eight.
+    static constexpr int kWaves = 2;
+    static_assert(FP * FQ <= 8, "results and two sets of operands in 256 registers");
+    static constexpr int kRoom = 163840 * kThreads / 512;     // bytes of LDS
     // Whether the waves meet before a step's last instructions, with the next step's first fragments on their way during
     // these: with eight waves in one workgroup all wait at the same time (8192^3, 256 x 256: 1146 TFLOP/s against 1120),
     // with two workgroups a CU the one works while the other waits (256 x 128: 1114 against 1081 with this).
     static constexpr bool kAhead = kThreads > 256;
-    static constexpr int kFit = kRoom / kStage, kStages = kFit < kMost ? kFit : kMost;
+    static constexpr int kStages = kRoom / kStage < 3 ? kRoom / kStage : 3;
     static_assert(kStages >= 2, "a step's operands on their way beside the one in use");
     static constexpr int kLds = kStages * kStage;
     static constexpr int kLoads = PLANES * (TileP::kLoads + TileQ::kLoads);

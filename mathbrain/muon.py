@@ -90,7 +90,7 @@ def _settings(what, steps, coefficients, eps):
 @torch.no_grad()
 def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=None):
     """The orthogonalised matrices, contiguous, of ``dtype`` (their own): ``matrices`` is a list of [rows, cols] tensors of
-    any shapes (a list comes back) or one tensor [..., rows, cols].  A matrix of zeros stays zero; a NaN or an infinity in a
+    any shapes (a list comes back) or one tensor [..., rows, cols].  A matrix of zeros stays zero (with eps = 0 it is 0 / 0, NaN); a NaN or an infinity in a
     matrix makes all of it NaN."""
     what = "orthogonalize"
     steps, coefficients, eps = _settings(what, steps, coefficients, eps)
