@@ -126,6 +126,21 @@ class RotaryFunction(torch.autograd.Function):
                      for x, shape, t in zip(tangents, ctx.rest[3:5], ctx.rest[5:7]))
 
 
+class TracedRotaryFunction(torch.autograd.Function):
+    """RotaryFunction for torch.compile, which takes no function with a jvp of its own: the first derivative backwards."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, start_rows, start, half, inverse):
+        ctx.save_for_backward(cos, sin, start_rows)
+        ctx.rest = (start, half, inverse)
+        return rotary_op(q, k, cos, sin, start_rows, start, half, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        start, half, inverse = ctx.rest
+        return (*rotary_op(gq, gk, *ctx.saved_tensors, start, half, not inverse), None, None, None, None, None, None)
+
+
 def _check(q, k, cos, sin, start, layout):
     what = "apply_rotary"
     rows = start if torch.is_tensor(start) else None
@@ -162,5 +177,5 @@ def apply_rotary(q, k, cos, sin, start=0, layout="interleaved"):
     rows = start.contiguous() if torch.is_tensor(start) else None
     args = (q, k, cos, sin, rows, 0 if rows is not None else int(start), layout == "half", False)
     if _lib.wants_derivatives(q, k):
-        return RotaryFunction.apply(*args)
+        return (TracedRotaryFunction if torch.compiler.is_compiling() else RotaryFunction).apply(*args)
     return rotary_op(*args)

@@ -242,3 +242,46 @@ def test_the_model_turns_as_it_did_and_with_options():
     for bad in (dict(rope_layout="x"), dict(rope_dims=7), dict(rope_dims=66), dict(qk_norm=True, rope_dims=16)):
         with pytest.raises(ValueError):
             baseline.RoPETransformerLM(300, 128, 2, 2, **bad)
+
+
+@pytest.mark.parametrize("options", [{}, dict(rope_layout="half", rope_dims=16), dict(rel_buckets=8)])
+@pytest.mark.parametrize("targets", [False, True])
+def test_the_model_traces_into_one_graph(options, targets):
+    """torch.compile of the training step makes one graph of the model, with the eager step's results.  The traced step
+    calls the same kernels in the same order; sums of shared gradients may be taken in another one: 2^-24 of the terms each."""
+    from mathbrain.baseline import RoPETransformerLM
+    torch.manual_seed(3)
+    m = RoPETransformerLM(400, 128, 2, 4, max_seq_len=64, dropout=0.0, **options).cuda()
+    args = [torch.randint(0, 400, (2, 48), device="cuda") for _ in range(1 + targets)]
+    torch._dynamo.reset()
+    assert torch._dynamo.explain(m)(*args).graph_break_count == 0
+    torch._dynamo.reset()
+    compiled = torch.compile(m, backend="aot_eager", fullgraph=True)
+    a, b = m(*args), compiled(*args)
+    assert torch.equal(a, b)
+    ga, gb = (torch.autograd.grad(x.square().mean(), list(m.parameters())) for x in (a, b))
+    for u, v in zip(ga, gb):
+        assert torch.allclose(u, v, rtol=1e-4, atol=1e-4 * float(u.abs().max()))
+
+
+@pytest.mark.parametrize("sides", ["both", "q", "k"])
+@pytest.mark.parametrize("start", ["int", "rows", "tokens"])
+def test_traced_gradients(start, sides):
+    """The same function compiled and not, with a gradient for both results or one of them."""
+    from mathbrain.rotary import apply_rotary, rotary_tables
+    torch.manual_seed(4)
+    q, k = torch.randn(3, 5, 4, 32, device="cuda"), torch.randn(3, 5, 2, 32, device="cuda")
+    cos, sin = rotary_tables(32, 40, device="cuda")
+    at = {"int": 3, "rows": torch.tensor([0, 30, 7], device="cuda"),
+          "tokens": torch.randint(0, 40, (3, 5), device="cuda", dtype=torch.int32)}[start]
+
+    def run(f):
+        x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+        a, b = f(x, y)
+        loss = sum((t * t * t).sum() for side, t in (("q", a), ("k", b)) if sides in ("both", side))
+        return a, b, *torch.autograd.grad(loss, [x, y], materialize_grads=True)
+
+    torch._dynamo.reset()
+    eager = run(lambda x, y: apply_rotary(x, y, cos, sin, at, "half"))
+    traced = run(torch.compile(lambda x, y: apply_rotary(x, y, cos, sin, at, "half"), backend="aot_eager", fullgraph=True))
+    assert all(torch.equal(a, b) for a, b in zip(eager, traced))
