@@ -243,7 +243,7 @@ __device__ inline float score_factor(const ScoreArgs& a) {
     return a.scale_w ? (1.f / *a.scale_w) * (1.f / *a.scale_h) * kLog2e : kLog2e;
 }
 
-// Matrix instructions bound it: 28672 rows, 50257 words of 512 in bf16 1.61 ms, 916 TFLOP/s; 16 rows 13.8 us, the weights' 51 MB at
+// Matrix instructions bound it: 28672 rows, 50257 words of 512 in bf16 1.57 - 1.61 ms, 916 - 941 TFLOP/s; 16 rows 13.8 us, the weights' 51 MB at
 // 3.7 TB/s.
 template <typename P>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const ScoreArgs a) {
@@ -379,8 +379,8 @@ __global__ void __launch_bounds__(kThreads) ce_total_kernel(const double* sums, 
     }
 }
 
-// U of a piece of the vocabulary, zeros behind its end and behind the last row.  28672 rows, 50257 words of 512 in bf16: 363 us a piece
-// of 9216 words on average, 677 TFLOP/s; 309 us without its 528 MB of stores.  Stores past the caches: 0.4 - 0.9 % less for the whole
+// U of a piece of the vocabulary, zeros behind its end and behind the last row.  28672 rows, 50257 words of 512 in bf16: 365 us a piece
+// of 9216 words on average, 674 TFLOP/s; 309 us without its 528 MB of stores.  Stores past the caches: 0.4 - 0.9 % less for the whole
 // call there and at 4096 rows of 1024, 1 % more at 1186.
 template <typename P, int PL>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const ScoreArgs a) {
@@ -565,7 +565,7 @@ struct Carve {
 // U's bytes in a piece (of 256 words at least): few launches and few passes over dh's sums against what stays in the
 // caches and the memory that is wanted.  56 x 512 rows, 50257 words: 256 MiB 7.14 ms, 512 6.88, 1024 6.93, 2048 7.05.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
-// From so many rows on the ones that count are put next to each other first: a launch more and a copy of the rows, 16 + 15 us a
+// From so many rows on the ones that count are put next to each other first: a launch more and a copy of the rows, 15.5 + 15.2 us a
 // direction (both directions: 6.8 ms) at 56 x 512; where 0.3 of 4093 rows are ignored (20011 words of 384, fp32) 929 -> 782 us.
 constexpr int64_t kGatherRows = 1024;
 
@@ -608,7 +608,7 @@ int64_t tiles_of(int64_t np, int64_t nq) { return ((np + P::TP - 1) / P::TP) * (
 // Splits of the two gradients' k: those (of 1 to 32 each, runs of 256 k at least) with the shortest launch.  A workgroup takes its
 // steps of k and about kOverhead more to begin and end, and its part of the sums is written and read again; the longer ones go
 // first, in rounds of kSlots, and the shorter ones fill what the last of these leaves.  56 x 512 rows, a piece of 9216 words of
-// 512: 448 workgroups of 144 steps and 576 of 112 in two full rounds; the six pieces' launches take 498 us on average, 988 TFLOP/s.
+// 512: 448 workgroups of 144 steps and 576 of 112 in two full rounds; the six pieces' launches take 500 us on average, 983 TFLOP/s.
 constexpr int kOverhead = 12, kSlots = 512;
 void choose_splits(int64_t tiles_h, int64_t k_h, int64_t tiles_w, int64_t k_w, int& s_h, int& s_w) {
     double best = 1e300;
