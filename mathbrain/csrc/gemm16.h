@@ -23,7 +23,7 @@
 // A lane holds, of each 32 x 32 block, column q = lane % 32 and the rows p = 8 (r / 4) + 4 (lane / 32) + r % 4.
 #pragma once
 
-#include "common.h"
+#include "lds_dma.h"
 
 #include <atomic>
 #include <type_traits>
@@ -59,23 +59,6 @@ struct Frag<_Float16> { typedef f16x8 type; };
 template <>
 struct Frag<__bf16> { typedef bf16x8 type; };
 
-// 16 bytes a lane from base + voff to LDS at lds + 16 * lane.  M0 holds the LDS address; the compiler reserves it for
-// its own instructions, which set it before they use it, warns of the clobber for that reason, and has to know of it.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ inline void dma16(uint32_t lds, uint32_t voff, const void* base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds), "v"(voff), "s"(base)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-// Waits until at most N of the wave's loads are on their way, and for the other waves.
-template <int N>
-__device__ inline void wait_and_meet() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
-}
-__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 // A value that is the same in all lanes, where the compiler cannot see that.
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 template <typename T>
@@ -86,9 +69,6 @@ __device__ inline T* uniform(T* p) {
 }
 __device__ inline int64_t uniform(int64_t x) { return (int64_t)uniform((char*)x); }
 __device__ inline Side uniform(const Side& s) { return {uniform((char*)s.p), uniform(s.plane), uniform(s.ld), uniform(s.n)}; }
-__device__ inline uint32_t lds_address(const void* p) {
-    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
 
 // A tile of N free indices by STEP k in LDS.
 template <typename T, int N, Order ORDER, int STEP, int THREADS>
