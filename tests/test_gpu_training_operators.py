@@ -206,3 +206,55 @@ def test_a_whole_step_captured():
         # the library's products may sum in another order within the graph: the matrices agree to that
         for p, q in zip(captured[2], eager[2]):
             assert float((p - q).norm()) < 1e-3 * 4**i * float(q.norm())
+
+
+def test_calls_on_two_streams_at_once():
+    """Each operator on two streams, in turn and without a wait between them, gives what it gives alone (all sums have a
+    fixed order: bit for bit)."""
+    from mathbrain.linear_cross_entropy import linear_cross_entropy
+    from mathbrain.muon import orthogonalize
+    from mathbrain.rotary import apply_rotary, rotary_tables
+    cos, sin = rotary_tables(32, 300, device="cuda")
+    made = []
+    for seed in range(2):
+        g = torch.Generator("cuda").manual_seed(seed)
+        made.append([torch.randn(1500, 128, device="cuda", generator=g) * 0.3, torch.randn(901, 128, device="cuda", generator=g) * 0.3,
+                     torch.randint(0, 901, (1500,), device="cuda", generator=g), torch.randn(260, 190, device="cuda", generator=g),
+                     torch.randn(2, 300, 3, 32, device="cuda", generator=g)])
+
+    def work(h, w, t, m, q):
+        h, w, q = (x.detach().requires_grad_() for x in (h, w, q))
+        loss = linear_cross_entropy(h, w, t)
+        a, b = apply_rotary(q, q, cos, sin)
+        return [loss, *torch.autograd.grad(loss, [h, w]), a, b, *torch.autograd.grad((a * b.detach()).sum(), [q]), orthogonalize(m)]
+
+    alone = [work(*x) for x in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    got = [[], []]
+    for _ in range(4):
+        for s, x, out in zip(streams, made, got):
+            with torch.cuda.stream(s):
+                out.append(work(*x))
+    torch.cuda.synchronize()
+    for want, runs in zip(alone, got):
+        assert all(torch.equal(x, y) for run in runs for x, y in zip(want, run))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_hidden_and_weight_are_one_tensor(t):
+    """F.cross_entropy(x x^T): x's gradient is the sum of both.  Scores of 48 products of values below 4 * 0.25: off by
+    48 * 2^-24 * |h| |w| at most, far below the outputs' own step: 2^-8 of the largest for bf16 (two roundings of half a step and
+    their sum's), 1e-5 of it for fp32."""
+    from mathbrain.linear_cross_entropy import linear_cross_entropy
+    torch.manual_seed(5)
+    x = (torch.randn(70, 48, device="cuda") * 0.25).to(t).requires_grad_()
+    target = torch.randint(0, 70, (70,), device="cuda")
+    y = x.detach().double().requires_grad_()
+    want = F.cross_entropy(y @ y.T, target)
+    loss = linear_cross_entropy(x, x, target)
+    assert abs(float(loss) - float(want)) < 1e-5 * float(want)
+    got, = torch.autograd.grad(loss, [x])
+    exact, = torch.autograd.grad(want, [y])
+    tol = 1e-5 if t == torch.float32 else 3 * 2.0**-8
+    assert float((got.double() - exact).abs().max()) < tol * float(exact.abs().max())
