@@ -88,6 +88,8 @@ struct Args {
     float lr, mu, keep;          // keep = 1 - lr decay
     int nesterov, is_step, last;
     Runs runs;                   // of this launch
+    float* parts;                // A's tiles, k split
+    int splits, tiles;
 };
 
 // The workgroup's tile, or -1.
@@ -237,26 +239,20 @@ __device__ inline void split4(const float* v, f16x4& hi, f16x4& lo) {
     }
 }
 
-// POLY: B = b A + c A^2 from A's planes; otherwise A = X X^T.  Matrix instructions bound it: 4 matrices of 2816 x 1024 67 us for
-// A (526 TFLOP/s, three products an element, one side of the diagonal counted: 36 tiles of 128 each on 256 CUs), 32 us for B.
-template <bool POLY, int TILE>
-__global__ void __launch_bounds__(By<TILE>::Gram::kThreads, By<TILE>::Gram::kWaves) muon_pair_kernel(const Args a) {
-    typedef typename By<TILE>::Gram Gram;
-    static_assert(2 * Gram::kOutPlane <= Gram::kLds, "results go out through LDS");
-    extern __shared__ char smem[];
-    int id = tile_of(a.runs);
-    if (id < 0) return;
-    const Mat m = find(a, TILE == 64 ? kFirstPair64 : kFirstPair, id);
-    int q = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);   // id = q (q + 1) / 2 + p, p <= q
+// Tile `id` of the pairs: id = q (q + 1) / 2 + p, p <= q.
+template <int TILE>
+__device__ inline void pair_place(int id, int& p0, int& q0) {
+    int q = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
     while (q * (q + 1) / 2 > id) --q;
     while ((q + 1) * (q + 2) / 2 <= id) ++q;
     q = uniform(q);
-    const int p = id - q * (q + 1) / 2, p0 = p * TILE, q0 = q * TILE;
+    p0 = (id - q * (q + 1) / 2) * TILE, q0 = q * TILE;
+}
+
+// The sums of a pair's tile to A or B, on both sides of the diagonal.
+template <bool POLY, typename Gram>
+__device__ inline void pair_out(const Args& a, const Mat& m, const Gram& g, int p0, int q0, char* smem) {
     const int64_t plane = (int64_t)m.mp * m.mp;
-    const Side side = POLY ? Side{m.a, plane * 2, m.mp, m.mp} : Side{m.x[a.from], (int64_t)m.mp * m.np * 2, m.np, m.mp};
-    Gram g;
-    g.run(side, side, p0, q0, 0, POLY ? m.mp : m.np, smem);
-    __syncthreads();
     if (POLY) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) Gram::fetch(smem, h, m.a + h * plane, m.mp, p0, q0, m.mp, m.mp);
@@ -284,8 +280,68 @@ __global__ void __launch_bounds__(By<TILE>::Gram::kThreads, By<TILE>::Gram::kWav
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         Gram::store(smem, h, out + h * plane, m.mp, p0, q0, m.mp, m.mp);
-        if (p != q) Gram::store_turned(smem, h, out + h * plane, m.mp, p0, q0, m.mp, m.mp);
+        if (p0 != q0) Gram::store_turned(smem, h, out + h * plane, m.mp, p0, q0, m.mp, m.mp);
     }
+}
+
+// POLY: B = b A + c A^2 from A's planes; otherwise A = X X^T.  Matrix instructions bound it: 4 matrices of 2816 x 1024 67 us for
+// A (526 TFLOP/s, three products an element, one side of the diagonal counted: 36 tiles of 128 each on 256 CUs), 32 us for B.
+template <bool POLY, int TILE>
+__global__ void __launch_bounds__(By<TILE>::Gram::kThreads, By<TILE>::Gram::kWaves) muon_pair_kernel(const Args a) {
+    typedef typename By<TILE>::Gram Gram;
+    static_assert(2 * Gram::kOutPlane <= Gram::kLds, "results go out through LDS");
+    extern __shared__ char smem[];
+    int id = tile_of(a.runs), p0, q0;
+    if (id < 0) return;
+    const Mat m = find(a, TILE == 64 ? kFirstPair64 : kFirstPair, id);
+    pair_place<TILE>(id, p0, q0);
+    const Side side = POLY ? Side{m.a, (int64_t)m.mp * m.mp * 2, m.mp, m.mp} : Side{m.x[a.from], (int64_t)m.mp * m.np * 2, m.np, m.mp};
+    Gram g;
+    g.run(side, side, p0, q0, 0, POLY ? m.mp : m.np, smem);
+    __syncthreads();
+    pair_out<POLY>(a, m, g, p0, q0, smem);
+}
+
+// A's tiles with k split, for few of them: the sums of a run of k, as the lanes hold them, to `parts` [splits][tiles][4096],
+// and a launch that adds them in the runs' order.  A matrix with fewer steps than runs has empty ones, zeros.
+typedef By<64>::Gram Part;
+static_assert(Part::FP * Part::FQ == 1 && Part::kThreads * 16 == kSquare * kSquare, "a block of 16 values a lane");
+__device__ inline f32x4v* part_at(const Args& a, int split, int id) {
+    return (f32x4v*)a.parts + ((int64_t)split * a.tiles + id) * (kSquare * kSquare / 4) + threadIdx.x;
+}
+__global__ void __launch_bounds__(Part::kThreads, Part::kWaves) muon_part_kernel(const Args a) {
+    extern __shared__ char smem[];
+    int id = tile_of(a.runs), p0, q0;
+    if (id < 0) return;
+    f32x4v* to = part_at(a, blockIdx.y, id);
+    const Mat m = find(a, kFirstPair64, id);
+    pair_place<64>(id, p0, q0);
+    const int steps = m.np / Part::kStep;
+    const int k0 = steps * (int)blockIdx.y / a.splits * Part::kStep, k1 = steps * ((int)blockIdx.y + 1) / a.splits * Part::kStep;
+    const Side side = {m.x[a.from], (int64_t)m.mp * m.np * 2, m.np, m.mp};
+    Part g;
+    if (k1 > k0) g.run(side, side, p0, q0, k0, k1, smem);
+    else g.clear();
+    const f32x16& v = g.acc[0][0];
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) to[r / 4 * Part::kThreads] = f32x4v{v[r], v[r + 1], v[r + 2], v[r + 3]};
+}
+__global__ void __launch_bounds__(Part::kThreads) muon_join_kernel(const Args a) {
+    extern __shared__ char smem[];
+    int id = blockIdx.x, p0, q0;
+    f32x4v v[4] = {};
+#pragma unroll 4
+    for (int split = 0; split < a.splits; ++split) {
+        const f32x4v* from = part_at(a, split, id);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += from[r * Part::kThreads];
+    }
+    const Mat m = find(a, kFirstPair64, id);
+    pair_place<64>(id, p0, q0);
+    Part g;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) g.acc[0][0][r] = v[r / 4][r % 4];
+    pair_out<false>(a, m, g, p0, q0, smem);
 }
 
 // X <- a X + B X.  4 matrices of 2816 x 1024: 97 us, 733 TFLOP/s of three products an element.
@@ -594,6 +650,8 @@ struct Layout {
     std::vector<Mat> mats;
     std::vector<int> first[kFirsts];
     int64_t blocks[kFirsts] = {};
+    int splits = 1;
+    float* parts = nullptr;
 
     // The XCDs' runs of a launch whose tiles cost their matrix's n (or m) each, and its grid.
     Runs runs(int which, bool by_n, unsigned& grid) const {
@@ -617,8 +675,14 @@ struct Layout {
     }
 };
 
+// Runs of k for A where its tiles of 64 leave places empty: as many as fill these, each of 8 steps at least.  A step is about
+// 0.77 us, so that the half of it and more that is saved pays for the join's launch, 5 - 6 us.  Whole calls, not split and
+// split: one of 4096 x 1024 616 and 537 us, one of 640 x 4000 462 and 332, 8 of 64 x 2816 215 and 147, one of 48 x 2816 207 and 132.
+constexpr int kPlaces = 512;
+int64_t splits_of(int64_t tiles, int64_t longest) { return tiles ? std::max<int64_t>(1, std::min(kPlaces / tiles, longest / kPad / 8)) : 1; }
+
 int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
-    int64_t used = 0;
+    int64_t used = 0, tiles = 0, longest = 0;
     auto take = [&](int64_t bytes) {
         char* at = base ? base + used : nullptr;
         used += pad(bytes, 256);
@@ -649,6 +713,7 @@ int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
         m.a = (_Float16*)take(a), m.b = (_Float16*)take(a);
         if (p->is_step) m.u = (float*)take(elements * 4);
         m.part = (double*)take(m.chunks * 8);
+        tiles += (int64_t)(m.mp / 64) * (m.mp / 64 + 1) / 2, longest = std::max<int64_t>(longest, m.np);
         if (out) {
             const int64_t m64 = m.mp / 64, n64 = m.np / 64, m128 = (m64 + 1) / 2, n128 = (n64 + 1) / 2;
             const int64_t items[kFirsts] = {m.chunks, m64 * n64, m128 * (m128 + 1) / 2, m64 * (m64 + 1) / 2, m128 * n128, m64 * n64};
@@ -659,6 +724,9 @@ int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
             out->mats.push_back(m);
         }
     }
+    const int64_t splits = splits_of(tiles, longest);
+    float* parts = splits > 1 ? (float*)take(splits * tiles * kSquare * kSquare * 4) : nullptr;
+    if (out) out->splits = (int)splits, out->parts = parts;
     return used;
 }
 
@@ -718,6 +786,7 @@ int run(const char* what, const mb_muon* p, hipStream_t st) {
     const bool small_pairs = rounds(l.blocks[kFirstPair64], 512) * 0.8 < rounds(l.blocks[kFirstPair], 256) * 1.4;
     const bool small_tiles = rounds(l.blocks[kFirstTile64], 512) * 1.35 < rounds(l.blocks[kFirstTile], 512) * 2.9;
     const int pairs = small_pairs ? kFirstPair64 : kFirstPair, tiles = small_tiles ? kFirstTile64 : kFirstTile;
+    a.parts = l.parts, a.splits = l.splits, a.tiles = (int)l.blocks[kFirstPair64];     // (few tiles are small pairs)
     unsigned gram_grid, poly_grid, apply_grid;
     const Runs gram_runs = l.runs(pairs, true, gram_grid), poly_runs = l.runs(pairs, false, poly_grid),
                apply_runs = l.runs(tiles, false, apply_grid);
@@ -731,7 +800,14 @@ int run(const char* what, const mb_muon* p, hipStream_t st) {
             if (const int rc = allow_lds(what, (const void*)muon_pair_kernel<false, TILE>, lds, told[0])) return rc;
             if (const int rc = allow_lds(what, (const void*)muon_pair_kernel<true, TILE>, lds, told[1])) return rc;
             a.runs = gram_runs;
-            hipLaunchKernelGGL((muon_pair_kernel<false, TILE>), dim3(gram_grid), blk, lds, st, a);
+            if (TILE == 64 && a.splits > 1) {
+                static Told part;
+                if (const int rc = allow_lds(what, (const void*)muon_part_kernel, lds, part)) return rc;
+                hipLaunchKernelGGL(muon_part_kernel, dim3(gram_grid, a.splits), blk, lds, st, a);
+                hipLaunchKernelGGL(muon_join_kernel, dim3(a.tiles), blk, 2 * Part::kOutPlane, st, a);
+            } else {
+                hipLaunchKernelGGL((muon_pair_kernel<false, TILE>), dim3(gram_grid), blk, lds, st, a);
+            }
             a.runs = poly_runs;
             hipLaunchKernelGGL((muon_pair_kernel<true, TILE>), dim3(poly_grid), blk, lds, st, a);
             return MB_OK;

@@ -255,3 +255,36 @@ def test_refusals():
         muon_step([x], [y], [z], math.nan)
     assert torch.equal(x, keep)
     muon_step([], [], [], 0.1)
+
+
+@pytest.mark.parametrize("shapes", [[(4096, 1024)], [(640, 4000)], [(48, 20000)], [(129, 1300)], [(130, 1023), (1023, 130)],
+                                    [(300, 2500), (65, 66), (200, 1), (640, 700)], [(1400, 1400)]])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_few_matrices_with_long_sums(shapes, t):
+    """Few matrices, whose first products are shared out along their sums; with short matrices among them, which have fewer
+    steps than there are shares; the same twice; and a step of the optimiser."""
+    from mathbrain.muon import muon_step, orthogonalize
+    g = torch.Generator("cuda").manual_seed(11)
+    mats = [torch.randn(s, generator=g, device="cuda").to(t) for s in shapes]
+    got, again = orthogonalize(mats), orthogonalize(mats)
+    for x, y, z in zip(got, mats, again):
+        check(x, definition(y), what=tuple(y.shape))
+        assert torch.equal(x, z)
+    params, momenta = [torch.zeros_like(x) for x in mats], [torch.zeros_like(x) for x in mats]
+    muon_step(params, mats, momenta, 1.0, momentum=0.9, nesterov=False)
+    for p, x in zip(params, mats):
+        check(-p / math.sqrt(max(1.0, x.shape[0] / x.shape[1])), definition(x), what=tuple(x.shape))
+
+
+def test_few_long_matrices_captured():
+    from mathbrain.muon import orthogonalize
+    x = torch.randn(300, 2500, device="cuda")
+    orthogonalize(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = orthogonalize(x)
+    for i in range(3):
+        x.copy_(torch.randn(300, 2500, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, orthogonalize(x))
