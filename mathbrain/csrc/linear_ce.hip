@@ -548,6 +548,250 @@ __global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const
     }
 }
 
+// ---- up to eight rows --------------------------------------------------------------------
+//
+// The time is the weights' read (and dw's write) then, so fp32 products from registers do: a wave takes a few words at a time, 16
+// bytes of each a lane and chunk, and reads hidden (fp32 in LDS) once for them.  The backward has the scores' words still in its
+// registers for dh, whose sums it keeps over all its words, and writes dw at once: w is read once a direction, without the copies
+// that the matrix instructions want.  A score's sum over the lanes leaves it with the lane whose number begins with it.
+constexpr int kFewThreads = 512;
+constexpr int kFewLanes = 64;
+struct FewArgs {
+    const void *hidden, *weight;
+    int64_t h_ld, w_ld;
+    RowGrad g;
+    int N, V, D, vec, out_vec;
+    float2* part;                 // forward: [workgroups, N] maximum and sum
+    float* target_score;          // forward: [N]
+    const float* lse;             // backward: [2, N]
+    float* part_h;                // backward: [workgroups, N, D4], or NULL
+    int D4;
+    void* dweight;                // backward: [V, D], or NULL
+};
+
+// R: rows; C: channels of a lane.  R C is at most 128, the sums of dh in registers.
+template <typename T, int R, int C>
+struct Few {
+    static constexpr int kVec = 16 / sizeof(T), kChunks = C / kVec, kQuads = kVec / 4;
+    static constexpr int kWords = C * sizeof(T) > 64 || R * C > 64 ? 2 : 4;   // at a time, what registers hold beside the sums
+    static constexpr int M = kWords * R;
+    static constexpr int kLds = R * C * kFewLanes * 4;
+    static_assert(R * C <= 128 && M <= kFewLanes && C % kVec == 0, "");
+    typedef T vec_t __attribute__((ext_vector_type(kVec), aligned(16)));
+
+    static __device__ int lane() { return threadIdx.x & 63; }
+    static __device__ int channel(int c) { return (c * kFewLanes + lane()) * kVec; }
+    static __device__ int at(int r, int c, int q) { return (((r * kChunks + c) * kQuads + q) * kFewLanes + lane()) * 4; }
+    // which of the wave's scores this lane has
+    static constexpr int kEach = kFewLanes / M;
+    static __device__ int word() { return lane() / kEach / R; }
+    static __device__ int row() { return lane() / kEach % R; }
+
+    // hidden in LDS, zeros in place of ignored rows and behind the end
+    static __device__ void stage(const FewArgs& a, float* h) {
+        for (int i = threadIdx.x; i < R * C * kFewLanes; i += kFewThreads) {
+            const int r = i / (C * kFewLanes), c = i / (kVec * kFewLanes) % kChunks, q = i / (4 * kFewLanes) % kQuads;
+            const int d = (c * kFewLanes + i / 4 % kFewLanes) * kVec + 4 * q + i % 4;
+            h[i] = r < a.N && d < a.D && a.g.t.at(r) != -1 ? (float)((const T*)a.hidden)[r * a.h_ld + d] : 0.f;
+        }
+        __syncthreads();
+    }
+    static __device__ void load(const FewArgs& a, int v0, vec_t (&w)[kWords][kChunks]) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            const T* from = (const T*)a.weight + (int64_t)min(v0 + i, a.V - 1) * a.w_ld;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = channel(c);
+                if (a.vec) {
+                    w[i][c] = d < a.D ? *reinterpret_cast<const vec_t*>(from + d) : vec_t{};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) w[i][c][e] = d + e < a.D ? from[d + e] : (T)0.f;
+                }
+            }
+        }
+    }
+    // this lane's score, in units of log 2
+    static __device__ float score(const float* h, const vec_t (&w)[kWords][kChunks]) {
+        float s[M] = {};
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                __builtin_amdgcn_sched_barrier(0);     // hidden's reads stay where they are: all of them at once would not fit
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const f32x4v x = *reinterpret_cast<const f32x4v*>(h + at(r, c, q));
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[i * R + r] = __builtin_fmaf((float)w[i][c][4 * q + e], x[e], s[i * R + r]);
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < 6; ++k) {
+            const int o = 32 >> k, left = M >> (k + 1);
+            if (left == 0) {
+                s[0] += __shfl_xor(s[0], o, 64);
+            } else {
+                const bool upper = lane() & o;
+#pragma unroll
+                for (int i = 0; i < left; ++i) {
+                    const float give = upper ? s[i] : s[i + left], keep = upper ? s[i + left] : s[i];
+                    s[i] = keep + __shfl_xor(give, o, 64);
+                }
+            }
+        }
+        return s[0] * kLog2e;
+    }
+};
+
+template <typename T, int R, int C>
+__global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewArgs a) {
+    typedef Few<T, R, C> F;
+    extern __shared__ char smem[];
+    float* h = (float*)smem;
+    F::stage(a, h);
+    constexpr int kWaves = kFewThreads / 64;
+    const int wave = wave_id(), r = F::row(), target = r < a.N ? a.g.t.at(r) : -1;
+    float m = -INFINITY, sum = 0.f;
+    for (int64_t v0 = ((int64_t)blockIdx.x * kWaves + wave) * F::kWords; v0 < a.V; v0 += (int64_t)gridDim.x * kWaves * F::kWords) {
+        typename F::vec_t w[F::kWords][F::kChunks];
+        F::load(a, (int)v0, w);
+        const float s = F::score(h, w);
+        const int v = (int)v0 + F::word();
+        if (v >= a.V) continue;
+        if (v == target) a.target_score[r] = s;
+        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
+        sum = sum * __builtin_amdgcn_exp2f(m - base) + __builtin_amdgcn_exp2f(s - base);
+        m = top;
+    }
+    __shared__ float2 both[kWaves][F::M];
+    if (F::lane() % F::kEach == 0) both[wave][F::lane() / F::kEach] = make_float2(m, sum);
+    __syncthreads();
+    if ((int)threadIdx.x < a.N) {
+        float top = -INFINITY, t = 0.f;
+        for (int i = 0; i < kWaves * F::kWords; ++i) top = fmaxf(top, both[i / F::kWords][i % F::kWords * R + threadIdx.x].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int i = 0; i < kWaves * F::kWords; ++i) {
+            const float2 x = both[i / F::kWords][i % F::kWords * R + threadIdx.x];
+            t += x.y * __builtin_amdgcn_exp2f(x.x - base);
+        }
+        a.part[(int64_t)blockIdx.x * a.N + threadIdx.x] = make_float2(top, t);
+    }
+}
+
+template <typename T, int R, int C>
+__global__ void __launch_bounds__(kFewThreads, 2) ce_few_grads_kernel(const FewArgs a) {
+    typedef Few<T, R, C> F;
+    extern __shared__ char smem[];
+    float* h = (float*)smem;
+    F::stage(a, h);
+    constexpr int kWaves = kFewThreads / 64;
+    const int wave = wave_id(), r = F::row(), target = r < a.N ? a.g.t.at(r) : -1;
+    const bool counts = target != -1;
+    const float g = counts ? a.g.at(r) : 0.f, m = counts ? a.lse[r] : 0.f, l = counts ? a.lse[a.N + r] : 0.f;
+    float dh[R][C] = {};
+    for (int64_t v0 = ((int64_t)blockIdx.x * kWaves + wave) * F::kWords; v0 < a.V; v0 += (int64_t)gridDim.x * kWaves * F::kWords) {
+        typename F::vec_t w[F::kWords][F::kChunks];
+        F::load(a, (int)v0, w);
+        const int v = (int)v0 + F::word();
+        float mine = __builtin_amdgcn_exp2f((F::score(h, w) - m) - l);
+        mine = v == target ? mine - 1.f : mine;
+        mine = v < a.V && g != 0.f ? mine * g : 0.f;
+        float u[F::kWords][R];
+#pragma unroll
+        for (int i = 0; i < F::M; ++i)
+            u[i / R][i % R] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i * F::kEach));
+#pragma unroll
+        for (int c = 0; c < F::kChunks; ++c) {
+            typename F::vec_t out[F::kWords];
+#pragma unroll
+            for (int q = 0; q < F::kQuads; ++q) {
+                __builtin_amdgcn_sched_barrier(0);
+                f32x4v y[F::kWords] = {};
+#pragma unroll
+                for (int n = 0; n < R; ++n) {
+                    const f32x4v x = *reinterpret_cast<const f32x4v*>(h + F::at(n, c, q));
+#pragma unroll
+                    for (int i = 0; i < F::kWords; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            y[i][e] = __builtin_fmaf(u[i][n], x[e], y[i][e]);
+                            float& sum = dh[n][c * F::kVec + 4 * q + e];
+                            sum = __builtin_fmaf(u[i][n], (float)w[i][c][4 * q + e], sum);
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < F::kWords; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[i][4 * q + e] = (T)y[i][e];
+            }
+            const int d = F::channel(c);
+            if (!a.dweight || d >= a.D) continue;
+#pragma unroll
+            for (int i = 0; i < F::kWords; ++i) {
+                if (v0 + i >= a.V) continue;
+                T* to = (T*)a.dweight + (v0 + i) * a.D + d;
+                if (a.out_vec) {
+                    *reinterpret_cast<typename F::vec_t*>(to) = out[i];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < F::kVec; ++e)
+                        if (d + e < a.D) to[e] = out[i][e];
+                }
+            }
+        }
+    }
+    if (!a.part_h) return;
+    // the waves' sums of dh in their order, in hidden's place
+    for (int i = 0; i < kWaves; ++i) {
+        __syncthreads();
+        if (wave != i) continue;
+#pragma unroll
+        for (int n = 0; n < R; ++n)
+#pragma unroll
+            for (int c = 0; c < F::kChunks; ++c)
+#pragma unroll
+                for (int q = 0; q < F::kQuads; ++q) {
+                    f32x4v& sum = *reinterpret_cast<f32x4v*>(h + F::at(n, c, q));
+                    const float* x = dh[n] + c * F::kVec + 4 * q;
+                    const f32x4v y = {x[0], x[1], x[2], x[3]};
+                    sum = i ? sum + y : y;
+                }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.N * C * kFewLanes / 4; i += kFewThreads) {
+        const int n = i / (C * kFewLanes / 4), c = i / (F::kQuads * kFewLanes) % F::kChunks, q = i / kFewLanes % F::kQuads;
+        const int d = (c * kFewLanes + i % kFewLanes) * F::kVec + 4 * q;
+        if (d < a.D4)
+            *reinterpret_cast<f32x4v*>(a.part_h + ((int64_t)blockIdx.x * a.N + n) * a.D4 + d) = *reinterpret_cast<const f32x4v*>(h + 4 * i);
+    }
+}
+
+// dh from the workgroups' parts: 16 pieces of a row a workgroup, each by 16 threads in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ce_few_sum_kernel(const float* part, int parts, int N, int D, int D4, T* out) {
+    constexpr int kCols = 16, kSlices = kThreads / kCols;
+    __shared__ f32x4v s[kSlices][kCols];
+    const int col = threadIdx.x % kCols, slice = threadIdx.x / kCols, pieces = D4 / 4;
+    const int i = blockIdx.x * kCols + col;
+    f32x4v v = {};
+    if (i < N * pieces)
+#pragma unroll 8
+        for (int n = slice; n < parts; n += kSlices) v += *reinterpret_cast<const f32x4v*>(part + ((int64_t)n * N * pieces + i) * 4);
+    s[slice][col] = v;
+    __syncthreads();
+    if (slice || i >= N * pieces) return;
+    for (int n = 1; n < kSlices; ++n) v += s[n][col];
+    const int d = i % pieces * 4;
+    T* to = out + (int64_t)(i / pieces) * D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (d + e < D) to[e] = (T)v[e];
+}
+
 // ---- host side ---------------------------------------------------------------------------
 
 // Cuts a workspace; with a null base only the size is wanted.
@@ -627,17 +871,20 @@ void choose_splits(int64_t tiles_h, int64_t k_h, int64_t tiles_w, int64_t k_w, i
         }
 }
 
+// Whether the scores' product takes a user's matrix without a copy.
+template <typename C>
+bool as_it_is(int64_t D, const void* x, int64_t ld) {
+    return C::kPlanes == 1 && D % C::Score::kStep == 0 && ((uintptr_t)x & 15) == 0 && ld % 8 == 0;
+}
+
 template <typename C>
 Plan plan_of(const mb_linear_ce* a) {
     Plan p = {};
     p.N = a->N, p.V = a->V, p.D = a->D;
     p.Dp = pad(p.D, kPad), p.Np = pad(p.N, kPad), p.Vp = pad(p.V, kPad);
     p.planes = C::kPlanes;
-    auto direct = [&](const void* x, int64_t ld) {
-        return p.planes == 1 && p.D % C::Score::kStep == 0 && ((uintptr_t)x & 15) == 0 && ld % 8 == 0;
-    };
     p.gather = p.N >= kGatherRows;
-    p.direct_h = !p.gather && direct(a->hidden, a->hidden_ld), p.direct_w = direct(a->weight, a->weight_ld);
+    p.direct_h = !p.gather && as_it_is<C>(p.D, a->hidden, a->hidden_ld), p.direct_w = as_it_is<C>(p.D, a->weight, a->weight_ld);
     p.tiles_p = (int)((p.V + C::Score::TP - 1) / C::Score::TP), p.tiles_q = (int)((p.N + C::Score::TQ - 1) / C::Score::TQ);
     p.width = std::min<int64_t>(pad(p.V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np * 2 * p.planes) / 256 * 256));
     choose_splits(tiles_of<typename C::GradH>(p.D, p.N), std::min(p.width, p.Vp), tiles_of<typename C::GradW>(p.D, std::min(p.width, p.V)), p.Np, p.s_h,
@@ -809,6 +1056,102 @@ int enough(const char* what, const mb_linear_ce* a, int64_t need) {
     return MB_OK;
 }
 
+// ---- up to eight rows, the host's part ----
+
+constexpr int kVectorRows = 8;
+constexpr int kFewStats = 512, kFewGrads = 256;      // workgroups, at most
+
+// Channels of a lane, and rows, of the kernels for these sizes; 0 where there are none.
+int few_channels(int64_t D, int size) {
+    for (int c = 16 / size; c <= 32; c *= 2)
+        if (c * kFewLanes >= D) return c;
+    return 0;
+}
+int few_rows(int64_t N) { return N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8; }
+// Both directions of one to eight rows (us, matrix instructions' kernels and these): fp32, 1 row on 128789 words of 256 395 and 131, 8 on
+// 50257 of 1024 458 and 158, 2 on 30000 of 2048 558 and 176; bf16, 5 on 100000 of 1024 327 and 181, 4 on 50257 of 2048 367 and 210, 2 on
+// 50257 of 101 146 and 127 (the host).  A bf16 forward that reads the weights as they are stays with the matrix instructions: 5 on
+// 100000 of 1024 41 and 50, 8 on 128000 of 256 25 and 39; with copies it does not, 2 on 50257 of 101 32 and 25.
+bool vector_rows(const mb_linear_ce* a, bool backward) {
+    const int c = few_channels(a->D, a->dtype == MB_DTYPE_F32 ? 4 : 2);
+    if (!backward && a->dtype == MB_DTYPE_BF16 && as_it_is<FewBf16>(a->D, a->weight, a->weight_ld)) return false;
+    return a->N <= kVectorRows && c && c * few_rows(a->N) <= 128;
+}
+
+struct FewBuffers {
+    float2* part;
+    float *target_score, *part_h;
+    double* sums;
+    int64_t bytes;
+};
+FewBuffers few_buffers(const mb_linear_ce* a, bool backward, void* base) {
+    Carve c = {(char*)base};
+    FewBuffers b = {};
+    if (backward) {
+        b.part_h = c.take<float>((int64_t)kFewGrads * a->N * pad(a->D, 4));
+    } else {
+        b.part = c.take<float2>((int64_t)kFewStats * a->N), b.target_score = c.take<float>(a->N), b.sums = c.take<double>(2);
+    }
+    b.bytes = c.used;
+    return b;
+}
+
+template <typename T, int R, int C>
+int few_launch(const char* what, FewArgs& f, bool backward, int& blocks, hipStream_t st) {
+    typedef Few<T, R, C> F;
+    const int64_t runs = ((int64_t)f.V + F::kWords - 1) / F::kWords, each = kFewThreads / 64;
+    blocks = (int)std::min<int64_t>(backward ? kFewGrads : kFewStats, (runs + each - 1) / each);
+    static_assert(F::kLds <= 65536, "no more than a kernel has without being told");
+    if (backward) hipLaunchKernelGGL((ce_few_grads_kernel<T, R, C>), dim3(blocks), dim3(kFewThreads), F::kLds, st, f);
+    else hipLaunchKernelGGL((ce_few_stats_kernel<T, R, C>), dim3(blocks), dim3(kFewThreads), F::kLds, st, f);
+    return check_launch(what);
+}
+template <typename T, int C>
+int few_by_rows(const char* what, FewArgs& f, bool backward, int& blocks, hipStream_t st) {
+    const int rows = few_rows(f.N);
+    if (rows == 1) return few_launch<T, 1, C>(what, f, backward, blocks, st);
+    if (rows == 2) return few_launch<T, 2, C>(what, f, backward, blocks, st);
+    if (rows == 4) return few_launch<T, 4, C>(what, f, backward, blocks, st);
+    if constexpr (8 * C <= 128) return few_launch<T, 8, C>(what, f, backward, blocks, st);
+    return fail(MB_ERR_UNSUPPORTED, "%s: %d rows of %d", what, f.N, f.D);
+}
+template <typename T>
+int few(const char* what, const mb_linear_ce* a, bool backward, hipStream_t st) {
+    const FewBuffers b = few_buffers(a, backward, a->workspace);
+    if (const int rc = enough(what, a, b.bytes)) return rc;
+    if (backward && !a->dhidden && !a->dweight) return MB_OK;
+    constexpr int vec = 16 / sizeof(T);
+    FewArgs f = {};
+    f.hidden = a->hidden, f.weight = a->weight, f.h_ld = a->hidden_ld, f.w_ld = a->weight_ld;
+    f.g = {{a->target, (int)a->target_bytes, a->ignore_index, a->V}, backward ? a->dloss : nullptr, a->count, (int)a->reduction};
+    f.N = (int)a->N, f.V = (int)a->V, f.D = (int)a->D, f.D4 = (int)pad(a->D, 4);
+    f.vec = ((uintptr_t)a->weight & 15) == 0 && a->weight_ld % vec == 0 && a->D % vec == 0;
+    f.part = b.part, f.target_score = b.target_score;
+    if (backward) {
+        f.lse = a->lse, f.part_h = a->dhidden ? b.part_h : nullptr, f.dweight = a->dweight;
+        f.out_vec = ((uintptr_t)a->dweight & 15) == 0 && a->D % vec == 0;
+    }
+    int blocks = 0, rc = MB_OK;
+    switch (few_channels(a->D, sizeof(T))) {
+        case 4: if constexpr (vec == 4) rc = few_by_rows<T, 4>(what, f, backward, blocks, st); break;
+        case 8: rc = few_by_rows<T, 8>(what, f, backward, blocks, st); break;
+        case 16: rc = few_by_rows<T, 16>(what, f, backward, blocks, st); break;
+        default: rc = few_by_rows<T, 32>(what, f, backward, blocks, st);
+    }
+    if (rc) return rc;
+    if (backward) {
+        if (a->dhidden)
+            hipLaunchKernelGGL((ce_few_sum_kernel<T>), dim3((unsigned)((a->N * f.D4 / 4 + 15) / 16)), dim3(kThreads), 0, st, (const float*)b.part_h,
+                               blocks, f.N, f.D, f.D4, (T*)a->dhidden);
+        return check_launch(what);
+    }
+    static_assert(kVectorRows <= kRowsPerBlock, "one workgroup joins");
+    const JoinArgs j = {b.part, b.target_score, f.g.t, {nullptr, nullptr, nullptr, f.N}, f.N, blocks, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
+    hipLaunchKernelGGL(ce_join_kernel, dim3(1), dim3(kThreads), 0, st, j);
+    if (a->reduction) hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(kThreads), 0, st, (const double*)b.sums, 1, (int)a->reduction, a->loss, a->count);
+    return check_launch(what);
+}
+
 template <typename C>
 int forward(const mb_linear_ce* a, hipStream_t st) {
     const Plan p = plan_of<C>(a);
@@ -881,6 +1224,7 @@ using namespace mb;
 
 extern "C" int64_t mb_linear_ce_workspace(const mb_linear_ce* a, int backward) {
     if (check("mb_linear_ce_workspace", a)) return -1;
+    if (vector_rows(a, backward != 0)) return few_buffers(a, backward != 0, nullptr).bytes;
     const bool few = a->N <= kFewRows;
     const Plan p = a->dtype == MB_DTYPE_F32 ? few ? plan_of<FewF32>(a) : plan_of<F32>(a) : few ? plan_of<FewBf16>(a) : plan_of<Bf16>(a);
     return buffers_of(p, backward != 0, nullptr).bytes;
@@ -890,6 +1234,7 @@ extern "C" int mb_linear_ce_fwd(const mb_linear_ce* a, void* stream) {
     if (const int rc = check("mb_linear_ce_fwd", a)) return rc;
     MB_REQUIRE(a->loss, "mb_linear_ce_fwd: null pointer argument");
     hipStream_t st = (hipStream_t)stream;
+    if (vector_rows(a, false)) return a->dtype == MB_DTYPE_F32 ? few<float>("mb_linear_ce_fwd", a, false, st) : few<__bf16>("mb_linear_ce_fwd", a, false, st);
     if (a->N <= kFewRows) return a->dtype == MB_DTYPE_F32 ? forward<FewF32>(a, st) : forward<FewBf16>(a, st);
     return a->dtype == MB_DTYPE_F32 ? forward<F32>(a, st) : forward<Bf16>(a, st);
 }
@@ -898,6 +1243,7 @@ extern "C" int mb_linear_ce_bwd(const mb_linear_ce* a, void* stream) {
     if (const int rc = check("mb_linear_ce_bwd", a)) return rc;
     MB_REQUIRE(a->dloss, "mb_linear_ce_bwd: null pointer argument");
     hipStream_t st = (hipStream_t)stream;
+    if (vector_rows(a, true)) return a->dtype == MB_DTYPE_F32 ? few<float>("mb_linear_ce_bwd", a, true, st) : few<__bf16>("mb_linear_ce_bwd", a, true, st);
     if (a->N <= kFewRows) return a->dtype == MB_DTYPE_F32 ? backward<FewF32>(a, st) : backward<FewBf16>(a, st);
     return a->dtype == MB_DTYPE_F32 ? backward<F32>(a, st) : backward<Bf16>(a, st);
 }

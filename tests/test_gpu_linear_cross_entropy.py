@@ -336,3 +336,73 @@ def test_refusals():
         linear_cross_entropy(h.cpu(), w, target)
     with pytest.raises(NotImplementedError):
         linear_cross_entropy(h, w, target.cpu())
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 8, 9])
+def test_few_rows(N, t):
+    """Up to eight rows have kernels of their own, by rows and by channels: each, and sizes on both sides of what they take."""
+    for V, D in ((3, 1), (33, 7), (64, 64), (1001, 101), (517, 256), (300, 257), (2050, 512), (129, 513), (1030, 1000), (515, 1024), (130, 1025),
+                 (259, 2047), (131, 2048), (70, 2049), (40003, 64)):
+        h, w, target = make(N, V, D, t, seed=N)
+        g = torch.Generator("cuda").manual_seed(N)
+        for reduction in ("mean", "none"):
+            dloss = 0.1 + torch.rand((N,) if reduction == "none" else (), generator=g, device="cuda")
+            check(call(h, w, target, reduction, dloss), definition(h, w, target, reduction, dloss), h, w, (V, D, reduction))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V,D", [(3, 700, 96), (8, 1003, 200), (4, 300, 1500), (8, 257, 1024)])
+def test_few_rows_at_the_edges(N, V, D, t):
+    from mathbrain.linear_cross_entropy import linear_cross_entropy
+    h, w, target = make(N, V, D, t, seed=9)
+    # ignored rows, with NaN in them; one gradient alone; the same twice
+    left = target.clone()
+    left[1] = IGN
+    hn = h.clone()
+    hn[1] = float("nan")
+    got, want = call(hn, w, left), definition(h, w, left, "mean")
+    check(got, want, h, w)
+    assert not got[1][1].any()
+    assert all(torch.equal(a, b) for a, b in zip(got, call(hn, w, left)))
+    for side in (0, 1):
+        x = [hn.clone(), w.clone()]
+        x[side].requires_grad_()
+        assert torch.equal(torch.autograd.grad(linear_cross_entropy(*x, left), x[side])[0], got[1 + side])
+    # all ignored; gradients of zero
+    loss, dh, dw = call(h, w, torch.full_like(target, IGN), "sum")
+    assert float(loss) == 0 and not dh.any() and not dw.any()
+    loss, dh, dw = call(h, w, target, "sum", torch.zeros((), device="cuda"))
+    assert not dh.any() and not dw.any()
+    # a target outside the vocabulary reaches its own row of dh and all of dw
+    out = target.clone()
+    out[0] = V
+    loss, dh, dw = call(h, w, out, "none")
+    assert torch.isnan(loss[0]) and not torch.isnan(loss[1:]).any()
+    assert torch.isnan(dh[0]).all() and not torch.isnan(dh[1:]).any() and torch.isnan(dw).all()
+    # rows that are further apart, and rows that begin anywhere
+    wide = torch.randn(V + 1, D + 9, device="cuda").to(t)
+    for at in (0, 1, 8):
+        wide[1:, at:at + D] = w
+        check(call(h, wide[1:, at:at + D], target), definition(h, w, target, "mean"), h, w, at)
+    # captured and replayed with other values
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+
+    def step():
+        loss = linear_cross_entropy(a, b, left)
+        return [loss.detach(), *torch.autograd.grad(loss, [a, b])]
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        with torch.no_grad():
+            a.mul_(0.9)
+            left.copy_(torch.where(torch.arange(N, device="cuda") == i, IGN, target))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(held, step()))
