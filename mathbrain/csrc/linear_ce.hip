@@ -548,23 +548,25 @@ __global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const
     }
 }
 
-// ---- up to eight rows --------------------------------------------------------------------
+// ---- few rows ----------------------------------------------------------------------------
 //
 // The time is the weights' read (and dw's write) then, so fp32 products from registers do: a wave takes a few words at a time, 16
 // bytes of each a lane and chunk, and reads hidden (fp32 in LDS) once for them.  The backward has the scores' words still in its
 // registers for dh, whose sums it keeps over all its words, and writes dw at once: w is read once a direction, without the copies
-// that the matrix instructions want.  A score's sum over the lanes leaves it with the lane whose number begins with it.
+// that the matrix instructions want.  One row on 128789 words of 256 in fp32: 22.6 us forward, 44.5 us backward, the weights' 132 MB at
+// 5.8 and (with dw) 5.9 TB/s; 5 rows on 100000 of 1024 in bf16 130.6 us backward, 3.1 TB/s (vector instructions).  A score's sum over the lanes leaves it with the lane whose number begins with it.
 constexpr int kFewThreads = 512;
 constexpr int kFewLanes = 64;
 struct FewArgs {
     const void *hidden, *weight;
     int64_t h_ld, w_ld;
     RowGrad g;
-    int N, V, D, vec, out_vec;
+    int n0, rows, N, V, D, vec, out_vec;   // the launch's rows, of all N
+    int n1, rows1;                // further rows, which count for dw alone
     float2* part;                 // forward: [workgroups, N] maximum and sum
     float* target_score;          // forward: [N]
     const float* lse;             // backward: [2, N]
-    float* part_h;                // backward: [workgroups, N, D4], or NULL
+    float* part_h;                // backward: [workgroups, rows, D4], or NULL
     int D4;
     void* dweight;                // backward: [V, D], or NULL
 };
@@ -588,11 +590,11 @@ struct Few {
     static __device__ int row() { return lane() / kEach % R; }
 
     // hidden in LDS, zeros in place of ignored rows and behind the end
-    static __device__ void stage(const FewArgs& a, float* h) {
+    static __device__ void stage(const FewArgs& a, int n0, int rows, float* h) {
         for (int i = threadIdx.x; i < R * C * kFewLanes; i += kFewThreads) {
             const int r = i / (C * kFewLanes), c = i / (kVec * kFewLanes) % kChunks, q = i / (4 * kFewLanes) % kQuads;
             const int d = (c * kFewLanes + i / 4 % kFewLanes) * kVec + 4 * q + i % 4;
-            h[i] = r < a.N && d < a.D && a.g.t.at(r) != -1 ? (float)((const T*)a.hidden)[r * a.h_ld + d] : 0.f;
+            h[i] = r < rows && d < a.D && a.g.t.at(n0 + r) != -1 ? (float)((const T*)a.hidden)[(n0 + r) * a.h_ld + d] : 0.f;
         }
         __syncthreads();
     }
@@ -645,6 +647,26 @@ struct Few {
         }
         return s[0] * kLog2e;
     }
+    // what this lane's row has to do with U, and all lanes' g U of the words
+    struct Row {
+        int target;
+        float g, m, l;
+        __device__ Row(const FewArgs& a, int n0, int rows) {
+            const int n = n0 + row();
+            target = row() < rows ? a.g.t.at(n) : -1;
+            const bool counts = target != -1;
+            g = counts ? a.g.at(n) : 0.f, m = counts ? a.lse[n] : 0.f, l = counts ? a.lse[a.N + n] : 0.f;
+        }
+    };
+    static __device__ void gradients(const FewArgs& a, const Row& o, const float* h, const vec_t (&w)[kWords][kChunks], int v0, float (&u)[kWords][R]) {
+        const int v = v0 + word();
+        float mine = __builtin_amdgcn_exp2f((score(h, w) - o.m) - o.l);
+        mine = v == o.target ? mine - 1.f : mine;
+        mine = v < a.V && o.g != 0.f ? mine * o.g : 0.f;
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            u[i / R][i % R] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i * kEach));
+    }
 };
 
 template <typename T, int R, int C>
@@ -652,9 +674,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewA
     typedef Few<T, R, C> F;
     extern __shared__ char smem[];
     float* h = (float*)smem;
-    F::stage(a, h);
+    F::stage(a, a.n0, a.rows, h);
     constexpr int kWaves = kFewThreads / 64;
-    const int wave = wave_id(), r = F::row(), target = r < a.N ? a.g.t.at(r) : -1;
+    const int wave = wave_id(), n = a.n0 + F::row(), target = F::row() < a.rows ? a.g.t.at(n) : -1;
     float m = -INFINITY, sum = 0.f;
     for (int64_t v0 = ((int64_t)blockIdx.x * kWaves + wave) * F::kWords; v0 < a.V; v0 += (int64_t)gridDim.x * kWaves * F::kWords) {
         typename F::vec_t w[F::kWords][F::kChunks];
@@ -662,7 +684,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewA
         const float s = F::score(h, w);
         const int v = (int)v0 + F::word();
         if (v >= a.V) continue;
-        if (v == target) a.target_score[r] = s;
+        if (v == target) a.target_score[n] = s;
         const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
         sum = sum * __builtin_amdgcn_exp2f(m - base) + __builtin_amdgcn_exp2f(s - base);
         m = top;
@@ -670,7 +692,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewA
     __shared__ float2 both[kWaves][F::M];
     if (F::lane() % F::kEach == 0) both[wave][F::lane() / F::kEach] = make_float2(m, sum);
     __syncthreads();
-    if ((int)threadIdx.x < a.N) {
+    if ((int)threadIdx.x < a.rows) {
         float top = -INFINITY, t = 0.f;
         for (int i = 0; i < kWaves * F::kWords; ++i) top = fmaxf(top, both[i / F::kWords][i % F::kWords * R + threadIdx.x].x);
         const float base = top == -INFINITY ? 0.f : top;
@@ -678,32 +700,28 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewA
             const float2 x = both[i / F::kWords][i % F::kWords * R + threadIdx.x];
             t += x.y * __builtin_amdgcn_exp2f(x.x - base);
         }
-        a.part[(int64_t)blockIdx.x * a.N + threadIdx.x] = make_float2(top, t);
+        a.part[(int64_t)blockIdx.x * a.N + a.n0 + threadIdx.x] = make_float2(top, t);
     }
 }
 
-template <typename T, int R, int C>
+// BOTH: dw of further rows too, whose dh another launch sums: nothing of dw is read again.
+template <typename T, int R, int C, bool BOTH>
 __global__ void __launch_bounds__(kFewThreads, 2) ce_few_grads_kernel(const FewArgs a) {
     typedef Few<T, R, C> F;
     extern __shared__ char smem[];
-    float* h = (float*)smem;
-    F::stage(a, h);
+    float *h = (float*)smem, *h1 = h + F::kLds / 4;
+    F::stage(a, a.n0, a.rows, h);
+    if (BOTH) F::stage(a, a.n1, a.rows1, h1);
     constexpr int kWaves = kFewThreads / 64;
-    const int wave = wave_id(), r = F::row(), target = r < a.N ? a.g.t.at(r) : -1;
-    const bool counts = target != -1;
-    const float g = counts ? a.g.at(r) : 0.f, m = counts ? a.lse[r] : 0.f, l = counts ? a.lse[a.N + r] : 0.f;
+    const int wave = wave_id();
+    const typename F::Row row(a, a.n0, a.rows), row1(a, a.n1, BOTH ? a.rows1 : 0);
     float dh[R][C] = {};
     for (int64_t v0 = ((int64_t)blockIdx.x * kWaves + wave) * F::kWords; v0 < a.V; v0 += (int64_t)gridDim.x * kWaves * F::kWords) {
         typename F::vec_t w[F::kWords][F::kChunks];
         F::load(a, (int)v0, w);
-        const int v = (int)v0 + F::word();
-        float mine = __builtin_amdgcn_exp2f((F::score(h, w) - m) - l);
-        mine = v == target ? mine - 1.f : mine;
-        mine = v < a.V && g != 0.f ? mine * g : 0.f;
-        float u[F::kWords][R];
-#pragma unroll
-        for (int i = 0; i < F::M; ++i)
-            u[i / R][i % R] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i * F::kEach));
+        float u[F::kWords][R], u1[F::kWords][R];
+        F::gradients(a, row, h, w, (int)v0, u);
+        if (BOTH) F::gradients(a, row1, h1, w, (int)v0, u1);
 #pragma unroll
         for (int c = 0; c < F::kChunks; ++c) {
             typename F::vec_t out[F::kWords];
@@ -722,6 +740,16 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_grads_kernel(const FewA
                             float& sum = dh[n][c * F::kVec + 4 * q + e];
                             sum = __builtin_fmaf(u[i][n], (float)w[i][c][4 * q + e], sum);
                         }
+                }
+                if (BOTH) {
+#pragma unroll
+                    for (int n = 0; n < R; ++n) {
+                        const f32x4v x = *reinterpret_cast<const f32x4v*>(h1 + F::at(n, c, q));
+#pragma unroll
+                        for (int i = 0; i < F::kWords; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) y[i][e] = __builtin_fmaf(u1[i][n], x[e], y[i][e]);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < F::kWords; ++i)
@@ -762,11 +790,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_grads_kernel(const FewA
                 }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < a.N * C * kFewLanes / 4; i += kFewThreads) {
+    for (int i = threadIdx.x; i < a.rows * C * kFewLanes / 4; i += kFewThreads) {
         const int n = i / (C * kFewLanes / 4), c = i / (F::kQuads * kFewLanes) % F::kChunks, q = i / kFewLanes % F::kQuads;
         const int d = (c * kFewLanes + i % kFewLanes) * F::kVec + 4 * q;
         if (d < a.D4)
-            *reinterpret_cast<f32x4v*>(a.part_h + ((int64_t)blockIdx.x * a.N + n) * a.D4 + d) = *reinterpret_cast<const f32x4v*>(h + 4 * i);
+            *reinterpret_cast<f32x4v*>(a.part_h + ((int64_t)blockIdx.x * a.rows + n) * a.D4 + d) = *reinterpret_cast<const f32x4v*>(h + 4 * i);
     }
 }
 
@@ -1056,9 +1084,9 @@ int enough(const char* what, const mb_linear_ce* a, int64_t need) {
     return MB_OK;
 }
 
-// ---- up to eight rows, the host's part ----
+// ---- few rows, the host's part ----
 
-constexpr int kVectorRows = 8;
+constexpr int kVectorRows = 8;                       // of a launch
 constexpr int kFewStats = 512, kFewGrads = 256;      // workgroups, at most
 
 // Channels of a lane, and rows, of the kernels for these sizes; 0 where there are none.
@@ -1067,15 +1095,22 @@ int few_channels(int64_t D, int size) {
         if (c * kFewLanes >= D) return c;
     return 0;
 }
+// Rows of a launch, at most (0: none).
+int launch_rows(int64_t D, int size) {
+    const int c = few_channels(D, size);
+    return c ? std::min(kVectorRows, 128 / c) : 0;
+}
 int few_rows(int64_t N) { return N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8; }
-// Both directions of one to eight rows (us, matrix instructions' kernels and these): fp32, 1 row on 128789 words of 256 395 and 131, 8 on
-// 50257 of 1024 458 and 158, 2 on 30000 of 2048 558 and 176; bf16, 5 on 100000 of 1024 327 and 181, 4 on 50257 of 2048 367 and 210, 2 on
-// 50257 of 101 146 and 127 (the host).  A bf16 forward that reads the weights as they are stays with the matrix instructions: 5 on
-// 100000 of 1024 41 and 50, 8 on 128000 of 256 25 and 39; with copies it does not, 2 on 50257 of 101 32 and 25.
+// A launch's rows; fp32 takes two launches a direction for twice as many, bf16 none (its matrix instructions' kernels read the weights
+// less often: 9 rows on 50257 of 512 120 us).  Both directions (us, matrix instructions' kernels and these): fp32, 1 row on 128789 words
+// of 256 395 and 131, 8 on 50257 of 1024 458 and 158, 2 on 30000 of 2048 558 and 176, 8 on 50257 of 2048 1100 and 629, 16 on 50257 of
+// 1024 458 and 290, 16 on 50257 of 512 248 and 172; bf16, 5 on 100000 of 1024 327 and 181, 4 on 50257 of 2048 367 and 210, 2 on 50257
+// of 101 146 and 127 (the host).  A bf16 forward that reads the weights as they are stays with the matrix instructions: 5 on 100000 of
+// 1024 41 and 50, 8 on 128000 of 256 25 and 39; with copies it does not, 2 on 50257 of 101 32 and 25.
 bool vector_rows(const mb_linear_ce* a, bool backward) {
-    const int c = few_channels(a->D, a->dtype == MB_DTYPE_F32 ? 4 : 2);
-    if (!backward && a->dtype == MB_DTYPE_BF16 && as_it_is<FewBf16>(a->D, a->weight, a->weight_ld)) return false;
-    return a->N <= kVectorRows && c && c * few_rows(a->N) <= 128;
+    const bool f32 = a->dtype == MB_DTYPE_F32;
+    if (!backward && !f32 && as_it_is<FewBf16>(a->D, a->weight, a->weight_ld)) return false;
+    return a->N <= (f32 ? 2 : 1) * launch_rows(a->D, f32 ? 4 : 2);
 }
 
 struct FewBuffers {
@@ -1097,23 +1132,27 @@ FewBuffers few_buffers(const mb_linear_ce* a, bool backward, void* base) {
 }
 
 template <typename T, int R, int C>
-int few_launch(const char* what, FewArgs& f, bool backward, int& blocks, hipStream_t st) {
+int few_launch(const char* what, const FewArgs& f, bool backward, int blocks, hipStream_t st) {
     typedef Few<T, R, C> F;
-    const int64_t runs = ((int64_t)f.V + F::kWords - 1) / F::kWords, each = kFewThreads / 64;
-    blocks = (int)std::min<int64_t>(backward ? kFewGrads : kFewStats, (runs + each - 1) / each);
-    static_assert(F::kLds <= 65536, "no more than a kernel has without being told");
-    if (backward) hipLaunchKernelGGL((ce_few_grads_kernel<T, R, C>), dim3(blocks), dim3(kFewThreads), F::kLds, st, f);
+    static_assert(2 * F::kLds <= 65536, "no more than a kernel has without being told");
+    if constexpr (sizeof(T) == 4 && R == std::min(kVectorRows, 128 / C)) {
+        if (backward && f.rows1) {
+            hipLaunchKernelGGL((ce_few_grads_kernel<T, R, C, true>), dim3(blocks), dim3(kFewThreads), 2 * F::kLds, st, f);
+            return check_launch(what);
+        }
+    }
+    if (backward) hipLaunchKernelGGL((ce_few_grads_kernel<T, R, C, false>), dim3(blocks), dim3(kFewThreads), F::kLds, st, f);
     else hipLaunchKernelGGL((ce_few_stats_kernel<T, R, C>), dim3(blocks), dim3(kFewThreads), F::kLds, st, f);
     return check_launch(what);
 }
 template <typename T, int C>
-int few_by_rows(const char* what, FewArgs& f, bool backward, int& blocks, hipStream_t st) {
-    const int rows = few_rows(f.N);
+int few_by_rows(const char* what, const FewArgs& f, bool backward, int blocks, hipStream_t st) {
+    const int rows = few_rows(f.rows);
     if (rows == 1) return few_launch<T, 1, C>(what, f, backward, blocks, st);
     if (rows == 2) return few_launch<T, 2, C>(what, f, backward, blocks, st);
     if (rows == 4) return few_launch<T, 4, C>(what, f, backward, blocks, st);
     if constexpr (8 * C <= 128) return few_launch<T, 8, C>(what, f, backward, blocks, st);
-    return fail(MB_ERR_UNSUPPORTED, "%s: %d rows of %d", what, f.N, f.D);
+    return fail(MB_ERR_UNSUPPORTED, "%s: %d rows of %d", what, f.rows, f.D);
 }
 template <typename T>
 int few(const char* what, const mb_linear_ce* a, bool backward, hipStream_t st) {
@@ -1131,21 +1170,30 @@ int few(const char* what, const mb_linear_ce* a, bool backward, hipStream_t st) 
         f.lse = a->lse, f.part_h = a->dhidden ? b.part_h : nullptr, f.dweight = a->dweight;
         f.out_vec = ((uintptr_t)a->dweight & 15) == 0 && a->D % vec == 0;
     }
-    int blocks = 0, rc = MB_OK;
-    switch (few_channels(a->D, sizeof(T))) {
-        case 4: if constexpr (vec == 4) rc = few_by_rows<T, 4>(what, f, backward, blocks, st); break;
-        case 8: rc = few_by_rows<T, 8>(what, f, backward, blocks, st); break;
-        case 16: rc = few_by_rows<T, 16>(what, f, backward, blocks, st); break;
-        default: rc = few_by_rows<T, 32>(what, f, backward, blocks, st);
+    // of every launch of the call, whose parts are joined together: one that finds no words has a sum of nothing
+    const int blocks = (int)std::min<int64_t>(backward ? kFewGrads : kFewStats, (a->V + kFewThreads / 32 - 1) / (kFewThreads / 32));
+    for (f.n0 = 0; f.n0 < f.N; f.n0 += f.rows) {
+        int rc = MB_OK;
+        f.rows = std::min(f.N - f.n0, launch_rows(a->D, sizeof(T)));
+        if (backward && f.n0) {      // dw has all rows from the first launch
+            f.dweight = nullptr, f.rows1 = 0;
+            if (!a->dhidden) break;
+        } else if (a->dweight) {
+            f.n1 = f.rows, f.rows1 = f.N - f.rows;
+        }
+        switch (few_channels(a->D, sizeof(T))) {
+            case 4: if constexpr (vec == 4) rc = few_by_rows<T, 4>(what, f, backward, blocks, st); break;
+            case 8: rc = few_by_rows<T, 8>(what, f, backward, blocks, st); break;
+            case 16: rc = few_by_rows<T, 16>(what, f, backward, blocks, st); break;
+            default: rc = few_by_rows<T, 32>(what, f, backward, blocks, st);
+        }
+        if (rc) return rc;
+        if (backward && a->dhidden)
+            hipLaunchKernelGGL((ce_few_sum_kernel<T>), dim3((unsigned)((f.rows * f.D4 / 4 + 15) / 16)), dim3(kThreads), 0, st, (const float*)b.part_h,
+                               blocks, f.rows, f.D, f.D4, (T*)a->dhidden + (int64_t)f.n0 * a->D);
     }
-    if (rc) return rc;
-    if (backward) {
-        if (a->dhidden)
-            hipLaunchKernelGGL((ce_few_sum_kernel<T>), dim3((unsigned)((a->N * f.D4 / 4 + 15) / 16)), dim3(kThreads), 0, st, (const float*)b.part_h,
-                               blocks, f.N, f.D, f.D4, (T*)a->dhidden);
-        return check_launch(what);
-    }
-    static_assert(kVectorRows <= kRowsPerBlock, "one workgroup joins");
+    if (backward) return check_launch(what);
+    static_assert(2 * kVectorRows <= kRowsPerBlock, "one workgroup joins");
     const JoinArgs j = {b.part, b.target_score, f.g.t, {nullptr, nullptr, nullptr, f.N}, f.N, blocks, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
     hipLaunchKernelGGL(ce_join_kernel, dim3(1), dim3(kThreads), 0, st, j);
     if (a->reduction) hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(kThreads), 0, st, (const double*)b.sums, 1, (int)a->reduction, a->loss, a->count);

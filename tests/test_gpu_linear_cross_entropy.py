@@ -339,9 +339,10 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 8, 9, 13, 16, 17])
 def test_few_rows(N, t):
-    """Up to eight rows have kernels of their own, by rows and by channels: each, and sizes on both sides of what they take."""
+    """Few rows have kernels of their own, by rows and by channels, in fp32 twice a call for up to 16 rows: each, and sizes on both sides of
+    what they take."""
     for V, D in ((3, 1), (33, 7), (64, 64), (1001, 101), (517, 256), (300, 257), (2050, 512), (129, 513), (1030, 1000), (515, 1024), (130, 1025),
                  (259, 2047), (131, 2048), (70, 2049), (40003, 64)):
         h, w, target = make(N, V, D, t, seed=N)
@@ -352,7 +353,7 @@ def test_few_rows(N, t):
 
 
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("N,V,D", [(3, 700, 96), (8, 1003, 200), (4, 300, 1500), (8, 257, 1024)])
+@pytest.mark.parametrize("N,V,D", [(3, 700, 96), (8, 1003, 200), (4, 300, 1500), (8, 257, 1024), (13, 301, 101), (16, 1003, 1024), (7, 200, 2048)])
 def test_few_rows_at_the_edges(N, V, D, t):
     from mathbrain.linear_cross_entropy import linear_cross_entropy
     h, w, target = make(N, V, D, t, seed=9)
