@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const
 // bytes of each a lane and chunk, and reads hidden (fp32 in LDS) once for them.  The backward has the scores' words still in its
 // registers for dh, whose sums it keeps over all its words, and writes dw at once: w is read once a direction, without the copies
 // that the matrix instructions want.  One row on 128789 words of 256 in fp32: 22.6 us forward, 44.5 us backward, the weights' 132 MB at
-// 5.8 and (with dw) 5.9 TB/s; 5 rows on 100000 of 1024 in bf16 130.6 us backward, 3.1 TB/s (vector instructions).  A score's sum over the lanes leaves it with the lane whose number begins with it.
+// 5.8 and (with dw) 5.9 TB/s, partly out of the last-level cache; 5 rows on 100000 of 1024 in bf16 130.6 us backward, 3.1 TB/s (vector instructions).  A score's sum over the lanes leaves it with the lane whose number begins with it.
 constexpr int kFewThreads = 512;
 constexpr int kFewLanes = 64;
 struct FewArgs {
