@@ -35,13 +35,16 @@ def rotary_tables(dim, positions, theta=10000.0, scaling=None, factor=1.0, train
     angle by the factor; "ntk" raises theta by factor^(dim / (dim - 2)), which keeps the fastest pair and divides the
     slowest by the factor; "yarn" divides the angles of the pairs that turn less than ``slow`` times within the
     ``trained`` positions, keeps those that turn more than ``fast`` times, goes from one to the other linearly over the
-    pairs between, and multiplies both tables by 0.1 ln(factor) + 1."""
+    pairs between (the ends of that range rounded outwards to whole pairs; the range may end beyond the last pair, which
+    is then divided in part), and multiplies both tables by 0.1 ln(factor) + 1."""
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary_tables: dim={dim} (an even number of channels, at least 2)")
     if scaling not in (None, "linear", "ntk", "yarn"):
         raise ValueError(f"rotary_tables: scaling={scaling!r} (None, 'linear', 'ntk' or 'yarn')")
     if not (factor >= 1.0 and math.isfinite(factor)):
         raise ValueError(f"rotary_tables: factor={factor} (1 or more)")
+    if not (theta > 0.0 and math.isfinite(theta)):
+        raise ValueError(f"rotary_tables: theta={theta} (above 0)")
     if scaling == "ntk":
         if dim < 4:
             raise ValueError("rotary_tables: 'ntk' wants dim of 4 or more")
@@ -53,11 +56,15 @@ def rotary_tables(dim, positions, theta=10000.0, scaling=None, factor=1.0, train
     elif scaling == "yarn":
         if trained is None or trained < 1:
             raise ValueError("rotary_tables: 'yarn' wants the number of trained positions")
+        if not (theta > 1.0 and fast >= slow > 0.0 and math.isfinite(fast)):
+            raise ValueError(f"rotary_tables: theta={theta}, fast={fast}, slow={slow} ('yarn' wants theta above 1 and fast >= slow > 0)")
         # pair (dim / 2) log(trained / (2 pi n)) / log(theta) turns n times within the trained positions
         first, last = (dim / 2 * math.log(trained / (2 * math.pi * n)) / math.log(theta) for n in (fast, slow))
-        first, last = max(math.floor(first), 0), min(math.ceil(last), dim // 2 - 1)
+        first, last = max(math.floor(first), 0), min(math.ceil(last), dim - 1)
         pair = torch.arange(dim // 2, dtype=torch.float64, device=device)
         share = ((pair - first) / max(last - first, 1e-3)).clamp(0, 1)
+        if last <= 0:      # the fastest pair, too, turns less than that
+            share.fill_(1.0)
         rate = rate * (1 - share) + rate / factor * share
         size = 0.1 * math.log(factor) + 1.0
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * rate
