@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _lib
 from .bias_attention import relative_bias_attention
 from .linear_cross_entropy import linear_cross_entropy
 from .model import RMSNorm, SwiGLU
@@ -46,6 +47,17 @@ def rotate(x, cos, sin):
     c = cos[None, :, None, :]
     s = sin[None, :, None, :]
     return torch.stack((a * c - b * s, a * s + b * c), dim=-1).flatten(-2).type_as(x)
+
+
+def _on_the_kernel(q, cos, sin):
+    """Whether apply_rotary takes the rotation of q by these tables: plain GPU tensors in fp32 or bf16, tables of fp32 at most
+    that get no derivative and have a row for every position, and no torch.func transform.  Everything else goes through
+    ``rotate``'s tensor operations."""
+    return (q.is_cuda and type(q) is torch.Tensor and q.dtype in (torch.float32, torch.bfloat16)
+            and all(t.dtype is not torch.float64 and t.shape[0] >= q.shape[1] and not (t.requires_grad and torch.is_grad_enabled())
+                    for t in (cos, sin))
+            and (torch.compiler.is_compiling()
+                 or (torch._C._functorch.peek_interpreter_stack() is None and not _lib.has_tangent(cos, sin))))
 
 
 class CausalSelfAttention(nn.Module):
@@ -77,11 +89,12 @@ class CausalSelfAttention(nn.Module):
         if self.qk_norm:
             q, k = qk_norm_rotary(q, k, self.q_norm.weight, self.k_norm.weight, cos.float(), sin.float(),
                                   self.q_norm.eps)
-        elif q.dtype in (torch.float32, torch.bfloat16):
-            q, k = apply_rotary(q, k, cos.float(), sin.float(), layout=self.rope_layout)
+        elif _on_the_kernel(q, cos, sin):
+            q, k = apply_rotary(q, k, cos.float().contiguous(), sin.float().contiguous(), layout=self.rope_layout)
         else:
             if self.rope_layout != "interleaved" or 2 * cos.shape[1] != self.head_dim:
-                raise ValueError(f"CausalSelfAttention: rope_layout and rope_dims take float32 or bfloat16 (got {q.dtype})")
+                raise ValueError("CausalSelfAttention: rope_layout and rope_dims take float32 or bfloat16 on the GPU, tables without "
+                                 f"gradients and no torch.func transform (got {q.dtype} on {q.device})")
             q, k = rotate(q, cos, sin), rotate(k, cos, sin)
         q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = self.wv(x).view(shape).transpose(1, 2)
