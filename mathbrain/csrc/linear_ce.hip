@@ -35,6 +35,12 @@ constexpr int kMaxBlocks = 2048;     // of the kernels that look for the largest
 constexpr int kRowRuns = 512;       // of the kernel that finds the rows' places
 constexpr int kRowsPerBlock = 16;   // of the joining kernel
 
+// A score in units of log 2, rounded: unrounded in a difference with a maximum that is, a large score would lie above its own maximum.
+__device__ inline float in_log2(float x, float f) {
+#pragma clang fp contract(off)
+    return x * f;
+}
+
 struct Targets {
     const void* target;
     int bytes;
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const 
         for (int i = 0; i < P::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float s = prod.acc[i][j][r] * f;
+                float s = in_log2(prod.acc[i][j][r], f);
                 if (tail && p0 + P::row(i, r) >= a.V) s = -INFINITY;
                 prod.acc[i][j][r] = s;
                 m[j] = fmaxf(m[j], s);
@@ -407,7 +413,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const Scor
                 f16x4 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float u = __builtin_amdgcn_exp2f((prod.acc[i][j][r + e] * f - m) - l);
+                    float u = __builtin_amdgcn_exp2f((in_log2(prod.acc[i][j][r + e], f) - m) - l);
                     u = v + e == target ? u - 1.f : u;
                     u = counts && v + e < a.v1 ? u * kUScale : 0.f;
                     if constexpr (PL == 2) {
@@ -645,7 +651,7 @@ struct Few {
                 }
             }
         }
-        return s[0] * kLog2e;
+        return in_log2(s[0], kLog2e);
     }
     // what this lane's row has to do with U, and all lanes' g U of the words
     struct Row {
