@@ -16,8 +16,8 @@
 // bf16 would round them to 8), w is exact down to 2^-31 of the matrix's largest value (8 bits above fp16's smallest step,
 // 2^-24, after scaling to 2^14 and more) and off by at most 2^-39 of that below.  For fp32 tensors they are two planes (24 bits).
 //
-// Scores are in units of log 2 (s log2 e, rounded once); a row's sum is kept as maximum and logarithm, two floats,
-// so that neither the loss nor a probability rounds their sum.
+// A row's sum of exponentials is kept as maximum and logarithm (of base 2), two floats, so that neither the loss nor a
+// probability rounds their sum.
 #include "gemm16.h"
 
 #include <algorithm>
@@ -35,11 +35,8 @@ constexpr int kMaxBlocks = 2048;     // of the kernels that look for the largest
 constexpr int kRowRuns = 512;       // of the kernel that finds the rows' places
 constexpr int kRowsPerBlock = 16;   // of the joining kernel
 
-// A score in units of log 2, rounded: unrounded in a difference with a maximum that is, a large score would lie above its own maximum.
-__device__ inline float in_log2(float x, float f) {
-#pragma clang fp contract(off)
-    return x * f;
-}
+// e^x.  Scores are natural ones, and the difference is taken before the factor: of equal scores it is 0, however large they are.
+__device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 struct Targets {
     const void* target;
@@ -246,7 +243,7 @@ struct ScoreArgs {
 
 template <typename P>
 __device__ inline float score_factor(const ScoreArgs& a) {
-    return a.scale_w ? (1.f / *a.scale_w) * (1.f / *a.scale_h) * kLog2e : kLog2e;
+    return a.scale_w ? (1.f / *a.scale_w) * (1.f / *a.scale_h) : 1.f;
 }
 
 // Matrix instructions bound it: 28672 rows, 50257 words of 512 in bf16 1.57 - 1.61 ms, 916 - 941 TFLOP/s; 16 rows 13.8 us, the weights' 51 MB at
@@ -273,7 +270,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const 
         for (int i = 0; i < P::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float s = in_log2(prod.acc[i][j][r], f);
+                float s = prod.acc[i][j][r] * f;
                 if (tail && p0 + P::row(i, r) >= a.V) s = -INFINITY;
                 prod.acc[i][j][r] = s;
                 m[j] = fmaxf(m[j], s);
@@ -284,7 +281,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const 
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) t += __builtin_amdgcn_exp2f(prod.acc[i][j][r] - base);
+            for (int r = 0; r < 16; ++r) t += exp_of(prod.acc[i][j][r] - base);
         sum[j] = t + __shfl_xor(t, 32, 64);
         // the target's score, from the lane that holds it
         const int at = target - p0 - P::wave_p();
@@ -309,7 +306,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const 
             for (int w = 1; w < P::kWavesP; ++w) top = fmaxf(top, both[w * P::TQ + c].x);
             const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int w = 0; w < P::kWavesP; ++w) t += both[w * P::TQ + c].y * __builtin_amdgcn_exp2f(both[w * P::TQ + c].x - base);
+            for (int w = 0; w < P::kWavesP; ++w) t += both[w * P::TQ + c].y * exp_of(both[w * P::TQ + c].x - base);
             a.part[(int64_t)tp * a.N + q0 + c] = make_float2(top, t);
         }
 }
@@ -333,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) ce_join_kernel(const JoinArgs a) {
     float m = -INFINITY, sum = 0.f;
     auto take = [&](float2 x) {
         const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.f : top;
-        sum = sum * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+        sum = sum * exp_of(m - base) + x.y * exp_of(x.x - base);
         m = top;
     };
     const int place = n < a.N ? a.r.of(n) : -1;
@@ -350,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) ce_join_kernel(const JoinArgs a) {
             const int target = a.t.at(n);
             counts = target != -1;
             const float l = __builtin_log2f(sum);
-            if (counts) loss = target < 0 ? NAN : kLn2 * ((m - a.target_score[place]) + l);
+            if (counts) loss = target < 0 ? NAN : (m - a.target_score[place]) + kLn2 * l;
             a.lse[n] = target < 0 && counts ? NAN : m;     // a target outside the vocabulary: NaN, in the gradients too
             a.lse[a.N + n] = l;
             if (a.reduction == 0) a.loss[n] = loss;
@@ -413,7 +410,7 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const Scor
                 f16x4 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float u = __builtin_amdgcn_exp2f((in_log2(prod.acc[i][j][r + e], f) - m) - l);
+                    float u = __builtin_amdgcn_exp2f((prod.acc[i][j][r + e] * f - m) * kLog2e - l);
                     u = v + e == target ? u - 1.f : u;
                     u = counts && v + e < a.v1 ? u * kUScale : 0.f;
                     if constexpr (PL == 2) {
@@ -620,7 +617,7 @@ struct Few {
             }
         }
     }
-    // this lane's score, in units of log 2
+    // this lane's score
     static __device__ float score(const float* h, const vec_t (&w)[kWords][kChunks]) {
         float s[M] = {};
 #pragma unroll
@@ -651,7 +648,7 @@ struct Few {
                 }
             }
         }
-        return in_log2(s[0], kLog2e);
+        return s[0];
     }
     // what this lane's row has to do with U, and all lanes' g U of the words
     struct Row {
@@ -666,7 +663,7 @@ struct Few {
     };
     static __device__ void gradients(const FewArgs& a, const Row& o, const float* h, const vec_t (&w)[kWords][kChunks], int v0, float (&u)[kWords][R]) {
         const int v = v0 + word();
-        float mine = __builtin_amdgcn_exp2f((score(h, w) - o.m) - o.l);
+        float mine = __builtin_amdgcn_exp2f((score(h, w) - o.m) * kLog2e - o.l);
         mine = v == o.target ? mine - 1.f : mine;
         mine = v < a.V && o.g != 0.f ? mine * o.g : 0.f;
 #pragma unroll
@@ -692,7 +689,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewA
         if (v >= a.V) continue;
         if (v == target) a.target_score[n] = s;
         const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-        sum = sum * __builtin_amdgcn_exp2f(m - base) + __builtin_amdgcn_exp2f(s - base);
+        sum = sum * exp_of(m - base) + exp_of(s - base);
         m = top;
     }
     __shared__ float2 both[kWaves][F::M];
@@ -704,7 +701,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_stats_kernel(const FewA
         const float base = top == -INFINITY ? 0.f : top;
         for (int i = 0; i < kWaves * F::kWords; ++i) {
             const float2 x = both[i / F::kWords][i % F::kWords * R + threadIdx.x];
-            t += x.y * __builtin_amdgcn_exp2f(x.x - base);
+            t += x.y * exp_of(x.x - base);
         }
         a.part[(int64_t)blockIdx.x * a.N + a.n0 + threadIdx.x] = make_float2(top, t);
     }
