@@ -722,8 +722,10 @@ int mb_bias_attn_bwd(const mb_bias_attn *args, void *stream);
  *   s_nv = hidden_n . weight_v,  loss_n = log sum_v exp(s_nv) - s_n,target(n)
  *   dhidden_n = g_n sum_v (softmax(s_n)_v - [v = target]) weight_v,  dweight_v = sum_n (...) g_n hidden_n
  *
- * Products of bf16 values are exact; fp32 values go as two fp16 planes (24 bits).  Sums have a fixed order.
- * The arguments come in a struct on the HOST, read before the call returns.
+ * Products of bf16 values are exact; fp32 values go as two fp16 planes (24 bits down to 2^-16 of the largest value of
+ * a row of hidden or weight, and of the largest term of the row's or word's sum in a gradient; smaller ones are off by
+ * 2^-39 of it).  bf16 gradients take softmax - [v = target] in 11 bits, with steps of 2^-39 at least.  Sums have a
+ * fixed order.  The arguments come in a struct on the HOST, read before the call returns.
  */
 typedef struct mb_linear_ce {
     const void *hidden, *weight;  /* [N, D], [V, D], elements of a row next to each other, rows */

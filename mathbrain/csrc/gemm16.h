@@ -2,9 +2,9 @@
 //
 //   acc[p][q] = sum_k P[p][k] Q[q][k],  fp32 accumulation in the 32 x 32 x 16 matrix instructions
 //
-// One plane: bf16 or fp16 values.  Two planes: fp32 values as x = hi + lo, both fp16 (24 bits of x
-// where it is within 2^-17 of the matrix's largest, see plane_scale), from three products
-// lo hi + hi lo + hi hi; the fourth is below fp32's own rounding.
+// One plane: bf16 or fp16 values.  Two planes: fp32 values as x = hi + lo, both fp16 (24 bits down
+// to 2^-16 of the largest value, see below), from three products lo hi + hi lo + hi hi; the fourth is
+// below fp32's own rounding.
 //
 // A workgroup of four or eight waves takes a TP x TQ tile of the result and walks k in steps of 32 or 64.  Operand tiles go
 // from memory straight into LDS, kStages - 1 steps ahead, 16 bytes a lane.  Such a
@@ -353,9 +353,10 @@ struct Product {
 
 // ---- planes ------------------------------------------------------------------------------
 //
-// fp16 holds 11 bits within 2^-14 .. 65504 and 24 - k below 2^-14 2^-k; a matrix is scaled by the power of two that
-// brings its largest value to 2^14 .. 2^15, so that one plane holds bf16 values exactly down to 2^-21 of the largest
-// and within 2^-39 of the largest below, and two planes hold fp32 values to 24 bits down to 2^-15 of the largest.
+// fp16 holds 11 bits within 2^-14 .. 65504, and multiples of 2^-24 below.  With the power of two that brings the largest value
+// to 2^14 .. 2^15 one plane holds bf16 values (8 bits) exactly from 2^-17 on, down to 2^-31 of the largest; two planes are off
+// by 2^-23 of a value from 2^-2 on (lo's half step is 2^-25 at least), down to 2^-16 of the largest.  Smaller values are off by 2^-25, 2^-39
+// of the largest, in either.
 
 // The scale for a largest (finite) magnitude of these bits: 2^-46 to 2^74.
 __device__ inline float plane_scale(uint32_t bits) {

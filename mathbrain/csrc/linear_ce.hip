@@ -8,19 +8,25 @@
 // Bound by the matrix instructions (gemm16.h).  Forward: workgroups take tiles of vocabulary x rows; a lane holds
 // the tile's vocabulary entries of a row in registers, so the tile's maximum and sum of exponentials need one
 // exchange; they go to memory, two floats for a tile's row, and a second kernel joins them in a fixed order.
-// Backward, for pieces of the vocabulary: the tile again, U as 16-bit planes to memory (U is within [-1, 1]: scaled
-// by 2^15, without g, whatever the gradient's size), then the two products with it.  Recomputing the scores takes
-// the time of one product; keeping them would take N V values.
+// Backward, for pieces of the vocabulary: the tile again, U as 16-bit planes to memory, then the two products with it.
+// Recomputing the scores takes the time of one product; keeping them would take N V values.
 //
-// For bf16 tensors U, w and g h are single fp16 planes: U and g h are rounded to 11 bits (elementwise tensor operations in
-// bf16 would round them to 8), w is exact down to 2^-31 of the matrix's largest value (8 bits above fp16's smallest step,
-// 2^-24, after scaling to 2^14 and more) and off by at most 2^-39 of that below.  For fp32 tensors they are two planes (24 bits).
+// For bf16 tensors U (times 2^15), w and g h (each matrix times one power of two) are single fp16 planes: U and g h are rounded
+// to 11 bits (elementwise tensor operations in bf16 would round them to 8), w is exact down to 2^-31 of the matrix's largest
+// value (plane_scale).  U's step is never below 2^-39: a probability has the 8 bits of a bf16 result down to 2^-32, and
+// one below 2^-40 counts as none, so dw of a word that improbable in every row is zero.
+//
+// For fp32 tensors they are two fp16 planes, 24 bits, with a power of two for every row of hidden and of the weights, and for
+// every row and word of a tile of U (scaled_u): what is held is as exact as fp32 down to 2^-16 of the largest value of its own row
+// (or of its word's or row's terms in the sum), whatever other rows and words hold.
 //
 // A row's sum of exponentials is kept as maximum and logarithm (of base 2), two floats, so that neither the loss nor a
 // probability rounds their sum.
 #include "gemm16.h"
 
 #include <algorithm>
+#include <climits>
+#include <cstdint>
 
 namespace mb {
 namespace {
@@ -34,6 +40,7 @@ constexpr float kUScale = 32768.f;
 constexpr int kMaxBlocks = 2048;     // of the kernels that look for the largest value
 constexpr int kRowRuns = 512;       // of the kernel that finds the rows' places
 constexpr int kRowsPerBlock = 16;   // of the joining kernel
+constexpr int kLeastExp = -126;     // of a row of fp32 values
 
 // e^x.  Scores are natural ones, and the difference is taken before the factor: of equal scores it is 0, however large they are.
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -122,6 +129,7 @@ struct Matrix {
     float* largest;              // the largest magnitudes of the workgroups' parts; copies without: not scaled
     int blocks, copy_blocks;
     float* scale;
+    int* exps;                   // of the rows' copies
     void* out;                   // planes [rows_pad, Dp]
     int rows_pad, Dp, gathered;  // gathered: rows in their places of Rows
 };
@@ -171,8 +179,8 @@ __device__ inline float scale_from(const float* part, int n) {
     return plane_scale(__builtin_bit_cast(uint32_t, block_max(m)));
 }
 
-// x (graded: g_n x_n) as PL planes [rows_pad, Dp] of O, zeros around it, scaled by its largest value, which goes to *scale.
-template <typename T, typename O, int PL>
+// x (graded: g_n x_n) as a plane [rows_pad, Dp] of O, zeros around it, scaled by its largest value, which goes to *scale.
+template <typename T, typename O>
 __global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Set a) {
     int block;
     const Matrix& x = a.mine(block);
@@ -195,19 +203,53 @@ __global__ void __launch_bounds__(kThreads) ce_planes_kernel(const Set a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = gn == 0.f ? 0.f : v[e] * gn * s;
         }
-        vec8 hi, lo;
+        vec8 y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (PL == 2) {
-                _Float16 h, l;
-                split(v[e], h, l);
-                hi[e] = h, lo[e] = l;
-            } else {
-                hi[e] = (O)v[e];
-            }
+        for (int e = 0; e < 8; ++e) y[e] = (O)v[e];
+        *reinterpret_cast<vec8*>(out + n * x.Dp + d) = y;
+    }
+}
+
+// fp32 rows as two fp16 planes [rows_pad, Dp], zeros around them and in place of ignored rows; each row by its own power of
+// two, 2^(14 - exps[n]), which brings its largest finite value to 2^14 .. 2^15.  A wave a row; the second read comes out of the caches.
+__global__ void __launch_bounds__(kThreads) ce_row_planes_kernel(const Set a) {
+    int block;
+    const Matrix& x = a.mine(block);
+    const int lane = threadIdx.x & 63, count = x.gathered ? a.r.count() : x.rows;
+    _Float16* out = (_Float16*)x.out;
+    for (int64_t n = (int64_t)block * (kThreads / 64) + wave_id(); n < x.rows_pad; n += (int64_t)x.copy_blocks * (kThreads / 64)) {
+        bool there = n < count;
+        int64_t row = 0;
+        if (there) {
+            row = x.gathered ? a.r.at((int)n) : n;
+            there = !x.graded || a.g.t.at(row) != -1;
         }
-        *reinterpret_cast<vec8*>(out + n * x.Dp + d) = hi;
-        if constexpr (PL == 2) *reinterpret_cast<vec8*>(out + ((int64_t)x.rows_pad + n) * x.Dp + d) = lo;
+        const float* from = (const float*)x.p + row * x.ld;
+        float most = 0.f, v[8];
+        if (there)
+#pragma unroll 4
+            for (int d = lane * 8; d < x.D; d += 512) {
+                load8(from + d, x.vec, x.D - d, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+            }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+        const int exp = std::max(kLeastExp, (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127);
+        if (lane == 0) x.exps[n] = exp;
+#pragma unroll 4
+        for (int d = lane * 8; d < x.Dp; d += 512) {
+            if (there) load8(from + d, x.vec, x.D - d, v);
+            f16x8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                _Float16 h, l;
+                split(there ? __builtin_amdgcn_ldexpf(v[e], 14 - exp) : 0.f, h, l);
+                hi[e] = h, lo[e] = l;
+            }
+            *reinterpret_cast<f16x8*>(out + n * x.Dp + d) = hi;
+            *reinterpret_cast<f16x8*>(out + ((int64_t)x.rows_pad + n) * x.Dp + d) = lo;
+        }
     }
 }
 
@@ -229,22 +271,44 @@ inline unsigned tile_grid(int64_t tiles) { return (unsigned)pad(tiles, kXcds); }
 
 struct ScoreArgs {
     Side w, h;                    // kRows: [V, Dp], [N, Dp]
-    const float *scale_w, *scale_h;   // NULL: 1
-    Targets t;
+    const int *exp_w, *exp_h;     // fp32: the rows' exponents
+    RowGrad g;
     Rows r;
     int V, N, Dp, tiles_p;
     float2* part;                 // forward: [tiles_p, N] maximum and sum
     float* target_score;          // forward: [N]
     const float* lse;             // backward: [2, N]
-    _Float16* u;                  // backward: [PL][rows, width], the piece's entries from v0 on
+    _Float16* u;                  // backward: [PL][rows, width], the piece's entries from v0 on; fp32: for dh
+    _Float16* u_w;                // fp32: the same for dw
+    int *exps_h, *exps_w;         // fp32: [tiles of the vocabulary, Np] and [tiles of rows, width]
+    int Np;
     int v0, v1;
     int64_t plane, width;         // elements to the second plane, and to the next row
 };
 
+// fp32 operands are planes scaled row by row: the scores have the exponents of both.
 template <typename P>
-__device__ inline float score_factor(const ScoreArgs& a) {
-    return a.scale_w ? (1.f / *a.scale_w) * (1.f / *a.scale_h) : 1.f;
-}
+constexpr bool kScaled = std::is_same<typename P::T, _Float16>::value;
+struct alignas(16) Int4 {
+    int v[4];
+};
+// The exponents of this lane's words (the array has whole tiles; what lies behind the vocabulary is not used).
+template <typename P>
+struct WordExps {
+    Int4 v[P::FP][4];
+    __device__ WordExps(const ScoreArgs& a, int p0) {
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                if constexpr (kScaled<P>) v[i][r / 4] = *reinterpret_cast<const Int4*>(a.exp_w + p0 + P::row(i, r));
+    }
+    __device__ int at(int i, int r) const { return kScaled<P> ? v[i][r / 4].v[r % 4] : 0; }
+};
+template <typename P>
+__device__ inline int row_exp(const ScoreArgs& a, int place, int count) { return kScaled<P> && place < count ? a.exp_h[place] : 0; }
+template <typename P>
+__device__ inline float score_of(float sum, int exps) { return kScaled<P> ? __builtin_amdgcn_ldexpf(sum, exps - 28) : sum; }
 
 // Matrix instructions bound it: 28672 rows, 50257 words of 512 in bf16 1.57 - 1.61 ms, 916 - 941 TFLOP/s; 16 rows 13.8 us, the weights' 51 MB at
 // 3.7 TB/s.
@@ -256,21 +320,21 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const 
     if (!tile_of(a.tiles_p, (count + P::TQ - 1) / P::TQ, tp, tq)) return;
     const int p0 = tp * P::TP, q0 = tq * P::TQ;
     P prod;
-    const float f = score_factor<P>(a);
     prod.run(a.w, Side{a.h.p, a.h.plane, a.h.ld, count}, p0, q0, 0, a.Dp, smem);
     float2* both = (float2*)smem;   // [2][TQ]
     float m[P::FQ], sum[P::FQ];
     const bool tail = p0 + P::TP > a.V;
+    const WordExps<P> exps(a, p0);
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j) {
-        const int n = q0 + P::col(j);
-        const int target = n < count ? a.t.at(a.r.at(n)) : -1;
+        const int n = q0 + P::col(j), exp = row_exp<P>(a, n, count);
+        const int target = n < count ? a.g.t.at(a.r.at(n)) : -1;
         m[j] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float s = prod.acc[i][j][r] * f;
+                float s = score_of<P>(prod.acc[i][j][r], exp + exps.at(i, r));
                 if (tail && p0 + P::row(i, r) >= a.V) s = -INFINITY;
                 prod.acc[i][j][r] = s;
                 m[j] = fmaxf(m[j], s);
@@ -382,10 +446,131 @@ __global__ void __launch_bounds__(kThreads) ce_total_kernel(const double* sums, 
     }
 }
 
+// U in fp32, as two fp16 planes, twice: the words' sum (dh) wants every row's largest term near the top of the planes' range, the rows' sum
+// (dw) every word's.  So a tile's values have a power of two for each row in the one copy and for each word in the other, with which go the
+// exponents of what they are multiplied with: the planes of w and hidden have largest values of 2^14 .. 2^15 in every row.
+//
+//   y = U 2^(exp_w(v) + 15 - E(n)),      sum_v U w_v   = 2^(E(n) - 29) sum_v y w'_v
+//   y = U g 2^(exp_h(n) + 15 - E(v)),    sum_n U g h_n = 2^(E(v) - 29) sum_n y h'_n       (U with its factor of 2^15)
+// A word that is improbable in every row keeps its 24 bits so, and rows (or words) beside one of another size theirs.  One copy with one
+// power of two would be less to write: 2865 rows, 20011 words of 384 218 us against 283, both gradients' products 337 against 373 (run_scaled),
+// but a word's probabilities of 4e-11 are left with 7 bits there, and those of 1e-13 with none.
+// 2^exponent(x) is above |x| (of zeros and denormals: 2^-126).
+__device__ inline int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 255) - 126; }
+
+template <typename P>
+constexpr int kULds = kScaled<P> ? (P::kLds > 2 * P::kOutPlane + 4096 ? P::kLds : 2 * P::kOutPlane + 4096) : P::kLds;
+template <typename P>
+__device__ inline void planes_out(P& prod, const ScoreArgs& a, _Float16* u, int p0, int q0, int p_end, int end, char* smem) {
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) P::store(smem, h, u + h * a.plane - a.v0, a.width, p0, q0, p_end, end);
+    __syncthreads();
+}
+template <typename P>
+__device__ inline void held_split(char* smem, int i, int j, int r, const float* y) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        _Float16 x, z;
+        split(y[e], x, z);
+        hi[e] = x, lo[e] = z;
+    }
+    P::held(smem, 0, i, j, r) = hi;
+    P::held(smem, 1, i, j, r) = lo;
+}
+
+// prod.acc holds U.  LDS is free.
+template <typename P>
+__device__ inline void scaled_u(const ScoreArgs& a, P& prod, const WordExps<P>& w, const float (&gm)[P::FQ], const int (&ge)[P::FQ], int tp, int tq, int p0, int q0, int end,
+                                int p_end, char* smem) {
+    constexpr int kWavesQ = P::TQ / P::WQ, kMine = P::FP * 16;
+    static_assert(2 * P::kOutPlane + 4 * (P::kWavesP * P::TQ + kWavesQ * P::TP) <= kULds<P> && kMine == 32, "");
+    int* row_exps = (int*)(smem + 2 * P::kOutPlane);            // [waves along the vocabulary][TQ]
+    int* word_most = row_exps + P::kWavesP * P::TQ;             // [waves along the rows][TP]
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave_p = wave_id() % P::kWavesP, wave_q = wave_id() / P::kWavesP;
+#pragma unroll
+    for (int j = 0; j < P::FQ; ++j) {
+        int most = INT_MIN;
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = max(most, exponent(prod.acc[i][j][r]) + (p0 + P::row(i, r) < a.v1 ? w.at(i, r) : kLeastExp));
+        most = max(most, __shfl_xor(most, 32, 64));
+        if (half == 0) row_exps[wave_p * P::TQ + P::col(j)] = most;
+    }
+    // the words' largest over the rows (|gm| is at most 1): each step leaves half of the values to half of the lanes
+    int t[kMine];
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+        t[n] = exponent(prod.acc[n / 16][0][n % 16]) + ge[0];
+#pragma unroll
+        for (int j = 1; j < P::FQ; ++j) t[n] = max(t[n], exponent(prod.acc[n / 16][j][n % 16]) + ge[j]);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int n = 0; n < o; ++n) {
+            const int give = upper ? t[n] : t[n + o], keep = upper ? t[n + o] : t[n];
+            t[n] = max(keep, __shfl_xor(give, o, 64));
+        }
+    }
+    const int mine = lane & 31;     // the value that this lane is left with
+    word_most[wave_q * P::TP + P::wave_p() + 32 * (mine / 16) + 8 * (mine % 16 / 4) + 4 * half + mine % 4] = t[0];
+    __syncthreads();
+    for (int c = threadIdx.x; c < P::TQ; c += P::kThreads) {
+        int most = row_exps[c];
+#pragma unroll
+        for (int i = 1; i < P::kWavesP; ++i) most = max(most, row_exps[i * P::TQ + c]);
+        row_exps[c] = most;
+        if (q0 + c < a.Np) a.exps_h[(int64_t)tp * a.Np + q0 + c] = most;
+    }
+    for (int c = threadIdx.x; c < P::TP; c += P::kThreads) {
+        int most = word_most[c];
+#pragma unroll
+        for (int i = 1; i < kWavesQ; ++i) most = max(most, word_most[i * P::TP + c]);
+        word_most[c] = most;
+        if (p0 + c < p_end) a.exps_w[tq * a.width + p0 - a.v0 + c] = most;
+    }
+    __syncthreads();
+    if (a.u) {     // dh is wanted
+#pragma unroll
+        for (int j = 0; j < P::FQ; ++j) {
+            const int exp = 15 - row_exps[P::col(j)];
+#pragma unroll
+            for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    float y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_ldexpf(prod.acc[i][j][r + e], w.at(i, r + e) + exp);
+                    held_split<P>(smem, i, j, r, y);
+                }
+        }
+        planes_out(prod, a, a.u, p0, q0, p_end, end, smem);
+    }
+    if (!a.u_w) return;
+#pragma unroll
+    for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const Int4 exps = *(const Int4*)(word_most + P::row(i, r));
+#pragma unroll
+            for (int j = 0; j < P::FQ; ++j) {
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_ldexpf(prod.acc[i][j][r + e] * gm[j], ge[j] + 15 - exps.v[e]);
+                held_split<P>(smem, i, j, r, y);
+            }
+        }
+    planes_out(prod, a, a.u_w, p0, q0, p_end, end, smem);
+}
+
 // U of a piece of the vocabulary, zeros behind its end and behind the last row.  28672 rows, 50257 words of 512 in bf16: 365 us a piece
 // of 9216 words on average, 674 TFLOP/s; 309 us without its 528 MB of stores.  Stores past the caches: 0.4 - 0.9 % less for the whole
 // call there and at 4096 rows of 1024, 1 % more at 1186.
-template <typename P, int PL>
+template <typename P>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const ScoreArgs a) {
     extern __shared__ char smem[];
     int tp, tq;
@@ -393,43 +578,46 @@ __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const Scor
     if (!tile_of(a.tiles_p, (count + P::TQ - 1) / P::TQ, tp, tq)) return;
     const int p0 = a.v0 + tp * P::TP, q0 = tq * P::TQ;
     P prod;
-    const float f = score_factor<P>(a);
     prod.run(a.w, Side{a.h.p, a.h.plane, a.h.ld, count}, p0, q0, 0, a.Dp, smem);
+    const int end = (count + kPad - 1) / kPad * kPad, p_end = a.v0 + (int)a.width;
+    const WordExps<P> exps(a, p0);
+    float gm[P::FQ];     // fp32: g_n (times its row of hidden's scale) is gm 2^ge
+    int ge[P::FQ];
+    static_assert(P::kOutPlane <= P::kLds, "");
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < P::FQ; ++j) {
-        const int n = q0 + P::col(j) < count ? a.r.at(q0 + P::col(j)) : -1;
-        const int target = n >= 0 ? a.t.at(n) : -1;
+        const int place = q0 + P::col(j), n = place < count ? a.r.at(place) : -1, exp = row_exp<P>(a, place, count);
+        const int target = n >= 0 ? a.g.t.at(n) : -1;
         const bool counts = target != -1;
         const float m = counts ? a.lse[n] : 0.f, l = counts ? a.lse[a.N + n] : 0.f;
+        if constexpr (kScaled<P>) {
+            const float g = counts ? a.g.at(n) : 0.f;
+            gm[j] = __builtin_amdgcn_frexp_mantf(g), ge[j] = g != 0.f ? __builtin_amdgcn_frexp_expf(g) + exp : 4 * kLeastExp;
+        }
 #pragma unroll
         for (int i = 0; i < P::FP; ++i)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int v = p0 + P::row(i, r);
-                f16x4 hi, lo;
+                f16x4 y;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float u = __builtin_amdgcn_exp2f((prod.acc[i][j][r + e] * f - m) * kLog2e - l);
+                    float u = __builtin_amdgcn_exp2f((score_of<P>(prod.acc[i][j][r + e], exp + exps.at(i, r + e)) - m) * kLog2e - l);
                     u = v + e == target ? u - 1.f : u;
-                    u = counts && v + e < a.v1 ? u * kUScale : 0.f;
-                    if constexpr (PL == 2) {
-                        _Float16 x, y;
-                        split(u, x, y);
-                        hi[e] = x, lo[e] = y;
-                    } else {
-                        hi[e] = (_Float16)u;
-                    }
+                    u = counts && v + e < a.v1 ? u * kUScale : 0.f;     // (of a product a select, of the exponential itself a branch)
+                    if constexpr (kScaled<P>) prod.acc[i][j][r + e] = u;
+                    else y[e] = (_Float16)u;
                 }
-                P::held(smem, 0, i, j, r) = hi;
-                if constexpr (PL == 2) P::held(smem, 1, i, j, r) = lo;
+                if constexpr (!kScaled<P>) P::held(smem, 0, i, j, r) = y;
             }
     }
-    static_assert(PL * P::kOutPlane <= P::kLds, "");
-    __syncthreads();
-    const int end = (count + kPad - 1) / kPad * kPad;
-#pragma unroll
-    for (int h = 0; h < PL; ++h) P::store(smem, h, a.u + h * a.plane - a.v0, a.width, p0, q0, a.v0 + (int)a.width, end);
+    if constexpr (kScaled<P>) {
+        scaled_u<P>(a, prod, exps, gm, ge, tp, tq, p0, q0, end, p_end, smem);
+    } else {
+        __syncthreads();
+        P::store(smem, 0, a.u - a.v0, a.width, p0, q0, p_end, end);
+    }
 }
 
 struct PartArgs {
@@ -440,12 +628,78 @@ struct PartArgs {
     float* out;                         // [splits][q.n, ld]
     int64_t ld;
     int add;                            // onto what is there
-    const float* scale;                 // set: the result itself, [q.n, p.n] of the tensors' type, to `result`
-    void* result;
+    void* result;                       // set: the result itself, [q.n, p.n] of the tensors' type
+    const float* scale;                 // its scale (fp32: none)
+    const int* exps;                    // fp32: [blocks of k, exps_ld] the exponents of q's columns
+    int64_t exps_ld;
     __host__ __device__ int blocks() const { return tiles_p * tiles_q * splits; }
 };
 
-template <typename T, typename P>
+// Sums over k of operands whose second one has a power of two for each column q in every BLOCK of k: the sum so far changes to the next
+// block's.  A block that is 2^60 below the column's largest counts as one that is just that: the sum stays below 2^(30 + 24 + 60).
+// The exponents wait in LDS behind the tiles, kExpBlocks of k at a time.
+constexpr int kExpBlocks = 64, kExpRange = 60;
+template <typename P>
+constexpr int kExpBytes = kExpBlocks * P::TQ * 2;
+template <typename P, int BLOCK>
+__device__ inline void run_scaled(P& prod, const PartArgs& a, const Side& q, int p0, int q0, int k0, int k1, char* smem) {
+    int16_t* exps = (int16_t*)(smem + P::kLds);
+    int first = k0 / BLOCK, most = INT16_MIN;
+    const int last = (k1 - 1) / BLOCK;
+    static_assert(P::kThreads >= P::TQ, "");
+    auto bring = [&] {
+        const int blocks = min(kExpBlocks, last + 1 - first);
+        for (int n = threadIdx.x; n < blocks * P::TQ; n += P::kThreads) {
+            const int c = n % P::TQ;
+            exps[n] = q0 + c < q.n ? (int16_t)a.exps[(first + n / P::TQ) * a.exps_ld + q0 + c] : (int16_t)0;
+        }
+        __syncthreads();
+        if (threadIdx.x < P::TQ) {
+            for (int n = 0; n < blocks; ++n) most = max(most, (int)exps[n * P::TQ + threadIdx.x]);
+            for (int n = 0; n < blocks; ++n) {
+                int16_t& x = exps[n * P::TQ + threadIdx.x];
+                x = (int16_t)max((int)x, most - kExpRange);
+            }
+        }
+    };
+    int now[P::FQ];
+    auto exponents = [&](int block, int (&x)[P::FQ]) {
+#pragma unroll
+        for (int j = 0; j < P::FQ; ++j) x[j] = exps[(block - first) * P::TQ + P::col(j)];
+    };
+    bring();
+    __syncthreads();
+    exponents(first, now);
+    prod.run(a.p, q, p0, q0, k0, k1, smem, [&](int k, uint32_t) {
+        if (k % BLOCK || k == k0) return;
+        const int block = k / BLOCK;
+        if (block == first + kExpBlocks) {
+            __syncthreads();
+            first = block;
+            bring();
+            __syncthreads();
+        }
+        int next[P::FQ];
+        exponents(block, next);
+#pragma unroll
+        for (int j = 0; j < P::FQ; ++j) {
+            const float f = __builtin_amdgcn_ldexpf(1.f, now[j] - next[j]);
+#pragma unroll
+            for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) prod.acc[i][j][r] *= f;
+            now[j] = next[j];
+        }
+    });
+#pragma unroll
+    for (int j = 0; j < P::FQ; ++j)
+#pragma unroll
+        for (int i = 0; i < P::FP; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) prod.acc[i][j][r] = __builtin_amdgcn_ldexpf(prod.acc[i][j][r], now[j] - 29 - 15);     // kUScale
+}
+
+template <typename T, typename P, int BLOCK>
 __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     const int tiles = a.tiles_p * a.tiles_q;
     const int split = block / tiles, tile = block - split * tiles;
@@ -455,8 +709,10 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
     const int steps = (a.k_rows ? (count + kPad - 1) / kPad * kPad : a.k1) / P::kStep;
     const int k0 = (int)((int64_t)steps * split / a.splits) * P::kStep, k1 = (int)((int64_t)steps * (split + 1) / a.splits) * P::kStep;
     P prod;
-    if (k1 > k0) prod.run(a.p, Side{a.q.p, a.q.plane, a.q.ld, end}, p0, q0, k0, k1, smem);
-    else prod.clear();
+    const Side q_side = {a.q.p, a.q.plane, a.q.ld, end};
+    if (k1 <= k0) prod.clear();
+    else if constexpr (sizeof(T) == 4) run_scaled<P, BLOCK>(prod, a, q_side, p0, q0, k0, k1, smem);
+    else prod.run(a.p, q_side, p0, q0, k0, k1, smem);
     // out by way of LDS, kAtOnce blocks of every wave at a time: a thread four values of a row, a wave whole rows
     constexpr int kAtOnce = P::kOut32 <= P::kLds ? P::FQ : 1;
     static_assert(P::kOut32 / P::FQ * kAtOnce <= P::kLds, "");
@@ -482,7 +738,7 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
             const int row = n / kPieces, p = p0 + n % kPieces * 4, q = q0 + P::out32_col(row, j0, kAtOnce);
             if (q >= end) continue;
             f32x4v v = P::out32x4(smem, row, p - p0);
-            if (a.scale) {
+            if (a.result) {
                 T* to = (T*)a.result + (int64_t)q * a.p.n + p;
                 const four_t y = {(T)(v[0] * f), (T)(v[1] * f), (T)(v[2] * f), (T)(v[3] * f)};
                 if (four && p < a.p.n) {
@@ -503,14 +759,14 @@ __device__ inline void part_of(const PartArgs& a, int block, char* smem) {
 
 // Both gradients' products with a piece of U in one launch, either without tiles where it is not wanted: the one's
 // workgroups fill what the other's leave of the card's last round.  The longer ones come first.
-template <typename T, typename H, typename W>
+template <typename T, typename H, typename W, int BLOCK_H, int BLOCK_W>
 __global__ void __launch_bounds__(H::kThreads, H::kWaves) ce_part_kernel(const PartArgs h, const PartArgs w) {
     static_assert(H::kThreads == W::kThreads && H::kWaves == W::kWaves, "");
     extern __shared__ char smem[];
     const bool h_first = (int64_t)h.k1 * w.splits >= (int64_t)w.k1 * h.splits;
     const int n = h_first ? h.blocks() : w.blocks(), block = blockIdx.x;
-    if ((block < n) == h_first) part_of<T, H>(h, h_first ? block : block - n, smem);
-    else part_of<T, W>(w, h_first ? block - n : block, smem);
+    if ((block < n) == h_first) part_of<T, H, BLOCK_H>(h, h_first ? block : block - n, smem);
+    else part_of<T, W, BLOCK_W>(w, h_first ? block - n : block, smem);
 }
 
 // out[n, d] = factor (g_n) sum_s part[s][n, d], in the parts' order; graded rows come from their places.
@@ -526,7 +782,7 @@ __global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const
     const bool first = (int)blockIdx.x < x.blocks;
     const SumArgs& a = first ? x : y;
     const int block = first ? blockIdx.x : blockIdx.x - x.blocks;
-    const float f = 1.f / *a.scale / kUScale;
+    const float f = a.scale ? 1.f / *a.scale / kUScale : 1.f;
     const int pieces = a.ld / 4;
     T* out = (T*)a.out;
     for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < (int64_t)a.rows * pieces; i += (int64_t)a.blocks * kThreads) {
@@ -837,18 +1093,20 @@ struct Carve {
     }
 };
 
-// U's bytes in a piece (of 256 words at least): few launches and few passes over dh's sums against what stays in the
+// Bytes of a copy of U in a piece (of 256 words at least): few launches and few passes over dh's sums against what stays in the
 // caches and the memory that is wanted.  56 x 512 rows, 50257 words: 256 MiB 7.14 ms, 512 6.88, 1024 6.93, 2048 7.05.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 // From so many rows on the ones that count are put next to each other first: a launch more and a copy of the rows, 15.5 + 15.2 us a
 // direction (both directions: 6.8 ms) at 56 x 512; where 0.3 of 4093 rows are ignored (20011 words of 384, fp32) 929 -> 782 us.
 constexpr int64_t kGatherRows = 1024;
+constexpr int64_t kWordTile = 256;      // words of the largest of the scores' tiles
 
 // The products of each type: the scores (vocabulary x rows), dh (D x rows) and dw (D x vocabulary).
 struct Bf16 {
     typedef __bf16 T;
     static constexpr int kPlanes = 1;
     typedef Product<__bf16, 1, 192, 128, kRows, kRows, 2, 2, 64> Score;
+    typedef Score U;
     typedef Product<_Float16, 1, 256, 128, kCols, kRows> GradH;
     typedef Product<_Float16, 1, 256, 128, kCols, kCols> GradW;
 };
@@ -856,6 +1114,7 @@ struct F32 {
     typedef float T;
     static constexpr int kPlanes = 2;
     typedef Product<_Float16, 2, 256, 128, kRows, kRows, 4, 2> Score;
+    typedef Product<_Float16, 2, 128, 128, kRows, kRows> U;
     typedef Product<_Float16, 2, 128, 128, kCols, kRows> GradH;
     typedef Product<_Float16, 2, 128, 128, kCols, kCols> GradW;
 };
@@ -865,15 +1124,18 @@ struct F32 {
 constexpr int64_t kFewRows = 64;
 struct FewBf16 : Bf16 {
     typedef Product<__bf16, 1, 256, 64, kRows, kRows, 2, 2, 64> Score;
+    typedef Score U;
 };
 struct FewF32 : F32 {
     typedef Product<_Float16, 2, 128, 64, kRows, kRows, 2, 2, 32> Score;
+    typedef Score U;
 };
 
 struct Plan {
     int64_t N, V, D, Dp, Np, Vp, width;
     bool direct_h, direct_w, gather;
     int planes, tiles_p, tiles_q;           // of the scores
+    int width_tiles;                         // of a piece's
     int s_h, s_w;                            // splits of the two gradients' products
 };
 
@@ -918,6 +1180,7 @@ Plan plan_of(const mb_linear_ce* a) {
     p.direct_h = !p.gather && as_it_is<C>(p.D, a->hidden, a->hidden_ld), p.direct_w = as_it_is<C>(p.D, a->weight, a->weight_ld);
     p.tiles_p = (int)((p.V + C::Score::TP - 1) / C::Score::TP), p.tiles_q = (int)((p.N + C::Score::TQ - 1) / C::Score::TQ);
     p.width = std::min<int64_t>(pad(p.V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np * 2 * p.planes) / 256 * 256));
+    p.width_tiles = (int)((p.width + C::U::TP - 1) / C::U::TP);
     choose_splits(tiles_of<typename C::GradH>(p.D, p.N), std::min(p.width, p.Vp), tiles_of<typename C::GradW>(p.D, std::min(p.width, p.V)), p.Np, p.s_h,
                   p.s_w);
     static_assert(C::GradH::kThreads == 256, "kSlots: two a CU");
@@ -926,12 +1189,13 @@ Plan plan_of(const mb_linear_ce* a) {
 
 struct Buffers {
     int *rows, *pos, *m;
-    float *largest_h, *largest_w, *largest_g, *scales;   // scales: h, w, g h
+    float *largest_w, *largest_g, *scales;   // bf16: scales of w and g h
+    int *exp_w, *exp_h, *exps_h, *exps_w;    // fp32: the rows' exponents, and those of U's copies
     void *h, *w;                 // copies for the scores (planes, or padded bf16)
     float2* part;
     float* target_score;
     double* sums;
-    _Float16 *w16, *h16, *u;     // backward
+    _Float16 *w16, *h16, *u, *u_w;   // backward
     float *part_h, *part_w;
     int64_t bytes;
 };
@@ -939,8 +1203,9 @@ struct Buffers {
 Buffers buffers_of(const Plan& p, bool backward, void* base) {
     Carve c = {(char*)base};
     Buffers b = {};
-    b.largest_h = c.take<float>(kMaxBlocks), b.largest_w = c.take<float>(kMaxBlocks), b.largest_g = c.take<float>(kMaxBlocks);
-    b.scales = c.take<float>(4);
+    const bool f32 = p.planes == 2;
+    if (f32) b.exp_h = c.take<int>(p.Np), b.exp_w = c.take<int>(pad(p.V, kWordTile));
+    else b.largest_w = c.take<float>(kMaxBlocks), b.largest_g = c.take<float>(kMaxBlocks), b.scales = c.take<float>(2);
     if (p.gather) b.rows = c.take<int>(p.N), b.pos = c.take<int>(p.N), b.m = c.take<int>(1);
     if (!p.direct_h) b.h = c.take<_Float16>(p.planes * p.Np * p.Dp);
     if (!p.direct_w) b.w = c.take<_Float16>(p.planes * p.Vp * p.Dp);
@@ -949,9 +1214,13 @@ Buffers buffers_of(const Plan& p, bool backward, void* base) {
         b.target_score = c.take<float>(p.N);
         b.sums = c.take<double>(2 * ((p.N + kRowsPerBlock - 1) / kRowsPerBlock));
     } else {
-        b.w16 = p.planes == 2 ? (_Float16*)b.w : c.take<_Float16>(p.Vp * p.Dp);
-        b.h16 = c.take<_Float16>(p.planes * p.Np * p.Dp);
+        b.w16 = f32 ? (_Float16*)b.w : c.take<_Float16>(p.Vp * p.Dp);
+        b.h16 = f32 ? (_Float16*)b.h : c.take<_Float16>(p.Np * p.Dp);
         b.u = c.take<_Float16>(p.planes * p.Np * p.width);
+        if (f32) {
+            b.u_w = c.take<_Float16>(p.planes * p.Np * p.width);
+            b.exps_h = c.take<int>(p.width_tiles * p.Np), b.exps_w = c.take<int>(p.tiles_q * p.width);
+        }
         b.part_h = c.take<float>(p.s_h * p.N * p.Dp);
         if (p.s_w > 1) b.part_w = c.take<float>(p.s_w * p.width * p.Dp);
     }
@@ -968,8 +1237,8 @@ Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t D, int size, floa
     x.blocks = (int)std::min<int64_t>(blocks_for(rows * ((D + 7) / 8)), kMaxBlocks);
     return x;
 }
-// Copies of the set's matrices; scaled ones after a launch that looks for their largest values.
-template <typename T, typename O, int PL>
+// Copies of the set's matrices as one plane; scaled ones after a launch that looks for their largest values.
+template <typename T, typename O>
 void copies(Set a, hipStream_t st) {
     if (a.n == 0) return;
     int total = 0;
@@ -982,21 +1251,29 @@ void copies(Set a, hipStream_t st) {
         a.x[i].copy_blocks = (int)blocks_for((int64_t)a.x[i].rows_pad * a.x[i].Dp / 8);
         a.first[i] = total, total += a.x[i].copy_blocks;
     }
-    hipLaunchKernelGGL((ce_planes_kernel<T, O, PL>), dim3(total), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((ce_planes_kernel<T, O>), dim3(total), dim3(kThreads), 0, st, a);
+}
+// fp32 matrices as two planes.
+void row_planes(Set a, hipStream_t st) {
+    int total = 0;
+    for (int i = 0; i < a.n; ++i) {
+        a.x[i].copy_blocks = (int)blocks_for((int64_t)a.x[i].rows_pad * 64);
+        a.first[i] = total, total += a.x[i].copy_blocks;
+    }
+    hipLaunchKernelGGL(ce_row_planes_kernel, dim3(total), dim3(kThreads), 0, st, a);
 }
 
 // The rows' places and the operands of the scores: the user's own, or copies of them; and what the gradients want copied: g h
-// for dw, and for dh w in fp16 (fp32: the scores' planes).
+// for dw, and for dh w in fp16 (fp32: the scores' planes serve both).
 template <typename C>
 void operands(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs& s, const RowGrad& g, bool wants_h, bool wants_w, hipStream_t st) {
     typedef typename C::T T;
-    s.t = g.t;
+    s.g = g;
     s.r = {b.rows, b.pos, b.m, (int)p.N};
     if (p.gather) {
         const int each = (int)pad((p.N + kRowRuns - 1) / kRowRuns, kThreads);
-        hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((p.N + each - 1) / each)), dim3(kThreads), 0, st, s.t, (int)p.N, each, b.rows, b.pos, b.m);
+        hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)((p.N + each - 1) / each)), dim3(kThreads), 0, st, g.t, (int)p.N, each, b.rows, b.pos, b.m);
     }
-    constexpr bool f32 = sizeof(T) == 4;
     Set scores = {}, grads = {};
     scores.g = grads.g = g, scores.r = grads.r = s.r;
     auto hidden = [&](float* largest, float* scale, void* out, int graded) {
@@ -1007,17 +1284,18 @@ void operands(const mb_linear_ce* a, const Plan& p, const Buffers& b, ScoreArgs&
     auto weight = [&](float* largest, float* scale, void* out) {
         return matrix(a->weight, a->weight_ld, p.V, p.D, sizeof(T), largest, scale, out, p.Vp, p.Dp);
     };
-    if (!p.direct_h) scores.x[scores.n++] = hidden(f32 ? b.largest_h : nullptr, b.scales, b.h, f32 ? 2 : 0);
-    if (!p.direct_w) scores.x[scores.n++] = weight(f32 ? b.largest_w : nullptr, b.scales + 1, b.w);
-    Set& more = f32 ? scores : grads;
-    if (wants_w) more.x[more.n++] = hidden(b.largest_g, b.scales + 2, b.h16, 1);
-    if (wants_h && !f32) more.x[more.n++] = weight(b.largest_w, b.scales + 1, b.w16);
-    if constexpr (f32) {
-        copies<T, _Float16, 2>(scores, st);
-        s.scale_h = b.scales, s.scale_w = b.scales + 1;
+    if constexpr (sizeof(T) == 4) {
+        scores.x[0] = hidden(nullptr, nullptr, b.h, 1), scores.x[1] = weight(nullptr, nullptr, b.w), scores.n = 2;
+        scores.x[0].exps = b.exp_h, scores.x[1].exps = b.exp_w;
+        row_planes(scores, st);
+        s.exp_h = b.exp_h, s.exp_w = b.exp_w;
     } else {
-        copies<T, __bf16, 1>(scores, st);
-        copies<T, _Float16, 1>(grads, st);
+        if (!p.direct_h) scores.x[scores.n++] = hidden(nullptr, nullptr, b.h, 0);
+        if (!p.direct_w) scores.x[scores.n++] = weight(nullptr, nullptr, b.w);
+        if (wants_w) grads.x[grads.n++] = hidden(b.largest_g, b.scales + 1, b.h16, 1);
+        if (wants_h) grads.x[grads.n++] = weight(b.largest_w, b.scales, b.w16);
+        copies<T, __bf16>(scores, st);
+        copies<T, _Float16>(grads, st);
     }
     s.h = {p.direct_h ? a->hidden : b.h, p.Np * p.Dp * 2, p.direct_h ? a->hidden_ld : p.Dp, (int)p.N};
     s.w = {p.direct_w ? a->weight : b.w, p.Vp * p.Dp * 2, p.direct_w ? a->weight_ld : p.Dp, (int)p.V};
@@ -1036,10 +1314,10 @@ int stats(const ScoreArgs& s, int tiles_q, hipStream_t st) {
     static Told told;
     return launch("mb_linear_ce_fwd", ce_stats_kernel<P>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * tiles_q), st, s);
 }
-template <typename P, int PL>
+template <typename P>
 int piece_of_u(const ScoreArgs& s, int tiles_q, hipStream_t st) {
     static Told told;
-    return launch("mb_linear_ce_bwd", ce_u_kernel<P, PL>, P::kThreads, P::kLds, told, tile_grid((int64_t)s.tiles_p * tiles_q), st, s);
+    return launch("mb_linear_ce_bwd", ce_u_kernel<P>, P::kThreads, kULds<P>, told, tile_grid((int64_t)s.tiles_p * tiles_q), st, s);
 }
 template <typename P>
 void tiles_for(PartArgs& a) {
@@ -1051,9 +1329,11 @@ int parts(const PartArgs& h, const PartArgs& w, hipStream_t st) {
     typedef typename C::GradH H;
     typedef typename C::GradW W;
     static Told told;
-    constexpr int lds = std::max(H::kLds, W::kLds);
-    if (const int rc = allow_lds("mb_linear_ce_bwd", (const void*)ce_part_kernel<T, H, W>, lds, told)) return rc;
-    hipLaunchKernelGGL((ce_part_kernel<T, H, W>), dim3((unsigned)(h.blocks() + w.blocks())), dim3(H::kThreads), lds, st, h, w);
+    constexpr int lds = std::max(H::kLds + (sizeof(T) == 4 ? kExpBytes<H> : 0), W::kLds + (sizeof(T) == 4 ? kExpBytes<W> : 0));
+    static_assert(lds <= H::kRoom, "two workgroups a CU");
+    constexpr auto kernel = ce_part_kernel<T, H, W, C::U::TP, C::U::TQ>;
+    if (const int rc = allow_lds("mb_linear_ce_bwd", (const void*)kernel, lds, told)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(h.blocks() + w.blocks())), dim3(H::kThreads), lds, st, h, w);
     return MB_OK;
 }
 
@@ -1215,7 +1495,7 @@ int forward(const mb_linear_ce* a, hipStream_t st) {
     s.part = b.part, s.target_score = b.target_score;
     if (const int rc = stats<typename C::Score>(s, p.tiles_q, st)) return rc;
     const int blocks = (int)((p.N + kRowsPerBlock - 1) / kRowsPerBlock);
-    const JoinArgs j = {b.part, b.target_score, s.t, s.r, (int)p.N, p.tiles_p, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
+    const JoinArgs j = {b.part, b.target_score, g.t, s.r, (int)p.N, p.tiles_p, (int)a->reduction, a->loss, a->lse, a->count, b.sums};
     hipLaunchKernelGGL(ce_join_kernel, dim3(blocks), dim3(kThreads), 0, st, j);
     if (a->reduction)
         hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(kThreads), 0, st, b.sums, blocks, (int)a->reduction, a->loss, a->count);
@@ -1225,7 +1505,6 @@ int forward(const mb_linear_ce* a, hipStream_t st) {
 template <typename C>
 int backward(const mb_linear_ce* a, hipStream_t st) {
     typedef typename C::T T;
-    constexpr int PL = C::kPlanes;
     const Plan p = plan_of<C>(a);
     const Buffers b = buffers_of(p, true, a->workspace);
     if (const int rc = fits("mb_linear_ce_bwd", a, p, (p.D + C::GradH::TP - 1) / C::GradH::TP)) return rc;
@@ -1235,30 +1514,34 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
     ScoreArgs s = {};
     const RowGrad g = {{a->target, (int)a->target_bytes, a->ignore_index, a->V}, a->dloss, a->count, (int)a->reduction};
     operands<C>(a, p, b, s, g, wants_h, wants_w, st);
-    s.lse = a->lse, s.u = b.u, s.width = p.width, s.plane = p.Np * p.width;
+    constexpr bool f32 = sizeof(T) == 4;
+    s.lse = a->lse, s.u = f32 && !wants_h ? nullptr : b.u, s.u_w = wants_w ? b.u_w : nullptr, s.exps_h = b.exps_h, s.exps_w = b.exps_w, s.Np = (int)p.Np, s.width = p.width, s.plane = p.Np * p.width;
+    const float *scale_h = f32 ? nullptr : b.scales, *scale_w = f32 ? nullptr : b.scales + 1;
     for (int64_t v0 = 0; v0 < p.V; v0 += p.width) {
         const int64_t v1 = std::min(p.V, v0 + p.width), kv = pad(v1 - v0, kPad);
         s.v0 = (int)v0, s.v1 = (int)v1;
-        s.tiles_p = (int)((v1 - v0 + C::Score::TP - 1) / C::Score::TP);
-        if (const int rc = piece_of_u<typename C::Score, PL>(s, p.tiles_q, st)) return rc;
+        s.tiles_p = (int)((v1 - v0 + C::U::TP - 1) / C::U::TP);
+        if (const int rc = piece_of_u<typename C::U>(s, p.tiles_q, st)) return rc;
         PartArgs ph = {}, pw = {};
         SumArgs sh = {}, sw = {};
         ph.r = pw.r = s.r, pw.k_rows = 1;
         if (wants_h) {
             ph.p = {b.w16 + v0 * p.Dp, p.Vp * p.Dp * 2, p.Dp, (int)p.D};
             ph.q = {b.u, s.plane * 2, p.width, (int)p.N};
+            ph.exps = b.exps_h, ph.exps_ld = p.Np;
             ph.splits = (int)std::min<int64_t>(p.s_h, kv / kPad), ph.k1 = (int)kv, ph.out = b.part_h, ph.ld = p.Dp, ph.add = v0 > 0;
             tiles_for<typename C::GradH>(ph);
             if (v1 == p.V)
-                sh = {b.part_h, p.s_h, (int)p.N, (int)p.D, (int)p.Dp, 1, (int)blocks_for(p.N * p.Dp / 4), b.scales + 1, a->dhidden};
+                sh = {b.part_h, p.s_h, (int)p.N, (int)p.D, (int)p.Dp, 1, (int)blocks_for(p.N * p.Dp / 4), scale_h, a->dhidden};
         }
         if (wants_w) {
             pw.p = {b.h16, p.Np * p.Dp * 2, p.Dp, (int)p.D};
-            pw.q = {b.u, s.plane * 2, p.width, (int)(v1 - v0)};
+            pw.q = {f32 ? b.u_w : b.u, s.plane * 2, p.width, (int)(v1 - v0)};
+            pw.exps = b.exps_w, pw.exps_ld = p.width;
             pw.splits = p.s_w, pw.k1 = (int)p.Np, pw.out = b.part_w, pw.ld = p.Dp;
             tiles_for<typename C::GradW>(pw);
-            if (p.s_w == 1) pw.scale = b.scales + 2, pw.result = (T*)a->dweight + v0 * p.D;
-            else sw = {b.part_w, p.s_w, (int)(v1 - v0), (int)p.D, (int)p.Dp, 0, (int)blocks_for((v1 - v0) * p.Dp / 4), b.scales + 2,
+            if (p.s_w == 1) pw.scale = scale_w, pw.result = (T*)a->dweight + v0 * p.D;
+            else sw = {b.part_w, p.s_w, (int)(v1 - v0), (int)p.D, (int)p.Dp, 0, (int)blocks_for((v1 - v0) * p.Dp / 4), scale_w,
                   (T*)a->dweight + v0 * p.D};
         }
         if (const int rc = parts<C>(ph, pw, st)) return rc;

@@ -4,9 +4,13 @@ mb_linear_ce_fwd / mb_linear_ce_bwd.
 ``linear_cross_entropy(hidden, weight, target)`` is F.cross_entropy(F.linear(hidden, weight), target)
 with gradients for hidden and weight, for the tied output matrix over a vocabulary of any size: the
 scores exist a tile at a time, and in the backward pass a piece of the vocabulary at a time (about
-512 MiB), where F.cross_entropy keeps [rows, vocabulary] several times.  fp32 and bf16; scores,
-maxima, sums and both gradients' sums are fp32 or more, the scores are never rounded to bf16, and the
-loss is fp32.  Sums have a fixed order.  CPU tensors raise NotImplementedError.  Both directions
+512 MiB, in fp32 twice that), where F.cross_entropy keeps [rows, vocabulary] several times.  fp32 and
+bf16; scores, maxima, sums and both gradients' sums are fp32 or more, the scores are never rounded to
+bf16, and the loss is fp32.  The gradients' products take softmax - onehot, and the rows of hidden times
+their gradients, in 11 bits for bf16 tensors: a word whose probability is below 2^-40 in every row
+has no gradient there, one below 2^-32 fewer than bf16's 8 bits.  For fp32 tensors all operands have 24 bits
+down to 2^-16 of their own row's largest value (or of the largest term of the row's or word's sum).
+Sums have a fixed order.  CPU tensors raise NotImplementedError.  Both directions
 are registered as torch ops (mathbrain::linear_ce_fwd / linear_ce_bwd) for tracing.
 """
 import functools
