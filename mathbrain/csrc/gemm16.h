@@ -358,11 +358,10 @@ struct Product {
 // by 2^-23 of a value from 2^-2 on (lo's half step is 2^-25 at least), down to 2^-16 of the largest.  Smaller values are off by 2^-25, 2^-39
 // of the largest, in either.
 
-// The scale for a largest (finite) magnitude of these bits: 2^-46 to 2^74.
+// The scale for a largest (finite) magnitude of these bits, which may be any: 2^-113 to 2^127 (magnitudes below 2^-113 stay below 2^14).
 __device__ inline float plane_scale(uint32_t bits) {
-    int e = (int)(bits >> 23);
-    e = e < 127 - 60 ? 127 - 60 : e > 127 + 60 ? 127 + 60 : e;
-    return __builtin_bit_cast(float, (uint32_t)(127 + 14 - (e - 127)) << 23);
+    const int e = (int)(bits >> 23);
+    return __builtin_bit_cast(float, (uint32_t)(127 + 14 - ((e < 14 ? 14 : e) - 127)) << 23);
 }
 // x = hi + lo; an infinite hi (or NaN) stands alone.
 __device__ inline void split(float x, _Float16& hi, _Float16& lo) {
