@@ -738,7 +738,8 @@ typedef struct mb_linear_ce {
     float *loss;                  /* forward: [N] or one */
     float *lse, *count;           /* [2, N] the rows' maxima and log2 of their sums; the rows that count: */
                                   /*   written by the forward, read by the backward */
-    const float *dloss;           /* backward: [N] or one */
+    const float *dloss;           /* backward: [N] or one. forward: not NULL (and not read) where a backward follows, which */
+                                  /*   wants the scores of the same kernels; NULL may be quicker for few rows */
     void *dhidden, *dweight;      /* backward: [N, D], [V, D] contiguous, of dtype; either may be NULL */
     void *workspace;              /* at a multiple of 256 bytes, mb_linear_ce_workspace(args, backward) */
     int64_t workspace_bytes;      /*   bytes (-1: the arguments are refused) */

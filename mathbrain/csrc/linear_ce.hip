@@ -1389,10 +1389,12 @@ int few_rows(int64_t N) { return N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8; }
 // of 256 395 and 131, 8 on 50257 of 1024 458 and 158, 2 on 30000 of 2048 558 and 176, 8 on 50257 of 2048 1100 and 629, 16 on 50257 of
 // 1024 458 and 290, 16 on 50257 of 512 248 and 172; bf16, 5 on 100000 of 1024 327 and 181, 4 on 50257 of 2048 367 and 210, 2 on 50257
 // of 101 146 and 127 (the host).  A bf16 forward that reads the weights as they are stays with the matrix instructions: 5 on 100000 of
-// 1024 41 and 50, 8 on 128000 of 256 25 and 39; with copies it does not, 2 on 50257 of 101 32 and 25.
+// 1024 41 and 50, 8 on 128000 of 256 25 and 39; with copies it does not, 2 on 50257 of 101 32 and 25.  But where a backward follows
+// the forward takes the backward's kernels: scores that are summed in another order are off by 2^-24 of themselves, which is
+// what a probability is off by then, and is not small for large ones.
 bool vector_rows(const mb_linear_ce* a, bool backward) {
     const bool f32 = a->dtype == MB_DTYPE_F32;
-    if (!backward && !f32 && as_it_is<FewBf16>(a->D, a->weight, a->weight_ld)) return false;
+    if (!backward && !a->dloss && !f32 && as_it_is<FewBf16>(a->D, a->weight, a->weight_ld)) return false;
     return a->N <= (f32 ? 2 : 1) * launch_rows(a->D, f32 ? 4 : 2);
 }
 

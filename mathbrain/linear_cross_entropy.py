@@ -34,21 +34,22 @@ def _rows(x):
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace(backward, h_at, w_at, h_ld, w_ld, N, V, D, dtype):
-    """The library's workspace for these sizes, row distances and addresses modulo 16."""
+def _workspace(backward, follows, h_at, w_at, h_ld, w_ld, N, V, D, dtype):
+    """The library's workspace for these sizes, row distances and addresses modulo 16; whether a backward follows."""
     nbytes = _lib.lib().mb_linear_ce_workspace(
-        _ARGS.pack(_ANY + h_at, _ANY + w_at, h_ld, w_ld, _ANY, 8, 0, N, V, D, dtype, 0, _ANY, _ANY, _ANY, 0, 0, 0, 0, 0), backward)
+        _ARGS.pack(_ANY + h_at, _ANY + w_at, h_ld, w_ld, _ANY, 8, 0, N, V, D, dtype, 0, _ANY, _ANY, _ANY, _ANY if follows else 0, 0, 0, 0, 0),
+        backward)
     if nbytes < 0:
         raise _lib.HipKernelError(_lib.lib().mb_last_error().decode(errors="replace"))
     return nbytes
 
 
-def _call(name, backward, hidden, weight, target, ignore_index, reduction, loss, stats, dloss=None, dh=None, dw=None):
+def _call(name, backward, hidden, weight, target, ignore_index, reduction, loss, stats, dloss, dh=None, dw=None):
     N, D = hidden.shape
     V = weight.shape[0]
     h, w, t = hidden.data_ptr(), weight.data_ptr(), _DTYPES[hidden.dtype]
     h_ld, w_ld = hidden.stride(0) if N > 1 else D, weight.stride(0) if V > 1 else D
-    nbytes = _workspace(backward, h % 16, w % 16, h_ld, w_ld, N, V, D, t)
+    nbytes = _workspace(backward, dloss is not None, h % 16, w % 16, h_ld, w_ld, N, V, D, t)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=hidden.device)
     lse = stats.data_ptr()
     _lib.call_on(hidden.device, name,
@@ -57,7 +58,7 @@ def _call(name, backward, hidden, weight, target, ignore_index, reduction, loss,
                             0 if dh is None else dh.data_ptr(), 0 if dw is None else dw.data_ptr(), ws.data_ptr(), nbytes))
 
 
-def _fwd_fake(hidden, weight, target, ignore_index, reduction):
+def _fwd_fake(hidden, weight, target, ignore_index, reduction, follows=True):
     N = hidden.shape[0]
     return (hidden.new_empty((N,) if reduction == 0 else (), dtype=torch.float32),
             hidden.new_empty((2 * N + 1,), dtype=torch.float32))
@@ -65,12 +66,14 @@ def _fwd_fake(hidden, weight, target, ignore_index, reduction):
 
 @_lib.traced_op("linear_ce_fwd", _fwd_fake)
 def linear_ce_fwd(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int,
-                  reduction: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """(loss, what the backward wants of the rows: their maxima, logarithms of sums and how many count [2 N + 1])."""
+                  reduction: int, follows: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss, what the backward wants of the rows: their maxima, logarithms of sums and how many count [2 N + 1]);
+    ``follows``: whether a backward may follow, which wants the scores of its own kernels."""
     loss, stats = _fwd_fake(hidden, weight, target, ignore_index, reduction)
     if hidden.shape[0] == 0:
         return loss.fill_(float("nan") if reduction == 1 else 0.0), stats.zero_()
-    _call("mb_linear_ce_fwd", 0, _rows(hidden), _rows(weight), target, ignore_index, reduction, loss, stats)
+    _call("mb_linear_ce_fwd", 0, _rows(hidden), _rows(weight), target, ignore_index, reduction, loss, stats,
+          stats if follows else None)
     return loss, stats
 
 
@@ -135,5 +138,5 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         raise ValueError(f"{what}: reduction={reduction!r} ('none', 'mean' or 'sum')")
     args = (hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1).contiguous(), int(ignore_index),
             REDUCTIONS.index(reduction))
-    loss = LinearCrossEntropyFunction.apply(*args) if _lib.wants_derivatives(hidden, weight) else linear_ce_fwd(*args)[0]
+    loss = LinearCrossEntropyFunction.apply(*args) if _lib.wants_derivatives(hidden, weight) else linear_ce_fwd(*args, False)[0]
     return loss.view(target.shape) if reduction == "none" else loss
