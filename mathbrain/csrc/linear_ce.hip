@@ -1057,9 +1057,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) ce_few_grads_kernel(const FewA
     }
 }
 
-// dh from the workgroups' parts: 16 pieces of a row a workgroup, each by 16 threads in a fixed order.
+// dh from the workgroups' parts: 16 pieces of a row a workgroup, each by 16 threads in a fixed order.  A row without a gradient has
+// sums of 0 w, which are not zeros where a weight is infinite.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) ce_few_sum_kernel(const float* part, int parts, int N, int D, int D4, T* out) {
+__global__ void __launch_bounds__(kThreads) ce_few_sum_kernel(const float* part, int parts, const RowGrad g, int n0, int N, int D, int D4, T* out) {
     constexpr int kCols = 16, kSlices = kThreads / kCols;
     __shared__ f32x4v s[kSlices][kCols];
     const int col = threadIdx.x % kCols, slice = threadIdx.x / kCols, pieces = D4 / 4;
@@ -1073,6 +1074,7 @@ __global__ void __launch_bounds__(kThreads) ce_few_sum_kernel(const float* part,
     if (slice || i >= N * pieces) return;
     for (int n = 1; n < kSlices; ++n) v += s[n][col];
     const int d = i % pieces * 4;
+    if (g.at(n0 + i / pieces) == 0.f) v = f32x4v{0.f, 0.f, 0.f, 0.f};
     T* to = out + (int64_t)(i / pieces) * D + d;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -1475,7 +1477,7 @@ int few(const char* what, const mb_linear_ce* a, bool backward, hipStream_t st) 
         if (rc) return rc;
         if (backward && a->dhidden)
             hipLaunchKernelGGL((ce_few_sum_kernel<T>), dim3((unsigned)((f.rows * f.D4 / 4 + 15) / 16)), dim3(kThreads), 0, st, (const float*)b.part_h,
-                               blocks, f.rows, f.D, f.D4, (T*)a->dhidden + (int64_t)f.n0 * a->D);
+                               blocks, f.g, f.n0, f.rows, f.D, f.D4, (T*)a->dhidden + (int64_t)f.n0 * a->D);
     }
     if (backward) return check_launch(what);
     static_assert(2 * kVectorRows <= kRowsPerBlock, "one workgroup joins");
