@@ -126,7 +126,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         _lib.require_gpu(hidden, weight, target, what=what)
     if torch.is_autocast_enabled("cuda"):
         t = torch.get_autocast_dtype("cuda")
-        hidden, weight = hidden.to(t), weight.to(t)
+        hidden, weight = (x if x.dtype is torch.float64 else x.to(t) for x in (hidden, weight))
     if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
         raise ValueError(f"{what}: hidden {hidden.dtype} and weight {weight.dtype} (supported: both float32 or both bfloat16)")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:

@@ -28,3 +28,13 @@ def test_rows_without_a_gradient(N, t, bad):
     s = h.detach().double() @ w.detach().double().t()
     want = torch.logsumexp(s, 1) - s.gather(1, target.clamp(min=0)[:, None])[:, 0]
     assert torch.equal(loss.isfinite()[2:], want.isfinite()[2:])
+
+
+def test_autocast_leaves_64_bits():
+    """As nn.Linear: tensors in 64 bits are not cast, and refused as they are outside of autocast."""
+    from mathbrain.linear_cross_entropy import linear_cross_entropy
+    h, w, target = torch.randn(4, 8, device="cuda"), torch.randn(9, 8, device="cuda"), torch.zeros(4, device="cuda", dtype=torch.long)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for a, b in ((h.double(), w.double()), (h.double(), w), (h, w.double())):
+            with pytest.raises(ValueError, match="float64"):
+                linear_cross_entropy(a, b, target)
