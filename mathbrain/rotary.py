@@ -14,6 +14,7 @@ gradient is the rotation by the opposite angles.  CPU tensors raise NotImplement
 Registered for tracing as mathbrain::apply_rotary.
 """
 import math
+import operator
 import struct
 from typing import Optional
 
@@ -169,6 +170,13 @@ def _check(q, k, cos, sin, start, layout):
         raise ValueError(f"{what}: the tables must be contiguous float32")
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad) or _lib.has_tangent(cos, sin):
         raise ValueError(f"{what}: the tables get no derivative, and one of them wants it")
+    if rows is None and not isinstance(start, (int, torch.SymInt)):
+        try:
+            start = operator.index(start)
+        except TypeError:
+            raise ValueError(f"{what}: start={start!r} is neither a whole number nor a tensor") from None
+    if rows is None and type(start) is int and not -2**63 <= start < 2**63:
+        raise ValueError(f"{what}: start={start} is no position")
     if rows is not None and (tuple(rows.shape) not in ((qs[0],), (qs[0], qs[1])) or rows.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"{what}: start {tuple(rows.shape)} {rows.dtype} is not one int32 or int64 for each of {qs[0]} rows, "
                          f"or for each of their {qs[1]} tokens")
