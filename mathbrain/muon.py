@@ -33,7 +33,7 @@ def _exponents(steps, coefficients):
     a, b, c = coefficients
     top, most = 1.0, [1.0, 1.0, 0.0]
     for _ in range(steps):
-        s = torch.linspace(0.0, top, 20001, dtype=torch.float64)
+        s = torch.linspace(0.0, top, 20001, dtype=torch.float64, device="cpu")
         gram = s * s
         second = b * gram + c * gram * gram
         most = [max(most[0], top), max(most[1], top * top), max(most[2], float(second.abs().max()))]
