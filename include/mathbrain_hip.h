@@ -664,7 +664,8 @@ typedef struct mb_rotary {
     int64_t layout;               /* 0: pairs (2i, 2i + 1), 1: pairs (i, i + turned / 2) */
     int64_t inverse;              /* 1: by the opposite angles (the gradients) */
     int64_t dtype;                /* MB_DTYPE_F32 or MB_DTYPE_BF16 */
-    void *q_out, *k_out;          /* [B, L, H | Hk, hd] contiguous; not the inputs' memory */
+    void *q_out, *k_out;          /* [B, L, H | Hk, hd] contiguous; not the inputs' memory, from their first */
+                                  /*   to their last element, nor each other's (checked) */
 } mb_rotary;
 
 int mb_apply_rotary(const mb_rotary *args, void *stream);
@@ -740,7 +741,8 @@ typedef struct mb_linear_ce {
                                   /*   written by the forward, read by the backward */
     const float *dloss;           /* backward: [N] or one. forward: not NULL (and not read) where a backward follows, which */
                                   /*   wants the scores of the same kernels; NULL may be quicker for few rows */
-    void *dhidden, *dweight;      /* backward: [N, D], [V, D] contiguous, of dtype; either may be NULL */
+    void *dhidden, *dweight;      /* backward: [N, D], [V, D] contiguous, of dtype; either may be NULL. What a */
+                                  /*   call writes must not share memory with anything else of it (checked) */
     void *workspace;              /* at a multiple of 256 bytes, mb_linear_ce_workspace(args, backward) */
     int64_t workspace_bytes;      /*   bytes (-1: the arguments are refused) */
 } mb_linear_ce;

@@ -25,6 +25,13 @@ int check_launch(const char* what);
         if (!(cond)) return ::mb::fail(MB_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
     } while (0)
 
+// Memory from the first to behind the last byte of a tensor (empty: none).
+struct Span {
+    uintptr_t from, to;
+};
+inline Span span(const void* p, int64_t bytes) { return p && bytes > 0 ? Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes} : Span{0, 0}; }
+inline bool touch(const Span& a, const Span& b) { return a.from < b.to && b.from < a.to; }
+
 // ---- small device utilities -----------------------------------------------------------------
 
 // Streaming stores (global_store ... nt) for outputs that no later access of the same kernel

@@ -1369,6 +1369,22 @@ int enough(const char* what, const mb_linear_ce* a, int64_t need) {
     return MB_OK;
 }
 
+// What the call writes must not be anything that it reads, nor twice the same.
+int apart(const char* what, const mb_linear_ce* a, bool backward) {
+    const int64_t size = a->dtype == MB_DTYPE_F32 ? 4 : 2, rows = a->reduction == 0 ? a->N : 1;
+    const Span read[] = {span(a->hidden, ((a->N - 1) * a->hidden_ld + a->D) * size), span(a->weight, ((a->V - 1) * a->weight_ld + a->D) * size),
+                         span(a->target, a->N * a->target_bytes), span(backward ? a->lse : nullptr, 8 * a->N), span(backward ? a->count : nullptr, 4),
+                         span(backward ? a->dloss : nullptr, 4 * rows)};
+    const Span written[] = {span(a->workspace, a->workspace_bytes), span(backward ? a->dhidden : nullptr, a->N * a->D * size),
+                            span(backward ? a->dweight : nullptr, a->V * a->D * size), span(backward ? nullptr : a->loss, 4 * rows),
+                            span(backward ? nullptr : a->lse, 8 * a->N), span(backward ? nullptr : a->count, 4)};
+    for (const Span& x : written) {
+        for (const Span& y : read) MB_REQUIRE(!touch(x, y), "%s: memory that is written is shared with an input", what);
+        for (const Span& y : written) MB_REQUIRE(&x == &y || !touch(x, y), "%s: two tensors that are written share memory", what);
+    }
+    return MB_OK;
+}
+
 // ---- few rows, the host's part ----
 
 constexpr int kVectorRows = 8;                       // of a launch
@@ -1445,6 +1461,7 @@ template <typename T>
 int few(const char* what, const mb_linear_ce* a, bool backward, hipStream_t st) {
     const FewBuffers b = few_buffers(a, backward, a->workspace);
     if (const int rc = enough(what, a, b.bytes)) return rc;
+    if (const int rc = apart(what, a, backward)) return rc;
     if (backward && !a->dhidden && !a->dweight) return MB_OK;
     constexpr int vec = 16 / sizeof(T);
     FewArgs f = {};
@@ -1493,6 +1510,7 @@ int forward(const mb_linear_ce* a, hipStream_t st) {
     const Buffers b = buffers_of(p, false, a->workspace);
     if (const int rc = fits("mb_linear_ce_fwd", a, p, 0)) return rc;
     if (const int rc = enough("mb_linear_ce_fwd", a, b.bytes)) return rc;
+    if (const int rc = apart("mb_linear_ce_fwd", a, false)) return rc;
     ScoreArgs s = {};
     const RowGrad g = {{a->target, (int)a->target_bytes, a->ignore_index, a->V}, nullptr, nullptr, 0};
     operands<C>(a, p, b, s, g, false, false, st);
@@ -1513,6 +1531,7 @@ int backward(const mb_linear_ce* a, hipStream_t st) {
     const Buffers b = buffers_of(p, true, a->workspace);
     if (const int rc = fits("mb_linear_ce_bwd", a, p, (p.D + C::GradH::TP - 1) / C::GradH::TP)) return rc;
     if (const int rc = enough("mb_linear_ce_bwd", a, b.bytes)) return rc;
+    if (const int rc = apart("mb_linear_ce_bwd", a, true)) return rc;
     const bool wants_h = a->dhidden, wants_w = a->dweight;
     if (!wants_h && !wants_w) return MB_OK;
     ScoreArgs s = {};

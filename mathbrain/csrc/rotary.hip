@@ -152,6 +152,13 @@ void dispatch(RotArgs& a, bool half, bool pieces, int64_t tokens, hipStream_t st
     }
 }
 
+// Of a strided input [B, L, H, hd].
+Span input_span(const void* p, const int64_t* st, const int64_t* n, int64_t hd, int64_t size) {
+    int64_t from = 0, to = hd;
+    for (int i = 0; i < 3; ++i) (st[i] < 0 ? from : to) += st[i] * (n[i] - 1);
+    return span(p ? (const char*)p + from * size : nullptr, (to - from) * size);
+}
+
 bool rows16(const void* p, const int64_t* st, int size) {
     return (((uintptr_t)p | (uint64_t)(st[0] * size) | (uint64_t)(st[1] * size) | (uint64_t)(st[2] * size)) & 15) == 0;
 }
@@ -182,6 +189,14 @@ extern "C" int mb_apply_rotary(const mb_rotary* p, void* stream) {
     if (tokens == 0) return MB_OK;
     MB_REQUIRE((p->H == 0 || (p->q && p->q_out)) && (p->Hk == 0 || (p->k && p->k_out)) && (p->turned == 0 || (p->cos && p->sin)),
                "%s: null pointer argument", what);
+    const int size = p->dtype == MB_DTYPE_F32 ? 4 : 2, n = 16 / size;
+    const int64_t q_n[3] = {p->B, p->L, p->H}, k_n[3] = {p->B, p->L, p->Hk}, table = p->table_rows * (p->turned / 2) * 4;
+    const Span out[] = {span(p->q_out, tokens * p->H * p->hd * size), span(p->k_out, tokens * p->Hk * p->hd * size)};
+    const Span in[] = {p->H ? input_span(p->q, p->q_st, q_n, p->hd, size) : Span{}, p->Hk ? input_span(p->k, p->k_st, k_n, p->hd, size) : Span{},
+                       span(p->cos, table), span(p->sin, table), span(p->start, (p->start_per_token ? tokens : p->B) * p->start_bytes)};
+    for (const Span& x : out)
+        for (const Span& y : in) MB_REQUIRE(!touch(x, y), "%s: an output's memory is shared with an input", what);
+    MB_REQUIRE(!touch(out[0], out[1]), "%s: the outputs share memory", what);
     RotArgs a = {};
     a.q = p->q, a.q_sb = p->q_st[0], a.q_sl = p->q_st[1], a.q_sh = p->q_st[2];
     a.k = p->k, a.k_sb = p->k_st[0], a.k_sl = p->k_st[1], a.k_sh = p->k_st[2];
@@ -192,7 +207,6 @@ extern "C" int mb_apply_rotary(const mb_rotary* p, void* stream) {
     a.q_out = p->q_out, a.k_out = p->k_out;
     // 16 bytes a thread where rows and the parts of them allow it, single channels otherwise (56 x 512: 20.8 against 50 us, 2 x 16384:
     // 28.9 against 67; 6 x 1021 in fp32, 10 + 5 heads of 64 of which half turns: 9.1 against 18)
-    const int size = p->dtype == MB_DTYPE_F32 ? 4 : 2, n = 16 / size;
     const bool half = p->layout == 1;
     const bool pieces = p->hd % n == 0 && p->turned % (half ? 2 * n : n) == 0 && (p->H == 0 || rows16(p->q, p->q_st, size))
                         && (p->Hk == 0 || rows16(p->k, p->k_st, size)) && (((uintptr_t)p->q_out | (uintptr_t)p->k_out) & 15) == 0;
