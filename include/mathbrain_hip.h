@@ -758,8 +758,8 @@ int mb_linear_ce_bwd(const mb_linear_ce *args, void *stream);
  *   is_step 0: dst = X.   is_step 1: momentum <- mu momentum + src,  G = src + mu momentum (nesterov) or momentum,
  *   dst <- dst (1 - lr weight_decay) - lr rate X
  *
- * All matrices go through every launch together; the products are those of fp32 values (24 bits, in two fp16
- * planes).  The arguments come in structs on the HOST, read before the call returns.
+ * All matrices go through every launch together, as far as 4 GiB of workspace hold them (8 bytes an element of X and of
+ * X X^T, 4 of a step's G); the products are those of fp32 values (24 bits, in two fp16 planes).  The arguments come in structs on the HOST, read before the call returns.
  */
 typedef struct mb_muon_matrix {
     const void *src;              /* [rows, cols] contiguous, as the others: the matrix, or a step's gradient */

@@ -681,22 +681,44 @@ struct Layout {
 constexpr int kPlaces = 512;
 int64_t splits_of(int64_t tiles, int64_t longest) { return tiles ? std::max<int64_t>(1, std::min(kPlaces / tiles, longest / kPad / 8)) : 1; }
 
-int64_t lay_out(const mb_muon* p, char* base, Layout* out) {
-    int64_t used = 0, tiles = 0, longest = 0;
-    auto take = [&](int64_t bytes) {
-        char* at = base ? base + used : nullptr;
-        used += pad(bytes, 256);
-        return at;
-    };
+// What a matrix takes of the workspace: two pairs of X's planes and of A's and B's, a step's G, the norm's parts.
+int64_t bytes_of_matrix(const mb_muon* p, int64_t i) {
+    const mb_muon_matrix& m = p->matrices[i];
+    const int64_t mp = pad(std::min(m.rows, m.cols), kPad), np = pad(std::max(m.rows, m.cols), kPad);
+    return 8 * mp * (np + mp) + (p->is_step ? 4 * m.rows * m.cols : 0) + m.rows * m.cols / kChunk * 8 + 6 * 256;
+}
+
+// The matrices that go through the launches together: all, or as many as this much memory holds; then the next ones with the same memory.
+// So much fills the card many times over (some 200 M elements); a list of all of a large model's matrices would want 12 to 20 bytes an element.
+constexpr int64_t kGroupBytes = (int64_t)4 << 30;
+typedef std::vector<int64_t> Group;
+std::vector<Group> groups_of(const mb_muon* p) {
     // the longest products first: what is left at a launch's end is short
-    std::vector<int64_t> order;
+    Group order;
     for (int64_t i = 0; i < p->count; ++i)
         if (p->matrices[i].rows && p->matrices[i].cols) order.push_back(i);
     std::stable_sort(order.begin(), order.end(), [&](int64_t i, int64_t j) {
         const mb_muon_matrix &x = p->matrices[i], &y = p->matrices[j];
         return std::max(x.rows, x.cols) > std::max(y.rows, y.cols);
     });
+    std::vector<Group> groups;
+    int64_t held = 0;
     for (const int64_t i : order) {
+        const int64_t bytes = bytes_of_matrix(p, i);
+        if (groups.empty() || held + bytes > kGroupBytes) groups.emplace_back(), held = 0;
+        groups.back().push_back(i), held += bytes;
+    }
+    return groups;
+}
+
+int64_t lay_out(const mb_muon* p, const Group& group, char* base, Layout* out) {
+    int64_t used = 0, tiles = 0, longest = 0;
+    auto take = [&](int64_t bytes) {
+        char* at = base ? base + used : nullptr;
+        used += pad(bytes, 256);
+        return at;
+    };
+    for (const int64_t i : group) {
         const mb_muon_matrix& from = p->matrices[i];
         Mat m = {};
         m.src = from.src, m.dst = from.dst, m.momentum = from.momentum;
@@ -738,10 +760,16 @@ bool small_ones(const std::vector<Mat>& mats) {
 
 int64_t table_bytes(int64_t count) { return pad(count * (int64_t)sizeof(Mat), 256) + pad(count * (int64_t)sizeof(int) * kFirsts, 256); }
 
-int run(const char* what, const mb_muon* p, hipStream_t st) {
+int64_t workspace_of(const mb_muon* p, const std::vector<Group>& groups) {
+    int64_t most = 0;
+    for (const Group& g : groups) most = std::max(most, lay_out(p, g, nullptr, nullptr));
+    return table_bytes(p->count) + most;
+}
+
+int run(const char* what, const mb_muon* p, const Group& group, hipStream_t st) {
     Layout l;
     const int64_t table = table_bytes(p->count);
-    lay_out(p, (char*)p->workspace + table, &l);
+    lay_out(p, group, (char*)p->workspace + table, &l);
     const int count = (int)l.mats.size();
     if (count == 0) return MB_OK;
     for (int f = 0; f < kFirsts; ++f)
@@ -838,7 +866,7 @@ using namespace mb;
 
 extern "C" int64_t mb_muon_workspace(const mb_muon* p) try {
     if (check("mb_muon_workspace", p)) return -1;
-    return table_bytes(p->count) + lay_out(p, nullptr, nullptr);
+    return workspace_of(p, groups_of(p));
 } catch (const std::bad_alloc&) {
     fail(MB_ERR_INVALID_ARGUMENT, "mb_muon_workspace: no host memory");
     return -1;
@@ -864,12 +892,15 @@ extern "C" int mb_muon_run(const mb_muon* p, void* stream) try {
         any = std::max(any, x.to);
         if (x.written) written = std::max(written, x.to);
     }
-    const int64_t need = table_bytes(p->count) + lay_out(p, nullptr, nullptr);
+    const std::vector<Group> groups = groups_of(p);
+    const int64_t need = workspace_of(p, groups);
     MB_REQUIRE(((uintptr_t)p->workspace & 255) == 0, "%s: the workspace has to begin at a multiple of 256 bytes", what);
     if (s.empty()) return MB_OK;
     if (!p->workspace || p->workspace_bytes < need)
         return fail(MB_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld are needed", what, (long long)p->workspace_bytes, (long long)need);
-    return run(what, p, (hipStream_t)stream);
+    for (const Group& g : groups)
+        if (const int rc = run(what, p, g, (hipStream_t)stream)) return rc;
+    return MB_OK;
 } catch (const std::bad_alloc&) {
     return fail(MB_ERR_INVALID_ARGUMENT, "mb_muon_run: no host memory");
 }

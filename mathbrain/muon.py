@@ -6,7 +6,8 @@ X = G / (|G| + eps), then ``steps`` times A = X X^T, X <- a X + (b A + c A^2) X 
 update and the decayed weights; ``Muon`` is the torch.optim.Optimizer of it, for the weight matrices of a model
 (its embeddings, norms and other vectors belong to another optimiser).
 
-All matrices of a call, of whatever shapes, go through every launch together.  The products are those of fp32 values
+All matrices of a call, of whatever shapes, go through every launch together, as far as a workspace of 4 GiB holds them
+(some 200 million elements; one matrix at least).  The products are those of fp32 values
 whatever the inputs' type (two fp16 planes a matrix, 24 bits; a single 16-bit plane would leave errors of the first
 iterations multiplied by some hundreds).  fp32 and bf16, mixed as they come; no gradients.  CPU tensors raise
 NotImplementedError.
