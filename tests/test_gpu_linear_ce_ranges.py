@@ -15,8 +15,9 @@ pytestmark = pytest.mark.gpu
 IGN = -100
 
 
-def expected(h, w, target, g):
-    """loss, dh, dw of sum_n g_n loss_n in 64 bits, and how far each row of them may be off."""
+def expected(h, w, target, g, spread=None):
+    """loss, dh, dw of sum_n g_n loss_n in 64 bits, and how far each row of them may be off, with scores off by `spread`
+    (2 sqrt(D) + 8) of 2^-24 |h_n| |w_v|."""
     h, w, g = h.double(), w.double(), g.double()
     N, D = h.shape
     use = target != IGN
@@ -25,7 +26,7 @@ def expected(h, w, target, g):
     p = torch.softmax(s, 1)
     lse = torch.logsumexp(s, 1, keepdim=True)
     loss = torch.where(use, (lse - s.gather(1, t[:, None]))[:, 0], 0.0)
-    e = (2 * math.sqrt(D) + 8) * 2.0**-24 * h.norm(dim=1)[:, None] * w.norm(dim=1) + 2.0**-23 * (s.abs() + lse.abs())
+    e = (spread or 2 * math.sqrt(D) + 8) * 2.0**-24 * h.norm(dim=1)[:, None] * w.norm(dim=1) + 2.0**-23 * (s.abs() + lse.abs())
     pe = (p * e).sum(1, keepdim=True)
     onehot = torch.nn.functional.one_hot(t, w.shape[0])
     pt, et = p.gather(1, t[:, None]), e.gather(1, t[:, None])
