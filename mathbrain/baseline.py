@@ -25,8 +25,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from .bias_attention import relative_bias_attention
-from .linear_cross_entropy import linear_cross_entropy
-from .model import RMSNorm, SwiGLU
+from .model import RMSNorm, SwiGLU, head_loss
 from .qk_norm import qk_norm_rotary
 from .rotary import LAYOUTS, apply_rotary
 from .rotary import rotary_tables as scaled_rotary_tables
@@ -176,5 +175,5 @@ class RoPETransformerLM(nn.Module):
             h = layer(h, cos, sin, self.rel_bias, self.rel_max_distance)
         h = self.final_norm(h)
         if targets is not None:
-            return linear_cross_entropy(h, self.lm_head.weight, targets, ignore_index)
+            return head_loss(self.lm_head, h, targets, ignore_index)
         return self.lm_head(h)

@@ -155,6 +155,14 @@ class SlotTransformerBlock(nn.Module):
         return h
 
 
+def head_loss(head, h, targets, ignore_index):
+    """The mean cross entropy of head(h), without the logits where the head is a plain linear layer (no bias, subclass or hooks that
+    would be passed over), with them otherwise."""
+    if type(head) is nn.Linear and head.bias is None and not head._forward_hooks and not head._forward_pre_hooks:
+        return linear_cross_entropy(h, head.weight, targets, ignore_index)
+    return F.cross_entropy(head(h).flatten(0, -2).float(), targets.flatten().long(), ignore_index=ignore_index)
+
+
 class SlotTransformerLM(nn.Module):
     """model.py:119-186.  forward(x, unique_slots=None, inverse_indices=None, c_base=None,
     doc_ids=None, pad_mask=None) -> logits [B, L, vocab_size].
@@ -251,5 +259,5 @@ class SlotTransformerLM(nn.Module):
             x_q = layer(x_q, x, E_slots, self.ema_rhos, C_seq, unique_tensor, K_max, C_bounds, E_active)
         x_q = self.final_norm(x_q)
         if targets is not None:
-            return linear_cross_entropy(x_q, self.lm_head.weight, targets, ignore_index)
+            return head_loss(self.lm_head, x_q, targets, ignore_index)
         return self.lm_head(x_q)
