@@ -128,3 +128,16 @@ def test_many_blocks_of_both_sums():
     check(h, w, target, g)
     h, w, target, g = make(6000, 15001, 32, seed=7)
     check(h, w, target, g)
+
+
+@pytest.mark.parametrize("N,V,D", [(17000, 8000, 2048), (4000, 20000, 2048)])
+def test_long_runs_of_blocks_of_different_sizes(N, V, D):
+    """Sums over rows (or words) that one workgroup takes from end to end, so that the exponents in LDS are replaced on the way (after 64
+    blocks of 128), of blocks whose terms lie up to 2^150 apart."""
+    h, w, target, g = make(N, V, D, seed=8)
+    at = torch.arange(N, device="cuda") // 128
+    g *= torch.exp2(((at * 37) % 25 - 12).float() * 6)
+    words = torch.arange(V, device="cuda") // 128
+    h[:, 0] = 8.0
+    w[:, 0] -= ((words * 29) % 11).float() * 0.5
+    check(h, w, target, g)
