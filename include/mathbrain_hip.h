@@ -725,8 +725,8 @@ int mb_bias_attn_bwd(const mb_bias_attn *args, void *stream);
  *
  * Products of bf16 values are exact; fp32 values go as two fp16 planes (24 bits down to 2^-16 of the largest value of
  * a row of hidden or weight, and of the largest term of the row's or word's sum in a gradient; smaller ones are off by
- * 2^-39 of it).  bf16 gradients take softmax - [v = target] in 11 bits, with steps of 2^-39 at least.  Sums have a
- * fixed order.  The arguments come in a struct on the HOST, read before the call returns.
+ * 2^-39 of it).  bf16 gradients take softmax - [v = target] in 11 bits, with steps of 2^-39 at least, and g_n hidden_n
+ * and weight_v with steps of 2^-38 of the matrix's largest value.  Sums have a fixed order.  The arguments come in a struct on the HOST, read before the call returns.
  */
 typedef struct mb_linear_ce {
     const void *hidden, *weight;  /* [N, D], [V, D], elements of a row next to each other, rows */

@@ -310,7 +310,7 @@ __device__ inline int row_exp(const ScoreArgs& a, int place, int count) { return
 template <typename P>
 __device__ inline float score_of(float sum, int exps) { return kScaled<P> ? __builtin_amdgcn_ldexpf(sum, exps - 28) : sum; }
 
-// Matrix instructions bound it: 28672 rows, 50257 words of 512 in bf16 1.57 - 1.61 ms, 916 - 941 TFLOP/s; 16 rows 13.8 us, the weights' 51 MB at
+// Matrix instructions bound it: 28672 rows, 50257 words of 512 in bf16 1.54 - 1.60 ms, 922 - 960 TFLOP/s; 16 rows 13.8 us, the weights' 51 MB at
 // 3.7 TB/s.
 template <typename P>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_stats_kernel(const ScoreArgs a) {
@@ -567,8 +567,8 @@ __device__ inline void scaled_u(const ScoreArgs& a, P& prod, const WordExps<P>& 
     planes_out(prod, a, a.u_w, p0, q0, p_end, end, smem);
 }
 
-// U of a piece of the vocabulary, zeros behind its end and behind the last row.  28672 rows, 50257 words of 512 in bf16: 365 us a piece
-// of 9216 words on average, 674 TFLOP/s; 309 us without its 528 MB of stores.  Stores past the caches: 0.4 - 0.9 % less for the whole
+// U of a piece of the vocabulary, zeros behind its end and behind the last row.  28672 rows, 50257 words of 512 in bf16: 358 us a piece
+// of 9216 words on average, 687 TFLOP/s; 309 us without its 528 MB of stores.  Stores past the caches: 0.4 - 0.9 % less for the whole
 // call there and at 4096 rows of 1024, 1 % more at 1186.
 template <typename P>
 __global__ void __launch_bounds__(P::kThreads, P::kWaves) ce_u_kernel(const ScoreArgs a) {
@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(kThreads) ce_sum_kernel(const SumArgs x, const
 // bytes of each a lane and chunk, and reads hidden (fp32 in LDS) once for them.  The backward has the scores' words still in its
 // registers for dh, whose sums it keeps over all its words, and writes dw at once: w is read once a direction, without the copies
 // that the matrix instructions want.  One row on 128789 words of 256 in fp32: 22.6 us forward, 44.5 us backward, the weights' 132 MB at
-// 5.8 and (with dw) 5.9 TB/s, partly out of the last-level cache; 5 rows on 100000 of 1024 in bf16 130.6 us backward, 3.1 TB/s (vector instructions).  A score's sum over the lanes leaves it with the lane whose number begins with it.
+// 5.8 and (with dw) 5.9 TB/s, partly out of the last-level cache; 5 rows on 100000 of 1024 in bf16 126.6 us backward, 3.2 TB/s (vector instructions).  A score's sum over the lanes leaves it with the lane whose number begins with it.
 constexpr int kFewThreads = 512;
 constexpr int kFewLanes = 64;
 struct FewArgs {
@@ -1404,9 +1404,9 @@ int launch_rows(int64_t D, int size) {
 int few_rows(int64_t N) { return N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8; }
 // A launch's rows; fp32 takes two launches a direction for twice as many, bf16 none (its matrix instructions' kernels read the weights
 // less often: 9 rows on 50257 of 512 120 us).  Both directions (us, matrix instructions' kernels and these): fp32, 1 row on 128789 words
-// of 256 395 and 131, 8 on 50257 of 1024 458 and 158, 2 on 30000 of 2048 558 and 176, 8 on 50257 of 2048 1100 and 629, 16 on 50257 of
-// 1024 458 and 290, 16 on 50257 of 512 248 and 172; bf16, 5 on 100000 of 1024 327 and 181, 4 on 50257 of 2048 367 and 210, 2 on 50257
-// of 101 146 and 127 (the host).  A bf16 forward that reads the weights as they are stays with the matrix instructions: 5 on 100000 of
+// of 256 385 and 81, 8 on 50257 of 1024 398 and 157, 2 on 30000 of 2048 499 and 173, 8 on 50257 of 2048 1027 and 624, 16 on 50257 of
+// 1024 400 and 286, 16 on 50257 of 512 219 and 167; bf16, 5 on 100000 of 1024 323 and 187, 4 on 50257 of 2048 359 and 213, 8 on 128000
+// of 256 158 and 138, 2 on 50257 of 101 141 and 136 (the host).  A bf16 forward that reads the weights as they are stays with the matrix instructions: 5 on 100000 of
 // 1024 41 and 50, 8 on 128000 of 256 25 and 39; with copies it does not, 2 on 50257 of 101 32 and 25.  But where a backward follows
 // the forward takes the backward's kernels: scores that are summed in another order are off by 2^-24 of themselves, which is
 // what a probability is off by then, and is not small for large ones.

@@ -8,7 +8,8 @@ scores exist a tile at a time, and in the backward pass a piece of the vocabular
 bf16; scores, maxima, sums and both gradients' sums are fp32 or more, the scores are never rounded to
 bf16, and the loss is fp32.  The gradients' products take softmax - onehot, and the rows of hidden times
 their gradients, in 11 bits for bf16 tensors: a word whose probability is below 2^-40 in every row
-has no gradient there, one below 2^-32 fewer than bf16's 8 bits.  For fp32 tensors all operands have 24 bits
+has no gradient there, one below 2^-32 fewer than bf16's 8 bits, and rows (times their gradients) or words
+below 2^-31 of the largest lose bits in the same way.  For fp32 tensors all operands have 24 bits
 down to 2^-16 of their own row's largest value (or of the largest term of the row's or word's sum).
 Sums have a fixed order.  CPU tensors raise NotImplementedError.  Both directions
 are registered as torch ops (mathbrain::linear_ce_fwd / linear_ce_bwd) for tracing.
