@@ -52,11 +52,11 @@ def _on_the_kernel(q, cos, sin):
     """Whether apply_rotary takes the rotation of q by these tables: plain GPU tensors in fp32 or bf16, tables of fp32 at most
     that get no derivative and have a row for every position, and no torch.func transform.  Everything else goes through
     ``rotate``'s tensor operations."""
-    return (q.is_cuda and type(q) is torch.Tensor and q.dtype in (torch.float32, torch.bfloat16)
+    return (q.is_cuda and q.dtype in (torch.float32, torch.bfloat16)
             and all(t.dtype is not torch.float64 and t.shape[0] >= q.shape[1] and not (t.requires_grad and torch.is_grad_enabled())
                     for t in (cos, sin))
             and (torch.compiler.is_compiling()
-                 or (torch._C._functorch.peek_interpreter_stack() is None and not _lib.has_tangent(cos, sin))))
+                 or (type(q) is torch.Tensor and torch._C._functorch.peek_interpreter_stack() is None and not _lib.has_tangent(cos, sin))))
 
 
 class CausalSelfAttention(nn.Module):

@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(kThreads) ce_total_kernel(const double* sums, 
 // A word that is improbable in every row keeps its 24 bits so, and rows (or words) beside one of another size theirs.  One copy with one
 // power of two would be less to write: 2865 rows, 20011 words of 384 218 us against 283, both gradients' products 337 against 373 (run_scaled),
 // but a word's probabilities of 4e-11 are left with 7 bits there, and those of 1e-13 with none.
+
 // 2^exponent(x) is above |x| (of zeros and denormals: 2^-126).
 __device__ inline int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 255) - 126; }
 

@@ -68,3 +68,18 @@ def test_options_of_the_kernel_are_refused_elsewhere():
     for m, d in ((module(rope_layout="half"), 16), (module(), 8)):
         with pytest.raises(ValueError, match="rope_layout and rope_dims"):
             m(x, *rotary_tables(d, 4))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("options", [{}, dict(rope_layout="half")])
+@pytest.mark.parametrize("strict", [True, False])
+def test_exported(options, strict):
+    """An exported attention holds the rotation's op and gives the eager results."""
+    from mathbrain.baseline import rotary_tables
+    m = module(**options).cuda().eval()
+    x = torch.randn(2, 6, 32, device="cuda")
+    args = (x, *(t.cuda() for t in rotary_tables(16, 6)))
+    with torch.no_grad():
+        program = torch.export.export(m, args, strict=strict)
+        assert any("apply_rotary" in str(n.target) for n in program.graph.nodes)
+        assert torch.equal(program.module()(*args), m(*args))
