@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kThreads) ce_total_kernel(const double* sums, 
 //   y = U g 2^(exp_h(n) + 15 - E(v)),    sum_n U g h_n = 2^(E(v) - 29) sum_n y h'_n       (U with its factor of 2^15)
 // A word that is improbable in every row keeps its 24 bits so, and rows (or words) beside one of another size theirs.  One copy with one
 // power of two would be less to write: 2865 rows, 20011 words of 384 218 us against 283, both gradients' products 337 against 373 (run_scaled),
-// but a word's probabilities of 4e-11 are left with 7 bits there, and those of 1e-13 with none.
+// but a probability of 4e-11 (2^-34.5, of steps of 2^-39) is left with 5 bits there, and one of 1e-13 with none.
 
 // 2^exponent(x) is above |x| (of zeros and denormals: 2^-126).
 __device__ inline int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 255) - 126; }
